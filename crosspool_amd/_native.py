@@ -23,6 +23,7 @@ XP_ERROR_NOT_FOUND = 4
 XP_ERROR_CAPACITY = 5
 XP_ERROR_UNSUPPORTED = 6
 XP_FAULT_SLOT_OUT_OF_RANGE = 1
+XP_FAULT_ADAPTER_OUT_OF_RANGE = 2
 
 class ActivationDesc(ctypes.Structure):
     """``xp_activation_desc`` of the header."""
@@ -62,6 +63,22 @@ class MoeLayerDesc(ctypes.Structure):
     ]
 
 
+class AdapterPool(ctypes.Structure):
+    """``xp_adapter_pool`` of the header."""
+
+    _fields_ = [
+        ("a", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("ranks", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("count", ctypes.c_int64),
+        ("max_rank", ctypes.c_int64),
+        ("input_width", ctypes.c_int64),
+        ("output_width", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+    ]
+
+
 XP_DTYPE_BF16 = 1
 XP_DTYPE_F16 = 2
 XP_DTYPE_F32 = 3
@@ -95,6 +112,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _INT, [_P, _I64, _I64, _P, _I64, _P, _P, _INT, ctypes.POINTER(ActivationDesc), _P, _SIZE, _P],
     ),
     "xp_activation": (_INT, [_P, _P, _I64, _I64, _INT, _INT, ctypes.POINTER(ActivationDesc), _P]),
+    "xp_adapter_workspace_bytes": (_SIZE, [_I64, _I64, _I64, _I64, _I64, _INT, _INT]),
+    "xp_adapter_apply": (
+        _INT,
+        [ctypes.POINTER(AdapterPool), _P, _I64, _P, _I64, _P, _I64, _P, _I64, ctypes.POINTER(ActivationDesc), _P,
+         _SIZE, _P, _P],
+    ),
+    "xp_adapter_backward": (
+        _INT,
+        [ctypes.POINTER(AdapterPool), _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _SIZE, _P, _P],
+    ),
     "xp_dense_workspace_bytes": (_SIZE, [_I64, _I64, _I64]),
     "xp_dense_workspace_layout": (_INT, [_I64, _I64, _I64, ctypes.POINTER(_SIZE)]),
     "xp_dense_step": (_INT, [_P, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _F32, _P, _SIZE, _P, _P]),

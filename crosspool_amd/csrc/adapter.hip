@@ -1,0 +1,516 @@
+// Low-rank adapters: the sort of a batch's rows by adapter, the small kernels of the backward pass
+// and the launches of all of them (the products are in adapter_kernels.hpp).
+
+#include "adapter_kernels.hpp"
+
+#include <algorithm>
+
+namespace xp {
+namespace {
+
+// ------------------------------------------------------------------ rows by adapter
+constexpr int kRouteThreads = 1024;
+constexpr int kRouteWaves = kRouteThreads / kWave;
+constexpr int kRouteGroups = kAdapterMaxCount + 2;
+
+// Exclusive scan of one value per thread over the workgroup; `total` is the sum.
+__device__ int block_exclusive_scan(int value, int *wave_totals, int &total) {
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  int inclusive = value;
+#pragma unroll
+  for (int offset = 1; offset < kWave; offset <<= 1) {
+    const int other = __shfl_up(inclusive, offset, kWave);
+    if (lane >= offset) {
+      inclusive += other;
+    }
+  }
+  __syncthreads();  // an earlier scan's totals are read
+  if (lane == kWave - 1) {
+    wave_totals[wave] = inclusive;
+  }
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kRouteWaves; ++w) {
+    before += w < wave ? wave_totals[w] : 0;
+    total += wave_totals[w];
+  }
+  return before + inclusive - value;
+}
+
+// A stable counting sort by one workgroup: every wave counts a contiguous sixteenth of the rows, the
+// counts are scanned over groups and waves, and each wave places its rows 64 at a time, a row's
+// place among the 64 being the number of earlier lanes of its group (from ballots over the bits of
+// the group).  Stable and free of racing increments, so the sums of the gradients have one order.
+// Bound by its own latency: 8 rows per lane at 8192 rows.
+__global__ __launch_bounds__(kRouteThreads) void adapter_route_kernel(AdapterRouteArgs a) {
+  __shared__ int counts[kRouteWaves][kRouteGroups];
+  __shared__ int starts[kRouteGroups + 1];
+  __shared__ int tile_starts[kRouteGroups + 1];
+  __shared__ int run_starts[kAdapterMaxCount + 1];
+  __shared__ int slot_starts[kAdapterMaxCount];
+  __shared__ int wave_totals[kRouteWaves];
+  const AdapterBatch &batch = a.batch;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = tid >> 6;
+  const int count = batch.count;
+  const int groups = count + 2;
+  const int rows = static_cast<int>(batch.rows);
+  for (int index = tid; index < kRouteWaves * kRouteGroups; index += kRouteThreads) {
+    (&counts[0][0])[index] = 0;
+  }
+  __syncthreads();
+  const int share = ((rows + kRouteWaves - 1) / kRouteWaves + kWave - 1) / kWave * kWave;
+  const int first = wave * share;
+  const int last = first + share < rows ? first + share : rows;
+  bool bad = false;
+  for (int row = first + lane; row < last; row += kWave) {
+    const int group = adapter_group(batch.ids[row], count);
+    bad |= group > count;
+    atomicAdd(&counts[wave][group], 1);
+  }
+  if (__ballot(bad) != 0 && lane == 0) {
+    raise_fault(a.fault, kFaultAdapterOutOfRange);
+  }
+  __syncthreads();
+  // Two groups per thread: their rows, tiles, runs and slots of partial sums.
+  int length[2] = {0, 0};
+  int tiles[2] = {0, 0};
+  int runs[2] = {0, 0};
+  int slots[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int group = 2 * tid + i;
+    if (group < groups) {
+      for (int w = 0; w < kRouteWaves; ++w) {
+        const int own = counts[w][group];
+        counts[w][group] = length[i];
+        length[i] += own;
+      }
+      tiles[i] = (length[i] + kAdapterTileRows - 1) / kAdapterTileRows;
+      if (group < count && batch.run_rows > 0) {
+        runs[i] = (length[i] + batch.run_rows - 1) / batch.run_rows;
+        slots[i] = runs[i] > 1 ? runs[i] : 0;
+      }
+    }
+  }
+  int total_rows;
+  int total_tiles;
+  int total_runs;
+  int total_slots;
+  const int row0 = block_exclusive_scan(length[0] + length[1], wave_totals, total_rows);
+  const int tile0 = block_exclusive_scan(tiles[0] + tiles[1], wave_totals, total_tiles);
+  const int run0 = block_exclusive_scan(runs[0] + runs[1], wave_totals, total_runs);
+  const int slot0 = block_exclusive_scan(slots[0] + slots[1], wave_totals, total_slots);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int group = 2 * tid + i;
+    if (group < groups) {
+      starts[group] = row0 + (i > 0 ? length[0] : 0);
+      tile_starts[group] = tile0 + (i > 0 ? tiles[0] : 0);
+      batch.starts[group] = starts[group];
+    }
+    if (group < count) {
+      const int slot = slot0 + (i > 0 ? slots[0] : 0);
+      run_starts[group] = run0 + (i > 0 ? runs[0] : 0);
+      slot_starts[group] = runs[i] > 1 ? slot : -1;
+      if (batch.run_rows > 0) {
+        batch.runs[2 * group] = slot;
+        batch.runs[2 * group + 1] = runs[i];
+      }
+    }
+  }
+  if (tid == 0) {
+    starts[groups] = rows;
+    batch.starts[groups] = rows;
+    tile_starts[groups] = total_tiles;
+    run_starts[count] = total_runs;
+    batch.head[1] = total_tiles;
+    batch.head[2] = total_runs;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    batch.head[0] = tile_starts[count];
+  }
+  // Placement.
+  for (int row64 = first; row64 < last; row64 += kWave) {
+    const int row = row64 + lane;
+    const bool live = row < last;
+    const int group = live ? adapter_group(batch.ids[row], count) : 0;
+    unsigned long long same = __ballot(live);
+    for (int bit = 1; bit < groups; bit <<= 1) {
+      const unsigned long long set = __ballot((group & bit) != 0);
+      same &= (group & bit) != 0 ? set : ~set;
+    }
+    if (live) {
+      const int before = __popcll(same & ((1ull << lane) - 1));
+      batch.perm[starts[group] + counts[wave][group] + before] = row;
+      if (before == 0) {
+        // After every lane of the wave has read the count: one wave runs in order.
+        __builtin_amdgcn_wave_barrier();
+        atomicAdd(&counts[wave][group], __popcll(same));
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  // The group of a tile (run): the last that starts at or before it and is not empty.
+  auto find = [](const int *table, int entries, int value) {
+    int low = 0;
+    int high = entries;
+    while (high - low > 1) {
+      const int middle = (low + high) / 2;
+      if (table[middle] <= value) {
+        low = middle;
+      } else {
+        high = middle;
+      }
+    }
+    return low;
+  };
+  for (int tile = tid; tile < total_tiles; tile += kRouteThreads) {
+    const int group = find(tile_starts, groups, tile);
+    batch.tiles[2 * tile] = group;
+    batch.tiles[2 * tile + 1] = starts[group] + (tile - tile_starts[group]) * kAdapterTileRows;
+  }
+  for (int run = tid; run < total_runs; run += kRouteThreads) {
+    const int group = find(run_starts, count, run);
+    const int begin = starts[group] + (run - run_starts[group]) * batch.run_rows;
+    const int end = begin + batch.run_rows < starts[group + 1] ? begin + batch.run_rows : starts[group + 1];
+    batch.outer[4 * run] = group;
+    batch.outer[4 * run + 1] = begin;
+    batch.outer[4 * run + 2] = end;
+    batch.outer[4 * run + 3] = slot_starts[group] < 0 ? -1 : slot_starts[group] + run - run_starts[group];
+  }
+}
+
+// ------------------------------------------------------------------ transposes
+// at[a][k][r] = A_a[r][k] and bt[a][r][n] = B_a[n][r] for the adapters that have rows: 64 columns of
+// A (rows of B) per workgroup through LDS.  Ranks past the adapter's are left unwritten.
+template <class E>
+__global__ __launch_bounds__(256) void adapter_transpose_kernel(AdapterTransposeArgs a) {
+  __shared__ E tile[kAdapterMaxRank][64 + 1];
+  const int64_t blocks0 = (a.k + 63) / 64;
+  const bool second = static_cast<int64_t>(blockIdx.x) >= blocks0;
+  const int64_t c0 = (blockIdx.x - (second ? blocks0 : 0)) * 64;
+  const int64_t length = second ? a.n : a.k;
+  const int columns = length - c0 < 64 ? static_cast<int>(length - c0) : 64;
+  for (int group = blockIdx.y; group < a.batch.count; group += gridDim.y) {
+    const int rank = adapter_rank(a.ranks, group, a.max_rank);
+    if (rank == 0 || a.batch.starts[group + 1] == a.batch.starts[group]) {
+      continue;
+    }
+    if (second) {
+      const E *source = static_cast<const E *>(a.b) + (group * a.n + c0) * a.max_rank;
+      E *target = static_cast<E *>(a.bt) + static_cast<int64_t>(group) * a.rp * a.n + c0;
+      for (int index = threadIdx.x; index < columns * rank; index += 256) {
+        const int column = index / rank;
+        const int r = index - column * rank;
+        tile[r][column] = source[static_cast<int64_t>(column) * a.max_rank + r];
+      }
+      __syncthreads();
+      for (int index = threadIdx.x; index < 64 * rank; index += 256) {
+        const int column = index & 63;
+        if (column < columns) {
+          target[(index >> 6) * a.n + column] = tile[index >> 6][column];
+        }
+      }
+    } else {
+      const E *source = static_cast<const E *>(a.a) + static_cast<int64_t>(group) * a.max_rank * a.k + c0;
+      E *target = static_cast<E *>(a.at) + (group * a.k + c0) * a.rp;
+      for (int index = threadIdx.x; index < 64 * rank; index += 256) {
+        const int column = index & 63;
+        if (column < columns) {
+          tile[index >> 6][column] = source[(index >> 6) * a.k + column];
+        }
+      }
+      __syncthreads();
+      for (int index = threadIdx.x; index < columns * rank; index += 256) {
+        const int column = index / rank;
+        const int r = index - column * rank;
+        target[static_cast<int64_t>(column) * a.rp + r] = tile[r][column];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ terms
+// The K ranges' sums of t (u) in range order, transposed to [rank][position] and split into the terms
+// that the outer products multiply.  One workgroup per tile of 64 positions.
+__global__ __launch_bounds__(256) void adapter_terms_kernel(AdapterTermsArgs a) {
+  __shared__ int list[kAdapterTileRows];
+  __shared__ float values[kAdapterTileRows][kAdapterMaxRank + 1];
+  for (int64_t slot = blockIdx.x;; slot += gridDim.x) {
+    const AdapterTile tile = adapter_tile(a.batch, slot, false, list);
+    if (tile.group < 0) {
+      return;
+    }
+    const int64_t position = a.batch.tiles[2 * slot + 1];
+    const int rank = adapter_rank(a.ranks, tile.group, a.max_rank);
+    int columns = 16;
+    while (columns < rank) {
+      columns *= 2;
+    }
+    if (rank > 0) {
+      const int job = blockIdx.y;
+      const int64_t plane = a.batch.rows * a.rp;
+      for (int index = threadIdx.x; index < tile.rows * columns; index += 256) {
+        const int row = index / columns;
+        const int r = index & (columns - 1);
+        const float *source = a.partials[job] + static_cast<int64_t>(list[row]) * a.rp + r;
+        float sum = 0.0f;
+#pragma unroll 8
+        for (int64_t range = 0; range < a.ranges[job]; ++range) {
+          sum += source[range * plane];
+        }
+        values[row][r] = sum;
+      }
+      __syncthreads();
+      const int64_t term = static_cast<int64_t>(a.rp) * a.stride;
+      for (int index = threadIdx.x; index < 64 * columns; index += 256) {
+        const int row = index & 63;
+        if (row < tile.rows) {
+          const float value = values[row][index >> 6];
+          const int64_t at = (index >> 6) * a.stride + position + row;
+          if (a.f32 != 0) {
+            static_cast<float *>(a.terms[job])[at] = value;
+          } else {
+            uint32_t high;
+            uint32_t low;
+            split_pair(value, 0.0f, high, low);
+            static_cast<uint16_t *>(a.terms[job])[at] = static_cast<uint16_t>(high);
+            static_cast<uint16_t *>(a.terms[job])[at + term] = static_cast<uint16_t>(low);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ gradients of several runs
+__global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterReduceArgs a) {
+  const bool second = static_cast<int64_t>(blockIdx.x) >= a.blocks0;
+  const AdapterOuterJob &job = a.job[second ? 1 : 0];
+  const int64_t block = blockIdx.x - (second ? a.blocks0 : 0);
+  const uint32_t elements = static_cast<uint32_t>(job.columns * a.max_rank);
+  for (int group = blockIdx.y; group < a.batch.count; group += gridDim.y) {
+    const int slot = a.batch.runs[2 * group];
+    const int runs = a.batch.runs[2 * group + 1];
+    if (runs == 1) {
+      continue;
+    }
+    const int rank = adapter_rank(a.ranks, group, a.max_rank);
+    const float scale = a.scales != nullptr ? a.scales[group] : 1.0f;
+    const int64_t plane = static_cast<int64_t>(a.rp) * job.columns;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t index = static_cast<uint32_t>(block * 1024) + i * 256 + threadIdx.x;
+      if (index >= elements) {
+        continue;
+      }
+      const uint32_t width = second ? static_cast<uint32_t>(a.max_rank) : static_cast<uint32_t>(job.columns);
+      const uint32_t major = index / width;
+      const uint32_t minor = index - major * width;
+      const int r = static_cast<int>(second ? minor : major);
+      float sum = 0.0f;
+      if (r < rank) {
+        const float *source = job.partials + slot * plane +
+                              (second ? static_cast<int64_t>(major) * a.rp + r
+                                      : static_cast<int64_t>(r) * job.columns + minor);
+#pragma unroll 4
+        for (int run = 0; run < runs; ++run) {
+          sum += source[run * plane];
+        }
+        sum *= scale;
+      }
+      store_value(job.grad, static_cast<int64_t>(group) * elements + index, sum, a.dtype);
+    }
+  }
+}
+
+int rank_tiles(int64_t max_rank) { return max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : max_rank <= 64 ? 4 : 8; }
+
+// Workgroups of the shrink kernel that fill the chip: two per CU.
+constexpr int64_t kShrinkWorkgroups = 512;
+constexpr int64_t kMaxRanges = 32;
+constexpr int64_t kStepsPerWorkgroup = 16;  // the least: two steps per wave
+constexpr int64_t kExpandWorkgroups = 1024;
+constexpr int64_t kOuterWorkgroups = 1024;
+constexpr int64_t kMinRunRows = 256;
+// Tiles of adapters with few rows come on top of the whole ones; workgroups past this many walk on.
+constexpr int64_t kExtraSlots = 64;
+
+int64_t align16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+unsigned tile_slots(const AdapterBatch &batch) {
+  if (batch.head == nullptr) {
+    return static_cast<unsigned>(batch.rows);
+  }
+  const int64_t tiles = (batch.rows + kAdapterTileRows - 1) / kAdapterTileRows;
+  return static_cast<unsigned>(std::min<int64_t>(tiles + std::min<int64_t>(batch.count + 1, kExtraSlots), 65535));
+}
+
+template <class Args>
+KernelLaunch launch_of(const void *func, dim3 grid, unsigned block, const Args &args) {
+  KernelLaunch kernel;
+  kernel.func = func;
+  kernel.grid = grid;
+  kernel.block = dim3(block, 1, 1);
+  kernel.set_args(args);
+  return kernel;
+}
+
+}  // namespace
+
+AdapterPlan plan_adapter(const AdapterShape &shape) {
+  AdapterPlan plan{};
+  const int64_t element = shape.dtype == kDtypeF32 ? 4 : 2;
+  const int64_t rows = shape.rows;
+  plan.rp = 16 * rank_tiles(shape.max_rank);
+  const bool routed = shape.backward || rows > kAdapterDirectRows;
+  const int64_t tiles = (rows + kAdapterTileRows - 1) / kAdapterTileRows;
+  const int64_t widths[2] = {shape.input_width, shape.output_width};
+  int64_t at = 0;
+  if (routed) {
+    plan.max_tiles = rows / kAdapterTileRows + std::min(rows, shape.count + 2);
+    int64_t ints = 4 + shape.count + 3 + rows + 2 * plan.max_tiles;
+    if (shape.backward) {
+      const int64_t blocks = (widths[0] + 63) / 64 + (widths[1] + 63) / 64;
+      const int64_t wanted = std::max<int64_t>(1, (kOuterWorkgroups + blocks - 1) / blocks);
+      const int64_t run_rows = ((rows + wanted - 1) / wanted + kAdapterTileRows - 1) / kAdapterTileRows * kAdapterTileRows;
+      plan.run_rows = std::max(kMinRunRows, run_rows);
+      plan.max_runs = rows / plan.run_rows + std::min(rows, shape.count);
+      // An adapter of several runs has more than run_rows rows.
+      plan.run_slots = std::min(2 * rows / kMinRunRows, 2 * wanted);
+      ints += 4 * plan.max_runs + 2 * shape.count;
+    }
+    at = align16(ints * 4);
+  }
+  for (int p = 0; p < (shape.backward ? 2 : 1); ++p) {
+    const int64_t steps = (widths[p] * element + 63) / 64;
+    const int64_t most = std::max<int64_t>(1, std::min(kMaxRanges, steps / kStepsPerWorkgroup));
+    const int64_t wanted = routed ? (kShrinkWorkgroups + tiles - 1) / tiles : kMaxRanges;
+    const int64_t ranges = std::min(most, wanted);
+    plan.steps_per_range[p] = ((steps + ranges - 1) / ranges + 3) / 4 * 4;
+    plan.ranges[p] = (steps + plan.steps_per_range[p] - 1) / plan.steps_per_range[p];
+    plan.partials[p] = static_cast<size_t>(at);
+    at += align16(plan.ranges[p] * rows * plan.rp * 4);
+  }
+  if (shape.backward) {
+    plan.stride = (rows + 15) / 8 * 8;  // a load of eight positions may pass the last by seven
+    for (int p = 0; p < 2; ++p) {
+      plan.terms[p] = static_cast<size_t>(at);
+      at += align16(plan.rp * plan.stride * 4);
+      plan.sums[p] = static_cast<size_t>(at);
+      at += align16(plan.run_slots * plan.rp * widths[p] * 4);
+    }
+    plan.at = static_cast<size_t>(at);
+    at += align16(shape.count * shape.input_width * plan.rp * element);
+    plan.bt = static_cast<size_t>(at);
+    at += align16(shape.count * shape.output_width * plan.rp * element);
+  }
+  plan.bytes = static_cast<size_t>(at);
+  return plan;
+}
+
+size_t adapter_workspace_bytes(const AdapterShape &shape) {
+  size_t most = plan_adapter(shape).bytes;
+  // The number of K ranges depends on the tiles alone, up to one range, and falls as they grow.
+  AdapterShape smaller = shape;
+  for (int64_t tiles = 1; tiles <= kShrinkWorkgroups && tiles * kAdapterTileRows < shape.rows; ++tiles) {
+    smaller.rows = tiles * kAdapterTileRows;
+    most = std::max(most, plan_adapter(smaller).bytes);
+  }
+  return most;
+}
+
+AdapterBatch adapter_batch(const AdapterShape &shape, const AdapterPlan &plan, const int32_t *ids,
+                           unsigned char *workspace) {
+  AdapterBatch batch{};
+  batch.ids = ids;
+  batch.rows = shape.rows;
+  batch.count = static_cast<int32_t>(shape.count);
+  if (plan.max_tiles > 0) {
+    int32_t *at = reinterpret_cast<int32_t *>(workspace + plan.route);
+    batch.head = at;
+    batch.starts = at + 4;
+    batch.perm = batch.starts + shape.count + 3;
+    batch.tiles = batch.perm + shape.rows;
+    batch.outer = batch.tiles + 2 * plan.max_tiles;
+    batch.runs = batch.outer + 4 * plan.max_runs;
+    batch.run_rows = static_cast<int32_t>(plan.run_rows);
+  }
+  return batch;
+}
+
+KernelLaunch make_adapter_route(const AdapterRouteArgs &args) {
+  return launch_of(reinterpret_cast<const void *>(&adapter_route_kernel), dim3(1, 1, 1), kRouteThreads, args);
+}
+
+KernelLaunch make_adapter_shrink(const AdapterShrinkArgs &args, const AdapterPlan &plan, int dtype) {
+  const int tiles = static_cast<int>(plan.rp / 16);
+  const void *func = dtype == kDtypeF32   ? AdapterKernels<F32Payload>::shrink(tiles)
+                     : dtype == kDtypeF16 ? AdapterKernels<F16Payload>::shrink(tiles)
+                                          : AdapterKernels<Bf16Payload>::shrink(tiles);
+  return launch_of(func, dim3(static_cast<unsigned>(args.job[0].ranges + args.job[1].ranges), tile_slots(args.batch), 1),
+                   kAdapterShrinkWaves * kWave, args);
+}
+
+KernelLaunch make_adapter_expand(const AdapterExpandArgs &args, const AdapterPlan &plan, int dtype) {
+  const int tiles = static_cast<int>(plan.rp / 16);
+  const bool act = args.act.function != kActivationNone;
+  const void *func = dtype == kDtypeF32   ? AdapterKernels<F32Payload>::expand(tiles, act)
+                     : dtype == kDtypeF16 ? AdapterKernels<F16Payload>::expand(tiles, act)
+                                          : AdapterKernels<Bf16Payload>::expand(tiles, act);
+  AdapterExpandArgs record = args;
+  constexpr int64_t kTurn = kAdapterExpandWaves * kAdapterExpandColumns;
+  const int64_t turns = (args.n + kTurn - 1) / kTurn;
+  const int64_t row_tiles = args.batch.head == nullptr ? 1 : (args.batch.rows + kAdapterTileRows - 1) / kAdapterTileRows;
+  const int64_t groups = std::min(turns, std::max<int64_t>(1, (kExpandWorkgroups + row_tiles - 1) / row_tiles));
+  record.columns = (turns + groups - 1) / groups * kTurn;
+  return launch_of(func,
+                   dim3(static_cast<unsigned>((args.n + record.columns - 1) / record.columns), tile_slots(args.batch), 1),
+                   kAdapterExpandWaves * kWave, record);
+}
+
+KernelLaunch make_adapter_transpose(const AdapterTransposeArgs &args) {
+  const void *func = args.element == 4 ? reinterpret_cast<const void *>(&adapter_transpose_kernel<uint32_t>)
+                                       : reinterpret_cast<const void *>(&adapter_transpose_kernel<uint16_t>);
+  return launch_of(func, dim3(static_cast<unsigned>((args.k + 63) / 64 + (args.n + 63) / 64),
+                              static_cast<unsigned>(std::min(args.batch.count, 32)), 1),
+                   256, args);
+}
+
+KernelLaunch make_adapter_terms(const AdapterTermsArgs &args, const AdapterPlan &) {
+  return launch_of(reinterpret_cast<const void *>(&adapter_terms_kernel), dim3(tile_slots(args.batch), 2, 1), 256, args);
+}
+
+KernelLaunch make_adapter_outer(const AdapterOuterArgs &args, const AdapterPlan &plan, int dtype) {
+  const int tiles = static_cast<int>(plan.rp / 16);
+  const void *func = dtype == kDtypeF32   ? AdapterKernels<F32Payload>::outer(tiles)
+                     : dtype == kDtypeF16 ? AdapterKernels<F16Payload>::outer(tiles)
+                                          : AdapterKernels<Bf16Payload>::outer(tiles);
+  AdapterOuterArgs record = args;
+  record.blocks0 = (args.job[0].columns + 63) / 64;
+  const int64_t runs = std::min<int64_t>(plan.max_runs, args.batch.rows / plan.run_rows + kExtraSlots);
+  return launch_of(func,
+                   dim3(static_cast<unsigned>(record.blocks0 + (args.job[1].columns + 63) / 64),
+                        static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(runs, 1), 65535)), 1),
+                   kAdapterOuterWaves * kWave, record);
+}
+
+KernelLaunch make_adapter_reduce(const AdapterReduceArgs &args) {
+  AdapterReduceArgs record = args;
+  record.blocks0 = (args.job[0].columns * args.max_rank + 1023) / 1024;
+  const int64_t blocks1 = (args.job[1].columns * args.max_rank + 1023) / 1024;
+  return launch_of(reinterpret_cast<const void *>(&adapter_reduce_kernel),
+                   dim3(static_cast<unsigned>(record.blocks0 + blocks1),
+                        static_cast<unsigned>(std::min(args.batch.count, 1024)), 1),
+                   256, record);
+}
+
+}  // namespace xp

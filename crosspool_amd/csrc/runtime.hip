@@ -1648,6 +1648,251 @@ int xp_activation(const void *inputs, void *output, int64_t rows, int64_t width,
   return XP_OK;
 }
 
+namespace {
+
+// Elements [first, first + (rows - 1) ld + width) of two operands: whether their bytes overlap.
+bool rows_overlap(const void *p, int64_t ld_p, int64_t width_p, const void *q, int64_t ld_q, int64_t width_q,
+                  int64_t rows, size_t element) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  const uintptr_t b = reinterpret_cast<uintptr_t>(q);
+  const uintptr_t a_end = a + static_cast<uintptr_t>((rows - 1) * ld_p + width_p) * element;
+  const uintptr_t b_end = b + static_cast<uintptr_t>((rows - 1) * ld_q + width_q) * element;
+  return a < b_end && b < a_end;
+}
+
+constexpr int64_t kAdapterMaxRows = int64_t{1} << 24;
+constexpr int64_t kAdapterMaxWidth = int64_t{1} << 22;
+
+bool adapter_shape_valid(const AdapterShape &shape) {
+  return shape.rows >= 0 && shape.rows <= kAdapterMaxRows && shape.count >= 1 && shape.count <= kAdapterMaxCount &&
+         shape.max_rank >= 1 && shape.max_rank <= kAdapterMaxRank && shape.input_width >= 1 &&
+         shape.input_width <= kAdapterMaxWidth && shape.output_width >= 1 &&
+         shape.output_width <= kAdapterMaxWidth && dtype_bytes(shape.dtype) != 0;
+}
+
+// The checks that both adapter entry points share; the shape of the call.
+int adapter_shape(const xp_adapter_pool *pool, const int32_t *ids, int64_t rows, bool backward, AdapterShape &shape) {
+  XP_REQUIRE(pool != nullptr, "the adapter pool must be non-null");
+  shape = AdapterShape{rows, pool->count, pool->max_rank, pool->input_width, pool->output_width, pool->dtype, backward};
+  XP_REQUIRE(adapter_shape_valid(shape),
+             "adapters: 1 to 1024 of 1 to 128 ranks, widths of 1 to 4194304, at most 16777216 rows, bf16, fp16 or fp32");
+  const size_t element = dtype_bytes(pool->dtype);
+  XP_REQUIRE(pool->a != nullptr && pool->b != nullptr && aligned_to(pool->a, element) && aligned_to(pool->b, element),
+             "adapter weights must be non-null and aligned to their element size");
+  XP_REQUIRE(aligned_to(pool->ranks, 4) && aligned_to(pool->scales, 4), "adapter ranks and scales must be 4-byte aligned");
+  XP_REQUIRE(rows == 0 || (ids != nullptr && aligned_to(ids, 4)), "adapter ids must be non-null and 4-byte aligned");
+  return XP_OK;
+}
+
+int adapter_rows(const char *name, const void *rows_pointer, int64_t ld, int64_t width, size_t element) {
+  XP_REQUIRE(rows_pointer != nullptr && aligned_to(rows_pointer, element),
+             std::string(name) + " must be non-null and aligned to its element size");
+  XP_REQUIRE(ld >= width && ld <= (int64_t{1} << 31), std::string(name) + " has a row stride below its width or above 2^31");
+  return XP_OK;
+}
+
+}  // namespace
+
+size_t xp_adapter_workspace_bytes(int64_t rows, int64_t count, int64_t max_rank, int64_t input_width,
+                                  int64_t output_width, int dtype, int backward) {
+  const AdapterShape shape{rows, count, max_rank, input_width, output_width, dtype, backward != 0};
+  return adapter_shape_valid(shape) ? adapter_workspace_bytes(shape) : 0;
+}
+
+int xp_adapter_apply(const xp_adapter_pool *pool, const int32_t *ids, int64_t rows, const void *x, int64_t ldx,
+                     const void *base, int64_t ld_base, void *out, int64_t ld_out,
+                     const xp_activation_desc *activation, void *workspace, size_t workspace_bytes,
+                     uint32_t *fault_word, xp_stream_t stream) {
+  AdapterShape shape{};
+  if (const int status = adapter_shape(pool, ids, rows, false, shape); status != XP_OK) {
+    return status;
+  }
+  AdapterExpandArgs expand{};
+  if (const int status = activation_record(activation, expand.act); status != XP_OK) {
+    return status;
+  }
+  const bool gated = expand.act.gated != 0;
+  XP_REQUIRE(!gated || shape.output_width % 2 == 0, "a gated activation needs an even number of (INTERLEAVED) columns");
+  if (rows == 0) {
+    return XP_OK;
+  }
+  const size_t element = dtype_bytes(shape.dtype);
+  const int64_t out_width = gated ? shape.output_width / 2 : shape.output_width;
+  if (const int status = adapter_rows("adapter input", x, ldx, shape.input_width, element); status != XP_OK) {
+    return status;
+  }
+  if (base != nullptr) {
+    if (const int status = adapter_rows("adapter base", base, ld_base, shape.output_width, element); status != XP_OK) {
+      return status;
+    }
+  }
+  if (const int status = adapter_rows("adapter output", out, ld_out, out_width, element); status != XP_OK) {
+    return status;
+  }
+  XP_REQUIRE(!rows_overlap(x, ldx, shape.input_width, out, ld_out, out_width, rows, element),
+             "the adapter output must not overlap its input");
+  const bool same = base == out && ld_base == ld_out && expand.act.function == kActivationNone;
+  XP_REQUIRE(base == nullptr || same ||
+                 !rows_overlap(base, ld_base, shape.output_width, out, ld_out, out_width, rows, element),
+             "the adapter output may be its base only whole and without an activation");
+  const AdapterPlan plan = plan_adapter(shape);
+  XP_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= plan.bytes,
+             "adapter workspace is missing, unaligned or smaller than xp_adapter_workspace_bytes");
+  unsigned char *bytes = static_cast<unsigned char *>(workspace);
+  const hipStream_t hip_stream = static_cast<hipStream_t>(stream);
+  const AdapterBatch batch = adapter_batch(shape, plan, ids, bytes);
+  if (batch.head != nullptr) {
+    XP_HIP_CHECK(launch(make_adapter_route(AdapterRouteArgs{batch, fault_word}), hip_stream));
+  }
+  AdapterShrinkArgs shrink{};
+  shrink.batch = batch;
+  shrink.ranks = pool->ranks;
+  shrink.job[0] = {x, pool->a, reinterpret_cast<float *>(bytes + plan.partials[0]), ldx, shape.input_width,
+                   shape.max_rank, plan.ranges[0], plan.steps_per_range[0]};
+  shrink.max_rank = static_cast<int32_t>(shape.max_rank);
+  shrink.rp = static_cast<int32_t>(plan.rp);
+  XP_HIP_CHECK(launch(make_adapter_shrink(shrink, plan, shape.dtype), hip_stream));
+  expand.batch = batch;
+  expand.ranks = pool->ranks;
+  expand.scales = pool->scales;
+  expand.partials = shrink.job[0].partials;
+  expand.w = pool->b;
+  expand.base = base;
+  expand.out = out;
+  expand.fault = fault_word;
+  expand.ranges = plan.ranges[0];
+  expand.n = shape.output_width;
+  expand.ld_base = ld_base;
+  expand.ld_out = ld_out;
+  expand.max_rank = shrink.max_rank;
+  expand.ld_w = shrink.max_rank;
+  expand.rp = shrink.rp;
+  expand.in_place = same;
+  XP_HIP_CHECK(launch(make_adapter_expand(expand, plan, shape.dtype), hip_stream));
+  return XP_OK;
+}
+
+int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t rows, const void *x, int64_t ldx,
+                        const void *grad_out, int64_t ld_grad_out, const void *base, int64_t ld_base, void *grad_x,
+                        int64_t ld_grad_x, void *grad_a, void *grad_b, void *workspace, size_t workspace_bytes,
+                        uint32_t *fault_word, xp_stream_t stream) {
+  AdapterShape shape{};
+  if (const int status = adapter_shape(pool, ids, rows, true, shape); status != XP_OK) {
+    return status;
+  }
+  const size_t element = dtype_bytes(shape.dtype);
+  XP_REQUIRE((grad_a == nullptr) == (grad_b == nullptr), "grad_a and grad_b are asked for together");
+  XP_REQUIRE(aligned_to(grad_a, element) && aligned_to(grad_b, element),
+             "adapter gradients must be aligned to their element size");
+  const hipStream_t hip_stream = static_cast<hipStream_t>(stream);
+  if (rows > 0) {
+    if (const int status = adapter_rows("adapter input", x, ldx, shape.input_width, element); status != XP_OK) {
+      return status;
+    }
+    if (const int status = adapter_rows("output gradient", grad_out, ld_grad_out, shape.output_width, element);
+        status != XP_OK) {
+      return status;
+    }
+    if (grad_x != nullptr) {
+      if (const int status = adapter_rows("input gradient", grad_x, ld_grad_x, shape.input_width, element);
+          status != XP_OK) {
+        return status;
+      }
+      XP_REQUIRE(!rows_overlap(x, ldx, shape.input_width, grad_x, ld_grad_x, shape.input_width, rows, element) &&
+                     !rows_overlap(grad_out, ld_grad_out, shape.output_width, grad_x, ld_grad_x, shape.input_width,
+                                   rows, element),
+                 "the input gradient must not overlap the input or the output gradient");
+      if (base != nullptr) {
+        if (const int status = adapter_rows("base gradient", base, ld_base, shape.input_width, element);
+            status != XP_OK) {
+          return status;
+        }
+        XP_REQUIRE((base == grad_x && ld_base == ld_grad_x) ||
+                       !rows_overlap(base, ld_base, shape.input_width, grad_x, ld_grad_x, shape.input_width, rows,
+                                     element),
+                   "the input gradient may be its base only whole");
+      }
+    }
+  }
+  if (grad_x == nullptr && grad_a == nullptr) {
+    return XP_OK;
+  }
+  // With no rows every adapter's gradient is zero: the plan of one row has what the sort needs.
+  AdapterShape planned = shape;
+  planned.rows = std::max<int64_t>(rows, 1);
+  const AdapterPlan plan = plan_adapter(planned);
+  XP_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= plan.bytes,
+             "adapter workspace is missing, unaligned or smaller than xp_adapter_workspace_bytes");
+  unsigned char *bytes = static_cast<unsigned char *>(workspace);
+  const AdapterBatch batch = adapter_batch(shape, plan, ids, bytes);
+  const int32_t max_rank = static_cast<int32_t>(shape.max_rank);
+  const int32_t rp = static_cast<int32_t>(plan.rp);
+  float *t = reinterpret_cast<float *>(bytes + plan.partials[0]);
+  float *u = reinterpret_cast<float *>(bytes + plan.partials[1]);
+  XP_HIP_CHECK(launch(make_adapter_route(AdapterRouteArgs{batch, fault_word}), hip_stream));
+  if (rows > 0) {
+    const AdapterTransposeArgs transpose{batch, pool->ranks, pool->a, pool->b, bytes + plan.at, bytes + plan.bt,
+                                         shape.input_width, shape.output_width, max_rank, rp,
+                                         static_cast<int32_t>(element)};
+    XP_HIP_CHECK(launch(make_adapter_transpose(transpose), hip_stream));
+    AdapterShrinkArgs shrink{};
+    shrink.batch = batch;
+    shrink.ranks = pool->ranks;
+    shrink.job[0] = {grad_out, bytes + plan.bt, u, ld_grad_out, shape.output_width, plan.rp, plan.ranges[1],
+                     plan.steps_per_range[1]};
+    if (grad_a != nullptr) {
+      shrink.job[1] = {x, pool->a, t, ldx, shape.input_width, shape.max_rank, plan.ranges[0], plan.steps_per_range[0]};
+    }
+    shrink.max_rank = max_rank;
+    shrink.rp = rp;
+    XP_HIP_CHECK(launch(make_adapter_shrink(shrink, plan, shape.dtype), hip_stream));
+    if (grad_x != nullptr) {
+      AdapterExpandArgs expand{};
+      expand.batch = batch;
+      expand.ranks = pool->ranks;
+      expand.scales = pool->scales;
+      expand.partials = u;
+      expand.w = bytes + plan.at;
+      expand.base = base;
+      expand.out = grad_x;
+      expand.ranges = plan.ranges[1];
+      expand.n = shape.input_width;
+      expand.ld_base = ld_base;
+      expand.ld_out = ld_grad_x;
+      expand.max_rank = max_rank;
+      expand.ld_w = rp;
+      expand.rp = rp;
+      expand.in_place = base == grad_x;
+      expand.act.function = kActivationNone;
+      XP_HIP_CHECK(launch(make_adapter_expand(expand, plan, shape.dtype), hip_stream));
+    }
+  }
+  if (grad_a != nullptr) {
+    AdapterOuterArgs outer{};
+    outer.batch = batch;
+    outer.ranks = pool->ranks;
+    outer.scales = pool->scales;
+    outer.job[0] = {x, bytes + plan.terms[0], grad_a, reinterpret_cast<float *>(bytes + plan.sums[0]), ldx,
+                    shape.input_width};
+    outer.job[1] = {grad_out, bytes + plan.terms[1], grad_b, reinterpret_cast<float *>(bytes + plan.sums[1]),
+                    ld_grad_out, shape.output_width};
+    outer.stride = plan.stride;
+    outer.max_rank = max_rank;
+    outer.rp = rp;
+    if (rows > 0) {
+      const AdapterTermsArgs terms{batch, pool->ranks, {u, t}, {bytes + plan.terms[0], bytes + plan.terms[1]},
+                                   {plan.ranges[1], plan.ranges[0]}, plan.stride, max_rank, rp,
+                                   shape.dtype == XP_DTYPE_F32 ? 1 : 0};
+      XP_HIP_CHECK(launch(make_adapter_terms(terms, plan), hip_stream));
+      XP_HIP_CHECK(launch(make_adapter_outer(outer, plan, shape.dtype), hip_stream));
+    }
+    const AdapterReduceArgs reduce{batch, pool->ranks, pool->scales, {outer.job[0], outer.job[1]}, 0, max_rank, rp,
+                                   shape.dtype};
+    XP_HIP_CHECK(launch(make_adapter_reduce(reduce), hip_stream));
+  }
+  return XP_OK;
+}
+
 size_t xp_dense_workspace_bytes(int64_t capacity, int64_t hidden, int64_t intermediate) {
   if (capacity <= 0 || hidden <= 0 || intermediate <= 0) {
     return 0;

@@ -20,6 +20,7 @@ constexpr int kWave = 64;
 // Fault bits raised by kernels into a caller-provided device word.  The word is
 // sticky: kernels only OR bits in, the host clears it explicitly.
 constexpr uint32_t kFaultSlotOutOfRange = 1u;
+constexpr uint32_t kFaultAdapterOutOfRange = 2u;
 
 __device__ __forceinline__ float bf16_to_float(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
 

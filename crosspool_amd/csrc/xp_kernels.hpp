@@ -339,6 +339,166 @@ struct ActivationLaunchArgs {
 
 KernelLaunch make_activation(const ActivationLaunchArgs &args);
 
+// ---------------------------------------------------------------- adapters
+constexpr int kAdapterMaxRank = 128;
+constexpr int kAdapterMaxCount = 1024;
+constexpr int kAdapterTileRows = 64;
+// Up to this many rows the tiles are found by ballots in every workgroup; above, rows are sorted.
+constexpr int64_t kAdapterDirectRows = 64;
+
+// The batch's rows by adapter.  With `head` null (up to kAdapterDirectRows rows) kernels read `ids`;
+// otherwise adapter_route_kernel filled the rest: group g (adapter g; count: no adapter; count + 1:
+// ids out of range) holds rows perm[starts[g], starts[g + 1]).
+struct AdapterBatch {
+  const int32_t *ids;     // [rows]
+  int32_t *head;          // tiles of adapters, tiles of all groups, runs
+  int32_t *starts;        // [count + 3]
+  int32_t *perm;          // [rows]
+  int32_t *tiles;         // group, first position of every tile of up to 64 rows
+  int32_t *outer;         // group, first, end, slot of partial sums (-1: none) of every run of rows
+  int32_t *runs;          // [count] first slot and number of runs of every adapter
+  int64_t rows;
+  int32_t count;
+  int32_t run_rows;       // rows of a run (a multiple of 64), or 0: no runs wanted
+};
+
+struct AdapterRouteArgs {
+  AdapterBatch batch;
+  uint32_t *fault;
+};
+
+// partials [range, row, rp] = the K range's part of A_a x[row].
+struct AdapterShrinkJob {
+  const void *x;             // [rows, k], row stride ldx
+  const void *w;             // [count, w_rows, k]
+  float *partials;
+  int64_t ldx;
+  int64_t k;
+  int64_t w_rows;
+  int64_t ranges;
+  int64_t steps_per_range;   // steps of 64 bytes
+};
+struct AdapterShrinkArgs {
+  AdapterBatch batch;
+  const int32_t *ranks;      // [count] or null: max_rank
+  AdapterShrinkJob job[2];   // the second with ranges 0: none
+  int32_t max_rank;
+  int32_t rp;                // columns of a partial row: 16, 32, 64 or 128
+};
+
+// out [rows, n] = act(base + scale_a (sum of partials) . w_a^T).
+struct AdapterExpandArgs {
+  AdapterBatch batch;
+  const int32_t *ranks;
+  const float *scales;       // [count] or null: 1
+  const float *partials;
+  const void *w;             // [count, n, ld_w]
+  const void *base;          // row stride ld_base, or null: 0
+  void *out;
+  uint32_t *fault;
+  int64_t ranges;
+  int64_t n;
+  int64_t ld_base;
+  int64_t ld_out;
+  int64_t columns;           // per workgroup
+  int32_t max_rank;
+  int32_t ld_w;
+  int32_t rp;
+  int32_t in_place;          // out is base and there is no activation
+  ActivationArgs act;
+};
+
+// Per-adapter transposes of the weights in use: at [count, k, rp], bt [count, rp, n].
+struct AdapterTransposeArgs {
+  AdapterBatch batch;
+  const int32_t *ranks;
+  const void *a;
+  const void *b;
+  void *at;
+  void *bt;
+  int64_t k;
+  int64_t n;
+  int32_t max_rank;
+  int32_t rp;
+  int32_t element;           // bytes
+};
+
+// terms [term, rp, stride]: coefficient r of position p (of the sorted rows), as the two bf16 terms
+// or one fp32 value, from the K ranges' partial sums.
+struct AdapterTermsArgs {
+  AdapterBatch batch;
+  const int32_t *ranks;
+  const float *partials[2];
+  void *terms[2];
+  int64_t ranges[2];
+  int64_t stride;
+  int32_t max_rank;
+  int32_t rp;
+  int32_t f32;
+};
+
+// Job 0: grad [count, max_rank, columns] (dA); job 1: grad [count, columns, max_rank] (dB).
+struct AdapterOuterJob {
+  const void *data;          // [rows, columns], row stride ld
+  const void *terms;
+  void *grad;
+  float *partials;           // [slot, rp, columns], or [slot, columns, rp]
+  int64_t ld;
+  int64_t columns;
+};
+struct AdapterOuterArgs {
+  AdapterBatch batch;
+  const int32_t *ranks;
+  const float *scales;
+  AdapterOuterJob job[2];
+  int64_t blocks0;           // 64-column blocks of job 0
+  int64_t stride;
+  int32_t max_rank;
+  int32_t rp;
+};
+
+// Gradients of adapters with no rows (zero) or with several runs (their sums).
+struct AdapterReduceArgs {
+  AdapterBatch batch;
+  const int32_t *ranks;
+  const float *scales;
+  AdapterOuterJob job[2];
+  int64_t blocks0;           // 1024-element blocks of job 0
+  int32_t max_rank;
+  int32_t rp;
+  int32_t dtype;
+};
+
+// Sizes and grids of the adapter operators at `rows` rows.
+struct AdapterPlan {
+  int64_t rp;
+  int64_t run_rows;          // backward
+  int64_t run_slots;         // backward: slots of partial sums
+  int64_t max_tiles;
+  int64_t max_runs;
+  int64_t ranges[2];         // K ranges of the products over input_width and over output_width
+  int64_t steps_per_range[2];
+  int64_t stride;            // backward: positions of a row of terms
+  // Byte offsets of the workspace's regions, and its size.
+  size_t route, partials[2], terms[2], sums[2], at, bt, bytes;
+};
+struct AdapterShape {
+  int64_t rows, count, max_rank, input_width, output_width;
+  int dtype;
+  bool backward;
+};
+AdapterPlan plan_adapter(const AdapterShape &shape);
+// What serves every row count up to `shape.rows`.
+size_t adapter_workspace_bytes(const AdapterShape &shape);
+AdapterBatch adapter_batch(const AdapterShape &shape, const AdapterPlan &plan, const int32_t *ids, unsigned char *workspace);
+KernelLaunch make_adapter_route(const AdapterRouteArgs &args);
+KernelLaunch make_adapter_shrink(const AdapterShrinkArgs &args, const AdapterPlan &plan, int dtype);
+KernelLaunch make_adapter_expand(const AdapterExpandArgs &args, const AdapterPlan &plan, int dtype);
+KernelLaunch make_adapter_transpose(const AdapterTransposeArgs &args);
+KernelLaunch make_adapter_terms(const AdapterTermsArgs &args, const AdapterPlan &plan);
+KernelLaunch make_adapter_outer(const AdapterOuterArgs &args, const AdapterPlan &plan, int dtype);
+KernelLaunch make_adapter_reduce(const AdapterReduceArgs &args);
+
 // ---------------------------------------------------------------- GEMMs
 // out[t, :] = epilogue(sum_k x[t, k] * w[n, k]) for the live rows t < rows.
 // With `gated`, w rows are interleaved Gate/Up (row 2j = gate_j, row 2j+1 = up_j)

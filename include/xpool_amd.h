@@ -63,6 +63,7 @@ enum { XP_GATE_UP_CONCATENATED = 1, XP_GATE_UP_INTERLEAVED = 2 };
 
 /* Sticky device fault bits. */
 #define XP_FAULT_SLOT_OUT_OF_RANGE 1u
+#define XP_FAULT_ADAPTER_OUT_OF_RANGE 2u
 
 typedef void *xp_stream_t;
 
@@ -173,6 +174,57 @@ int xp_projection_split(const void *x, int64_t rows, int64_t k, const void *w, i
  * Dense order runs between its projections (operators/dense.py:80-85). */
 int xp_activation(const void *inputs, void *output, int64_t rows, int64_t width, int dtype, int order,
                   const xp_activation_desc *activation, xp_stream_t stream);
+
+/* Low-rank adapters of one projection, as a pool on the device: a [count, max_rank, input_width],
+ * b [count, output_width, max_rank], of dtype (XP_DTYPE_BF16 / F16 / F32).  Adapter i has ranks[i]
+ * ranks (NULL: max_rank; clamped to 0..max_rank; what a and b hold past it is ignored) and the factor
+ * scales[i] (NULL: 1).  Up to 1024 adapters of at most 128 ranks.  No counterpart in the reference. */
+typedef struct {
+  const void *a;
+  const void *b;
+  const int32_t *ranks;
+  const float *scales;
+  int64_t count;
+  int64_t max_rank;
+  int64_t input_width;
+  int64_t output_width;
+  int dtype;
+} xp_adapter_pool;
+
+/* Workspace bytes that xp_adapter_apply (or, with `backward`, xp_adapter_backward) needs for every
+ * row count up to `rows`; 0 for sizes that they refuse.  The workspace is 16-byte aligned, its
+ * contents do not matter on entry, and calls that may overlap in time must not share one. */
+size_t xp_adapter_workspace_bytes(int64_t rows, int64_t count, int64_t max_rank, int64_t input_width,
+                                  int64_t output_width, int dtype, int backward);
+
+/* out[i] = act(base[i] + scale_a (x[i] . A_a^T) . B_a^T), a = ids[i] the adapter of row i's request;
+ * ids[i] = -1: no adapter, out[i] = act(base[i]).  base is the shared projection's result (NULL: 0), x
+ * [rows, input_width], base [rows, output_width], out [rows, output_width] (a gated activation:
+ * [rows, output_width / 2] over INTERLEAVED Gate/Up columns), element-aligned, with row strides of
+ * ldx, ld_base and ld_out elements.  Without an activation out may be base itself (same pointer and
+ * stride); no other overlap.  All sums are fp32; one rounding, at the store (with an activation the
+ * sum is not rounded before it, unlike xp_projection's).  The result of a row depends on its own
+ * values and id and on the row count, not on the other rows' adapters or order.  An id outside
+ * [-1, count) gives a row of quiet NaNs and ORs XP_FAULT_ADAPTER_OUT_OF_RANGE into fault_word (may be
+ * NULL). */
+int xp_adapter_apply(const xp_adapter_pool *pool, const int32_t *ids, int64_t rows, const void *x, int64_t ldx,
+                     const void *base, int64_t ld_base, void *out, int64_t ld_out,
+                     const xp_activation_desc *activation, void *workspace, size_t workspace_bytes,
+                     uint32_t *fault_word, xp_stream_t stream);
+
+/* Gradients of xp_adapter_apply without an activation, for grad_out [rows, output_width]:
+ *   grad_x[i] = base[i] + scale_a (grad_out[i] . B_a) . A_a   [rows, input_width]; base is the gradient
+ *     through the shared projection (NULL: 0) and may be grad_x itself; ids[i] = -1: base[i];
+ *   grad_a [count, max_rank, input_width]  = scale_a sum over a's rows of (grad_out[i] . B_a)^T x[i];
+ *   grad_b [count, output_width, max_rank] = scale_a sum over a's rows of grad_out[i]^T (x[i] . A_a^T).
+ * grad_a and grad_b are written whole: zero past an adapter's rank and for adapters without rows.
+ * grad_x may be NULL, and so may grad_a and grad_b together.  Sums run in an order that ids and
+ * sizes fix: repeated calls give the same bits.  Rows with an id outside [-1, count) give NaN rows of
+ * grad_x, nothing to the other two, and the fault bit.  rows = 0 clears grad_a and grad_b. */
+int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t rows, const void *x, int64_t ldx,
+                        const void *grad_out, int64_t ld_grad_out, const void *base, int64_t ld_base, void *grad_x,
+                        int64_t ld_grad_x, void *grad_a, void *grad_b, void *workspace, size_t workspace_bytes,
+                        uint32_t *fault_word, xp_stream_t stream);
 
 /* Scratch bytes the two projections above need for `rows` rows, n weight rows and
  * reduction length k (0 when the chosen kernel keeps the K reduction inside one
