@@ -112,6 +112,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _INT, [_P, _I64, _I64, _P, _I64, _P, _P, _INT, ctypes.POINTER(ActivationDesc), _P, _SIZE, _P],
     ),
     "xp_activation": (_INT, [_P, _P, _I64, _I64, _INT, _INT, ctypes.POINTER(ActivationDesc), _P]),
+    "xp_activation_backward": (_INT, [_P, _P, _P, _I64, _I64, _INT, _INT, ctypes.POINTER(ActivationDesc), _P]),
     "xp_adapter_workspace_bytes": (_SIZE, [_I64, _I64, _I64, _I64, _I64, _INT, _INT]),
     "xp_adapter_apply": (
         _INT,
@@ -156,6 +157,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "xp_moe_router_topk": (_INT, [_P, _INT, _I64, _I64, _I64, _INT, _P, _INT, _INT, _P, _P, _P]),
     "xp_moe_router_workspace_bytes": (_SIZE, [_I64, _I64, _I64, _INT]),
     "xp_moe_router": (_INT, [_P, _I64, _I64, _P, _I64, _I64, _INT, _INT, _INT, _P, _INT, _INT, _P, _P, _P, _SIZE, _P]),
+    "xp_moe_balance_workspace_bytes": (_SIZE, [_I64, _I64]),
+    "xp_moe_balance_loss": (_INT, [_P, _INT, _P, _I64, _I64, _I64, _INT, _P, _F32, _P, _P, _P, _SIZE, _P]),
+    "xp_moe_balance_backward": (_INT, [_P, _INT, _P, _I64, _I64, _I64, _INT, _P, _F32, _P, _P, _P]),
     "xp_moe_finalize_routing": (_INT, [_P, _P, _I64, _I64, _P, _P, _I64, _P, _I64, _F32, _P]),
     "xp_moe_workspace_bytes": (_SIZE, [_I64, _I64, _I64, _I64, _I64]),
     "xp_moe_workspace_layout": (_INT, [_I64, _I64, _I64, _I64, _I64, ctypes.POINTER(_SIZE)]),

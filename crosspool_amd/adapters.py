@@ -27,7 +27,7 @@ from crosspool_amd.operators import _DTYPE_CODES, Activation
 MAX_RANK = 128
 MAX_ADAPTERS = 1024
 
-__all__ = ["Adapter", "AdapterPlan", "AdapterWeights", "interleave_gate_up_adapters"]
+__all__ = ["Adapter", "AdapterPlan", "AdapterWeights", "DenseAdapterWeights", "interleave_gate_up_adapters"]
 
 
 def _require_pool(tensor: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, ...], device: torch.device) -> None:
@@ -66,6 +66,14 @@ class AdapterWeights:
             scales=None if scales is None else scales.data_ptr(), count=count, max_rank=max_rank,
             input_width=input_width, output_width=b.shape[1], dtype=_DTYPE_CODES[a.dtype],
         )
+
+
+@dataclass(frozen=True, slots=True)
+class DenseAdapterWeights:
+    """Adapter pools of a Dense layer's projections (``operators.Dense.run_into``), either left out."""
+
+    i_proj: AdapterWeights | None = None
+    o_proj: AdapterWeights | None = None
 
 
 def interleave_gate_up_adapters(

@@ -351,6 +351,164 @@ __global__ __launch_bounds__(256) void activation_kernel(ActivationLaunchArgs a)
   }
 }
 
+// ------------------------------------------------------------------ gradient of the activation
+// f(v) and f'(v) of one activation, in fp32 with the hardware's exp and reciprocal (relative error
+// below 2^-17 at any v that a 16-bit payload holds, against the store's 2^-9 or 2^-12).  The sigmoid
+// forms keep their relative accuracy in the tails; 0.5 (1 + tanh(y)) is sigmoid(2 y).
+enum class Slope : int { Silu = 1, Relu = 2, GeluErf = 3, GeluTanh = 4 };
+
+template <Slope KIND>
+__device__ __forceinline__ void value_and_slope(float v, float alpha, float &value, float &slope) {
+  if constexpr (KIND == Slope::Relu) {
+    const bool on = v > 0.0f || v != v;
+    value = on ? v : 0.0f;
+    slope = on ? 1.0f : 0.0f;
+  } else if constexpr (KIND == Slope::GeluErf) {
+    const float share = 0.5f * (1.0f + erff(v * 0.7071067811865476f));
+    value = v * share;
+    slope = share + v * 0.3989422804014327f * __expf(-0.5f * v * v);
+  } else if constexpr (KIND == Slope::GeluTanh) {
+    // Past 16 the sigmoid is 0 or 1 and its slope 0 (and v^3 may overflow).
+    const float near = fminf(fmaxf(v, -16.0f), 16.0f);
+    const float square = near * near;
+    const float twice = 2.0f * 0.7978845608028654f * near * (1.0f + 0.044715f * square);
+    const float share = v != v ? v : __builtin_amdgcn_rcpf(1.0f + __expf(-twice));
+    value = v * share;
+    slope = share + near * share * (1.0f - share) * (2.0f * 0.7978845608028654f) * (1.0f + 3.0f * 0.044715f * square);
+  } else {
+    const float share = __builtin_amdgcn_rcpf(1.0f + __expf(-alpha * v));
+    value = v * share;
+    // Past 128 one of the two factors is 0 (and alpha v may overflow).
+    const float near = fminf(fmaxf(alpha * v, -128.0f), 128.0f);
+    slope = share * (1.0f + near * (1.0f - share));
+  }
+}
+
+enum class GateLayout : int { Ungated = 0, Interleaved = 1, Concatenated = 2 };
+
+// Eight values (16 bytes) at any element alignment; past `count`, zeros are read and nothing written.
+template <class P>
+__device__ __forceinline__ void load_eight(const uint16_t *source, int count, float (&value)[8]) {
+  const unsigned char *bytes = reinterpret_cast<const unsigned char *>(source);
+  const u32x4 chunk = count >= 8 ? load16_any(bytes) : load_chunk_tail<P, P>(bytes, count);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    value[j] = P::widen(j % 2 == 0 ? chunk[j / 2] & 0xffffu : chunk[j / 2] >> 16);
+  }
+}
+template <class P>
+__device__ __forceinline__ void store_eight(uint16_t *target, int count, const float (&value)[8]) {
+  u32x4 packed;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    packed[j] = P::pack2(value[2 * j], value[2 * j + 1]);
+  }
+  if (count >= 8) {
+    __builtin_memcpy(target, &packed, 16);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 7; ++j) {
+    if (j < count) {
+      target[j] = static_cast<uint16_t>(packed[j / 2] >> (16 * (j % 2)));
+    }
+  }
+}
+
+// out = f(min(g, limit)) (clamp(u, -limit, limit) + offset) =: f h, so dg = dout h f' where g <= limit,
+// du = dout f where |u| <= limit; ungated dv = dout f'.  A thread takes eight output columns: INTERLEAVED
+// pairs and ungated values are flat arrays (the only ragged group is the last); CONCATENATED rows go
+// by row.  Bound by memory: five values of traffic per output column.
+template <class P, Slope KIND, GateLayout LAYOUT>
+__global__ __launch_bounds__(256) void activation_backward_kernel(ActivationBackwardArgs a) {
+  // The group's row (CONCATENATED: whole rows are cut into groups) and first column.
+  const uint32_t group = blockIdx.x * 256u + threadIdx.x;
+  int64_t row = 0;
+  int64_t index = static_cast<int64_t>(group) * 8;
+  int64_t length = a.elements;
+  if constexpr (LAYOUT == GateLayout::Concatenated) {
+    row = group / a.row_groups;
+    index = static_cast<int64_t>(group - static_cast<uint32_t>(row) * a.row_groups) * 8;
+    length = row * a.width < a.elements ? a.width : 0;
+  }
+  if (index >= length) {
+    return;
+  }
+  const int count = length - index < 8 ? static_cast<int>(length - index) : 8;
+  const ActivationArgs &act = a.act;
+  const uint16_t *inputs = static_cast<const uint16_t *>(a.inputs);
+  uint16_t *out = static_cast<uint16_t *>(a.grad_inputs);
+  float grad[8];
+  if constexpr (LAYOUT == GateLayout::Ungated) {
+    float value[8];
+    load_eight<P>(inputs + index, count, value);
+    load_eight<P>(static_cast<const uint16_t *>(a.grad_output) + index, count, grad);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float unused;
+      float slope;
+      value_and_slope<KIND>(value[j], act.alpha, unused, slope);
+      grad[j] *= slope;
+    }
+    store_eight<P>(out + index, count, grad);
+  } else {
+    float first[8];   // INTERLEAVED: the first four pairs; CONCATENATED: Gate
+    float second[8];  // the other four pairs; Up
+    constexpr bool PAIRS = LAYOUT == GateLayout::Interleaved;
+    const int64_t gate_at = PAIRS ? 2 * index : row * 2 * a.width + index;
+    const int64_t up_at = PAIRS ? gate_at + 8 : gate_at + a.width;
+    const int gate_count = PAIRS ? (count >= 4 ? 8 : 2 * count) : count;
+    const int up_count = PAIRS ? 2 * count - gate_count : count;
+    load_eight<P>(inputs + gate_at, gate_count, first);
+    load_eight<P>(inputs + up_at, up_count, second);
+    load_eight<P>(static_cast<const uint16_t *>(a.grad_output) + (PAIRS ? index : row * a.width + index), count, grad);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float &gate = PAIRS ? (j < 4 ? first[2 * j] : second[2 * j - 8]) : first[j];
+      float &up = PAIRS ? (j < 4 ? first[2 * j + 1] : second[2 * j - 7]) : second[j];
+      float clipped = gate;
+      float factor = up;
+      bool gate_on = true;
+      bool up_on = true;
+      if (act.has_limit) {
+        clipped = fminf(gate, act.limit);
+        factor = fminf(fmaxf(up, -act.limit), act.limit);
+        gate_on = gate <= act.limit;
+        up_on = fabsf(up) <= act.limit;
+      }
+      float value;
+      float slope;
+      value_and_slope<KIND>(clipped, act.alpha, value, slope);
+      gate = gate_on ? grad[j] * slope * (factor + act.up_offset) : 0.0f;
+      up = up_on ? grad[j] * value : 0.0f;
+    }
+    store_eight<P>(out + gate_at, gate_count, first);
+    store_eight<P>(out + up_at, up_count, second);
+  }
+}
+
+template <class P, Slope KIND>
+const void *activation_backward_for(const ActivationBackwardArgs &args) {
+  if (args.act.gated == 0) {
+    return reinterpret_cast<const void *>(&activation_backward_kernel<P, KIND, GateLayout::Ungated>);
+  }
+  return args.interleaved ? reinterpret_cast<const void *>(&activation_backward_kernel<P, KIND, GateLayout::Interleaved>)
+                          : reinterpret_cast<const void *>(&activation_backward_kernel<P, KIND, GateLayout::Concatenated>);
+}
+
+template <class P>
+const void *activation_backward_for(const ActivationBackwardArgs &args) {
+  switch (args.act.function) {
+    case kActivationRelu:
+      return activation_backward_for<P, Slope::Relu>(args);
+    case kActivationGelu:
+      return args.act.approximate_tanh ? activation_backward_for<P, Slope::GeluTanh>(args)
+                                       : activation_backward_for<P, Slope::GeluErf>(args);
+    default:
+      return activation_backward_for<P, Slope::Silu>(args);
+  }
+}
+
 }  // namespace
 
 // Tile and K ranges of a projection from a cost model in microseconds.  A workgroup's slabs
@@ -466,6 +624,19 @@ KernelLaunch make_activation(const ActivationLaunchArgs &args) {
   kernel.grid = dim3(static_cast<unsigned>(blocks < 4096 ? (blocks > 0 ? blocks : 1) : 4096), 1, 1);
   kernel.block = dim3(256, 1, 1);
   kernel.set_args(args);
+  return kernel;
+}
+
+KernelLaunch make_activation_backward(const ActivationBackwardArgs &args) {
+  KernelLaunch kernel;
+  kernel.func = args.dtype == kDtypeF16 ? activation_backward_for<F16Payload>(args) : activation_backward_for<Bf16Payload>(args);
+  ActivationBackwardArgs record = args;
+  record.row_groups = static_cast<uint32_t>((args.width + 7) / 8);
+  const bool by_row = args.act.gated != 0 && !args.interleaved;
+  const int64_t groups = by_row ? args.elements / args.width * record.row_groups : (args.elements + 7) / 8;
+  kernel.grid = dim3(static_cast<unsigned>((groups + 255) / 256), 1, 1);
+  kernel.block = dim3(256, 1, 1);
+  kernel.set_args(record);
   return kernel;
 }
 

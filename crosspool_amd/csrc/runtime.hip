@@ -1648,6 +1648,47 @@ int xp_activation(const void *inputs, void *output, int64_t rows, int64_t width,
   return XP_OK;
 }
 
+int xp_activation_backward(const void *inputs, const void *grad_output, void *grad_inputs, int64_t rows, int64_t width,
+                           int dtype, int order, const xp_activation_desc *activation, xp_stream_t stream) {
+  XP_REQUIRE(activation != nullptr, "activation descriptor must be non-null");
+  XP_REQUIRE(rows >= 0 && width >= 0 && (width == 0 || rows <= (int64_t{1} << 31) / width),
+             "activation extents must be non-negative and hold at most 2^31 values");
+  XP_REQUIRE(dtype == XP_DTYPE_BF16 || dtype == XP_DTYPE_F16, "standalone activations take bf16 or fp16 payloads");
+  ActivationBackwardArgs args{};
+  if (const int status = activation_record(activation, args.act); status != XP_OK) {
+    return status;
+  }
+  const bool gated = args.act.gated != 0;
+  XP_REQUIRE(!gated || order == XP_GATE_UP_INTERLEAVED || order == XP_GATE_UP_CONCATENATED,
+             "gated activation requires a Gate/Up order");
+  const int64_t elements = rows * width;
+  if (elements == 0) {
+    return XP_OK;
+  }
+  XP_REQUIRE(inputs != nullptr && grad_output != nullptr && grad_inputs != nullptr, "activation pointers must be non-null");
+  XP_REQUIRE(aligned_to(inputs, 2) && aligned_to(grad_output, 2) && aligned_to(grad_inputs, 2),
+             "activation payloads must be 2-byte aligned");
+  const auto overlaps = [&](const void *other, int64_t values) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(grad_inputs);
+    const uintptr_t b = reinterpret_cast<uintptr_t>(other);
+    const int64_t own = elements * (gated ? 2 : 1);
+    return a < b + static_cast<uintptr_t>(values * 2) && b < a + static_cast<uintptr_t>(own * 2);
+  };
+  XP_REQUIRE(inputs == grad_inputs || !overlaps(inputs, elements * (gated ? 2 : 1)),
+             "the input gradient may be the inputs only whole");
+  XP_REQUIRE(!overlaps(grad_output, elements) || (!gated && grad_output == grad_inputs),
+             "the input gradient may be the output gradient only whole and ungated");
+  args.inputs = inputs;
+  args.grad_output = grad_output;
+  args.grad_inputs = grad_inputs;
+  args.elements = elements;
+  args.width = width;
+  args.dtype = dtype;
+  args.interleaved = order == XP_GATE_UP_INTERLEAVED;
+  XP_HIP_CHECK(launch(make_activation_backward(args), static_cast<hipStream_t>(stream)));
+  return XP_OK;
+}
+
 namespace {
 
 // Elements [first, first + (rows - 1) ld + width) of two operands: whether their bytes overlap.
@@ -2638,6 +2679,92 @@ size_t xp_moe_router_workspace_bytes(int64_t rows, int64_t hidden, int64_t exper
   }
   // For every row count up to `rows`: an operator's workspace serves fewer live rows.
   return offset + align_up(projection_scratch_bytes(rows, experts, hidden, precision == XP_ROUTER_PRECISION_FP32 ? 4 : 2), 256);
+}
+
+namespace {
+
+constexpr int64_t kBalanceMaxRows = int64_t{1} << 24;
+
+// The checks that both balance entry points share.
+int balance_record(const void *logits, int logits_dtype, int64_t rows, int64_t experts, int64_t topk, int algorithm,
+                   const int32_t *payload_rows, float coefficient, BalanceArgs &args) {
+  XP_REQUIRE(rows >= 0 && rows <= kBalanceMaxRows, "balance rows must be between 0 and 16777216");
+  XP_REQUIRE(logits_dtype == XP_DTYPE_BF16 || logits_dtype == XP_DTYPE_F16 || logits_dtype == XP_DTYPE_F32,
+             "logits must be bf16, fp16 or fp32");
+  XP_REQUIRE(experts >= 1 && experts <= kMoeMaxExperts, "the router supports 1 to 1024 experts");
+  XP_REQUIRE(topk >= 1 && topk <= experts && topk <= 64, "topk must be between 1 and min(experts, 64)");
+  XP_REQUIRE(algorithm == XP_ROUTER_SOFTMAX || algorithm == XP_ROUTER_SIGMOID, "router algorithm is unknown");
+  XP_REQUIRE(std::isfinite(coefficient), "the balance coefficient must be finite");
+  XP_REQUIRE(aligned_to(logits, dtype_bytes(logits_dtype)) && aligned_to(payload_rows, 4),
+             "balance operands must be aligned to their element size");
+  args.logits = logits;
+  args.payload_rows = payload_rows;
+  args.rows = rows;
+  args.experts = static_cast<int32_t>(experts);
+  args.topk = static_cast<int32_t>(topk);
+  args.softmax = algorithm == XP_ROUTER_SOFTMAX ? 1 : 0;
+  args.dtype = logits_dtype;
+  args.coefficient = coefficient;
+  return XP_OK;
+}
+
+}  // namespace
+
+size_t xp_moe_balance_workspace_bytes(int64_t rows, int64_t experts) {
+  if (rows < 0 || rows > kBalanceMaxRows || experts < 1 || experts > kMoeMaxExperts) {
+    return 0;
+  }
+  const int64_t blocks = balance_blocks(rows, experts);
+  return blocks > 1 ? static_cast<size_t>(blocks * experts * 8) : 0;
+}
+
+int xp_moe_balance_loss(const void *logits, int logits_dtype, const int32_t *ids, int64_t rows, int64_t experts,
+                        int64_t topk, int algorithm, const int32_t *payload_rows, float coefficient, int32_t *counts,
+                        float *loss, void *workspace, size_t workspace_bytes, xp_stream_t stream) {
+  BalanceArgs args{};
+  if (const int status = balance_record(logits, logits_dtype, rows, experts, topk, algorithm, payload_rows, coefficient,
+                                        args);
+      status != XP_OK) {
+    return status;
+  }
+  XP_REQUIRE((rows == 0 || ids != nullptr) && counts != nullptr && (logits == nullptr || loss != nullptr),
+             "balance pointers must be non-null (logits and loss may be left out together)");
+  XP_REQUIRE(rows == 0 || logits != nullptr || loss == nullptr, "a balance loss needs the logits");
+  XP_REQUIRE(aligned_to(ids, 4) && aligned_to(counts, 4) && aligned_to(loss, 4), "balance operands must be 4-byte aligned");
+  args.blocks = balance_blocks(rows, experts);
+  XP_REQUIRE(args.blocks == 1 || (workspace != nullptr && aligned16(workspace) &&
+                                  workspace_bytes >= xp_moe_balance_workspace_bytes(rows, experts)),
+             "balance workspace is missing, unaligned or smaller than xp_moe_balance_workspace_bytes");
+  args.ids = ids;
+  args.counts = counts;
+  args.loss = loss;
+  args.partial_counts = static_cast<int32_t *>(workspace);
+  args.partial_shares = reinterpret_cast<float *>(args.partial_counts + args.blocks * experts);
+  XP_HIP_CHECK(launch(make_balance(args), static_cast<hipStream_t>(stream)));
+  XP_HIP_CHECK(launch(make_balance_finish(args), static_cast<hipStream_t>(stream)));
+  return XP_OK;
+}
+
+int xp_moe_balance_backward(const void *logits, int logits_dtype, const int32_t *counts, int64_t rows, int64_t experts,
+                            int64_t topk, int algorithm, const int32_t *payload_rows, float coefficient,
+                            const float *grad_loss, void *grad_logits, xp_stream_t stream) {
+  BalanceArgs args{};
+  if (const int status = balance_record(logits, logits_dtype, rows, experts, topk, algorithm, payload_rows, coefficient,
+                                        args);
+      status != XP_OK) {
+    return status;
+  }
+  if (rows == 0) {
+    return XP_OK;
+  }
+  XP_REQUIRE(logits != nullptr && counts != nullptr && grad_logits != nullptr, "balance pointers must be non-null");
+  XP_REQUIRE(aligned_to(counts, 4) && aligned_to(grad_loss, 4) && aligned_to(grad_logits, dtype_bytes(logits_dtype)),
+             "balance operands must be aligned to their element size");
+  args.counts = const_cast<int32_t *>(counts);
+  args.grad_loss = grad_loss;
+  args.grad_logits = grad_logits;
+  XP_HIP_CHECK(launch(make_balance_backward(args), static_cast<hipStream_t>(stream)));
+  return XP_OK;
 }
 
 int xp_moe_router_topk(const void *logits, int logits_dtype, int64_t rows, int64_t experts, int64_t topk,

@@ -339,6 +339,45 @@ struct ActivationLaunchArgs {
 
 KernelLaunch make_activation(const ActivationLaunchArgs &args);
 
+// grad_inputs (shaped as inputs) = the activation's gradient for grad_output [elements].
+struct ActivationBackwardArgs {
+  const void *inputs;
+  const void *grad_output;
+  void *grad_inputs;
+  int64_t elements;
+  int64_t width;
+  int32_t dtype;
+  int32_t interleaved;
+  uint32_t row_groups;  // CONCATENATED: groups of eight columns per row (set by make_activation_backward)
+  ActivationArgs act;
+};
+KernelLaunch make_activation_backward(const ActivationBackwardArgs &args);
+
+// ---------------------------------------------------------------- expert balance
+struct BalanceArgs {
+  const void *logits;            // [rows, experts] of dtype, or null: counts alone
+  const int32_t *ids;            // [rows, topk]
+  const int32_t *payload_rows;   // live rows, or null: all
+  int32_t *counts;               // [experts]
+  float *loss;
+  int32_t *partial_counts;       // [blocks, experts]
+  float *partial_shares;
+  const float *grad_loss;        // backward: one value, or null: 1
+  void *grad_logits;             // backward: [rows, experts] of dtype
+  int64_t rows;
+  int64_t blocks;
+  int32_t experts;
+  int32_t topk;
+  int32_t softmax;
+  int32_t dtype;
+  float coefficient;
+};
+// Workgroups of the loss; more than one leave their sums to make_balance_finish's launch.
+int64_t balance_blocks(int64_t rows, int64_t experts);
+KernelLaunch make_balance(const BalanceArgs &args);
+KernelLaunch make_balance_finish(const BalanceArgs &args);
+KernelLaunch make_balance_backward(const BalanceArgs &args);
+
 // ---------------------------------------------------------------- adapters
 constexpr int kAdapterMaxRank = 128;
 constexpr int kAdapterMaxCount = 1024;

@@ -34,6 +34,7 @@ from crosspool_amd.ffn import (
 from crosspool_amd.weights import validate_weight_tensor
 
 __all__ = [
+    "BalanceLoss",
     "Experts",
     "MoeFfnWeights",
     "MoeLayerSpec",
@@ -328,6 +329,119 @@ def router_topk(
         _ptr(correction_bias), int(renormalize), int(weight_rounding), _ptr(ids), _ptr(weights), _stream(),
     )
     return ids, weights
+
+
+class BalanceLoss:
+    """Per-expert route counts and the balance loss of a Router, with the gradient of its logits.
+
+    ``loss = coefficient * sum_e f_e * P_e`` with ``f_e`` expert e's share of the routes (times the
+    expert count) and ``P_e`` its mean score over the live rows: the softmax of the logits, or their
+    sigmoids divided by the row's sum.  ``counts`` (int32 ``[experts]``) and ``loss`` (fp32 ``[1]``) are
+    the outputs of :meth:`run_into`; served layers read ``counts`` as the experts' load.  The reference
+    has no counterpart; the operator follows ``Router``'s.
+    """
+
+    def __init__(
+        self,
+        *,
+        row_capacity: int,
+        routed_expert_count: int,
+        routed_topk: int,
+        algorithm: RouterAlgorithm = RouterAlgorithm.SOFTMAX,
+        coefficient: float = 1.0,
+        device: torch.device | None = None,
+    ) -> None:
+        if not 1 <= routed_topk <= min(routed_expert_count, 64) or routed_expert_count > 1024:
+            raise ValueError("balance supports up to 1024 experts and a TopK of at most min(experts, 64)")
+        if not 1 <= row_capacity <= 1 << 24:
+            raise ValueError("balance rows must be between 1 and 16777216")
+        if not math.isfinite(coefficient):
+            raise ValueError("the balance coefficient must be finite")
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.row_capacity = row_capacity
+        self.routed_expert_count = routed_expert_count
+        self.routed_topk = routed_topk
+        self.algorithm = RouterAlgorithm(algorithm)
+        self.coefficient = float(coefficient)
+        nbytes = int(_native.library().xp_moe_balance_workspace_bytes(row_capacity, routed_expert_count))
+        self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=self.device)
+        self.counts = torch.zeros(routed_expert_count, dtype=torch.int32, device=self.device)
+        self.loss = torch.zeros(1, dtype=torch.float32, device=self.device)
+
+    def _check(self, tensor: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, ...]) -> None:
+        if tensor.dtype is not dtype or tensor.shape != shape or tensor.device != self.device or not tensor.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {self.device}")
+
+    def _logits_code(self, logits: torch.Tensor, rows: int) -> int:
+        if logits.dtype is torch.float32:
+            code = _native.XP_DTYPE_F32
+        else:
+            code = _native.payload_dtype_code(logits.dtype)
+        self._check(logits, "logits", logits.dtype, (rows, self.routed_expert_count))
+        return code
+
+    def _live(self, rows: int, payload_rows: torch.Tensor | None) -> int | None:
+        if rows > self.row_capacity:
+            raise ValueError(f"{rows} balance rows exceed the prepared capacity {self.row_capacity}")
+        if torch.cuda.current_device() != self.device.index:
+            raise ValueError(f"the balance operator of {self.device} needs it as the current device")
+        if payload_rows is None:
+            return None
+        if payload_rows.dtype is not torch.int32 or payload_rows.numel() != 1 or payload_rows.device != self.device:
+            raise ValueError(f"payload rows must be one int32 value on {self.device}")
+        return payload_rows.data_ptr()
+
+    def run_into(
+        self, *, ids: torch.Tensor, logits: torch.Tensor | None = None, payload_rows: torch.Tensor | None = None
+    ) -> None:
+        """Write ``counts`` of the routes ``ids`` ``[rows, topk]`` and, given the ``logits``
+        ``[rows, experts]`` (bf16, fp16 or fp32), ``loss``; over the first ``payload_rows`` rows (an int32
+        value on the device, default all).  Ids outside ``[0, experts)`` are not counted."""
+
+        rows = ids.shape[0]
+        live = self._live(rows, payload_rows)
+        self._check(ids, "ids", torch.int32, (rows, self.routed_topk))
+        code = _native.XP_DTYPE_F32 if logits is None else self._logits_code(logits, rows)
+        _native.call(
+            "xp_moe_balance_loss", None if logits is None else logits.data_ptr(), code, ids.data_ptr(), rows,
+            self.routed_expert_count, self.routed_topk, int(self.algorithm), live, self.coefficient,
+            self.counts.data_ptr(), None if logits is None else self.loss.data_ptr(), self.workspace.data_ptr(),
+            self.workspace.numel(), _native.current_stream(self.device.index),
+        )
+
+    def backward_into(
+        self,
+        *,
+        logits: torch.Tensor,
+        grad_logits: torch.Tensor,
+        grad_loss: torch.Tensor | None = None,
+        payload_rows: torch.Tensor | None = None,
+        counts: torch.Tensor | None = None,
+    ) -> None:
+        """Write the gradient of ``loss`` times ``grad_loss`` (an fp32 value on the device, default 1) in
+        the logits to ``grad_logits`` (which may be ``logits``); zero past ``payload_rows``.  ``counts``,
+        default those of the last :meth:`run_into`, are constants of the gradient."""
+
+        if logits.ndim != 2:
+            raise ValueError("logits must be a matrix")
+        rows = logits.shape[0]
+        live = self._live(rows, payload_rows)
+        code = self._logits_code(logits, rows)
+        self._check(grad_logits, "grad_logits", logits.dtype, (rows, self.routed_expert_count))
+        counts = self.counts if counts is None else counts
+        self._check(counts, "counts", torch.int32, (self.routed_expert_count,))
+        if grad_loss is not None and (
+            grad_loss.dtype is not torch.float32 or grad_loss.numel() != 1 or grad_loss.device != self.device
+        ):
+            raise ValueError(f"the loss gradient must be one fp32 value on {self.device}")
+        _native.call(
+            "xp_moe_balance_backward", logits.data_ptr(), code, counts.data_ptr(), rows, self.routed_expert_count,
+            self.routed_topk, int(self.algorithm), live, self.coefficient,
+            None if grad_loss is None else grad_loss.data_ptr(), grad_logits.data_ptr(),
+            _native.current_stream(self.device.index),
+        )
 
 
 def finalize_moe_routing(

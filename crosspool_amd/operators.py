@@ -23,6 +23,7 @@ from __future__ import annotations
 import ctypes
 import math
 from dataclasses import dataclass
+from typing import TYPE_CHECKING
 
 import torch
 
@@ -30,6 +31,9 @@ from crosspool_amd import _native
 from crosspool_amd.execution import WorkspaceLayout
 from crosspool_amd.ffn import GateTransform, GateUpOrder, GeluActivation, ReluActivation, SiluActivation
 from crosspool_amd.weights import DenseFfnWeights, ProjectionWeights
+
+if TYPE_CHECKING:
+    from crosspool_amd.adapters import AdapterPlan, DenseAdapterWeights
 
 ActivationSpec = SiluActivation | ReluActivation | GeluActivation
 
@@ -142,6 +146,45 @@ class Activation:
         _native.call(
             "xp_activation", _ptr(inputs), _ptr(output), rows, width, _DTYPE_CODES[output.dtype],
             _ORDER_CODES.get(order, 0), ctypes.byref(desc), _stream(),
+        )
+
+    def backward_into(
+        self,
+        *,
+        inputs: torch.Tensor,
+        grad_output: torch.Tensor,
+        grad_inputs: torch.Tensor,
+        order: GateUpOrder | None,
+    ) -> None:
+        """Gradient of :meth:`apply_into`'s inputs, in their shape and order (no counterpart in the reference).
+
+        A value clipped by the gate transform's limit gets none; one at the limit does.  ``grad_inputs``
+        may be ``inputs`` itself, and for an ungated activation ``grad_output`` itself.
+        """
+
+        if self.gate is not None and order is None:
+            raise ValueError("gated activation requires a Gate/Up order")
+        dtype = inputs.dtype
+        if dtype not in (torch.bfloat16, torch.float16) or grad_output.dtype is not dtype or grad_inputs.dtype is not dtype:
+            raise ValueError("activation payloads must share one bf16 or fp16 dtype")
+        device = inputs.device
+        if device.type != "cuda" or grad_output.device != device or grad_inputs.device != device:
+            raise ValueError("activation payloads must share one GPU")
+        if device.index != torch.cuda.current_device():
+            raise ValueError(f"activation payloads of {device} need it as the current device")
+        if not (inputs.is_contiguous() and grad_output.is_contiguous() and grad_inputs.is_contiguous()):
+            raise ValueError("activation payloads must be contiguous")
+        if grad_output.ndim < 1:
+            raise ValueError("activation payloads must have rows")
+        width = grad_output.shape[-1]
+        wide = width if self.gate is None else 2 * width
+        if inputs.shape != (*grad_output.shape[:-1], wide) or grad_inputs.shape != inputs.shape:
+            raise ValueError("gated inputs hold two values per output, ungated ones one")
+        rows = grad_output.numel() // width if width else 0
+        desc = self.descriptor()
+        _native.call(
+            "xp_activation_backward", _ptr(inputs), _ptr(grad_output), _ptr(grad_inputs), rows, width,
+            _DTYPE_CODES[dtype], _ORDER_CODES.get(order, 0), ctypes.byref(desc), _stream(),
         )
 
 
@@ -273,58 +316,136 @@ class DenseSignature:
 
 
 @dataclass(frozen=True, slots=True)
+class DenseAdapterLayout:
+    """Adapter pools beside a Dense layer's projections: their adapters, and the largest rank of each
+    projection's (None: that projection has no pool)."""
+
+    adapter_count: int
+    i_proj_rank: int | None = None
+    o_proj_rank: int | None = None
+
+    def __post_init__(self) -> None:
+        if self.i_proj_rank is None and self.o_proj_rank is None:
+            raise ValueError("a Dense adapter layout names a rank for at least one projection")
+
+
+@dataclass(frozen=True, slots=True)
 class DenseExecutionPlan:
-    """Two prepared projections and their shared intermediate storage (dense.py:14-52)."""
+    """Two prepared projections and their shared intermediate storage (dense.py:14-52).
+
+    With ``adapters`` the layer also takes low-rank adapters by row (``crosspool_amd.adapters``); an i_proj
+    with a pool leaves the activation to the kernel that adds its adapters.
+    """
 
     signature: DenseSignature
     i_proj: GemmPlan
     o_proj: GemmPlan
     workspace: WorkspaceLayout
+    adapters: DenseAdapterLayout | None = None
+    i_proj_adapter: AdapterPlan | None = None
+    o_proj_adapter: AdapterPlan | None = None
 
     @classmethod
-    def prepare(cls, signature: DenseSignature) -> DenseExecutionPlan:
+    def prepare(cls, signature: DenseSignature, *, adapters: DenseAdapterLayout | None = None) -> DenseExecutionPlan:
         dtype = signature.payload_dtype
         capacity = signature.payload_row_capacity
         activated = TensorLayout((capacity, signature.local_intermediate_size), dtype)
+        adapted = adapters is not None and adapters.i_proj_rank is not None
+        activation = None if adapted else signature.activation
+        fused = activation is not None and activation.fused(order=signature.i_proj.gate_up_order) is not None
         i_proj = GemmPlan.prepare(
             input_layout=TensorLayout(signature.payload_shape, dtype),
             weight_layout=signature.i_proj,
-            result_layout=activated if signature.activation.fused(order=signature.i_proj.gate_up_order) is not None
-            else TensorLayout((capacity, signature.i_proj.values.shape[0]), dtype),
-            activation=signature.activation,
+            result_layout=activated if fused else TensorLayout((capacity, signature.i_proj.values.shape[0]), dtype),
+            activation=activation,
         )
         o_proj = GemmPlan.prepare(
             input_layout=activated, weight_layout=signature.o_proj,
             result_layout=TensorLayout(signature.payload_shape, dtype), activation=None,
         )
         regions = [(dtype, i_proj.output_layout.shape)]
-        if i_proj.fused_activation is None and not signature.activation.supports_inplace:
+        if i_proj.fused_activation is None and (adapted or not signature.activation.supports_inplace):
             regions.append((dtype, activated.shape))
         regions += [(torch.uint8, (i_proj.workspace.nbytes,)), (torch.uint8, (o_proj.workspace.nbytes,))]
-        return cls(signature, i_proj, o_proj, WorkspaceLayout.from_regions(tuple(regions)))
+        plans: list[AdapterPlan | None] = [None, None]
+        if adapters is not None:
+            from crosspool_amd.adapters import AdapterPlan
+
+            for index, (rank, layout) in enumerate(
+                ((adapters.i_proj_rank, signature.i_proj), (adapters.o_proj_rank, signature.o_proj))
+            ):
+                if rank is not None:
+                    width, reduction = layout.values.shape
+                    plans[index] = AdapterPlan.prepare(
+                        row_capacity=capacity, adapter_count=adapters.adapter_count, max_rank=rank,
+                        input_width=reduction, output_width=width, dtype=dtype,
+                    )
+            # One region serves both: their calls follow one another.
+            regions.append((torch.uint8, (max(plan.workspace.nbytes for plan in plans if plan is not None),)))
+        return cls(signature, i_proj, o_proj, WorkspaceLayout.from_regions(tuple(regions)), adapters, *plans)
 
 
 class Dense:
     """Capture-time Dense computation over a prepared workspace (dense.py:55-86)."""
 
     def __init__(self, plan: DenseExecutionPlan, workspace: torch.Tensor) -> None:
-        views = plan.workspace.views(workspace)
+        views = list(plan.workspace.views(workspace))
         self.plan = plan
+        self.i_adapter = self.o_adapter = None
+        if plan.adapters is not None:
+            from crosspool_amd.adapters import Adapter
+
+            scratch = views.pop()
+            self.i_adapter = None if plan.i_proj_adapter is None else Adapter(plan.i_proj_adapter, scratch)
+            self.o_adapter = None if plan.o_proj_adapter is None else Adapter(plan.o_proj_adapter, scratch)
         self.projected = views[0]
-        separate = plan.i_proj.fused_activation is None and not plan.signature.activation.supports_inplace
+        separate = plan.i_proj.fused_activation is None and (
+            self.i_adapter is not None or not plan.signature.activation.supports_inplace
+        )
         self.activated = views[1] if separate else self.projected
         self.i_proj = Gemm(plan.i_proj, views[-2])
         self.o_proj = Gemm(plan.o_proj, views[-1])
 
-    def run_into(self, *, hidden_states: torch.Tensor, layer_weights: DenseFfnWeights, output: torch.Tensor) -> None:
-        """Write the complete rank-local partial of ``hidden_states`` into ``output``."""
+    def run_into(
+        self,
+        *,
+        hidden_states: torch.Tensor,
+        layer_weights: DenseFfnWeights,
+        output: torch.Tensor,
+        adapters: DenseAdapterWeights | None = None,
+        adapter_ids: torch.Tensor | None = None,
+        fault_word: torch.Tensor | None = None,
+    ) -> None:
+        """Write the complete rank-local partial of ``hidden_states`` into ``output``.
 
+        ``adapters`` (of a plan prepared for them) adds the low-rank adapters that ``adapter_ids`` (int32,
+        one per row, -1: none) names to each projection; an id outside the pool gives a row of NaN and a
+        bit in ``fault_word``.
+        """
+
+        if (adapters is None) != (adapter_ids is None):
+            raise ValueError("adapters and adapter ids come together")
+        if adapters is not None:
+            if (adapters.i_proj is None) != (self.i_adapter is None) or (adapters.o_proj is None) != (self.o_adapter is None):
+                raise ValueError("Dense adapters disagree with the prepared plan")
         rows = hidden_states.shape[0]
         projected = self.projected[:rows]
         self.i_proj.run_into(hidden_states, layer_weights.i_proj, output=projected)
         activated = self.activated[:rows]
-        if self.plan.i_proj.fused_activation is None:
-            self.plan.signature.activation.apply_into(
-                inputs=projected, output=activated, order=self.plan.i_proj.weight_layout.gate_up_order
+        activation, order = self.plan.signature.activation, self.plan.signature.i_proj.gate_up_order
+        pending = self.plan.i_proj.fused_activation is None
+        if adapters is not None and adapters.i_proj is not None:
+            fused = activation.fused(order=order)
+            self.i_adapter.run_into(
+                hidden_states, adapters.i_proj, adapter_ids=adapter_ids, base=projected,
+                output=projected if fused is None else activated, activation=fused, fault_word=fault_word,
             )
+            pending = fused is None
+        if pending:
+            activation.apply_into(inputs=projected, output=activated, order=order)
         self.o_proj.run_into(activated, layer_weights.o_proj, output=output)
+        if adapters is not None and adapters.o_proj is not None:
+            self.o_adapter.run_into(
+                activated, adapters.o_proj, adapter_ids=adapter_ids, base=output[:rows], output=output[:rows],
+                fault_word=fault_word,
+            )

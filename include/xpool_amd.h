@@ -175,6 +175,15 @@ int xp_projection_split(const void *x, int64_t rows, int64_t k, const void *w, i
 int xp_activation(const void *inputs, void *output, int64_t rows, int64_t width, int dtype, int order,
                   const xp_activation_desc *activation, xp_stream_t stream);
 
+/* Gradient of xp_activation: grad_inputs, shaped and ordered as inputs, from the projected inputs and
+ * grad_output [rows, width] (bf16 / fp16).  Gated, with h = clamp(u, -limit, limit) + up_offset:
+ * dg = dout h f'(min(g, limit)) where g <= limit, du = dout f(min(g, limit)) where |u| <= limit, else 0
+ * (limits only with has_limit); ungated: dv = dout f'(v).  fp32 inside, one rounding.  grad_inputs may be
+ * inputs itself, and ungated grad_output itself.  At most 2^31 values of grad_output.  No counterpart
+ * in the reference. */
+int xp_activation_backward(const void *inputs, const void *grad_output, void *grad_inputs, int64_t rows, int64_t width,
+                           int dtype, int order, const xp_activation_desc *activation, xp_stream_t stream);
+
 /* Low-rank adapters of one projection, as a pool on the device: a [count, max_rank, input_width],
  * b [count, output_width, max_rank], of dtype (XP_DTYPE_BF16 / F16 / F32).  Adapter i has ranks[i]
  * ranks (NULL: max_rank; clamped to 0..max_rank; what a and b hold past it is ignored) and the factor
@@ -483,6 +492,27 @@ int xp_moe_router(const void *hidden_states, int64_t rows, int64_t hidden, const
                   int64_t experts, int64_t topk, int algorithm, int precision, int payload_dtype,
                   const float *correction_bias, int renormalize, int weight_rounding, int32_t *ids, float *weights,
                   void *workspace, size_t workspace_bytes, xp_stream_t stream);
+
+/* Per-expert counts of the routes ids [rows, topk] (ids outside [0, experts) are not counted) and the
+ * balance loss of the Router's logits [rows, experts] (bf16 / fp16 / fp32) over the first *payload_rows
+ * rows (NULL: all):
+ *   loss = coefficient * sum_e (counts[e] * experts / (topk * T)) * (sum_t p[t, e] / T),
+ * T the live rows, p the softmax of a row's logits or their sigmoids divided by their sum
+ * (XP_ROUTER_SIGMOID); a row without any score (all logits -inf) has p = 0, no live row a loss of 0.
+ * counts is int32 [experts], loss one fp32 value.  logits and loss NULL: the counts alone.  The sums have
+ * one order: repeated calls give the same bits.  The workspace (16-byte aligned) serves every row count
+ * up to the one asked for; its contents do not matter on entry.  No counterpart in the reference. */
+size_t xp_moe_balance_workspace_bytes(int64_t rows, int64_t experts);
+int xp_moe_balance_loss(const void *logits, int logits_dtype, const int32_t *ids, int64_t rows, int64_t experts,
+                        int64_t topk, int algorithm, const int32_t *payload_rows, float coefficient, int32_t *counts,
+                        float *loss, void *workspace, size_t workspace_bytes, xp_stream_t stream);
+
+/* Gradient of that loss in the logits (counts, from xp_moe_balance_loss, are constants of it), times
+ * *grad_loss (NULL: 1): grad_logits [rows, experts] of the logits' dtype, which may be the logits
+ * themselves; rows past *payload_rows get zero. */
+int xp_moe_balance_backward(const void *logits, int logits_dtype, const int32_t *counts, int64_t rows, int64_t experts,
+                            int64_t topk, int algorithm, const int32_t *payload_rows, float coefficient,
+                            const float *grad_loss, void *grad_logits, xp_stream_t stream);
 
 /* Final Routing Metadata [capacity, effective_topk]: routed slots copy the Router's ids and
  * weights, shared slots s name expert routed_expert_count + s with weight

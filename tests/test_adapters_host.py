@@ -1,0 +1,156 @@
+"""What the adapter, activation-gradient and balance entry points refuse before any device call, and the
+sizes they ask for: no GPU needed."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from crosspool_amd import _native
+from crosspool_amd.adapters import AdapterPlan, AdapterWeights, interleave_gate_up_adapters
+from crosspool_amd.operators import DenseAdapterLayout
+
+BAD = _native.XP_ERROR_INVALID_ARGUMENT
+# Addresses that no refused call reads.
+P = 0x1000
+
+
+def pool(**changes):
+    fields = dict(a=P, b=P, ranks=None, scales=None, count=4, max_rank=16, input_width=64, output_width=48,
+                  dtype=_native.XP_DTYPE_BF16)
+    return ctypes.byref(_native.AdapterPool(**{**fields, **changes}))
+
+
+def workspace(rows, backward=0, count=4, rank=16, k=64, n=48, dtype=_native.XP_DTYPE_BF16):
+    return _native.library().xp_adapter_workspace_bytes(rows, count, rank, k, n, dtype, backward)
+
+
+def apply(target=None, **changes):
+    call = dict(ids=P, rows=8, x=0x10000, ldx=64, base=0x20000, ld_base=48, out=0x30000, ld_out=48, act=None, ws=0x40000,
+                ws_bytes=1 << 30)
+    call.update(changes)
+    return _native.library().xp_adapter_apply(target or pool(), *call.values(), None, None)
+
+
+def backward(target=None, **changes):
+    call = dict(ids=P, rows=8, x=0x10000, ldx=64, grad=0x20000, ld_grad=48, base=0x30000, ld_base=64, gx=0x50000, ld_gx=64,
+                ga=0x60000, gb=0x70000, ws=0x80000, ws_bytes=1 << 30)
+    call.update(changes)
+    return _native.library().xp_adapter_backward(target or pool(), *call.values(), None, None)
+
+
+@pytest.mark.parametrize("changes", [
+    dict(a=None), dict(b=None), dict(a=P + 1), dict(count=0), dict(count=1025), dict(max_rank=0), dict(max_rank=129),
+    dict(input_width=0), dict(output_width=-3), dict(input_width=(1 << 22) + 1), dict(dtype=0), dict(dtype=4),
+    dict(ranks=P + 2), dict(scales=P + 1),
+])
+def test_pools_are_checked(changes):
+    assert apply(pool(**changes)) == BAD
+    assert "adapter" in _native.last_error()
+    assert backward(pool(**changes)) == BAD
+
+
+def test_apply_refusals():
+    gated = _native.ActivationDesc(function=_native.XP_ACTIVATION_SILU, gated=1, alpha=1.0)
+    unknown = _native.ActivationDesc(function=9)
+    ungated = _native.ActivationDesc(function=_native.XP_ACTIVATION_RELU)
+    assert _native.library().xp_adapter_apply(None, P, 1, P, 64, None, 0, P, 48, None, P, 1, None, None) == BAD
+    for changes in (
+        dict(ids=None), dict(ids=P + 2), dict(rows=-1), dict(rows=(1 << 24) + 1), dict(x=None), dict(x=0x10001),
+        dict(ldx=63), dict(ldx=1 << 40), dict(base=0x20001), dict(ld_base=47), dict(out=None), dict(ld_out=0),
+        dict(ws=None), dict(ws=0x40008), dict(ws_bytes=workspace(8) - 1), dict(act=ctypes.byref(unknown)),
+        dict(out=0x10000),                                      # over the input
+        dict(out=0x20010), dict(out=0x20000, ld_out=64),        # over part of the base
+        dict(out=0x20000, act=ctypes.byref(ungated)),           # over the base with an activation
+    ):
+        assert apply(**changes) == BAD, changes
+        assert _native.last_error()
+    assert apply(pool(output_width=47), act=ctypes.byref(gated)) == BAD
+    assert apply(rows=0, x=None, out=None, ids=None, ws=None) == _native.XP_OK
+
+
+def test_backward_refusals():
+    for changes in (
+        dict(ids=None), dict(rows=-1), dict(x=None), dict(ldx=63), dict(grad=None), dict(ld_grad=47), dict(gx=0x50001),
+        dict(ld_gx=63), dict(ga=None), dict(gb=None), dict(ga=0x60001), dict(base=0x30001), dict(ld_base=2),
+        dict(gx=0x10000), dict(gx=0x20000), dict(gx=0x30010), dict(gx=0x30000, ld_gx=70), dict(ws=None),
+        dict(ws_bytes=workspace(8, 1) - 1),
+    ):
+        assert backward(**changes) == BAD, changes
+    assert backward(gx=None, ga=None, gb=None, base=None) == _native.XP_OK  # nothing asked for
+
+
+@pytest.mark.parametrize("backward", [0, 1])
+@pytest.mark.parametrize("k,n,rank,count", [(64, 48, 16, 4), (4096, 24576, 32, 32), (12288, 4096, 128, 1), (33, 5000, 3, 1024)])
+def test_a_workspace_serves_every_smaller_batch(k, n, rank, count, backward):
+    sizes = [1, 2, 63, 64, 65, 100, 128, 129, 1000, 2047, 8192, 8193, 33000, 70000]
+    asked = [workspace(rows, backward, count, rank, k, n) for rows in sizes]
+    assert asked == sorted(asked) and asked[0] > 0
+
+
+def test_workspace_of_refused_sizes_is_zero():
+    assert workspace(-1) == workspace(8, rank=0) == workspace(8, rank=129) == workspace(8, count=1025) == 0
+    assert workspace(8, k=0) == workspace(8, n=0) == workspace(8, dtype=0) == workspace((1 << 24) + 1) == 0
+    with pytest.raises(ValueError):
+        AdapterPlan.prepare(row_capacity=8, adapter_count=4, max_rank=129, input_width=8, output_width=8, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        AdapterPlan.prepare(row_capacity=0, adapter_count=4, max_rank=8, input_width=8, output_width=8, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        AdapterPlan.prepare(row_capacity=8, adapter_count=4, max_rank=8, input_width=8, output_width=8, dtype=torch.float64)
+
+
+def test_pools_on_the_cpu_are_refused():
+    with pytest.raises(ValueError, match="GPU"):
+        AdapterWeights(torch.zeros(1, 2, 3), torch.zeros(1, 4, 2))
+    with pytest.raises(ValueError):
+        DenseAdapterLayout(4)
+
+
+def test_interleaved_gate_and_up_adapters():
+    g = torch.Generator().manual_seed(0)
+    gate_a, up_a = torch.randn((2, 5), generator=g), torch.randn((3, 5), generator=g)
+    gate_b, up_b = torch.randn((4, 2), generator=g), torch.randn((4, 3), generator=g)
+    a, b = interleave_gate_up_adapters(gate_a, gate_b, up_a, up_b)
+    assert a.shape == (5, 5) and b.shape == (8, 5)
+    assert torch.allclose((b @ a)[0::2], gate_b @ gate_a) and torch.allclose((b @ a)[1::2], up_b @ up_a)
+    with pytest.raises(ValueError):
+        interleave_gate_up_adapters(gate_a, up_b, up_a, gate_b)
+
+
+def test_activation_backward_refusals():
+    call = _native.library().xp_activation_backward
+    silu = _native.ActivationDesc(function=_native.XP_ACTIVATION_SILU, gated=1, alpha=1.0)
+    desc, bf16, pairs = ctypes.byref(silu), _native.XP_DTYPE_BF16, _native.XP_GATE_UP_INTERLEAVED
+    good = dict(inputs=0x10000, grad=0x20000, out=0x30000, rows=4, width=8, dtype=bf16, order=pairs, desc=desc)
+    for changes in (
+        dict(desc=None), dict(rows=-1), dict(width=-1), dict(rows=1 << 31, width=2), dict(dtype=_native.XP_DTYPE_F32),
+        dict(order=0), dict(inputs=None), dict(grad=None), dict(out=None), dict(out=0x30001), dict(out=0x10002),
+        dict(out=0x20000),
+        dict(desc=ctypes.byref(_native.ActivationDesc(function=9))),
+    ):
+        assert call(*{**good, **changes}.values(), None) == BAD, changes
+    assert call(*{**good, "rows": 0}.values(), None) == _native.XP_OK
+
+
+def test_balance_refusals():
+    lib = _native.library()
+    good = dict(logits=P, dtype=_native.XP_DTYPE_F32, ids=P, rows=1000, experts=16, topk=2, algorithm=1, live=None,
+                coefficient=1.0, counts=P, loss=P, ws=P, ws_bytes=1 << 30)
+    for changes in (
+        dict(dtype=0), dict(ids=None), dict(rows=-1), dict(rows=(1 << 24) + 1), dict(experts=0), dict(experts=1025),
+        dict(topk=0), dict(topk=17), dict(algorithm=3), dict(coefficient=float("nan")), dict(coefficient=float("inf")),
+        dict(counts=None), dict(loss=None), dict(logits=None), dict(logits=P + 2), dict(live=P + 1), dict(ws=None),
+        dict(ws=P + 8), dict(ws_bytes=lib.xp_moe_balance_workspace_bytes(1000, 16) - 1),
+    ):
+        assert lib.xp_moe_balance_loss(*{**good, **changes}.values(), None) == BAD, changes
+    back = dict(logits=P, dtype=_native.XP_DTYPE_BF16, counts=P, rows=10, experts=16, topk=2, algorithm=2, live=None,
+                coefficient=1.0, grad_loss=None, out=P)
+    for changes in (dict(logits=None), dict(counts=None), dict(out=None), dict(out=P + 1), dict(grad_loss=P + 2),
+                    dict(algorithm=0), dict(dtype=9)):
+        assert lib.xp_moe_balance_backward(*{**back, **changes}.values(), None) == BAD, changes
+    assert lib.xp_moe_balance_backward(*{**back, "rows": 0}.values(), None) == _native.XP_OK
+    sizes = [lib.xp_moe_balance_workspace_bytes(rows, 128) for rows in (0, 1, 256, 257, 1000, 5000, 100000)]
+    assert sizes == sorted(sizes)
+    assert lib.xp_moe_balance_workspace_bytes(10, 0) == lib.xp_moe_balance_workspace_bytes(-1, 8) == 0
