@@ -13,45 +13,39 @@ constexpr int kRouteThreads = 1024;
 constexpr int kRouteWaves = kRouteThreads / kWave;
 constexpr int kRouteGroups = kAdapterMaxCount + 2;
 
-// Exclusive scan of one value per thread over the workgroup; `total` is the sum.
-__device__ int block_exclusive_scan(int value, int *wave_totals, int &total) {
+// Rows, tiles, runs and slots of partial sums of some groups, added up.
+struct RouteSums {
+  int value[4];
+};
+
+__device__ __forceinline__ RouteSums wave_inclusive_scan(RouteSums sums) {
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
-  int inclusive = value;
 #pragma unroll
   for (int offset = 1; offset < kWave; offset <<= 1) {
-    const int other = __shfl_up(inclusive, offset, kWave);
-    if (lane >= offset) {
-      inclusive += other;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int other = __shfl_up(sums.value[i], offset, kWave);
+      sums.value[i] += lane >= offset ? other : 0;
     }
   }
-  __syncthreads();  // an earlier scan's totals are read
-  if (lane == kWave - 1) {
-    wave_totals[wave] = inclusive;
-  }
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kRouteWaves; ++w) {
-    before += w < wave ? wave_totals[w] : 0;
-    total += wave_totals[w];
-  }
-  return before + inclusive - value;
+  return sums;
 }
 
 // A stable counting sort by one workgroup: every wave counts a contiguous sixteenth of the rows, the
 // counts are scanned over groups and waves, and each wave places its rows 64 at a time, a row's
 // place among the 64 being the number of earlier lanes of its group (from ballots over the bits of
 // the group).  Stable and free of racing increments, so the sums of the gradients have one order.
-// Bound by its own latency: 8 rows per lane at 8192 rows.
+// Bound by the latency of its steps: one read of the ids (kept in registers up to 8192 rows), four
+// barriers, one wave's scan where two groups per lane hold all of them.
+constexpr int kRouteKept = 8;
+
 __global__ __launch_bounds__(kRouteThreads) void adapter_route_kernel(AdapterRouteArgs a) {
-  __shared__ int counts[kRouteWaves][kRouteGroups];
+  __shared__ int counts[kRouteWaves * kRouteGroups];
   __shared__ int starts[kRouteGroups + 1];
   __shared__ int tile_starts[kRouteGroups + 1];
-  __shared__ int run_starts[kAdapterMaxCount + 1];
-  __shared__ int slot_starts[kAdapterMaxCount];
-  __shared__ int wave_totals[kRouteWaves];
+  __shared__ int run_starts[kRouteGroups + 1];
+  __shared__ int slot_starts[kRouteGroups];
+  __shared__ RouteSums wave_sums[kRouteWaves];
   const AdapterBatch &batch = a.batch;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -59,107 +53,150 @@ __global__ __launch_bounds__(kRouteThreads) void adapter_route_kernel(AdapterRou
   const int count = batch.count;
   const int groups = count + 2;
   const int rows = static_cast<int>(batch.rows);
-  for (int index = tid; index < kRouteWaves * kRouteGroups; index += kRouteThreads) {
-    (&counts[0][0])[index] = 0;
-  }
-  __syncthreads();
   const int share = ((rows + kRouteWaves - 1) / kRouteWaves + kWave - 1) / kWave * kWave;
   const int first = wave * share;
   const int last = first + share < rows ? first + share : rows;
+  int kept[kRouteKept];
+#pragma unroll
+  for (int i = 0; i < kRouteKept; ++i) {
+    const int row = first + i * kWave + lane;
+    kept[i] = row < last ? batch.ids[row] : -1;
+  }
+  for (int index = tid; index < kRouteWaves * groups; index += kRouteThreads) {
+    counts[index] = 0;
+  }
+  __syncthreads();
+  int *own = counts + wave * groups;
   bool bad = false;
-  for (int row = first + lane; row < last; row += kWave) {
-    const int group = adapter_group(batch.ids[row], count);
-    bad |= group > count;
-    atomicAdd(&counts[wave][group], 1);
+  auto count_row = [&](int row, int id) __attribute__((always_inline)) {
+    if (row < last) {
+      const int group = adapter_group(id, count);
+      bad |= group > count;
+      atomicAdd(&own[group], 1);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kRouteKept; ++i) {
+    count_row(first + i * kWave + lane, kept[i]);
+  }
+  for (int row = first + kRouteKept * kWave + lane; row < last; row += kWave) {
+    count_row(row, batch.ids[row]);
   }
   if (__ballot(bad) != 0 && lane == 0) {
     raise_fault(a.fault, kFaultAdapterOutOfRange);
   }
   __syncthreads();
-  // Two groups per thread: their rows, tiles, runs and slots of partial sums.
-  int length[2] = {0, 0};
-  int tiles[2] = {0, 0};
-  int runs[2] = {0, 0};
-  int slots[2] = {0, 0};
+  // Two groups per thread.
+  RouteSums mine[2] = {};
+  RouteSums both = {};
+  if (2 * tid < groups) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int group = 2 * tid + i;
-    if (group < groups) {
-      for (int w = 0; w < kRouteWaves; ++w) {
-        const int own = counts[w][group];
-        counts[w][group] = length[i];
-        length[i] += own;
-      }
-      tiles[i] = (length[i] + kAdapterTileRows - 1) / kAdapterTileRows;
-      if (group < count && batch.run_rows > 0) {
-        runs[i] = (length[i] + batch.run_rows - 1) / batch.run_rows;
-        slots[i] = runs[i] > 1 ? runs[i] : 0;
+    for (int i = 0; i < 2; ++i) {
+      const int group = 2 * tid + i;
+      if (group < groups) {
+        int length = 0;
+#pragma unroll
+        for (int w = 0; w < kRouteWaves; ++w) {
+          const int part = counts[w * groups + group];
+          counts[w * groups + group] = length;
+          length += part;
+        }
+        const bool runs = group < count && batch.run_rows > 0;
+        const int pieces = runs ? (length + batch.run_rows - 1) / batch.run_rows : 0;
+        mine[i] = {{length, (length + kAdapterTileRows - 1) / kAdapterTileRows, pieces, pieces > 1 ? pieces : 0}};
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          both.value[v] += mine[i].value[v];
+        }
       }
     }
   }
-  int total_rows;
-  int total_tiles;
-  int total_runs;
-  int total_slots;
-  const int row0 = block_exclusive_scan(length[0] + length[1], wave_totals, total_rows);
-  const int tile0 = block_exclusive_scan(tiles[0] + tiles[1], wave_totals, total_tiles);
-  const int run0 = block_exclusive_scan(runs[0] + runs[1], wave_totals, total_runs);
-  const int slot0 = block_exclusive_scan(slots[0] + slots[1], wave_totals, total_slots);
+  RouteSums before = {};
+  if (groups <= 2 * kWave) {
+    if (wave == 0) {
+      const RouteSums inclusive = wave_inclusive_scan(both);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int group = 2 * tid + i;
-    if (group < groups) {
-      starts[group] = row0 + (i > 0 ? length[0] : 0);
-      tile_starts[group] = tile0 + (i > 0 ? tiles[0] : 0);
-      batch.starts[group] = starts[group];
+      for (int v = 0; v < 4; ++v) {
+        before.value[v] = inclusive.value[v] - both.value[v];
+      }
     }
-    if (group < count) {
-      const int slot = slot0 + (i > 0 ? slots[0] : 0);
-      run_starts[group] = run0 + (i > 0 ? runs[0] : 0);
-      slot_starts[group] = runs[i] > 1 ? slot : -1;
-      if (batch.run_rows > 0) {
-        batch.runs[2 * group] = slot;
-        batch.runs[2 * group + 1] = runs[i];
+  } else {
+    const RouteSums inclusive = wave_inclusive_scan(both);
+    if (lane == kWave - 1) {
+      wave_sums[wave] = inclusive;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      before.value[v] = inclusive.value[v] - both.value[v];
+      for (int w = 0; w < wave; ++w) {
+        before.value[v] += wave_sums[w].value[v];
       }
     }
   }
-  if (tid == 0) {
-    starts[groups] = rows;
-    batch.starts[groups] = rows;
-    tile_starts[groups] = total_tiles;
-    run_starts[count] = total_runs;
-    batch.head[1] = total_tiles;
-    batch.head[2] = total_runs;
+  if (2 * tid < groups) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int group = 2 * tid + i;
+      if (group < groups) {
+        starts[group] = before.value[0];
+        tile_starts[group] = before.value[1];
+        run_starts[group] = before.value[2];
+        slot_starts[group] = mine[i].value[2] > 1 ? before.value[3] : -1;
+        if (group <= count) {
+          batch.starts[group] = before.value[0];
+        }
+        if (group < count && batch.run_rows > 0) {
+          batch.run_slots[2 * group] = before.value[3];
+          batch.run_slots[2 * group + 1] = mine[i].value[2];
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          before.value[v] += mine[i].value[v];
+        }
+        if (group == groups - 1) {
+          starts[groups] = before.value[0];
+          tile_starts[groups] = before.value[1];
+          run_starts[groups] = before.value[2];
+        }
+      }
+    }
   }
   __syncthreads();
-  if (tid == 0) {
-    batch.head[0] = tile_starts[count];
-  }
   // Placement.
-  for (int row64 = first; row64 < last; row64 += kWave) {
-    const int row = row64 + lane;
+  auto place = [&](int row, int id) __attribute__((always_inline)) {
     const bool live = row < last;
-    const int group = live ? adapter_group(batch.ids[row], count) : 0;
+    const int group = live ? adapter_group(id, count) : 0;
     unsigned long long same = __ballot(live);
     for (int bit = 1; bit < groups; bit <<= 1) {
       const unsigned long long set = __ballot((group & bit) != 0);
       same &= (group & bit) != 0 ? set : ~set;
     }
     if (live) {
-      const int before = __popcll(same & ((1ull << lane) - 1));
-      batch.perm[starts[group] + counts[wave][group] + before] = row;
-      if (before == 0) {
-        // After every lane of the wave has read the count: one wave runs in order.
-        __builtin_amdgcn_wave_barrier();
-        atomicAdd(&counts[wave][group], __popcll(same));
+      const int earlier = __popcll(same & ((1ull << lane) - 1));
+      batch.perm[starts[group] + own[group] + earlier] = row;
+      // Every lane of the wave has read the count before it moves on: one wave runs in order.
+      __builtin_amdgcn_wave_barrier();
+      if (earlier == 0) {
+        atomicAdd(&own[group], __popcll(same));
       }
     }
     __builtin_amdgcn_wave_barrier();
+  };
+#pragma unroll
+  for (int i = 0; i < kRouteKept; ++i) {
+    if (first + i * kWave < last) {
+      place(first + i * kWave + lane, kept[i]);
+    }
   }
-  // The group of a tile (run): the last that starts at or before it and is not empty.
-  auto find = [](const int *table, int entries, int value) {
+  for (int row = first + kRouteKept * kWave; row < last; row += kWave) {
+    place(row + lane, row + lane < last ? batch.ids[row + lane] : -1);
+  }
+  // The group of a tile (run): the last that starts at or before it (an empty one starts where the
+  // next does).
+  auto find = [&](const int *table, int value) {
     int low = 0;
-    int high = entries;
+    int high = groups;
     while (high - low > 1) {
       const int middle = (low + high) / 2;
       if (table[middle] <= value) {
@@ -170,19 +207,32 @@ __global__ __launch_bounds__(kRouteThreads) void adapter_route_kernel(AdapterRou
     }
     return low;
   };
-  for (int tile = tid; tile < total_tiles; tile += kRouteThreads) {
-    const int group = find(tile_starts, groups, tile);
-    batch.tiles[2 * tile] = group;
-    batch.tiles[2 * tile + 1] = starts[group] + (tile - tile_starts[group]) * kAdapterTileRows;
+  for (int tile = tid; tile < batch.max_tiles; tile += kRouteThreads) {
+    int *entry = batch.tiles + 4 * tile;
+    if (tile >= tile_starts[groups]) {
+      entry[0] = -1;
+      continue;
+    }
+    const int group = find(tile_starts, tile);
+    const int begin = starts[group] + (tile - tile_starts[group]) * kAdapterTileRows;
+    const int left = starts[group + 1] - begin;
+    entry[0] = group;
+    entry[1] = begin;
+    entry[2] = left < kAdapterTileRows ? left : kAdapterTileRows;
+    entry[3] = group < count ? adapter_rank_of(a.ranks, group, a.max_rank) : 0;
   }
-  for (int run = tid; run < total_runs; run += kRouteThreads) {
-    const int group = find(run_starts, count, run);
+  for (int run = tid; run < batch.max_runs; run += kRouteThreads) {
+    int *entry = batch.runs + 4 * run;
+    if (run >= run_starts[groups]) {
+      entry[0] = -1;
+      continue;
+    }
+    const int group = find(run_starts, run);
     const int begin = starts[group] + (run - run_starts[group]) * batch.run_rows;
-    const int end = begin + batch.run_rows < starts[group + 1] ? begin + batch.run_rows : starts[group + 1];
-    batch.outer[4 * run] = group;
-    batch.outer[4 * run + 1] = begin;
-    batch.outer[4 * run + 2] = end;
-    batch.outer[4 * run + 3] = slot_starts[group] < 0 ? -1 : slot_starts[group] + run - run_starts[group];
+    entry[0] = group;
+    entry[1] = begin;
+    entry[2] = begin + batch.run_rows < starts[group + 1] ? begin + batch.run_rows : starts[group + 1];
+    entry[3] = slot_starts[group] < 0 ? -1 : slot_starts[group] + run - run_starts[group];
   }
 }
 
@@ -244,12 +294,16 @@ __global__ __launch_bounds__(256) void adapter_terms_kernel(AdapterTermsArgs a) 
   __shared__ int list[kAdapterTileRows];
   __shared__ float values[kAdapterTileRows][kAdapterMaxRank + 1];
   for (int64_t slot = blockIdx.x;; slot += gridDim.x) {
-    const AdapterTile tile = adapter_tile(a.batch, slot, false, list);
+    const AdapterTile tile = adapter_tile(a.batch, a.ranks, a.max_rank, slot, false);
     if (tile.group < 0) {
       return;
     }
-    const int64_t position = a.batch.tiles[2 * slot + 1];
-    const int rank = adapter_rank(a.ranks, tile.group, a.max_rank);
+    if (threadIdx.x < kAdapterTileRows) {
+      list[threadIdx.x] = tile.row;
+    }
+    __syncthreads();
+    const int64_t position = a.batch.tiles[4 * slot + 1];
+    const int rank = tile.rank;
     int columns = 16;
     while (columns < rank) {
       columns *= 2;
@@ -298,8 +352,8 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterReduceArgs a
   const int64_t block = blockIdx.x - (second ? a.blocks0 : 0);
   const uint32_t elements = static_cast<uint32_t>(job.columns * a.max_rank);
   for (int group = blockIdx.y; group < a.batch.count; group += gridDim.y) {
-    const int slot = a.batch.runs[2 * group];
-    const int runs = a.batch.runs[2 * group + 1];
+    const int slot = a.batch.run_slots[2 * group];
+    const int runs = a.batch.run_slots[2 * group + 1];
     if (runs == 1) {
       continue;
     }
@@ -336,7 +390,7 @@ int rank_tiles(int64_t max_rank) { return max_rank <= 16 ? 1 : max_rank <= 32 ? 
 
 // Workgroups of the shrink kernel that fill the chip: two per CU.
 constexpr int64_t kShrinkWorkgroups = 512;
-constexpr int64_t kMaxRanges = 32;
+constexpr int64_t kMaxRanges = 8;
 constexpr int64_t kStepsPerWorkgroup = 16;  // the least: two steps per wave
 constexpr int64_t kExpandWorkgroups = 1024;
 constexpr int64_t kOuterWorkgroups = 1024;
@@ -347,11 +401,11 @@ constexpr int64_t kExtraSlots = 64;
 int64_t align16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 unsigned tile_slots(const AdapterBatch &batch) {
-  if (batch.head == nullptr) {
+  if (batch.tiles == nullptr) {
     return static_cast<unsigned>(batch.rows);
   }
-  const int64_t tiles = (batch.rows + kAdapterTileRows - 1) / kAdapterTileRows;
-  return static_cast<unsigned>(std::min<int64_t>(tiles + std::min<int64_t>(batch.count + 1, kExtraSlots), 65535));
+  const int64_t whole = (batch.rows + kAdapterTileRows - 1) / kAdapterTileRows;
+  return static_cast<unsigned>(std::min<int64_t>({whole + kExtraSlots, batch.max_tiles, 65535}));
 }
 
 template <class Args>
@@ -377,7 +431,7 @@ AdapterPlan plan_adapter(const AdapterShape &shape) {
   int64_t at = 0;
   if (routed) {
     plan.max_tiles = rows / kAdapterTileRows + std::min(rows, shape.count + 2);
-    int64_t ints = 4 + shape.count + 3 + rows + 2 * plan.max_tiles;
+    int64_t ints = 4 * plan.max_tiles + shape.count + 1 + rows;
     if (shape.backward) {
       const int64_t blocks = (widths[0] + 63) / 64 + (widths[1] + 63) / 64;
       const int64_t wanted = std::max<int64_t>(1, (kOuterWorkgroups + blocks - 1) / blocks);
@@ -435,13 +489,13 @@ AdapterBatch adapter_batch(const AdapterShape &shape, const AdapterPlan &plan, c
   batch.rows = shape.rows;
   batch.count = static_cast<int32_t>(shape.count);
   if (plan.max_tiles > 0) {
-    int32_t *at = reinterpret_cast<int32_t *>(workspace + plan.route);
-    batch.head = at;
-    batch.starts = at + 4;
-    batch.perm = batch.starts + shape.count + 3;
-    batch.tiles = batch.perm + shape.rows;
-    batch.outer = batch.tiles + 2 * plan.max_tiles;
-    batch.runs = batch.outer + 4 * plan.max_runs;
+    batch.tiles = reinterpret_cast<int32_t *>(workspace + plan.route);
+    batch.runs = batch.tiles + 4 * plan.max_tiles;
+    batch.run_slots = batch.runs + 4 * plan.max_runs;
+    batch.starts = batch.run_slots + (plan.run_rows > 0 ? 2 * shape.count : 0);
+    batch.perm = batch.starts + shape.count + 1;
+    batch.max_tiles = static_cast<int32_t>(plan.max_tiles);
+    batch.max_runs = static_cast<int32_t>(plan.max_runs);
     batch.run_rows = static_cast<int32_t>(plan.run_rows);
   }
   return batch;
@@ -456,20 +510,24 @@ KernelLaunch make_adapter_shrink(const AdapterShrinkArgs &args, const AdapterPla
   const void *func = dtype == kDtypeF32   ? AdapterKernels<F32Payload>::shrink(tiles)
                      : dtype == kDtypeF16 ? AdapterKernels<F16Payload>::shrink(tiles)
                                           : AdapterKernels<Bf16Payload>::shrink(tiles);
-  return launch_of(func, dim3(static_cast<unsigned>(args.job[0].ranges + args.job[1].ranges), tile_slots(args.batch), 1),
-                   kAdapterShrinkWaves * kWave, args);
+  AdapterShrinkArgs record = args;
+  record.slots = tile_slots(args.batch);
+  return launch_of(func, dim3(static_cast<unsigned>((args.job[0].ranges + args.job[1].ranges) * record.slots), 1, 1),
+                   kAdapterShrinkWaves * kWave, record);
 }
 
 KernelLaunch make_adapter_expand(const AdapterExpandArgs &args, const AdapterPlan &plan, int dtype) {
   const int tiles = static_cast<int>(plan.rp / 16);
-  const bool act = args.act.function != kActivationNone;
+  const AdapterAct act = args.act.function == kActivationNone                                       ? AdapterAct::None
+                         : args.act.gated != 0 && args.act.function == kActivationSilu ? AdapterAct::GatedSilu
+                                                                                       : AdapterAct::Any;
   const void *func = dtype == kDtypeF32   ? AdapterKernels<F32Payload>::expand(tiles, act)
                      : dtype == kDtypeF16 ? AdapterKernels<F16Payload>::expand(tiles, act)
                                           : AdapterKernels<Bf16Payload>::expand(tiles, act);
   AdapterExpandArgs record = args;
   constexpr int64_t kTurn = kAdapterExpandWaves * kAdapterExpandColumns;
   const int64_t turns = (args.n + kTurn - 1) / kTurn;
-  const int64_t row_tiles = args.batch.head == nullptr ? 1 : (args.batch.rows + kAdapterTileRows - 1) / kAdapterTileRows;
+  const int64_t row_tiles = args.batch.tiles == nullptr ? 1 : (args.batch.rows + kAdapterTileRows - 1) / kAdapterTileRows;
   const int64_t groups = std::min(turns, std::max<int64_t>(1, (kExpandWorkgroups + row_tiles - 1) / row_tiles));
   record.columns = (turns + groups - 1) / groups * kTurn;
   return launch_of(func,

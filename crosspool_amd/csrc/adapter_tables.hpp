@@ -19,7 +19,7 @@ const void *AdapterKernels<P>::shrink(int rank_tiles) {
   }
 }
 
-template <class P, bool ACT>
+template <class P, AdapterAct ACT>
 const void *adapter_expand_for(int rank_tiles) {
   switch (rank_tiles) {
     case 1:
@@ -34,8 +34,15 @@ const void *adapter_expand_for(int rank_tiles) {
 }
 
 template <class P>
-const void *AdapterKernels<P>::expand(int rank_tiles, bool activation) {
-  return activation ? adapter_expand_for<P, true>(rank_tiles) : adapter_expand_for<P, false>(rank_tiles);
+const void *AdapterKernels<P>::expand(int rank_tiles, AdapterAct activation) {
+  switch (activation) {
+    case AdapterAct::None:
+      return adapter_expand_for<P, AdapterAct::None>(rank_tiles);
+    case AdapterAct::GatedSilu:
+      return adapter_expand_for<P, AdapterAct::GatedSilu>(rank_tiles);
+    default:
+      return adapter_expand_for<P, AdapterAct::Any>(rank_tiles);
+  }
 }
 
 template <class P>

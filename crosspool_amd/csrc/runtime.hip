@@ -1782,8 +1782,10 @@ int xp_adapter_apply(const xp_adapter_pool *pool, const int32_t *ids, int64_t ro
   unsigned char *bytes = static_cast<unsigned char *>(workspace);
   const hipStream_t hip_stream = static_cast<hipStream_t>(stream);
   const AdapterBatch batch = adapter_batch(shape, plan, ids, bytes);
-  if (batch.head != nullptr) {
-    XP_HIP_CHECK(launch(make_adapter_route(AdapterRouteArgs{batch, fault_word}), hip_stream));
+  if (batch.tiles != nullptr) {
+    XP_HIP_CHECK(launch(make_adapter_route(AdapterRouteArgs{batch, pool->ranks, fault_word,
+                                                            static_cast<int32_t>(shape.max_rank)}),
+                        hip_stream));
   }
   AdapterShrinkArgs shrink{};
   shrink.batch = batch;
@@ -1870,7 +1872,7 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
   const int32_t rp = static_cast<int32_t>(plan.rp);
   float *t = reinterpret_cast<float *>(bytes + plan.partials[0]);
   float *u = reinterpret_cast<float *>(bytes + plan.partials[1]);
-  XP_HIP_CHECK(launch(make_adapter_route(AdapterRouteArgs{batch, fault_word}), hip_stream));
+  XP_HIP_CHECK(launch(make_adapter_route(AdapterRouteArgs{batch, pool->ranks, fault_word, max_rank}), hip_stream));
   if (rows > 0) {
     const AdapterTransposeArgs transpose{batch, pool->ranks, pool->a, pool->b, bytes + plan.at, bytes + plan.bt,
                                          shape.input_width, shape.output_width, max_rank, rp,

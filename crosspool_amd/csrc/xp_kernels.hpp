@@ -385,25 +385,28 @@ constexpr int kAdapterTileRows = 64;
 // Up to this many rows the tiles are found by ballots in every workgroup; above, rows are sorted.
 constexpr int64_t kAdapterDirectRows = 64;
 
-// The batch's rows by adapter.  With `head` null (up to kAdapterDirectRows rows) kernels read `ids`;
-// otherwise adapter_route_kernel filled the rest: group g (adapter g; count: no adapter; count + 1:
-// ids out of range) holds rows perm[starts[g], starts[g + 1]).
+// The batch's rows by adapter.  With `tiles` null (up to kAdapterDirectRows rows) kernels read `ids`;
+// otherwise adapter_route_kernel filled the rest: rows in the order perm, by group (adapters, then rows
+// without one, then rows with an id out of range).
 struct AdapterBatch {
   const int32_t *ids;     // [rows]
-  int32_t *head;          // tiles of adapters, tiles of all groups, runs
-  int32_t *starts;        // [count + 3]
+  int32_t *starts;        // [count + 1] first position of every adapter's rows and of the rest
   int32_t *perm;          // [rows]
-  int32_t *tiles;         // group, first position of every tile of up to 64 rows
-  int32_t *outer;         // group, first, end, slot of partial sums (-1: none) of every run of rows
-  int32_t *runs;          // [count] first slot and number of runs of every adapter
+  int32_t *tiles;         // [max_tiles] group (-1: no tile), first position, rows, rank
+  int32_t *runs;          // [max_runs] group (-1: no run), first position, end, slot of partial sums (-1: none)
+  int32_t *run_slots;     // [count] first slot and number of runs of every adapter
   int64_t rows;
+  int32_t max_tiles;
+  int32_t max_runs;
   int32_t count;
   int32_t run_rows;       // rows of a run (a multiple of 64), or 0: no runs wanted
 };
 
 struct AdapterRouteArgs {
   AdapterBatch batch;
+  const int32_t *ranks;
   uint32_t *fault;
+  int32_t max_rank;
 };
 
 // partials [range, row, rp] = the K range's part of A_a x[row].
@@ -421,6 +424,7 @@ struct AdapterShrinkArgs {
   AdapterBatch batch;
   const int32_t *ranks;      // [count] or null: max_rank
   AdapterShrinkJob job[2];   // the second with ranges 0: none
+  int64_t slots;             // workgroups per range (set by make_adapter_shrink)
   int32_t max_rank;
   int32_t rp;                // columns of a partial row: 16, 32, 64 or 128
 };
