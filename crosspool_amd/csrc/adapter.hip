@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kRouteThreads) void adapter_route_kernel(AdapterRou
     entry[3] = group < count ? adapter_rank_of(a.ranks, group, a.max_rank) : 0;
   }
   for (int run = tid; run < batch.max_runs; run += kRouteThreads) {
-    int *entry = batch.runs + 4 * run;
+    int *entry = batch.runs + 8 * run;
     if (run >= run_starts[groups]) {
       entry[0] = -1;
       continue;
@@ -233,6 +233,7 @@ __global__ __launch_bounds__(kRouteThreads) void adapter_route_kernel(AdapterRou
     entry[1] = begin;
     entry[2] = begin + batch.run_rows < starts[group + 1] ? begin + batch.run_rows : starts[group + 1];
     entry[3] = slot_starts[group] < 0 ? -1 : slot_starts[group] + run - run_starts[group];
+    entry[4] = tile_starts[group] + (run - run_starts[group]) * (batch.run_rows / kAdapterTileRows);
   }
 }
 
@@ -288,11 +289,17 @@ __global__ __launch_bounds__(256) void adapter_transpose_kernel(AdapterTranspose
 }
 
 // ------------------------------------------------------------------ terms
-// The K ranges' sums of t (u) in range order, transposed to [rank][position] and split into the terms
-// that the outer products multiply.  One workgroup per tile of 64 positions.
+// The K ranges' sums of t (u) in range order as the coefficient operands of the outer products: for each
+// tile of 64 positions, step of 32 (fp32: 16) positions and 16 ranks, lane l's 16 bytes are those of rank
+// l % 16 and the 8 (4) positions from 8 (4) (l / 16), 16-bit payloads' as two planes of bf16 terms;
+// positions past the tile are zero.  One workgroup per tile.
 __global__ __launch_bounds__(256) void adapter_terms_kernel(AdapterTermsArgs a) {
   __shared__ int list[kAdapterTileRows];
   __shared__ float values[kAdapterTileRows][kAdapterMaxRank + 1];
+  const int planes = a.f32 != 0 ? 1 : 2;
+  const int per_lane = a.f32 != 0 ? 4 : 8;
+  const int steps = kAdapterTileRows / (4 * per_lane);
+  const int rank_tiles = a.rp / 16;
   for (int64_t slot = blockIdx.x;; slot += gridDim.x) {
     const AdapterTile tile = adapter_tile(a.batch, a.ranks, a.max_rank, slot, false);
     if (tile.group < 0) {
@@ -302,43 +309,58 @@ __global__ __launch_bounds__(256) void adapter_terms_kernel(AdapterTermsArgs a) 
       list[threadIdx.x] = tile.row;
     }
     __syncthreads();
-    const int64_t position = a.batch.tiles[4 * slot + 1];
-    const int rank = tile.rank;
     int columns = 16;
-    while (columns < rank) {
+    while (columns < tile.rank) {
       columns *= 2;
     }
-    if (rank > 0) {
+    if (tile.rank > 0) {
       const int job = blockIdx.y;
       const int64_t plane = a.batch.rows * a.rp;
-      for (int index = threadIdx.x; index < tile.rows * columns; index += 256) {
-        const int row = index / columns;
-        const int r = index & (columns - 1);
-        const float *source = a.partials[job] + static_cast<int64_t>(list[row]) * a.rp + r;
-        float sum = 0.0f;
-#pragma unroll 8
-        for (int64_t range = 0; range < a.ranges[job]; ++range) {
-          sum += source[range * plane];
-        }
-        values[row][r] = sum;
-      }
-      __syncthreads();
-      const int64_t term = static_cast<int64_t>(a.rp) * a.stride;
-      for (int index = threadIdx.x; index < 64 * columns; index += 256) {
-        const int row = index & 63;
+      const int quads = columns / 4;
+      for (int index = threadIdx.x; index < kAdapterTileRows * quads; index += 256) {
+        const int row = index / quads;
+        const int r = 4 * (index & (quads - 1));
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
         if (row < tile.rows) {
-          const float value = values[row][index >> 6];
-          const int64_t at = (index >> 6) * a.stride + position + row;
-          if (a.f32 != 0) {
-            static_cast<float *>(a.terms[job])[at] = value;
-          } else {
-            uint32_t high;
-            uint32_t low;
-            split_pair(value, 0.0f, high, low);
-            static_cast<uint16_t *>(a.terms[job])[at] = static_cast<uint16_t>(high);
-            static_cast<uint16_t *>(a.terms[job])[at + term] = static_cast<uint16_t>(low);
+          const float *source = a.partials[job] + static_cast<int64_t>(list[row]) * a.rp + r;
+#pragma unroll 8
+          for (int64_t range = 0; range < a.ranges[job]; ++range) {
+            sum += *reinterpret_cast<const f32x4 *>(source + range * plane);
           }
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          values[row][r + j] = sum[j];
+        }
+      }
+      __syncthreads();
+      unsigned char *out = static_cast<unsigned char *>(a.terms[job]) + slot * steps * rank_tiles * planes * 1024;
+      for (int index = threadIdx.x; index < steps * (columns / 16) * kWave; index += 256) {
+        const int lane = index & 63;
+        const int r = index / kWave % (columns / 16);
+        const int step = index / kWave / (columns / 16);
+        const int rank = r * 16 + (lane & 15);
+        const int row = (step * 4 + (lane >> 4)) * per_lane;
+        unsigned char *target = out + ((step * rank_tiles + r) * planes * kWave + lane) * 16;
+        u32x4 high;
+        u32x4 low;
+        if (a.f32 != 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            high[j] = __float_as_uint(values[row + j][rank]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t h;
+            uint32_t l;
+            split_pair(values[row + 2 * j][rank], values[row + 2 * j + 1][rank], h, l);
+            high[j] = h;
+            low[j] = l;
+          }
+          *reinterpret_cast<u32x4 *>(target + 1024) = low;
+        }
+        *reinterpret_cast<u32x4 *>(target) = high;
       }
     }
     __syncthreads();
@@ -392,8 +414,8 @@ int rank_tiles(int64_t max_rank) { return max_rank <= 16 ? 1 : max_rank <= 32 ? 
 constexpr int64_t kShrinkWorkgroups = 512;
 constexpr int64_t kMaxRanges = 8;
 constexpr int64_t kStepsPerWorkgroup = 16;  // the least: two steps per wave
-constexpr int64_t kExpandWorkgroups = 1024;
-constexpr int64_t kOuterWorkgroups = 1024;
+constexpr int64_t kExpandWorkgroups = 512;
+constexpr int64_t kOuterWorkgroups = 512;
 constexpr int64_t kMinRunRows = 256;
 // Tiles of adapters with few rows come on top of the whole ones; workgroups past this many walk on.
 constexpr int64_t kExtraSlots = 64;
@@ -440,7 +462,7 @@ AdapterPlan plan_adapter(const AdapterShape &shape) {
       plan.max_runs = rows / plan.run_rows + std::min(rows, shape.count);
       // An adapter of several runs has more than run_rows rows.
       plan.run_slots = std::min(2 * rows / kMinRunRows, 2 * wanted);
-      ints += 4 * plan.max_runs + 2 * shape.count;
+      ints += 8 * plan.max_runs + 2 * shape.count;
     }
     at = align16(ints * 4);
   }
@@ -455,10 +477,9 @@ AdapterPlan plan_adapter(const AdapterShape &shape) {
     at += align16(plan.ranges[p] * rows * plan.rp * 4);
   }
   if (shape.backward) {
-    plan.stride = (rows + 15) / 8 * 8;  // a load of eight positions may pass the last by seven
     for (int p = 0; p < 2; ++p) {
       plan.terms[p] = static_cast<size_t>(at);
-      at += align16(plan.rp * plan.stride * 4);
+      at += plan.max_tiles * kAdapterTileRows * plan.rp * 4;
       plan.sums[p] = static_cast<size_t>(at);
       at += align16(plan.run_slots * plan.rp * widths[p] * 4);
     }
@@ -491,7 +512,7 @@ AdapterBatch adapter_batch(const AdapterShape &shape, const AdapterPlan &plan, c
   if (plan.max_tiles > 0) {
     batch.tiles = reinterpret_cast<int32_t *>(workspace + plan.route);
     batch.runs = batch.tiles + 4 * plan.max_tiles;
-    batch.run_slots = batch.runs + 4 * plan.max_runs;
+    batch.run_slots = batch.runs + 8 * plan.max_runs;
     batch.starts = batch.run_slots + (plan.run_rows > 0 ? 2 * shape.count : 0);
     batch.perm = batch.starts + shape.count + 1;
     batch.max_tiles = static_cast<int32_t>(plan.max_tiles);
@@ -518,18 +539,20 @@ KernelLaunch make_adapter_shrink(const AdapterShrinkArgs &args, const AdapterPla
 
 KernelLaunch make_adapter_expand(const AdapterExpandArgs &args, const AdapterPlan &plan, int dtype) {
   const int tiles = static_cast<int>(plan.rp / 16);
+  const bool direct = args.batch.tiles == nullptr;
   const AdapterAct act = args.act.function == kActivationNone                                       ? AdapterAct::None
                          : args.act.gated != 0 && args.act.function == kActivationSilu ? AdapterAct::GatedSilu
                                                                                        : AdapterAct::Any;
-  const void *func = dtype == kDtypeF32   ? AdapterKernels<F32Payload>::expand(tiles, act)
-                     : dtype == kDtypeF16 ? AdapterKernels<F16Payload>::expand(tiles, act)
-                                          : AdapterKernels<Bf16Payload>::expand(tiles, act);
+  const void *func = dtype == kDtypeF32   ? AdapterKernels<F32Payload>::expand(tiles, act, direct)
+                     : dtype == kDtypeF16 ? AdapterKernels<F16Payload>::expand(tiles, act, direct)
+                                          : AdapterKernels<Bf16Payload>::expand(tiles, act, direct);
   AdapterExpandArgs record = args;
-  constexpr int64_t kTurn = kAdapterExpandWaves * kAdapterExpandColumns;
-  const int64_t turns = (args.n + kTurn - 1) / kTurn;
-  const int64_t row_tiles = args.batch.tiles == nullptr ? 1 : (args.batch.rows + kAdapterTileRows - 1) / kAdapterTileRows;
+  const int64_t unit = dtype == kDtypeF32 ? 64 : 128;  // columns of a turn; in decode of each wave
+  const int64_t turn = direct ? kAdapterExpandWaves * unit : unit;
+  const int64_t turns = (args.n + turn - 1) / turn;
+  const int64_t row_tiles = direct ? 1 : (args.batch.rows + kAdapterTileRows - 1) / kAdapterTileRows;
   const int64_t groups = std::min(turns, std::max<int64_t>(1, (kExpandWorkgroups + row_tiles - 1) / row_tiles));
-  record.columns = (turns + groups - 1) / groups * kTurn;
+  record.columns = (turns + groups - 1) / groups * turn;
   return launch_of(func,
                    dim3(static_cast<unsigned>((args.n + record.columns - 1) / record.columns), tile_slots(args.batch), 1),
                    kAdapterExpandWaves * kWave, record);
@@ -552,13 +575,13 @@ KernelLaunch make_adapter_outer(const AdapterOuterArgs &args, const AdapterPlan 
   const void *func = dtype == kDtypeF32   ? AdapterKernels<F32Payload>::outer(tiles)
                      : dtype == kDtypeF16 ? AdapterKernels<F16Payload>::outer(tiles)
                                           : AdapterKernels<Bf16Payload>::outer(tiles);
-  AdapterOuterArgs record = args;
-  record.blocks0 = (args.job[0].columns + 63) / 64;
+  const int64_t columns = dtype == kDtypeF32 || tiles > 2 ? 64 : 128;  // of a workgroup (kOuterColumns)
+  const int64_t blocks = (args.job[0].columns + columns - 1) / columns + (args.job[1].columns + columns - 1) / columns;
   const int64_t runs = std::min<int64_t>(plan.max_runs, args.batch.rows / plan.run_rows + kExtraSlots);
   return launch_of(func,
-                   dim3(static_cast<unsigned>(record.blocks0 + (args.job[1].columns + 63) / 64),
+                   dim3(static_cast<unsigned>(blocks),
                         static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(runs, 1), 65535)), 1),
-                   kAdapterOuterWaves * kWave, record);
+                   kAdapterOuterWaves * kWave, args);
 }
 
 KernelLaunch make_adapter_reduce(const AdapterReduceArgs &args) {

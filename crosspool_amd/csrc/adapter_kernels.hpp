@@ -46,6 +46,15 @@ __device__ __forceinline__ int lane_here() {
   return lane;
 }
 
+// A run of rows whose outer products one workgroup sums.
+struct AdapterRun {
+  int group;
+  int first;  // positions first .. end - 1
+  int end;
+  int slot;   // of its partial sums, or -1: the adapter's only run
+  int tile;   // its first tile
+};
+
 struct AdapterTile {
   int group;  // the adapter; count: rows without one; count + 1: rows whose id is out of range; -1: no tile
   int rows;
@@ -160,34 +169,41 @@ __device__ __forceinline__ float element(const void *base, int64_t index) {
 }
 
 // ------------------------------------------------------------------ shrink
-// One tile of rows against all of its adapter's A rows over one K range.  The workgroup's four
-// waves take the range's groups of U steps in turn (a step is 64 bytes of every row: full lines
-// when U is even), rows straight from global memory as MFMA operands: a row is read by one wave
-// only, so LDS would add a copy and no reuse; A comes from L2.  Partial sums of the waves meet in
-// LDS, those of the ranges in `partials` [range][row][rp].
-template <class P, int NRT, int TT, int U>
+// One tile of rows against all of its adapter's A rows over one K range.  The workgroup's four waves
+// take the range's groups of U steps in turn; a step is 64 bytes of every row.  Loads have four
+// neighbouring lanes on a row's 64 bytes and go through 1 KB of LDS per operand, the wave's own, to the
+// lanes that the MFMA wants them in: loaded in those (rows along the lanes) every lane is an access of
+// its own, four times the address cycles (8192 x 12288 at rank 64 in bf16: 59 us, NEW so).  Partial sums
+// of the waves meet in LDS, those of the ranges in `partials` [range][row][rp].
+template <int RT>
+constexpr int kShrinkRegion = (4 + RT) * 1024;  // bytes of LDS per wave
+
+template <class P, int NRT, int TT, int U, int REGION>
 __device__ __forceinline__ void shrink_body(const AdapterShrinkArgs &a, const AdapterShrinkJob &job, int64_t range,
-                                            const AdapterTile &tile, f32x4 (*sums)[4 * kWave]) {
+                                            const AdapterTile &tile, unsigned char *lds) {
   constexpr int ES = kElementBytes<P>;
   constexpr int STEP = kStep<P>;
   const int64_t k = made_here(job.k);
   const int lane = lane_here();
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int row16 = lane & 15;
-  const int quarter = lane >> 4;
+  unsigned char *own = lds + wave * REGION;
+  // Loading, lane l has chunk l % 4 of row l / 4; multiplying, chunk l / 16 of row l % 16.  A row's chunks
+  // are exchanged by its number so that 16 lanes reading one chunk of 16 rows use all banks.
+  const int put = (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 4)) << 4);
+  const int get = (lane & 15) * 64 + (((lane >> 4) ^ (lane >> 2 & 3)) << 4);
   // Rows past the tile read another, ranks past the adapter's the first: their sums go nowhere.
   const unsigned char *x[TT];
   const unsigned char *w = static_cast<const unsigned char *>(job.w) + static_cast<int64_t>(tile.group) * job.w_rows * k * ES;
   uint32_t w_offset[NRT];
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
-    const int64_t row = __shfl(tile.row, t * 16 + row16, kWave);
-    x[t] = static_cast<const unsigned char *>(job.x) + (row * job.ldx + quarter * kChunk<P>) * ES;
+    const int64_t row = __shfl(tile.row, t * 16 + (lane >> 2), kWave);
+    x[t] = static_cast<const unsigned char *>(job.x) + row * job.ldx * ES + (lane & 3) * 16;
   }
 #pragma unroll
   for (int r = 0; r < NRT; ++r) {
-    const int at = r * 16 + row16;
-    w_offset[r] = static_cast<uint32_t>(((at < tile.rank ? at : 0) * k + quarter * kChunk<P>) * ES);
+    const int at = r * 16 + (lane >> 2);
+    w_offset[r] = static_cast<uint32_t>((at < tile.rank ? at : 0) * k * ES + (lane & 3) * 16);
   }
   f32x4 acc[NRT][TT];
 #pragma unroll
@@ -197,11 +213,32 @@ __device__ __forceinline__ void shrink_body(const AdapterShrinkArgs &a, const Ad
       acc[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
   }
+  auto multiply = [&](const u32x4 (&xs)[TT], const u32x4 (&ws)[NRT]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      *reinterpret_cast<u32x4 *>(own + t * 1024 + put) = xs[t];
+    }
+#pragma unroll
+    for (int r = 0; r < NRT; ++r) {
+      *reinterpret_cast<u32x4 *>(own + (TT + r) * 1024 + put) = ws[r];
+    }
+    u32x4 rows[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      rows[t] = *reinterpret_cast<const u32x4 *>(own + t * 1024 + get);
+    }
+#pragma unroll
+    for (int r = 0; r < NRT; ++r) {
+      const u32x4 weights = *reinterpret_cast<const u32x4 *>(own + (TT + r) * 1024 + get);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        acc[r][t] = P::mfma16(weights, rows[t], acc[r][t]);
+      }
+    }
+  };
   const int64_t steps = (k + STEP - 1) / STEP;
   const int64_t begin = range * job.steps_per_range;
   const int64_t end = begin + job.steps_per_range < steps ? begin + job.steps_per_range : steps;
-  // Groups of U whole steps.  Sixteen waves a CU keep enough loads in flight; a second buffer per wave
-  // would halve them.
   const int64_t whole_end = end < k / STEP ? end : k / STEP;
   const int64_t groups = whole_end > begin ? (whole_end - begin) / U : 0;
   for (int64_t at = wave; at < groups; at += kAdapterShrinkWaves) {
@@ -221,39 +258,31 @@ __device__ __forceinline__ void shrink_body(const AdapterShrinkArgs &a, const Ad
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int r = 0; r < NRT; ++r) {
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          acc[r][t] = P::mfma16(ws[u][r], xs[u][t], acc[r][t]);
-        }
-      }
+      multiply(xs[u], ws[u]);
     }
   }
-  // The steps past the last whole group, one per wave (at most U <= 4).  Chunks that the width
-  // cuts are zero here: their columns are added one by one below.
+  // The steps past the last whole group, one per wave (at most U <= 4).  Chunks that the width cuts are
+  // zero here: their columns are added one by one below.
   if (const int64_t step = begin + groups * U + wave; step < end) {
-    const bool whole = (step * 4 + quarter + 1) * kChunk<P> <= k;
+    const bool whole = (step * 4 + (lane & 3) + 1) * kChunk<P> <= k;
     const int64_t offset = step * (STEP * ES);
-    u32x4 tail[TT];
+    u32x4 xs[TT];
+    u32x4 ws[NRT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      tail[t] = u32x4{0u, 0u, 0u, 0u};
+      xs[t] = u32x4{0u, 0u, 0u, 0u};
       if (whole) {
-        tail[t] = load16_any(x[t] + offset);
+        xs[t] = load16_any(x[t] + offset);
       }
     }
 #pragma unroll
     for (int r = 0; r < NRT; ++r) {
-      u32x4 weights = {0u, 0u, 0u, 0u};
+      ws[r] = u32x4{0u, 0u, 0u, 0u};
       if (whole) {
-        weights = load16_any(w + offset + w_offset[r]);
-      }
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        acc[r][t] = P::mfma16(weights, tail[t], acc[r][t]);
+        ws[r] = load16_any(w + offset + w_offset[r]);
       }
     }
+    multiply(xs, ws);
   }
   // This range's columns that are added one by one.
   const int64_t width = made_here(job.k);
@@ -264,16 +293,16 @@ __device__ __forceinline__ void shrink_body(const AdapterShrinkArgs &a, const Ad
   for (int r = 0; r < NRT; ++r) {
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      sums[wave][t * kWave + out_lane] = acc[r][t];
+      *reinterpret_cast<f32x4 *>(own + (t * kWave + out_lane) * 16) = acc[r][t];
     }
     __syncthreads();
     const int at = static_cast<int>(threadIdx.x >> 6) * 16 + (out_lane & 15);
     const int64_t row = __shfl(tile.row, at, kWave);
     if (threadIdx.x < TT * kWave) {
-      f32x4 sum = sums[0][threadIdx.x];
+      f32x4 sum = *reinterpret_cast<const f32x4 *>(lds + threadIdx.x * 16);
 #pragma unroll
       for (int v = 1; v < kAdapterShrinkWaves; ++v) {
-        sum += sums[v][threadIdx.x];
+        sum += *reinterpret_cast<const f32x4 *>(lds + v * REGION + threadIdx.x * 16);
       }
       const int first = r * 16 + 4 * (out_lane >> 4);
       if (at < tile.rows) {
@@ -295,23 +324,23 @@ __device__ __forceinline__ void shrink_body(const AdapterShrinkArgs &a, const Ad
   }
 }
 
-template <class P, int RT, int TT>
+template <class P, int RT, int TT, int REGION>
 __device__ __forceinline__ void shrink_ranks(const AdapterShrinkArgs &a, const AdapterShrinkJob &job, int64_t range,
-                                             const AdapterTile &tile, f32x4 (*sums)[4 * kWave]) {
+                                             const AdapterTile &tile, unsigned char *lds) {
   if constexpr (RT > 1) {
     if (tile.rank <= 8 * RT) {
-      return shrink_ranks<P, RT / 2, TT>(a, job, range, tile, sums);
+      return shrink_ranks<P, RT / 2, TT, REGION>(a, job, range, tile, lds);
     }
   }
   // U steps of TT row and RT weight operands, 16 bytes per lane each, beside the sums: within the 128
   // registers of two workgroups a CU up to two rank tiles, the 256 of one above.
   constexpr int U = RT + TT <= 2 ? 4 : RT <= 4 ? 2 : 1;
-  shrink_body<P, RT, TT, U>(a, job, range, tile, sums);
+  shrink_body<P, RT, TT, U, REGION>(a, job, range, tile, lds);
 }
 
 template <class P, int RT>
 __global__ __launch_bounds__(kAdapterShrinkWaves *kWave, RT <= 2 ? 4 : 2) void adapter_shrink_kernel(AdapterShrinkArgs a) {
-  __shared__ f32x4 sums[kAdapterShrinkWaves][4 * kWave];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kAdapterShrinkWaves * kShrinkRegion<RT>];
   // A tile's ranges follow one another, so that whole rows are read at about one time (ranges of one
   // part of all rows first: 63 us instead of 48 for 4096 x 24576 in bf16).  The second job comes after
   // the first: side by side, the dispatcher's round over the CUs gave half of them the longer ranges only.
@@ -327,9 +356,9 @@ __global__ __launch_bounds__(kAdapterShrinkWaves *kWave, RT <= 2 ? 4 : 2) void a
     }
     if (tile.rank > 0) {
       if (tile.rows <= 16) {
-        shrink_ranks<P, RT, 1>(a, job, range, tile, sums);
+        shrink_ranks<P, RT, 1, kShrinkRegion<RT>>(a, job, range, tile, lds);
       } else {
-        shrink_ranks<P, RT, 4>(a, job, range, tile, sums);
+        shrink_ranks<P, RT, 4, kShrinkRegion<RT>>(a, job, range, tile, lds);
       }
     }
   }
@@ -338,13 +367,17 @@ __global__ __launch_bounds__(kAdapterShrinkWaves *kWave, RT <= 2 ? 4 : 2) void a
 // ------------------------------------------------------------------ expand
 // One tile of rows against a range of its adapter's B rows (output columns): t is summed over its K
 // ranges once per workgroup into LDS as MFMA operands ([leading terms | rests] of 16-bit payloads:
-// one product over 2 r columns), then each wave takes 64 columns at a time (of half the rows where a
-// tile has more than 32).  B rows are the MFMA's M operand in an order that leaves every lane 16
-// bytes of consecutive output columns of one row: base is added, and the row written, in 64-byte
-// runs straight from the accumulators.  The next columns' B rows are in flight while the last ones'
-// results are converted and stored.
+// one product over 2 r columns).  Rows are the MFMA's M operand and output columns its N, column
+// CH i + j of a unit of 16 CH being column i of MFMA tile j: a lane's sums over the CH tiles are then 16
+// bytes of consecutive columns of one row, and 16 lanes hold 256 contiguous bytes of it, so that base is
+// read and the result stored in whole lines by neighbouring lanes.  (With rows along the lanes, as the
+// products' natural layout has them, every lane of a load or store is an access of its own: four
+// times the address cycles, 60 us instead of NEW for 8192 x 4096 at rank 64 in bf16.)
+//
+// Sorted batches give each wave 16 rows of a tile and stage a unit's B rows in LDS, read from memory
+// once and in order, one unit ahead.  Small ones (decode) give each wave a unit of its own and take the B
+// rows straight as operands.
 constexpr int kAdapterExpandWaves = 4;
-constexpr int kAdapterExpandColumns = 64;  // per wave and turn
 
 // The epilogue's activation: none, a gated SiLU, or any.
 enum class AdapterAct : int { None = 0, GatedSilu = 1, Any = 2 };
@@ -352,37 +385,21 @@ enum class AdapterAct : int { None = 0, GatedSilu = 1, Any = 2 };
 template <class P, int RT>
 constexpr int kAdapterTermStride = std::is_same_v<P, F32Payload> ? 4 * (RT * 16 + 4) : 2 * (2 * RT * 16 + 8);  // bytes
 
-// `count` consecutive values to an element-aligned address.
+// Consecutive values to an element-aligned address.
 template <class P, int N>
-__device__ __forceinline__ void store_values(unsigned char *out, const float (&value)[N], int count) {
-  if constexpr (kElementBytes<P> == 4) {
-    if (count == N) {
-      __builtin_memcpy(out, value, sizeof(value));
+__device__ __forceinline__ void store_values(unsigned char *out, const float (&value)[N]) {
+  constexpr int WORDS = N * kElementBytes<P> / 4;
+  using Words = uint32_t __attribute__((ext_vector_type(WORDS), aligned(kElementBytes<P>)));
+  Words packed;
+#pragma unroll
+  for (int j = 0; j < WORDS; ++j) {
+    if constexpr (kElementBytes<P> == 4) {
+      packed[j] = __float_as_uint(value[j]);
     } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if (j < count) {
-          reinterpret_cast<float *>(out)[j] = value[j];
-        }
-      }
-    }
-  } else {
-    uint32_t packed[N / 2];
-#pragma unroll
-    for (int j = 0; j < N / 2; ++j) {
       packed[j] = P::pack2(value[2 * j], value[2 * j + 1]);
     }
-    if (count == N) {
-      __builtin_memcpy(out, packed, sizeof(packed));
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if (j < count) {
-          reinterpret_cast<uint16_t *>(out)[j] = static_cast<uint16_t>(packed[j / 2] >> (16 * (j % 2)));
-        }
-      }
-    }
   }
+  *reinterpret_cast<Words *>(out) = packed;
 }
 
 // silu(g) (u + offset).  16-bit results take the hardware's exp and reciprocal (relative error below
@@ -399,177 +416,6 @@ __device__ __forceinline__ float gated_silu_value(float gate, float up, const Ac
     return gate * __builtin_amdgcn_rcpf(1.0f + __expf(-act.alpha * gate)) * (up + act.up_offset);
   }
 }
-
-template <class P, int RT, int TT, AdapterAct ACT>
-struct AdapterExpand {
-  static constexpr int ES = kElementBytes<P>;
-  static constexpr int CH = kChunk<P>;
-  static constexpr bool F32 = std::is_same_v<P, F32Payload>;
-  static constexpr int CHUNKS = kAdapterExpandColumns / (4 * CH);  // 16-byte runs per lane and row
-  static constexpr int PER = CH / 4;                               // MFMA tiles per run
-  static constexpr int C = RT * 16 / CH;                           // B chunks of a row
-  static constexpr int STEPS = F32 ? C / 4 : C / 2;                // MFMA steps: r columns, or 2 r
-  static constexpr int FRAGS = F32 ? C / 4 : (C + 3) / 4;          // distinct B operands among them
-
-  const AdapterExpandArgs &a;
-  const unsigned char *w;
-  int64_t whole;  // columns before it are stored here
-  int rank;
-  int row16;
-  int quarter;
-  int row[TT];    // past the tile: another, which is not stored
-  bool live[TT];
-  u32x4 ws[4][FRAGS];
-  u32x4 base[TT][CHUNKS];
-
-  __device__ __forceinline__ AdapterExpand(const AdapterExpandArgs &args, int64_t whole_columns, int group, int tile_rank,
-                                           int first_row, int rows, int tile_row)
-      : a(args),
-        w(static_cast<const unsigned char *>(args.w) + static_cast<int64_t>(group) * args.n * args.ld_w * ES),
-        whole(whole_columns),
-        rank(tile_rank),
-        row16(lane_here() & 15),
-        quarter(lane_here() >> 4) {
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      const int at = first_row + t * 16 + row16;
-      live[t] = at < rows;
-      row[t] = __shfl(tile_row, at, kWave);
-    }
-  }
-
-  // The lane's part of base and of B rows for the 64 columns from c0, with no branch per load: columns
-  // past the whole ones read the last of those, chunks past the rank the row's first, neither of which
-  // is used.
-  __device__ __forceinline__ void load_base(int64_t c0) {
-    if (a.base != nullptr) {
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-#pragma unroll
-        for (int p = 0; p < CHUNKS; ++p) {
-          const int64_t n = c0 + p * 4 * CH + quarter * CH;
-          base[t][p] = load16_any(static_cast<const unsigned char *>(a.base) +
-                                  (row[t] * a.ld_base + (n < whole ? n : whole - CH)) * ES);
-        }
-      }
-    }
-  }
-  __device__ __forceinline__ void load_weights(int64_t c0) {
-    if (rank > 0) {
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const int64_t n = c0 + (m / PER) * 4 * CH + (row16 >> 2) * CH + (m % PER) * 4 + (row16 & 3);
-        const uint32_t row_offset = static_cast<uint32_t>(n < whole ? n : whole - 1) * static_cast<uint32_t>(a.ld_w * ES);
-#pragma unroll
-        for (int f = 0; f < FRAGS; ++f) {
-          const int chunk = (f * 4 + quarter) % C;
-          ws[m][f] = load16_any(w + (row_offset + (chunk * CH < rank ? chunk * 16 : 0)));
-        }
-      }
-    }
-  }
-
-  __device__ __forceinline__ void multiply(const unsigned char *terms, f32x4 (&acc)[4][TT]) {
-    if (rank != RT * 16) {
-      // Columns past the rank may hold anything.
-#pragma unroll
-      for (int f = 0; f < FRAGS; ++f) {
-        const int within = rank - (f * 4 + quarter) % C * CH;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t mask = chunk_mask<P>(j, within);
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            ws[m][f][j] &= mask;
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      if (RT > 2 && (s * 4 % C) * CH >= rank) {
-        continue;  // a pool of larger ranks: nothing there
-      }
-      u32x4 ts[TT];
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        ts[t] = *reinterpret_cast<const u32x4 *>(terms + (t * 16 + row16) * kAdapterTermStride<P, RT> + (s * 4 + quarter) * 16);
-      }
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        if constexpr (F32) {
-#pragma unroll
-          for (int t = 0; t < TT; ++t) {
-            acc[m][t] = F32Payload::mfma16(ws[m][s % FRAGS], ts[t], acc[m][t]);
-          }
-        } else {
-          u32x4 high;
-          u32x4 low;
-          chunk_terms<P>(ws[m][s % FRAGS], high, low);
-#pragma unroll
-          for (int t = 0; t < TT; ++t) {
-            acc[m][t] = Bf16Payload::mfma16(high, ts[t], acc[m][t]);
-            if constexpr (std::is_same_v<P, F16Payload>) {
-              acc[m][t] = Bf16Payload::mfma16(low, ts[t], acc[m][t]);
-            }
-          }
-        }
-      }
-    }
-  }
-
-  // Lane holds columns 4 (lane / 16) + j of every B tile for row lane % 16.
-  __device__ __forceinline__ void store(int64_t c0, float scale, bool poison, const f32x4 (&acc)[4][TT]) {
-    const bool gated = ACT == AdapterAct::GatedSilu || (ACT == AdapterAct::Any && a.act.gated != 0);
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-#pragma unroll
-      for (int p = 0; p < CHUNKS; ++p) {
-        const int64_t n = c0 + p * 4 * CH + quarter * CH;
-        if (!live[t] || n >= whole) {
-          continue;
-        }
-        float value[CH];
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          float from_base = 0.0f;
-          if (a.base != nullptr) {
-            const u32x4 &chunk = base[t][p];
-            if constexpr (F32) {
-              from_base = __uint_as_float(chunk[j]);
-            } else {
-              from_base = P::widen(j % 2 == 0 ? chunk[j / 2] & 0xffffu : chunk[j / 2] >> 16);
-            }
-          }
-          // A row without an adapter keeps base's bits (-0 among them).
-          value[j] = rank > 0 ? from_base + scale * acc[p * PER + j / 4][t][j % 4] : from_base;
-          value[j] = poison ? __builtin_nanf("") : value[j];
-        }
-        unsigned char *out = static_cast<unsigned char *>(a.out);
-        if (gated) {
-          float activated[CH / 2];
-#pragma unroll
-          for (int j = 0; j < CH / 2; ++j) {
-            if constexpr (ACT == AdapterAct::GatedSilu) {
-              activated[j] = gated_silu_value<P>(value[2 * j], value[2 * j + 1], a.act);
-            } else {
-              activated[j] = apply_gated(value[2 * j], value[2 * j + 1], a.act);
-            }
-          }
-          store_values<P>(out + (row[t] * a.ld_out + n / 2) * ES, activated, CH / 2);
-        } else {
-          if constexpr (ACT == AdapterAct::Any) {
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
-              value[j] = apply_function(value[j], a.act);
-            }
-          }
-          store_values<P>(out + (row[t] * a.ld_out + n) * ES, value, CH);
-        }
-      }
-    }
-  }
-};
 
 // t of the tile's rows: the K ranges' sums, in range order, as the operands that the products read
 // (zero past the rank).  The workgroup meets after it.
@@ -670,66 +516,355 @@ __device__ __forceinline__ void expand_columns(const AdapterExpandArgs &a, const
   }
 }
 
-template <class P, int RT, int TT, AdapterAct ACT>
-__device__ __forceinline__ void expand_tile(const AdapterExpandArgs &a, const AdapterTile &tile, unsigned char *terms,
-                                            int64_t begin, int64_t end) {
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  // Tiles of more than 16 TT rows: the waves' halves take a half each.
-  const int halves = tile.rows > 16 * TT ? 2 : 1;
-  const int half = halves > 1 ? wave & 1 : 0;
-  const bool poison = tile.group > a.batch.count;
-  const bool own = tile.group < a.batch.count;
-  const float scale = own && a.scales != nullptr ? a.scales[tile.group] : 1.0f;
-  const int64_t stride = kAdapterExpandWaves / halves * kAdapterExpandColumns;
-  // Whole chunks of columns go 64 at a time, the rest one by one; so do the last B rows of a pool whose
-  // rows are not whole chunks, since a row's last chunk passes its end, by less than a chunk.
-  constexpr int CH = kChunk<P>;
-  const int64_t within = a.n - (a.ld_w % CH != 0 ? (CH - 1 + a.ld_w - 1) / a.ld_w : 0);
-  const int64_t whole = within < CH ? 0 : within - within % CH;
-  const int64_t stop = end < whole ? end : whole;
-  AdapterExpand<P, RT, TT, ACT> work(a, whole, tile.group, tile.rank, half * 16 * TT, tile.rows, tile.row);
-  int64_t c0 = begin + wave / halves * kAdapterExpandColumns;
-  if (c0 < stop) {
-    work.load_base(c0);
-    work.load_weights(c0);
-  }
-  if (tile.rank > 0) {
-    stage_terms<P, RT>(a, tile, terms);
-    __syncthreads();
-  }
-  const unsigned char *operands = terms + half * 16 * TT * kAdapterTermStride<P, RT>;
-#pragma unroll 1
-  while (c0 < stop) {
-    f32x4 acc[4][TT];
+template <class P, int RT, AdapterAct ACT>
+struct AdapterExpand {
+  static constexpr int ES = kElementBytes<P>;
+  static constexpr int CH = kChunk<P>;
+  static constexpr bool F32 = std::is_same_v<P, F32Payload>;
+  static constexpr bool F16 = std::is_same_v<P, F16Payload>;
+  static constexpr int UNIT = 16 * CH;                     // columns
+  static constexpr int C = RT * 16 / CH;                   // chunks of a B row
+  static constexpr int STEPS = F32 ? C / 4 : C / 2;        // MFMA steps: r columns, or 2 r
+  static constexpr int FRAGS = F32 ? C / 4 : (C + 3) / 4;  // distinct B operands among them
+  static constexpr int STAGED = UNIT * C / (kAdapterExpandWaves * kWave);  // chunks per thread: RT
+  static constexpr int PLANES = F16 ? 2 : 1;               // fp16 is staged as its two bf16 terms
+  static constexpr int PLANE_BYTES = UNIT * C * 16;
+  static constexpr int TERM_BYTES = kAdapterTileRows * kAdapterTermStride<P, RT>;
+  static constexpr int LDS_BYTES = 2 * PLANES * PLANE_BYTES > TERM_BYTES ? 2 * PLANES * PLANE_BYTES : TERM_BYTES;
+
+  const AdapterExpandArgs &a;
+  const unsigned char *w;
+  int64_t whole;  // columns before it are stored here
+  int rank;
+  int lane16;
+  int quarter;
+  int row[4];     // the lane's rows; past the tile: another, which is not stored
+  bool live[4];
+  u32x4 ts[STEPS];
+  u32x4 base[4];       // of this turn
+  u32x4 next_base[4];  // of the next
+
+  // Rows first .. first + 15 of the tile.
+  __device__ __forceinline__ AdapterExpand(const AdapterExpandArgs &args, int64_t whole_columns, const AdapterTile &tile,
+                                           int first)
+      : a(args),
+        w(static_cast<const unsigned char *>(args.w) + static_cast<int64_t>(tile.group) * args.n * args.ld_w * ES),
+        whole(whole_columns),
+        rank(tile.rank),
+        lane16(lane_here() & 15),
+        quarter(lane_here() >> 4) {
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
+    for (int q = 0; q < 4; ++q) {
+      const int at = first + 4 * quarter + q;
+      row[q] = __shfl(tile.row, at, kWave);
+      live[q] = at < tile.rows;
+    }
+  }
+
+  // Columns past the whole ones read the last of those; they are not stored.
+  __device__ __forceinline__ void load_base(int64_t c0) {
+    if (a.base != nullptr) {
+      const int64_t n = c0 + CH * lane16;
+      const int64_t column = n < whole ? n : whole - CH;
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        acc[m][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int q = 0; q < 4; ++q) {
+        next_base[q] = load16_any(static_cast<const unsigned char *>(a.base) + (row[q] * a.ld_base + column) * ES);
       }
     }
-    if (tile.rank > 0) {
-      work.multiply(operands, acc);
-    }
-    // The next B rows are in flight while this turn's results leave.
-    const int64_t next = c0 + stride;
-    if (next < stop) {
-      work.load_weights(next);
-    }
-    work.store(c0, scale, poison, acc);
-    if (next < stop) {
-      work.load_base(next);
-    }
-    c0 = next;
   }
-  if (end == a.n && whole < a.n) {
-    expand_columns<P, RT, ACT>(a, tile, terms, scale, poison, whole);
+
+  __device__ __forceinline__ void load_terms(const unsigned char *terms, int first) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      ts[s] = *reinterpret_cast<const u32x4 *>(terms + (first + lane16) * kAdapterTermStride<P, RT> + (s * 4 + quarter) * 16);
+    }
+  }
+
+  // A chunk of a B row with what lies past the rank cleared (the pool may hold anything there).
+  __device__ __forceinline__ u32x4 within_rank(u32x4 value, int chunk) const {
+    if (rank != RT * 16) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        value[j] &= chunk_mask<P>(j, rank - chunk * CH);
+      }
+    }
+    return value;
+  }
+  // Its bytes: chunks past the rank read the row's first, rows past the whole columns the last of those.
+  __device__ __forceinline__ u32x4 load_chunk_of(int64_t n, int chunk) const {
+    const uint32_t row_offset = static_cast<uint32_t>(n < whole ? n : whole - 1) * static_cast<uint32_t>(a.ld_w * ES);
+    return load16_any(w + (row_offset + (chunk * CH < rank ? chunk * 16 : 0)));
+  }
+
+  __device__ __forceinline__ void add_products(f32x4 (&acc)[CH], int j, int s, u32x4 high, u32x4 low) const {
+    if constexpr (F32) {
+      acc[j] = F32Payload::mfma16(ts[s], high, acc[j]);
+    } else {
+      acc[j] = Bf16Payload::mfma16(ts[s], high, acc[j]);
+      if constexpr (F16) {
+        acc[j] = Bf16Payload::mfma16(ts[s], low, acc[j]);
+      }
+    }
+  }
+
+  // B rows of a unit in LDS: row CH i + j at place 16 j + i, whose chunks are exchanged so that the 16
+  // lanes that read one chunk of neighbouring places use all banks.
+  __device__ static __forceinline__ int staged_offset(int place, int chunk) {
+    const int exchange = C >= 16 ? place & 15 : place * C / 16 & (C - 1);
+    return (place * C + (chunk ^ exchange)) * 16;
+  }
+  __device__ __forceinline__ void fetch(int64_t c0, u32x4 (&staged)[STAGED]) const {
+#pragma unroll
+    for (int i = 0; i < STAGED; ++i) {
+      const int e = i * kAdapterExpandWaves * kWave + static_cast<int>(threadIdx.x);
+      staged[i] = load_chunk_of(c0 + e / C, e % C);
+    }
+  }
+  __device__ __forceinline__ void stage(const u32x4 (&staged)[STAGED], unsigned char *lds) const {
+#pragma unroll
+    for (int i = 0; i < STAGED; ++i) {
+      const int e = i * kAdapterExpandWaves * kWave + static_cast<int>(threadIdx.x);
+      const int n = e / C;
+      const int offset = staged_offset(n % CH * 16 + n / CH, e % C);
+      u32x4 high;
+      u32x4 low;
+      chunk_terms<P>(within_rank(staged[i], e % C), high, low);
+      *reinterpret_cast<u32x4 *>(lds + offset) = high;
+      if constexpr (F16) {
+        *reinterpret_cast<u32x4 *>(lds + PLANE_BYTES + offset) = low;
+      }
+    }
+  }
+  __device__ __forceinline__ void multiply_staged(const unsigned char *lds, f32x4 (&acc)[CH]) const {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+#pragma unroll
+      for (int f = 0; f < FRAGS; ++f) {
+        const int offset = staged_offset(16 * j + lane16, (f * 4 + quarter) % C);
+        const u32x4 high = *reinterpret_cast<const u32x4 *>(lds + offset);
+        u32x4 low = high;
+        if constexpr (F16) {
+          low = *reinterpret_cast<const u32x4 *>(lds + PLANE_BYTES + offset);
+        }
+#pragma unroll
+        for (int s = f; s < STEPS; s += FRAGS) {
+          add_products(acc, j, s, high, low);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void store(int64_t c0, float scale, bool poison, const f32x4 (&acc)[CH]) const {
+    const bool gated = ACT == AdapterAct::GatedSilu || (ACT == AdapterAct::Any && a.act.gated != 0);
+    const int64_t n = c0 + CH * lane16;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (!live[q] || n >= whole) {
+        continue;
+      }
+      float value[CH];
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        float from_base = 0.0f;
+        if (a.base != nullptr) {
+          if constexpr (F32) {
+            from_base = __uint_as_float(base[q][j]);
+          } else {
+            from_base = P::widen(j % 2 == 0 ? base[q][j / 2] & 0xffffu : base[q][j / 2] >> 16);
+          }
+        }
+        // A row without an adapter keeps base's bits (-0 among them).
+        value[j] = rank > 0 ? from_base + scale * acc[j][q] : from_base;
+        value[j] = poison ? __builtin_nanf("") : value[j];
+      }
+      unsigned char *out = static_cast<unsigned char *>(a.out);
+      if (gated) {
+        float activated[CH / 2];
+#pragma unroll
+        for (int j = 0; j < CH / 2; ++j) {
+          if constexpr (ACT == AdapterAct::GatedSilu) {
+            activated[j] = gated_silu_value<P>(value[2 * j], value[2 * j + 1], a.act);
+          } else {
+            activated[j] = apply_gated(value[2 * j], value[2 * j + 1], a.act);
+          }
+        }
+        store_values<P>(out + (row[q] * a.ld_out + n / 2) * ES, activated);
+      } else {
+        if constexpr (ACT == AdapterAct::Any) {
+#pragma unroll
+          for (int j = 0; j < CH; ++j) {
+            value[j] = apply_function(value[j], a.act);
+          }
+        }
+        store_values<P>(out + (row[q] * a.ld_out + n) * ES, value);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void take_base() {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      base[q] = next_base[q];
+    }
+  }
+};
+
+template <int CH>
+__device__ __forceinline__ void clear(f32x4 (&acc)[CH]) {
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 }
 
+// The columns of a unit go to the waves (decode): B rows straight from memory as operands, for each 16
+// of the tile's rows.
 template <class P, int RT, AdapterAct ACT>
-__global__ __launch_bounds__(kAdapterExpandWaves *kWave, RT <= 2 ? 4 : RT <= 4 ? 3 : 2) void adapter_expand_kernel(AdapterExpandArgs a) {
-  __shared__ __attribute__((aligned(16))) unsigned char terms[kAdapterTileRows * kAdapterTermStride<P, RT>];
+__device__ __forceinline__ void expand_by_columns(const AdapterExpandArgs &a, const AdapterTile &tile, unsigned char *lds,
+                                                  float scale, bool poison, int64_t whole, int64_t begin, int64_t stop,
+                                                  bool stage_here) {
+  using Work = AdapterExpand<P, RT, ACT>;
+  constexpr int CH = Work::CH;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+#pragma unroll 1
+  for (int first = 0; first < tile.rows; first += 16) {
+    Work work(a, whole, tile, first);
+#pragma unroll 1
+    for (int64_t c0 = begin + wave * Work::UNIT; c0 < stop; c0 += kAdapterExpandWaves * Work::UNIT) {
+      work.load_base(c0);
+      f32x4 acc[CH];
+      clear(acc);
+      if (tile.rank > 0) {
+        u32x4 ws[CH][Work::FRAGS];
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+#pragma unroll
+          for (int f = 0; f < Work::FRAGS; ++f) {
+            ws[j][f] = work.load_chunk_of(c0 + CH * work.lane16 + j, (f * 4 + work.quarter) % Work::C);
+          }
+        }
+        if (stage_here && first == 0 && c0 == begin + wave * Work::UNIT) {
+          // Every wave has columns: t is summed while B is on its way.
+          stage_terms<P, RT>(a, tile, lds);
+          __syncthreads();
+        }
+        work.load_terms(lds, first);
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+#pragma unroll
+          for (int f = 0; f < Work::FRAGS; ++f) {
+            u32x4 high;
+            u32x4 low;
+            chunk_terms<P>(work.within_rank(ws[j][f], (f * 4 + work.quarter) % Work::C), high, low);
+#pragma unroll
+            for (int s = f; s < Work::STEPS; s += Work::FRAGS) {
+              work.add_products(acc, j, s, high, low);
+            }
+          }
+        }
+      }
+      work.take_base();
+      work.store(c0, scale, poison, acc);
+    }
+  }
+}
+
+// The rows of a tile go to the waves, 16 each: B rows through LDS, the next unit's on their way while
+// this one's results leave.
+template <class P, int RT, AdapterAct ACT>
+__device__ __forceinline__ void expand_by_rows(const AdapterExpandArgs &a, const AdapterTile &tile, unsigned char *lds,
+                                               float scale, bool poison, int64_t whole, int64_t begin, int64_t stop) {
+  using Work = AdapterExpand<P, RT, ACT>;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int first = 16 * wave;
+  Work work(a, whole, tile, first);
+  int64_t c0 = begin;
+  u32x4 staged[Work::STAGED];
+  if (c0 < stop) {
+    work.load_base(c0);
+    if (tile.rank > 0) {
+      work.fetch(c0, staged);
+    }
+  }
+  if (tile.rank > 0) {
+    stage_terms<P, RT>(a, tile, lds);
+    __syncthreads();
+    work.load_terms(lds, first);
+    __syncthreads();  // the terms' place is B's now
+  }
+  unsigned char *now = lds;
+  unsigned char *then = lds + Work::PLANES * Work::PLANE_BYTES;
+  if (tile.rank > 0 && c0 < stop) {
+    work.stage(staged, now);
+    __syncthreads();
+  }
+#pragma unroll 1
+  while (c0 < stop) {
+    const int64_t next = c0 + Work::UNIT;
+    work.take_base();
+    if (next < stop) {
+      work.load_base(next);
+      if (tile.rank > 0) {
+        work.fetch(next, staged);
+      }
+    }
+    if (first < tile.rows) {
+      f32x4 acc[Work::CH];
+      clear(acc);
+      if (tile.rank > 0) {
+        work.multiply_staged(now, acc);
+      }
+      work.store(c0, scale, poison, acc);
+    }
+    if (tile.rank > 0 && next < stop) {
+      work.stage(staged, then);
+      __syncthreads();
+      unsigned char *other = now;
+      now = then;
+      then = other;
+    }
+    c0 = next;
+  }
+}
+
+// DIRECT: batches of up to kAdapterDirectRows rows.
+template <class P, int RT, AdapterAct ACT, bool DIRECT>
+__device__ __forceinline__ void expand_tile(const AdapterExpandArgs &a, const AdapterTile &tile, unsigned char *lds,
+                                            int64_t begin, int64_t end) {
+  constexpr int CH = kChunk<P>;
+  const bool poison = tile.group > a.batch.count;
+  const bool own = tile.group < a.batch.count;
+  const float scale = own && a.scales != nullptr ? a.scales[tile.group] : 1.0f;
+  // Whole chunks of columns go a unit at a time, the rest one by one; so do the last B rows of a pool whose
+  // rows are not whole chunks, since a row's last chunk passes its end, by less than a chunk.
+  const int64_t within = a.n - (a.ld_w % CH != 0 ? (CH - 1 + a.ld_w - 1) / a.ld_w : 0);
+  const int64_t whole = within < CH ? 0 : within - within % CH;
+  const int64_t stop = end < whole ? end : whole;
+  if constexpr (DIRECT) {
+    const bool all = stop > begin + (kAdapterExpandWaves - 1) * AdapterExpand<P, RT, ACT>::UNIT;
+    if (tile.rank > 0 && !all) {
+      // Some waves have no columns to load first.
+      stage_terms<P, RT>(a, tile, lds);
+      __syncthreads();
+    }
+    expand_by_columns<P, RT, ACT>(a, tile, lds, scale, poison, whole, begin, stop, all);
+  } else {
+    expand_by_rows<P, RT, ACT>(a, tile, lds, scale, poison, whole, begin, stop);
+    if (tile.rank > 0 && whole < a.n && end == a.n) {
+      __syncthreads();  // B's place is the terms' again for the columns left over
+      stage_terms<P, RT>(a, tile, lds);
+      __syncthreads();
+    }
+  }
+  if (end == a.n && whole < a.n) {
+    expand_columns<P, RT, ACT>(a, tile, lds, scale, poison, whole);
+  }
+}
+
+template <class P, int RT, AdapterAct ACT, bool DIRECT>
+__global__ __launch_bounds__(kAdapterExpandWaves *kWave, RT <= 2 ? 3 : 2) void adapter_expand_kernel(AdapterExpandArgs a) {
+  using Work = AdapterExpand<P, RT, ACT>;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[DIRECT ? Work::TERM_BYTES : Work::LDS_BYTES];
   const int64_t begin = static_cast<int64_t>(blockIdx.x) * a.columns;
   const int64_t end = begin + a.columns < a.n ? begin + a.columns : a.n;
   for (int64_t slot = blockIdx.y;; slot += gridDim.y) {
@@ -738,72 +873,102 @@ __global__ __launch_bounds__(kAdapterExpandWaves *kWave, RT <= 2 ? 4 : RT <= 4 ?
       return;
     }
     const bool poison = tile.group > a.batch.count;
-    if (poison && a.batch.tiles == nullptr && threadIdx.x == 0) {
+    if (DIRECT && poison && threadIdx.x == 0) {
       raise_fault(a.fault, kFaultAdapterOutOfRange);
     }
     if (tile.rank > 0 || poison || !a.in_place) {
-      if (tile.rows <= 16) {
-        expand_tile<P, RT, 1, ACT>(a, tile, terms, begin, end);
-      } else {
-        expand_tile<P, RT, 2, ACT>(a, tile, terms, begin, end);
-      }
+      expand_tile<P, RT, ACT, DIRECT>(a, tile, lds, begin, end);
     }
     __syncthreads();  // the terms are rewritten
   }
 }
 
 // ------------------------------------------------------------------ outer products
-// dA_a = s sum_i u[i] x[i]^T and dB_a = s sum_i dy[i] t[i]^T over one run of an adapter's rows and 64
-// columns of x (dy): the rows are the MFMA's K.  A lane loads four columns of eight rows (fp32: of
-// four), and pairs of rows' words give, by one byte permutation each, the operand of every fourth
-// column; which 16 columns an MFMA holds is free, so no LDS transposition is needed.  The
-// coefficients (u or t) come transposed and split into terms from adapter_terms_kernel.  Four waves
-// take the run's rows in turn and meet in LDS; a run that is its adapter's only one stores the
-// gradient, others their sums, which adapter_reduce_kernel adds in run order.
+// dA_a = s sum_i u[i] x[i]^T and dB_a = s sum_i dy[i] t[i]^T over one run of an adapter's rows and 16 CL
+// columns of x (dy): the rows are the MFMA's K.  A lane loads CL columns of eight rows (fp32: of four),
+// neighbouring lanes neighbouring columns, and pairs of rows' words give, by one byte permutation each,
+// the operand of every CL-th column; which 16 columns an MFMA holds is free, so no LDS transposition is
+// needed.  The coefficients (u or t) come from adapter_terms_kernel as the operands themselves, a
+// kilobyte per load.  Four waves take the run's tiles of 64 rows in turn and meet in LDS; a run that is
+// its adapter's only one stores the gradient, others their sums, which adapter_reduce_kernel adds in
+// run order.
 constexpr int kAdapterOuterWaves = 4;
 
-template <class P, int NRT, bool SWAP>
-__device__ __forceinline__ void outer_body(const AdapterOuterArgs &a, const AdapterOuterJob &job, int64_t c0, int first,
-                                           int end, int rank, float scale, int64_t slot, int group,
-                                           f32x4 (*sums)[4 * kWave]) {
+template <class P>
+constexpr int kOuterRows = std::is_same_v<P, F32Payload> ? 4 : 8;  // rows per lane and step
+// Columns per lane: 16 bytes, or half where the sums of four and eight rank tiles take the registers.
+template <class P, int RT>
+constexpr int kOuterColumns = std::is_same_v<P, F32Payload> || RT > 2 ? 4 : 8;
+
+template <class P, int RT, int NRT, bool SWAP>
+__device__ __forceinline__ void outer_body(const AdapterOuterArgs &a, const AdapterOuterJob &job, int64_t block,
+                                           const AdapterRun &run, int rank, float scale, unsigned char *lds) {
   constexpr bool F32 = std::is_same_v<P, F32Payload>;
   constexpr bool F16 = std::is_same_v<P, F16Payload>;
   constexpr int ES = kElementBytes<P>;
-  constexpr int ROWS = F32 ? 4 : 8;  // rows per lane and step
-  const int lane = threadIdx.x & 63;
+  constexpr int ROWS = kOuterRows<P>;
+  constexpr int BLOCKS = kAdapterTileRows / (4 * ROWS);  // steps per tile
+  constexpr int CL = kOuterColumns<P, RT>;
+  constexpr int WORDS = CL * ES / 4;
+  constexpr int PLANES = F32 ? 1 : 2;
+  using Words = uint32_t __attribute__((ext_vector_type(WORDS)));
+  const int lane = lane_here();
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int col16 = lane & 15;
+  const int lane16 = lane & 15;
   const int quarter = lane >> 4;
-  f32x4 acc[NRT][4];
+  const int64_t columns = made_here(job.columns);
+  const int64_t c0 = block * 16 * CL;
+  // The last lane of a width that CL does not divide takes its last CL columns, some of them twice.
+  const bool narrow = columns < CL;
+  auto column_of = [&](int index) __attribute__((always_inline)) {
+    const int64_t column = c0 + CL * index;
+    return narrow ? 0 : column + CL <= columns ? column : columns - CL;
+  };
+  const unsigned char *data = static_cast<const unsigned char *>(job.data) + column_of(lane16) * ES;
+  f32x4 acc[NRT][CL];
 #pragma unroll
   for (int r = 0; r < NRT; ++r) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < CL; ++j) {
       acc[r][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
   }
-  const int64_t column = c0 + 4 * col16;
-  const int64_t valid = job.columns - column;
-  const unsigned char *data = static_cast<const unsigned char *>(job.data) + column * ES;
-  const int64_t terms_plane = static_cast<int64_t>(a.rp) * a.stride;
-  for (int p0 = first + wave * 4 * ROWS; p0 < end; p0 += kAdapterOuterWaves * 4 * ROWS) {
-    const int p = p0 + quarter * ROWS;
-    // words[e]: columns 0..3 of row e (16-bit payloads: two words).
-    uint32_t words[ROWS][F32 ? 4 : 2];
+#pragma unroll 1
+  for (int tile = wave; run.first + tile * kAdapterTileRows < run.end; tile += kAdapterOuterWaves) {
+    const int position = run.first + tile * kAdapterTileRows;
+    const int rows = run.end - position < kAdapterTileRows ? run.end - position : kAdapterTileRows;
+    const int mine = a.batch.perm[position + (lane < rows ? lane : 0)];
+    const unsigned char *terms = static_cast<const unsigned char *>(job.terms) +
+                                 static_cast<int64_t>(run.tile + tile) * (BLOCKS * PLANES * 1024) * (a.rp / 16) + lane * 16;
 #pragma unroll
-    for (int e = 0; e < ROWS; ++e) {
-#pragma unroll
-      for (int j = 0; j < (F32 ? 4 : 2); ++j) {
-        words[e][j] = 0u;
+    for (int b = 0; b < BLOCKS; ++b) {
+      if (b * 4 * ROWS >= rows) {
+        continue;
       }
-      if (p + e < end && valid > 0) {
-        const unsigned char *source = data + a.batch.perm[p + e] * job.ld * ES;
-        if (valid >= 4) {
-          __builtin_memcpy(words[e], source, sizeof(words[e]));
+      u32x4 coefficient[NRT][PLANES];
+#pragma unroll
+      for (int r = 0; r < NRT; ++r) {
+#pragma unroll
+        for (int plane = 0; plane < PLANES; ++plane) {
+          coefficient[r][plane] =
+              *reinterpret_cast<const u32x4 *>(terms + ((b * (a.rp / 16) + r) * PLANES + plane) * 1024);
+        }
+      }
+      Words words[ROWS];
+#pragma unroll
+      for (int e = 0; e < ROWS; ++e) {
+        const int64_t row = __shfl(mine, b * 4 * ROWS + quarter * ROWS + e, kWave);
+        const unsigned char *source = data + row * job.ld * ES;
+        if (!narrow) {
+          __builtin_memcpy(&words[e], source, sizeof(Words));
         } else {
 #pragma unroll
-          for (int j = 0; j < 3; ++j) {
-            if (j < valid) {
+          for (int j = 0; j < WORDS; ++j) {
+            words[e][j] = 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < CL - 1; ++j) {
+            if (j < columns) {
               if constexpr (F32) {
                 words[e][j] = reinterpret_cast<const uint32_t *>(source)[j];
               } else {
@@ -813,187 +978,153 @@ __device__ __forceinline__ void outer_body(const AdapterOuterArgs &a, const Adap
           }
         }
       }
-    }
-    // Coefficients of the lane's rows for rank 16 r + lane % 16; rows past the run count zero.
-    auto coefficients = [&](int r, int term) __attribute__((always_inline)) {
-      u32x4 value = {0u, 0u, 0u, 0u};
-      if (p < end) {
-        const unsigned char *source =
-            reinterpret_cast<const unsigned char *>(job.terms) +
-            (term * terms_plane + static_cast<int64_t>(r * 16 + col16) * a.stride + p) * (F32 ? 4 : 2);
-        value = load16_any(source);
-        if (p + ROWS > end) {
+      if ((b + 1) * 4 * ROWS > rows) {
+        // Rows past the tile have coefficients of zero, which an infinity or NaN would turn into NaN.
 #pragma unroll
-          for (int e = 0; e < ROWS; ++e) {
-            if (p + e >= end) {
-              if constexpr (F32) {
-                value[e] = 0u;
-              } else {
-                value[e / 2] &= e % 2 == 0 ? 0xffff0000u : 0x0000ffffu;
-              }
+        for (int e = 0; e < ROWS; ++e) {
+          if (b * 4 * ROWS + quarter * ROWS + e >= rows) {
+#pragma unroll
+            for (int j = 0; j < WORDS; ++j) {
+              words[e][j] = 0u;
             }
           }
         }
       }
-      return value;
-    };
-    // operand[j]: column 4 (lane % 16) + j of the lane's rows.
-    u32x4 operand[4];
-    u32x4 rest[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < CL; ++j) {
+        // Column CL (lane % 16) + j of the lane's rows.
+        u32x4 operand;
+        u32x4 rest;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if constexpr (F32) {
-          operand[j][q] = words[q][j];
-        } else {
-          operand[j][q] = __builtin_amdgcn_perm(words[2 * q + 1][j / 2], words[2 * q][j / 2],
-                                                j % 2 == 0 ? 0x05040100u : 0x07060302u);
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (F32) {
+            operand[q] = words[q][j];
+          } else {
+            operand[q] = __builtin_amdgcn_perm(words[2 * q + 1][j / 2], words[2 * q][j / 2],
+                                               j % 2 == 0 ? 0x05040100u : 0x07060302u);
+          }
         }
-      }
-      if constexpr (F16) {
-        u32x4 high;
-        chunk_terms<P>(operand[j], high, rest[j]);
-        operand[j] = high;
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < NRT; ++r) {
-      const u32x4 high = coefficients(r, 0);
-      if constexpr (F32) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          acc[r][j] = SWAP ? F32Payload::mfma16(operand[j], high, acc[r][j])
-                           : F32Payload::mfma16(high, operand[j], acc[r][j]);
+        if constexpr (F16) {
+          const u32x4 both = operand;
+          chunk_terms<P>(both, operand, rest);
         }
-      } else {
-        const u32x4 low = coefficients(r, 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          auto add = [&](u32x4 coefficient, u32x4 rows) __attribute__((always_inline)) {
-            acc[r][j] = SWAP ? Bf16Payload::mfma16(rows, coefficient, acc[r][j])
-                             : Bf16Payload::mfma16(coefficient, rows, acc[r][j]);
+        for (int r = 0; r < NRT; ++r) {
+          auto add = [&](u32x4 with, u32x4 rows_of) __attribute__((always_inline)) {
+            using M = std::conditional_t<F32, F32Payload, Bf16Payload>;
+            acc[r][j] = SWAP ? M::mfma16(rows_of, with, acc[r][j]) : M::mfma16(with, rows_of, acc[r][j]);
           };
-          add(high, operand[j]);
-          add(low, operand[j]);
-          if constexpr (F16) {
-            add(high, rest[j]);
-            add(low, rest[j]);
+#pragma unroll
+          for (int plane = 0; plane < PLANES; ++plane) {
+            add(coefficient[r][plane], operand);
+            if constexpr (F16) {
+              add(coefficient[r][plane], rest);
+            }
           }
         }
       }
     }
   }
-  // SWAP: lane holds rank lane % 16 and columns 16 (lane / 16) + 4 q + j; otherwise ranks
-  // 4 (lane / 16) + q and columns 4 (lane % 16) + j.
+  // SWAP: lane holds rank lane % 16 and, of column group 4 (lane / 16) + q, column j; otherwise ranks
+  // 4 (lane / 16) + q and column group lane % 16.
   const int q = wave;
-  unsigned char *grad = static_cast<unsigned char *>(job.grad);
+  const int out_lane = lane_here();
+  const int group = SWAP ? 4 * (out_lane >> 4) + q : out_lane & 15;
+  const int64_t first = c0 + CL * group;  // as if CL divided the width
+  const int64_t column = column_of(group);
+  // The group's columns that are its own: from CL - valid on.
+  const int skip = first + CL <= columns ? 0 : first < columns ? static_cast<int>(first - column) : CL;
+  const int limit = narrow ? static_cast<int>(columns) : CL;
+  const int begin_j = narrow ? (group == 0 && block == 0 ? 0 : CL) : skip;
 #pragma unroll
   for (int r = 0; r < NRT; ++r) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      sums[wave][j * kWave + lane] = acc[r][j];
+    for (int j = 0; j < CL; ++j) {
+      *reinterpret_cast<f32x4 *>(lds + ((wave * CL + j) * kWave + out_lane) * 16) = acc[r][j];
     }
     __syncthreads();
-    float total[4];
+    float total[CL];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float *flat = reinterpret_cast<const float *>(&sums[0][j * kWave + lane]) + q;
+    for (int j = 0; j < CL; ++j) {
+      const float *flat = reinterpret_cast<const float *>(lds) + (j * kWave + out_lane) * 4 + q;
       total[j] = flat[0];
 #pragma unroll
       for (int v = 1; v < kAdapterOuterWaves; ++v) {
-        total[j] += flat[v * 16 * kWave];
+        total[j] += flat[v * CL * kWave * 4];
       }
     }
-    const int at = r * 16 + (SWAP ? col16 : 4 * quarter + q);
-    const int64_t n = c0 + (SWAP ? 16 * quarter + 4 * q : 4 * col16);
-    const int count = job.columns - n < 4 ? static_cast<int>(job.columns - n) : 4;
-    if (slot >= 0) {
-      if (SWAP) {
-        float *target = job.partials + (slot * job.columns + n) * a.rp + at;
+    const int at = r * 16 + (SWAP ? out_lane & 15 : 4 * (out_lane >> 4) + q);
+    if (run.slot >= 0) {
+      float *target = SWAP ? job.partials + (run.slot * columns + column) * a.rp + at
+                           : job.partials + (static_cast<int64_t>(run.slot) * a.rp + at) * columns + column;
+      const int64_t stride = SWAP ? a.rp : 1;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j < count) {
-            target[static_cast<int64_t>(j) * a.rp] = total[j];
-          }
-        }
-      } else {
-        float *target = job.partials + (slot * a.rp + at) * job.columns + n;
-        if (count == 4) {
-          __builtin_memcpy(target, total, sizeof(total));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 3; ++j) {
-            if (j < count) {
-              target[j] = total[j];
-            }
-          }
+      for (int j = 0; j < CL; ++j) {
+        if (j >= begin_j && j < limit) {
+          target[j * stride] = total[j];
         }
       }
     } else if (at < a.max_rank) {
+      const int64_t index = SWAP ? (run.group * columns + column) * a.max_rank + at
+                                 : (static_cast<int64_t>(run.group) * a.max_rank + at) * columns + column;
+      const int64_t stride = SWAP ? a.max_rank : 1;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        total[j] = at < rank ? scale * total[j] : 0.0f;
-      }
-      if (SWAP) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j < count) {
-            const float one[2] = {total[j], 0.0f};
-            store_values<P>(grad + ((group * job.columns + n + j) * a.max_rank + at) * ES, one, 1);
-          }
+      for (int j = 0; j < CL; ++j) {
+        if (j >= begin_j && j < limit) {
+          store_value(job.grad, index + j * stride, at < rank ? scale * total[j] : 0.0f, kDtypeOf<P>);
         }
-      } else if (count > 0) {
-        store_values<P>(grad + ((static_cast<int64_t>(group) * a.max_rank + at) * job.columns + n) * ES, total, count);
       }
     }
     __syncthreads();
   }
-  if (slot < 0) {
+  if (run.slot < 0) {
     // Ranks past the tiles above: no gradient.
     for (int at = NRT * 16 + wave; at < a.max_rank; at += kAdapterOuterWaves) {
-      const int64_t n = c0 + lane;
-      if (n < job.columns) {
-        const float zero[2] = {0.0f, 0.0f};
-        const int64_t index = SWAP ? (group * job.columns + n) * a.max_rank + at
-                                   : (static_cast<int64_t>(group) * a.max_rank + at) * job.columns + n;
-        store_values<P>(grad + index * ES, zero, 1);
+      for (int64_t n = c0 + out_lane; n < c0 + 16 * CL && n < columns; n += kWave) {
+        store_value(job.grad, SWAP ? (run.group * columns + n) * a.max_rank + at
+                                   : (static_cast<int64_t>(run.group) * a.max_rank + at) * columns + n,
+                    0.0f, kDtypeOf<P>);
       }
     }
   }
 }
 
-template <class P, int RT, bool SWAP>
-__device__ __forceinline__ void outer_ranks(const AdapterOuterArgs &a, const AdapterOuterJob &job, int64_t c0, int first,
-                                            int end, int rank, float scale, int64_t slot, int group,
-                                            f32x4 (*sums)[4 * kWave]) {
-  if constexpr (RT > 1) {
-    if (rank <= 8 * RT) {
-      return outer_ranks<P, RT / 2, SWAP>(a, job, c0, first, end, rank, scale, slot, group, sums);
+template <class P, int RT, int NRT, bool SWAP>
+__device__ __forceinline__ void outer_ranks(const AdapterOuterArgs &a, const AdapterOuterJob &job, int64_t block,
+                                            const AdapterRun &run, int rank, float scale, unsigned char *lds) {
+  if constexpr (NRT > 1) {
+    if (rank <= 8 * NRT) {
+      return outer_ranks<P, RT, NRT / 2, SWAP>(a, job, block, run, rank, scale, lds);
     }
   }
-  outer_body<P, RT, SWAP>(a, job, c0, first, end, rank, scale, slot, group, sums);
+  outer_body<P, RT, NRT, SWAP>(a, job, block, run, rank, scale, lds);
 }
 
 template <class P, int RT>
 __global__ __launch_bounds__(kAdapterOuterWaves *kWave) void adapter_outer_kernel(AdapterOuterArgs a) {
-  __shared__ f32x4 sums[kAdapterOuterWaves][4 * kWave];
-  const bool second = static_cast<int64_t>(blockIdx.x) >= a.blocks0;
-  const int64_t c0 = (blockIdx.x - (second ? a.blocks0 : 0)) * 64;
-  for (int64_t run = blockIdx.y; run < a.batch.max_runs; run += gridDim.y) {
-    const int group = __builtin_amdgcn_readfirstlane(a.batch.runs[4 * run]);
-    if (group < 0) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kAdapterOuterWaves * kOuterColumns<P, RT> * 1024];
+  constexpr int kColumns = 16 * kOuterColumns<P, RT>;
+  // The blocks of job 0, then those of job 1.
+  const int64_t blocks0 = (a.job[0].columns + kColumns - 1) / kColumns;
+  const bool second = static_cast<int64_t>(blockIdx.x) >= blocks0;
+  const int64_t block = blockIdx.x - (second ? blocks0 : 0);
+  for (int64_t index = blockIdx.y; index < a.batch.max_runs; index += gridDim.y) {
+    const u32x4 entry = *reinterpret_cast<const u32x4 *>(a.batch.runs + 8 * index);
+    AdapterRun run;
+    run.group = __builtin_amdgcn_readfirstlane(static_cast<int>(entry[0]));
+    if (run.group < 0) {
       return;
     }
-    const int first = __builtin_amdgcn_readfirstlane(a.batch.runs[4 * run + 1]);
-    const int end = __builtin_amdgcn_readfirstlane(a.batch.runs[4 * run + 2]);
-    const int slot = __builtin_amdgcn_readfirstlane(a.batch.runs[4 * run + 3]);
-    const int rank = adapter_rank(a.ranks, group, a.max_rank);
-    const float scale = a.scales != nullptr ? a.scales[group] : 1.0f;
+    run.first = __builtin_amdgcn_readfirstlane(static_cast<int>(entry[1]));
+    run.end = __builtin_amdgcn_readfirstlane(static_cast<int>(entry[2]));
+    run.slot = __builtin_amdgcn_readfirstlane(static_cast<int>(entry[3]));
+    run.tile = __builtin_amdgcn_readfirstlane(a.batch.runs[8 * index + 4]);
+    const int rank = adapter_rank(a.ranks, run.group, a.max_rank);
+    const float scale = a.scales != nullptr ? a.scales[run.group] : 1.0f;
     if (second) {
-      outer_ranks<P, RT, true>(a, a.job[1], c0, first, end, rank, scale, slot, group, sums);
+      outer_ranks<P, RT, RT, true>(a, a.job[1], block, run, rank, scale, lds);
     } else {
-      outer_ranks<P, RT, false>(a, a.job[0], c0, first, end, rank, scale, slot, group, sums);
+      outer_ranks<P, RT, RT, false>(a, a.job[0], block, run, rank, scale, lds);
     }
   }
 }
@@ -1002,7 +1133,7 @@ __global__ __launch_bounds__(kAdapterOuterWaves *kWave) void adapter_outer_kerne
 template <class P>
 struct AdapterKernels {
   static const void *shrink(int rank_tiles);
-  static const void *expand(int rank_tiles, AdapterAct activation);
+  static const void *expand(int rank_tiles, AdapterAct activation, bool direct);
   static const void *outer(int rank_tiles);
 };
 extern template struct AdapterKernels<Bf16Payload>;

@@ -1919,12 +1919,11 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
                     shape.input_width};
     outer.job[1] = {grad_out, bytes + plan.terms[1], grad_b, reinterpret_cast<float *>(bytes + plan.sums[1]),
                     ld_grad_out, shape.output_width};
-    outer.stride = plan.stride;
     outer.max_rank = max_rank;
     outer.rp = rp;
     if (rows > 0) {
       const AdapterTermsArgs terms{batch, pool->ranks, {u, t}, {bytes + plan.terms[0], bytes + plan.terms[1]},
-                                   {plan.ranges[1], plan.ranges[0]}, plan.stride, max_rank, rp,
+                                   {plan.ranges[1], plan.ranges[0]}, max_rank, rp,
                                    shape.dtype == XP_DTYPE_F32 ? 1 : 0};
       XP_HIP_CHECK(launch(make_adapter_terms(terms, plan), hip_stream));
       XP_HIP_CHECK(launch(make_adapter_outer(outer, plan, shape.dtype), hip_stream));

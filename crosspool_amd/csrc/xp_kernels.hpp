@@ -393,7 +393,7 @@ struct AdapterBatch {
   int32_t *starts;        // [count + 1] first position of every adapter's rows and of the rest
   int32_t *perm;          // [rows]
   int32_t *tiles;         // [max_tiles] group (-1: no tile), first position, rows, rank
-  int32_t *runs;          // [max_runs] group (-1: no run), first position, end, slot of partial sums (-1: none)
+  int32_t *runs;          // [max_runs][8] group (-1: no run), first position, end, slot of partial sums (-1: none), tile
   int32_t *run_slots;     // [count] first slot and number of runs of every adapter
   int64_t rows;
   int32_t max_tiles;
@@ -466,15 +466,14 @@ struct AdapterTransposeArgs {
   int32_t element;           // bytes
 };
 
-// terms [term, rp, stride]: coefficient r of position p (of the sorted rows), as the two bf16 terms
-// or one fp32 value, from the K ranges' partial sums.
+// terms [tile of 64 positions]: the coefficients of the sorted rows as operands of the outer products (two
+// bf16 terms or one fp32 value each), from the K ranges' partial sums.
 struct AdapterTermsArgs {
   AdapterBatch batch;
   const int32_t *ranks;
   const float *partials[2];
   void *terms[2];
   int64_t ranges[2];
-  int64_t stride;
   int32_t max_rank;
   int32_t rp;
   int32_t f32;
@@ -494,8 +493,6 @@ struct AdapterOuterArgs {
   const int32_t *ranks;
   const float *scales;
   AdapterOuterJob job[2];
-  int64_t blocks0;           // 64-column blocks of job 0
-  int64_t stride;
   int32_t max_rank;
   int32_t rp;
 };
