@@ -39,13 +39,22 @@ __device__ __forceinline__ RouteSums wave_inclusive_scan(RouteSums sums) {
 // barriers, one wave's scan where two groups per lane hold all of them.
 constexpr int kRouteKept = 8;
 
-__global__ __launch_bounds__(kRouteThreads) void adapter_route_kernel(AdapterRouteArgs a) {
-  __shared__ int counts[kRouteWaves * kRouteGroups];
-  __shared__ int starts[kRouteGroups + 1];
-  __shared__ int tile_starts[kRouteGroups + 1];
-  __shared__ int run_starts[kRouteGroups + 1];
-  __shared__ int slot_starts[kRouteGroups];
-  __shared__ RouteSums wave_sums[kRouteWaves];
+struct RouteLds {
+  int counts[kRouteWaves * kRouteGroups];
+  int starts[kRouteGroups + 1];
+  int tile_starts[kRouteGroups + 1];
+  int run_starts[kRouteGroups + 1];
+  int slot_starts[kRouteGroups];
+  RouteSums wave_sums[kRouteWaves];
+};
+
+__device__ __forceinline__ void route_rows(const AdapterRouteArgs &a, RouteLds &lds) {
+  int *counts = lds.counts;
+  int *starts = lds.starts;
+  int *tile_starts = lds.tile_starts;
+  int *run_starts = lds.run_starts;
+  int *slot_starts = lds.slot_starts;
+  RouteSums *wave_sums = lds.wave_sums;
   const AdapterBatch &batch = a.batch;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -237,32 +246,54 @@ __global__ __launch_bounds__(kRouteThreads) void adapter_route_kernel(AdapterRou
   }
 }
 
+__global__ __launch_bounds__(kRouteThreads) void adapter_route_kernel(AdapterRouteArgs a) {
+  __shared__ RouteLds lds;
+  route_rows(a, lds);
+}
+
 // ------------------------------------------------------------------ transposes
 // at[a][k][r] = A_a[r][k] and bt[a][r][n] = B_a[n][r] for the adapters that have rows: 64 columns of
-// A (rows of B) per workgroup through LDS.  Ranks past the adapter's are left unwritten.
+// A (rows of B) per workgroup through LDS.  Ranks past the adapter's are left unwritten.  The backward
+// pass's sort is the first workgroup of the same launch, so the others look for rows in the ids
+// themselves; both are bound by latency, and one after the other they took 13 us where they take 9
+// together (4096 rows, an adapter of rank 16 of 4096 x 24576).
 template <class E>
-__global__ __launch_bounds__(256) void adapter_transpose_kernel(AdapterTransposeArgs a) {
-  __shared__ E tile[kAdapterMaxRank][64 + 1];
-  const int64_t blocks0 = (a.k + 63) / 64;
-  const bool second = static_cast<int64_t>(blockIdx.x) >= blocks0;
-  const int64_t c0 = (blockIdx.x - (second ? blocks0 : 0)) * 64;
+struct TransposeLds {
+  E tile[kAdapterMaxRank][64 + 1];
+};
+
+template <class E>
+__device__ __forceinline__ void transpose_columns(const AdapterTransposeArgs &a, int64_t block, int group0, int groups,
+                                                  TransposeLds<E> &lds) {
+  auto &tile = lds.tile;
+  const int64_t blocks0 = a.at != nullptr ? (a.k + 63) / 64 : 0;
+  const bool second = block >= blocks0;
+  const int64_t c0 = (block - (second ? blocks0 : 0)) * 64;
   const int64_t length = second ? a.n : a.k;
   const int columns = length - c0 < 64 ? static_cast<int>(length - c0) : 64;
-  for (int group = blockIdx.y; group < a.batch.count; group += gridDim.y) {
+  for (int group = group0; group < a.batch.count; group += groups) {
     const int rank = adapter_rank(a.ranks, group, a.max_rank);
-    if (rank == 0 || a.batch.starts[group + 1] == a.batch.starts[group]) {
+    if (rank == 0) {
+      continue;
+    }
+    int found = 0;
+#pragma unroll 4
+    for (int64_t row = threadIdx.x; row < a.batch.rows; row += kRouteThreads) {
+      found |= a.batch.ids[row] == group ? 1 : 0;
+    }
+    if (__syncthreads_or(found) == 0) {
       continue;
     }
     if (second) {
       const E *source = static_cast<const E *>(a.b) + (group * a.n + c0) * a.max_rank;
       E *target = static_cast<E *>(a.bt) + static_cast<int64_t>(group) * a.rp * a.n + c0;
-      for (int index = threadIdx.x; index < columns * rank; index += 256) {
+      for (int index = threadIdx.x; index < columns * rank; index += kRouteThreads) {
         const int column = index / rank;
         const int r = index - column * rank;
         tile[r][column] = source[static_cast<int64_t>(column) * a.max_rank + r];
       }
       __syncthreads();
-      for (int index = threadIdx.x; index < 64 * rank; index += 256) {
+      for (int index = threadIdx.x; index < 64 * rank; index += kRouteThreads) {
         const int column = index & 63;
         if (column < columns) {
           target[(index >> 6) * a.n + column] = tile[index >> 6][column];
@@ -271,14 +302,14 @@ __global__ __launch_bounds__(256) void adapter_transpose_kernel(AdapterTranspose
     } else {
       const E *source = static_cast<const E *>(a.a) + static_cast<int64_t>(group) * a.max_rank * a.k + c0;
       E *target = static_cast<E *>(a.at) + (group * a.k + c0) * a.rp;
-      for (int index = threadIdx.x; index < 64 * rank; index += 256) {
+      for (int index = threadIdx.x; index < 64 * rank; index += kRouteThreads) {
         const int column = index & 63;
         if (column < columns) {
           tile[index >> 6][column] = source[(index >> 6) * a.k + column];
         }
       }
       __syncthreads();
-      for (int index = threadIdx.x; index < columns * rank; index += 256) {
+      for (int index = threadIdx.x; index < columns * rank; index += kRouteThreads) {
         const int column = index / rank;
         const int r = index - column * rank;
         target[static_cast<int64_t>(column) * a.rp + r] = tile[r][column];
@@ -286,6 +317,22 @@ __global__ __launch_bounds__(256) void adapter_transpose_kernel(AdapterTranspose
     }
     __syncthreads();
   }
+}
+
+template <class E>
+__global__ __launch_bounds__(kRouteThreads) void adapter_route_transpose_kernel(
+    AdapterRouteTransposeArgs a) {
+  __shared__ union {
+    RouteLds route;
+    TransposeLds<E> transpose;
+  } lds;
+  if (blockIdx.x == 0) {
+    if (blockIdx.y == 0) {
+      route_rows(a.route, lds.route);
+    }
+    return;
+  }
+  transpose_columns<E>(a.transpose, blockIdx.x - 1, blockIdx.y, gridDim.y, lds.transpose);
 }
 
 // ------------------------------------------------------------------ terms
@@ -413,8 +460,12 @@ int rank_tiles(int64_t max_rank) { return max_rank <= 16 ? 1 : max_rank <= 32 ? 
 // Workgroups of the shrink kernel that fill the chip: two per CU.
 constexpr int64_t kShrinkWorkgroups = 512;
 constexpr int64_t kMaxRanges = 8;
-constexpr int64_t kStepsPerWorkgroup = 16;  // the least: two steps per wave
+constexpr int64_t kStepsPerWorkgroup = 16;  // the least: four steps per wave
 constexpr int64_t kExpandWorkgroups = 512;
+// Decode has a tile per adapter at most, of a few rows each: three workgroups per CU, were each row its
+// own tile, read B faster than more of them with a fixed cost each (48 rows of 8 adapters of rank 32 x
+// 24576 columns: 16.2 us, of 512 workgroups per tile 19.9).
+constexpr int64_t kDirectWorkgroups = 768;
 constexpr int64_t kOuterWorkgroups = 512;
 constexpr int64_t kMinRunRows = 256;
 // Tiles of adapters with few rows come on top of the whole ones; workgroups past this many walk on.
@@ -459,7 +510,8 @@ AdapterPlan plan_adapter(const AdapterShape &shape) {
       const int64_t wanted = std::max<int64_t>(1, (kOuterWorkgroups + blocks - 1) / blocks);
       const int64_t run_rows = ((rows + wanted - 1) / wanted + kAdapterTileRows - 1) / kAdapterTileRows * kAdapterTileRows;
       plan.run_rows = std::max(kMinRunRows, run_rows);
-      plan.max_runs = rows / plan.run_rows + std::min(rows, shape.count);
+      // At least rows / run_rows, and growing with the rows as the workspace's size has to.
+      plan.max_runs = std::min(rows / kMinRunRows, wanted) + std::min(rows, shape.count);
       // An adapter of several runs has more than run_rows rows.
       plan.run_slots = std::min(2 * rows / kMinRunRows, 2 * wanted);
       ints += 8 * plan.max_runs + 2 * shape.count;
@@ -550,20 +602,22 @@ KernelLaunch make_adapter_expand(const AdapterExpandArgs &args, const AdapterPla
   const int64_t unit = dtype == kDtypeF32 ? 64 : 128;  // columns of a turn; in decode of each wave
   const int64_t turn = direct ? kAdapterExpandWaves * unit : unit;
   const int64_t turns = (args.n + turn - 1) / turn;
-  const int64_t row_tiles = direct ? 1 : (args.batch.rows + kAdapterTileRows - 1) / kAdapterTileRows;
-  const int64_t groups = std::min(turns, std::max<int64_t>(1, (kExpandWorkgroups + row_tiles - 1) / row_tiles));
+  const int64_t row_tiles = direct ? args.batch.rows : (args.batch.rows + kAdapterTileRows - 1) / kAdapterTileRows;
+  const int64_t wanted = direct ? kDirectWorkgroups : kExpandWorkgroups;
+  const int64_t groups = std::min(turns, std::max<int64_t>(1, (wanted + row_tiles - 1) / row_tiles));
   record.columns = (turns + groups - 1) / groups * turn;
   return launch_of(func,
                    dim3(static_cast<unsigned>((args.n + record.columns - 1) / record.columns), tile_slots(args.batch), 1),
                    kAdapterExpandWaves * kWave, record);
 }
 
-KernelLaunch make_adapter_transpose(const AdapterTransposeArgs &args) {
-  const void *func = args.element == 4 ? reinterpret_cast<const void *>(&adapter_transpose_kernel<uint32_t>)
-                                       : reinterpret_cast<const void *>(&adapter_transpose_kernel<uint16_t>);
-  return launch_of(func, dim3(static_cast<unsigned>((args.k + 63) / 64 + (args.n + 63) / 64),
-                              static_cast<unsigned>(std::min(args.batch.count, 32)), 1),
-                   256, args);
+KernelLaunch make_adapter_route_transpose(const AdapterRouteTransposeArgs &args) {
+  const AdapterTransposeArgs &a = args.transpose;
+  const void *func = a.element == 4 ? reinterpret_cast<const void *>(&adapter_route_transpose_kernel<uint32_t>)
+                                    : reinterpret_cast<const void *>(&adapter_route_transpose_kernel<uint16_t>);
+  const int64_t blocks = (a.at != nullptr ? (a.k + 63) / 64 : 0) + (a.n + 63) / 64;
+  return launch_of(func, dim3(static_cast<unsigned>(1 + blocks), static_cast<unsigned>(std::min(a.batch.count, 32)), 1),
+                   kRouteThreads, args);
 }
 
 KernelLaunch make_adapter_terms(const AdapterTermsArgs &args, const AdapterPlan &) {

@@ -173,7 +173,7 @@ __device__ __forceinline__ float element(const void *base, int64_t index) {
 // take the range's groups of U steps in turn; a step is 64 bytes of every row.  Loads have four
 // neighbouring lanes on a row's 64 bytes and go through 1 KB of LDS per operand, the wave's own, to the
 // lanes that the MFMA wants them in: loaded in those (rows along the lanes) every lane is an access of
-// its own, four times the address cycles (8192 x 12288 at rank 64 in bf16: 59 us, NEW so).  Partial sums
+// its own, four times the address cycles (8192 x 12288 at rank 64 in bf16: 59 us, 53 so).  Partial sums
 // of the waves meet in LDS, those of the ranges in `partials` [range][row][rp].
 template <int RT>
 constexpr int kShrinkRegion = (4 + RT) * 1024;  // bytes of LDS per wave
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(kAdapterShrinkWaves *kWave, RT <= 2 ? 4 : 2) void a
 // bytes of consecutive columns of one row, and 16 lanes hold 256 contiguous bytes of it, so that base is
 // read and the result stored in whole lines by neighbouring lanes.  (With rows along the lanes, as the
 // products' natural layout has them, every lane of a load or store is an access of its own: four
-// times the address cycles, 60 us instead of NEW for 8192 x 4096 at rank 64 in bf16.)
+// times the address cycles, 60 us instead of 39 for 8192 x 4096 at rank 64 in bf16.)
 //
 // Sorted batches give each wave 16 rows of a tile and stage a unit's B rows in LDS, read from memory
 // once and in order, one unit ahead.  Small ones (decode) give each wave a unit of its own and take the B
@@ -484,6 +484,7 @@ __device__ __forceinline__ void expand_columns(const AdapterExpandArgs &a, const
     const unsigned char *t = terms + at * kAdapterTermStride<P, RT>;
     auto column = [&](int64_t n) __attribute__((always_inline)) {
       float sum = 0.0f;
+#pragma unroll 4
       for (int r = 0; r < tile.rank; ++r) {
         float coefficient;
         if constexpr (std::is_same_v<P, F32Payload>) {
@@ -849,7 +850,9 @@ __device__ __forceinline__ void expand_tile(const AdapterExpandArgs &a, const Ad
     }
     expand_by_columns<P, RT, ACT>(a, tile, lds, scale, poison, whole, begin, stop, all);
   } else {
-    expand_by_rows<P, RT, ACT>(a, tile, lds, scale, poison, whole, begin, stop);
+    if (begin < stop) {
+      expand_by_rows<P, RT, ACT>(a, tile, lds, scale, poison, whole, begin, stop);
+    }
     if (tile.rank > 0 && whole < a.n && end == a.n) {
       __syncthreads();  // B's place is the terms' again for the columns left over
       stage_terms<P, RT>(a, tile, lds);

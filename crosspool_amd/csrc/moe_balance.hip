@@ -8,7 +8,9 @@
 // (every logit -inf) has p = 0.
 //
 // Bound by memory: the loss reads the logits and ids once, the gradient reads the logits and writes
-// as much.  A row is held by a 16-, 32- or 64-lane part of a wave, four consecutive experts per lane
+// as much (65536 rows of 128 fp32 logits, eight routes each: the loss 12.2 us, 2.9 TB/s, and 5.2 us for
+// the workgroups' sums, the gradient 16.5 us, 4.1 TB/s; both launches end in a few microseconds of
+// latency that does not shrink with the rows).  A row is held by a 16-, 32- or 64-lane part of a wave, four consecutive experts per lane
 // and load, so that a wave takes several narrow rows at once; sums over a row go through DPP within
 // 16 lanes.  The loss keeps sum_t p_te of the lane's own experts in registers over all of its
 // rows and adds waves, then workgroups, in a fixed order: no floating-point atomics, equal bits
@@ -52,6 +54,7 @@ __device__ __forceinline__ float group_sum(float value) {
 }
 
 constexpr float kLowest = -__builtin_inff();
+constexpr float kLargest = 3.402823466e38f;
 
 // Experts 4 (c L + lane) + j, c < CN, of one row of logits; past the last expert -inf.
 template <class T, int L, int CN>
@@ -119,7 +122,9 @@ __device__ __forceinline__ float scores(float (&value)[CN][4], bool softmax) {
     }
   }
   sum = group_sum<L>(sum);
-  return sum == 0.0f ? 0.0f : 1.0f / sum;
+  // The inverse of the smallest sums would round to infinity.
+  const float inverse = 1.0f / sum;
+  return sum == 0.0f ? 0.0f : inverse > kLargest ? kLargest : inverse;
 }
 
 __device__ __forceinline__ int64_t live_rows(const int32_t *payload_rows, int64_t rows) {
@@ -414,8 +419,10 @@ int64_t lanes_per_row(int64_t experts) { return experts <= 64 ? 16 : experts <= 
 
 // Rows that one workgroup takes alone, without a second launch to add the sums.
 constexpr int64_t kBalanceOneWorkgroupRows = 256;
-constexpr int64_t kBalanceWorkgroups = 512;
-constexpr int64_t kBalanceBackwardWorkgroups = 2048;
+// One per CU: 512 read 65536 x 128 fp32 logits and eight ids a row in 11.4 us instead of 12.2, but leave
+// twice the sums, which the finishing launch adds in 8.1 us instead of 5.2.
+constexpr int64_t kBalanceWorkgroups = 256;
+constexpr int64_t kBalanceBackwardWorkgroups = 1024;
 
 }  // namespace
 

@@ -1872,12 +1872,15 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
   const int32_t rp = static_cast<int32_t>(plan.rp);
   float *t = reinterpret_cast<float *>(bytes + plan.partials[0]);
   float *u = reinterpret_cast<float *>(bytes + plan.partials[1]);
-  XP_HIP_CHECK(launch(make_adapter_route(AdapterRouteArgs{batch, pool->ranks, fault_word, max_rank}), hip_stream));
-  if (rows > 0) {
-    const AdapterTransposeArgs transpose{batch, pool->ranks, pool->a, pool->b, bytes + plan.at, bytes + plan.bt,
+  const AdapterRouteArgs route{batch, pool->ranks, fault_word, max_rank};
+  if (rows == 0) {
+    XP_HIP_CHECK(launch(make_adapter_route(route), hip_stream));
+  } else {
+    const AdapterTransposeArgs transpose{batch, pool->ranks, pool->a, pool->b,
+                                         grad_x != nullptr ? bytes + plan.at : nullptr, bytes + plan.bt,
                                          shape.input_width, shape.output_width, max_rank, rp,
                                          static_cast<int32_t>(element)};
-    XP_HIP_CHECK(launch(make_adapter_transpose(transpose), hip_stream));
+    XP_HIP_CHECK(launch(make_adapter_route_transpose(AdapterRouteTransposeArgs{route, transpose}), hip_stream));
     AdapterShrinkArgs shrink{};
     shrink.batch = batch;
     shrink.ranks = pool->ranks;

@@ -457,13 +457,17 @@ struct AdapterTransposeArgs {
   const int32_t *ranks;
   const void *a;
   const void *b;
-  void *at;
+  void *at;                  // or null: not wanted
   void *bt;
   int64_t k;
   int64_t n;
   int32_t max_rank;
   int32_t rp;
   int32_t element;           // bytes
+};
+struct AdapterRouteTransposeArgs {
+  AdapterRouteArgs route;
+  AdapterTransposeArgs transpose;
 };
 
 // terms [tile of 64 positions]: the coefficients of the sorted rows as operands of the outer products (two
@@ -534,7 +538,7 @@ AdapterBatch adapter_batch(const AdapterShape &shape, const AdapterPlan &plan, c
 KernelLaunch make_adapter_route(const AdapterRouteArgs &args);
 KernelLaunch make_adapter_shrink(const AdapterShrinkArgs &args, const AdapterPlan &plan, int dtype);
 KernelLaunch make_adapter_expand(const AdapterExpandArgs &args, const AdapterPlan &plan, int dtype);
-KernelLaunch make_adapter_transpose(const AdapterTransposeArgs &args);
+KernelLaunch make_adapter_route_transpose(const AdapterRouteTransposeArgs &args);
 KernelLaunch make_adapter_terms(const AdapterTermsArgs &args, const AdapterPlan &plan);
 KernelLaunch make_adapter_outer(const AdapterOuterArgs &args, const AdapterPlan &plan, int dtype);
 KernelLaunch make_adapter_reduce(const AdapterReduceArgs &args);

@@ -142,6 +142,21 @@ def test_nan_stays_in_its_row_of_the_gradient(device):
     assert torch.equal(grad[keep], clean[keep])
 
 
+def test_scores_at_the_end_of_the_exponents_range(device):
+    """exp(88.72) is within half a unit of the largest fp32 number, and the inverse of its inverse past it."""
+
+    first = torch.linspace(-88.75, -88.69, 61)
+    logits = torch.full((61, 8), -200.0)
+    logits[:, 3] = first
+    ids = torch.full((61, 2), 3, dtype=torch.int32)
+    operator = BalanceLoss(row_capacity=61, routed_expert_count=8, routed_topk=2, coefficient=0.5,
+                           algorithm=RouterAlgorithm.SIGMOID)
+    grad = torch.full((61, 8), float("nan"), device=device)
+    operator.run_into(logits=logits.to(device), ids=ids.to(device))
+    operator.backward_into(logits=logits.to(device), grad_logits=grad)
+    assert bool(torch.isfinite(grad).all()) and 0.0 <= float(operator.loss) <= 0.5 * 8 * (1 + 2.0**-16)
+
+
 def test_gradient_matches_differences(device):
     """Central differences with a step of 2^-6: the third derivative (below c f_max / T) leaves h^2 / 6 of it,
     and the fp32 loss (about 1) 2^-24 / 2^-6 of rounding: 2^-13 / T in all is ample for the first."""
