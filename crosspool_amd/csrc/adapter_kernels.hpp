@@ -470,7 +470,7 @@ __device__ __forceinline__ void stage_terms(const AdapterExpandArgs &a, const Ad
 // The columns from `first` on, one (a gated pair) per thread: those past the last whole chunk.
 template <class P, int RT, AdapterAct ACT>
 __device__ __forceinline__ void expand_columns(const AdapterExpandArgs &a, const AdapterTile &tile,
-                                               const unsigned char *terms, float scale, bool poison, int64_t first) {
+                                               const unsigned char *terms, float scale, int64_t first) {
   const bool gated = ACT == AdapterAct::GatedSilu || (ACT == AdapterAct::Any && a.act.gated != 0);
   const int columns = static_cast<int>(a.n - first) / (gated ? 2 : 1);
   const int64_t weights = static_cast<int64_t>(tile.group) * a.n * a.ld_w;
@@ -496,7 +496,7 @@ __device__ __forceinline__ void expand_columns(const AdapterExpandArgs &a, const
         sum += coefficient * element<P>(a.w, weights + n * a.ld_w + r);
       }
       const float from_base = a.base != nullptr ? element<P>(a.base, row * a.ld_base + n) : 0.0f;
-      return poison ? __builtin_nanf("") : tile.rank > 0 ? from_base + scale * sum : from_base;
+      return tile.rank > 0 ? from_base + scale * sum : from_base;
     };
     const int64_t n = index - at * columns;
     if (gated) {
@@ -655,8 +655,19 @@ struct AdapterExpand {
     }
   }
 
-  __device__ __forceinline__ void store(int64_t c0, float scale, bool poison, const f32x4 (&acc)[CH]) const {
-    const bool gated = ACT == AdapterAct::GatedSilu || (ACT == AdapterAct::Any && a.act.gated != 0);
+  // Whether the limit holds is decided once per unit, not by a selection per value.
+  __device__ __forceinline__ void store(int64_t c0, float scale, const f32x4 (&acc)[CH]) const {
+    if (ACT != AdapterAct::None && a.act.has_limit) {
+      store_rows<true>(c0, scale, acc);
+    } else {
+      store_rows<false>(c0, scale, acc);
+    }
+  }
+  template <bool LIMIT>
+  __device__ __forceinline__ void store_rows(int64_t c0, float scale, const f32x4 (&acc)[CH]) const {
+    ActivationArgs act = a.act;
+    act.has_limit = LIMIT ? 1 : 0;
+    const bool gated = ACT == AdapterAct::GatedSilu || (ACT == AdapterAct::Any && act.gated != 0);
     const int64_t n = c0 + CH * lane16;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -674,9 +685,7 @@ struct AdapterExpand {
             from_base = P::widen(j % 2 == 0 ? base[q][j / 2] & 0xffffu : base[q][j / 2] >> 16);
           }
         }
-        // A row without an adapter keeps base's bits (-0 among them).
-        value[j] = rank > 0 ? from_base + scale * acc[j][q] : from_base;
-        value[j] = poison ? __builtin_nanf("") : value[j];
+        value[j] = fmaf(scale, acc[j][q], from_base);
       }
       unsigned char *out = static_cast<unsigned char *>(a.out);
       if (gated) {
@@ -684,9 +693,9 @@ struct AdapterExpand {
 #pragma unroll
         for (int j = 0; j < CH / 2; ++j) {
           if constexpr (ACT == AdapterAct::GatedSilu) {
-            activated[j] = gated_silu_value<P>(value[2 * j], value[2 * j + 1], a.act);
+            activated[j] = gated_silu_value<P>(value[2 * j], value[2 * j + 1], act);
           } else {
-            activated[j] = apply_gated(value[2 * j], value[2 * j + 1], a.act);
+            activated[j] = apply_gated(value[2 * j], value[2 * j + 1], act);
           }
         }
         store_values<P>(out + (row[q] * a.ld_out + n / 2) * ES, activated);
@@ -694,7 +703,7 @@ struct AdapterExpand {
         if constexpr (ACT == AdapterAct::Any) {
 #pragma unroll
           for (int j = 0; j < CH; ++j) {
-            value[j] = apply_function(value[j], a.act);
+            value[j] = apply_function(value[j], act);
           }
         }
         store_values<P>(out + (row[q] * a.ld_out + n) * ES, value);
@@ -722,7 +731,7 @@ __device__ __forceinline__ void clear(f32x4 (&acc)[CH]) {
 // of the tile's rows.
 template <class P, int RT, AdapterAct ACT>
 __device__ __forceinline__ void expand_by_columns(const AdapterExpandArgs &a, const AdapterTile &tile, unsigned char *lds,
-                                                  float scale, bool poison, int64_t whole, int64_t begin, int64_t stop,
+                                                  float scale, int64_t whole, int64_t begin, int64_t stop,
                                                   bool stage_here) {
   using Work = AdapterExpand<P, RT, ACT>;
   constexpr int CH = Work::CH;
@@ -765,7 +774,7 @@ __device__ __forceinline__ void expand_by_columns(const AdapterExpandArgs &a, co
         }
       }
       work.take_base();
-      work.store(c0, scale, poison, acc);
+      work.store(c0, scale, acc);
     }
   }
 }
@@ -774,7 +783,7 @@ __device__ __forceinline__ void expand_by_columns(const AdapterExpandArgs &a, co
 // this one's results leave.
 template <class P, int RT, AdapterAct ACT>
 __device__ __forceinline__ void expand_by_rows(const AdapterExpandArgs &a, const AdapterTile &tile, unsigned char *lds,
-                                               float scale, bool poison, int64_t whole, int64_t begin, int64_t stop) {
+                                               float scale, int64_t whole, int64_t begin, int64_t stop) {
   using Work = AdapterExpand<P, RT, ACT>;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int first = 16 * wave;
@@ -815,7 +824,7 @@ __device__ __forceinline__ void expand_by_rows(const AdapterExpandArgs &a, const
       if (tile.rank > 0) {
         work.multiply_staged(now, acc);
       }
-      work.store(c0, scale, poison, acc);
+      work.store(c0, scale, acc);
     }
     if (tile.rank > 0 && next < stop) {
       work.stage(staged, then);
@@ -828,14 +837,28 @@ __device__ __forceinline__ void expand_by_rows(const AdapterExpandArgs &a, const
   }
 }
 
+// Rows with an id out of range: NaN past the activation, whose limit (ReLU's zero) could hide one before it.
+template <class P, AdapterAct ACT>
+__device__ __forceinline__ void fill_with_nan(const AdapterExpandArgs &a, const AdapterTile &tile, int64_t begin,
+                                              int64_t end) {
+  const int per_value = ACT == AdapterAct::GatedSilu || (ACT == AdapterAct::Any && a.act.gated != 0) ? 2 : 1;
+  for (int at = 0; at < tile.rows; ++at) {
+    const int64_t row = __shfl(tile.row, at, kWave);
+    for (int64_t n = begin / per_value + threadIdx.x; n < end / per_value; n += kAdapterExpandWaves * kWave) {
+      store_value(a.out, row * a.ld_out + n, __builtin_nanf(""), kDtypeOf<P>);
+    }
+  }
+}
+
 // DIRECT: batches of up to kAdapterDirectRows rows.
 template <class P, int RT, AdapterAct ACT, bool DIRECT>
 __device__ __forceinline__ void expand_tile(const AdapterExpandArgs &a, const AdapterTile &tile, unsigned char *lds,
                                             int64_t begin, int64_t end) {
   constexpr int CH = kChunk<P>;
-  const bool poison = tile.group > a.batch.count;
   const bool own = tile.group < a.batch.count;
   const float scale = own && a.scales != nullptr ? a.scales[tile.group] : 1.0f;
+  // A row without an adapter has sums of +0 and keeps its base through base + -1 * 0 (-0 too).
+  const float factor = tile.rank > 0 ? scale : -1.0f;
   // Whole chunks of columns go a unit at a time, the rest one by one; so do the last B rows of a pool whose
   // rows are not whole chunks, since a row's last chunk passes its end, by less than a chunk.
   const int64_t within = a.n - (a.ld_w % CH != 0 ? (CH - 1 + a.ld_w - 1) / a.ld_w : 0);
@@ -848,10 +871,10 @@ __device__ __forceinline__ void expand_tile(const AdapterExpandArgs &a, const Ad
       stage_terms<P, RT>(a, tile, lds);
       __syncthreads();
     }
-    expand_by_columns<P, RT, ACT>(a, tile, lds, scale, poison, whole, begin, stop, all);
+    expand_by_columns<P, RT, ACT>(a, tile, lds, factor, whole, begin, stop, all);
   } else {
     if (begin < stop) {
-      expand_by_rows<P, RT, ACT>(a, tile, lds, scale, poison, whole, begin, stop);
+      expand_by_rows<P, RT, ACT>(a, tile, lds, factor, whole, begin, stop);
     }
     if (tile.rank > 0 && whole < a.n && end == a.n) {
       __syncthreads();  // B's place is the terms' again for the columns left over
@@ -860,7 +883,7 @@ __device__ __forceinline__ void expand_tile(const AdapterExpandArgs &a, const Ad
     }
   }
   if (end == a.n && whole < a.n) {
-    expand_columns<P, RT, ACT>(a, tile, lds, scale, poison, whole);
+    expand_columns<P, RT, ACT>(a, tile, lds, scale, whole);
   }
 }
 
@@ -875,11 +898,12 @@ __global__ __launch_bounds__(kAdapterExpandWaves *kWave, RT <= 2 ? 3 : 2) void a
     if (tile.group < 0) {
       return;
     }
-    const bool poison = tile.group > a.batch.count;
-    if (DIRECT && poison && threadIdx.x == 0) {
-      raise_fault(a.fault, kFaultAdapterOutOfRange);
-    }
-    if (tile.rank > 0 || poison || !a.in_place) {
+    if (tile.group > a.batch.count) {
+      if (DIRECT && threadIdx.x == 0) {
+        raise_fault(a.fault, kFaultAdapterOutOfRange);
+      }
+      fill_with_nan<P, ACT>(a, tile, begin, end);
+    } else if (tile.rank > 0 || !a.in_place) {
       expand_tile<P, RT, ACT, DIRECT>(a, tile, lds, begin, end);
     }
     __syncthreads();  // the terms are rewritten

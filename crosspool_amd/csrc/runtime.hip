@@ -1892,26 +1892,6 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
     shrink.max_rank = max_rank;
     shrink.rp = rp;
     XP_HIP_CHECK(launch(make_adapter_shrink(shrink, plan, shape.dtype), hip_stream));
-    if (grad_x != nullptr) {
-      AdapterExpandArgs expand{};
-      expand.batch = batch;
-      expand.ranks = pool->ranks;
-      expand.scales = pool->scales;
-      expand.partials = u;
-      expand.w = bytes + plan.at;
-      expand.base = base;
-      expand.out = grad_x;
-      expand.ranges = plan.ranges[1];
-      expand.n = shape.input_width;
-      expand.ld_base = ld_base;
-      expand.ld_out = ld_grad_x;
-      expand.max_rank = max_rank;
-      expand.ld_w = rp;
-      expand.rp = rp;
-      expand.in_place = base == grad_x;
-      expand.act.function = kActivationNone;
-      XP_HIP_CHECK(launch(make_adapter_expand(expand, plan, shape.dtype), hip_stream));
-    }
   }
   if (grad_a != nullptr) {
     AdapterOuterArgs outer{};
@@ -1928,12 +1908,34 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
       const AdapterTermsArgs terms{batch, pool->ranks, {u, t}, {bytes + plan.terms[0], bytes + plan.terms[1]},
                                    {plan.ranges[1], plan.ranges[0]}, max_rank, rp,
                                    shape.dtype == XP_DTYPE_F32 ? 1 : 0};
+      // Before the input's gradient: grad_out and x are still in the last level of cache (4096 rows of
+      // 4096 x 24576: the outer products take 37 us instead of 43).
       XP_HIP_CHECK(launch(make_adapter_terms(terms, plan), hip_stream));
       XP_HIP_CHECK(launch(make_adapter_outer(outer, plan, shape.dtype), hip_stream));
     }
     const AdapterReduceArgs reduce{batch, pool->ranks, pool->scales, {outer.job[0], outer.job[1]}, 0, max_rank, rp,
                                    shape.dtype};
     XP_HIP_CHECK(launch(make_adapter_reduce(reduce), hip_stream));
+  }
+  if (grad_x != nullptr && rows > 0) {
+    AdapterExpandArgs expand{};
+    expand.batch = batch;
+    expand.ranks = pool->ranks;
+    expand.scales = pool->scales;
+    expand.partials = u;
+    expand.w = bytes + plan.at;
+    expand.base = base;
+    expand.out = grad_x;
+    expand.ranges = plan.ranges[1];
+    expand.n = shape.input_width;
+    expand.ld_base = ld_base;
+    expand.ld_out = ld_grad_x;
+    expand.max_rank = max_rank;
+    expand.ld_w = rp;
+    expand.rp = rp;
+    expand.in_place = base == grad_x;
+    expand.act.function = kActivationNone;
+    XP_HIP_CHECK(launch(make_adapter_expand(expand, plan, shape.dtype), hip_stream));
   }
   return XP_OK;
 }

@@ -227,6 +227,29 @@ def test_ids_out_of_range_poison_their_rows_and_raise_the_fault(device, rows):
     assert torch.equal(got[keep], expected[keep])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows", [6, 100])
+@pytest.mark.parametrize("activation", [
+    Activation(SiluActivation(1.7), GateTransform(1.5, 1.0)),
+    Activation(GeluActivation(), GateTransform(2.0)),
+    Activation(ReluActivation(), None),
+], ids=["silu_clipped", "gelu_clipped", "relu_ungated"])
+def test_no_limit_hides_the_nan_of_an_id_out_of_range(device, activation, rows, dtype):
+    ids = [i % 4 - 1 for i in range(rows)]
+    case = Case(device, rows=rows, k=64, n=542, count=3, max_rank=8, dtype=dtype, ids=ids)
+    outs = []
+    for bad in (False, True):
+        if bad:
+            case.ids[1], case.ids[4] = 3, -2
+        out = torch.zeros((rows, 271 if activation.gate is not None else 542), dtype=case.dtype, device=device)
+        case.operator().run_into(case.x.to(device), case.weights(), adapter_ids=case.ids.to(device),
+                                 base=case.base.to(device), output=out, activation=activation)
+        outs.append(out.cpu())
+    assert bool(outs[1][[1, 4]].isnan().all())
+    keep = [r for r in range(rows) if r not in (1, 4)]
+    assert torch.equal(outs[1][keep], outs[0][keep])
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("rows", [3, 130])
 @pytest.mark.parametrize("activation", [
