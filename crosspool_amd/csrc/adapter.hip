@@ -253,16 +253,13 @@ __global__ __launch_bounds__(kRouteThreads) void adapter_route_kernel(AdapterRou
 
 // ------------------------------------------------------------------ transposes
 // at[a][k][r] = A_a[r][k] and bt[a][r][n] = B_a[n][r] for the adapters that have rows: 64 columns of
-// A (rows of B) per workgroup through LDS.  Ranks past the adapter's are left unwritten.  The backward
-// pass's sort is the first workgroup of the same launch, so the others look for rows in the ids
-// themselves; both are bound by latency, and one after the other they took 13 us where they take 9
-// together (4096 rows, an adapter of rank 16 of 4096 x 24576).
+// A (rows of B) per workgroup through LDS.  Ranks past the adapter's are left unwritten.
 template <class E>
 struct TransposeLds {
   E tile[kAdapterMaxRank][64 + 1];
 };
 
-template <class E>
+template <class E, bool SORTED>
 __device__ __forceinline__ void transpose_columns(const AdapterTransposeArgs &a, int64_t block, int group0, int groups,
                                                   TransposeLds<E> &lds) {
   auto &tile = lds.tile;
@@ -276,13 +273,19 @@ __device__ __forceinline__ void transpose_columns(const AdapterTransposeArgs &a,
     if (rank == 0) {
       continue;
     }
-    int found = 0;
+    if constexpr (SORTED) {
+      if (a.batch.starts[group + 1] == a.batch.starts[group]) {
+        continue;
+      }
+    } else {
+      int found = 0;
 #pragma unroll 4
-    for (int64_t row = threadIdx.x; row < a.batch.rows; row += kRouteThreads) {
-      found |= a.batch.ids[row] == group ? 1 : 0;
-    }
-    if (__syncthreads_or(found) == 0) {
-      continue;
+      for (int64_t row = threadIdx.x; row < a.batch.rows; row += kRouteThreads) {
+        found |= a.batch.ids[row] == group ? 1 : 0;
+      }
+      if (__syncthreads_or(found) == 0) {
+        continue;
+      }
     }
     if (second) {
       const E *source = static_cast<const E *>(a.b) + (group * a.n + c0) * a.max_rank;
@@ -319,6 +322,19 @@ __device__ __forceinline__ void transpose_columns(const AdapterTransposeArgs &a,
   }
 }
 
+// Few rows and adapters: the sort is the first workgroup of the transposes' launch, and the others look
+// for their adapter's rows in the ids themselves.  Both are bound by latency: one after the other they
+// took 13 us where they take 9 together (4096 rows, an adapter of rank 16 of 4096 x 24576).  With more,
+// reading the ids once per workgroup and adapter would cost more than a launch.
+constexpr int kTransposeGroups = 32;
+constexpr int64_t kRoutesBesideRows = 8192;
+
+template <class E>
+__global__ __launch_bounds__(kRouteThreads) void adapter_transpose_kernel(AdapterRouteTransposeArgs a) {
+  __shared__ TransposeLds<E> lds;
+  transpose_columns<E, true>(a.transpose, blockIdx.x, blockIdx.y, gridDim.y, lds);
+}
+
 template <class E>
 __global__ __launch_bounds__(kRouteThreads) void adapter_route_transpose_kernel(
     AdapterRouteTransposeArgs a) {
@@ -332,7 +348,7 @@ __global__ __launch_bounds__(kRouteThreads) void adapter_route_transpose_kernel(
     }
     return;
   }
-  transpose_columns<E>(a.transpose, blockIdx.x - 1, blockIdx.y, gridDim.y, lds.transpose);
+  transpose_columns<E, false>(a.transpose, blockIdx.x - 1, blockIdx.y, gridDim.y, lds.transpose);
 }
 
 // ------------------------------------------------------------------ terms
@@ -491,6 +507,11 @@ KernelLaunch launch_of(const void *func, dim3 grid, unsigned block, const Args &
   return kernel;
 }
 
+dim3 transpose_grid(const AdapterTransposeArgs &a) {
+  const int64_t blocks = (a.at != nullptr ? (a.k + 63) / 64 : 0) + (a.n + 63) / 64;
+  return dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min(a.batch.count, kTransposeGroups)), 1);
+}
+
 }  // namespace
 
 AdapterPlan plan_adapter(const AdapterShape &shape) {
@@ -611,13 +632,23 @@ KernelLaunch make_adapter_expand(const AdapterExpandArgs &args, const AdapterPla
                    kAdapterExpandWaves * kWave, record);
 }
 
+bool adapter_routes_beside_transpose(const AdapterBatch &batch) {
+  return batch.count <= kTransposeGroups && batch.rows <= kRoutesBesideRows;
+}
+
 KernelLaunch make_adapter_route_transpose(const AdapterRouteTransposeArgs &args) {
-  const AdapterTransposeArgs &a = args.transpose;
-  const void *func = a.element == 4 ? reinterpret_cast<const void *>(&adapter_route_transpose_kernel<uint32_t>)
-                                    : reinterpret_cast<const void *>(&adapter_route_transpose_kernel<uint16_t>);
-  const int64_t blocks = (a.at != nullptr ? (a.k + 63) / 64 : 0) + (a.n + 63) / 64;
-  return launch_of(func, dim3(static_cast<unsigned>(1 + blocks), static_cast<unsigned>(std::min(a.batch.count, 32)), 1),
-                   kRouteThreads, args);
+  const void *func = args.transpose.element == 4
+                         ? reinterpret_cast<const void *>(&adapter_route_transpose_kernel<uint32_t>)
+                         : reinterpret_cast<const void *>(&adapter_route_transpose_kernel<uint16_t>);
+  dim3 grid = transpose_grid(args.transpose);
+  grid.x += 1;
+  return launch_of(func, grid, kRouteThreads, args);
+}
+
+KernelLaunch make_adapter_transpose(const AdapterRouteTransposeArgs &args) {
+  const void *func = args.transpose.element == 4 ? reinterpret_cast<const void *>(&adapter_transpose_kernel<uint32_t>)
+                                                 : reinterpret_cast<const void *>(&adapter_transpose_kernel<uint16_t>);
+  return launch_of(func, transpose_grid(args.transpose), kRouteThreads, args);
 }
 
 KernelLaunch make_adapter_terms(const AdapterTermsArgs &args, const AdapterPlan &) {

@@ -813,10 +813,10 @@ __device__ __forceinline__ void expand_by_rows(const AdapterExpandArgs &a, const
     const int64_t next = c0 + Work::UNIT;
     work.take_base();
     if (next < stop) {
-      work.load_base(next);
       if (tile.rank > 0) {
         work.fetch(next, staged);
       }
+      work.load_base(next);
     }
     if (first < tile.rows) {
       f32x4 acc[Work::CH];

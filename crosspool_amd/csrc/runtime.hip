@@ -1701,6 +1701,23 @@ bool rows_overlap(const void *p, int64_t ld_p, int64_t width_p, const void *q, i
   return a < b_end && b < a_end;
 }
 
+// A call's operand as a range of bytes.
+struct Span {
+  uintptr_t begin;
+  uintptr_t end;
+};
+Span span_of(const void *p, size_t bytes) {
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(p);
+  return {begin, p == nullptr ? begin : begin + bytes};
+}
+Span span_of_rows(const void *p, int64_t ld, int64_t width, int64_t rows, size_t element) {
+  return span_of(p, static_cast<size_t>((rows - 1) * ld + width) * element);
+}
+bool touches(const Span &span, std::initializer_list<Span> others) {
+  return std::any_of(others.begin(), others.end(),
+                     [&](const Span &other) { return span.begin < other.end && other.begin < span.end; });
+}
+
 constexpr int64_t kAdapterMaxRows = int64_t{1} << 24;
 constexpr int64_t kAdapterMaxWidth = int64_t{1} << 22;
 
@@ -1723,6 +1740,10 @@ int adapter_shape(const xp_adapter_pool *pool, const int32_t *ids, int64_t rows,
   XP_REQUIRE(aligned_to(pool->ranks, 4) && aligned_to(pool->scales, 4), "adapter ranks and scales must be 4-byte aligned");
   XP_REQUIRE(rows == 0 || (ids != nullptr && aligned_to(ids, 4)), "adapter ids must be non-null and 4-byte aligned");
   return XP_OK;
+}
+
+Span pool_span(const xp_adapter_pool &pool, const void *weights, int64_t width) {
+  return span_of(weights, static_cast<size_t>(pool.count * pool.max_rank * width) * dtype_bytes(pool.dtype));
 }
 
 int adapter_rows(const char *name, const void *rows_pointer, int64_t ld, int64_t width, size_t element) {
@@ -1779,6 +1800,13 @@ int xp_adapter_apply(const xp_adapter_pool *pool, const int32_t *ids, int64_t ro
   const AdapterPlan plan = plan_adapter(shape);
   XP_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= plan.bytes,
              "adapter workspace is missing, unaligned or smaller than xp_adapter_workspace_bytes");
+  const Span scratch = span_of(workspace, plan.bytes);
+  XP_REQUIRE(!touches(span_of_rows(out, ld_out, out_width, rows, element),
+                      {scratch, span_of(ids, static_cast<size_t>(rows) * 4), pool_span(*pool, pool->a, pool->input_width),
+                       pool_span(*pool, pool->b, pool->output_width)}) &&
+                 !touches(scratch, {span_of_rows(x, ldx, shape.input_width, rows, element),
+                                    span_of_rows(base, ld_base, shape.output_width, rows, element)}),
+             "the adapter output and workspace must not overlap the pool, the ids, the operands or each other");
   unsigned char *bytes = static_cast<unsigned char *>(workspace);
   const hipStream_t hip_stream = static_cast<hipStream_t>(stream);
   const AdapterBatch batch = adapter_batch(shape, plan, ids, bytes);
@@ -1866,6 +1894,27 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
   const AdapterPlan plan = plan_adapter(planned);
   XP_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= plan.bytes,
              "adapter workspace is missing, unaligned or smaller than xp_adapter_workspace_bytes");
+  {
+    const Span none = span_of(nullptr, 0);
+    const auto rows_span = [&](const void *p, int64_t ld, int64_t width) {
+      return rows > 0 ? span_of_rows(p, ld, width, rows, element) : none;
+    };
+    const Span scratch = span_of(workspace, plan.bytes);
+    const Span read_x = rows_span(x, ldx, shape.input_width);
+    const Span read_grad = rows_span(grad_out, ld_grad_out, shape.output_width);
+    const Span read_base = grad_x != nullptr ? rows_span(base, ld_base, shape.input_width) : none;
+    const Span read_ids = span_of(ids, static_cast<size_t>(rows) * 4);
+    const Span pool_a = pool_span(*pool, pool->a, pool->input_width);
+    const Span pool_b = pool_span(*pool, pool->b, pool->output_width);
+    const Span write_x = rows_span(grad_x, ld_grad_x, shape.input_width);
+    const Span write_a = pool_span(*pool, grad_a, pool->input_width);
+    const Span write_b = pool_span(*pool, grad_b, pool->output_width);
+    XP_REQUIRE(!touches(write_a, {read_x, read_grad, read_base, read_ids, pool_a, pool_b, write_x, write_b, scratch}) &&
+                   !touches(write_b, {read_x, read_grad, read_base, read_ids, pool_a, pool_b, write_x, scratch}) &&
+                   !touches(write_x, {read_ids, pool_a, pool_b, scratch}) &&
+                   !touches(scratch, {read_x, read_grad, read_base}),
+               "adapter gradients and the workspace must not overlap the pool, the ids, the operands or each other");
+  }
   unsigned char *bytes = static_cast<unsigned char *>(workspace);
   const AdapterBatch batch = adapter_batch(shape, plan, ids, bytes);
   const int32_t max_rank = static_cast<int32_t>(shape.max_rank);
@@ -1880,7 +1929,13 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
                                          grad_x != nullptr ? bytes + plan.at : nullptr, bytes + plan.bt,
                                          shape.input_width, shape.output_width, max_rank, rp,
                                          static_cast<int32_t>(element)};
-    XP_HIP_CHECK(launch(make_adapter_route_transpose(AdapterRouteTransposeArgs{route, transpose}), hip_stream));
+    const AdapterRouteTransposeArgs both{route, transpose};
+    if (adapter_routes_beside_transpose(batch)) {
+      XP_HIP_CHECK(launch(make_adapter_route_transpose(both), hip_stream));
+    } else {
+      XP_HIP_CHECK(launch(make_adapter_route(route), hip_stream));
+      XP_HIP_CHECK(launch(make_adapter_transpose(both), hip_stream));
+    }
     AdapterShrinkArgs shrink{};
     shrink.batch = batch;
     shrink.ranks = pool->ranks;
@@ -2766,6 +2821,12 @@ int xp_moe_balance_backward(const void *logits, int logits_dtype, const int32_t 
   XP_REQUIRE(logits != nullptr && counts != nullptr && grad_logits != nullptr, "balance pointers must be non-null");
   XP_REQUIRE(aligned_to(counts, 4) && aligned_to(grad_loss, 4) && aligned_to(grad_logits, dtype_bytes(logits_dtype)),
              "balance operands must be aligned to their element size");
+  const size_t bytes = static_cast<size_t>(rows * experts) * dtype_bytes(logits_dtype);
+  XP_REQUIRE(grad_logits == logits || !touches(span_of(grad_logits, bytes), {span_of(logits, bytes)}),
+             "the logits' gradient may be the logits only whole");
+  XP_REQUIRE(!touches(span_of(grad_logits, bytes), {span_of(counts, static_cast<size_t>(experts) * 4), span_of(grad_loss, 4),
+                                                    span_of(payload_rows, 4)}),
+             "the logits' gradient must not overlap the counts, the loss's gradient or the live rows");
   args.counts = const_cast<int32_t *>(counts);
   args.grad_loss = grad_loss;
   args.grad_logits = grad_logits;

@@ -538,7 +538,10 @@ AdapterBatch adapter_batch(const AdapterShape &shape, const AdapterPlan &plan, c
 KernelLaunch make_adapter_route(const AdapterRouteArgs &args);
 KernelLaunch make_adapter_shrink(const AdapterShrinkArgs &args, const AdapterPlan &plan, int dtype);
 KernelLaunch make_adapter_expand(const AdapterExpandArgs &args, const AdapterPlan &plan, int dtype);
+// Whether the transposes go with the sort in one launch or follow it in their own (of the same record).
+bool adapter_routes_beside_transpose(const AdapterBatch &batch);
 KernelLaunch make_adapter_route_transpose(const AdapterRouteTransposeArgs &args);
+KernelLaunch make_adapter_transpose(const AdapterRouteTransposeArgs &args);
 KernelLaunch make_adapter_terms(const AdapterTermsArgs &args, const AdapterPlan &plan);
 KernelLaunch make_adapter_outer(const AdapterOuterArgs &args, const AdapterPlan &plan, int dtype);
 KernelLaunch make_adapter_reduce(const AdapterReduceArgs &args);

@@ -400,6 +400,8 @@ class BalanceLoss:
         ``[rows, experts]`` (bf16, fp16 or fp32), ``loss``; over the first ``payload_rows`` rows (an int32
         value on the device, default all).  Ids outside ``[0, experts)`` are not counted."""
 
+        if ids.ndim != 2:
+            raise ValueError("ids must be a matrix")
         rows = ids.shape[0]
         live = self._live(rows, payload_rows)
         self._check(ids, "ids", torch.int32, (rows, self.routed_topk))

@@ -351,6 +351,11 @@ class DenseExecutionPlan:
         capacity = signature.payload_row_capacity
         activated = TensorLayout((capacity, signature.local_intermediate_size), dtype)
         adapted = adapters is not None and adapters.i_proj_rank is not None
+        apart = signature.activation.fused(order=signature.i_proj.gate_up_order) is None
+        gate = signature.activation.gate
+        if adapted and apart and adapters.o_proj_rank is None and gate is not None and gate.limit is not None:
+            # The limit would make a NaN row of an id out of range finite, and no later pool restores it.
+            raise ValueError("a clipped gate over CONCATENATED columns takes i_proj adapters only beside o_proj adapters")
         activation = None if adapted else signature.activation
         fused = activation is not None and activation.fused(order=signature.i_proj.gate_up_order) is not None
         i_proj = GemmPlan.prepare(
@@ -428,6 +433,8 @@ class Dense:
         if adapters is not None:
             if (adapters.i_proj is None) != (self.i_adapter is None) or (adapters.o_proj is None) != (self.o_adapter is None):
                 raise ValueError("Dense adapters disagree with the prepared plan")
+        elif self.i_adapter is not None and self.plan.signature.payload_dtype is torch.float32:
+            raise ValueError("an fp32 Dense layer prepared for i_proj adapters takes them in every call (id -1: none)")
         rows = hidden_states.shape[0]
         projected = self.projected[:rows]
         self.i_proj.run_into(hidden_states, layer_weights.i_proj, output=projected)

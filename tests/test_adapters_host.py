@@ -82,6 +82,29 @@ def test_backward_refusals():
     assert backward(gx=None, ga=None, gb=None, base=None) == _native.XP_OK  # nothing asked for
 
 
+def test_nothing_written_may_overlap_what_is_read():
+    far = dict(a=0x1000000, b=0x2000000)
+    for changes in (dict(out=0x1000010), dict(out=0x2000010), dict(out=0x40000), dict(out=P), dict(ws=0x10000),
+                    dict(ws=0x20000)):
+        assert apply(pool(**far), **changes) == BAD and "overlap" in _native.last_error(), changes
+    for changes in (
+        dict(ga=0x10000), dict(ga=0x20000), dict(ga=0x30000), dict(ga=0x50000), dict(ga=0x70000), dict(ga=0x1000010),
+        dict(ga=0x2000010), dict(ga=0x80000), dict(ga=P), dict(gb=0x10010), dict(gb=0x20000), dict(gb=0x1000000),
+        dict(gb=0x2000000), dict(gb=0x80000), dict(gx=0x1000000), dict(gx=0x2000000), dict(gx=0x60000), dict(gx=0x80000),
+        dict(gx=P), dict(ws=0x10000), dict(ws=0x20000), dict(ws=0x30000),
+    ):
+        assert backward(pool(**far), **changes) == BAD and "overlap" in _native.last_error(), changes
+
+
+def test_the_sorts_tables_grow_with_the_rows():
+    """Runs of an adapter's rows lengthen where rows pass 256 per run: the capacity's scratch holds both sides."""
+
+    for k, n in ((64, 64), (200, 60), (1000, 40)):
+        wanted = max(1, 512 // ((k + 63) // 64 + (n + 63) // 64))
+        sizes = [workspace(256 * wanted * step + extra, 1, 4, 16, k, n) for step in (1, 2, 3) for extra in (0, 1)]
+        assert sizes == sorted(sizes)
+
+
 @pytest.mark.parametrize("backward", [0, 1])
 @pytest.mark.parametrize("k,n,rank,count", [(64, 48, 16, 4), (4096, 24576, 32, 32), (12288, 4096, 128, 1), (33, 5000, 3, 1024)])
 def test_a_workspace_serves_every_smaller_batch(k, n, rank, count, backward):
@@ -150,6 +173,10 @@ def test_balance_refusals():
     for changes in (dict(logits=None), dict(counts=None), dict(out=None), dict(out=P + 1), dict(grad_loss=P + 2),
                     dict(algorithm=0), dict(dtype=9)):
         assert lib.xp_moe_balance_backward(*{**back, **changes}.values(), None) == BAD, changes
+    for changes in (dict(out=P + 2), dict(counts=0x20000, out=0x20010), dict(live=0x20004, out=0x20000),
+                    dict(grad_loss=0x20004, out=0x20000)):
+        assert lib.xp_moe_balance_backward(*{**back, **changes}.values(), None) == BAD, changes
+        assert "logits' gradient" in _native.last_error()
     assert lib.xp_moe_balance_backward(*{**back, "rows": 0}.values(), None) == _native.XP_OK
     sizes = [lib.xp_moe_balance_workspace_bytes(rows, 128) for rows in (0, 1, 256, 257, 1000, 5000, 100000)]
     assert sizes == sorted(sizes)

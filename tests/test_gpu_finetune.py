@@ -176,6 +176,38 @@ def test_dense_adapter_refusals(device):
     assert not bool(out[[0, 1, 3]].isnan().any())
 
 
+def test_dense_plans_that_cannot_keep_their_word(device):
+    """A limit applied apart from the adapters would hide an id out of range; fp32 has no activation apart."""
+
+    layer = Layer(device, rows=4, hidden=64, width=48, count=2, rank=4, dtype=torch.bfloat16)
+    weights = DenseFfnWeights.from_tensors(layer.w_in.to(device), layer.w_out.to(device))
+
+    def signature(dtype, order, gate):
+        return DenseSignature(
+            payload_dtype=dtype, payload_row_capacity=4, hidden_size=64, local_intermediate_size=48,
+            activation=Activation(SiluActivation(), gate), i_proj=ProjectionLayout.of(weights.i_proj, order=order),
+            o_proj=ProjectionLayout.of(weights.o_proj))
+
+    halves = signature(torch.bfloat16, GateUpOrder.CONCATENATED, GateTransform(7.0, 1.0))
+    with pytest.raises(ValueError, match="clipped"):
+        DenseExecutionPlan.prepare(halves, adapters=DenseAdapterLayout(2, 4))
+    DenseExecutionPlan.prepare(halves, adapters=DenseAdapterLayout(2, 4, 4))
+    DenseExecutionPlan.prepare(halves, adapters=DenseAdapterLayout(2, None, 4))
+
+    weights = DenseFfnWeights.from_tensors(layer.w_in.float().to(device), layer.w_out.float().to(device))
+    plan = DenseExecutionPlan.prepare(signature(torch.float32, GateUpOrder.INTERLEAVED, GateTransform()),
+                                      adapters=DenseAdapterLayout(2, 4))
+    dense = Dense(plan, torch.empty(plan.workspace.nbytes, dtype=torch.uint8, device=device))
+    x = layer.x.float().to(device)
+    with pytest.raises(ValueError, match="every call"):
+        dense.run_into(hidden_states=x, layer_weights=weights, output=torch.empty_like(x))
+    pool = AdapterWeights(layer.a_in.float().to(device), layer.b_in.float().to(device))
+    out = torch.full_like(x, float("nan"))
+    dense.run_into(hidden_states=x, layer_weights=weights, output=out, adapters=DenseAdapterWeights(pool),
+                   adapter_ids=torch.full((4,), -1, dtype=torch.int32, device=device))
+    assert bool(torch.isfinite(out).all())
+
+
 def _gemm(device, rows, w):
     plan = GemmPlan.prepare(input_layout=TensorLayout((rows, w.shape[1]), w.dtype),
                             weight_layout=ProjectionLayout.of(w_weights := ProjectionWeights(w)),
