@@ -187,6 +187,17 @@ def test_large_pools_and_many_groups(device):
     check_forward(case, run(case))
 
 
+@pytest.mark.parametrize("count", [5, 70])
+@pytest.mark.parametrize("rows", [8192, 8193, 20011])
+def test_more_rows_than_the_sort_keeps(device, rows, count):
+    case = Case(device, rows=rows, k=24, n=40, count=count, max_rank=4, seed=rows)
+    check_forward(case, run(case))
+    got = backward(case)
+    check_backward(case, got)
+    again = backward(case)
+    assert all(torch.equal(got[name], again[name]) for name in got)
+
+
 def test_padding_of_the_pool_is_ignored(device):
     for rows in (20, 150):
         case = Case(device, rows=rows, k=200, n=96, count=3, max_rank=20, ranks=[20, 7, 8], seed=rows)
