@@ -235,6 +235,14 @@ def call(name: str, *args: object) -> int:
     return status
 
 
+def current_device() -> int:
+    """``torch.cuda.current_device()`` where a GPU tensor is there already, without its check for one."""
+
+    import torch
+
+    return torch._C._cuda_getDevice()
+
+
 def current_stream(device_index: int | None = None) -> ctypes.c_void_p:
     """Handle of torch's current stream on a device (default: the current device).
 

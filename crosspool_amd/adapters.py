@@ -160,7 +160,7 @@ class Adapter:
     def _rows(self, tensor: torch.Tensor, name: str, rows: int, width: int) -> int:
         """The row stride of an operand (checked)."""
 
-        if tensor.dtype is not self.plan.dtype or tensor.shape != (rows, width) or tensor.device != self._device:
+        if tensor.dtype is not self.plan.dtype or tensor.shape != (rows, width) or tensor.get_device() != self._index:
             raise ValueError(f"adapter {name} must be a {self.plan.dtype} tensor of shape {(rows, width)} on {self._device}")
         stride, column = tensor.stride()
         if (column != 1 and width > 1) or (stride < width and rows > 1):
@@ -173,19 +173,19 @@ class Adapter:
             raise ValueError(f"{rows} adapter rows exceed the prepared capacity {plan.row_capacity}")
         if (
             weights.a.shape != self._pool_shape or weights.b.shape[1] != plan.output_width
-            or weights.a.dtype is not plan.dtype or weights.a.device != self._device
+            or weights.a.dtype is not plan.dtype or weights.a.get_device() != self._index
         ):
             raise ValueError("adapter weights disagree with the prepared plan")
         if (
-            adapter_ids.dtype is not torch.int32 or adapter_ids.shape != (rows,) or adapter_ids.device != self._device
+            adapter_ids.dtype is not torch.int32 or adapter_ids.shape != (rows,) or adapter_ids.get_device() != self._index
             or not adapter_ids.is_contiguous()
         ):
             raise ValueError(f"adapter ids must be a contiguous int32 tensor with one id for each of {rows} rows")
         if fault_word is not None and (
-            fault_word.dtype is not torch.int32 or fault_word.numel() < 1 or fault_word.device != self._device
+            fault_word.dtype is not torch.int32 or fault_word.numel() < 1 or fault_word.get_device() != self._index
         ):
             raise ValueError("an adapter fault word must be an int32 tensor on the workspace's device")
-        if torch.cuda.current_device() != self._index:
+        if _native.current_device() != self._index:
             raise ValueError(f"adapters of {self._device} need it as the current device")
 
     def run_into(

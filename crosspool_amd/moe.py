@@ -360,18 +360,21 @@ class BalanceLoss:
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        self._index = self.device.index
         self.row_capacity = row_capacity
         self.routed_expert_count = routed_expert_count
         self.routed_topk = routed_topk
         self.algorithm = RouterAlgorithm(algorithm)
+        self._algorithm_code = int(self.algorithm)
         self.coefficient = float(coefficient)
         nbytes = int(_native.library().xp_moe_balance_workspace_bytes(row_capacity, routed_expert_count))
         self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=self.device)
+        self._scratch, self._scratch_bytes = self.workspace.data_ptr(), self.workspace.numel()
         self.counts = torch.zeros(routed_expert_count, dtype=torch.int32, device=self.device)
         self.loss = torch.zeros(1, dtype=torch.float32, device=self.device)
 
     def _check(self, tensor: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, ...]) -> None:
-        if tensor.dtype is not dtype or tensor.shape != shape or tensor.device != self.device or not tensor.is_contiguous():
+        if tensor.dtype is not dtype or tensor.shape != shape or tensor.get_device() != self._index or not tensor.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {self.device}")
 
     def _logits_code(self, logits: torch.Tensor, rows: int) -> int:
@@ -385,11 +388,11 @@ class BalanceLoss:
     def _live(self, rows: int, payload_rows: torch.Tensor | None) -> int | None:
         if rows > self.row_capacity:
             raise ValueError(f"{rows} balance rows exceed the prepared capacity {self.row_capacity}")
-        if torch.cuda.current_device() != self.device.index:
+        if _native.current_device() != self._index:
             raise ValueError(f"the balance operator of {self.device} needs it as the current device")
         if payload_rows is None:
             return None
-        if payload_rows.dtype is not torch.int32 or payload_rows.numel() != 1 or payload_rows.device != self.device:
+        if payload_rows.dtype is not torch.int32 or payload_rows.numel() != 1 or payload_rows.get_device() != self._index:
             raise ValueError(f"payload rows must be one int32 value on {self.device}")
         return payload_rows.data_ptr()
 
@@ -408,9 +411,9 @@ class BalanceLoss:
         code = _native.XP_DTYPE_F32 if logits is None else self._logits_code(logits, rows)
         _native.call(
             "xp_moe_balance_loss", None if logits is None else logits.data_ptr(), code, ids.data_ptr(), rows,
-            self.routed_expert_count, self.routed_topk, int(self.algorithm), live, self.coefficient,
-            self.counts.data_ptr(), None if logits is None else self.loss.data_ptr(), self.workspace.data_ptr(),
-            self.workspace.numel(), _native.current_stream(self.device.index),
+            self.routed_expert_count, self.routed_topk, self._algorithm_code, live, self.coefficient,
+            self.counts.data_ptr(), None if logits is None else self.loss.data_ptr(), self._scratch,
+            self._scratch_bytes, _native.current_stream(self._index),
         )
 
     def backward_into(
@@ -435,14 +438,14 @@ class BalanceLoss:
         counts = self.counts if counts is None else counts
         self._check(counts, "counts", torch.int32, (self.routed_expert_count,))
         if grad_loss is not None and (
-            grad_loss.dtype is not torch.float32 or grad_loss.numel() != 1 or grad_loss.device != self.device
+            grad_loss.dtype is not torch.float32 or grad_loss.numel() != 1 or grad_loss.get_device() != self._index
         ):
             raise ValueError(f"the loss gradient must be one fp32 value on {self.device}")
         _native.call(
             "xp_moe_balance_backward", logits.data_ptr(), code, counts.data_ptr(), rows, self.routed_expert_count,
-            self.routed_topk, int(self.algorithm), live, self.coefficient,
+            self.routed_topk, self._algorithm_code, live, self.coefficient,
             None if grad_loss is None else grad_loss.data_ptr(), grad_logits.data_ptr(),
-            _native.current_stream(self.device.index),
+            _native.current_stream(self._index),
         )
 
 

@@ -167,11 +167,11 @@ class Activation:
         dtype = inputs.dtype
         if dtype not in (torch.bfloat16, torch.float16) or grad_output.dtype is not dtype or grad_inputs.dtype is not dtype:
             raise ValueError("activation payloads must share one bf16 or fp16 dtype")
-        device = inputs.device
-        if device.type != "cuda" or grad_output.device != device or grad_inputs.device != device:
+        device = inputs.get_device()  # -1: not on a GPU
+        if device < 0 or grad_output.get_device() != device or grad_inputs.get_device() != device:
             raise ValueError("activation payloads must share one GPU")
-        if device.index != torch.cuda.current_device():
-            raise ValueError(f"activation payloads of {device} need it as the current device")
+        if device != _native.current_device():
+            raise ValueError(f"activation payloads of {inputs.device} need it as the current device")
         if not (inputs.is_contiguous() and grad_output.is_contiguous() and grad_inputs.is_contiguous()):
             raise ValueError("activation payloads must be contiguous")
         if grad_output.ndim < 1:
@@ -183,8 +183,9 @@ class Activation:
         rows = grad_output.numel() // width if width else 0
         desc = self.descriptor()
         _native.call(
-            "xp_activation_backward", _ptr(inputs), _ptr(grad_output), _ptr(grad_inputs), rows, width,
-            _DTYPE_CODES[dtype], _ORDER_CODES.get(order, 0), ctypes.byref(desc), _stream(),
+            "xp_activation_backward", inputs.data_ptr(), grad_output.data_ptr(), grad_inputs.data_ptr(), rows, width,
+            _DTYPE_CODES[dtype], 0 if order is None else _ORDER_CODES[order], ctypes.byref(desc),
+            _native.current_stream(device),
         )
 
 
