@@ -377,7 +377,8 @@ __global__ __launch_bounds__(kRouteThreads) void adapter_route_transpose_kernel(
 // The K ranges' sums of t (u) in range order as the coefficient operands of the outer products: for each
 // tile of 64 positions, step of 32 (fp32: 16) positions and 16 ranks, lane l's 16 bytes are those of rank
 // l % 16 and the 8 (4) positions from 8 (4) (l / 16), 16-bit payloads' as two planes of bf16 terms;
-// positions past the tile are zero.  One workgroup per tile.
+// positions past the tile are zero.  One workgroup per tile.  Bound by latency (4.8 us at 4096 rows); the
+// outer products' many workgroups of a tile read the result as often as there are column blocks.
 __global__ __launch_bounds__(256) void adapter_terms_kernel(AdapterTermsArgs a) {
   __shared__ int list[kAdapterTileRows];
   __shared__ float values[kAdapterTileRows][kAdapterMaxRank + 1];
@@ -453,6 +454,9 @@ __global__ __launch_bounds__(256) void adapter_terms_kernel(AdapterTermsArgs a) 
 }
 
 // ------------------------------------------------------------------ gradients of several runs
+// The runs' sums of an adapter's gradients in run order, times its scale; zeros for an adapter without
+// rows.  Reads what the outer products left in the last-level cache: 5.8 us for two runs of 28672 columns
+// of rank 16, 2 to 4 where there is nothing to add.
 __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterReduceArgs a) {
   const bool second = static_cast<int64_t>(blockIdx.x) >= a.blocks0;
   const AdapterOuterJob &job = a.job[second ? 1 : 0];
