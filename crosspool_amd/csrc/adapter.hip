@@ -505,8 +505,7 @@ constexpr int64_t kMaxRanges = 8;
 constexpr int64_t kStepsPerWorkgroup = 16;  // the least: four steps per wave
 constexpr int64_t kExpandWorkgroups = 512;
 // Decode has a tile per adapter at most, of a few rows each: three workgroups per CU, were each row its
-// own tile, read B faster than more of them with a fixed cost each (48 rows of 8 adapters of rank 32 x
-// 24576 columns: 16.2 us, of 512 workgroups per tile 19.9).
+// own tile (48 rows of 32 adapters of rank 32 x 24576 columns: 13.8 us; with half or twice as many 17.5).
 constexpr int64_t kDirectWorkgroups = 768;
 constexpr int64_t kOuterWorkgroups = 512;
 constexpr int64_t kMinRunRows = 256;

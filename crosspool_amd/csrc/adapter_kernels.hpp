@@ -377,8 +377,9 @@ __global__ __launch_bounds__(kAdapterShrinkWaves *kWave, RT <= 2 ? 4 : 2) void a
 // times the address cycles, 60 us instead of 39 for 8192 x 4096 at rank 64 in bf16.)
 //
 // Sorted batches give each wave 16 rows of a tile and stage a unit's B rows in LDS, read from memory
-// once and in order, one unit ahead.  Small ones (decode) give each wave a unit of its own and take the B
-// rows straight as operands.  Bound by base and output, whose 256-byte pieces of 64 rows read and write
+// once and in order, one unit ahead.  Small ones (decode) give each wave a unit of its own and turn the B
+// rows in its LDS as shrink does (48 rows of 32 adapters of rank 32 x 24576: 16.4 us, 13.8 so, 4 TB/s of B's
+// 64-byte rows).  Bound by base and output, whose 256-byte pieces of 64 rows read and write
 // below a plain copy's rate: 2048 x 24576 with a gated SiLU at rank 32 40.7 us (3.8 TB/s), 8192 x 4096 at
 // rank 64 39 us (3.4 TB/s).  A second unit in flight, two to three times the workgroups and nontemporal
 // stores changed nothing or cost up to a fifth.
@@ -536,6 +537,7 @@ struct AdapterExpand {
   static constexpr int PLANES = F16 ? 2 : 1;               // fp16 is staged as its two bf16 terms
   static constexpr int PLANE_BYTES = UNIT * C * 16;
   static constexpr int TERM_BYTES = kAdapterTileRows * kAdapterTermStride<P, RT>;
+  static constexpr int TURN_BYTES = kAdapterExpandWaves * CH * 1024;
   static constexpr int LDS_BYTES = 2 * PLANES * PLANE_BYTES > TERM_BYTES ? 2 * PLANES * PLANE_BYTES : TERM_BYTES;
 
   const AdapterExpandArgs &a;
@@ -732,8 +734,7 @@ __device__ __forceinline__ void clear(f32x4 (&acc)[CH]) {
   }
 }
 
-// The columns of a unit go to the waves (decode): B rows straight from memory as operands, for each 16
-// of the tile's rows.
+// The units of columns go to the waves (decode), for each 16 of the tile's rows.
 template <class P, int RT, AdapterAct ACT>
 __device__ __forceinline__ void expand_by_columns(const AdapterExpandArgs &a, const AdapterTile &tile, unsigned char *lds,
                                                   float scale, int64_t whole, int64_t begin, int64_t stop,
@@ -741,6 +742,12 @@ __device__ __forceinline__ void expand_by_columns(const AdapterExpandArgs &a, co
   using Work = AdapterExpand<P, RT, ACT>;
   constexpr int CH = Work::CH;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int lane = lane_here();
+  // Loading, lane l has chunk l % 4 of the l / 4-th row; multiplying, chunk l / 16 of the l % 16-th (shrink's
+  // exchange of chunks).
+  unsigned char *own = lds + Work::TERM_BYTES + wave * CH * 1024;
+  const int put = (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 4)) << 4);
+  const int get = (lane & 15) * 64 + (((lane >> 4) ^ (lane >> 2 & 3)) << 4);
 #pragma unroll 1
   for (int first = 0; first < tile.rows; first += 16) {
     Work work(a, whole, tile, first);
@@ -755,7 +762,7 @@ __device__ __forceinline__ void expand_by_columns(const AdapterExpandArgs &a, co
         for (int j = 0; j < CH; ++j) {
 #pragma unroll
           for (int f = 0; f < Work::FRAGS; ++f) {
-            ws[j][f] = work.load_chunk_of(c0 + CH * work.lane16 + j, (f * 4 + work.quarter) % Work::C);
+            ws[j][f] = work.load_chunk_of(c0 + CH * (lane >> 2) + j, (f * 4 + (lane & 3)) % Work::C);
           }
         }
         if (stage_here && first == 0 && c0 == begin + wave * Work::UNIT) {
@@ -765,12 +772,17 @@ __device__ __forceinline__ void expand_by_columns(const AdapterExpandArgs &a, co
         }
         work.load_terms(lds, first);
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
+        for (int f = 0; f < Work::FRAGS; ++f) {
 #pragma unroll
-          for (int f = 0; f < Work::FRAGS; ++f) {
+          for (int j = 0; j < CH; ++j) {
+            *reinterpret_cast<u32x4 *>(own + j * 1024 + put) = ws[j][f];
+          }
+#pragma unroll
+          for (int j = 0; j < CH; ++j) {
+            const u32x4 turned = *reinterpret_cast<const u32x4 *>(own + j * 1024 + get);
             u32x4 high;
             u32x4 low;
-            chunk_terms<P>(work.within_rank(ws[j][f], (f * 4 + work.quarter) % Work::C), high, low);
+            chunk_terms<P>(work.within_rank(turned, (f * 4 + work.quarter) % Work::C), high, low);
 #pragma unroll
             for (int s = f; s < Work::STEPS; s += Work::FRAGS) {
               work.add_products(acc, j, s, high, low);
@@ -895,7 +907,7 @@ __device__ __forceinline__ void expand_tile(const AdapterExpandArgs &a, const Ad
 template <class P, int RT, AdapterAct ACT, bool DIRECT>
 __global__ __launch_bounds__(kAdapterExpandWaves *kWave, RT <= 2 ? 3 : 2) void adapter_expand_kernel(AdapterExpandArgs a) {
   using Work = AdapterExpand<P, RT, ACT>;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[DIRECT ? Work::TERM_BYTES : Work::LDS_BYTES];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[DIRECT ? Work::TERM_BYTES + Work::TURN_BYTES : Work::LDS_BYTES];
   const int64_t begin = static_cast<int64_t>(blockIdx.x) * a.columns;
   const int64_t end = begin + a.columns < a.n ? begin + a.columns : a.n;
   for (int64_t slot = blockIdx.y;; slot += gridDim.y) {
