@@ -187,6 +187,30 @@ def test_large_pools_and_many_groups(device):
     check_forward(case, run(case))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("k", [3, 4, 5, 7, 8, 9, 15, 31, 32, 39, 66, 1030])
+def test_widths_that_cut_a_chunk(device, k, dtype):
+    for rows in (7, 80):
+        case = Case(device, rows=rows, k=k, n=k, count=2, max_rank=20, ranks=[20, 9], dtype=dtype, seed=k)
+        check_forward(case, run(case))
+        check_backward(case, backward(case))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows", [5, 70])
+def test_an_infinity_before_a_cut_chunk_is_counted_once(device, rows, dtype):
+    """Rank 1: an infinite product is the sum, its sign B's; taken a second time times zero it would be NaN."""
+
+    for column in (5, 6, 11, 12):
+        case = Case(device, rows=rows, k=13, n=24, count=1, max_rank=1, dtype=dtype, ids=[0] * rows)
+        case.a.abs_().clamp_(min=0.25)
+        case.x[2, column] = float("inf")
+        got = run(case).cpu()
+        expected = torch.where(case.b[0, :, 0] > 0, float("inf"), -float("inf"))
+        assert torch.equal(got[2].float(), expected)
+        assert bool(torch.isfinite(got[torch.arange(rows) != 2]).all())
+
+
 @pytest.mark.parametrize("count", [5, 70])
 @pytest.mark.parametrize("rows", [8192, 8193, 20011])
 def test_more_rows_than_the_sort_keeps(device, rows, count):
