@@ -490,7 +490,8 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterReduceArgs a
         for (int run = 0; run < runs; ++run) {
           sum += source[run * plane];
         }
-        sum *= scale;
+        // No rows: zero whatever the scale.
+        sum = runs > 0 ? sum * scale : 0.0f;
       }
       store_value(job.grad, static_cast<int64_t>(group) * elements + index, sum, a.dtype);
     }

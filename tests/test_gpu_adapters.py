@@ -460,6 +460,19 @@ def test_backward_of_no_rows_clears_the_gradients(device):
     run(case)
 
 
+@pytest.mark.parametrize("rows", [9, 700])
+def test_scales_of_unused_adapters_do_not_matter(device, rows):
+    case = Case(device, rows=rows, k=72, n=40, count=4, max_rank=8, ids=[(i % 3 - 1) * 2 if i % 3 else 0 for i in range(rows)])
+    case.ids[case.ids < 0] = -1
+    unused = [adapter for adapter in range(4) if not bool((case.ids == adapter).any())]
+    assert unused
+    expected, gradients = run(case), backward(case)
+    case.scales[unused] = float("inf")
+    got = backward(case)
+    assert torch.equal(run(case), expected)
+    assert all(torch.equal(got[name], gradients[name]) for name in got)
+
+
 def test_bad_ids_and_nan_rows_in_the_backward(device):
     case = Case(device, rows=100, k=64, n=72, count=3, max_rank=8, ids=[i % 3 for i in range(100)])
     case.ids[7] = 9
