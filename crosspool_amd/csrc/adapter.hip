@@ -677,7 +677,7 @@ KernelLaunch make_adapter_transpose(const AdapterRouteTransposeArgs &args) {
   return launch_of(func, transpose_grid(args.transpose), kRouteThreads, args);
 }
 
-KernelLaunch make_adapter_terms(const AdapterTermsArgs &args, const AdapterPlan &) {
+KernelLaunch make_adapter_terms(const AdapterTermsArgs &args) {
   return launch_of(reinterpret_cast<const void *>(&adapter_terms_kernel), dim3(tile_slots(args.batch), 2, 1), 256, args);
 }
 

@@ -914,9 +914,17 @@ __device__ __forceinline__ void expand_tile(const AdapterExpandArgs &a, const Ad
 }
 
 template <class P, int RT, AdapterAct ACT, bool DIRECT>
-__global__ __launch_bounds__(kAdapterExpandWaves *kWave, RT <= 2 ? 3 : 2) void adapter_expand_kernel(AdapterExpandArgs a) {
-  using Work = AdapterExpand<P, RT, ACT>;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[DIRECT ? Work::TERM_BYTES + Work::TURN_BYTES : Work::LDS_BYTES];
+constexpr int kExpandLds = DIRECT ? AdapterExpand<P, RT, ACT>::TERM_BYTES + AdapterExpand<P, RT, ACT>::TURN_BYTES
+                                  : AdapterExpand<P, RT, ACT>::LDS_BYTES;
+
+// Workgroups per CU: what the registers hold, or one where the LDS (160 KB) holds no second.
+template <class P, int RT, AdapterAct ACT, bool DIRECT>
+constexpr int kExpandPerCu = (2 * kExpandLds<P, RT, ACT, DIRECT> > 160 * 1024) ? 1 : RT <= 2 ? 3 : 2;
+
+template <class P, int RT, AdapterAct ACT, bool DIRECT>
+__global__ __launch_bounds__(kAdapterExpandWaves *kWave, (kExpandPerCu<P, RT, ACT, DIRECT>))
+void adapter_expand_kernel(AdapterExpandArgs a) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kExpandLds<P, RT, ACT, DIRECT>];
   const int64_t begin = static_cast<int64_t>(blockIdx.x) * a.columns;
   const int64_t end = begin + a.columns < a.n ? begin + a.columns : a.n;
   for (int64_t slot = blockIdx.y;; slot += gridDim.y) {

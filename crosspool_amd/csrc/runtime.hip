@@ -1965,7 +1965,7 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
                                    shape.dtype == XP_DTYPE_F32 ? 1 : 0};
       // Before the input's gradient: grad_out and x are still in the last level of cache (4096 rows of
       // 4096 x 24576: the outer products take 37 us instead of 43).
-      XP_HIP_CHECK(launch(make_adapter_terms(terms, plan), hip_stream));
+      XP_HIP_CHECK(launch(make_adapter_terms(terms), hip_stream));
       XP_HIP_CHECK(launch(make_adapter_outer(outer, plan, shape.dtype), hip_stream));
     }
     const AdapterReduceArgs reduce{batch, pool->ranks, pool->scales, {outer.job[0], outer.job[1]}, 0, max_rank, rp,

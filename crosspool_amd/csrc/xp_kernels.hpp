@@ -522,7 +522,6 @@ struct AdapterPlan {
   int64_t max_runs;
   int64_t ranges[2];         // K ranges of the products over input_width and over output_width
   int64_t steps_per_range[2];
-  int64_t stride;            // backward: positions of a row of terms
   // Byte offsets of the workspace's regions, and its size.
   size_t route, partials[2], terms[2], sums[2], at, bt, bytes;
 };
@@ -542,7 +541,7 @@ KernelLaunch make_adapter_expand(const AdapterExpandArgs &args, const AdapterPla
 bool adapter_routes_beside_transpose(const AdapterBatch &batch);
 KernelLaunch make_adapter_route_transpose(const AdapterRouteTransposeArgs &args);
 KernelLaunch make_adapter_transpose(const AdapterRouteTransposeArgs &args);
-KernelLaunch make_adapter_terms(const AdapterTermsArgs &args, const AdapterPlan &plan);
+KernelLaunch make_adapter_terms(const AdapterTermsArgs &args);
 KernelLaunch make_adapter_outer(const AdapterOuterArgs &args, const AdapterPlan &plan, int dtype);
 KernelLaunch make_adapter_reduce(const AdapterReduceArgs &args);
 
