@@ -460,6 +460,57 @@ def test_backward_of_no_rows_clears_the_gradients(device):
     run(case)
 
 
+@pytest.mark.parametrize("wide", ["x", "base", "out", "grad", "grad_base", "grad_x"])
+def test_rows_whose_offsets_pass_32_bits(device, wide):
+    """2100 rows, 2^21 elements apart: 8.8 GB from the first row to the last."""
+
+    case = Case(device, rows=2100, k=72, n=48, count=3, max_rank=8, seed=3)
+    expected, gradients = run(case), backward(case)
+    far = torch.empty((2100, 1 << 21), dtype=case.dtype, device=device)
+    operands = {"x": case.x.to(device), "base": case.base.to(device), "grad": case.grad.to(device),
+                "grad_base": case.grad_base.to(device), "out": torch.zeros_like(expected),
+                "grad_x": torch.zeros_like(gradients["x"])}
+    spread = far[:, -operands[wide].shape[1]:]
+    spread.copy_(operands[wide])
+    operands[wide] = spread
+    operator, weights, ids = case.operator(backward=True), case.weights(), case.ids.to(device)
+    operator.run_into(operands["x"], weights, adapter_ids=ids, base=operands["base"], output=operands["out"])
+    assert torch.equal(operands["out"], expected)
+    ga, gb = torch.empty_like(gradients["a"]), torch.empty_like(gradients["b"])
+    operator.backward_into(operands["x"], operands["grad"], weights, adapter_ids=ids, base=operands["grad_base"],
+                           grad_inputs=operands["grad_x"], grad_a=ga, grad_b=gb)
+    assert torch.equal(operands["grad_x"], gradients["x"])
+    assert torch.equal(ga, gradients["a"]) and torch.equal(gb, gradients["b"])
+
+
+@pytest.mark.parametrize("k,n", [(20000, 64), (64, 20000)])
+def test_pools_whose_offsets_pass_32_bits(device, k, n):
+    """1024 adapters of 5 MB each, two of them in use at the end, against a pool of those two."""
+
+    for rows in (40, 150):
+        small = Case(device, rows=rows, k=k, n=n, count=2, max_rank=128, seed=rows)
+        expected, gradients = run(small), backward(small)
+        a = torch.zeros((1024, 128, k), dtype=small.dtype, device=device)
+        b = torch.zeros((1024, n, 128), dtype=small.dtype, device=device)
+        scales = torch.ones(1024, device=device)
+        used = [1022, 1023]
+        a[used], b[used], scales[used] = small.a.to(device), small.b.to(device), small.scales.to(device)
+        plan = AdapterPlan.prepare(row_capacity=rows, adapter_count=1024, max_rank=128, input_width=k, output_width=n,
+                                   dtype=small.dtype, backward=True)
+        operator = Adapter(plan, torch.empty(plan.workspace.nbytes, dtype=torch.uint8, device=device))
+        weights = AdapterWeights(a, b, scales)
+        ids = torch.where(small.ids >= 0, small.ids + 1022, -1).to(device)
+        x, out = small.x.to(device), torch.empty_like(expected)
+        operator.run_into(x, weights, adapter_ids=ids, base=small.base.to(device), output=out)
+        assert torch.equal(out, expected)
+        gx, ga, gb = torch.empty_like(x), torch.full_like(a, 1.0), torch.full_like(b, 1.0)
+        operator.backward_into(x, small.grad.to(device), weights, adapter_ids=ids, base=small.grad_base.to(device),
+                               grad_inputs=gx, grad_a=ga, grad_b=gb)
+        assert torch.equal(gx, gradients["x"])
+        assert torch.equal(ga[used], gradients["a"]) and torch.equal(gb[used], gradients["b"])
+        assert not bool(ga[:1022].any()) and not bool(gb[:1022].any())
+
+
 @pytest.mark.parametrize("rows", [9, 700])
 def test_scales_of_unused_adapters_do_not_matter(device, rows):
     case = Case(device, rows=rows, k=72, n=40, count=4, max_rank=8, ids=[(i % 3 - 1) * 2 if i % 3 else 0 for i in range(rows)])
