@@ -171,6 +171,28 @@ def test_in_place_and_graph(device):
         assert torch.equal(out, eager)
 
 
+@pytest.mark.parametrize("order", [GateUpOrder.INTERLEAVED, GateUpOrder.CONCATENATED, None])
+def test_as_many_values_as_a_call_takes(device, order):
+    """2^31 outputs: the rows at both ends and in the middle are those of calls of their own."""
+
+    rows, width = 1 << 16, 1 << 15
+    wide = width if order is None else 2 * width
+    activation = Activation(SiluActivation(), None if order is None else GateTransform())
+    inputs = torch.zeros((rows, wide), dtype=torch.bfloat16, device=device)
+    grad = torch.zeros((rows, width), dtype=torch.bfloat16, device=device)
+    out = torch.full_like(inputs, 1.0)
+    parts = [slice(0, 3), slice((1 << 15) - 2, (1 << 15) + 2), slice(rows - 3, rows)]
+    for part in parts:
+        inputs[part].normal_()
+        grad[part].normal_()
+    activation.backward_into(inputs=inputs, grad_output=grad, grad_inputs=out, order=order)
+    for part in parts:
+        own = torch.empty_like(inputs[part])
+        activation.backward_into(inputs=inputs[part], grad_output=grad[part], grad_inputs=own, order=order)
+        assert torch.equal(out[part], own) and bool(own.any())
+    assert not bool(out[100:200].any())
+
+
 def test_refusals(device):
     activation = Activation(SiluActivation(), GateTransform())
     inputs = torch.zeros((4, 16), dtype=torch.bfloat16, device=device)

@@ -352,6 +352,21 @@ def test_in_place_base_absent_base_and_strided_rows(device, rows):
     assert torch.equal(out + 0.0, with_zero + 0.0)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("max_rank", [8, 16, 32, 100])
+@pytest.mark.parametrize("rows", [60, 200])
+def test_rows_do_not_depend_on_who_shares_their_adapter(device, rows, max_rank, dtype):
+    """fp32 bits (bf16 ones of a sum that the store's rounding would hide are spread by a base of zero)."""
+
+    outs = []
+    for alone in (False, True):
+        ids = [0 if i < 5 or not alone else 1 for i in range(rows)]
+        case = Case(device, rows=rows, k=2100, n=136, count=2, max_rank=max_rank, dtype=dtype, ids=ids, seed=11)
+        case.base.zero_()
+        outs.append(run(case).cpu()[:5])
+    assert torch.equal(outs[0], outs[1])
+
+
 def test_rows_of_a_batch_do_not_depend_on_their_order(device):
     case = Case(device, rows=333, k=264, n=136, count=6, max_rank=16, seed=11)
     out = run(case)
