@@ -17,7 +17,7 @@
 // need a fraction of the time that the rows' bytes do.  t, u and all sums are fp32.  16-bit
 // payloads multiply t (u) as two bf16 terms, its leading 16 bits truncated and the rest rounded
 // (relative error 2^-17, below the 2^-9 of the output's rounding); fp16 weights and rows beside it
-// are split the same way, exactly, because fp16 terms of t would overflow or lose the small ones.
+// are split the same way (within 2^-133), because fp16 terms of t would overflow or lose the small ones.
 #pragma once
 
 #include "xp_elements.hpp"
@@ -120,14 +120,18 @@ __device__ __forceinline__ AdapterTile adapter_tile(const AdapterBatch &batch, c
   return tile;
 }
 
-// The two bf16 terms of a pair of values: leading bits truncated, the rest to nearest even.  An
-// infinite or NaN value has no rest.
+// The two bf16 terms of a pair of values: leading bits truncated, the rest to nearest even.  Both have the
+// value's sign, and neither is zero unless the value is: a rest of zero would make NaN of an infinite factor, so
+// bf16's smallest number (2^-133; the matrix cores keep subnormal operands) is added to every rest, far
+// below the rest's own rounding where the value is above 2^-110.
 __device__ __forceinline__ float leading_term(float value) {
   const uint32_t bits = __float_as_uint(value);
   return __uint_as_float((bits & 0xffff0000u) | (value != value ? 0x00400000u : 0u));
 }
 __device__ __forceinline__ float rest_term(float value, float leading) {
-  return (__float_as_uint(value) & 0x7f800000u) == 0x7f800000u ? 0.0f : value - leading;
+  constexpr float kLeast = 0x1p-133f;
+  const float rest = (__float_as_uint(value) & 0x7f800000u) == 0x7f800000u ? 0.0f : value - leading;
+  return rest + __builtin_amdgcn_fmed3f(value, -kLeast, kLeast);
 }
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t &high, uint32_t &low) {
   const float ha = leading_term(a);
@@ -136,7 +140,7 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t &high, uin
   low = Bf16Payload::pack2(rest_term(a, ha), rest_term(b, hb));
 }
 
-// A chunk of P as bf16 terms: itself (bf16), or the exact pair (fp16).
+// A chunk of P as bf16 terms: itself (bf16), or two terms (fp16).
 template <class P>
 __device__ __forceinline__ void chunk_terms(u32x4 chunk, u32x4 &high, u32x4 &low) {
   if constexpr (std::is_same_v<P, F16Payload>) {

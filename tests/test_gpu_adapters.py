@@ -662,3 +662,47 @@ def test_refusals_on_the_device(device):
     both = torch.zeros((5, 48), dtype=torch.bfloat16, device=device)
     with pytest.raises(_native.NativeError, match="base"):
         square.operator().run_into(xs, square.weights(), adapter_ids=square.ids.to(device), base=both[:4], output=both[1:])
+
+
+def powers(shape, g, dtype):
+    """Signed powers of two: exact in bf16, so that every rest of a two-term split is zero."""
+
+    return (torch.randint(0, 2, shape, generator=g) * 2.0 - 1.0).mul(2.0 ** torch.randint(-2, 3, shape, generator=g)).to(dtype)
+
+
+def assert_same_kinds(actual, value, what):
+    """Infinities with their signs and NaN exactly where the definition has them."""
+
+    actual = actual.cpu().double()
+    assert torch.equal(actual.isnan(), value.isnan()), f"{what}: NaN at {(actual.isnan() != value.isnan()).nonzero()[:4].tolist()}"
+    for sign in (1, -1):
+        assert torch.equal(actual == sign * float("inf"), value == sign * float("inf")), what
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows", [5, 90])
+@pytest.mark.parametrize("where", ["x", "a", "b", "grad", "x_and_b"])
+@pytest.mark.parametrize("exact", [True, False], ids=["powers_of_two", "random"])
+def test_infinities_are_those_of_the_definition(device, exact, where, rows, dtype):
+    """An infinite factor times a finite one is infinite, whatever terms the finite one is split into."""
+
+    g = torch.Generator().manual_seed(rows)
+    case = Case(device, rows=rows, k=70, n=146, count=2, max_rank=12, ranks=[12, 1], dtype=dtype,
+                ids=[i % 3 - 1 for i in range(rows)])
+    if exact:
+        case.a, case.b = powers(case.a.shape, g, case.dtype), powers(case.b.shape, g, case.dtype)
+        case.x, case.grad = powers(case.x.shape, g, case.dtype), powers(case.grad.shape, g, case.dtype)
+    infinity = float("inf")
+    if where in ("x", "x_and_b"):
+        case.x[2, 33], case.x[4, 69] = infinity, -infinity
+    if where in ("b", "x_and_b"):
+        case.b[1, 7, 0], case.b[1, 145, 0], case.b[0, 100, 3] = infinity, -infinity, infinity
+    if where == "a":
+        case.a[1, 0, 9], case.a[0, 3, 69] = -infinity, infinity
+    if where == "grad":
+        case.grad[2, 5], case.grad[4, 140] = infinity, -infinity
+    value, _ = case.forward()
+    assert_same_kinds(run(case), value, "output")
+    got = backward(case)
+    for name, (value, _) in case.backward().items():
+        assert_same_kinds(got[name], value, f"gradient of {name}")
