@@ -422,13 +422,21 @@ __device__ __forceinline__ void store_values(unsigned char *out, const float (&v
   *reinterpret_cast<Words *>(out) = packed;
 }
 
+// f(g) (u + offset) of the sum, any f.
+__device__ __forceinline__ float gated_value(float gate, float up, ActivationArgs act) {
+  if (act.has_limit) {
+    clip_keep_nan(gate, up, act.limit);
+  }
+  act.has_limit = 0;
+  return apply_gated(gate, up, act);
+}
+
 // silu(g) (u + offset).  16-bit results take the hardware's exp and reciprocal (relative error below
 // 2^-16, under the store's 2^-9 or 2^-12), fp32 ones expf and an IEEE divide as elsewhere.
 template <class P>
 __device__ __forceinline__ float gated_silu_value(float gate, float up, const ActivationArgs &act) {
   if (act.has_limit) {
-    gate = fminf(gate, act.limit);
-    up = fminf(fmaxf(up, -act.limit), act.limit);
+    clip_keep_nan(gate, up, act.limit);
   }
   if constexpr (kElementBytes<P> == 4) {
     return gate / (1.0f + expf(-act.alpha * gate)) * (up + act.up_offset);
@@ -526,7 +534,7 @@ __device__ __forceinline__ void expand_columns(const AdapterExpandArgs &a, const
       if constexpr (ACT == AdapterAct::GatedSilu) {
         value = gated_silu_value<P>(gate, up, a.act);
       } else {
-        value = apply_gated(gate, up, a.act);
+        value = gated_value(gate, up, a.act);
       }
       store_value(a.out, row * a.ld_out + first / 2 + n, value, kDtypeOf<P>);
     } else {
@@ -716,7 +724,7 @@ struct AdapterExpand {
           if constexpr (ACT == AdapterAct::GatedSilu) {
             activated[j] = gated_silu_value<P>(value[2 * j], value[2 * j + 1], act);
           } else {
-            activated[j] = apply_gated(value[2 * j], value[2 * j + 1], act);
+            activated[j] = gated_value(value[2 * j], value[2 * j + 1], act);
           }
         }
         store_values<P>(out + (row[q] * a.ld_out + n / 2) * ES, activated);
@@ -868,7 +876,7 @@ __device__ __forceinline__ void expand_by_rows(const AdapterExpandArgs &a, const
   }
 }
 
-// Rows with an id out of range: NaN past the activation, whose limit (ReLU's zero) could hide one before it.
+// Rows with an id out of range: NaN past the activation.
 template <class P, AdapterAct ACT>
 __device__ __forceinline__ void fill_with_nan(const AdapterExpandArgs &a, const AdapterTile &tile, int64_t begin,
                                               int64_t end) {

@@ -73,6 +73,13 @@ __device__ __forceinline__ float apply_gated(float gate, float up, const Activat
   return apply_function(gate, act) * (up + act.up_offset);
 }
 
+// A gated pair within the limit.  NaN is past no limit and stays (fminf and fmaxf, which the projections'
+// and the standalone activation's epilogues above take, would make the limit of it).
+__device__ __forceinline__ void clip_keep_nan(float &gate, float &up, float limit) {
+  gate = gate > limit ? limit : gate;
+  up = up > limit ? limit : up < -limit ? -limit : up;
+}
+
 // The fp32 element type beside Bf16Payload / F16Payload: a 16-byte chunk holds 4 columns, and
 // its MFMA step covers 8 (lane half h multiplies columns 4 h + j of both operands at step j).
 struct F32Payload {

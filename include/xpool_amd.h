@@ -212,7 +212,8 @@ size_t xp_adapter_workspace_bytes(int64_t rows, int64_t count, int64_t max_rank,
  * [rows, output_width / 2] over INTERLEAVED Gate/Up columns), element-aligned, with row strides of
  * ldx, ld_base and ld_out elements.  Without an activation out may be base itself (same pointer and
  * stride); no other overlap.  All sums are fp32; one rounding, at the store (with an activation the
- * sum is not rounded before it, unlike xp_projection's).  The result of a row depends on its own
+ * sum is not rounded before it, unlike xp_projection's; a NaN sum stays NaN past a limit, which
+ * xp_projection and xp_activation make the limit of).  The result of a row depends on its own
  * values and id and on the row count, not on the other rows' adapters or order.  An id outside
  * [-1, count) gives a row of quiet NaNs and ORs XP_FAULT_ADAPTER_OUT_OF_RANGE into fault_word (may be
  * NULL). */

@@ -706,3 +706,34 @@ def test_infinities_are_those_of_the_definition(device, exact, where, rows, dtyp
     got = backward(case)
     for name, (value, _) in case.backward().items():
         assert_same_kinds(got[name], value, f"gradient of {name}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows", [6, 100])
+@pytest.mark.parametrize("function", [SiluActivation(), GeluActivation(), ReluActivation()], ids=["silu", "gelu", "relu"])
+def test_no_limit_hides_a_nan_of_the_sum(device, function, rows, dtype):
+    """NaN in a row, in a base's Gate or in its Up: neither is below a limit nor above one."""
+
+    case = Case(device, rows=rows, k=64, n=542, count=3, max_rank=8, dtype=dtype, ids=[i % 4 - 1 for i in range(rows)])
+    activation = Activation(function, GateTransform(1.5, 1.0))
+    outs = []
+    for bad in (False, True):
+        if bad:
+            case.x[1, 5] = float("nan")
+            case.base[2, 40], case.base[3, 41] = float("nan"), float("nan")   # Gate and Up of column 20
+            case.base[2, 540], case.base[3, 541] = float("nan"), float("nan")  # of the last column, past whole chunks
+            case.base[0, 100], case.base[0, 103] = float("inf"), -float("inf")  # clipped
+        out = torch.zeros((rows, 271), dtype=case.dtype, device=device)
+        case.operator().run_into(case.x.to(device), case.weights(), adapter_ids=case.ids.to(device),
+                                 base=case.base.to(device), output=out, activation=activation)
+        outs.append(out.cpu())
+    clean, got = outs
+    assert bool(got[1].isnan().all())
+    expected = torch.zeros_like(got, dtype=torch.bool)
+    expected[1] = True
+    expected[2:4, [20, 270]] = True
+    assert torch.equal(got.isnan(), expected)
+    assert bool(got[0].isfinite().all())
+    keep = torch.ones_like(expected)
+    keep[:4] = False
+    assert torch.equal(got[keep], clean[keep])
