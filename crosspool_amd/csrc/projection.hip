@@ -360,13 +360,14 @@ enum class Slope : int { Silu = 1, Relu = 2, GeluErf = 3, GeluTanh = 4 };
 template <Slope KIND>
 __device__ __forceinline__ void value_and_slope(float v, float alpha, float &value, float &slope) {
   if constexpr (KIND == Slope::Relu) {
-    const bool on = v > 0.0f || v != v;
-    value = on ? v : 0.0f;
-    slope = on ? 1.0f : 0.0f;
+    value = relu_keep_nan(v);
+    slope = v != v ? v : v > 0.0f ? 1.0f : 0.0f;
   } else if constexpr (KIND == Slope::GeluErf) {
     const float share = 0.5f * (1.0f + erff(v * 0.7071067811865476f));
     value = v * share;
-    slope = share + v * 0.3989422804014327f * __expf(-0.5f * v * v);
+    // Past 16 the density is 0 (and infinity times it would be NaN).
+    const float near = fminf(fmaxf(v, -16.0f), 16.0f);
+    slope = share + near * 0.3989422804014327f * __expf(-0.5f * near * near);
   } else if constexpr (KIND == Slope::GeluTanh) {
     // Past 16 the sigmoid is 0 or 1 and its slope 0 (and v^3 may overflow).
     const float near = fminf(fmaxf(v, -16.0f), 16.0f);
@@ -415,8 +416,9 @@ __device__ __forceinline__ void store_eight(uint16_t *target, int count, const f
   }
 }
 
-// out = f(min(g, limit)) (clamp(u, -limit, limit) + offset) =: f h, so dg = dout h f' where g <= limit,
-// du = dout f where |u| <= limit; ungated dv = dout f'.  A thread takes eight output columns: INTERLEAVED
+// out = f(min(g, limit)) (clamp(u, -limit, limit) + offset) =: f h, so dg = dout h f' but 0 where g > limit,
+// du = dout f but 0 where |u| > limit; ungated dv = dout f'.  NaN is past no limit: a NaN gate makes f and f'
+// NaN, a NaN up h.  A thread takes eight output columns: INTERLEAVED
 // pairs and ungated values are flat arrays (the only ragged group is the last); CONCATENATED rows go
 // by row.  Bound by memory: five values of traffic per output column (SiLU over 4096 rows of 12288
 // INTERLEAVED bf16 pairs: 87.4 us, 5.8 TB/s; 333 rows of 2053 CONCATENATED fp16 pairs 6.1 us, latency).
@@ -472,10 +474,9 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(ActivationBack
       bool gate_on = true;
       bool up_on = true;
       if (act.has_limit) {
-        clipped = fminf(gate, act.limit);
-        factor = fminf(fmaxf(up, -act.limit), act.limit);
-        gate_on = gate <= act.limit;
-        up_on = fabsf(up) <= act.limit;
+        clip_keep_nan(clipped, factor, act.limit);
+        gate_on = !(gate > act.limit);
+        up_on = !(fabsf(up) > act.limit);
       }
       float value;
       float slope;

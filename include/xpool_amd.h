@@ -177,8 +177,9 @@ int xp_activation(const void *inputs, void *output, int64_t rows, int64_t width,
 
 /* Gradient of xp_activation: grad_inputs, shaped and ordered as inputs, from the projected inputs and
  * grad_output [rows, width] (bf16 / fp16).  Gated, with h = clamp(u, -limit, limit) + up_offset:
- * dg = dout h f'(min(g, limit)) where g <= limit, du = dout f(min(g, limit)) where |u| <= limit, else 0
- * (limits only with has_limit); ungated: dv = dout f'(v).  fp32 inside, one rounding.  grad_inputs may be
+ * dg = dout h f'(min(g, limit)) but 0 where g > limit, du = dout f(min(g, limit)) but 0 where |u| > limit
+ * (limits only with has_limit); ungated: dv = dout f'(v).  A NaN g or u is not clipped (xp_activation makes the
+ * limit of it): a NaN g makes dg and du NaN, a NaN u dg.  fp32 inside, one rounding.  grad_inputs may be
  * inputs itself, and ungated grad_output itself.  At most 2^31 values of grad_output.  No counterpart
  * in the reference. */
 int xp_activation_backward(const void *inputs, const void *grad_output, void *grad_inputs, int64_t rows, int64_t width,

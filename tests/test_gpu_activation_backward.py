@@ -211,3 +211,47 @@ def test_refusals(device):
                                  order=GateUpOrder.INTERLEAVED)
     empty = torch.empty((0, 16), dtype=torch.bfloat16, device=device)
     activation.backward_into(inputs=empty, grad_output=empty[:, :8].contiguous(), grad_inputs=empty, order=GateUpOrder.INTERLEAVED)
+
+
+NAN, INFINITY = float("nan"), float("inf")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("name", list(ACTIVATIONS))
+@pytest.mark.parametrize("order", [GateUpOrder.INTERLEAVED, GateUpOrder.CONCATENATED], ids=["pairs", "halves"])
+@pytest.mark.parametrize("limit", [None, 2.0])
+def test_nan_reaches_the_gradients_of_its_pair(device, limit, order, name, dtype):
+    """A NaN Gate gives NaN for both, a NaN Up for the Gate's (its factor) while Up's own is dout f(g); a NaN in
+    the output's gradient gives NaN for both.  A limit clips infinities, not NaN."""
+
+    gate = torch.tensor([[1.0, NAN, 0.5, 1.0, NAN, INFINITY, 1.0, 0.5]])
+    up = torch.tensor([[1.0, 1.0, NAN, -0.5, NAN, 1.0, -INFINITY, 0.5]])
+    grad = torch.tensor([[1.0, 1.0, 1.0, NAN, 1.0, 1.0, 1.0, 2.0]]).to(DTYPES[dtype])
+    inputs = torch.stack((gate, up), dim=2).flatten(1) if order is GateUpOrder.INTERLEAVED else torch.cat((gate, up), dim=1)
+    got = torch.zeros(inputs.shape, dtype=DTYPES[dtype], device=device)
+    Activation(ACTIVATIONS[name], GateTransform(limit, 1.0)).backward_into(
+        inputs=inputs.to(DTYPES[dtype]).to(device), grad_output=grad.to(device), grad_inputs=got, order=order)
+    grad_gate, grad_up = split(got.cpu().float(), order, 8)
+    assert grad_gate.isnan().tolist() == [[False, True, True, True, True, False, False, False]]
+    assert grad_up.isnan().tolist() == [[False, True, False, True, True, False, False, False]]
+    # A finite Gate beside a NaN Up: dout f(g), as beside any other Up.
+    assert torch.equal(grad_up[0, 2], grad_up[0, 7] / 2)
+    if limit is None:
+        # f(inf) = inf, f'(inf) = 1 and h = 2; an infinite Up makes the Gate's gradient infinite.
+        assert grad_up[0, 5] == INFINITY and grad_gate[0, 5] == 2.0
+        assert grad_gate[0, 6] == -INFINITY
+    else:
+        # Clipped: the Gate's gradient and the Up's are zero, the other factors those at the limit.
+        assert grad_gate[0, 5] == 0.0 and grad_up[0, 6] == 0.0
+        assert bool(grad_up[0, 5].isfinite()) and grad_up[0, 5] > 0 and bool(grad_gate[0, 6].isfinite())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("name", list(ACTIVATIONS))
+def test_nan_and_infinity_of_ungated_values(device, name, dtype):
+    values = torch.tensor([[NAN, INFINITY, 1.0, 0.0]], dtype=DTYPES[dtype], device=device)
+    grad = torch.tensor([[1.0, 1.0, NAN, 1.0]], dtype=DTYPES[dtype], device=device)
+    out = torch.zeros_like(values)
+    Activation(ACTIVATIONS[name], None).backward_into(inputs=values, grad_output=grad, grad_inputs=out, order=None)
+    assert out.isnan().tolist() == [[True, False, True, False]]
+    assert out[0, 1] == 1.0 and out[0, 3] == (0.0 if name == "relu" else 0.5)
