@@ -255,3 +255,50 @@ def test_nan_and_infinity_of_ungated_values(device, name, dtype):
     Activation(ACTIVATIONS[name], None).backward_into(inputs=values, grad_output=grad, grad_inputs=out, order=None)
     assert out.isnan().tolist() == [[True, False, True, False]]
     assert out[0, 1] == 1.0 and out[0, 3] == (0.0 if name == "relu" else 0.5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("name", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("order", [GateUpOrder.INTERLEAVED, GateUpOrder.CONCATENATED], ids=["pairs", "halves"])
+def test_tails_keep_their_relative_accuracy(device, order, name, dtype):
+    """Gates from -8 to -3, where f and f' are down to 1e-14, relative to the sizes of their own terms.
+
+    erf form: the argument v / sqrt 2 is off by 2^-23 relatively, and (v^2 + 2) is how much more its
+    complementary error function is; exp(-v^2 / 2) likewise, with the exponent's product by log2 e rounded
+    once more: (v^2 + 2) 2^-22 covers both.  tanh form: sigmoid(2 y) with 2 y off by four roundings and the exponent's
+    product: (|2 y| + 2) 2^-21.  SiLU: (|v| + 2) 2^-21 the same way.  The library's complementary error
+    function and the hardware's exp and reciprocal add units in the last place: 2^-20.
+    """
+
+    g = torch.Generator().manual_seed(3)
+    rows, width = 64, 129
+    gate = (torch.rand((rows, width), generator=g) * -5 - 3).to(DTYPES[dtype])
+    up = torch.randn((rows, width), generator=g).to(DTYPES[dtype])
+    # fp16 outputs of 1e-14 would round to zero: gradients as large as a loss scale makes them.
+    grad = (torch.rand((rows, width), generator=g) + 0.5).mul(1.0 if dtype == "bf16" else 2.0**14).to(DTYPES[dtype])
+    inputs = torch.stack((gate, up), dim=2).flatten(1) if order is GateUpOrder.INTERLEAVED else torch.cat((gate, up), dim=1)
+    got = torch.full(inputs.shape, NAN, dtype=DTYPES[dtype], device=device)
+    Activation(ACTIVATIONS[name], GateTransform()).backward_into(
+        inputs=inputs.to(device), grad_output=grad.to(device), grad_inputs=got, order=order)
+    v, u, d = gate.double(), up.double(), grad.double()
+    if name == "gelu":
+        share, density = 0.5 * torch.special.erfc(-v * 2**-0.5), torch.exp(-v * v / 2) * (2 * torch.pi) ** -0.5
+        terms, relative = (share, v * density), (v * v + 2) * 2.0**-22 + 2.0**-20
+    elif name == "gelu_tanh":
+        c = (2 / torch.pi) ** 0.5
+        twice = 2 * c * (v + 0.044715 * v**3)
+        share = torch.sigmoid(twice)
+        terms = (share, v * share * torch.sigmoid(-twice) * 2 * c * (1 + 3 * 0.044715 * v * v))
+        relative = (twice.abs() + 2) * 2.0**-21 + 2.0**-20
+    else:
+        share = torch.sigmoid(v)
+        terms, relative = (share, v * share * torch.sigmoid(-v)), (v.abs() + 2) * 2.0**-21 + 2.0**-20
+    smallest = {"bf16": 2.0**-134, "fp16": 2.0**-25}[dtype]
+    for actual, value, size in zip(
+        split(got.cpu().double(), order, width), (d * u * (terms[0] + terms[1]), d * v * share),
+        ((d * u).abs() * (terms[0].abs() + terms[1].abs()), (d * v * share).abs()),
+    ):
+        bound = size * relative
+        allowed = bound + (value.abs() + bound) * torch.finfo(DTYPES[dtype]).eps / 2 + smallest
+        excess = (actual - value).abs() - allowed
+        assert bool((excess <= 0).all()), f"{int((~(excess <= 0)).sum())} beyond the bound"
