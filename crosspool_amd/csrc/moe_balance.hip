@@ -88,9 +88,10 @@ __device__ __forceinline__ void load_logits(const void *logits, int64_t row, int
 }
 
 // Scores of a row in place of its logits, not yet divided by their sum, and the sum's inverse (0 for
-// a row whose scores are all zero).
+// a row whose scores are all zero).  `slope` gets s of the gradient; 1 - sigmoid(l) is sigmoid(-l), which the
+// difference from a rounded sigmoid loses from l = 10 on (all of it from 17.4).
 template <int L, int CN>
-__device__ __forceinline__ float scores(float (&value)[CN][4], bool softmax) {
+__device__ __forceinline__ float scores(float (&value)[CN][4], bool softmax, float (&slope)[CN][4]) {
   float sum = 0.0f;
   if (softmax) {
     float most = kLowest;
@@ -108,6 +109,7 @@ __device__ __forceinline__ float scores(float (&value)[CN][4], bool softmax) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         value[c][j] = expf(value[c][j] - most);
+        slope[c][j] = 1.0f;
         sum += value[c][j];
       }
     }
@@ -116,7 +118,11 @@ __device__ __forceinline__ float scores(float (&value)[CN][4], bool softmax) {
     for (int c = 0; c < CN; ++c) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        value[c][j] = 1.0f / (1.0f + expf(-value[c][j]));
+        const float small = expf(-fabsf(value[c][j]));
+        const float whole = 1.0f / (1.0f + small);
+        const float part = small * whole;
+        slope[c][j] = value[c][j] > 0.0f ? part : whole;
+        value[c][j] = value[c][j] > 0.0f ? whole : part;
         sum += value[c][j];
       }
     }
@@ -211,7 +217,8 @@ __global__ __launch_bounds__(kBalanceThreads) void moe_balance_kernel(BalanceArg
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (row0 + u * stride < live) {
-          const float inverse = scores<L, CN>(value[u], a.softmax != 0);
+          float unused[CN][4];
+          const float inverse = scores<L, CN>(value[u], a.softmax != 0, unused);
 #pragma unroll
           for (int c = 0; c < CN; ++c) {
 #pragma unroll
@@ -332,7 +339,8 @@ __global__ __launch_bounds__(256) void moe_balance_backward_kernel(BalanceArgs a
         continue;
       }
       if (row < live) {
-        const float inverse = scores<L, CN>(value[u], a.softmax != 0);
+        float slope[CN][4];
+        const float inverse = scores<L, CN>(value[u], a.softmax != 0, slope);
         float mean = 0.0f;
 #pragma unroll
         for (int c = 0; c < CN; ++c) {
@@ -346,8 +354,7 @@ __global__ __launch_bounds__(256) void moe_balance_backward_kernel(BalanceArgs a
         for (int c = 0; c < CN; ++c) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float slope = a.softmax != 0 ? 1.0f : 1.0f - value[u][c][j];
-            const float grad = factor * (value[u][c][j] * inverse) * slope * (load[c][j] - mean);
+            const float grad = factor * (value[u][c][j] * inverse) * slope[c][j] * (load[c][j] - mean);
             value[u][c][j] = inverse == 0.0f ? 0.0f : grad;
           }
         }

@@ -272,3 +272,54 @@ def test_refusals_on_the_device(device):
     assert operator.workspace.numel() == 16
     big = BalanceLoss(row_capacity=4096, routed_expert_count=16, routed_topk=2)
     assert big.workspace.numel() == _native.library().xp_moe_balance_workspace_bytes(4096, 16) > 0
+
+
+def sigmoid_definition(logits, ids, topk, coefficient, upstream=1.0):
+    """(loss, gradient, its size) of the sigmoid scores in 64 bits for logits of any finite size: with m the row's
+    largest logit or 0, score_e = exp(min(l, 0) - m) / (1 + exp(-|l|)) keeps the ratios where sigmoids underflow."""
+
+    rows, experts = logits.shape
+    values = logits.double()
+    most = values.amax(dim=1, keepdim=True).clamp(max=0)
+    small = torch.exp(-values.abs())
+    score = torch.exp(values.clamp(max=0) - most) / (1 + small)
+    slope = torch.where(values > 0, small, 1.0) / (1 + small)
+    share = score / score.sum(dim=1, keepdim=True)
+    counts = torch.bincount(ids.flatten().long(), minlength=experts)
+    load = counts.double() * experts / (topk * rows)
+    loss = coefficient * float((load * share.sum(dim=0)).sum()) / rows
+    factor = coefficient * upstream / rows
+    mean = (share * load).sum(dim=1, keepdim=True)
+    return loss, factor * share * slope * (load - mean), abs(factor) * share * slope * (load + mean)
+
+
+def check_sigmoid(device, logits, ids, topk, spread):
+    """``spread``: the largest exponent that an exp of the case takes (the file's X)."""
+
+    rows, experts = logits.shape
+    operator = BalanceLoss(row_capacity=rows, routed_expert_count=experts, routed_topk=topk, coefficient=0.5,
+                           algorithm=RouterAlgorithm.SIGMOID)
+    grad = torch.full_like(logits.to(device), float("nan"))
+    upstream = torch.tensor([float(rows) * 16], device=device)
+    operator.run_into(logits=logits.to(device), ids=ids.to(device))
+    operator.backward_into(logits=logits.to(device), grad_logits=grad, grad_loss=upstream)
+    loss, expected, size = sigmoid_definition(logits, ids, topk, 0.5, float(rows) * 16)
+    assert abs(float(operator.loss) - loss) <= abs(loss) * (experts + rows + 2 * spread + 16) * UNIT
+    allowed = size * (2 * experts + 4 * spread + 32) * UNIT
+    allowed = allowed + rounding(expected.abs() + allowed, logits.dtype)
+    assert bool(((grad.cpu().double() - expected).abs() <= allowed).all())
+    return grad
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("experts", [8, 128, 300])
+def test_saturated_sigmoids_keep_their_slope(device, experts, dtype):
+    """Logits of 10 to 30: 1 - sigmoid is e^-l / (1 + e^-l), from 5e-5 to 1e-13 and not zero."""
+
+    g = torch.Generator().manual_seed(experts)
+    logits = (torch.rand((300, experts), generator=g) * 20 + 10).to(DTYPES[dtype])
+    ids = torch.topk(logits.float(), 2, dim=1).indices.to(torch.int32)
+    grad = check_sigmoid(device, logits, ids, 2, 30.0)
+    # Every share is 1 / experts within 2^-14: an expert of the average load, f = 1, is alone in having no gradient.
+    uneven = torch.bincount(ids.flatten().long(), minlength=experts) * experts != ids.numel()
+    assert bool((grad.cpu()[:, uneven] != 0).all())
