@@ -323,3 +323,22 @@ def test_saturated_sigmoids_keep_their_slope(device, experts, dtype):
     # Every share is 1 / experts within 2^-14: an expert of the average load, f = 1, is alone in having no gradient.
     uneven = torch.bincount(ids.flatten().long(), minlength=experts) * experts != ids.numel()
     assert bool((grad.cpu()[:, uneven] != 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("experts", [8, 64, 100, 300])
+@pytest.mark.parametrize("level", [-70.0, -95.0, -200.0, -30000.0])
+def test_rows_of_low_sigmoid_logits_keep_their_ratios(device, level, experts, dtype):
+    """A row of finite logits has a share for each of them, however low they all are."""
+
+    logits, ids = make(300, experts, 2, dtype, seed=experts)
+    logits[5:] = (logits[5:].float() + level).to(DTYPES[dtype])   # beside rows of ordinary ones
+    grad = check_sigmoid(device, logits, ids, 2, 40.0)
+    if dtype == "fp32":   # (in 16 bits the lowest levels round to ties)
+        assert bool((grad[5:].abs().amax(dim=1) > 0).all())
+
+
+def test_the_lowest_logits_share_alike(device):
+    logits = torch.full((300, 16), torch.finfo(torch.float32).min)
+    ids = torch.zeros((300, 1), dtype=torch.int32)
+    check_sigmoid(device, logits, ids, 1, 1.0)
