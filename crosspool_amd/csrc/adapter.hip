@@ -546,7 +546,7 @@ AdapterPlan plan_adapter(const AdapterShape &shape) {
   const int64_t rows = shape.rows;
   plan.rp = 16 * rank_tiles(shape.max_rank);
   const bool routed = shape.backward || rows > kAdapterDirectRows;
-  const int64_t tiles = (rows + kAdapterTileRows - 1) / kAdapterTileRows;
+  const int64_t tiles = std::max<int64_t>(1, (rows + kAdapterTileRows - 1) / kAdapterTileRows);
   const int64_t widths[2] = {shape.input_width, shape.output_width};
   int64_t at = 0;
   if (routed) {
@@ -592,9 +592,12 @@ AdapterPlan plan_adapter(const AdapterShape &shape) {
 }
 
 size_t adapter_workspace_bytes(const AdapterShape &shape) {
-  size_t most = plan_adapter(shape).bytes;
-  // The number of K ranges depends on the tiles alone, up to one range, and falls as they grow.
   AdapterShape smaller = shape;
+  if (shape.backward) {
+    smaller.rows = std::max<int64_t>(shape.rows, 1);  // no rows are planned as one
+  }
+  size_t most = plan_adapter(smaller).bytes;
+  // The number of K ranges depends on the tiles alone, up to one range, and falls as they grow.
   for (int64_t tiles = 1; tiles <= kShrinkWorkgroups && tiles * kAdapterTileRows < shape.rows; ++tiles) {
     smaller.rows = tiles * kAdapterTileRows;
     most = std::max(most, plan_adapter(smaller).bytes);

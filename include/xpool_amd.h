@@ -202,7 +202,8 @@ typedef struct {
 } xp_adapter_pool;
 
 /* Workspace bytes that xp_adapter_apply (or, with `backward`, xp_adapter_backward) needs for every
- * row count up to `rows`; 0 for sizes that they refuse.  The workspace is 16-byte aligned, its
+ * row count up to `rows`; 0 for sizes that they refuse and where nothing is needed (rows = 0 without
+ * `backward`).  The workspace is 16-byte aligned, its
  * contents do not matter on entry, and calls that may overlap in time must not share one. */
 size_t xp_adapter_workspace_bytes(int64_t rows, int64_t count, int64_t max_rank, int64_t input_width,
                                   int64_t output_width, int dtype, int backward);

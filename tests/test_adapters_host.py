@@ -181,3 +181,15 @@ def test_balance_refusals():
     sizes = [lib.xp_moe_balance_workspace_bytes(rows, 128) for rows in (0, 1, 256, 257, 1000, 5000, 100000)]
     assert sizes == sorted(sizes)
     assert lib.xp_moe_balance_workspace_bytes(10, 0) == lib.xp_moe_balance_workspace_bytes(-1, 8) == 0
+
+
+@pytest.mark.parametrize("k,n,rank,count", [(64, 48, 16, 4), (4096, 24576, 32, 32), (33, 5000, 3, 1024)])
+def test_the_workspace_of_no_rows(k, n, rank, count):
+    """Gradients of no rows are cleared, with the scratch of one row; the forward needs none."""
+
+    assert workspace(0, 0, count, rank, k, n) == 0
+    assert 0 < workspace(0, 1, count, rank, k, n) <= workspace(1, 1, count, rank, k, n)
+    asked = pool(a=0x100000000, b=0x200000000, count=count, max_rank=rank, input_width=k, output_width=n)
+    assert backward(asked, rows=0, ids=None, x=None, ldx=0, grad=None, ld_grad=0, base=None, gx=None, ga=0x300000000,
+                    gb=0x400000000, ws=0x500000000, ws_bytes=workspace(0, 1, count, rank, k, n) - 1) == BAD
+    assert "smaller" in _native.last_error()

@@ -10,6 +10,8 @@ subnormal of fp16.
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -737,3 +739,16 @@ def test_no_limit_hides_a_nan_of_the_sum(device, function, rows, dtype):
     keep = torch.ones_like(expected)
     keep[:4] = False
     assert torch.equal(got[keep], clean[keep])
+
+
+@pytest.mark.parametrize("count", [3, 70])
+def test_no_rows_with_the_scratch_asked_for_them(device, count):
+    case = Case(device, rows=0, k=300, n=520, count=count, max_rank=12)
+    nbytes = _native.library().xp_adapter_workspace_bytes(0, count, 12, 300, 520, _native.XP_DTYPE_BF16, 1)
+    scratch = torch.full((nbytes + 64,), 0xFF, dtype=torch.uint8, device=device)
+    weights = case.weights()
+    ga, gb = torch.full_like(weights.a, float("nan")), torch.full_like(weights.b, float("nan"))
+    _native.call("xp_adapter_backward", ctypes.byref(weights.descriptor), None, 0, None, 0, None, 0, None, 0, None, 0,
+                 ga.data_ptr(), gb.data_ptr(), scratch.data_ptr(), nbytes, None, torch.cuda.current_stream().cuda_stream)
+    assert not bool(ga.any()) and not bool(gb.any())
+    assert bool((scratch[nbytes:] == 0xFF).all())
