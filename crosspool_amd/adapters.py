@@ -16,7 +16,7 @@ be captured into a graph; replays read the ids, weights and rows that the tensor
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -35,19 +35,24 @@ def _require_pool(tensor: torch.Tensor, name: str, dtype: torch.dtype, shape: tu
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}")
 
 
+@dataclass(frozen=True, slots=True, eq=False)
 class AdapterWeights:
     """A pool of adapters of one projection: ``a`` ``[adapters, max_rank, K]``, ``b`` ``[adapters, N, max_rank]``.
 
     ``scales`` (fp32, default 1) holds every adapter's factor and ``ranks`` (int32, default
     ``max_rank``) its rank: what ``a`` and ``b`` hold past it is ignored, and a rank of 0 is an empty
-    slot.  The tensors are borrowed; a slot may be rewritten in place between calls.
+    slot.  The tensors are borrowed; a slot may be rewritten in place between calls, but a tensor whose
+    storage is exchanged needs a pool of its own.
     """
 
-    __slots__ = ("a", "b", "scales", "ranks", "descriptor")
+    a: torch.Tensor
+    b: torch.Tensor
+    scales: torch.Tensor | None = None
+    ranks: torch.Tensor | None = None
+    descriptor: _native.AdapterPool = field(init=False, repr=False)
 
-    def __init__(
-        self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor | None = None, ranks: torch.Tensor | None = None
-    ) -> None:
+    def __post_init__(self) -> None:
+        a, b = self.a, self.b
         if a.device.type != "cuda":
             raise ValueError("adapter weights must be GPU-resident")
         if a.dtype not in _DTYPE_CODES or a.ndim != 3 or b.ndim != 3 or not a.is_contiguous():
@@ -56,15 +61,24 @@ class AdapterWeights:
         if not 1 <= count <= MAX_ADAPTERS or not 1 <= max_rank <= MAX_RANK or input_width < 1 or b.shape[1] < 1:
             raise ValueError(f"an adapter pool holds 1 to {MAX_ADAPTERS} adapters of 1 to {MAX_RANK} ranks and positive widths")
         _require_pool(b, "adapter b", a.dtype, (count, b.shape[1], max_rank), a.device)
-        if scales is not None:
-            _require_pool(scales, "adapter scales", torch.float32, (count,), a.device)
-        if ranks is not None:
-            _require_pool(ranks, "adapter ranks", torch.int32, (count,), a.device)
-        self.a, self.b, self.scales, self.ranks = a, b, scales, ranks
-        self.descriptor = _native.AdapterPool(
-            a=a.data_ptr(), b=b.data_ptr(), ranks=None if ranks is None else ranks.data_ptr(),
-            scales=None if scales is None else scales.data_ptr(), count=count, max_rank=max_rank,
+        if self.scales is not None:
+            _require_pool(self.scales, "adapter scales", torch.float32, (count,), a.device)
+        if self.ranks is not None:
+            _require_pool(self.ranks, "adapter ranks", torch.int32, (count,), a.device)
+        object.__setattr__(self, "descriptor", _native.AdapterPool(
+            a=a.data_ptr(), b=b.data_ptr(), ranks=None if self.ranks is None else self.ranks.data_ptr(),
+            scales=None if self.scales is None else self.scales.data_ptr(), count=count, max_rank=max_rank,
             input_width=input_width, output_width=b.shape[1], dtype=_DTYPE_CODES[a.dtype],
+        ))
+
+    def keeps_storage(self) -> bool:
+        """Whether the tensors still are where the pool was made (``.data`` can be exchanged under them)."""
+
+        pool = self.descriptor
+        return (
+            self.a.data_ptr() == pool.a and self.b.data_ptr() == pool.b
+            and (self.scales is None or self.scales.data_ptr() == pool.scales)
+            and (self.ranks is None or self.ranks.data_ptr() == pool.ranks)
         )
 
 
@@ -156,6 +170,7 @@ class Adapter:
         self._scratch = self.scratch.data_ptr()
         self._scratch_bytes = self.scratch.numel()
         self._pool_shape = (plan.adapter_count, plan.max_rank, plan.input_width)
+        self._output_shape = (plan.adapter_count, plan.output_width, plan.max_rank)
 
     def _rows(self, tensor: torch.Tensor, name: str, rows: int, width: int) -> int:
         """The row stride of an operand (checked)."""
@@ -172,10 +187,12 @@ class Adapter:
         if rows > plan.row_capacity:
             raise ValueError(f"{rows} adapter rows exceed the prepared capacity {plan.row_capacity}")
         if (
-            weights.a.shape != self._pool_shape or weights.b.shape[1] != plan.output_width
+            weights.a.shape != self._pool_shape or weights.b.shape != self._output_shape
             or weights.a.dtype is not plan.dtype or weights.a.get_device() != self._index
         ):
             raise ValueError("adapter weights disagree with the prepared plan")
+        if not weights.keeps_storage():
+            raise ValueError("the storage of adapter weights was exchanged since their pool was made")
         if (
             adapter_ids.dtype is not torch.int32 or adapter_ids.shape != (rows,) or adapter_ids.get_device() != self._index
             or not adapter_ids.is_contiguous()
@@ -261,7 +278,7 @@ class Adapter:
             raise ValueError("grad_a and grad_b are asked for together")
         if grad_a is not None:
             _require_pool(grad_a, "grad_a", plan.dtype, self._pool_shape, self._device)
-            _require_pool(grad_b, "grad_b", plan.dtype, tuple(weights.b.shape), self._device)
+            _require_pool(grad_b, "grad_b", plan.dtype, self._output_shape, self._device)
         ldx = self._rows(inputs, "inputs", rows, plan.input_width)
         ld_grad = self._rows(grad_output, "output gradient", rows, plan.output_width)
         ld_base = ld_grad_inputs = 0

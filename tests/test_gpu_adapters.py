@@ -752,3 +752,31 @@ def test_no_rows_with_the_scratch_asked_for_them(device, count):
                  ga.data_ptr(), gb.data_ptr(), scratch.data_ptr(), nbytes, None, torch.cuda.current_stream().cuda_stream)
     assert not bool(ga.any()) and not bool(gb.any())
     assert bool((scratch[nbytes:] == 0xFF).all())
+
+
+def test_a_pool_keeps_the_tensors_that_it_was_made_of(device):
+    case = Case(device, rows=4, k=64, n=48, count=2, max_rank=8, ranks=[8, 4])
+    weights = case.weights()
+    for name in ("a", "b", "scales", "ranks", "descriptor"):
+        with pytest.raises(AttributeError):
+            setattr(weights, name, getattr(weights, name))
+    operator, ids = case.operator(backward=True), case.ids.to(device)
+    x, base = case.x.to(device), case.base.to(device)
+    out, gx = torch.empty_like(base), torch.empty_like(x)
+    # Storage that moved under a tensor (as a module's conversion moves its parameters).
+    for name in ("a", "b", "scales", "ranks"):
+        moved = case.weights()
+        tensor = getattr(moved, name)
+        kept = tensor.data
+        tensor.data = kept.clone()
+        with pytest.raises(ValueError, match="pool"):
+            operator.run_into(x, moved, adapter_ids=ids, base=base, output=out)
+        with pytest.raises(ValueError, match="pool"):
+            operator.backward_into(x, base, moved, adapter_ids=ids, grad_inputs=gx)
+        tensor.data = kept
+        operator.run_into(x, moved, adapter_ids=ids, base=base, output=out)
+    moved = case.weights()
+    moved.b.data = moved.b.data[:, :, :4]
+    with pytest.raises(ValueError, match="pool|plan"):
+        operator.run_into(x, moved, adapter_ids=ids, base=base, output=out)
+    check_forward(case, run(case))
