@@ -1691,31 +1691,51 @@ int xp_activation_backward(const void *inputs, const void *grad_output, void *gr
 
 namespace {
 
-// Elements [first, first + (rows - 1) ld + width) of two operands: whether their bytes overlap.
-bool rows_overlap(const void *p, int64_t ld_p, int64_t width_p, const void *q, int64_t ld_q, int64_t width_q,
-                  int64_t rows, size_t element) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-  const uintptr_t b = reinterpret_cast<uintptr_t>(q);
-  const uintptr_t a_end = a + static_cast<uintptr_t>((rows - 1) * ld_p + width_p) * element;
-  const uintptr_t b_end = b + static_cast<uintptr_t>((rows - 1) * ld_q + width_q) * element;
-  return a < b_end && b < a_end;
-}
-
-// A call's operand as a range of bytes.
+// A call's operand: `rows` runs of `width` bytes, `stride` bytes from one's begin to the next's.
 struct Span {
-  uintptr_t begin;
-  uintptr_t end;
+  int64_t begin;
+  int64_t stride;
+  int64_t width;
+  int64_t rows;
+  int64_t end() const { return begin + (rows - 1) * stride + width; }
 };
 Span span_of(const void *p, size_t bytes) {
-  const uintptr_t begin = reinterpret_cast<uintptr_t>(p);
-  return {begin, p == nullptr ? begin : begin + bytes};
+  const int64_t width = static_cast<int64_t>(bytes);
+  return {reinterpret_cast<intptr_t>(p), width, width, p == nullptr || bytes == 0 ? 0 : 1};
 }
 Span span_of_rows(const void *p, int64_t ld, int64_t width, int64_t rows, size_t element) {
-  return span_of(p, static_cast<size_t>((rows - 1) * ld + width) * element);
+  const int64_t bytes = static_cast<int64_t>(element);
+  return {reinterpret_cast<intptr_t>(p), ld * bytes, width * bytes, p == nullptr ? 0 : rows};
+}
+// Quotient rounded down.
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b != 0 && (a < 0) != (b < 0) ? 1 : 0); }
+
+// Whether two operands share a byte: not where the rows of one lie between those of the other, as columns of
+// one wider tensor do.
+bool overlaps(const Span &p, const Span &q) {
+  if (p.rows == 0 || q.rows == 0 || p.begin >= q.end() || q.begin >= p.end()) {
+    return false;
+  }
+  if (p.rows > 1 && q.rows > 1 && p.stride != q.stride) {
+    // Row by row of the operand of fewer rows; the ranges have to overlap for this to be reached.
+    const Span &few = p.rows <= q.rows ? p : q;
+    const Span &many = p.rows <= q.rows ? q : p;
+    for (int64_t row = 0; row < few.rows; ++row) {
+      if (overlaps({few.begin + row * few.stride, few.width, few.width, 1}, many)) {
+        return true;
+      }
+    }
+    return false;
+  }
+  // Row i of p and row j of q meet where -q.width < (q.begin - p.begin) + (j - i) stride < p.width.
+  const int64_t stride = p.rows > 1 ? p.stride : q.stride;
+  const int64_t distance = q.begin - p.begin;
+  const int64_t least = std::max(floor_div(-q.width - distance, stride) + 1, 1 - p.rows);
+  const int64_t most = std::min(-floor_div(distance - p.width, stride) - 1, q.rows - 1);
+  return least <= most;
 }
 bool touches(const Span &span, std::initializer_list<Span> others) {
-  return std::any_of(others.begin(), others.end(),
-                     [&](const Span &other) { return span.begin < other.end && other.begin < span.end; });
+  return std::any_of(others.begin(), others.end(), [&](const Span &other) { return overlaps(span, other); });
 }
 
 constexpr int64_t kAdapterMaxRows = int64_t{1} << 24;
@@ -1791,21 +1811,21 @@ int xp_adapter_apply(const xp_adapter_pool *pool, const int32_t *ids, int64_t ro
   if (const int status = adapter_rows("adapter output", out, ld_out, out_width, element); status != XP_OK) {
     return status;
   }
-  XP_REQUIRE(!rows_overlap(x, ldx, shape.input_width, out, ld_out, out_width, rows, element),
-             "the adapter output must not overlap its input");
+  const Span read_x = span_of_rows(x, ldx, shape.input_width, rows, element);
+  const Span read_base = span_of_rows(base, ld_base, shape.output_width, rows, element);
+  const Span write_out = span_of_rows(out, ld_out, out_width, rows, element);
+  XP_REQUIRE(!overlaps(read_x, write_out), "the adapter output must not overlap its input");
   const bool same = base == out && ld_base == ld_out && expand.act.function == kActivationNone;
-  XP_REQUIRE(base == nullptr || same ||
-                 !rows_overlap(base, ld_base, shape.output_width, out, ld_out, out_width, rows, element),
+  XP_REQUIRE(same || !overlaps(read_base, write_out),
              "the adapter output may be its base only whole and without an activation");
   const AdapterPlan plan = plan_adapter(shape);
   XP_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= plan.bytes,
              "adapter workspace is missing, unaligned or smaller than xp_adapter_workspace_bytes");
   const Span scratch = span_of(workspace, plan.bytes);
-  XP_REQUIRE(!touches(span_of_rows(out, ld_out, out_width, rows, element),
+  XP_REQUIRE(!touches(write_out,
                       {scratch, span_of(ids, static_cast<size_t>(rows) * 4), pool_span(*pool, pool->a, pool->input_width),
                        pool_span(*pool, pool->b, pool->output_width)}) &&
-                 !touches(scratch, {span_of_rows(x, ldx, shape.input_width, rows, element),
-                                    span_of_rows(base, ld_base, shape.output_width, rows, element)}),
+                 !touches(scratch, {read_x, read_base}),
              "the adapter output and workspace must not overlap the pool, the ids, the operands or each other");
   unsigned char *bytes = static_cast<unsigned char *>(workspace);
   const hipStream_t hip_stream = static_cast<hipStream_t>(stream);
@@ -1869,9 +1889,9 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
           status != XP_OK) {
         return status;
       }
-      XP_REQUIRE(!rows_overlap(x, ldx, shape.input_width, grad_x, ld_grad_x, shape.input_width, rows, element) &&
-                     !rows_overlap(grad_out, ld_grad_out, shape.output_width, grad_x, ld_grad_x, shape.input_width,
-                                   rows, element),
+      const Span write_x = span_of_rows(grad_x, ld_grad_x, shape.input_width, rows, element);
+      XP_REQUIRE(!touches(write_x, {span_of_rows(x, ldx, shape.input_width, rows, element),
+                                    span_of_rows(grad_out, ld_grad_out, shape.output_width, rows, element)}),
                  "the input gradient must not overlap the input or the output gradient");
       if (base != nullptr) {
         if (const int status = adapter_rows("base gradient", base, ld_base, shape.input_width, element);
@@ -1879,8 +1899,7 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
           return status;
         }
         XP_REQUIRE((base == grad_x && ld_base == ld_grad_x) ||
-                       !rows_overlap(base, ld_base, shape.input_width, grad_x, ld_grad_x, shape.input_width, rows,
-                                     element),
+                       !overlaps(write_x, span_of_rows(base, ld_base, shape.input_width, rows, element)),
                    "the input gradient may be its base only whole");
       }
     }
@@ -1895,14 +1914,13 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
   XP_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= plan.bytes,
              "adapter workspace is missing, unaligned or smaller than xp_adapter_workspace_bytes");
   {
-    const Span none = span_of(nullptr, 0);
     const auto rows_span = [&](const void *p, int64_t ld, int64_t width) {
-      return rows > 0 ? span_of_rows(p, ld, width, rows, element) : none;
+      return span_of_rows(p, ld, width, rows, element);
     };
     const Span scratch = span_of(workspace, plan.bytes);
     const Span read_x = rows_span(x, ldx, shape.input_width);
     const Span read_grad = rows_span(grad_out, ld_grad_out, shape.output_width);
-    const Span read_base = grad_x != nullptr ? rows_span(base, ld_base, shape.input_width) : none;
+    const Span read_base = rows_span(grad_x != nullptr ? base : nullptr, ld_base, shape.input_width);
     const Span read_ids = span_of(ids, static_cast<size_t>(rows) * 4);
     const Span pool_a = pool_span(*pool, pool->a, pool->input_width);
     const Span pool_b = pool_span(*pool, pool->b, pool->output_width);

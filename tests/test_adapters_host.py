@@ -4,6 +4,7 @@ sizes they ask for: no GPU needed."""
 from __future__ import annotations
 
 import ctypes
+import random
 
 import pytest
 import torch
@@ -193,3 +194,59 @@ def test_the_workspace_of_no_rows(k, n, rank, count):
     assert backward(asked, rows=0, ids=None, x=None, ldx=0, grad=None, ld_grad=0, base=None, gx=None, ga=0x300000000,
                     gb=0x400000000, ws=0x500000000, ws_bytes=workspace(0, 1, count, rank, k, n) - 1) == BAD
     assert "smaller" in _native.last_error()
+
+
+def refusal(call, k=72, n=104, **changes):
+    """What a call without a workspace is refused for: "workspace" where its rows are taken."""
+
+    assert call(pool(input_width=k, output_width=n), ws=None, **changes) == BAD
+    return next(word for word in ("workspace", "overlap", "whole") if word in _native.last_error())
+
+
+def test_rows_side_by_side_do_not_overlap():
+    """Columns of one tensor of 600 bf16 columns, at byte offsets of twice their first."""
+
+    base = 0x1000000
+    wide = dict(rows=300, x=base, ldx=600, base=base + 144, ld_base=600, out=base + 352, ld_out=600)
+    assert refusal(apply, **wide) == "workspace"
+    assert refusal(apply, **{**wide, "out": base + 350}) == "whole"            # the base's last column
+    assert refusal(apply, **{**wide, "out": base + 1200 - 206}) == "overlap"   # one column into the next rows of x
+    assert refusal(apply, **{**wide, "out": base + 1200 - 208}) == "workspace"
+    assert refusal(apply, **{**wide, "out": base - 206, "base": None}) == "overlap"
+    assert refusal(apply, **{**wide, "out": base - 208, "base": None}) == "workspace"
+    # Past the last row, and before the first, where no row of x follows or precedes.
+    last = base + 299 * 1200
+    assert refusal(apply, **{**wide, "out": last + 142, "base": None}) == "overlap"
+    assert refusal(apply, **{**wide, "out": last + 144, "base": None}) == "workspace"
+    assert refusal(apply, **{**wide, "out": base - 299 * 1200 - 206, "base": None}) == "overlap"
+    assert refusal(apply, **{**wide, "out": base - 299 * 1200 - 208, "base": None}) == "workspace"
+    # Every other row, and rows of another stride.
+    assert refusal(apply, **{**wide, "ldx": 1200, "out": base + 1200, "ld_out": 1200, "base": None}) == "workspace"
+    assert refusal(apply, **{**wide, "out": base + 1200, "ld_out": 1200, "base": None}) == "overlap"
+    assert refusal(apply, **{**wide, "out": base + 144, "ld_out": 1200, "base": None}) == "workspace"
+    # One row.
+    assert refusal(apply, **{**wide, "rows": 1, "out": base + 142, "base": None}) == "overlap"
+    assert refusal(apply, **{**wide, "rows": 1, "out": base + 144, "base": None}) == "workspace"
+    back = dict(rows=300, x=base, ldx=600, grad=base + 144, ld_grad=600, base=base + 352, ld_base=600, gx=base + 496,
+                ld_gx=600, ga=0x4000000, gb=0x5000000)
+    assert refusal(backward, **back) == "workspace"
+    assert refusal(backward, **{**back, "gx": base + 494}) == "whole"
+    assert refusal(backward, **{**back, "gx": base + 350, "base": None}) == "overlap"
+
+
+def test_rows_overlap_where_they_share_a_byte():
+    """Rows of any strides and places, against the bytes counted one by one."""
+
+    rng = random.Random(0)
+    found = []
+    for _ in range(3000):
+        k, n, rows = rng.randint(1, 5), rng.randint(1, 5), rng.randint(1, 6)
+        ldx = k + rng.choice((0, 1, rng.randint(0, 20)))
+        ld_out = n + rng.choice((0, rng.randint(0, 20))) if rng.random() < 0.4 else max(ldx, n)
+        start = 2 * rng.randint(-60, 60)
+        read = {i * ldx * 2 + byte for i in range(rows) for byte in range(2 * k)}
+        written = {start + i * ld_out * 2 + byte for i in range(rows) for byte in range(2 * n)}
+        found.append(bool(read & written))
+        reason = refusal(apply, k, n, rows=rows, x=0x10000, ldx=ldx, base=None, out=0x10000 + start, ld_out=ld_out)
+        assert reason == ("overlap" if found[-1] else "workspace"), (k, n, rows, ldx, ld_out, start)
+    assert 500 < sum(found) < 2500

@@ -780,3 +780,35 @@ def test_a_pool_keeps_the_tensors_that_it_was_made_of(device):
     with pytest.raises(ValueError, match="pool|plan"):
         operator.run_into(x, moved, adapter_ids=ids, base=base, output=out)
     check_forward(case, run(case))
+
+
+@pytest.mark.parametrize("rows", [5, 200])
+def test_operands_in_columns_of_one_tensor(device, rows):
+    """Rows of several operands side by side in one buffer share no byte."""
+
+    case = Case(device, rows=rows, k=72, n=104, count=3, max_rank=8, seed=rows)
+    expected, gradients = run(case), backward(case)
+    wide = torch.zeros((rows, 600), dtype=case.dtype, device=device)
+    places = {"x": (0, 72), "base": (72, 176), "out": (176, 280), "grad": (281, 385), "grad_base": (385, 457),
+              "grad_x": (457, 529)}
+    views = {name: wide[:, begin:end] for name, (begin, end) in places.items()}
+    for name, source in (("x", case.x), ("base", case.base), ("grad", case.grad), ("grad_base", case.grad_base)):
+        views[name].copy_(source)
+    operator, weights, ids = case.operator(backward=True), case.weights(), case.ids.to(device)
+    operator.run_into(views["x"], weights, adapter_ids=ids, base=views["base"], output=views["out"])
+    assert torch.equal(views["out"], expected)
+    ga, gb = torch.empty_like(gradients["a"]), torch.empty_like(gradients["b"])
+    operator.backward_into(views["x"], views["grad"], weights, adapter_ids=ids, base=views["grad_base"],
+                           grad_inputs=views["grad_x"], grad_a=ga, grad_b=gb)
+    assert torch.equal(views["grad_x"], gradients["x"])
+    assert torch.equal(ga, gradients["a"]) and torch.equal(gb, gradients["b"])
+    assert not bool(wide[:, 280].any()) and not bool(wide[:, 529:].any())
+    for name, source in (("x", case.x), ("base", case.base), ("grad", case.grad), ("grad_base", case.grad_base)):
+        assert torch.equal(views[name].cpu(), source)
+    # One column in common, or rows of one operand among those of another.
+    with pytest.raises(_native.NativeError, match="overlap"):
+        operator.run_into(views["x"], weights, adapter_ids=ids, base=None, output=wide[:, 71:175])
+    tall = torch.zeros((2 * rows, 104), dtype=case.dtype, device=device)
+    operator.run_into(tall[0::2, :72], weights, adapter_ids=ids, base=None, output=tall[1::2])
+    with pytest.raises(_native.NativeError, match="overlap"):
+        operator.run_into(tall[0::2, :72], weights, adapter_ids=ids, base=None, output=tall[:rows])
