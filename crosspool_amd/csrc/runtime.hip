@@ -1765,6 +1765,15 @@ int adapter_shape(const xp_adapter_pool *pool, const int32_t *ids, int64_t rows,
 Span pool_span(const xp_adapter_pool &pool, const void *weights, int64_t width) {
   return span_of(weights, static_cast<size_t>(pool.count * pool.max_rank * width) * dtype_bytes(pool.dtype));
 }
+// All that the kernels read of a pool.
+struct PoolSpans {
+  Span a, b, ranks, scales;
+};
+PoolSpans pool_spans(const xp_adapter_pool &pool) {
+  const size_t table = static_cast<size_t>(pool.count) * 4;
+  return {pool_span(pool, pool.a, pool.input_width), pool_span(pool, pool.b, pool.output_width),
+          span_of(pool.ranks, table), span_of(pool.scales, table)};
+}
 
 int adapter_rows(const char *name, const void *rows_pointer, int64_t ld, int64_t width, size_t element) {
   XP_REQUIRE(rows_pointer != nullptr && aligned_to(rows_pointer, element),
@@ -1822,11 +1831,13 @@ int xp_adapter_apply(const xp_adapter_pool *pool, const int32_t *ids, int64_t ro
   XP_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= plan.bytes,
              "adapter workspace is missing, unaligned or smaller than xp_adapter_workspace_bytes");
   const Span scratch = span_of(workspace, plan.bytes);
-  XP_REQUIRE(!touches(write_out,
-                      {scratch, span_of(ids, static_cast<size_t>(rows) * 4), pool_span(*pool, pool->a, pool->input_width),
-                       pool_span(*pool, pool->b, pool->output_width)}) &&
-                 !touches(scratch, {read_x, read_base}),
-             "the adapter output and workspace must not overlap the pool, the ids, the operands or each other");
+  const PoolSpans reads = pool_spans(*pool);
+  const Span read_ids = span_of(ids, static_cast<size_t>(rows) * 4);
+  const Span fault = span_of(fault_word, sizeof(uint32_t));
+  XP_REQUIRE(!touches(write_out, {read_ids, reads.a, reads.b, reads.ranks, reads.scales, scratch, fault}) &&
+                 !touches(scratch, {read_x, read_base, read_ids, reads.a, reads.b, reads.ranks, reads.scales, fault}) &&
+                 !touches(fault, {read_x, read_base, read_ids, reads.a, reads.b, reads.ranks, reads.scales}),
+             "the adapter output, workspace and fault word must not overlap the pool, the ids, the operands or each other");
   unsigned char *bytes = static_cast<unsigned char *>(workspace);
   const hipStream_t hip_stream = static_cast<hipStream_t>(stream);
   const AdapterBatch batch = adapter_batch(shape, plan, ids, bytes);
@@ -1922,16 +1933,21 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
     const Span read_grad = rows_span(grad_out, ld_grad_out, shape.output_width);
     const Span read_base = rows_span(grad_x != nullptr ? base : nullptr, ld_base, shape.input_width);
     const Span read_ids = span_of(ids, static_cast<size_t>(rows) * 4);
-    const Span pool_a = pool_span(*pool, pool->a, pool->input_width);
-    const Span pool_b = pool_span(*pool, pool->b, pool->output_width);
+    const PoolSpans reads = pool_spans(*pool);
     const Span write_x = rows_span(grad_x, ld_grad_x, shape.input_width);
     const Span write_a = pool_span(*pool, grad_a, pool->input_width);
     const Span write_b = pool_span(*pool, grad_b, pool->output_width);
-    XP_REQUIRE(!touches(write_a, {read_x, read_grad, read_base, read_ids, pool_a, pool_b, write_x, write_b, scratch}) &&
-                   !touches(write_b, {read_x, read_grad, read_base, read_ids, pool_a, pool_b, write_x, scratch}) &&
-                   !touches(write_x, {read_ids, pool_a, pool_b, scratch}) &&
-                   !touches(scratch, {read_x, read_grad, read_base}),
-               "adapter gradients and the workspace must not overlap the pool, the ids, the operands or each other");
+    const Span fault = span_of(fault_word, sizeof(uint32_t));
+    const auto apart = [&](const Span &written, std::initializer_list<Span> also) {
+      return !touches(written, {read_ids, reads.a, reads.b, reads.ranks, reads.scales}) && !touches(written, also);
+    };
+    XP_REQUIRE(apart(write_a, {read_x, read_grad, read_base, write_x, write_b, scratch, fault}) &&
+                   apart(write_b, {read_x, read_grad, read_base, write_x, scratch, fault}) &&
+                   apart(write_x, {scratch, fault}) &&  // against the operands: above
+                   apart(scratch, {read_x, read_grad, read_base, fault}) &&
+                   apart(fault, {read_x, read_grad, read_base}),
+               "adapter gradients, the workspace and the fault word must not overlap the pool, the ids, the operands or "
+               "each other");
   }
   unsigned char *bytes = static_cast<unsigned char *>(workspace);
   const AdapterBatch batch = adapter_batch(shape, plan, ids, bytes);
@@ -2814,6 +2830,16 @@ int xp_moe_balance_loss(const void *logits, int logits_dtype, const int32_t *ids
   XP_REQUIRE(args.blocks == 1 || (workspace != nullptr && aligned16(workspace) &&
                                   workspace_bytes >= xp_moe_balance_workspace_bytes(rows, experts)),
              "balance workspace is missing, unaligned or smaller than xp_moe_balance_workspace_bytes");
+  const Span read_logits = span_of(logits, static_cast<size_t>(rows * experts) * dtype_bytes(logits_dtype));
+  const Span read_ids = span_of(ids, static_cast<size_t>(rows * topk) * 4);
+  const Span read_live = span_of(payload_rows, 4);
+  const Span write_counts = span_of(counts, static_cast<size_t>(experts) * 4);
+  const Span write_loss = span_of(loss, 4);
+  const Span scratch = span_of(workspace, args.blocks > 1 ? xp_moe_balance_workspace_bytes(rows, experts) : 0);
+  XP_REQUIRE(!touches(write_counts, {read_logits, read_ids, read_live, write_loss, scratch}) &&
+                 !touches(write_loss, {read_logits, read_ids, read_live, scratch}) &&
+                 !touches(scratch, {read_logits, read_ids, read_live}),
+             "the balance counts, loss and workspace must not overlap the operands or each other");
   args.ids = ids;
   args.counts = counts;
   args.loss = loss;

@@ -250,3 +250,46 @@ def test_rows_overlap_where_they_share_a_byte():
         reason = refusal(apply, k, n, rows=rows, x=0x10000, ldx=ldx, base=None, out=0x10000 + start, ld_out=ld_out)
         assert reason == ("overlap" if found[-1] else "workspace"), (k, n, rows, ldx, ld_out, start)
     assert 500 < sum(found) < 2500
+
+
+def test_nothing_written_may_overlap_the_pools_tables_or_the_workspace():
+    """The workspace over the pool or the ids, anything over ranks and scales, and the fault word over anything."""
+
+    tables = dict(a=0x100000000, b=0x200000000, ranks=0x300000000, scales=0x400000000)
+    size = workspace(8)
+    for at in (0x100000000, 0x200000000, 0x300000000, 0x400000000, P):
+        for shift in (0, 0x10 - size // 16 * 16):   # its first bytes over the table, or its last
+            assert apply(pool(**tables), ws=at + shift) == BAD and "overlap" in _native.last_error(), (at, shift)
+            assert backward(pool(**tables), ws=at + shift) == BAD and "overlap" in _native.last_error(), (at, shift)
+    for at in (0x300000000, 0x300000008, 0x400000000, 0x40000000c):
+        assert apply(pool(**tables), out=at) == BAD and "overlap" in _native.last_error()
+        for name in ("gx", "ga", "gb"):
+            assert backward(pool(**tables), **{name: at}) == BAD and "overlap" in _native.last_error(), name
+
+    def with_fault(call, word):
+        descriptor = _native.AdapterPool(**dict(count=4, max_rank=16, input_width=64, output_width=48,
+                                                dtype=_native.XP_DTYPE_BF16, **tables))
+        function = "xp_adapter_apply" if call is apply else "xp_adapter_backward"
+        given = ([P, 8, 0x10000, 64, 0x20000, 48, 0x30000, 48, None, 0x40000] if call is apply
+                 else [P, 8, 0x10000, 64, 0x20000, 48, 0x30000, 64, 0x50000, 64, 0x60000, 0x70000, 0x80000])
+        return getattr(_native.library(), function)(ctypes.byref(descriptor), *given, 1 << 30, word, None)
+
+    for word in (P, 0x10000, 0x20004, 0x30000, 0x40000, *tables.values()):
+        assert with_fault(apply, word) == BAD and "overlap" in _native.last_error(), hex(word)
+    for word in (P + 4, 0x10000, 0x20004, 0x30000, 0x50000, 0x60000, 0x70000, 0x80000, *tables.values()):
+        assert with_fault(backward, word) == BAD and "overlap" in _native.last_error(), hex(word)
+
+
+def test_nothing_of_the_balance_loss_may_overlap():
+    lib = _native.library()
+    good = dict(logits=0x1000000, dtype=_native.XP_DTYPE_F32, ids=0x2000000, rows=1000, experts=16, topk=2, algorithm=1,
+                live=0x3000000, coefficient=1.0, counts=0x4000000, loss=0x5000000, ws=0x6000000, ws_bytes=1 << 30)
+    for changes in (
+        dict(ws=0x1000000), dict(ws=0x1000000 + 63984), dict(ws=0x2000000), dict(ws=0x3000000), dict(ws=0x4000000),
+        dict(ws=0x5000000), dict(counts=0x1000000), dict(counts=0x2000000 + 7996), dict(counts=0x3000000 - 60),
+        dict(counts=0x5000000 - 4), dict(loss=0x1000000 + 63996), dict(loss=0x2000000), dict(loss=0x3000000),
+        dict(loss=0x4000000 + 60), dict(rows=10, ws=None, ws_bytes=0, counts=0x2000000),
+        dict(logits=None, loss=None, counts=0x2000000),
+    ):
+        assert lib.xp_moe_balance_loss(*{**good, **changes}.values(), None) == BAD, changes
+        assert "overlap" in _native.last_error(), changes
