@@ -1749,8 +1749,10 @@ bool adapter_shape_valid(const AdapterShape &shape) {
 }
 
 // The checks that both adapter entry points share; the shape of the call.
-int adapter_shape(const xp_adapter_pool *pool, const int32_t *ids, int64_t rows, bool backward, AdapterShape &shape) {
+int adapter_shape(const xp_adapter_pool *pool, const int32_t *ids, int64_t rows, bool backward, const uint32_t *fault_word,
+                  AdapterShape &shape) {
   XP_REQUIRE(pool != nullptr, "the adapter pool must be non-null");
+  XP_REQUIRE(aligned_to(fault_word, 4), "the adapter fault word must be 4-byte aligned");
   shape = AdapterShape{rows, pool->count, pool->max_rank, pool->input_width, pool->output_width, pool->dtype, backward};
   XP_REQUIRE(adapter_shape_valid(shape),
              "adapters: 1 to 1024 of 1 to 128 ranks, widths of 1 to 4194304, at most 16777216 rows, bf16, fp16 or fp32");
@@ -1795,7 +1797,7 @@ int xp_adapter_apply(const xp_adapter_pool *pool, const int32_t *ids, int64_t ro
                      const xp_activation_desc *activation, void *workspace, size_t workspace_bytes,
                      uint32_t *fault_word, xp_stream_t stream) {
   AdapterShape shape{};
-  if (const int status = adapter_shape(pool, ids, rows, false, shape); status != XP_OK) {
+  if (const int status = adapter_shape(pool, ids, rows, false, fault_word, shape); status != XP_OK) {
     return status;
   }
   AdapterExpandArgs expand{};
@@ -1879,7 +1881,7 @@ int xp_adapter_backward(const xp_adapter_pool *pool, const int32_t *ids, int64_t
                         int64_t ld_grad_x, void *grad_a, void *grad_b, void *workspace, size_t workspace_bytes,
                         uint32_t *fault_word, xp_stream_t stream) {
   AdapterShape shape{};
-  if (const int status = adapter_shape(pool, ids, rows, true, shape); status != XP_OK) {
+  if (const int status = adapter_shape(pool, ids, rows, true, fault_word, shape); status != XP_OK) {
     return status;
   }
   const size_t element = dtype_bytes(shape.dtype);

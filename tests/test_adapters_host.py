@@ -293,3 +293,12 @@ def test_nothing_of_the_balance_loss_may_overlap():
     ):
         assert lib.xp_moe_balance_loss(*{**good, **changes}.values(), None) == BAD, changes
         assert "overlap" in _native.last_error(), changes
+
+
+def test_the_fault_words_alignment():
+    lib, far = _native.library(), pool(a=0x1000000, b=0x2000000)
+    assert lib.xp_adapter_apply(far, P, 8, 0x10000, 64, 0x20000, 48, 0x30000, 48, None, 0x40000, 1 << 30, 0x3000002, None) == BAD
+    assert "aligned" in _native.last_error()
+    assert lib.xp_adapter_backward(far, P, 8, 0x10000, 64, 0x20000, 48, None, 0, 0x50000, 64, None, None, 0x80000, 1 << 30,
+                                   0x3000001, None) == BAD
+    assert "aligned" in _native.last_error()
