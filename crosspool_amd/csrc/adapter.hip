@@ -13,10 +13,12 @@ constexpr int kRouteThreads = 1024;
 constexpr int kRouteWaves = kRouteThreads / kWave;
 constexpr int kRouteGroups = kAdapterMaxCount + 2;
 
-// Rows, tiles, runs and slots of partial sums of some groups, added up.
+// Rows, tiles, runs and, in one value, slots of partial sums (at most 2^17) and adapters with rows of some
+// groups, added up.
 struct RouteSums {
   int value[4];
 };
+constexpr int kRouteAdapter = 1 << 20;
 
 __device__ __forceinline__ RouteSums wave_inclusive_scan(RouteSums sums) {
   const int lane = threadIdx.x & 63;
@@ -46,6 +48,7 @@ struct RouteLds {
   int tile_starts[kRouteGroups + 1];
   int run_starts[kRouteGroups + 1];
   int slot_starts[kRouteGroups];
+  int transposes[kRouteGroups];
   RouteSums wave_sums[kRouteWaves];
 };
 
@@ -136,7 +139,8 @@ __device__ __forceinline__ void route_rows(const AdapterRouteArgs &a, RouteLds &
         }
         const bool runs = group < count && batch.run_rows > 0;
         const int pieces = runs ? (length + batch.run_rows - 1) / batch.run_rows : 0;
-        mine[i] = {{length, (length + kAdapterTileRows - 1) / kAdapterTileRows, pieces, pieces > 1 ? pieces : 0}};
+        mine[i] = {{length, (length + kAdapterTileRows - 1) / kAdapterTileRows, pieces,
+                    (pieces > 1 ? pieces : 0) + (length > 0 ? kRouteAdapter : 0)}};
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           both.value[v] += mine[i].value[v];
@@ -175,12 +179,17 @@ __device__ __forceinline__ void route_rows(const AdapterRouteArgs &a, RouteLds &
         starts[group] = before.value[0];
         tile_starts[group] = before.value[1];
         run_starts[group] = before.value[2];
-        slot_starts[group] = mine[i].value[2] > 1 ? before.value[3] : -1;
+        const int first_slot = before.value[3] % kRouteAdapter;
+        slot_starts[group] = mine[i].value[2] > 1 ? first_slot : -1;
+        lds.transposes[group] = batch.transposes != nullptr ? before.value[3] / kRouteAdapter : group;
         if (group <= count) {
           batch.starts[group] = before.value[0];
         }
+        if (group < count && batch.transposes != nullptr) {
+          batch.transposes[group] = lds.transposes[group];
+        }
         if (group < count && batch.run_rows > 0) {
-          batch.run_slots[2 * group] = before.value[3];
+          batch.run_slots[2 * group] = first_slot;
           batch.run_slots[2 * group + 1] = mine[i].value[2];
         }
 #pragma unroll
@@ -250,7 +259,7 @@ __device__ __forceinline__ void route_rows(const AdapterRouteArgs &a, RouteLds &
     entry[0] = group;
     entry[1] = begin;
     entry[2] = left < kAdapterTileRows ? left : kAdapterTileRows;
-    entry[3] = group < count ? adapter_rank_of(a.ranks, group, a.max_rank) : 0;
+    entry[3] = group < count ? adapter_rank_of(a.ranks, group, a.max_rank) + 256 * lds.transposes[group] : 0;
   }
   for (int run = tid; run < batch.max_runs; run += kRouteThreads) {
     int *entry = batch.runs + 8 * run;
@@ -275,7 +284,9 @@ __global__ __launch_bounds__(kRouteThreads) void adapter_route_kernel(AdapterRou
 
 // ------------------------------------------------------------------ transposes
 // at[a][k][r] = A_a[r][k] and bt[a][r][n] = B_a[n][r] for the adapters that have rows: 64 columns of
-// A (rows of B) per workgroup through LDS.  Ranks past the adapter's are left unwritten.
+// A (rows of B) per workgroup through LDS.  Ranks past the adapter's are left unwritten.  Pools of more
+// than kTransposeGroups adapters have places for those with rows only (a batch of one row would ask for
+// gigabytes beside a large pool), in the pool's order.
 template <class E>
 struct TransposeLds {
   E tile[kAdapterMaxRank][64 + 1];
@@ -309,9 +320,10 @@ __device__ __forceinline__ void transpose_columns(const AdapterTransposeArgs &a,
         continue;
       }
     }
+    const int64_t place = SORTED && a.batch.transposes != nullptr ? a.batch.transposes[group] : group;
     if (second) {
       const E *source = static_cast<const E *>(a.b) + (group * a.n + c0) * a.max_rank;
-      E *target = static_cast<E *>(a.bt) + static_cast<int64_t>(group) * a.rp * a.n + c0;
+      E *target = static_cast<E *>(a.bt) + place * a.rp * a.n + c0;
       for (int index = threadIdx.x; index < columns * rank; index += kRouteThreads) {
         const int column = index / rank;
         const int r = index - column * rank;
@@ -326,7 +338,7 @@ __device__ __forceinline__ void transpose_columns(const AdapterTransposeArgs &a,
       }
     } else {
       const E *source = static_cast<const E *>(a.a) + static_cast<int64_t>(group) * a.max_rank * a.k + c0;
-      E *target = static_cast<E *>(a.at) + (group * a.k + c0) * a.rp;
+      E *target = static_cast<E *>(a.at) + (place * a.k + c0) * a.rp;
       for (int index = threadIdx.x; index < 64 * rank; index += kRouteThreads) {
         const int column = index & 63;
         if (column < columns) {
@@ -538,6 +550,9 @@ dim3 transpose_grid(const AdapterTransposeArgs &a) {
   return dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min(a.batch.count, kTransposeGroups)), 1);
 }
 
+// Whether transposes have places for the adapters with rows only.
+bool transposes_compact(const AdapterShape &shape) { return shape.backward && shape.count > kTransposeGroups; }
+
 }  // namespace
 
 AdapterPlan plan_adapter(const AdapterShape &shape) {
@@ -561,7 +576,7 @@ AdapterPlan plan_adapter(const AdapterShape &shape) {
       plan.max_runs = std::min(rows / kMinRunRows, wanted) + std::min(rows, shape.count);
       // An adapter of several runs has more than run_rows rows.
       plan.run_slots = std::min(2 * rows / kMinRunRows, 2 * wanted);
-      ints += 8 * plan.max_runs + 2 * shape.count;
+      ints += 8 * plan.max_runs + 2 * shape.count + (transposes_compact(shape) ? shape.count : 0);
     }
     at = align16(ints * 4);
   }
@@ -582,10 +597,11 @@ AdapterPlan plan_adapter(const AdapterShape &shape) {
       plan.sums[p] = static_cast<size_t>(at);
       at += align16(plan.run_slots * plan.rp * widths[p] * 4);
     }
+    const int64_t transposes = transposes_compact(shape) ? std::min(rows, shape.count) : shape.count;
     plan.at = static_cast<size_t>(at);
-    at += align16(shape.count * shape.input_width * plan.rp * element);
+    at += align16(transposes * shape.input_width * plan.rp * element);
     plan.bt = static_cast<size_t>(at);
-    at += align16(shape.count * shape.output_width * plan.rp * element);
+    at += align16(transposes * shape.output_width * plan.rp * element);
   }
   plan.bytes = static_cast<size_t>(at);
   return plan;
@@ -617,6 +633,7 @@ AdapterBatch adapter_batch(const AdapterShape &shape, const AdapterPlan &plan, c
     batch.run_slots = batch.runs + 8 * plan.max_runs;
     batch.starts = batch.run_slots + (plan.run_rows > 0 ? 2 * shape.count : 0);
     batch.perm = batch.starts + shape.count + 1;
+    batch.transposes = transposes_compact(shape) ? batch.perm + shape.rows : nullptr;
     batch.max_tiles = static_cast<int32_t>(plan.max_tiles);
     batch.max_runs = static_cast<int32_t>(plan.max_runs);
     batch.run_rows = static_cast<int32_t>(plan.run_rows);

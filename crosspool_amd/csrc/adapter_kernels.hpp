@@ -59,6 +59,7 @@ struct AdapterTile {
   int group;  // the adapter; count: rows without one; count + 1: rows whose id is out of range; -1: no tile
   int rows;
   int rank;   // 0 without an adapter
+  int place;  // of its weights: the adapter, or in a backward pass its transposes' place
   int row;    // lane i: the tile's row i (past the tile: any row of the batch)
 };
 
@@ -80,7 +81,7 @@ __device__ __forceinline__ int adapter_rank(const int32_t *ranks, int group, int
 __device__ __forceinline__ AdapterTile adapter_tile(const AdapterBatch &batch, const int32_t *ranks, int max_rank,
                                                     int64_t slot, bool all) {
   const int lane = lane_here();
-  AdapterTile tile{-1, 0, 0, 0};
+  AdapterTile tile{-1, 0, 0, 0, 0};
   if (batch.tiles == nullptr) {
     // One slot per row: the first row of each adapter leads its tile.
     if (slot >= batch.rows) {
@@ -94,6 +95,7 @@ __device__ __forceinline__ AdapterTile adapter_tile(const AdapterBatch &batch, c
       return tile;
     }
     tile.group = mine;
+    tile.place = mine;
     tile.rows = __popcll(mask);
     tile.rank = mine < batch.count ? adapter_rank(ranks, mine, max_rank) : 0;
     // Every row of the tile sends its number to the lane of its place, the others to the last lanes.
@@ -114,7 +116,9 @@ __device__ __forceinline__ AdapterTile adapter_tile(const AdapterBatch &batch, c
     const int first = __builtin_amdgcn_readfirstlane(static_cast<int>(entry[1]));
     tile.group = group;
     tile.rows = __builtin_amdgcn_readfirstlane(static_cast<int>(entry[2]));
-    tile.rank = __builtin_amdgcn_readfirstlane(static_cast<int>(entry[3]));
+    const int rank_and_place = __builtin_amdgcn_readfirstlane(static_cast<int>(entry[3]));
+    tile.rank = rank_and_place % 256;
+    tile.place = rank_and_place / 256;
     tile.row = batch.perm[first + (lane < tile.rows ? lane : 0)];
   }
   return tile;
@@ -186,7 +190,7 @@ constexpr int kShrinkRegion = (4 + RT) * 1024;  // bytes of LDS per wave
 
 template <class P, int NRT, int TT, int U, int REGION>
 __device__ __forceinline__ void shrink_body(const AdapterShrinkArgs &a, const AdapterShrinkJob &job, int64_t range,
-                                            const AdapterTile &tile, unsigned char *lds) {
+                                            const AdapterTile &tile, int place, unsigned char *lds) {
   constexpr int ES = kElementBytes<P>;
   constexpr int STEP = kStep<P>;
   const int64_t k = made_here(job.k);
@@ -199,7 +203,7 @@ __device__ __forceinline__ void shrink_body(const AdapterShrinkArgs &a, const Ad
   const int get = (lane & 15) * 64 + (((lane >> 4) ^ (lane >> 2 & 3)) << 4);
   // Rows past the tile read another, ranks past the adapter's the first: their sums go nowhere.
   const unsigned char *x[TT];
-  const unsigned char *w = static_cast<const unsigned char *>(job.w) + static_cast<int64_t>(tile.group) * job.w_rows * k * ES;
+  const unsigned char *w = static_cast<const unsigned char *>(job.w) + static_cast<int64_t>(place) * job.w_rows * k * ES;
   uint32_t w_offset[NRT];
 #pragma unroll
   for (int t = 0; t < TT; ++t) {
@@ -341,17 +345,17 @@ __device__ __forceinline__ void shrink_body(const AdapterShrinkArgs &a, const Ad
 
 template <class P, int RT, int TT, int REGION>
 __device__ __forceinline__ void shrink_ranks(const AdapterShrinkArgs &a, const AdapterShrinkJob &job, int64_t range,
-                                             const AdapterTile &tile, unsigned char *lds) {
+                                             const AdapterTile &tile, int place, unsigned char *lds) {
   if constexpr (RT > 1) {
     if (tile.rank <= 8 * RT) {
-      return shrink_ranks<P, RT / 2, TT, REGION>(a, job, range, tile, lds);
+      return shrink_ranks<P, RT / 2, TT, REGION>(a, job, range, tile, place, lds);
     }
   }
   // U steps of TT row and RT weight operands, 16 bytes per lane each, beside the sums: within the 128
   // registers of two workgroups a CU up to two rank tiles, the 256 of one above.  Not of TT: a row's sums
   // have one order however many rows share its adapter (four steps of one operand each would save 0.2 us).
   constexpr int U = RT <= 4 ? 2 : 1;
-  shrink_body<P, RT, TT, U, REGION>(a, job, range, tile, lds);
+  shrink_body<P, RT, TT, U, REGION>(a, job, range, tile, place, lds);
 }
 
 template <class P, int RT>
@@ -371,10 +375,11 @@ __global__ __launch_bounds__(kAdapterShrinkWaves *kWave, RT <= 2 ? 4 : 2) void a
       return;
     }
     if (tile.rank > 0) {
+      const int place = second ? tile.group : tile.place;  // the second job's weights are the pool's own
       if (tile.rows <= 16) {
-        shrink_ranks<P, RT, 1, kShrinkRegion<RT>>(a, job, range, tile, lds);
+        shrink_ranks<P, RT, 1, kShrinkRegion<RT>>(a, job, range, tile, place, lds);
       } else {
-        shrink_ranks<P, RT, 4, kShrinkRegion<RT>>(a, job, range, tile, lds);
+        shrink_ranks<P, RT, 4, kShrinkRegion<RT>>(a, job, range, tile, place, lds);
       }
     }
   }
@@ -501,7 +506,7 @@ __device__ __forceinline__ void expand_columns(const AdapterExpandArgs &a, const
                                                const unsigned char *terms, float scale, int64_t first) {
   const bool gated = ACT == AdapterAct::GatedSilu || (ACT == AdapterAct::Any && a.act.gated != 0);
   const int columns = static_cast<int>(a.n - first) / (gated ? 2 : 1);
-  const int64_t weights = static_cast<int64_t>(tile.group) * a.n * a.ld_w;
+  const int64_t weights = static_cast<int64_t>(tile.place) * a.n * a.ld_w;
   for (int start = 0; start < tile.rows * columns; start += kAdapterExpandWaves * kWave) {
     const int index = start + static_cast<int>(threadIdx.x);
     const int at = index / columns;
@@ -578,7 +583,7 @@ struct AdapterExpand {
   __device__ __forceinline__ AdapterExpand(const AdapterExpandArgs &args, int64_t whole_columns, const AdapterTile &tile,
                                            int first)
       : a(args),
-        w(static_cast<const unsigned char *>(args.w) + static_cast<int64_t>(tile.group) * args.n * args.ld_w * ES),
+        w(static_cast<const unsigned char *>(args.w) + static_cast<int64_t>(tile.place) * args.n * args.ld_w * ES),
         whole(whole_columns),
         rank(tile.rank),
         lane16(lane_here() & 15),

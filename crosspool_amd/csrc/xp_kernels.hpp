@@ -392,9 +392,10 @@ struct AdapterBatch {
   const int32_t *ids;     // [rows]
   int32_t *starts;        // [count + 1] first position of every adapter's rows and of the rest
   int32_t *perm;          // [rows]
-  int32_t *tiles;         // [max_tiles] group (-1: no tile), first position, rows, rank
+  int32_t *tiles;         // [max_tiles] group (-1: no tile), first position, rows, rank + 256 place of its weights
   int32_t *runs;          // [max_runs][8] group (-1: no run), first position, end, slot of partial sums (-1: none), tile
   int32_t *run_slots;     // [count] first slot and number of runs of every adapter
+  int32_t *transposes;    // [count] place of every adapter's transposed weights, or null: its number
   int64_t rows;
   int32_t max_tiles;
   int32_t max_runs;
@@ -451,7 +452,7 @@ struct AdapterExpandArgs {
   ActivationArgs act;
 };
 
-// Per-adapter transposes of the weights in use: at [count, k, rp], bt [count, rp, n].
+// Per-adapter transposes of the weights in use: at [places, k, rp], bt [places, rp, n].
 struct AdapterTransposeArgs {
   AdapterBatch batch;
   const int32_t *ranks;

@@ -302,3 +302,16 @@ def test_the_fault_words_alignment():
     assert lib.xp_adapter_backward(far, P, 8, 0x10000, 64, 0x20000, 48, None, 0, 0x50000, 64, None, None, 0x80000, 1 << 30,
                                    0x3000001, None) == BAD
     assert "aligned" in _native.last_error()
+
+
+def test_transposes_have_room_for_the_adapters_with_rows_only():
+    """Weights of 1024 adapters of rank 8 (padded to 16) are 940 MB; a batch of one row uses one of them."""
+
+    k, n = 4096, 24576
+    one = 16 * (k + n) * 2
+    for rows in (1, 2, 40, 64):
+        # Beside the transposes: partial sums and coefficients of a tile, tables of ints of the pool.
+        assert rows * one < workspace(rows, 1, 1024, 8, k, n) < (rows + 1) * one + 512 * 1024, rows
+    assert workspace(5000, 1, 1024, 8, k, n) > 1024 * one
+    # Up to 32 adapters every one has its place.
+    assert workspace(1, 1, 32, 8, k, n) > 32 * one

@@ -812,3 +812,22 @@ def test_operands_in_columns_of_one_tensor(device, rows):
     operator.run_into(tall[0::2, :72], weights, adapter_ids=ids, base=None, output=tall[1::2])
     with pytest.raises(_native.NativeError, match="overlap"):
         operator.run_into(tall[0::2, :72], weights, adapter_ids=ids, base=None, output=tall[:rows])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,count,used", [
+    (1, 33, [32]), (2, 1024, [5, 1023]), (40, 33, [0, 3, 31, 32]), (64, 200, list(range(64, 128))), (70, 40, [39]),
+    (500, 100, [7, 8, 50, 99, -1]), (500, 32, [7, 31, -1]), (8193, 40, [1, 38, -1]), (8193, 32, [1, 30, -1]),
+])
+def test_backward_of_large_pools_stays_in_its_scratch(device, rows, count, used, dtype):
+    """Few of a pool's adapters in use, in scratch of the size asked for and no larger."""
+
+    case = Case(device, rows=rows, k=136, n=72, count=count, max_rank=12, dtype=dtype,
+                ids=[used[i * 7 % len(used)] for i in range(rows)], seed=rows + count)
+    plan = case.operator(backward=True).plan
+    nbytes = plan.workspace.nbytes
+    assert nbytes - 256 <= _native.library().xp_adapter_workspace_bytes(
+        rows, count, 12, 136, 72, {"bf16": _native.XP_DTYPE_BF16, "fp32": _native.XP_DTYPE_F32}[dtype], 1) <= nbytes
+    scratch = torch.full((nbytes + (1 << 20),), 0xFF, dtype=torch.uint8, device=device)
+    check_backward(case, backward(case, Adapter(plan, scratch[:nbytes])))
+    assert bool((scratch[nbytes:] == 0xFF).all())
