@@ -39,7 +39,8 @@ __device__ __forceinline__ RouteSums wave_inclusive_scan(RouteSums sums) {
 // the gradients have one order.  Bound by the latency of its steps: one read of the ids (kept in registers
 // with their places up to 8192 rows), four barriers, one wave's scan where two groups per lane hold all of
 // them.  One increment per group and 64 rows: with one per row the LDS took a cycle for each (8192 rows of
-// 8 adapters: 14 us, 9.7 so).
+// 8 adapters: 14 us, 9.8 so).  Past 8192 rows the ids are read twice and the time grows with the rows: 20 us
+// for 16384 of 8 adapters, 72 for 65536 and 1.4 ms for 2^20 (512 adapters: 32, 114 and 2.0 ms).
 constexpr int kRouteKept = 8;
 
 struct RouteLds {
@@ -467,7 +468,7 @@ __global__ __launch_bounds__(256) void adapter_terms_kernel(AdapterTermsArgs a) 
 
 // ------------------------------------------------------------------ gradients of several runs
 // The runs' sums of an adapter's gradients in run order, times its scale; zeros for an adapter without
-// rows.  Reads what the outer products left in the last-level cache: 5.8 us for two runs of 28672 columns
+// rows.  Reads what the outer products wrote just before: 5.8 us for two runs of 28672 columns
 // of rank 16, 2 to 4 where there is nothing to add.
 __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterReduceArgs a) {
   const bool second = static_cast<int64_t>(blockIdx.x) >= a.blocks0;

@@ -180,11 +180,11 @@ __device__ __forceinline__ float element(const void *base, int64_t index) {
 // One tile of rows against all of its adapter's A rows over one K range.  The workgroup's four waves
 // take the range's groups of U steps in turn; a step is 64 bytes of every row.  Loads have four
 // neighbouring lanes on a row's 64 bytes and go through 1 KB of LDS per operand, the wave's own, to the
-// lanes that the MFMA wants them in: loaded in those (rows along the lanes) every lane is an access of
-// its own, four times the address cycles (8192 x 12288 at rank 64 in bf16: 59 us, 53 so).  Partial sums
+// lanes that the MFMA wants them in: loaded in those, with rows along the lanes, every lane is an access of
+// its own (8192 x 12288 of one adapter of rank 64 in bf16: 59 us, 53 to 55 so).  Partial sums
 // of the waves meet in LDS, those of the ranges in `partials` [range][row][rp].  Bound by the rows' bytes:
-// 4096 rows of 24576 and of 4096 columns at rank 16 take 53 us (4.4 TB/s); at rank 64 A brings as many
-// bytes through the L2 as the rows do (8192 x 12288, eight adapters: 57 us, 3.5 TB/s).
+// 4096 rows of 24576 and of 4096 columns at rank 16 take 53 us (4.4 TB/s); at rank 64 every tile of 64 rows
+// reads as many bytes of A, from the L2, as of the rows (8192 x 12288, eight adapters: 57 to 59 us, 3.5 TB/s).
 template <int RT>
 constexpr int kShrinkRegion = (4 + RT) * 1024;  // bytes of LDS per wave
 
@@ -392,8 +392,8 @@ __global__ __launch_bounds__(kAdapterShrinkWaves *kWave, RT <= 2 ? 4 : 2) void a
 // CH i + j of a unit of 16 CH being column i of MFMA tile j: a lane's sums over the CH tiles are then 16
 // bytes of consecutive columns of one row, and 16 lanes hold 256 contiguous bytes of it, so that base is
 // read and the result stored in whole lines by neighbouring lanes.  (With rows along the lanes, as the
-// products' natural layout has them, every lane of a load or store is an access of its own: four
-// times the address cycles, 60 us instead of 39 for 8192 x 4096 at rank 64 in bf16.)
+// products' natural layout has them, every lane of a load or store is an access of its own: 60 us instead
+// of 39 for 8192 x 4096 at rank 64 in bf16.)
 //
 // Sorted batches give each wave 16 rows of a tile and stage a unit's B rows in LDS, read from memory
 // once and in order, one unit ahead.  Small ones (decode) give each wave a unit of its own and turn the B
@@ -971,7 +971,7 @@ void adapter_expand_kernel(AdapterExpandArgs a) {
 // kilobyte per load.  Four waves take the run's tiles of 64 rows in turn and meet in LDS; a run that is
 // its adapter's only one stores the gradient, others their sums, which adapter_reduce_kernel adds in
 // run order.  Bound by the rows' bytes: 4096 rows of 4096 and 24576 columns at rank 16 take 37 us in two
-// runs per column block (6.4 TB/s, part of it from the last-level cache), 44 us in one, 38 to 39 in three
+// runs per column block (6.4 TB/s, more than a copy's rate: the pass before read the same rows), 44 us in one, 38 to 39 in three
 // or four, whose sums cost the reduction more as well.
 constexpr int kAdapterOuterWaves = 4;
 

@@ -7,11 +7,11 @@
 // over the T live rows; counts are constants of the gradient.  A row whose logits are all -inf has p = 0.
 //
 // Bound by memory: the loss reads the logits and ids once, the gradient reads the logits and writes
-// as much (65536 rows of 128 fp32 logits, eight routes each: the loss 12.2 us, 2.9 TB/s, and 5.2 us for
-// the workgroups' sums, the gradient 16.5 us, 4.1 TB/s; both launches end in a few microseconds of
-// latency that does not shrink with the rows).  A row is held by a 16-, 32- or 64-lane part of a wave, four consecutive experts per lane
-// and load, so that a wave takes several narrow rows at once; sums over a row go through DPP within
-// 16 lanes.  The loss keeps sum_t p_te of the lane's own experts in registers over all of its
+// as much (65536 rows of 128 fp32 logits, eight routes each: the loss 12.5 us, 2.8 TB/s, and 5.5 us for
+// the workgroups' sums, the gradient 17 to 18 us, 3.8 TB/s; both launches end in a few microseconds of
+// latency that does not shrink with the rows).  A row is held by a 16-, 32- or 64-lane part of a wave, four
+// consecutive experts per lane and load, so that a wave takes several narrow rows at once; sums over a row go
+// through DPP within 16 lanes.  The loss keeps sum_t p_te of the lane's own experts in registers over all of its
 // rows and adds waves, then workgroups, in a fixed order: no floating-point atomics, equal bits
 // every time.  Counts are integers, added by LDS atomics.
 

@@ -337,8 +337,8 @@ class BalanceLoss:
     ``loss = coefficient * sum_e f_e * P_e`` with ``f_e`` expert e's share of the routes (times the
     expert count) and ``P_e`` its mean score over the live rows: the softmax of the logits, or their
     sigmoids divided by the row's sum.  ``counts`` (int32 ``[experts]``) and ``loss`` (fp32 ``[1]``) are
-    the outputs of :meth:`run_into`; served layers read ``counts`` as the experts' load.  The reference
-    has no counterpart; the operator follows ``Router``'s.
+    the outputs of :meth:`run_into`.  ``payload_rows`` is an int32 value here (``finalize_moe_routing`` takes an
+    int64 one).  The reference has no counterpart; the operator follows ``Router``'s.
     """
 
     def __init__(

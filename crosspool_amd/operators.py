@@ -158,7 +158,8 @@ class Activation:
     ) -> None:
         """Gradient of :meth:`apply_into`'s inputs, in their shape and order (no counterpart in the reference).
 
-        A value clipped by the gate transform's limit gets none; one at the limit does.  ``grad_inputs``
+        A value clipped by the gate transform's limit gets none; one at the limit does, and NaN is not clipped:
+        a NaN Gate makes both gradients of its pair NaN, a NaN Up the Gate's.  ``grad_inputs``
         may be ``inputs`` itself, and for an ungated activation ``grad_output`` itself.
         """
 
@@ -426,7 +427,9 @@ class Dense:
 
         ``adapters`` (of a plan prepared for them) adds the low-rank adapters that ``adapter_ids`` (int32,
         one per row, -1: none) names to each projection; an id outside the pool gives a row of NaN and a
-        bit in ``fault_word``.
+        bit in ``fault_word``.  With i_proj adapters the activation is that of
+        ``Adapter.run_into``: rows without an adapter may differ in a last bit from those of a layer without
+        pools, and a NaN that a limit hides there stays.
         """
 
         if (adapters is None) != (adapter_ids is None):

@@ -831,3 +831,17 @@ def test_backward_of_large_pools_stays_in_its_scratch(device, rows, count, used,
     scratch = torch.full((nbytes + (1 << 20),), 0xFF, dtype=torch.uint8, device=device)
     check_backward(case, backward(case, Adapter(plan, scratch[:nbytes])))
     assert bool((scratch[nbytes:] == 0xFF).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows", [64, 128])
+def test_rows_without_an_adapter_keep_every_bit_of_any_value(device, rows, dtype):
+    """All 65536 patterns: zeros of both signs, subnormals and infinities as they are, NaN as some NaN."""
+
+    case = Case(device, rows=rows, k=16, n=65536 // rows, count=2, max_rank=4, dtype=dtype, ids=[-1] * rows)
+    case.base = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(case.dtype).reshape(rows, -1)
+    case.a.fill_(float("nan"))
+    got = run(case).cpu()
+    assert torch.equal(got.isnan(), case.base.isnan())
+    keep = ~case.base.isnan()
+    assert torch.equal(got.view(torch.int16)[keep], case.base.view(torch.int16)[keep])
