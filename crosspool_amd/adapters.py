@@ -163,27 +163,35 @@ class Adapter:
     def __init__(self, plan: AdapterPlan, workspace: torch.Tensor) -> None:
         if workspace.device.type != "cuda":
             raise ValueError("adapter scratch must reside on its execution device")
-        (self.scratch,) = plan.workspace.views(workspace)
-        self.plan = plan
+        (self._workspace,) = plan.workspace.views(workspace)
+        self._plan = plan
         self._device = workspace.device
         self._index = workspace.device.index
-        self._scratch = self.scratch.data_ptr()
-        self._scratch_bytes = self.scratch.numel()
+        self._scratch = self._workspace.data_ptr()
+        self._scratch_bytes = self._workspace.numel()
         self._pool_shape = (plan.adapter_count, plan.max_rank, plan.input_width)
         self._output_shape = (plan.adapter_count, plan.output_width, plan.max_rank)
+
+    @property
+    def plan(self) -> AdapterPlan:
+        return self._plan
+
+    @property
+    def scratch(self) -> torch.Tensor:
+        return self._workspace
 
     def _rows(self, tensor: torch.Tensor, name: str, rows: int, width: int) -> int:
         """The row stride of an operand (checked)."""
 
-        if tensor.dtype is not self.plan.dtype or tensor.shape != (rows, width) or tensor.get_device() != self._index:
-            raise ValueError(f"adapter {name} must be a {self.plan.dtype} tensor of shape {(rows, width)} on {self._device}")
+        if tensor.dtype is not self._plan.dtype or tensor.shape != (rows, width) or tensor.get_device() != self._index:
+            raise ValueError(f"adapter {name} must be a {self._plan.dtype} tensor of shape {(rows, width)} on {self._device}")
         stride, column = tensor.stride()
         if (column != 1 and width > 1) or (stride < width and rows > 1):
             raise ValueError(f"adapter {name} must have contiguous, separate rows")
         return stride if rows > 1 else width
 
     def _batch(self, weights: AdapterWeights, adapter_ids: torch.Tensor, rows: int, fault_word: torch.Tensor | None) -> None:
-        plan = self.plan
+        plan = self._plan
         if rows > plan.row_capacity:
             raise ValueError(f"{rows} adapter rows exceed the prepared capacity {plan.row_capacity}")
         if (
@@ -224,7 +232,7 @@ class Adapter:
         ``[-1, adapters)`` gives a row of NaN and ORs ``XP_FAULT_ADAPTER_OUT_OF_RANGE`` into ``fault_word``.
         """
 
-        plan = self.plan
+        plan = self._plan
         if inputs.ndim != 2:
             raise ValueError("adapter inputs must be a matrix")
         rows = inputs.shape[0]
@@ -267,7 +275,7 @@ class Adapter:
         for adapters without rows.
         """
 
-        plan = self.plan
+        plan = self._plan
         if not plan.backward:
             raise ValueError("the adapter plan was prepared without backward")
         if inputs.ndim != 2:

@@ -368,10 +368,22 @@ class BalanceLoss:
         self._algorithm_code = int(self.algorithm)
         self.coefficient = float(coefficient)
         nbytes = int(_native.library().xp_moe_balance_workspace_bytes(row_capacity, routed_expert_count))
-        self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=self.device)
-        self._scratch, self._scratch_bytes = self.workspace.data_ptr(), self.workspace.numel()
-        self.counts = torch.zeros(routed_expert_count, dtype=torch.int32, device=self.device)
-        self.loss = torch.zeros(1, dtype=torch.float32, device=self.device)
+        self._workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=self.device)
+        self._scratch, self._scratch_bytes = self._workspace.data_ptr(), self._workspace.numel()
+        self._counts = torch.zeros(routed_expert_count, dtype=torch.int32, device=self.device)
+        self._loss = torch.zeros(1, dtype=torch.float32, device=self.device)
+
+    @property
+    def workspace(self) -> torch.Tensor:
+        return self._workspace
+
+    @property
+    def counts(self) -> torch.Tensor:
+        return self._counts
+
+    @property
+    def loss(self) -> torch.Tensor:
+        return self._loss
 
     def _check(self, tensor: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple[int, ...]) -> None:
         if tensor.dtype is not dtype or tensor.shape != shape or tensor.get_device() != self._index or not tensor.is_contiguous():
@@ -412,7 +424,7 @@ class BalanceLoss:
         _native.call(
             "xp_moe_balance_loss", None if logits is None else logits.data_ptr(), code, ids.data_ptr(), rows,
             self.routed_expert_count, self.routed_topk, self._algorithm_code, live, self.coefficient,
-            self.counts.data_ptr(), None if logits is None else self.loss.data_ptr(), self._scratch,
+            self._counts.data_ptr(), None if logits is None else self._loss.data_ptr(), self._scratch,
             self._scratch_bytes, _native.current_stream(self._index),
         )
 
@@ -435,7 +447,7 @@ class BalanceLoss:
         live = self._live(rows, payload_rows)
         code = self._logits_code(logits, rows)
         self._check(grad_logits, "grad_logits", logits.dtype, (rows, self.routed_expert_count))
-        counts = self.counts if counts is None else counts
+        counts = self._counts if counts is None else counts
         self._check(counts, "counts", torch.int32, (self.routed_expert_count,))
         if grad_loss is not None and (
             grad_loss.dtype is not torch.float32 or grad_loss.numel() != 1 or grad_loss.get_device() != self._index

@@ -845,3 +845,12 @@ def test_rows_without_an_adapter_keep_every_bit_of_any_value(device, rows, dtype
     assert torch.equal(got.isnan(), case.base.isnan())
     keep = ~case.base.isnan()
     assert torch.equal(got.view(torch.int16)[keep], case.base.view(torch.int16)[keep])
+
+
+def test_an_operators_scratch_stays_its_own(device):
+    case = Case(device, rows=70, k=64, n=48, count=2, max_rank=8)
+    operator = case.operator()
+    for name in ("scratch", "plan"):
+        with pytest.raises(AttributeError):
+            setattr(operator, name, getattr(case.operator(), name))
+    check_forward(case, run(case, operator))

@@ -342,3 +342,12 @@ def test_the_lowest_logits_share_alike(device):
     logits = torch.full((300, 16), torch.finfo(torch.float32).min)
     ids = torch.zeros((300, 1), dtype=torch.int32)
     check_sigmoid(device, logits, ids, 1, 1.0)
+
+
+def test_an_operators_buffers_stay_its_own(device):
+    operator = BalanceLoss(row_capacity=4096, routed_expert_count=16, routed_topk=2)
+    for name in ("workspace", "counts", "loss"):
+        with pytest.raises(AttributeError):
+            setattr(operator, name, getattr(operator, name)[:1].clone())
+    logits, ids = make(4096, 16, 2, "fp32")
+    check(operator, logits, ids, device=device)
