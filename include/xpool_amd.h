@@ -203,8 +203,8 @@ typedef struct {
 
 /* Workspace bytes that xp_adapter_apply (or, with `backward`, xp_adapter_backward) needs for every
  * row count up to `rows`; 0 for sizes that they refuse and where nothing is needed (rows = 0 without
- * `backward`).  The workspace is 16-byte aligned, its
- * contents do not matter on entry, and calls that may overlap in time must not share one. */
+ * `backward`).  The workspace is 16-byte aligned, its contents do not matter on entry, and calls that
+ * may overlap in time must not share one. */
 size_t xp_adapter_workspace_bytes(int64_t rows, int64_t count, int64_t max_rank, int64_t input_width,
                                   int64_t output_width, int dtype, int backward);
 
@@ -213,12 +213,13 @@ size_t xp_adapter_workspace_bytes(int64_t rows, int64_t count, int64_t max_rank,
  * [rows, input_width], base [rows, output_width], out [rows, output_width] (a gated activation:
  * [rows, output_width / 2] over INTERLEAVED Gate/Up columns), element-aligned, with row strides of
  * ldx, ld_base and ld_out elements.  Without an activation out may be base itself (same pointer and
- * stride); no other overlap.  All sums are fp32; one rounding, at the store (with an activation the
- * sum is not rounded before it, unlike xp_projection's; a NaN sum stays NaN past a limit, which
- * xp_projection and xp_activation make the limit of).  The result of a row depends on its own
- * values and id and on the row count, not on the other rows' adapters or order.  An id outside
- * [-1, count) gives a row of quiet NaNs and ORs XP_FAULT_ADAPTER_OUT_OF_RANGE into fault_word (may be
- * NULL). */
+ * stride); else nothing written (the workspace and the fault word too) may share a byte with what is read or
+ * written beside it, in either call.  Rows between another operand's rows, as columns of one tensor are,
+ * do not.  All sums are fp32; one rounding, at the store (with an activation the sum is not rounded before
+ * it, unlike xp_projection's; a NaN sum stays NaN past a limit, which xp_projection and xp_activation make
+ * the limit of).  The result of a row depends on its own values and id and on the row count, not on the
+ * other rows' adapters or order.  An id outside [-1, count) gives a row of quiet NaNs and ORs
+ * XP_FAULT_ADAPTER_OUT_OF_RANGE into fault_word (may be NULL). */
 int xp_adapter_apply(const xp_adapter_pool *pool, const int32_t *ids, int64_t rows, const void *x, int64_t ldx,
                      const void *base, int64_t ld_base, void *out, int64_t ld_out,
                      const xp_activation_desc *activation, void *workspace, size_t workspace_bytes,
@@ -503,7 +504,8 @@ int xp_moe_router(const void *hidden_states, int64_t rows, int64_t hidden, const
  * T the live rows, p the softmax of a row's logits or their sigmoids divided by their sum
  * (XP_ROUTER_SIGMOID); a row without any score (all logits -inf) has p = 0, no live row a loss of 0.
  * counts is int32 [experts], loss one fp32 value.  logits and loss NULL: the counts alone.  The sums have
- * one order: repeated calls give the same bits.  The workspace (16-byte aligned) serves every row count
+ * one order: repeated calls give the same bits.  Counts, loss and workspace may overlap neither the operands
+ * nor each other.  The workspace (16-byte aligned) serves every row count
  * up to the one asked for; its contents do not matter on entry.  No counterpart in the reference. */
 size_t xp_moe_balance_workspace_bytes(int64_t rows, int64_t experts);
 int xp_moe_balance_loss(const void *logits, int logits_dtype, const int32_t *ids, int64_t rows, int64_t experts,

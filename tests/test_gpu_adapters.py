@@ -854,3 +854,27 @@ def test_an_operators_scratch_stays_its_own(device):
         with pytest.raises(AttributeError):
             setattr(operator, name, getattr(case.operator(), name))
     check_forward(case, run(case, operator))
+
+
+@pytest.mark.parametrize("k,n", [(20000, 64), (64, 20000)])
+def test_transposes_whose_offsets_pass_32_bits(device, k, n):
+    """1024 adapters with rows, the last two's weights alone not zero: their transposes lie past 5 GB."""
+
+    rows, used = 1100, [1022, 1023]
+    small = Case(device, rows=rows, k=k, n=n, count=2, max_rank=128, ids=[i % 3 - 1 if i < 60 else -1 for i in range(rows)])
+    gradients = backward(small)
+    a = torch.zeros((1024, 128, k), dtype=small.dtype, device=device)
+    b = torch.zeros((1024, n, 128), dtype=small.dtype, device=device)
+    scales = torch.ones(1024, device=device)
+    a[used], b[used], scales[used] = small.a.to(device), small.b.to(device), small.scales.to(device)
+    ids = torch.where(small.ids >= 0, small.ids + 1022, -1)
+    ids[60:60 + 1022] = torch.arange(1022, dtype=torch.int32)
+    plan = AdapterPlan.prepare(row_capacity=rows, adapter_count=1024, max_rank=128, input_width=k, output_width=n,
+                               dtype=small.dtype, backward=True)
+    operator = Adapter(plan, torch.empty(plan.workspace.nbytes, dtype=torch.uint8, device=device))
+    x, gx, ga, gb = small.x.to(device), torch.empty_like(gradients["x"]), torch.full_like(a, 1.0), torch.full_like(b, 1.0)
+    operator.backward_into(x, small.grad.to(device), AdapterWeights(a, b, scales), adapter_ids=ids.to(device),
+                           base=small.grad_base.to(device), grad_inputs=gx, grad_a=ga, grad_b=gb)
+    assert torch.equal(gx, gradients["x"])
+    assert torch.equal(ga[used], gradients["a"]) and torch.equal(gb[used], gradients["b"])
+    assert not bool(ga[:1022].any()) and not bool(gb[:1022].any())
