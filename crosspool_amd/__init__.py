@@ -6,7 +6,9 @@ Public surface, mirroring the reference's FfnAgent API:
 * :mod:`crosspool_amd.ops`       -- ``ffn_shim`` (SGLang drop-in Tensor op), ``attach``
 * :mod:`crosspool_amd.dense`     -- ``DenseExecutionPlan``, ``Dense`` and kernel-level ops
 * :mod:`crosspool_amd.execution` -- Execution Signatures, capacity buckets, workspaces
-* :mod:`crosspool_amd.operators` -- the operator layer (other dtypes, biases, orders; activation gradients)
+* :mod:`crosspool_amd.operators` -- the operator layer (other dtypes, biases, orders; gradients of the activation,
+  of projections and of a Dense layer)
+* :mod:`crosspool_amd.muon`      -- orthogonal updates of weight matrices and their optimiser's step
 * :mod:`crosspool_amd.adapters`  -- low-rank adapters of many requests beside a projection, and their gradients
 * :mod:`crosspool_amd.moe`       -- MoE operators (Router, Experts, expert counts and balance loss)
 * :mod:`crosspool_amd.weights`   -- Dense weight containers (interleaved Gate/Up)

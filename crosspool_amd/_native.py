@@ -79,6 +79,12 @@ class AdapterPool(ctypes.Structure):
     ]
 
 
+class Matrices(ctypes.Structure):
+    """``xp_matrices`` of the header."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("matrix_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64)]
+
+
 XP_DTYPE_BF16 = 1
 XP_DTYPE_F16 = 2
 XP_DTYPE_F32 = 3
@@ -122,6 +128,31 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "xp_adapter_backward": (
         _INT,
         [ctypes.POINTER(AdapterPool), _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _SIZE, _P, _P],
+    ),
+    "xp_projection_backward_workspace_bytes": (_SIZE, [_I64, _I64, _I64, _INT]),
+    "xp_projection_backward": (
+        _INT, [_P, _I64, _I64, _I64, _P, _I64, _P, _I64, _INT, _P, _I64, _P, _INT, _P, _INT, _I64, _P, _SIZE, _P],
+    ),
+    "xp_projection_keep_workspace_bytes": (_SIZE, [_I64, _I64, _I64, _INT]),
+    "xp_projection_keep": (
+        _INT,
+        [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _INT, ctypes.POINTER(ActivationDesc), _I64, _P, _SIZE, _P],
+    ),
+    "xp_dense_backward_workspace_bytes": (_SIZE, [_I64, _I64, _I64, _INT, _INT]),
+    "xp_dense_backward": (
+        _INT,
+        [_P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _P, _I64, _INT, _INT, ctypes.POINTER(ActivationDesc), _P, _I64, _P,
+         _P, _INT, _P, _P, _INT, _I64, _P, _SIZE, _P],
+    ),
+    "xp_muon_workspace_bytes": (_SIZE, [_I64, _I64, _I64, _INT]),
+    "xp_muon_orthogonalize": (
+        _INT,
+        [ctypes.POINTER(Matrices), _I64, _I64, _I64, _INT, _INT, _F32, ctypes.POINTER(Matrices), _P, _SIZE, _P],
+    ),
+    "xp_muon_step": (
+        _INT,
+        [ctypes.POINTER(Matrices), ctypes.POINTER(Matrices), ctypes.POINTER(Matrices), ctypes.POINTER(Matrices),
+         ctypes.POINTER(Matrices), _I64, _I64, _I64, _INT, _INT, _INT, _F32, _F32, _F32, _F32, _INT, _F32, _P, _SIZE, _P],
     ),
     "xp_dense_workspace_bytes": (_SIZE, [_I64, _I64, _I64]),
     "xp_dense_workspace_layout": (_INT, [_I64, _I64, _I64, ctypes.POINTER(_SIZE)]),

@@ -30,15 +30,12 @@
 #pragma once
 
 #include "xp_kernels.hpp"
+#include "xp_tiles.hpp"
 
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
 #include <utility>
-
-// Lambdas of the kernels below are forced inline: a lambda left out of line takes the
-// accumulator array by reference, which then lives in scratch memory instead of registers.
-#define XP_INLINE __attribute__((always_inline))
 
 namespace xp {
 namespace {
@@ -53,10 +50,6 @@ __device__ __forceinline__ uint16_t *output_row(const GemmArgs &a, int64_t token
   }
   return a.out + token * a.ldo;
 }
-
-// Offset that is always past a buffer resource's end (resources stay below 2^31 bytes, and
-// adding a row's byte offset keeps it below 2^32).
-constexpr uint32_t kOutOfRange = 0x7ffffff0u;
 
 // Fused mailbox gather of token rows [0, TP) into LDS rows of stride `rs` (elements),
 // columns [kbase, kbase + 8 vectors_per_row) of which the first kvalid hold data: token row
@@ -207,25 +200,6 @@ __device__ __forceinline__ void stage_gathered_rows(const GemmArgs &a, uint16_t 
       }
     }
   }
-}
-
-using lds_void_t = __attribute__((address_space(3))) void *;
-
-// Direct global -> LDS load of 16 bytes per lane through a buffer resource: lane i's
-// data lands at `lds_row_base + 16 i`; offsets past the resource's end write zeros.
-template <int POLICY = 0>
-__device__ __forceinline__ void buffer_load_lds16(__amdgpu_buffer_rsrc_t rsrc, void *lds_base, uint32_t voffset,
-                                                  uint32_t soffset) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t)(lds_base), 16, static_cast<int>(voffset),
-                                           static_cast<int>(soffset), 0, POLICY);
-}
-
-// s_waitcnt with vmcnt <= N and the LDS / export counters left unconstrained (gfx9 encoding:
-// vmcnt bits [3:0] and [15:14], expcnt [6:4], lgkmcnt [11:8]).
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-  static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit counter");
-  __builtin_amdgcn_s_waitcnt((N & 0xf) | ((N >> 4) << 14) | (0x7 << 4) | (0xf << 8));
 }
 
 // ------------------------------------------------------------------ split (decode)
@@ -1597,22 +1571,6 @@ __global__ __launch_bounds__(64 * kResidentWaves) __attribute__((amdgpu_waves_pe
 }
 
 // ------------------------------------------------------------------ tile
-// LDS tiles are rows of 64 bf16 (128 bytes = eight 16-byte chunks).  gfx950 serves
-// ds_read_b128 sixteen lanes at a time from a 256-byte bank line, i.e. two tile rows, so
-// the 16 rows one MFMA fragment read touches must occupy 16 distinct 16-byte slots:
-// logical chunk c of row r is stored at physical chunk c ^ ((r / 2) % 8).
-__device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
-
-// Calls f(std::integral_constant<int, 0>{}) .. f(std::integral_constant<int, N - 1>{}).
-template <class F, int... I>
-__device__ __forceinline__ void static_for_impl(F &&f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, class F>
-__device__ __forceinline__ void static_for(F &&f) {
-  static_for_impl(f, std::make_integer_sequence<int, N>{});
-}
-
 // Weight tile tn and token tile tm of this workgroup (grid x spans the weight tiles, y the
 // token tiles).  Workgroups go to the 8 XCDs round robin by linear id L = x + y gridDim.x,
 // so XCD c runs L = c, c + 8, c + 16, ... in that order, 32 at a time (one per CU).  When

@@ -1,0 +1,89 @@
+// Matrix products of the training operators: out[m][n] = epilogue(sum over k of A(m, k) B(n, k)), every
+// operand stored with its reduction axis along its rows or across them.  Argument records and plans; the
+// kernels are in product_kernels.hpp, instantiated for one payload in product_{bf16,f16,f32}.hip.
+#pragma once
+
+#include "xp_kernels.hpp"
+
+namespace xp {
+
+// What a product does with its fp32 sums.
+enum class ProductEpilogue : int {
+  kStore = 0,     // out = alpha sum + beta base + bias; or keep extra - step (alpha sum + beta base)
+  kActivate = 1,  // out = sum + bias rounded to the payload, extra = the activation of that
+  kGradient = 2,  // a gradient of an activation's outputs: out = the gradient of its inputs (base), extra = its outputs
+};
+
+// One operand [rows, k]: element (r, k) at data[r ld + k], or where the reduction axis runs across its rows
+// (`cols` of a kernel) at data[k ld + r].
+struct ProductOperand {
+  const void *data;
+  int64_t ld;
+  int64_t batch;  // elements between the matrices of a batch
+};
+
+struct ProductArgs {
+  ProductOperand a;
+  ProductOperand b;
+  int64_t m;
+  int64_t n;
+  int64_t k;
+  int64_t k_slice;     // columns of one K range
+  float *partials;     // [batch, ranges, m, n rounded up to 8] sums of K ranges, where there are several
+  void *out;
+  int64_t ld_out;
+  int64_t batch_out;
+  const void *base;
+  int64_t ld_base;
+  int64_t batch_base;
+  void *extra;         // kStore: values read (weights), may be null; else written
+  int64_t ld_extra;
+  int64_t batch_extra;
+  const float *bias;   // fp32 [n] or null
+  float *column_sums;  // kGradient: sums of the unrounded gradients over bands of rows [bands, 2 n or n], or null
+  float alpha;
+  float beta;          // 0: base is not read
+  float keep;
+  float step;
+  int32_t ranges;
+  int32_t batch;
+  int8_t out_dtype;
+  int8_t base_dtype;
+  int8_t extra_dtype;
+  int8_t symmetric;    // A and B are one operand: tiles below the diagonal are computed and mirrored
+  int8_t padded_out;   // kStore: the output's rows are whole groups of eight columns, zeros behind column n
+  int8_t interleaved;  // kActivate, kGradient: Gate/Up pairs in neighbouring columns, else in halves
+  ActivationArgs act;
+};
+static_assert(sizeof(ProductArgs) <= 256, "a kernel's argument record");
+
+struct ProductPlan {
+  int tile;          // square tiles of 256, 128 or 64
+  int64_t ranges;
+  int64_t k_slice;
+  int64_t bands;     // rows of column_sums
+};
+
+// The fastest tile and K ranges for a product in a workspace of `scratch` bytes for its partial sums.
+ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int64_t batch, int element_bytes, bool symmetric, size_t scratch);
+size_t product_scratch_bytes(const ProductPlan &plan, int64_t m, int64_t n, int64_t batch);
+
+struct ProductLaunch {
+  KernelLaunch main;
+  KernelLaunch reduce;  // empty with one K range
+};
+// `dtype` is that of the operands.  Fills ranges and k_slice of the record from the plan.
+ProductLaunch make_product(const ProductArgs &args, const ProductPlan &plan, ProductEpilogue epilogue, bool a_cols, bool b_cols,
+                           int dtype);
+
+// The product as planned for its sizes; `chosen` gets the plan.
+hipError_t launch_product(const ProductArgs &args, ProductEpilogue epilogue, bool a_cols, bool b_cols, int dtype,
+                          size_t scratch_bytes, hipStream_t stream, ProductPlan *chosen = nullptr);
+
+template <class P>
+struct ProductKernels {
+  static const void *tile(int tile, ProductEpilogue epilogue, bool a_cols, bool b_cols);
+  static const void *reduce(ProductEpilogue epilogue);
+};
+
+}  // namespace xp

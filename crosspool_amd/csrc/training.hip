@@ -1,0 +1,670 @@
+// Training a layer's projections: their gradients, the gated block's forward pass with what its backward pass
+// reads, and that backward pass.  No counterpart in the reference.
+//
+// Every product is one of product_kernels.hpp: y = x w^T + b has dx = dy w, whose reduction runs along dy's rows
+// and across w's, and dw = dy^T x, whose reduction runs across the rows of both.  The gradient of the
+// activation's outputs is never written: its product's epilogue reads the kept projection and writes the
+// projection's gradient and the activation's outputs, both of which the weights' gradients read next.
+//
+// Operands whose rows are not whole 16-byte chunks are first copied with padded rows into the workspace.
+
+#include "product.hpp"
+#include "xp_elements.hpp"
+#include "xp_entry.hpp"
+
+#include <cmath>
+
+namespace xp {
+namespace {
+
+// ------------------------------------------------------------------ rows of whole chunks
+struct PadArgs {
+  const void *source;
+  void *target;
+  int64_t rows;
+  int64_t width;
+  int64_t ld;
+  int64_t padded;  // row length of the target, a whole number of chunks
+};
+
+// Rows of any alignment into rows of whole 16-byte chunks, zeros behind them.  One thread a chunk.
+template <class P>
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
+  constexpr int CHUNK = 16 / kElementBytes<P>;
+  const int64_t chunks = a.padded / CHUNK;
+  const int64_t index = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = index / chunks;
+  if (row >= a.rows) {
+    return;
+  }
+  const int64_t column = (index - row * chunks) * CHUNK;
+  const unsigned char *from = static_cast<const unsigned char *>(a.source) + (row * a.ld + column) * kElementBytes<P>;
+  const u32x4 chunk = a.width - column >= CHUNK ? load16_any(from) : load_chunk_tail<P, P>(from, a.width - column);
+  store16(static_cast<unsigned char *>(a.target) + (row * a.padded + column) * kElementBytes<P>, chunk);
+}
+
+// Zeros in columns [width, padded) of every row of the target.
+__global__ __launch_bounds__(256) void clear_pad_kernel(PadArgs a, int element) {
+  const int64_t behind = (a.padded - a.width) * element / 2;  // 16-bit words
+  const int64_t index = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = index / behind;
+  if (row < a.rows) {
+    uint16_t *words = reinterpret_cast<uint16_t *>(static_cast<unsigned char *>(a.target) + (row * a.padded + a.width) * element);
+    words[index - row * behind] = 0;
+  }
+}
+
+// ------------------------------------------------------------------ sums over rows
+struct ColumnSumArgs {
+  const void *source;  // [rows, n]
+  float *bands;        // [bands, n]
+  float *out;          // [n]
+  int64_t rows;
+  int64_t n;
+  int64_t ld;
+  int64_t band_rows;
+  int64_t band_count;
+  int32_t accumulate;
+};
+
+// fp32 sums of a band's rows, eight columns a thread.
+template <class P>
+__global__ __launch_bounds__(256) void column_sum_kernel(ColumnSumArgs a) {
+  constexpr int ES = kElementBytes<P>;
+  constexpr int CHUNK = 16 / ES;
+  const int64_t column = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * CHUNK;
+  if (column >= a.n) {
+    return;
+  }
+  const int64_t first = static_cast<int64_t>(blockIdx.y) * a.band_rows;
+  const int64_t last = first + a.band_rows < a.rows ? first + a.band_rows : a.rows;
+  const bool whole = a.n - column >= CHUNK;
+  float sum[CHUNK] = {};
+  const unsigned char *from = static_cast<const unsigned char *>(a.source) + (first * a.ld + column) * ES;
+#pragma unroll 4
+  for (int64_t row = first; row < last; ++row) {
+    const u32x4 chunk = whole ? load16_any(from) : load_chunk_tail<P, P>(from, a.n - column);
+    from += a.ld * ES;
+#pragma unroll
+    for (int j = 0; j < CHUNK; ++j) {
+      if constexpr (ES == 4) {
+        sum[j] += __uint_as_float(chunk[j]);
+      } else {
+        sum[j] += P::widen(j % 2 == 0 ? chunk[j / 2] & 0xffffu : chunk[j / 2] >> 16);
+      }
+    }
+  }
+  float *to = a.bands + static_cast<int64_t>(blockIdx.y) * a.n + column;
+#pragma unroll
+  for (int j = 0; j < CHUNK; ++j) {
+    if (column + j < a.n) {
+      to[j] = sum[j];
+    }
+  }
+}
+
+// The bands' sums in band order.
+__global__ __launch_bounds__(64) void band_sum_kernel(ColumnSumArgs a) {
+  const int64_t column = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x;
+  if (column >= a.n) {
+    return;
+  }
+  float sum = 0.0f;
+  const float *from = a.bands + column;
+#pragma unroll 8
+  for (int64_t band = 0; band < a.band_count; ++band) {
+    sum += from[band * a.n];
+  }
+  a.out[column] = a.accumulate ? a.out[column] + sum : sum;
+}
+
+// Zeros over whole rows of an output (its gradient over no rows).
+__global__ __launch_bounds__(256) void clear_kernel(uint16_t *target, int64_t words) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t index = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; index < words; index += stride) {
+    target[index] = 0;
+  }
+}
+
+unsigned blocks_of(int64_t items, int64_t per_block) { return static_cast<unsigned>((items + per_block - 1) / per_block); }
+
+constexpr size_t kAlign = 256;
+constexpr int64_t kMaxRows = int64_t{1} << 24;
+constexpr int64_t kMaxWidth = int64_t{1} << 20;
+constexpr int64_t kMaxStride = int64_t{1} << 20;
+
+size_t aligned_bytes(size_t bytes) { return (bytes + kAlign - 1) / kAlign * kAlign; }
+int64_t padded_width(int64_t width, size_t element) {
+  const int64_t chunk = static_cast<int64_t>(16 / element);
+  return (width + chunk - 1) / chunk * chunk;
+}
+bool whole_rows(int64_t width, size_t element) { return width % static_cast<int64_t>(16 / element) == 0; }
+
+// Regions of a workspace, one behind another.
+struct Regions {
+  unsigned char *base;
+  size_t used = 0;
+  void *take(size_t bytes) {
+    void *at = base == nullptr ? nullptr : base + used;
+    used += aligned_bytes(bytes);
+    return at;
+  }
+};
+
+// Partial sums of a product for every number of rows up to a capacity, at powers of two below it.
+template <class Plan>
+size_t scratch_upto(int64_t capacity, Plan &&plan) {
+  size_t most = 0;
+  for (int64_t rows = capacity; rows >= 1; rows /= 2) {
+    most = std::max(most, plan(rows));
+  }
+  return most;
+}
+
+size_t unlimited_scratch(int64_t m, int64_t n, int64_t k, int element) {
+  return product_scratch_bytes(plan_product(m, n, k, 1, element, false, SIZE_MAX), m, n, 1);
+}
+
+// ------------------------------------------------------------------ launches
+struct Caller {
+  hipStream_t stream;
+  int dtype;
+  size_t element;
+  float *scratch;
+  size_t scratch_bytes;
+
+  hipError_t product(ProductArgs &args, ProductEpilogue epilogue, bool a_cols, bool b_cols, ProductPlan *chosen = nullptr) const {
+    args.partials = scratch;
+    args.batch = 1;
+    return launch_product(args, epilogue, a_cols, b_cols, dtype, scratch_bytes, stream, chosen);
+  }
+
+  // `source` itself where its rows are whole chunks, else a padded copy in `target`.
+  hipError_t padded(const void *source, int64_t rows, int64_t width, int64_t ld, void *target, ProductOperand &operand) const {
+    if (whole_rows(width, element)) {
+      operand = {source, ld, 0};
+      return hipSuccess;
+    }
+    const int64_t length = padded_width(width, element);
+    operand = {target, length, 0};
+    KernelLaunch kernel;
+    kernel.func = element == 4 ? reinterpret_cast<const void *>(&pad_rows_kernel<F32Payload>)
+                               : reinterpret_cast<const void *>(&pad_rows_kernel<Bf16Payload>);
+    kernel.grid = dim3(blocks_of(rows * (length / static_cast<int64_t>(16 / element)), 256));
+    kernel.block = dim3(256);
+    kernel.set_args(PadArgs{source, target, rows, width, ld, length});
+    return launch(kernel, stream);
+  }
+
+  hipError_t clear(void *target, size_t bytes) const {
+    const int64_t words = static_cast<int64_t>(bytes / 2);
+    clear_kernel<<<std::min(blocks_of(words, 256), 4096u), 256, 0, stream>>>(static_cast<uint16_t *>(target), words);
+    return hipGetLastError();
+  }
+
+  hipError_t band_sums(ColumnSumArgs args) const {
+    KernelLaunch kernel;
+    kernel.func = reinterpret_cast<const void *>(&band_sum_kernel);
+    kernel.grid = dim3(blocks_of(args.n, 64));
+    kernel.block = dim3(64);
+    kernel.set_args(args);
+    return launch(kernel, stream);
+  }
+
+  hipError_t column_sums(const void *source, int64_t rows, int64_t n, int64_t ld, float *bands, float *out, bool accumulate) const;
+};
+
+// Bands of a column sum: enough workgroups for the chip, at least 16 rows each.
+int64_t column_sum_bands(int64_t rows) { return std::min<int64_t>((rows + 15) / 16, 64); }
+
+hipError_t Caller::column_sums(const void *source, int64_t rows, int64_t n, int64_t ld, float *bands, float *out,
+                               bool accumulate) const {
+  ColumnSumArgs args{source, bands, out, rows, n, ld, 0, 0, accumulate};
+  const int64_t wanted = column_sum_bands(rows);
+  args.band_rows = (rows + wanted - 1) / wanted;
+  args.band_count = (rows + args.band_rows - 1) / args.band_rows;
+  KernelLaunch kernel;
+  kernel.func = dtype == kDtypeF32   ? reinterpret_cast<const void *>(&column_sum_kernel<F32Payload>)
+                : dtype == kDtypeF16 ? reinterpret_cast<const void *>(&column_sum_kernel<F16Payload>)
+                                     : reinterpret_cast<const void *>(&column_sum_kernel<Bf16Payload>);
+  kernel.grid = dim3(blocks_of(n, 256 * static_cast<int64_t>(16 / element)), static_cast<unsigned>(args.band_count));
+  kernel.block = dim3(256);
+  kernel.set_args(args);
+  if (const hipError_t status = launch(kernel, stream); status != hipSuccess) {
+    return status;
+  }
+  return band_sums(args);
+}
+
+// out (+)= sum over rows t of a[t][i] b[t][j]: a weight's gradient.
+ProductArgs outer_args(const ProductOperand &a, int64_t m, const ProductOperand &b, int64_t n, int64_t rows, void *out,
+                       int out_dtype, bool accumulate) {
+  ProductArgs args{};
+  args.a = a;
+  args.b = b;
+  args.m = m;
+  args.n = n;
+  args.k = rows;
+  args.out = out;
+  args.ld_out = n;
+  args.base = out;
+  args.ld_base = n;
+  args.out_dtype = args.base_dtype = static_cast<int8_t>(out_dtype);
+  args.alpha = 1.0f;
+  args.beta = accumulate ? 1.0f : 0.0f;
+  return args;
+}
+
+// out = a w: the gradient of a projection's inputs.
+ProductArgs inputs_args(const ProductOperand &a, const ProductOperand &w, int64_t rows, int64_t n, int64_t k, void *out,
+                        int64_t ld_out, int dtype) {
+  ProductArgs args{};
+  args.a = a;
+  args.b = w;
+  args.m = rows;
+  args.n = k;
+  args.k = n;
+  args.out = out;
+  args.ld_out = ld_out;
+  args.out_dtype = static_cast<int8_t>(dtype);
+  args.alpha = 1.0f;
+  return args;
+}
+
+// ------------------------------------------------------------------ workspaces
+struct ProjectionRegions {
+  void *x;
+  void *w;
+  void *grad;
+  float *bands;
+  float *scratch;
+  size_t scratch_bytes;
+  size_t bytes;
+};
+
+ProjectionRegions projection_regions(unsigned char *base, int64_t rows, int64_t n, int64_t k, size_t element) {
+  Regions regions{base};
+  ProjectionRegions found{};
+  const size_t padded_k = static_cast<size_t>(padded_width(k, element)) * element;
+  if (!whole_rows(k, element)) {
+    found.x = regions.take(static_cast<size_t>(rows) * padded_k);
+    found.w = regions.take(static_cast<size_t>(n) * padded_k);
+  }
+  if (!whole_rows(n, element)) {
+    found.grad = regions.take(static_cast<size_t>(rows * padded_width(n, element)) * element);
+  }
+  found.bands = static_cast<float *>(regions.take(static_cast<size_t>(column_sum_bands(rows) * n) * 4));
+  found.scratch_bytes = scratch_upto(rows, [&](int64_t live) {
+    return std::max(unlimited_scratch(live, k, n, static_cast<int>(element)),
+                    unlimited_scratch(n, k, live, static_cast<int>(element)));
+  });
+  found.scratch = static_cast<float *>(regions.take(found.scratch_bytes));
+  found.bytes = regions.used;
+  return found;
+}
+
+struct KeepRegions {
+  void *x;
+  void *w;
+  float *scratch;
+  size_t scratch_bytes;
+  size_t bytes;
+};
+
+KeepRegions keep_regions(unsigned char *base, int64_t rows, int64_t n, int64_t k, size_t element) {
+  Regions regions{base};
+  KeepRegions found{};
+  const size_t padded_k = static_cast<size_t>(padded_width(k, element)) * element;
+  if (!whole_rows(k, element)) {
+    found.x = regions.take(static_cast<size_t>(rows) * padded_k);
+    found.w = regions.take(static_cast<size_t>(n) * padded_k);
+  }
+  found.scratch_bytes =
+      scratch_upto(rows, [&](int64_t live) { return unlimited_scratch(live, n, k, static_cast<int>(element)); });
+  found.scratch = static_cast<float *>(regions.take(found.scratch_bytes));
+  found.bytes = regions.used;
+  return found;
+}
+
+struct DenseRegions {
+  void *x;
+  void *w_in;
+  void *w_out;
+  void *grad;
+  void *through;    // [rows, wide padded]: the projection's gradient
+  void *activated;  // [rows, width padded]
+  float *bands;
+  float *scratch;
+  size_t scratch_bytes;
+  size_t bytes;
+};
+
+DenseRegions dense_regions(unsigned char *base, int64_t rows, int64_t hidden, int64_t width, int64_t wide, size_t element) {
+  Regions regions{base};
+  DenseRegions found{};
+  const size_t padded_hidden = static_cast<size_t>(padded_width(hidden, element)) * element;
+  const size_t padded_inner = static_cast<size_t>(padded_width(width, element)) * element;
+  if (!whole_rows(hidden, element)) {
+    found.x = regions.take(static_cast<size_t>(rows) * padded_hidden);
+    found.w_in = regions.take(static_cast<size_t>(wide) * padded_hidden);
+    found.grad = regions.take(static_cast<size_t>(rows) * padded_hidden);
+  }
+  if (!whole_rows(width, element)) {
+    found.w_out = regions.take(static_cast<size_t>(hidden) * padded_inner);
+  }
+  found.through = regions.take(static_cast<size_t>(rows * padded_width(wide, element)) * element);
+  found.activated = regions.take(static_cast<size_t>(rows) * padded_inner);
+  found.bands = static_cast<float *>(
+      regions.take(static_cast<size_t>(std::max((rows + 31) / 32 * wide, column_sum_bands(rows) * hidden)) * 4));
+  found.scratch_bytes = scratch_upto(rows, [&](int64_t live) {
+    const int es = static_cast<int>(element);
+    return std::max(std::max(unlimited_scratch(live, width, hidden, es), unlimited_scratch(live, hidden, wide, es)),
+                    std::max(unlimited_scratch(wide, hidden, live, es), unlimited_scratch(hidden, width, live, es)));
+  });
+  found.scratch = static_cast<float *>(regions.take(found.scratch_bytes));
+  found.bytes = regions.used;
+  return found;
+}
+
+bool extents_valid(int64_t rows, int64_t a, int64_t b) {
+  return rows >= 0 && rows <= kMaxRows && a >= 1 && a <= kMaxWidth && b >= 1 && b <= kMaxWidth;
+}
+constexpr const char *kExtents = "training operators take up to 2^24 rows and widths of 1 to 2^20";
+
+// A matrix [rows, width]: non-null, aligned to an element, and where its rows are whole 16-byte chunks and the
+// kernels load it (`loaded`), every row on a 16-byte boundary.
+int check_rows(const char *name, const void *pointer, int64_t ld, int64_t width, size_t element, bool loaded) {
+  XP_REQUIRE(pointer != nullptr && aligned_to(pointer, element), std::string(name) + " must be non-null and aligned to its element size");
+  XP_REQUIRE(ld >= width && ld <= kMaxStride, std::string(name) + " has a row stride below its width or above 2^20");
+  XP_REQUIRE(!loaded || !whole_rows(width, element) || (aligned16(pointer) && whole_rows(ld, element)),
+             std::string(name) + " has rows of whole 16 bytes that do not start on 16-byte boundaries");
+  return XP_OK;
+}
+
+#define XP_TRY(expr)                                  \
+  do {                                                \
+    if (const int xp_status_ = (expr); xp_status_ != XP_OK) { \
+      return xp_status_;                              \
+    }                                                 \
+  } while (0)
+
+int check_weight_gradient(const char *name, const void *pointer, int grad_dtype, int dtype) {
+  XP_REQUIRE(grad_dtype == dtype || grad_dtype == XP_DTYPE_F32, "weight gradients are of the payload dtype or fp32");
+  XP_REQUIRE(aligned_to(pointer, dtype_bytes(grad_dtype)), std::string(name) + " must be aligned to its element size");
+  return XP_OK;
+}
+
+bool apart(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+  for (auto at = written.begin(); at != written.end(); ++at) {
+    for (auto other = at + 1; other != written.end(); ++other) {
+      if (overlaps(*at, *other)) {
+        return false;
+      }
+    }
+    if (touches(*at, read)) {
+      return false;
+    }
+  }
+  return true;
+}
+
+}  // namespace
+
+}  // namespace xp
+
+using namespace xp;
+
+extern "C" {
+
+size_t xp_projection_backward_workspace_bytes(int64_t rows, int64_t n, int64_t k, int dtype) {
+  const size_t element = dtype_bytes(dtype);
+  return element == 0 || !extents_valid(rows, n, k) || rows == 0 ? 0 : projection_regions(nullptr, rows, n, k, element).bytes;
+}
+
+int xp_projection_backward(const void *x, int64_t ld_x, int64_t rows, int64_t k, const void *w, int64_t n, const void *grad_out,
+                           int64_t ld_grad, int dtype, void *grad_x, int64_t ld_grad_x, void *grad_w, int grad_w_dtype,
+                           float *grad_bias, int accumulate, int64_t capacity, void *workspace, size_t workspace_bytes,
+                           xp_stream_t stream) {
+  const size_t element = dtype_bytes(dtype);
+  XP_REQUIRE(element != 0, "payload dtype must be bf16, fp16 or fp32");
+  XP_REQUIRE(extents_valid(rows, n, k) && rows <= capacity && capacity <= kMaxRows, kExtents);
+  XP_REQUIRE(w != nullptr && aligned16(w), "projection weights must be non-null and 16-byte aligned");
+  if (grad_w != nullptr) {
+    XP_TRY(check_weight_gradient("weight gradient", grad_w, grad_w_dtype, dtype));
+  }
+  XP_REQUIRE(aligned_to(grad_bias, 4), "the bias gradient must be 4-byte aligned");
+  const size_t kept = grad_w == nullptr ? 0 : dtype_bytes(grad_w_dtype);
+  Caller call{static_cast<hipStream_t>(stream), dtype, element, nullptr, 0};
+  if (rows == 0) {
+    if (accumulate == 0) {
+      if (grad_w != nullptr) {
+        XP_HIP_CHECK(call.clear(grad_w, static_cast<size_t>(n * k) * kept));
+      }
+      if (grad_bias != nullptr) {
+        XP_HIP_CHECK(call.clear(grad_bias, static_cast<size_t>(n) * 4));
+      }
+    }
+    return XP_OK;
+  }
+  XP_TRY(check_rows("output gradient", grad_out, ld_grad, n, element, true));
+  if (grad_w != nullptr) {
+    XP_TRY(check_rows("projection input", x, ld_x, k, element, true));
+  }
+  if (grad_x != nullptr) {
+    XP_TRY(check_rows("input gradient", grad_x, ld_grad_x, k, element, false));
+  }
+  const ProjectionRegions at = projection_regions(static_cast<unsigned char *>(workspace), capacity, n, k, element);
+  XP_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= at.bytes,
+             "workspace is missing, unaligned or smaller than xp_projection_backward_workspace_bytes");
+  const Span read_x = span_of_rows(grad_w == nullptr ? nullptr : x, ld_x, k, rows, element);
+  const Span read_grad = span_of_rows(grad_out, ld_grad, n, rows, element);
+  const Span read_w = span_of(w, static_cast<size_t>(n * k) * element);
+  XP_REQUIRE(apart({span_of_rows(grad_x, ld_grad_x, k, rows, element), span_of(grad_w, static_cast<size_t>(n * k) * kept),
+                    span_of(grad_bias, static_cast<size_t>(n) * 4), span_of(workspace, at.bytes)},
+                   {read_x, read_grad, read_w}),
+             "gradients and workspace must overlap neither the operands nor each other");
+  call.scratch = at.scratch;
+  call.scratch_bytes = at.scratch_bytes;
+  ProductOperand grad{};
+  XP_HIP_CHECK(call.padded(grad_out, rows, n, ld_grad, at.grad, grad));
+  if (grad_x != nullptr) {
+    ProductOperand weights{};
+    XP_HIP_CHECK(call.padded(w, n, k, k, at.w, weights));
+    ProductArgs args = inputs_args(grad, weights, rows, n, k, grad_x, ld_grad_x, dtype);
+    XP_HIP_CHECK(call.product(args, ProductEpilogue::kStore, false, true));
+  }
+  if (grad_w != nullptr) {
+    ProductOperand inputs{};
+    XP_HIP_CHECK(call.padded(x, rows, k, ld_x, at.x, inputs));
+    ProductArgs args = outer_args(grad, n, inputs, k, rows, grad_w, grad_w_dtype, accumulate != 0);
+    XP_HIP_CHECK(call.product(args, ProductEpilogue::kStore, true, true));
+  }
+  if (grad_bias != nullptr) {
+    XP_HIP_CHECK(call.column_sums(grad_out, rows, n, ld_grad, at.bands, grad_bias, accumulate != 0));
+  }
+  return XP_OK;
+}
+
+size_t xp_projection_keep_workspace_bytes(int64_t rows, int64_t n, int64_t k, int dtype) {
+  const size_t element = dtype_bytes(dtype);
+  return element == 0 || !extents_valid(rows, n, k) || rows == 0 ? 0 : keep_regions(nullptr, rows, n, k, element).bytes;
+}
+
+int xp_projection_keep(const void *x, int64_t ld_x, int64_t rows, int64_t k, const void *w, int64_t n, const float *bias,
+                       void *projected, int64_t ld_projected, void *activated, int dtype, const xp_activation_desc *activation,
+                       int64_t capacity, void *workspace, size_t workspace_bytes, xp_stream_t stream) {
+  const size_t element = dtype_bytes(dtype);
+  XP_REQUIRE(element != 0, "payload dtype must be bf16, fp16 or fp32");
+  XP_REQUIRE(extents_valid(rows, n, k) && rows <= capacity && capacity <= kMaxRows, kExtents);
+  ProductArgs args{};
+  XP_REQUIRE(activated == nullptr || activation != nullptr, "activated outputs need an activation");
+  XP_TRY(activation_record(activation, args.act));
+  XP_REQUIRE(args.act.gated == 0 || n % 2 == 0, "a gated projection needs an even number of weight rows");
+  if (rows == 0) {
+    return XP_OK;
+  }
+  XP_REQUIRE(w != nullptr && aligned16(w), "projection weights must be non-null and 16-byte aligned");
+  XP_TRY(check_rows("projection input", x, ld_x, k, element, true));
+  XP_TRY(check_rows("kept projection", projected, ld_projected, n, element, false));
+  XP_REQUIRE(aligned_to(bias, 4) && aligned_to(activated, element), "bias and activated outputs must be aligned to their element size");
+  const KeepRegions at = keep_regions(static_cast<unsigned char *>(workspace), capacity, n, k, element);
+  XP_REQUIRE(at.bytes == 0 || (workspace != nullptr && aligned16(workspace) && workspace_bytes >= at.bytes),
+             "workspace is missing, unaligned or smaller than xp_projection_keep_workspace_bytes");
+  const int64_t outputs = args.act.gated != 0 ? n / 2 : n;
+  XP_REQUIRE(apart({span_of_rows(projected, ld_projected, n, rows, element),
+                    span_of(activated, activated == nullptr ? 0 : static_cast<size_t>(rows * outputs) * element),
+                    span_of(workspace, at.bytes)},
+                   {span_of_rows(x, ld_x, k, rows, element), span_of(w, static_cast<size_t>(n * k) * element),
+                    span_of(bias, bias == nullptr ? 0 : static_cast<size_t>(n) * 4)}),
+             "outputs and workspace must overlap neither the operands nor each other");
+  const Caller call{static_cast<hipStream_t>(stream), dtype, element, at.scratch, at.scratch_bytes};
+  XP_HIP_CHECK(call.padded(x, rows, k, ld_x, at.x, args.a));
+  XP_HIP_CHECK(call.padded(w, n, k, k, at.w, args.b));
+  args.m = rows;
+  args.n = n;
+  args.k = k;
+  args.out = projected;
+  args.ld_out = ld_projected;
+  args.out_dtype = static_cast<int8_t>(dtype);
+  args.bias = bias;
+  args.alpha = 1.0f;
+  if (activated != nullptr) {
+    args.extra = activated;
+    args.ld_extra = outputs;
+    args.interleaved = 1;
+  }
+  XP_HIP_CHECK(call.product(args, activated != nullptr ? ProductEpilogue::kActivate : ProductEpilogue::kStore, false, false));
+  return XP_OK;
+}
+
+size_t xp_dense_backward_workspace_bytes(int64_t rows, int64_t hidden, int64_t intermediate, int gated, int dtype) {
+  const size_t element = dtype_bytes(dtype);
+  const int64_t wide = gated != 0 ? 2 * intermediate : intermediate;
+  return element == 0 || !extents_valid(rows, hidden, wide) || rows == 0
+             ? 0
+             : dense_regions(nullptr, rows, hidden, intermediate, wide, element).bytes;
+}
+
+int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden, const void *w_in, const void *w_out,
+                      int64_t intermediate, const void *projected, int64_t ld_projected, const void *grad_out, int64_t ld_grad,
+                      int dtype, int order, const xp_activation_desc *activation, void *grad_x, int64_t ld_grad_x, void *grad_w_in,
+                      void *grad_w_out, int grad_w_dtype, float *grad_bias_in, float *grad_bias_out, int accumulate,
+                      int64_t capacity, void *workspace, size_t workspace_bytes, xp_stream_t stream) {
+  const size_t element = dtype_bytes(dtype);
+  XP_REQUIRE(element != 0, "payload dtype must be bf16, fp16 or fp32");
+  XP_REQUIRE(activation != nullptr, "activation descriptor must be non-null");
+  ProductArgs args{};
+  XP_TRY(activation_record(activation, args.act));
+  const bool gated = args.act.gated != 0;
+  XP_REQUIRE(!gated || order == XP_GATE_UP_INTERLEAVED || order == XP_GATE_UP_CONCATENATED,
+             "gated activation requires a Gate/Up order");
+  const int64_t width = intermediate;
+  XP_REQUIRE(width >= 1 && width <= kMaxWidth, kExtents);
+  const int64_t wide = gated ? 2 * width : width;
+  XP_REQUIRE(extents_valid(rows, hidden, wide) && rows <= capacity && capacity <= kMaxRows, kExtents);
+  for (const void *gradient : {grad_w_in, grad_w_out}) {
+    if (gradient != nullptr) {
+      XP_TRY(check_weight_gradient("weight gradient", gradient, grad_w_dtype, dtype));
+    }
+  }
+  XP_REQUIRE(aligned_to(grad_bias_in, 4) && aligned_to(grad_bias_out, 4), "bias gradients must be 4-byte aligned");
+  const size_t kept = grad_w_in == nullptr && grad_w_out == nullptr ? 0 : dtype_bytes(grad_w_dtype);
+  const size_t in_bytes = grad_w_in == nullptr ? 0 : static_cast<size_t>(wide * hidden) * kept;
+  const size_t out_bytes = grad_w_out == nullptr ? 0 : static_cast<size_t>(hidden * width) * kept;
+  Caller call{static_cast<hipStream_t>(stream), dtype, element, nullptr, 0};
+  if (rows == 0) {
+    if (accumulate == 0) {
+      if (grad_w_in != nullptr) {
+        XP_HIP_CHECK(call.clear(grad_w_in, in_bytes));
+      }
+      if (grad_w_out != nullptr) {
+        XP_HIP_CHECK(call.clear(grad_w_out, out_bytes));
+      }
+      if (grad_bias_in != nullptr) {
+        XP_HIP_CHECK(call.clear(grad_bias_in, static_cast<size_t>(wide) * 4));
+      }
+      if (grad_bias_out != nullptr) {
+        XP_HIP_CHECK(call.clear(grad_bias_out, static_cast<size_t>(hidden) * 4));
+      }
+    }
+    return XP_OK;
+  }
+  XP_REQUIRE(w_in != nullptr && w_out != nullptr && aligned16(w_in) && aligned16(w_out),
+             "projection weights must be non-null and 16-byte aligned");
+  XP_TRY(check_rows("kept projection", projected, ld_projected, wide, element, false));
+  XP_TRY(check_rows("output gradient", grad_out, ld_grad, hidden, element, true));
+  if (grad_w_in != nullptr) {
+    XP_TRY(check_rows("hidden states", x, ld_x, hidden, element, true));
+  }
+  if (grad_x != nullptr) {
+    XP_TRY(check_rows("gradient of the hidden states", grad_x, ld_grad_x, hidden, element, false));
+  }
+  const DenseRegions at = dense_regions(static_cast<unsigned char *>(workspace), capacity, hidden, width, wide, element);
+  XP_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= at.bytes,
+             "workspace is missing, unaligned or smaller than xp_dense_backward_workspace_bytes");
+  XP_REQUIRE(apart({span_of_rows(grad_x, ld_grad_x, hidden, rows, element), span_of(grad_w_in, in_bytes),
+                    span_of(grad_w_out, out_bytes), span_of(grad_bias_in, static_cast<size_t>(wide) * 4),
+                    span_of(grad_bias_out, static_cast<size_t>(hidden) * 4), span_of(workspace, at.bytes)},
+                   {span_of_rows(grad_w_in == nullptr ? nullptr : x, ld_x, hidden, rows, element),
+                    span_of_rows(projected, ld_projected, wide, rows, element), span_of_rows(grad_out, ld_grad, hidden, rows, element),
+                    span_of(w_in, static_cast<size_t>(wide * hidden) * element),
+                    span_of(w_out, static_cast<size_t>(hidden * width) * element)}),
+             "gradients and workspace must overlap neither the operands nor each other");
+  call.scratch = at.scratch;
+  call.scratch_bytes = at.scratch_bytes;
+
+  ProductOperand grad{};
+  XP_HIP_CHECK(call.padded(grad_out, rows, hidden, ld_grad, at.grad, grad));
+  const int64_t through_ld = padded_width(wide, element);
+  const ProductOperand through{at.through, through_ld, 0};
+  const ProductOperand activated{at.activated, padded_width(width, element), 0};
+  if (grad_x != nullptr || grad_w_in != nullptr || grad_bias_in != nullptr || grad_w_out != nullptr) {
+    args.a = grad;
+    XP_HIP_CHECK(call.padded(w_out, hidden, width, width, at.w_out, args.b));
+    args.m = rows;
+    args.n = width;
+    args.k = hidden;
+    args.out = at.through;
+    args.ld_out = through_ld;
+    args.base = projected;
+    args.ld_base = ld_projected;
+    args.extra = at.activated;
+    args.ld_extra = activated.ld;
+    args.interleaved = order == XP_GATE_UP_INTERLEAVED;
+    args.column_sums = grad_bias_in != nullptr ? at.bands : nullptr;
+    args.alpha = 1.0f;
+    ProductPlan plan{};
+    XP_HIP_CHECK(call.product(args, ProductEpilogue::kGradient, false, true, &plan));
+    if (grad_bias_in != nullptr) {
+      XP_HIP_CHECK(call.band_sums(ColumnSumArgs{nullptr, at.bands, grad_bias_in, rows, wide, 0, 0, plan.bands, accumulate}));
+    }
+  }
+  if (grad_x != nullptr) {
+    if (through_ld != wide) {
+      const int64_t words = rows * (through_ld - wide) * static_cast<int64_t>(element) / 2;
+      clear_pad_kernel<<<blocks_of(words, 256), 256, 0, call.stream>>>(
+          PadArgs{nullptr, at.through, rows, wide, 0, through_ld}, static_cast<int>(element));
+      XP_HIP_CHECK(hipGetLastError());
+    }
+    ProductOperand weights{};
+    XP_HIP_CHECK(call.padded(w_in, wide, hidden, hidden, at.w_in, weights));
+    ProductArgs product = inputs_args(through, weights, rows, wide, hidden, grad_x, ld_grad_x, dtype);
+    XP_HIP_CHECK(call.product(product, ProductEpilogue::kStore, false, true));
+  }
+  if (grad_w_in != nullptr) {
+    ProductOperand inputs{};
+    XP_HIP_CHECK(call.padded(x, rows, hidden, ld_x, at.x, inputs));
+    ProductArgs product = outer_args(through, wide, inputs, hidden, rows, grad_w_in, grad_w_dtype, accumulate != 0);
+    XP_HIP_CHECK(call.product(product, ProductEpilogue::kStore, true, true));
+  }
+  if (grad_w_out != nullptr) {
+    ProductArgs product = outer_args(grad, hidden, activated, width, rows, grad_w_out, grad_w_dtype, accumulate != 0);
+    XP_HIP_CHECK(call.product(product, ProductEpilogue::kStore, true, true));
+  }
+  if (grad_bias_out != nullptr) {
+    XP_HIP_CHECK(call.column_sums(grad_out, rows, hidden, ld_grad, at.bands, grad_bias_out, accumulate != 0));
+  }
+  return XP_OK;
+}
+
+}  // extern "C"

@@ -80,6 +80,78 @@ __device__ __forceinline__ void clip_keep_nan(float &gate, float &up, float limi
   up = up > limit ? limit : up < -limit ? -limit : up;
 }
 
+// ------------------------------------------------------------------ gradient of the activation
+// f(v) and f'(v) of one activation, in fp32 with the hardware's exp and reciprocal.  f is off by at most
+// 2^-15 of itself, f' by 2^-15 of its two terms' magnitudes (next to its root they cancel, so its relative error
+// has no bound there), against the store's 2^-9 or 2^-12: exponents x are off by a few 2^-24 |x| with |x| < 90.
+// A sigmoid or density below 2^-126 may be 0.  The tails keep this: the sigmoid forms by themselves,
+// 0.5 (1 + tanh(y)) as sigmoid(2 y), and Phi(v) by a form of its own, where 0.5 (1 + erff) cancels (nothing is
+// left of that from v = -5.5) and erfcf takes longer than the memory (4096 rows of 12288 INTERLEAVED bf16 pairs:
+// 106-112 us with it, 88 so; ungated 80 and 46-48).  PRECISE, for fp32 payloads, calls the library's exp and erfc and
+// divides: a few steps of fp32 off.
+enum class Slope : int { Silu = 1, Relu = 2, GeluErf = 3, GeluTanh = 4 };
+
+template <Slope KIND, bool PRECISE = false>
+__device__ __forceinline__ void value_and_slope(float v, float alpha, float &value, float &slope) {
+  if constexpr (PRECISE && KIND != Slope::Relu) {
+    if constexpr (KIND == Slope::GeluErf) {
+      const float share = 0.5f * erfcf(v * -0.7071067811865476f);
+      value = v * share;
+      // Past 16 the density is 0 (and v may be infinite).
+      const float near = fminf(fmaxf(v, -16.0f), 16.0f);
+      slope = share + near * 0.3989422804014327f * expf(-0.5f * near * near);
+    } else if constexpr (KIND == Slope::GeluTanh) {
+      const float near = fminf(fmaxf(v, -16.0f), 16.0f);
+      const float square = near * near;
+      const float twice = 2.0f * 0.7978845608028654f * near * (1.0f + 0.044715f * square);
+      const float share = v != v ? v : 1.0f / (1.0f + expf(-twice));
+      value = v * share;
+      slope = share + near * share * (1.0f - share) * (2.0f * 0.7978845608028654f) * (1.0f + 3.0f * 0.044715f * square);
+    } else {
+      const float share = 1.0f / (1.0f + expf(-alpha * v));
+      value = v * share;
+      const float near = fminf(fmaxf(alpha * v, -128.0f), 128.0f);
+      slope = share * (1.0f + near * (1.0f - share));
+    }
+  } else if constexpr (KIND == Slope::Relu) {
+    value = relu_keep_nan(v);
+    slope = v != v ? v : v > 0.0f ? 1.0f : 0.0f;
+  } else if constexpr (KIND == Slope::GeluErf) {
+    // Phi(-x) = exp(-x^2 / 2) t P(t) for x >= 0, t = 1 / (1 + 0.3 x) (Hastings' form of approximation): it shares
+    // the density's exp.  P has the least largest relative error over 0..16, found by reweighted least squares
+    // against the scaled complementary error function; 2^-21 in fp32.  Past 16 all of it is 0.
+    const float near = v > 16.0f ? 16.0f : v < -16.0f ? -16.0f : v;
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3f * fabsf(near));
+    float ratio = 0.0347050946f;
+    ratio = ratio * t - 0.153187922f;
+    ratio = ratio * t + 0.199489063f;
+    ratio = ratio * t - 0.0474273508f;
+    ratio = ratio * t + 0.125292216f;
+    ratio = ratio * t + 0.100889168f;
+    ratio = ratio * t + 0.120600548f;
+    ratio = ratio * t + 0.119639082f;
+    const float density = __expf(-0.5f * near * near);
+    const float tail = density * t * ratio;
+    const float share = v > 0.0f ? 1.0f - tail : tail;
+    value = v * share;
+    slope = share + near * 0.3989422804014327f * density;
+  } else if constexpr (KIND == Slope::GeluTanh) {
+    // Past 16 the sigmoid is 0 or 1 and its slope 0 (and v^3 may overflow).
+    const float near = fminf(fmaxf(v, -16.0f), 16.0f);
+    const float square = near * near;
+    const float twice = 2.0f * 0.7978845608028654f * near * (1.0f + 0.044715f * square);
+    const float share = v != v ? v : __builtin_amdgcn_rcpf(1.0f + __expf(-twice));
+    value = v * share;
+    slope = share + near * share * (1.0f - share) * (2.0f * 0.7978845608028654f) * (1.0f + 3.0f * 0.044715f * square);
+  } else {
+    const float share = __builtin_amdgcn_rcpf(1.0f + __expf(-alpha * v));
+    value = v * share;
+    // Past 128 one of the two factors is 0 (and alpha v may overflow).
+    const float near = fminf(fmaxf(alpha * v, -128.0f), 128.0f);
+    slope = share * (1.0f + near * (1.0f - share));
+  }
+}
+
 // The fp32 element type beside Bf16Payload / F16Payload: a 16-byte chunk holds 4 columns, and
 // its MFMA step covers 8 (lane half h multiplies columns 4 h + j of both operands at step j).
 struct F32Payload {

@@ -16,6 +16,9 @@ Projections of bf16 payloads with aligned shapes, no bias and either no epilogue
 gated SiLU epilogue over INTERLEAVED rows take ``xp_gemm_down`` / ``xp_gemm_gate_up_silu``;
 every other projection -- fp16 and fp32 payloads, odd K or N, a bias, ReLU / GELU epilogues --
 takes ``xp_projection_split``.
+
+Training (no counterpart in the reference): ``Gemm.backward_into`` and, for a whole layer, ``Dense.run_into`` with
+``projected`` and ``Dense.backward_into``, of plans prepared with ``backward``; ``crosspool_amd.muon`` updates the weights.
 """
 
 from __future__ import annotations
@@ -200,6 +203,7 @@ class GemmPlan:
     fused_activation: Activation | None
     workspace: WorkspaceLayout
     kernel: str  # "gate_up_silu" or "down" (xp_gemm_*) or "projection" (xp_projection_split)
+    backward: bool = False
 
     @classmethod
     def prepare(
@@ -209,9 +213,14 @@ class GemmPlan:
         weight_layout: ProjectionLayout,
         result_layout: TensorLayout,
         activation: Activation | None,
+        backward: bool = False,
     ) -> GemmPlan:
         """Choose the kernel and size its scratch; the fused epilogue keeps the projection
-        rounding to the result dtype (linear.py:42-96)."""
+        rounding to the result dtype (linear.py:42-96).  ``backward``: the scratch of ``backward_into`` too
+        (a projection without an activation)."""
+
+        if backward and activation is not None:
+            raise ValueError("the gradients of a projection with an activation are those of a Dense layer's backward pass")
 
         if len(input_layout.shape) != 2 or len(result_layout.shape) != 2 or len(weight_layout.values.shape) != 2:
             raise ValueError("GEMM input, weights and result must be matrices")
@@ -242,6 +251,12 @@ class GemmPlan:
         else:
             kernel = "projection"
             scratch = _native.library().xp_projection_workspace_bytes(rows, width, hidden, _DTYPE_CODES[dtype])
+        if backward:
+            query = _native.library().xp_projection_backward_workspace_bytes
+            needed = int(query(rows, width, hidden, _DTYPE_CODES.get(dtype, 0)))
+            if needed == 0:
+                raise ValueError("projection gradients take 1 to 2^24 rows, widths of 1 to 2^20 and bf16, fp16 or fp32 payloads")
+            scratch = max(scratch, needed)  # a call of either kind uses it whole
         regions = ((torch.uint8, (scratch,)),) if scratch else ()
         return cls(
             input_layout=input_layout,
@@ -250,7 +265,45 @@ class GemmPlan:
             fused_activation=fused,
             workspace=WorkspaceLayout.from_regions(regions),
             kernel=kernel,
+            backward=backward,
         )
+
+
+def _row_stride(tensor: torch.Tensor, name: str, shape: tuple[int, int], dtype: torch.dtype, index: int) -> int:
+    """The row stride of an operand of a training operator (checked)."""
+
+    if tensor.shape != shape or tensor.dtype is not dtype or tensor.get_device() != index:
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on cuda:{index}")
+    stride, column = tensor.stride()
+    if (column != 1 and shape[1] > 1) or (stride < shape[1] and shape[0] > 1):
+        raise ValueError(f"{name} must have contiguous, separate rows")
+    return stride if shape[0] > 1 else shape[1]
+
+
+def _check_gradient(tensor: torch.Tensor | None, name: str, shape: tuple[int, ...], dtypes: tuple[torch.dtype, ...],
+                    index: int) -> int | None:
+    """The address of a weight's or bias's gradient (checked), or None."""
+
+    if tensor is None:
+        return None
+    if tensor.shape != shape or tensor.dtype not in dtypes or tensor.get_device() != index or not tensor.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of shape {tuple(shape)} on cuda:{index}, {' or '.join(map(str, dtypes))}")
+    return tensor.data_ptr()
+
+
+def _check_projection(projection: ProjectionWeights, layout: ProjectionLayout, name: str, index: int) -> None:
+    """Weights as they were prepared for, on the device of a training operator."""
+
+    values = projection.values
+    if values.shape != layout.values.shape or values.dtype is not layout.values.dtype or values.get_device() != index:
+        raise ValueError(f"{name} weights disagree with the prepared layout")
+    if (projection.bias is None) != (layout.bias is None):
+        raise ValueError(f"{name} bias presence disagrees with the prepared layout")
+
+
+def _require_current(index: int) -> None:
+    if _native.current_device() != index:
+        raise ValueError(f"operands on cuda:{index} need it as the current device")
 
 
 class Gemm:
@@ -299,6 +352,54 @@ class Gemm:
             )
 
 
+    def backward_into(
+        self,
+        inputs: torch.Tensor,
+        grad_output: torch.Tensor,
+        projection: ProjectionWeights,
+        *,
+        grad_inputs: torch.Tensor | None = None,
+        grad_values: torch.Tensor | None = None,
+        grad_bias: torch.Tensor | None = None,
+        accumulate: bool = False,
+    ) -> None:
+        """Gradients of :meth:`run_into` without an activation (no counterpart in the reference), those that are asked for.
+
+        ``grad_inputs`` gets ``grad_output @ values``, ``grad_values`` (of the payload dtype or fp32)
+        ``grad_output.T @ inputs`` and ``grad_bias`` (fp32) the sum of ``grad_output``'s rows; ``accumulate`` adds the last
+        two to what they hold.  Rows may lie any stride apart, but rows of whole 16 bytes on 16-byte boundaries.
+        Without rows the weights' and the bias's gradients are zero.
+        """
+
+        plan = self.plan
+        if not plan.backward:
+            raise ValueError("the GEMM plan was prepared without backward")
+        capacity, hidden = plan.input_layout.shape
+        width = plan.output_layout.shape[1]
+        dtype = plan.input_layout.dtype
+        if grad_output.ndim != 2 or grad_output.shape[0] > capacity:
+            raise ValueError("GEMM output gradient disagrees with the prepared layout")
+        rows = grad_output.shape[0]
+        index = self.scratch.get_device()
+        _check_projection(projection, plan.weight_layout, "GEMM", index)
+        _require_current(index)
+        if grad_bias is not None and plan.weight_layout.bias is None:
+            raise ValueError("a bias gradient of a projection without a bias")
+        ld_grad = _row_stride(grad_output, "output gradient", (rows, width), dtype, index)
+        ld_inputs = _row_stride(inputs, "inputs", (rows, hidden), dtype, index)
+        ld_grad_inputs = hidden
+        if grad_inputs is not None:
+            ld_grad_inputs = _row_stride(grad_inputs, "input gradient", (rows, hidden), dtype, index)
+        values_at = _check_gradient(grad_values, "grad_values", (width, hidden), (dtype, torch.float32), index)
+        bias_at = _check_gradient(grad_bias, "grad_bias", (width,), (torch.float32,), index)
+        _native.call(
+            "xp_projection_backward", inputs.data_ptr(), ld_inputs, rows, hidden, projection.values.data_ptr(), width,
+            grad_output.data_ptr(), ld_grad, _DTYPE_CODES[dtype], None if grad_inputs is None else grad_inputs.data_ptr(),
+            ld_grad_inputs, values_at, _DTYPE_CODES[dtype if grad_values is None else grad_values.dtype], bias_at,
+            int(accumulate), capacity, self.scratch.data_ptr(), self.scratch.numel(), _native.current_stream(index),
+        )
+
+
 @dataclass(frozen=True, slots=True)
 class DenseSignature:
     """Dense operator identity (execution.py:73-95 DenseFfnExecutionSignature): payload
@@ -332,11 +433,27 @@ class DenseAdapterLayout:
 
 
 @dataclass(frozen=True, slots=True)
+class DenseGradients:
+    """Where a Dense layer's backward pass writes the gradients of its weights, each left out where None: values of
+    the payload dtype or fp32 (both the same), biases fp32."""
+
+    i_values: torch.Tensor | None = None
+    o_values: torch.Tensor | None = None
+    i_bias: torch.Tensor | None = None
+    o_bias: torch.Tensor | None = None
+
+    def __post_init__(self) -> None:
+        if self.i_values is not None and self.o_values is not None and self.i_values.dtype is not self.o_values.dtype:
+            raise ValueError("gradients of a Dense layer's values share one dtype")
+
+
+@dataclass(frozen=True, slots=True)
 class DenseExecutionPlan:
     """Two prepared projections and their shared intermediate storage (dense.py:14-52).
 
     With ``adapters`` the layer also takes low-rank adapters by row (``crosspool_amd.adapters``); an i_proj
-    with a pool leaves the activation to the kernel that adds its adapters.
+    with a pool leaves the activation to the kernel that adds its adapters.  With ``backward`` it can be trained:
+    its forward pass keeps the projected values, and ``Dense.backward_into`` gives the gradients.
     """
 
     signature: DenseSignature
@@ -346,11 +463,19 @@ class DenseExecutionPlan:
     adapters: DenseAdapterLayout | None = None
     i_proj_adapter: AdapterPlan | None = None
     o_proj_adapter: AdapterPlan | None = None
+    backward: bool = False
 
     @classmethod
-    def prepare(cls, signature: DenseSignature, *, adapters: DenseAdapterLayout | None = None) -> DenseExecutionPlan:
+    def prepare(
+        cls, signature: DenseSignature, *, adapters: DenseAdapterLayout | None = None, backward: bool = False
+    ) -> DenseExecutionPlan:
         dtype = signature.payload_dtype
         capacity = signature.payload_row_capacity
+        if backward and adapters is not None:
+            raise ValueError("a Dense layer with adapters is trained through Gemm, Adapter and Activation")
+        if (backward and dtype is torch.float32 and signature.activation.gate is not None
+                and signature.i_proj.gate_up_order is not GateUpOrder.INTERLEAVED):
+            raise ValueError("a gated fp32 Dense layer takes INTERLEAVED Gate/Up rows")
         activated = TensorLayout((capacity, signature.local_intermediate_size), dtype)
         adapted = adapters is not None and adapters.i_proj_rank is not None
         apart = signature.activation.fused(order=signature.i_proj.gate_up_order) is None
@@ -389,7 +514,16 @@ class DenseExecutionPlan:
                     )
             # One region serves both: their calls follow one another.
             regions.append((torch.uint8, (max(plan.workspace.nbytes for plan in plans if plan is not None),)))
-        return cls(signature, i_proj, o_proj, WorkspaceLayout.from_regions(tuple(regions)), adapters, *plans)
+        if backward:
+            wide, hidden = signature.i_proj.values.shape
+            code, lib = _DTYPE_CODES.get(dtype, 0), _native.library()
+            needed = int(lib.xp_dense_backward_workspace_bytes(
+                capacity, hidden, signature.local_intermediate_size, int(signature.activation.gate is not None), code))
+            if needed == 0:
+                raise ValueError("a Dense layer's backward pass takes 1 to 2^24 rows, widths of 1 to 2^20 and bf16, fp16 or fp32")
+            needed = max(needed, int(lib.xp_projection_keep_workspace_bytes(capacity, wide, hidden, code)))
+            regions.append((torch.uint8, (needed,)))
+        return cls(signature, i_proj, o_proj, WorkspaceLayout.from_regions(tuple(regions)), adapters, *plans, backward)
 
 
 class Dense:
@@ -399,6 +533,7 @@ class Dense:
         views = list(plan.workspace.views(workspace))
         self.plan = plan
         self.i_adapter = self.o_adapter = None
+        self.training_scratch = views.pop() if plan.backward else None
         if plan.adapters is not None:
             from crosspool_amd.adapters import Adapter
 
@@ -422,8 +557,12 @@ class Dense:
         adapters: DenseAdapterWeights | None = None,
         adapter_ids: torch.Tensor | None = None,
         fault_word: torch.Tensor | None = None,
+        projected: torch.Tensor | None = None,
     ) -> None:
         """Write the complete rank-local partial of ``hidden_states`` into ``output``.
+
+        ``projected`` (of a plan prepared with ``backward``; contiguous ``[rows, i_proj width]`` of the payload dtype)
+        gets the projected values that :meth:`backward_into` reads.
 
         ``adapters`` (of a plan prepared for them) adds the low-rank adapters that ``adapter_ids`` (int32,
         one per row, -1: none) names to each projection; an id outside the pool gives a row of NaN and a
@@ -439,6 +578,9 @@ class Dense:
                 raise ValueError("Dense adapters disagree with the prepared plan")
         elif self.i_adapter is not None and self.plan.signature.payload_dtype is torch.float32:
             raise ValueError("an fp32 Dense layer prepared for i_proj adapters takes them in every call (id -1: none)")
+        if projected is not None:
+            self._run_keeping(hidden_states, layer_weights, output, projected)
+            return
         rows = hidden_states.shape[0]
         projected = self.projected[:rows]
         self.i_proj.run_into(hidden_states, layer_weights.i_proj, output=projected)
@@ -460,3 +602,99 @@ class Dense:
                 activated, adapters.o_proj, adapter_ids=adapter_ids, base=output[:rows], output=output[:rows],
                 fault_word=fault_word,
             )
+
+    def _trained(self, layer_weights: DenseFfnWeights, rows: int) -> int:
+        """The device index of a training call (checked)."""
+
+        signature = self.plan.signature
+        if self.training_scratch is None:
+            raise ValueError("the Dense plan was prepared without backward")
+        if rows > signature.payload_row_capacity:
+            raise ValueError(f"{rows} Dense rows exceed the prepared capacity {signature.payload_row_capacity}")
+        index = self.training_scratch.get_device()
+        _check_projection(layer_weights.i_proj, signature.i_proj, "i_proj", index)
+        _check_projection(layer_weights.o_proj, signature.o_proj, "o_proj", index)
+        _require_current(index)
+        return index
+
+    def _run_keeping(
+        self, hidden_states: torch.Tensor, layer_weights: DenseFfnWeights, output: torch.Tensor, projected: torch.Tensor
+    ) -> None:
+        signature = self.plan.signature
+        if hidden_states.ndim != 2:
+            raise ValueError("hidden states must be a matrix")
+        rows = hidden_states.shape[0]
+        index = self._trained(layer_weights, rows)
+        dtype, hidden, wide = signature.payload_dtype, signature.hidden_size, signature.i_proj.values.shape[0]
+        ld_hidden = _row_stride(hidden_states, "hidden states", (rows, hidden), dtype, index)
+        for name, tensor, shape in (("projected", projected, (rows, wide)), ("output", output, (rows, hidden))):
+            _check_gradient(tensor, name, shape, (dtype,), index)
+        order = signature.i_proj.gate_up_order
+        activated = self.activated[:rows]
+        fused = signature.activation.fused(order=order) is not None
+        bias = layer_weights.i_proj.bias
+        scratch = self.training_scratch
+        desc = signature.activation.descriptor()
+        _native.call(
+            "xp_projection_keep", hidden_states.data_ptr(), ld_hidden, rows, hidden, layer_weights.i_proj.values.data_ptr(),
+            wide, None if bias is None else bias.data_ptr(), projected.data_ptr(), wide,
+            activated.data_ptr() if fused else None, _DTYPE_CODES[dtype], ctypes.byref(desc) if fused else None,
+            signature.payload_row_capacity, scratch.data_ptr(), scratch.numel(), _native.current_stream(index),
+        )
+        if not fused:
+            signature.activation.apply_into(inputs=projected, output=activated, order=order)
+        self.o_proj.run_into(activated, layer_weights.o_proj, output=output)
+
+    def backward_into(
+        self,
+        *,
+        hidden_states: torch.Tensor,
+        layer_weights: DenseFfnWeights,
+        projected: torch.Tensor,
+        grad_output: torch.Tensor,
+        grad_hidden_states: torch.Tensor | None = None,
+        gradients: DenseGradients | None = None,
+        accumulate: bool = False,
+    ) -> None:
+        """Gradients of :meth:`run_into` of the same rows, weights and kept ``projected`` (no counterpart in the reference).
+
+        ``grad_hidden_states`` and what ``gradients`` names are written; ``accumulate`` adds the weights' and biases'
+        gradients to what they hold.  The gradient of the projected values is rounded to the payload dtype between
+        the products, as the activated values are; the biases' gradients sum unrounded values.  Clipped values
+        get no gradient, as in :meth:`Activation.backward_into`.
+        """
+
+        signature = self.plan.signature
+        if grad_output.ndim != 2:
+            raise ValueError("a Dense layer's output gradient must be a matrix")
+        rows = grad_output.shape[0]
+        index = self._trained(layer_weights, rows)
+        dtype, hidden, width = signature.payload_dtype, signature.hidden_size, signature.local_intermediate_size
+        wide = signature.i_proj.values.shape[0]
+        ld_hidden = _row_stride(hidden_states, "hidden states", (rows, hidden), dtype, index)
+        ld_projected = _row_stride(projected, "projected", (rows, wide), dtype, index)
+        ld_grad = _row_stride(grad_output, "output gradient", (rows, hidden), dtype, index)
+        ld_grad_hidden = hidden
+        if grad_hidden_states is not None:
+            ld_grad_hidden = _row_stride(grad_hidden_states, "gradient of the hidden states", (rows, hidden), dtype, index)
+        into = DenseGradients() if gradients is None else gradients
+        for name, bias, projection in (("i_proj", into.i_bias, signature.i_proj), ("o_proj", into.o_bias, signature.o_proj)):
+            if bias is not None and projection.bias is None:
+                raise ValueError(f"a bias gradient of an {name} without a bias")
+        kinds = (dtype, torch.float32)
+        i_values = _check_gradient(into.i_values, "i_proj gradient", (wide, hidden), kinds, index)
+        o_values = _check_gradient(into.o_values, "o_proj gradient", (hidden, width), kinds, index)
+        i_bias = _check_gradient(into.i_bias, "i_proj bias gradient", (wide,), (torch.float32,), index)
+        o_bias = _check_gradient(into.o_bias, "o_proj bias gradient", (hidden,), (torch.float32,), index)
+        kept = into.i_values if into.i_values is not None else into.o_values
+        order = signature.i_proj.gate_up_order
+        scratch = self.training_scratch
+        desc = signature.activation.descriptor()
+        _native.call(
+            "xp_dense_backward", hidden_states.data_ptr(), ld_hidden, rows, hidden, layer_weights.i_proj.values.data_ptr(),
+            layer_weights.o_proj.values.data_ptr(), width, projected.data_ptr(), ld_projected, grad_output.data_ptr(), ld_grad,
+            _DTYPE_CODES[dtype], 0 if order is None else _ORDER_CODES[order], ctypes.byref(desc),
+            None if grad_hidden_states is None else grad_hidden_states.data_ptr(), ld_grad_hidden, i_values, o_values,
+            _DTYPE_CODES[dtype if kept is None else kept.dtype], i_bias, o_bias, int(accumulate),
+            signature.payload_row_capacity, scratch.data_ptr(), scratch.numel(), _native.current_stream(index),
+        )

@@ -561,6 +561,69 @@ int xp_moe_experts(const void *hidden_states, int64_t rows, int64_t hidden, int6
                    float up_offset, int payload_dtype, void *output, void *workspace, size_t workspace_bytes,
                    xp_stream_t stream);
 
+/* ---------------------------------------------------------------- training
+ * Gradients of a projection y = x . w^T + bias (x [rows, k], w [n, k]), of grad_out [rows, n]:
+ *   grad_x [rows, k] = grad_out . w,  grad_w [n, k] = grad_out^T . x,  grad_bias [n] (fp32) = sum of grad_out's rows,
+ * each left out where NULL.  All of dtype (XP_DTYPE_BF16, F16 or F32) but grad_w, of grad_w_dtype: dtype or fp32.
+ * accumulate adds grad_w and grad_bias to what they hold.  ld_x, ld_grad and ld_grad_x are row strides in elements;
+ * w and grad_w are contiguous.  x and grad_out rows of whole 16 bytes must start on 16-byte boundaries, as must w.
+ * Sums are fp32 and have one order: repeated calls give the same bits.  No rows: grad_w and grad_bias are
+ * cleared (accumulate: left).  Outputs and workspace may overlap neither the operands nor each other.
+ * The workspace serves every row count up to `capacity`, the rows that its size was asked for.  No counterpart in the
+ * reference. */
+size_t xp_projection_backward_workspace_bytes(int64_t rows, int64_t n, int64_t k, int dtype);
+int xp_projection_backward(const void *x, int64_t ld_x, int64_t rows, int64_t k, const void *w, int64_t n, const void *grad_out,
+                           int64_t ld_grad, int dtype, void *grad_x, int64_t ld_grad_x, void *grad_w, int grad_w_dtype,
+                           float *grad_bias, int accumulate, int64_t capacity, void *workspace, size_t workspace_bytes,
+                           xp_stream_t stream);
+
+/* A projection whose values before the activation are kept for a backward pass: projected [rows, n] = x . w^T + bias
+ * rounded to dtype, and activated (contiguous [rows, n], gated [rows, n / 2]) = the activation of the rounded values, Gate/Up
+ * INTERLEAVED; activated NULL: the projection alone.  Strides, alignment, workspace and capacity as above. */
+size_t xp_projection_keep_workspace_bytes(int64_t rows, int64_t n, int64_t k, int dtype);
+int xp_projection_keep(const void *x, int64_t ld_x, int64_t rows, int64_t k, const void *w, int64_t n, const float *bias,
+                       void *projected, int64_t ld_projected, void *activated, int dtype, const xp_activation_desc *activation,
+                       int64_t capacity, void *workspace, size_t workspace_bytes, xp_stream_t stream);
+
+/* Backward pass of a layer y = act(projected) . w_out^T + bias_out, projected = x . w_in^T + bias_in as kept by
+ * xp_projection_keep: x [rows, hidden], w_in [2 intermediate (gated) or intermediate, hidden] in the Gate/Up `order`,
+ * w_out [hidden, intermediate], grad_out [rows, hidden].  Writes the gradients that are asked for (not NULL) as
+ * xp_projection_backward does; gradients of the biases sum unrounded values.  The gradient of `projected` is rounded
+ * to dtype where it enters grad_x and grad_w_in, the activated values where they enter grad_w_out.  A value clipped by
+ * the gate transform's limit gets none, as in xp_activation_backward. */
+size_t xp_dense_backward_workspace_bytes(int64_t rows, int64_t hidden, int64_t intermediate, int gated, int dtype);
+int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden, const void *w_in, const void *w_out,
+                      int64_t intermediate, const void *projected, int64_t ld_projected, const void *grad_out, int64_t ld_grad,
+                      int dtype, int order, const xp_activation_desc *activation, void *grad_x, int64_t ld_grad_x, void *grad_w_in,
+                      void *grad_w_out, int grad_w_dtype, float *grad_bias_in, float *grad_bias_out, int accumulate,
+                      int64_t capacity, void *workspace, size_t workspace_bytes, xp_stream_t stream);
+
+/* A batch of matrices: row r of matrix i begins at element i matrix_stride + r row_stride.  Their rows lie apart: matrices
+ * one behind another, or (Gate and Up of an INTERLEAVED i_proj) their rows between one another's. */
+typedef struct {
+  void *data;
+  int64_t matrix_stride;
+  int64_t row_stride;
+} xp_matrices;
+
+/* Orthogonalised updates: every matrix G of `updates` [matrices, rows, columns] (bf16, fp16 or fp32) becomes
+ *   X0 = G / (|G| + eps) (Frobenius), then `steps` times X = a X + (b A + c A A) X with A = X X^T
+ * (a, b, c = 3.4445, -4.7750, 2.0315; on the short side), rounded to dtype.  16-bit dtypes run on fp16 products with fp32
+ * sums, fp32 on fp32 ones.  A matrix with an infinity or NaN becomes all NaN, a zero matrix zero.  The output may be
+ * the updates themselves.  No counterpart in the reference. */
+size_t xp_muon_workspace_bytes(int64_t matrices, int64_t rows, int64_t columns, int dtype);
+int xp_muon_orthogonalize(const xp_matrices *updates, int64_t matrices, int64_t rows, int64_t columns, int dtype, int steps,
+                          float eps, const xp_matrices *output, void *workspace, size_t workspace_bytes, xp_stream_t stream);
+
+/* A step of an optimiser with orthogonal updates: new_momentum = momentum_factor momentum + gradients (fp32),
+ * u = gradients + momentum_factor new_momentum (nesterov) or new_momentum,
+ * new_weights = (1 - learning_rate weight_decay) weights - learning_rate update_scale orthogonal(u), in fp32, rounded to
+ * weights_dtype: that of the gradients (dtype) or fp32.  New momentum and weights may be the old ones themselves. */
+int xp_muon_step(const xp_matrices *weights, const xp_matrices *gradients, const xp_matrices *momentum,
+                 const xp_matrices *new_weights, const xp_matrices *new_momentum, int64_t matrices, int64_t rows, int64_t columns,
+                 int dtype, int weights_dtype, int steps, float eps, float learning_rate, float weight_decay, float momentum_factor,
+                 int nesterov, float update_scale, void *workspace, size_t workspace_bytes, xp_stream_t stream);
+
 /* ---------------------------------------------------------------- MoE layer kind
  * One MoE layer's execution identity: the fields of MoeFfnExecutionSignature
  * (src/xpool/runtime/ffnagent/execution.py:98-123, router signature included) that the
