@@ -205,7 +205,7 @@ MuonRegions muon_regions(unsigned char *base, const MuonShape &shape) {
   found.squares = static_cast<double *>(take(static_cast<size_t>(shape.matrices * found.parts) * sizeof(double)));
   const int es = static_cast<int>(element);
   const auto scratch = [&](int64_t m, int64_t n, int64_t k, bool symmetric) {
-    return product_scratch_bytes(plan_product(m, n, k, shape.matrices, es, symmetric, SIZE_MAX), m, n, shape.matrices);
+    return product_scratch_bytes(plan_product(m, n, k, shape.matrices, es, symmetric, SIZE_MAX));
   };
   found.scratch_bytes = std::max({scratch(s, s, shape.longer(), true), scratch(s, s, s, true),
                                   scratch(shape.rows, shape.columns, s, false)});

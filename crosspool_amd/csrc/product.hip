@@ -7,60 +7,91 @@
 
 namespace xp {
 
-// A product's time in microseconds: a CU's workgroups share its throughput and a workgroup's slabs follow one
-// another at no less than the slab latency; a K split adds the reduction's launch and its sums' traffic.
+// A product's time in microseconds.  A CU's workgroups share its throughput: `slab[i]` is the time of one slab in
+// each of i + 1 workgroups on it (as many as fit), and a tile costs `tile` besides (first loads, epilogue), a split
+// piece `piece` (its sums go out in fp32).  Measured on MI355X with 12 and 48 slabs on 128 to 1024 workgroups, for the
+// three storage orders, whose times differ by less than 10 %.
 namespace {
 struct ProductCost {
-  int tile;
-  double latency;     // us per slab of a workgroup alone on its CU
-  double throughput;  // us per slab and workgroup of a full CU
-  double together;    // workgroups that a CU holds
+  ProductTiles tiles;
+  int together;
+  double slab[3];
+  double tile;
+  double piece;
 };
-constexpr ProductCost kCosts16[] = {{256, 1.55, 1.55, 1}, {128, 0.62, 0.48, 2}, {64, 0.33, 0.17, 5}};
-constexpr ProductCost kCosts32[] = {{256, 7.0, 7.0, 1}, {128, 2.2, 1.9, 2}, {64, 0.9, 0.55, 5}};
-constexpr double kCus = 256.0;
-constexpr double kLaunchUs = 4.0;
-constexpr double kReduceUs = 3.0;
-constexpr double kPartialBytesPerUs = 8e6;
-constexpr int64_t kMaxRanges = 32;
+constexpr ProductCost kCosts16[] = {{ProductTiles::k256, 1, {1.36, 0.0, 0.0}, 9.5, 14.0},
+                                    {ProductTiles::k128Pairs, 2, {0.72, 0.87, 0.0}, 5.0, 6.0},
+                                    {ProductTiles::k128Deep, 1, {0.49, 0.0, 0.0}, 5.0, 6.0},
+                                    {ProductTiles::k64, 3, {0.25, 0.41, 0.57}, 1.5, 2.0}};
+constexpr ProductCost kCosts32[] = {{ProductTiles::k256, 1, {7.45, 0.0, 0.0}, 13.0, 16.0},
+                                    {ProductTiles::k128Pairs, 2, {2.03, 3.8, 0.0}, 7.0, 8.0},
+                                    {ProductTiles::k128Deep, 1, {2.0, 0.0, 0.0}, 7.0, 8.0},
+                                    {ProductTiles::k64, 3, {0.59, 1.02, 1.5}, 2.0, 2.5}};
+constexpr int64_t kCus = 256;
+constexpr double kLaunchUs = 3.5;
+constexpr double kJoinUs = 3.0;
+constexpr double kBytesPerUs = 4e6;
+constexpr int64_t kMinSlabs = 2;  // of a worker
+
+// `groups` workgroups of `slabs` slabs each, all of one kind, on the chip.
+double rounds_us(const ProductCost &cost, int64_t groups, double slabs, double each) {
+  const int64_t full = groups / (kCus * cost.together);
+  const int64_t rest = (groups - full * kCus * cost.together + kCus - 1) / kCus;
+  return static_cast<double>(full) * (slabs * cost.slab[cost.together - 1] + each) +
+         (rest > 0 ? slabs * cost.slab[rest - 1] + each : 0.0);
+}
 }  // namespace
 
-size_t product_scratch_bytes(const ProductPlan &plan, int64_t m, int64_t n, int64_t batch) {
-  return plan.ranges > 1 ? static_cast<size_t>(batch * plan.ranges * m * ((n + 7) / 8 * 8)) * 4 : 0;
+size_t product_scratch_bytes(const ProductPlan &plan) {
+  const size_t size = static_cast<size_t>(tile_size(plan.tiles));
+  return plan.split > 0 ? static_cast<size_t>(plan.workers + plan.split) * size * size * sizeof(float) : 0;
 }
 
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int64_t batch, int element_bytes, bool symmetric, size_t scratch) {
   const int64_t slab = 128 / element_bytes;
   const int64_t slabs = (k + slab - 1) / slab;
   ProductPlan best{};
-  double best_us = -1.0;
+  best.us = -1.0;
   for (const ProductCost &cost : element_bytes == 4 ? kCosts32 : kCosts16) {
-    const int64_t rows = (m + cost.tile - 1) / cost.tile;
-    const int64_t cols = (n + cost.tile - 1) / cost.tile;
+    const int64_t size = tile_size(cost.tiles);
+    const int64_t rows = (m + size - 1) / size;
+    const int64_t cols = (n + size - 1) / size;
     const int64_t tiles = batch * (symmetric ? rows * (rows + 1) / 2 : rows * cols);
-    for (int64_t ranges = 1; ranges <= kMaxRanges; ++ranges) {
-      const int64_t per_range = (slabs + ranges - 1) / ranges;
-      if (ranges > 1 && (per_range < 2 || (ranges - 1) * per_range >= slabs)) {
-        continue;
+    const auto consider = [&](int64_t whole, int64_t workers) {
+      ProductPlan plan{cost.tiles, whole, tiles - whole, workers, kLaunchUs};
+      const int64_t together = plan.split * slabs;
+      if (plan.split > 0 && (workers < plan.split || workers * kMinSlabs > together || product_scratch_bytes(plan) > scratch)) {
+        return;
       }
-      const ProductPlan plan{cost.tile, ranges, ranges > 1 ? per_range * slab : k, 0};
-      const size_t bytes = product_scratch_bytes(plan, m, n, batch);
-      if (bytes > scratch) {
-        continue;
+      if (whole > 0) {
+        plan.us += rounds_us(cost, whole, static_cast<double>(slabs), cost.tile);
       }
-      const double groups = static_cast<double>(tiles * ranges);
-      const double full = std::floor(groups / (kCus * cost.together));
-      const double rest = std::ceil((groups - full * kCus * cost.together) / kCus);
-      const double us = static_cast<double>(per_range) *
-                            (full * cost.together * cost.throughput + (rest > 0.0 ? std::max(cost.latency, rest * cost.throughput) : 0.0)) +
-                        (ranges > 1 ? kReduceUs + 2.0 * static_cast<double>(bytes) / kPartialBytesPerUs : 0.0);
-      if (best_us < 0.0 || us < best_us) {
+      if (plan.split > 0) {
+        // A worker whose run crosses a tile's end stores twice.
+        const double pieces = workers % plan.split == 0 ? 1.0 : 2.0;
+        plan.us += rounds_us(cost, workers, std::ceil(static_cast<double>(together) / static_cast<double>(workers)), cost.piece * pieces) +
+                   kJoinUs + static_cast<double>(product_scratch_bytes(plan)) / kBytesPerUs;
+      }
+      if (best.us < 0.0 || plan.us < best.us) {
         best = plan;
-        best_us = us;
       }
+    };
+    consider(tiles, 0);
+    const int64_t slots = kCus * cost.together;
+    const int64_t full = tiles / slots * slots;
+    if (full == tiles || cost.tiles == ProductTiles::k256) {
+      continue;
+    }
+    const int64_t split = tiles - full;
+    for (int64_t per_cu = 1; per_cu <= cost.together; ++per_cu) {
+      consider(full, kCus * per_cu);
+      // The same number of workers for every tile: none crosses a tile's end.
+      consider(full, kCus * per_cu / split * split);
+    }
+    for (int64_t each = 2; each * split < kCus; ++each) {
+      consider(full, each * split);
     }
   }
-  best.bands = best.ranges > 1 ? (m + 31) / 32 : (m + best.tile / 2 - 1) / (best.tile / 2);
   return best;
 }
 
@@ -68,40 +99,36 @@ ProductLaunch make_product(const ProductArgs &args, const ProductPlan &plan, Pro
                            int dtype) {
   ProductLaunch launches;
   ProductArgs record = args;
-  record.ranges = static_cast<int32_t>(plan.ranges);
-  record.k_slice = plan.k_slice;
-  const int64_t rows = (args.m + plan.tile - 1) / plan.tile;
-  const int64_t cols = (args.n + plan.tile - 1) / plan.tile;
-  const int64_t tiles = (args.symmetric != 0 ? rows * (rows + 1) / 2 : rows * cols) * args.batch * plan.ranges;
-  launches.main.func = dtype == kDtypeF32   ? ProductKernels<F32Payload>::tile(plan.tile, epilogue, a_cols, b_cols)
-                       : dtype == kDtypeF16 ? ProductKernels<F16Payload>::tile(plan.tile, epilogue, a_cols, b_cols)
-                                            : ProductKernels<Bf16Payload>::tile(plan.tile, epilogue, a_cols, b_cols);
-  launches.main.grid = dim3(static_cast<unsigned>(tiles));
-  launches.main.block = dim3(plan.tile == 256 ? 512 : 256);
+  record.whole = static_cast<int32_t>(plan.whole);
+  record.split = static_cast<int32_t>(plan.split);
+  record.workers = static_cast<int32_t>(plan.workers);
+  const int size = tile_size(plan.tiles);
+  launches.main.func = dtype == kDtypeF32   ? ProductKernels<F32Payload>::main(plan.tiles, epilogue, a_cols, b_cols)
+                       : dtype == kDtypeF16 ? ProductKernels<F16Payload>::main(plan.tiles, epilogue, a_cols, b_cols)
+                                            : ProductKernels<Bf16Payload>::main(plan.tiles, epilogue, a_cols, b_cols);
+  launches.main.grid = dim3(static_cast<unsigned>(plan.whole + plan.workers));
+  launches.main.block = dim3(size == 256 ? 512 : 256);
   launches.main.set_args(record);
-  if (plan.ranges > 1) {
-    launches.reduce.func = dtype == kDtypeF32   ? ProductKernels<F32Payload>::reduce(epilogue)
-                           : dtype == kDtypeF16 ? ProductKernels<F16Payload>::reduce(epilogue)
-                                                : ProductKernels<Bf16Payload>::reduce(epilogue);
-    launches.reduce.grid = dim3(static_cast<unsigned>((args.n + 63) / 64), static_cast<unsigned>((args.m + 127) / 128),
-                                static_cast<unsigned>(args.batch));
-    launches.reduce.block = dim3(256);
-    launches.reduce.set_args(record);
+  if (plan.split > 0) {
+    launches.join.func = dtype == kDtypeF32   ? ProductKernels<F32Payload>::join(size, epilogue)
+                         : dtype == kDtypeF16 ? ProductKernels<F16Payload>::join(size, epilogue)
+                                              : ProductKernels<Bf16Payload>::join(size, epilogue);
+    launches.join.grid = dim3(static_cast<unsigned>(plan.split * (size / 64) * (size / 32)));
+    launches.join.block = dim3(256);
+    launches.join.set_args(record);
   }
   return launches;
 }
 
 hipError_t launch_product(const ProductArgs &args, ProductEpilogue epilogue, bool a_cols, bool b_cols, int dtype,
-                          size_t scratch_bytes, hipStream_t stream, ProductPlan *chosen) {
-  const ProductPlan plan = plan_product(args.m, args.n, args.k, args.batch, dtype == kDtypeF32 ? 4 : 2, args.symmetric != 0, scratch_bytes);
-  if (chosen != nullptr) {
-    *chosen = plan;
-  }
+                          size_t scratch_bytes, hipStream_t stream) {
+  const ProductPlan plan =
+      plan_product(args.m, args.n, args.k, args.batch, dtype == kDtypeF32 ? 4 : 2, args.symmetric != 0, scratch_bytes);
   const ProductLaunch launches = make_product(args, plan, epilogue, a_cols, b_cols, dtype);
   if (const hipError_t status = launch(launches.main, stream); status != hipSuccess) {
     return status;
   }
-  return launch(launches.reduce, stream);
+  return launch(launches.join, stream);
 }
 
 }  // namespace xp

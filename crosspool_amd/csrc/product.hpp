@@ -28,8 +28,7 @@ struct ProductArgs {
   int64_t m;
   int64_t n;
   int64_t k;
-  int64_t k_slice;     // columns of one K range
-  float *partials;     // [batch, ranges, m, n rounded up to 8] sums of K ranges, where there are several
+  float *partials;     // [workers + split, tile, tile]: sums of the split tiles' pieces
   void *out;
   int64_t ld_out;
   int64_t batch_out;
@@ -45,8 +44,10 @@ struct ProductArgs {
   float beta;          // 0: base is not read
   float keep;
   float step;
-  int32_t ranges;
   int32_t batch;
+  int32_t whole;       // tiles that one workgroup computes each
+  int32_t split;       // the tiles behind them, shared by
+  int32_t workers;     // as many workgroups
   int8_t out_dtype;
   int8_t base_dtype;
   int8_t extra_dtype;
@@ -57,33 +58,41 @@ struct ProductArgs {
 };
 static_assert(sizeof(ProductArgs) <= 256, "a kernel's argument record");
 
+// Tile sizes, stages of LDS and workgroups that a CU holds.
+enum class ProductTiles : int { k256 = 0, k128Pairs = 1, k128Deep = 2, k64 = 3 };
+constexpr int tile_size(ProductTiles tiles) { return tiles == ProductTiles::k256 ? 256 : tiles == ProductTiles::k64 ? 64 : 128; }
+
 struct ProductPlan {
-  int tile;          // square tiles of 256, 128 or 64
-  int64_t ranges;
-  int64_t k_slice;
-  int64_t bands;     // rows of column_sums
+  ProductTiles tiles;
+  int64_t whole;
+  int64_t split;
+  int64_t workers;
+  double us;  // as modelled
 };
 
-// The fastest tile and K ranges for a product in a workspace of `scratch` bytes for its partial sums.
+// The fastest plan for a product in a workspace of `scratch` bytes for its split tiles' sums.
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int64_t batch, int element_bytes, bool symmetric, size_t scratch);
-size_t product_scratch_bytes(const ProductPlan &plan, int64_t m, int64_t n, int64_t batch);
+size_t product_scratch_bytes(const ProductPlan &plan);
+
+// Rows of a band of ProductArgs::column_sums.
+constexpr int64_t kBandRows = 32;
 
 struct ProductLaunch {
   KernelLaunch main;
-  KernelLaunch reduce;  // empty with one K range
+  KernelLaunch join;  // empty without split tiles
 };
-// `dtype` is that of the operands.  Fills ranges and k_slice of the record from the plan.
+// `dtype` is that of the operands.  Fills whole, split and workers of the record from the plan.
 ProductLaunch make_product(const ProductArgs &args, const ProductPlan &plan, ProductEpilogue epilogue, bool a_cols, bool b_cols,
                            int dtype);
 
-// The product as planned for its sizes; `chosen` gets the plan.
+// The product as planned for its sizes.
 hipError_t launch_product(const ProductArgs &args, ProductEpilogue epilogue, bool a_cols, bool b_cols, int dtype,
-                          size_t scratch_bytes, hipStream_t stream, ProductPlan *chosen = nullptr);
+                          size_t scratch_bytes, hipStream_t stream);
 
 template <class P>
 struct ProductKernels {
-  static const void *tile(int tile, ProductEpilogue epilogue, bool a_cols, bool b_cols);
-  static const void *reduce(ProductEpilogue epilogue);
+  static const void *main(ProductTiles tiles, ProductEpilogue epilogue, bool a_cols, bool b_cols);
+  static const void *join(int tile, ProductEpilogue epilogue);
 };
 
 }  // namespace xp

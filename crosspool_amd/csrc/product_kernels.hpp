@@ -22,6 +22,20 @@ namespace xp {
 namespace {
 
 // ------------------------------------------------------------------ eight values of a row
+// Runtime dtypes are wave-uniform: branches, not selects.
+template <class P>
+__device__ __forceinline__ void widen_chunk(u32x4 chunk, float (&value)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    value[j] = P::widen(j % 2 == 0 ? chunk[j / 2] & 0xffffu : chunk[j / 2] >> 16);
+  }
+}
+template <class P>
+__device__ __forceinline__ u32x4 pack_chunk(const float (&value)[8]) {
+  return u32x4{P::pack2(value[0], value[1]), P::pack2(value[2], value[3]), P::pack2(value[4], value[5]),
+               P::pack2(value[6], value[7])};
+}
+
 __device__ __forceinline__ void load_values(const void *source, int64_t index, int dtype, int count, float (&value)[8]) {
   if (dtype == kDtypeF32) {
     const float *from = static_cast<const float *>(source) + index;
@@ -38,10 +52,10 @@ __device__ __forceinline__ void load_values(const void *source, int64_t index, i
   const uint16_t *from = static_cast<const uint16_t *>(source) + index;
   const unsigned char *bytes = reinterpret_cast<const unsigned char *>(from);
   const u32x4 chunk = count >= 8 ? load16_any(bytes) : load_chunk_tail<Bf16Payload, Bf16Payload>(bytes, count);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t bits = j % 2 == 0 ? chunk[j / 2] & 0xffffu : chunk[j / 2] >> 16;
-    value[j] = dtype == kDtypeF16 ? F16Payload::widen(bits) : Bf16Payload::widen(bits);
+  if (dtype == kDtypeF16) {
+    widen_chunk<F16Payload>(chunk, value);
+  } else {
+    widen_chunk<Bf16Payload>(chunk, value);
   }
 }
 
@@ -62,10 +76,10 @@ __device__ __forceinline__ void store_values(void *target, int64_t index, int dt
   }
   uint16_t *to = static_cast<uint16_t *>(target) + index;
   u32x4 packed;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    packed[j] = dtype == kDtypeF16 ? F16Payload::pack2(value[2 * j], value[2 * j + 1])
-                                   : Bf16Payload::pack2(value[2 * j], value[2 * j + 1]);
+  if (dtype == kDtypeF16) {
+    packed = pack_chunk<F16Payload>(value);
+  } else {
+    packed = pack_chunk<Bf16Payload>(value);
   }
   if (count >= 8) {
     __builtin_memcpy(to, &packed, 16);
@@ -79,32 +93,139 @@ __device__ __forceinline__ void store_values(void *target, int64_t index, int dt
   }
 }
 
-template <class P>
-__device__ __forceinline__ void slope_of(float v, const ActivationArgs &act, float &value, float &slope) {
-  constexpr bool PRECISE = kElementBytes<P> == 4;
+// Calls use with the activation as a compile-time constant (it is the same for the whole launch).
+template <class F>
+__device__ __forceinline__ void with_function(const ActivationArgs &act, F &&use) {
   switch (act.function) {
     case kActivationRelu:
-      value_and_slope<Slope::Relu, PRECISE>(v, act.alpha, value, slope);
+      use(std::integral_constant<Slope, Slope::Relu>{});
       break;
     case kActivationGelu:
       if (act.approximate_tanh) {
-        value_and_slope<Slope::GeluTanh, PRECISE>(v, act.alpha, value, slope);
+        use(std::integral_constant<Slope, Slope::GeluTanh>{});
       } else {
-        value_and_slope<Slope::GeluErf, PRECISE>(v, act.alpha, value, slope);
+        use(std::integral_constant<Slope, Slope::GeluErf>{});
       }
       break;
     default:
-      value_and_slope<Slope::Silu, PRECISE>(v, act.alpha, value, slope);
+      use(std::integral_constant<Slope, Slope::Silu>{});
       break;
   }
 }
 
-// The epilogue of columns col .. col + 7 (those below n) of one row.  `sums` gathers kGradient's gradients by
-// column: [0, 8) of Gate (or of ungated values), [8, 16) of Up.
+// Where eight columns of a row lie: elements from the begin of the output, the base and the extra operand.
+struct ChunkPlace {
+  int64_t out;
+  int64_t base;
+  int64_t extra;
+};
+// Columns of the output, base and extra operands that one column of the sums stands for.
+template <ProductEpilogue EPI>
+__device__ __forceinline__ ChunkPlace chunk_place(const ProductArgs &a, int64_t matrix, int64_t row, int64_t col) {
+  if constexpr (EPI == ProductEpilogue::kStore) {
+    return {matrix * a.batch_out + row * a.ld_out + col, matrix * a.batch_base + row * a.ld_base + col,
+            matrix * a.batch_extra + row * a.ld_extra + col};
+  } else if constexpr (EPI == ProductEpilogue::kActivate) {
+    return {row * a.ld_out + col, 0, row * a.ld_extra + (a.act.gated ? col / 2 : col)};
+  } else {
+    const int64_t wide = a.act.gated && a.interleaved ? 2 * col : col;
+    return {row * a.ld_out + wide, row * a.ld_base + wide, row * a.ld_extra + col};
+  }
+}
+
+// What an epilogue reads beside the sums, as it lies in memory: requested for a whole block of rows before the first of
+// them is used, since a workgroup in its epilogue has no other work to hide that latency under.
 template <class P, ProductEpilogue EPI>
-__device__ __forceinline__ void finish(const ProductArgs &a, int64_t matrix, int64_t row, int64_t col, float (&value)[8],
-                                       float (&sums)[16]) {
+struct Beside {
+  u32x4 base[2];
+  u32x4 extra[2];
+};
+__device__ __forceinline__ void request_values(const void *source, int64_t index, int dtype, int count, u32x4 (&raw)[2]) {
+  if (dtype == kDtypeF32) {
+    const unsigned char *from = reinterpret_cast<const unsigned char *>(static_cast<const float *>(source) + index);
+    if (count >= 8) {
+      raw[0] = load16_any(from);
+      raw[1] = load16_any(from + 16);
+    } else {
+      raw[0] = count >= 4 ? load16_any(from) : load_chunk_tail<F32Payload, F32Payload>(from, count);
+      raw[1] = load_chunk_tail<F32Payload, F32Payload>(from + 16, count - 4);
+    }
+    return;
+  }
+  const unsigned char *from = reinterpret_cast<const unsigned char *>(static_cast<const uint16_t *>(source) + index);
+  raw[0] = count >= 8 ? load16_any(from) : load_chunk_tail<Bf16Payload, Bf16Payload>(from, count);
+}
+__device__ __forceinline__ void take_values(const u32x4 (&raw)[2], int dtype, float (&value)[8]) {
+  if (dtype == kDtypeF32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      value[j] = __uint_as_float(raw[j / 4][j % 4]);
+    }
+  } else if (dtype == kDtypeF16) {
+    widen_chunk<F16Payload>(raw[0], value);
+  } else {
+    widen_chunk<Bf16Payload>(raw[0], value);
+  }
+}
+
+// Four values of a row, as they lie in memory.
+template <class P>
+__device__ __forceinline__ void request_four(const void *source, int64_t index, int count, u32x4 &raw) {
+  if constexpr (kElementBytes<P> == 4) {
+    const unsigned char *from = reinterpret_cast<const unsigned char *>(static_cast<const float *>(source) + index);
+    raw = count >= 4 ? load16_any(from) : load_chunk_tail<P, P>(from, count);
+  } else {
+    const unsigned char *from = reinterpret_cast<const unsigned char *>(static_cast<const uint16_t *>(source) + index);
+    if (count >= 4) {
+      const u32x2 packed = load8_any(from);
+      raw = u32x4{packed[0], packed[1], 0u, 0u};
+    } else {
+      raw = load_chunk_tail<P, P>(from, count);
+    }
+  }
+}
+template <class P>
+__device__ __forceinline__ void take_four(const u32x4 &raw, float (&value)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (kElementBytes<P> == 4) {
+      value[j] = __uint_as_float(raw[j]);
+    } else {
+      value[j] = P::widen(j % 2 == 0 ? raw[j / 2] & 0xffffu : raw[j / 2] >> 16);
+    }
+  }
+}
+
+template <class P, ProductEpilogue EPI>
+__device__ __forceinline__ void request(const ProductArgs &a, const ChunkPlace &at, int64_t col, Beside<P, EPI> &beside) {
+  if constexpr (EPI == ProductEpilogue::kStore) {
+    const int count = a.n - col < 8 ? static_cast<int>(a.n - col) : 8;
+    if (a.beta != 0.0f) {
+      request_values(a.base, at.base, a.base_dtype, count, beside.base);
+    }
+    if (a.extra != nullptr) {
+      request_values(a.extra, at.extra, a.extra_dtype, count, beside.extra);
+    }
+  } else if constexpr (EPI == ProductEpilogue::kGradient) {
+    const int count = a.n - col < 4 ? static_cast<int>(a.n - col) : 4;
+    constexpr int dtype = kDtypeOf<P>;
+    if (a.act.gated != 0 && a.interleaved != 0) {
+      request_values(a.base, at.base, dtype, 2 * count, beside.base);
+    } else {
+      request_four<P>(a.base, at.base, count, beside.base[0]);
+      if (a.act.gated) {
+        request_four<P>(a.base, at.base + a.n, count, beside.base[1]);
+      }
+    }
+  }
+}
+
+// The epilogue (but kGradient's) of columns col .. col + 7, those below n, of one row.
+template <class P, ProductEpilogue EPI>
+__device__ __forceinline__ void finish(const ProductArgs &a, const ChunkPlace &at, int64_t col, const Beside<P, EPI> &beside,
+                                       float (&value)[8]) {
   constexpr int dtype = kDtypeOf<P>;
+  constexpr bool PRECISE = kElementBytes<P> == 4;
   const int count = a.n - col < 8 ? static_cast<int>(a.n - col) : 8;
   if constexpr (EPI == ProductEpilogue::kStore) {
 #pragma unroll
@@ -113,7 +234,7 @@ __device__ __forceinline__ void finish(const ProductArgs &a, int64_t matrix, int
     }
     if (a.beta != 0.0f) {
       float other[8];
-      load_values(a.base, matrix * a.batch_base + row * a.ld_base + col, a.base_dtype, count, other);
+      take_values(beside.base, a.base_dtype, other);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         value[j] += a.beta * other[j];
@@ -127,112 +248,172 @@ __device__ __forceinline__ void finish(const ProductArgs &a, int64_t matrix, int
     }
     if (a.extra != nullptr) {
       float other[8];
-      load_values(a.extra, matrix * a.batch_extra + row * a.ld_extra + col, a.extra_dtype, count, other);
+      take_values(beside.extra, a.extra_dtype, other);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         value[j] = a.keep * other[j] - a.step * value[j];
       }
     }
-    store_values(a.out, matrix * a.batch_out + row * a.ld_out + col, a.out_dtype, a.padded_out ? 8 : count, value);
-  } else if constexpr (EPI == ProductEpilogue::kActivate) {
+    store_values(a.out, at.out, a.out_dtype, a.padded_out ? 8 : count, value);
+  } else {
+    if (a.bias != nullptr) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      value[j] += a.bias != nullptr && j < count ? a.bias[col + j] : 0.0f;
+      for (int j = 0; j < 8; ++j) {
+        value[j] += j < count ? a.bias[col + j] : 0.0f;
+      }
     }
-    store_values(a.out, row * a.ld_out + col, dtype, count, value);
+    store_values(a.out, at.out, dtype, count, value);
+    with_function(a.act, [&](auto kind) XP_INLINE {
+      constexpr Slope KIND = decltype(kind)::value;
+      float unused;
+      if (!a.act.gated) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      value[j] = round_to(value[j], dtype);
-    }
-    if (a.act.gated) {
+        for (int j = 0; j < 8; ++j) {
+          value_and_slope<KIND, PRECISE>(value[j], a.act.alpha, value[j], unused);
+        }
+        return;
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        value[j] = apply_gated(value[2 * j], value[2 * j + 1], a.act);
+        float gate = value[2 * j];
+        float up = value[2 * j + 1];
+        if (a.act.has_limit) {
+          gate = fminf(gate, a.act.limit);
+          up = fminf(fmaxf(up, -a.act.limit), a.act.limit);
+        }
+        float f;
+        value_and_slope<KIND, PRECISE>(gate, a.act.alpha, f, unused);
+        value[j] = f * (up + a.act.up_offset);
       }
-      // n is even: a pair is whole or absent.
-      store_values(a.extra, row * a.ld_extra + col / 2, dtype, count / 2, value);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        value[j] = apply_function(value[j], a.act);
-      }
-      store_values(a.extra, row * a.ld_extra + col, dtype, count, value);
-    }
-  } else {
+    });
     if (!a.act.gated) {
-      float input[8];
-      load_values(a.base, row * a.ld_base + col, dtype, count, input);
-      float activated[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float slope;
-        slope_of<P>(input[j], a.act, activated[j], slope);
-        value[j] *= slope;
-        sums[j] += value[j];
+      store_values(a.extra, at.extra, dtype, count, value);
+    } else if (count == 8) {
+      if constexpr (PRECISE) {
+        __builtin_memcpy(static_cast<float *>(a.extra) + at.extra, value, 16);
+      } else {
+        const u32x2 packed = {P::pack2(value[0], value[1]), P::pack2(value[2], value[3])};
+        __builtin_memcpy(static_cast<uint16_t *>(a.extra) + at.extra, &packed, 8);
       }
-      store_values(a.extra, row * a.ld_extra + col, dtype, count, activated);
-      store_values(a.out, row * a.ld_out + col, dtype, count, value);
+    } else {
+      // n is even: a pair is whole or absent.
+      store_values(a.extra, at.extra, dtype, count / 2, value);
+    }
+  }
+}
+
+// kGradient for columns col .. col + 3: four pairs of INTERLEAVED Gate/Up are one 16-byte chunk of 16-bit values, so
+// that neighbouring lanes read and write neighbouring chunks.  `sums` gathers the gradients by column: [0, 4) of
+// Gate (or of ungated values), [4, 8) of Up.
+template <class P>
+__device__ __forceinline__ void store_four(void *target, int64_t index, int count, const float (&value)[4]) {
+  if constexpr (kElementBytes<P> == 4) {
+    float *to = static_cast<float *>(target) + index;
+    if (count >= 4) {
+      __builtin_memcpy(to, value, 16);
       return;
     }
-    float first[8];   // interleaved: the first four pairs; else Gate
-    float second[8] = {};  // the other four pairs; Up
-    const bool pairs = a.interleaved != 0;
-    const int64_t gate_at = row * a.ld_base + (pairs ? 2 * col : col);
-    const int64_t up_at = gate_at + (pairs ? 8 : a.n);
-    const int gate_count = pairs ? (count >= 4 ? 8 : 2 * count) : count;
-    const int up_count = pairs ? 2 * count - gate_count : count;
-    load_values(a.base, gate_at, dtype, gate_count, first);
-    if (up_count > 0) {
-      load_values(a.base, up_at, dtype, up_count, second);
-    }
-    float activated[8];
-    float grad_ups[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float gate = pairs ? (j < 4 ? first[(2 * j) & 7] : second[(2 * j) & 7]) : first[j];
-      const float up = pairs ? (j < 4 ? first[(2 * j + 1) & 7] : second[(2 * j + 1) & 7]) : second[j];
-      float clipped = gate;
-      float factor = up;
+    for (int j = 0; j < 4; ++j) {
+      if (j < count) {
+        to[j] = value[j];
+      }
+    }
+  } else {
+    uint16_t *to = static_cast<uint16_t *>(target) + index;
+    const u32x2 packed = {P::pack2(value[0], value[1]), P::pack2(value[2], value[3])};
+    if (count >= 4) {
+      __builtin_memcpy(to, &packed, 8);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j < count) {
+        to[j] = static_cast<uint16_t>(packed[j / 2] >> (16 * (j % 2)));
+      }
+    }
+  }
+}
+
+template <class P>
+__device__ __forceinline__ void finish_gradient(const ProductArgs &a, const ChunkPlace &at, int64_t col,
+                                                const Beside<P, ProductEpilogue::kGradient> &beside, const float (&through)[4],
+                                                float (&sums)[8]) {
+  constexpr int dtype = kDtypeOf<P>;
+  constexpr bool PRECISE = kElementBytes<P> == 4;
+  const int count = a.n - col < 4 ? static_cast<int>(a.n - col) : 4;
+  float gate[4];
+  float up[4];
+  const bool pairs = a.act.gated != 0 && a.interleaved != 0;
+  if (pairs) {
+    float both[8];
+    take_values(beside.base, dtype, both);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      gate[j] = both[2 * j];
+      up[j] = both[2 * j + 1];
+    }
+  } else {
+    take_four<P>(beside.base[0], gate);
+    take_four<P>(beside.base[1], up);
+  }
+  float activated[4];
+  with_function(a.act, [&](auto kind) XP_INLINE {
+    constexpr Slope KIND = decltype(kind)::value;
+    if (!a.act.gated) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float slope;
+        value_and_slope<KIND, PRECISE>(gate[j], a.act.alpha, activated[j], slope);
+        gate[j] = through[j] * slope;
+        up[j] = 0.0f;
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float clipped = gate[j];
+      float factor = up[j];
       bool gate_on = true;
       bool up_on = true;
       if (a.act.has_limit) {
         clip_keep_nan(clipped, factor, a.act.limit);
-        gate_on = !(gate > a.act.limit);
-        up_on = !(fabsf(up) > a.act.limit);
+        gate_on = !(gate[j] > a.act.limit);
+        up_on = !(fabsf(up[j]) > a.act.limit);
       }
       float f;
       float slope;
-      slope_of<P>(clipped, a.act, f, slope);
+      value_and_slope<KIND, PRECISE>(clipped, a.act.alpha, f, slope);
       factor += a.act.up_offset;
+      gate[j] = gate_on ? through[j] * slope * factor : 0.0f;
+      up[j] = up_on ? through[j] * f : 0.0f;
       activated[j] = f * factor;
-      const float through = value[j];
-      const float grad_gate = gate_on && j < count ? through * slope * factor : 0.0f;
-      const float grad_up = up_on && j < count ? through * f : 0.0f;
-      sums[j] += grad_gate;
-      sums[8 + j] += grad_up;
-      value[j] = grad_gate;
-      grad_ups[j] = grad_up;
     }
-    store_values(a.extra, row * a.ld_extra + col, dtype, count, activated);
+  });
+  if (a.column_sums != nullptr) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int pair = j / 2;
-      first[j] = pairs ? (j % 2 == 0 ? value[pair] : grad_ups[pair]) : value[j];
-      second[j] = pairs ? (j % 2 == 0 ? value[4 + pair] : grad_ups[4 + pair]) : grad_ups[j];
+    for (int j = 0; j < 4; ++j) {
+      sums[j] += gate[j];
+      sums[4 + j] += up[j];
     }
-    const int64_t to = row * a.ld_out + (pairs ? 2 * col : col);
-    store_values(a.out, to, dtype, gate_count, first);
-    if (up_count > 0) {
-      store_values(a.out, to + (pairs ? 8 : a.n), dtype, up_count, second);
+  }
+  store_four<P>(a.extra, at.extra, count, activated);
+  if (pairs) {
+    const float both[8] = {gate[0], up[0], gate[1], up[1], gate[2], up[2], gate[3], up[3]};
+    store_values(a.out, at.out, dtype, 2 * count, both);
+  } else {
+    store_four<P>(a.out, at.out, count, gate);
+    if (a.act.gated) {
+      store_four<P>(a.out, at.out + a.n, count, up);
     }
   }
 }
 
 // Column sums of a wave's band: lanes with one chunk (lane % LANES) hold parts of the same columns.
 template <int LANES>
-__device__ __forceinline__ void store_column_sums(const ProductArgs &a, int64_t band, int64_t col, float (&sums)[16], int lane) {
+__device__ __forceinline__ void store_column_sums(const ProductArgs &a, int64_t band, int64_t col, float (&sums)[8], int lane) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
+  for (int j = 0; j < 8; ++j) {
 #pragma unroll
     for (int offset = LANES; offset < 64; offset *= 2) {
       sums[j] += __shfl_xor(sums[j], offset, kWave);
@@ -244,16 +425,16 @@ __device__ __forceinline__ void store_column_sums(const ProductArgs &a, int64_t 
   const int64_t wide = a.act.gated ? 2 * a.n : a.n;
   float *to = a.column_sums + band * wide;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 4; ++j) {
     if (col + j < a.n) {
       if (!a.act.gated) {
         to[col + j] = sums[j];
       } else if (a.interleaved) {
         to[2 * (col + j)] = sums[j];
-        to[2 * (col + j) + 1] = sums[8 + j];
+        to[2 * (col + j) + 1] = sums[4 + j];
       } else {
         to[col + j] = sums[j];
-        to[a.n + col + j] = sums[8 + j];
+        to[a.n + col + j] = sums[4 + j];
       }
     }
   }
@@ -271,6 +452,25 @@ __device__ __forceinline__ u32x4 read_chunk(lds_bytes_t at) {
 }
 __device__ __forceinline__ uint32_t read_word(lds_bytes_t at) {
   return *(const __attribute__((address_space(3))) uint32_t *)at;
+}
+
+// Direct global -> LDS load of 16 bytes per lane: lane i's data lands at LDS byte `to` + 16 i; offsets past the
+// resource's `bytes` write zeros.  Written as an instruction because the compiler, which does not know the stages
+// apart, waits for every load in flight before a ds_read_b64_tr (64 x 64 tiles: 0.57 us a slab instead of 0.27).  It
+// has no result in a register; the kernel waits for its arrival itself, before a barrier that is a memory clobber.
+// (One wait state between writing M0 and the load that takes its LDS address from it.)
+__device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t to, uint32_t voffset, uint32_t soffset) {
+  __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                   :
+                   : "s"(to), "v"(voffset), "s"(rsrc), "s"(soffset)
+                   : "m0");
+}
+// The words of a raw buffer resource (make_rsrc), in scalar registers.
+__device__ __forceinline__ u32x4 resource_words(const void *base, uint32_t bytes) {
+  const uint64_t address = reinterpret_cast<uint64_t>(base);
+  return u32x4{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(address))),
+               static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>((address >> 32) & 0xffffu))),
+               static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bytes))), 0x00020000u};
 }
 
 // The loads of one operand's tile of ROWS rows (columns, for COLS) into the stages.
@@ -339,29 +539,40 @@ struct OperandLoads {
     }
   }
 
-  // Slab at column k_pos of a range that ends at k_end into `stage`; a slab past the end loads zeros.
-  __device__ __forceinline__ void issue(int64_t k_pos, int64_t k_end, unsigned char *stage) const {
+  // Load q of the slab at column k_pos of a range that ends at k_end, into the stage at LDS byte `stage`; a slab past
+  // the end loads zeros.
+  struct Slab {
+    u32x4 rsrc;
+    uint32_t k_bytes;
+    int chunks_left;
+  };
+  __device__ __forceinline__ Slab slab(int64_t k_pos, int64_t k_end) const {
+    Slab found;
+    const int64_t left = k_end - k_pos;
     if constexpr (COLS) {
-      const int64_t left = k_end - k_pos;
       const uint32_t rows = left <= 0 ? 0u : left < BK ? static_cast<uint32_t>(left) : static_cast<uint32_t>(BK);
-      const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(origin + (left <= 0 ? 0 : k_pos * static_cast<int64_t>(ld_bytes)), rows * ld_bytes);
-#pragma unroll
-      for (int q = 0; q < LOADS; ++q) {
-        const uint32_t rows_before = static_cast<uint32_t>((first + q) * ROWS_PER_LOAD);
-        buffer_load_lds16(rsrc, stage + (first + q) * 1024, lane_offset[variant(q)] + rows_before * ld_bytes, 0);
-      }
+      found.rsrc = resource_words(origin + k_pos * static_cast<int64_t>(ld_bytes), rows * ld_bytes);
+      found.k_bytes = 0;
+      found.chunks_left = 0;
     } else {
-      const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(origin, span);
-      const uint32_t k_bytes = static_cast<uint32_t>(k_pos * ES);
+      found.rsrc = resource_words(origin, span);
+      found.k_bytes = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(k_pos * ES)));
       // A chunk that the range's end cuts holds zeros past it (the operands' rows are whole chunks).
-      const int64_t chunks_left = (k_end - k_pos + 16 / ES - 1) / (16 / ES);
+      const int64_t limit = left <= 0 ? 0 : left < BK ? left : BK;
+      found.chunks_left = static_cast<int>((limit + 16 / ES - 1) / (16 / ES));
+    }
+    return found;
+  }
+  __device__ __forceinline__ void load(const Slab &from, int q, uint32_t stage) const {
+    const uint32_t to = stage + static_cast<uint32_t>(first + q) * 1024u;
+    if constexpr (COLS) {
+      const uint32_t rows_before = static_cast<uint32_t>((first + q) * ROWS_PER_LOAD);
+      load_lds16(from.rsrc, to, lane_offset[variant(q)] + rows_before * ld_bytes, 0);
+    } else {
       const uint32_t row = static_cast<uint32_t>((threadIdx.x & 63) >> 3);
-#pragma unroll
-      for (int q = 0; q < LOADS; ++q) {
-        const uint32_t chunk = lane_offset[variant(q)];
-        const uint32_t offset = (static_cast<uint32_t>((first + q) * 8) + row) * ld_bytes + chunk * 16;
-        buffer_load_lds16(rsrc, stage + (first + q) * 1024, static_cast<int64_t>(chunk) < chunks_left ? offset : kOutOfRange, k_bytes);
-      }
+      const uint32_t chunk = lane_offset[variant(q)];
+      const uint32_t offset = (static_cast<uint32_t>((first + q) * 8) + row) * ld_bytes + chunk * 16;
+      load_lds16(from.rsrc, to, static_cast<int>(chunk) < from.chunks_left ? offset : kOutOfRange, from.k_bytes);
     }
   }
 };
@@ -425,31 +636,22 @@ struct OperandFragments {
 };
 
 // ------------------------------------------------------------------ tiles of a launch
+// Tile t of all matrices' tiles, in blocks of GROUP tile rows walked column by column, so that neighbouring tiles
+// share the slabs of a few rows and columns.
 struct ProductTile {
   int64_t m;       // tile row
   int64_t n;       // tile column
   int64_t matrix;  // of the batch
-  int64_t range;   // of K
 };
 
-// Workgroups go to the 8 XCDs round robin by their number; XCD c takes one run of consecutive tiles, and a run
-// walks blocks of GROUP tile rows column by column, so that the tiles an XCD works on together share the slabs
-// of a few rows and columns in its L2.
 template <int GROUP>
-__device__ __forceinline__ ProductTile product_tile(const ProductArgs &a, int tile) {
+__device__ __forceinline__ ProductTile product_tile(const ProductArgs &a, int tile, int64_t t) {
   const int64_t rows = (a.m + tile - 1) / tile;
   const int64_t cols = (a.n + tile - 1) / tile;
   const int64_t tiles = a.symmetric ? rows * (rows + 1) / 2 : rows * cols;
-  const uint32_t all = gridDim.x;
-  const uint32_t xcd = blockIdx.x % 8;
-  const uint32_t run = all / 8;
-  const uint32_t more = all % 8;
-  const int64_t t = static_cast<int64_t>(xcd * run + (xcd < more ? xcd : more) + blockIdx.x / 8);
   ProductTile found;
-  const int64_t z = t / tiles;
-  const int64_t within = t - z * tiles;
-  found.matrix = z / a.ranges;
-  found.range = z - found.matrix * a.ranges;
+  found.matrix = t / tiles;
+  const int64_t within = t - found.matrix * tiles;
   if (a.symmetric) {
     int64_t i = static_cast<int64_t>((sqrtf(8.0f * static_cast<float>(within) + 1.0f) - 1.0f) * 0.5f);
     while (i * (i + 1) / 2 > within) {
@@ -470,6 +672,21 @@ __device__ __forceinline__ ProductTile product_tile(const ProductArgs &a, int ti
   return found;
 }
 
+// Workgroups go to the 8 XCDs round robin by their number; XCD c takes one run of consecutive places among `count`,
+// so that the tiles it works on together meet in its L2.
+__device__ __forceinline__ int64_t place_of(uint32_t number, uint32_t count) {
+  const uint32_t xcd = number % 8;
+  const uint32_t more = count % 8;
+  return static_cast<int64_t>(xcd * (count / 8) + (xcd < more ? xcd : more) + number / 8);
+}
+
+// The split tiles' slabs, all in one row, are shared out evenly: worker q takes [split_begin(q), split_begin(q + 1)).
+__device__ __forceinline__ int64_t split_begin(const ProductArgs &a, int64_t slabs_together, int64_t q) {
+  return slabs_together * q / a.workers;
+}
+template <int TILE>
+constexpr int kTileGroup = TILE == 256 ? 4 : 8;
+
 // ------------------------------------------------------------------ tile
 // TILE x TILE tiles, WAVES_M x WAVES_N waves of 32x32 accumulators.  STAGES slabs of both operands live in LDS:
 // while one is multiplied the loads of the next are in flight.  With eight waves only four load (a wave that
@@ -477,7 +694,8 @@ __device__ __forceinline__ ProductTile product_tile(const ProductArgs &a, int ti
 // projections' tile kernel: fragments are read one k step ahead of their MFMAs from two register sets, and the
 // barrier sits where the slab's last fragments have been read.
 template <class P, int TILE, int WAVES_M, int WAVES_N, int STAGES, bool A_COLS, bool B_COLS, ProductEpilogue EPI>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(ProductArgs a) {
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 128 && STAGES > 2 ? 1 : 2) void product_kernel(
+    ProductArgs a) {
   constexpr int ES = kElementBytes<P>;
   constexpr int BK = 128 / ES;
   constexpr int WAVES = WAVES_M * WAVES_N;
@@ -498,31 +716,56 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(Product
 
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * REGION];
 
-  const ProductTile at = product_tile<(TILE == 256 ? 4 : 8)>(a, TILE);
-  const int64_t m0 = at.m * TILE;
-  const int64_t n0 = at.n * TILE;
-  const int64_t k_begin = at.range * a.k_slice;
-  const int64_t k_end = a.k - k_begin < a.k_slice ? a.k : k_begin + a.k_slice;
-  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int wm = wave % WAVES_M;
   const int wn = wave / WAVES_M;
   const bool loading_wave = wave < LOAD_WAVES;
 
-  ALoads a_loads;
-  BLoads b_loads;
-  a_loads.setup(static_cast<const unsigned char *>(a.a.data) + at.matrix * a.a.batch * ES, a.a.ld, m0, a.m - m0, wave, lane);
-  b_loads.setup(static_cast<const unsigned char *>(a.b.data) + at.matrix * a.b.batch * ES, a.b.ld, n0, a.n - n0, wave, lane);
+  const int64_t tile_slabs = (a.k + BK - 1) / BK;
+  // Whole tiles first, one a workgroup; then the workers of the split tiles, each with one run of their slabs, the end
+  // of one tile and the begin of the next among them (the host gives a worker at least one slab).
+  constexpr bool SPLITS = TILE != 256;  // what a split saves 256 x 256 tiles goes into their pieces' 256 KB
+  const bool worker = SPLITS && blockIdx.x >= static_cast<uint32_t>(a.whole);
+  const int64_t q = worker ? place_of(blockIdx.x - static_cast<uint32_t>(a.whole), static_cast<uint32_t>(a.workers)) : 0;
+  const int64_t together = static_cast<int64_t>(a.split) * tile_slabs;
+  int64_t next = worker ? split_begin(a, together, q) : 0;
+  const int64_t stop = worker ? split_begin(a, together, q + 1) : tile_slabs;
+  do {
+  // Opaque, here and before the epilogue: what follows from it is computed where it is used, not kept in registers
+  // around the loop (two workgroups of 128 x 128 no longer fit a CU then).
+  int lane = threadIdx.x & 63;
+  __asm__ volatile("" : "+v"(lane));
   OperandFragments<P, TILE, A_COLS, MT, STAGES> a_fragments;
   OperandFragments<P, TILE, B_COLS, NT, STAGES> b_fragments;
   a_fragments.setup(0, wm * MT, lane);
   b_fragments.setup(REGION, wn * NT, lane);
   const lds_bytes_t shared = (lds_bytes_t)lds;
-  // The host makes no empty range: every workgroup runs at least one slab.
-  const int64_t slabs = (k_end - k_begin + BK - 1) / BK;
-  auto issue = [&](int64_t slab, int stage) XP_INLINE {
-    a_loads.issue(k_begin + slab * BK, k_end, lds + stage * STAGE);
-    b_loads.issue(k_begin + slab * BK, k_end, lds + REGION + stage * STAGE);
+  const int64_t local = next / tile_slabs;  // among the split tiles
+  const ProductTile at = product_tile<kTileGroup<TILE>>(
+      a, TILE, worker ? a.whole + local : place_of(blockIdx.x, static_cast<uint32_t>(a.whole)));
+  const int64_t first_slab = next - local * tile_slabs;
+  const int64_t slabs = tile_slabs - first_slab < stop - next ? tile_slabs - first_slab : stop - next;
+  next += slabs;
+  const int64_t m0 = at.m * TILE;
+  const int64_t n0 = at.n * TILE;
+  const int64_t k_begin = first_slab * BK;
+  const int64_t k_end = a.k - k_begin < slabs * BK ? a.k : k_begin + slabs * BK;
+  ALoads a_loads;
+  BLoads b_loads;
+  a_loads.setup(static_cast<const unsigned char *>(a.a.data) + at.matrix * a.a.batch * ES, a.a.ld, m0, a.m - m0, wave, lane);
+  b_loads.setup(static_cast<const unsigned char *>(a.b.data) + at.matrix * a.b.batch * ES, a.b.ld, n0, a.n - n0, wave, lane);
+  const uint32_t lds_begin = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>((uintptr_t)shared)));
+  auto issue = [&](int64_t number, int stage) XP_INLINE {
+    const typename ALoads::Slab a_slab = a_loads.slab(k_begin + number * BK, k_end);
+    const typename BLoads::Slab b_slab = b_loads.slab(k_begin + number * BK, k_end);
+#pragma unroll
+    for (int q = 0; q < ALoads::LOADS; ++q) {
+      a_loads.load(a_slab, q, lds_begin + stage * STAGE);
+    }
+#pragma unroll
+    for (int q = 0; q < BLoads::LOADS; ++q) {
+      b_loads.load(b_slab, q, lds_begin + REGION + stage * STAGE);
+    }
   };
 
   f32x16 acc[MT][NT];
@@ -536,8 +779,11 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(Product
       }
     }
   }
-  u32x4 af[2][MT];
-  u32x4 bf[2][NT];
+  // Wave tiles of up to four accumulators hold a whole slab's fragments twice: their few MFMAs a k step are shorter than
+  // the LDS latency, so the next slab's are all read under this slab's MFMAs.  Larger ones read one k step ahead.
+  constexpr bool WHOLE_SLABS = MT * NT == 1 || (MT * NT == 4 && STAGES > 2);
+  u32x4 af[WHOLE_SLABS ? 8 : 2][MT];
+  u32x4 bf[WHOLE_SLABS ? 8 : 2][NT];
   auto read_fragments = [&](int stage, int ks, int slot) XP_INLINE {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -575,12 +821,40 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(Product
   }
   wait_vmcnt<LOADS * (STAGES - 1)>();
   __syncthreads();
-  read_fragments(0, 0, 0);
+  auto read_slab = [&](int stage, int set) XP_INLINE {
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      read_fragments(stage, ks, set * 4 + ks);
+    }
+  };
+  auto multiply_slab = [&](int set) XP_INLINE {
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      multiply(set * 4 + ks);
+    }
+  };
+  if constexpr (WHOLE_SLABS) {
+    read_slab(0, 0);
+  } else {
+    read_fragments(0, 0, 0);
+  }
 
+  constexpr int UNROLL = WHOLE_SLABS && STAGES % 2 != 0 ? 2 * STAGES : STAGES;
   auto slab = [&](auto index, auto loads, int64_t number) XP_INLINE {
     constexpr int S = decltype(index)::value % STAGES;
     constexpr int NEXT = (S + 1) % STAGES;
     constexpr bool LOADING = decltype(loads)::value;
+    if constexpr (WHOLE_SLABS) {
+      constexpr int SET = decltype(index)::value % 2;
+      stage_barrier();
+      if constexpr (LOADING) {
+        issue(number + STAGES, S);
+      }
+      read_slab(NEXT, 1 - SET);
+      multiply_slab(SET);
+      __builtin_amdgcn_sched_barrier(0);
+      return;
+    }
     read_fragments(S, 1, 1);
     multiply(0);
     __builtin_amdgcn_sched_barrier(0);
@@ -599,88 +873,126 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(Product
   };
   int64_t number = 0;
   auto main_loop = [&](auto loads) XP_INLINE {
-    for (; number + STAGES < slabs; number += STAGES) {
-      static_for<STAGES>([&](auto j) XP_INLINE { slab(j, loads, number + decltype(j)::value); });
+    for (; number + UNROLL < slabs; number += UNROLL) {
+      static_for<UNROLL>([&](auto j) XP_INLINE { slab(j, loads, number + decltype(j)::value); });
     }
-    static_for<STAGES - 1>([&](auto j) XP_INLINE {
+    static_for<UNROLL - 1>([&](auto j) XP_INLINE {
       if (number + decltype(j)::value + 1 < slabs) {
         slab(j, loads, number + decltype(j)::value);
       }
     });
   };
-  if (loading_wave) {
+  if constexpr (LOAD_WAVES == WAVES) {
+    main_loop(std::true_type{});
+  } else if (loading_wave) {
     main_loop(std::true_type{});
   } else {
     main_loop(std::false_type{});
   }
-  static_for<STAGES>([&](auto j) XP_INLINE {
-    if ((slabs - 1) % STAGES == decltype(j)::value) {
-      constexpr int S = decltype(j)::value;
-      read_fragments(S, 1, 1);
-      multiply(0);
-      read_fragments(S, 2, 0);
-      multiply(1);
-      read_fragments(S, 3, 1);
-      multiply(0);
-      multiply(1);
+  static_for<UNROLL>([&](auto j) XP_INLINE {
+    if ((slabs - 1) % UNROLL == decltype(j)::value) {
+      if constexpr (WHOLE_SLABS) {
+        multiply_slab(decltype(j)::value % 2);
+      } else {
+        constexpr int S = decltype(j)::value % STAGES;
+        read_fragments(S, 1, 1);
+        multiply(0);
+        read_fragments(S, 2, 0);
+        multiply(1);
+        read_fragments(S, 3, 1);
+        multiply(0);
+        multiply(1);
+      }
     }
   });
   // Refills past the end may still be landing in the stages that the epilogue reuses, and other waves reading.
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
+  __asm__ volatile("" : "+v"(lane));
 
-  // 32 rows at a time go through a part of LDS of the wave's own, so that a lane then holds eight neighbouring
+  // 32 rows at a time go through a part of LDS of the wave's own, so that a lane then holds CHUNK neighbouring
   // columns of a row: whole 16-byte loads and stores, 128 contiguous bytes and more of each row.
-  float *rows = reinterpret_cast<float *>(lds) + wave * 32 * PITCH;
-  constexpr int LANES = WTN / 8;        // per row
+  constexpr int CHUNK = EPI == ProductEpilogue::kGradient ? 4 : 8;
+  constexpr int LANES = WTN / CHUNK;    // per row
   constexpr int ROWS_PER_PASS = 64 / LANES;
+  float *rows = reinterpret_cast<float *>(lds) + wave * 32 * PITCH;
   const int64_t row0 = m0 + wm * WTM;
   const int64_t col0 = n0 + wn * WTN;
-  const int64_t pitch_n = (a.n + 7) / 8 * 8;
-  float *partial = a.ranges > 1 ? a.partials + (at.matrix * a.ranges + at.range) * a.m * pitch_n : nullptr;
+  // A worker's sums go to its piece of the tile, [TILE, TILE]: piece q + local, counted along the split tiles' slabs.
+  float *partial = worker ? a.partials + (q + local) * (TILE * TILE) + (wm * WTM) * TILE + wn * WTN : nullptr;
   const bool mirrored = a.symmetric != 0 && at.m != at.n;
-  float sums[16] = {};
-  auto put = [&](int64_t row, int64_t col, float (&value)[8]) XP_INLINE {
-    if (partial != nullptr) {
-      __builtin_memcpy(__builtin_assume_aligned(partial + row * pitch_n + col, 16), value, 32);
-    } else {
-      finish<P, EPI>(a, at.matrix, row, col, value, sums);
-    }
-  };
-#pragma unroll
+  const int chunk = lane % LANES;
+  const int64_t col = col0 + chunk * CHUNK;
+  ChunkPlace place = chunk_place<EPI>(a, at.matrix, row0 + lane / LANES, col);
+  constexpr int PASSES = 32 / ROWS_PER_PASS;
+  constexpr int AHEAD = EPI == ProductEpilogue::kGradient ? PASSES : PASSES < 2 ? PASSES : 2;  // passes whose loads are in flight
+  Beside<P, EPI> beside[AHEAD];
+  // One copy of this code for all blocks: it runs once a tile, and straight-line code of several times the size took
+  // longer to fetch than to run (10 us a tile at 256 x 256).
+#pragma unroll 1
   for (int mt = 0; mt < MT; ++mt) {
     if (row0 + mt * 32 >= a.m) {
       break;
     }
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 four = {acc[mt][nt][4 * q], acc[mt][nt][4 * q + 1], acc[mt][nt][4 * q + 2], acc[mt][nt][4 * q + 3]};
-        *reinterpret_cast<f32x4 *>(rows + (lane & 31) * PITCH + nt * 32 + 8 * q + 4 * (lane >> 5)) = four;
+    [[maybe_unused]] float sums[8] = {};
+    ChunkPlace there = place;
+    auto request_pass = [&](int pass) XP_INLINE {
+      if (partial == nullptr && row0 + mt * 32 + pass * ROWS_PER_PASS + lane / LANES < a.m && col < a.n) {
+        request<P, EPI>(a, there, col, beside[pass % AHEAD]);
       }
+      there.base += ROWS_PER_PASS * a.ld_base;
+      there.extra += ROWS_PER_PASS * a.ld_extra;
+    };
+#pragma unroll
+    for (int pass = 0; pass < AHEAD; ++pass) {
+      request_pass(pass);
     }
     __builtin_amdgcn_wave_barrier();
-    const int chunk = lane % LANES;
-    for (int pass = 0; pass < 32 / ROWS_PER_PASS; ++pass) {
+    static_for<MT>([&](auto block) XP_INLINE {
+      constexpr int B = decltype(block)::value;
+      if (__builtin_amdgcn_readfirstlane(mt) == B) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 four = {acc[B][nt][4 * q], acc[B][nt][4 * q + 1], acc[B][nt][4 * q + 2], acc[B][nt][4 * q + 3]};
+            *reinterpret_cast<f32x4 *>(rows + (lane & 31) * PITCH + nt * 32 + 8 * q + 4 * (lane >> 5)) = four;
+          }
+        }
+      }
+    });
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
       const int row = pass * ROWS_PER_PASS + lane / LANES;
       const int64_t to_row = row0 + mt * 32 + row;
-      const int64_t to_col = col0 + chunk * 8;
-      if (to_row < a.m && to_col < a.n) {
-        float value[8];
-        const f32x4 low = *reinterpret_cast<const f32x4 *>(rows + row * PITCH + chunk * 8);
-        const f32x4 high = *reinterpret_cast<const f32x4 *>(rows + row * PITCH + chunk * 8 + 4);
+      if (to_row < a.m && col < a.n) {
+        float value[CHUNK];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          value[j] = low[j];
-          value[4 + j] = high[j];
+        for (int part = 0; part < CHUNK / 4; ++part) {
+          const f32x4 four = *reinterpret_cast<const f32x4 *>(rows + row * PITCH + chunk * CHUNK + part * 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            value[part * 4 + j] = four[j];
+          }
         }
-        put(to_row, to_col, value);
+        if (partial != nullptr) {
+          __builtin_memcpy(__builtin_assume_aligned(partial + (mt * 32 + row) * TILE + chunk * CHUNK, 16), value, CHUNK * 4);
+        } else if constexpr (EPI == ProductEpilogue::kGradient) {
+          finish_gradient<P>(a, place, col, beside[pass % AHEAD], value, sums);
+        } else {
+          finish<P, EPI>(a, place, col, beside[pass % AHEAD], value);
+        }
       }
+      if (pass + AHEAD < PASSES) {
+        request_pass(pass + AHEAD);
+      }
+      place.out += ROWS_PER_PASS * a.ld_out;
+      place.base += ROWS_PER_PASS * a.ld_base;
+      place.extra += ROWS_PER_PASS * a.ld_extra;
     }
     if constexpr (EPI == ProductEpilogue::kStore) {
-      if (mirrored) {
+      if (mirrored && partial == nullptr) {
         // The tile's transpose: eight rows of a column are eight neighbouring columns there.
         for (int pass = 0; pass < WTN * 4 / 64; ++pass) {
           const int column = (pass * 64 + lane) % WTN;
@@ -693,54 +1005,144 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(Product
             for (int j = 0; j < 8; ++j) {
               value[j] = rows[(group * 8 + j) * PITCH + column];
             }
-            put(to_row, to_col, value);
+            const ChunkPlace across = chunk_place<EPI>(a, at.matrix, to_row, to_col);
+            Beside<P, EPI> beside_it;
+            request<P, EPI>(a, across, to_col, beside_it);
+            finish<P, EPI>(a, across, to_col, beside_it, value);
           }
         }
       }
     }
-  }
-  if constexpr (EPI == ProductEpilogue::kGradient) {
-    if (partial == nullptr && a.column_sums != nullptr && row0 < a.m) {
-      store_column_sums<LANES>(a, at.m * WAVES_M + wm, col0 + (lane % LANES) * 8, sums, lane);
+    if constexpr (EPI == ProductEpilogue::kGradient) {
+      if (partial == nullptr && a.column_sums != nullptr) {
+        store_column_sums<LANES>(a, (row0 + mt * 32) / 32, col, sums, lane);
+      }
     }
   }
+  if constexpr (SPLITS) {
+    __syncthreads();  // the next tile's loads land where the waves staged their rows
+  }
+  } while (SPLITS && next < stop);
 }
 
-// ------------------------------------------------------------------ sum of the K ranges
-// In range order, then the epilogue.  A wave takes 32 rows of 64 columns (a band of the column sums).
-template <class P, ProductEpilogue EPI>
-__global__ __launch_bounds__(256) void product_reduce_kernel(ProductArgs a) {
+// ------------------------------------------------------------------ split tiles
+// The sum of a split tile's pieces in the order of their slabs, then the epilogue.  A workgroup takes 32 rows of 64
+// columns, with the loads of four pieces in flight; the column sums of its band are added through LDS in wave order.
+template <class P, int TILE, ProductEpilogue EPI>
+__global__ __launch_bounds__(256) void product_join_kernel(ProductArgs a) {
+  constexpr int CHUNK = EPI == ProductEpilogue::kGradient ? 4 : 8;
+  constexpr int LANES = 64 / CHUNK;
+  constexpr int ROWS_PER_PASS = 64 / LANES;
+  constexpr int BLOCKS = TILE / 64 * (TILE / 32);  // of a tile
+  constexpr int PITCH = 64 + 1;
+  __shared__ float staged[EPI == ProductEpilogue::kStore ? 32 * PITCH : 4 * 64 * 8];
   const int lane = threadIdx.x & 63;
-  const int64_t band = static_cast<int64_t>(blockIdx.y) * 4 + (threadIdx.x >> 6);
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * 64 + (lane & 7) * 8;
-  const int64_t matrix = blockIdx.z;
-  const int64_t pitch_n = (a.n + 7) / 8 * 8;
-  const int64_t plane = a.m * pitch_n;
-  const float *partial = a.partials + matrix * a.ranges * plane;
-  float sums[16] = {};
-  if (band * 32 >= a.m) {
+  const int wave = threadIdx.x >> 6;
+  const int64_t local = blockIdx.x / BLOCKS;
+  const int block = static_cast<int>(blockIdx.x % BLOCKS);
+  const int row_in = block / (TILE / 64) * 32;
+  const int col_in = block % (TILE / 64) * 64;
+  const ProductTile at = product_tile<kTileGroup<TILE>>(a, TILE, a.whole + local);
+  const int64_t row0 = at.m * TILE + row_in;
+  const int64_t col0 = at.n * TILE + col_in;
+  if (row0 >= a.m || col0 >= a.n) {
     return;
   }
-  for (int pass = 0; pass < 4; ++pass) {
-    const int64_t row = band * 32 + pass * 8 + (lane >> 3);
-    if (row < a.m && col < a.n) {
-      const float *from = partial + row * pitch_n + col;
-      float value[8];
-      __builtin_memcpy(value, __builtin_assume_aligned(from, 16), 32);
-      for (int64_t range = 1; range < a.ranges; ++range) {
-        float more[8];
-        __builtin_memcpy(more, __builtin_assume_aligned(from + range * plane, 16), 32);
+  const int64_t tile_slabs = (a.k + 128 / kElementBytes<P> - 1) / (128 / kElementBytes<P>);
+  const int64_t together = static_cast<int64_t>(a.split) * tile_slabs;
+  // The workers that hold the tile's first and last slab: the last q that begins at or before them.
+  const int64_t first = ((local * tile_slabs + 1) * a.workers - 1) / together;
+  const int64_t last = ((local + 1) * tile_slabs * a.workers - 1) / together;
+  const int64_t col = col0 + (lane % LANES) * CHUNK;
+  const bool mirrored = a.symmetric != 0 && at.m != at.n;
+  [[maybe_unused]] float sums[8] = {};
+  for (int pass = 0; pass < 8 / ROWS_PER_PASS; ++pass) {
+    const int row_at = wave * 8 + pass * ROWS_PER_PASS + lane / LANES;
+    const int64_t row = row0 + row_at;
+    const bool live = row < a.m && col < a.n;
+    float value[CHUNK] = {};
+    if (live) {
+      const ChunkPlace place = chunk_place<EPI>(a, at.matrix, row, col);
+      Beside<P, EPI> beside;
+      request<P, EPI>(a, place, col, beside);
+      const float *from = a.partials + (first + local) * (TILE * TILE) + (row_in + row_at) * TILE + col_in + (lane % LANES) * CHUNK;
+      __builtin_memcpy(value, __builtin_assume_aligned(from, 16), CHUNK * 4);
+      int64_t more = last - first;
+      for (; more >= 4; more -= 4) {
+        float pieces[4][CHUNK];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          value[j] += more[j];
+        for (int i = 0; i < 4; ++i) {
+          from += TILE * TILE;
+          __builtin_memcpy(pieces[i], __builtin_assume_aligned(from, 16), CHUNK * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) {
+            value[j] += pieces[i][j];
+          }
         }
       }
-      finish<P, EPI>(a, matrix, row, col, value, sums);
+      for (; more > 0; --more) {
+        float piece[CHUNK];
+        from += TILE * TILE;
+        __builtin_memcpy(piece, __builtin_assume_aligned(from, 16), CHUNK * 4);
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) {
+          value[j] += piece[j];
+        }
+      }
+      if constexpr (EPI == ProductEpilogue::kStore) {
+        if (mirrored) {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) {
+            staged[row_at * PITCH + (lane % LANES) * CHUNK + j] = value[j];
+          }
+        }
+      }
+      if constexpr (EPI == ProductEpilogue::kGradient) {
+        finish_gradient<P>(a, place, col, beside, value, sums);
+      } else {
+        finish<P, EPI>(a, place, col, beside, value);
+      }
+    }
+  }
+  if constexpr (EPI == ProductEpilogue::kStore) {
+    if (mirrored) {
+      // The block's transpose, one chunk of eight a thread.  (Chunks past the operand's end are not stored.)
+      __syncthreads();
+      const int column = threadIdx.x & 63;
+      const int group = threadIdx.x >> 6;
+      const int64_t to_row = col0 + column;
+      const int64_t to_col = row0 + group * 8;
+      if (to_row < a.n && to_col < a.m) {
+        float value[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          value[j] = to_col + j < a.m ? staged[(group * 8 + j) * PITCH + column] : 0.0f;
+        }
+        const ChunkPlace across = chunk_place<EPI>(a, at.matrix, to_row, to_col);
+        Beside<P, EPI> beside;
+        request<P, EPI>(a, across, to_col, beside);
+        finish<P, EPI>(a, across, to_col, beside, value);
+      }
     }
   }
   if constexpr (EPI == ProductEpilogue::kGradient) {
     if (a.column_sums != nullptr) {
-      store_column_sums<8>(a, band, col, sums, lane);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        staged[wave * 512 + j * 64 + lane] = sums[j];
+      }
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int at_lane = j * 64 + lane;
+          sums[j] = (staged[at_lane] + staged[512 + at_lane]) + (staged[1024 + at_lane] + staged[1536 + at_lane]);
+        }
+        store_column_sums<LANES>(a, row0 / 32, col, sums, lane);
+      }
     }
   }
 }
@@ -767,23 +1169,35 @@ const void *product_tile_kernel(ProductEpilogue epilogue, bool a_cols, bool b_co
   }
 }
 
-template <class P>
-const void *ProductKernels<P>::tile(int tile, ProductEpilogue epilogue, bool a_cols, bool b_cols) {
-  return tile == 256   ? product_tile_kernel<P, 256, 2, 4, 2>(epilogue, a_cols, b_cols)
-         : tile == 128 ? product_tile_kernel<P, 128, 2, 2, 2>(epilogue, a_cols, b_cols)
-                       : product_tile_kernel<P, 64, 2, 2, 2>(epilogue, a_cols, b_cols);
+template <class P, int TILE>
+const void *product_join_for(ProductEpilogue epilogue) {
+  switch (epilogue) {
+    case ProductEpilogue::kActivate:
+      return reinterpret_cast<const void *>(&product_join_kernel<P, TILE, ProductEpilogue::kActivate>);
+    case ProductEpilogue::kGradient:
+      return reinterpret_cast<const void *>(&product_join_kernel<P, TILE, ProductEpilogue::kGradient>);
+    default:
+      return reinterpret_cast<const void *>(&product_join_kernel<P, TILE, ProductEpilogue::kStore>);
+  }
 }
 
 template <class P>
-const void *ProductKernels<P>::reduce(ProductEpilogue epilogue) {
-  switch (epilogue) {
-    case ProductEpilogue::kActivate:
-      return reinterpret_cast<const void *>(&product_reduce_kernel<P, ProductEpilogue::kActivate>);
-    case ProductEpilogue::kGradient:
-      return reinterpret_cast<const void *>(&product_reduce_kernel<P, ProductEpilogue::kGradient>);
+const void *ProductKernels<P>::main(ProductTiles tiles, ProductEpilogue epilogue, bool a_cols, bool b_cols) {
+  switch (tiles) {
+    case ProductTiles::k256:
+      return product_tile_kernel<P, 256, 2, 4, 2>(epilogue, a_cols, b_cols);
+    case ProductTiles::k128Pairs:
+      return product_tile_kernel<P, 128, 2, 2, 2>(epilogue, a_cols, b_cols);
+    case ProductTiles::k128Deep:
+      return product_tile_kernel<P, 128, 2, 2, 4>(epilogue, a_cols, b_cols);
     default:
-      return reinterpret_cast<const void *>(&product_reduce_kernel<P, ProductEpilogue::kStore>);
+      return product_tile_kernel<P, 64, 2, 2, 3>(epilogue, a_cols, b_cols);
   }
+}
+
+template <class P>
+const void *ProductKernels<P>::join(int tile, ProductEpilogue epilogue) {
+  return tile == 256 ? product_join_for<P, 256>(epilogue) : tile == 128 ? product_join_for<P, 128>(epilogue) : product_join_for<P, 64>(epilogue);
 }
 
 }  // namespace xp

@@ -162,7 +162,7 @@ size_t scratch_upto(int64_t capacity, Plan &&plan) {
 }
 
 size_t unlimited_scratch(int64_t m, int64_t n, int64_t k, int element) {
-  return product_scratch_bytes(plan_product(m, n, k, 1, element, false, SIZE_MAX), m, n, 1);
+  return product_scratch_bytes(plan_product(m, n, k, 1, element, false, SIZE_MAX));
 }
 
 // ------------------------------------------------------------------ launches
@@ -173,10 +173,10 @@ struct Caller {
   float *scratch;
   size_t scratch_bytes;
 
-  hipError_t product(ProductArgs &args, ProductEpilogue epilogue, bool a_cols, bool b_cols, ProductPlan *chosen = nullptr) const {
+  hipError_t product(ProductArgs &args, ProductEpilogue epilogue, bool a_cols, bool b_cols) const {
     args.partials = scratch;
     args.batch = 1;
-    return launch_product(args, epilogue, a_cols, b_cols, dtype, scratch_bytes, stream, chosen);
+    return launch_product(args, epilogue, a_cols, b_cols, dtype, scratch_bytes, stream);
   }
 
   // `source` itself where its rows are whole chunks, else a padded copy in `target`.
@@ -355,7 +355,7 @@ DenseRegions dense_regions(unsigned char *base, int64_t rows, int64_t hidden, in
   found.through = regions.take(static_cast<size_t>(rows * padded_width(wide, element)) * element);
   found.activated = regions.take(static_cast<size_t>(rows) * padded_inner);
   found.bands = static_cast<float *>(
-      regions.take(static_cast<size_t>(std::max((rows + 31) / 32 * wide, column_sum_bands(rows) * hidden)) * 4));
+      regions.take(static_cast<size_t>(std::max((rows + kBandRows - 1) / kBandRows * wide, column_sum_bands(rows) * hidden)) * 4));
   found.scratch_bytes = scratch_upto(rows, [&](int64_t live) {
     const int es = static_cast<int>(element);
     return std::max(std::max(unlimited_scratch(live, width, hidden, es), unlimited_scratch(live, hidden, wide, es)),
@@ -633,10 +633,9 @@ int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden,
     args.interleaved = order == XP_GATE_UP_INTERLEAVED;
     args.column_sums = grad_bias_in != nullptr ? at.bands : nullptr;
     args.alpha = 1.0f;
-    ProductPlan plan{};
-    XP_HIP_CHECK(call.product(args, ProductEpilogue::kGradient, false, true, &plan));
+    XP_HIP_CHECK(call.product(args, ProductEpilogue::kGradient, false, true));
     if (grad_bias_in != nullptr) {
-      XP_HIP_CHECK(call.band_sums(ColumnSumArgs{nullptr, at.bands, grad_bias_in, rows, wide, 0, 0, plan.bands, accumulate}));
+      XP_HIP_CHECK(call.band_sums(ColumnSumArgs{nullptr, at.bands, grad_bias_in, rows, wide, 0, 0, (rows + kBandRows - 1) / kBandRows, accumulate}));
     }
   }
   if (grad_x != nullptr) {
