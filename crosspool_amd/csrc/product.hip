@@ -7,38 +7,44 @@
 
 namespace xp {
 
-// A product's time in microseconds.  A CU's workgroups share its throughput: `slab[i]` is the time of one slab in
-// each of i + 1 workgroups on it (as many as fit), and a tile costs `tile` besides (first loads, epilogue), a split
-// piece `piece` (its sums go out in fp32).  Measured on MI355X with 12 and 48 slabs on 128 to 1024 workgroups, for the
-// three storage orders, whose times differ by less than 10 %.
+// A product's time in microseconds.  A CU's workgroups share its throughput: with i + 1 of them on it (as many as fit),
+// a slab in each takes `slab[i]`, and the first loads and the epilogue `around[i]`.  Fitted on MI355X to 1, 4, 12 and 48
+// slabs on 64 to 1536 workgroups; the three storage orders differ by less than 10 %.  Model and measured, us: bf16
+// 4096 x 12288 x 4096 299 / 294, 1000 x 2048 x 12288 63 / 61, fp16 symmetric 4096 x 12288 199 / 200; fp32 700 x 1536 x
+// 1536 40 / 41.
 namespace {
 struct ProductCost {
   ProductTiles tiles;
   int together;
   double slab[3];
-  double tile;
-  double piece;
+  double around[3];
 };
-constexpr ProductCost kCosts16[] = {{ProductTiles::k256, 1, {1.36, 0.0, 0.0}, 9.5, 14.0},
-                                    {ProductTiles::k128Pairs, 2, {0.72, 0.87, 0.0}, 5.0, 6.0},
-                                    {ProductTiles::k128Deep, 1, {0.49, 0.0, 0.0}, 5.0, 6.0},
-                                    {ProductTiles::k64, 3, {0.25, 0.41, 0.57}, 1.5, 2.0}};
-constexpr ProductCost kCosts32[] = {{ProductTiles::k256, 1, {7.45, 0.0, 0.0}, 13.0, 16.0},
-                                    {ProductTiles::k128Pairs, 2, {2.03, 3.8, 0.0}, 7.0, 8.0},
-                                    {ProductTiles::k128Deep, 1, {2.0, 0.0, 0.0}, 7.0, 8.0},
-                                    {ProductTiles::k64, 3, {0.59, 1.02, 1.5}, 2.0, 2.5}};
+constexpr ProductCost kCosts16[] = {{ProductTiles::k256, 1, {1.38, 0.0, 0.0}, {8.2, 0.0, 0.0}},
+                                    {ProductTiles::k128Pairs, 2, {0.73, 0.85, 0.0}, {4.7, 5.9, 0.0}},
+                                    {ProductTiles::k128Deep, 1, {0.5, 0.0, 0.0}, {6.3, 0.0, 0.0}},
+                                    {ProductTiles::k64, 3, {0.245, 0.38, 0.52}, {2.3, 3.0, 3.9}}};
+constexpr ProductCost kCosts32[] = {{ProductTiles::k256, 1, {7.4, 0.0, 0.0}, {14.0, 0.0, 0.0}},
+                                    {ProductTiles::k128Pairs, 2, {1.95, 3.67, 0.0}, {7.0, 7.5, 0.0}},
+                                    {ProductTiles::k128Deep, 1, {2.08, 0.0, 0.0}, {7.0, 0.0, 0.0}},
+                                    {ProductTiles::k64, 3, {0.62, 1.05, 1.49}, {2.4, 3.4, 4.6}}};
 constexpr int64_t kCus = 256;
-constexpr double kLaunchUs = 3.5;
-constexpr double kJoinUs = 3.0;
-constexpr double kBytesPerUs = 4e6;
-constexpr int64_t kMinSlabs = 2;  // of a worker
+constexpr double kLaunchUs = 2.3;
+constexpr double kJoinUs = 3.0;       // its launch,
+constexpr double kPieceUs = 0.25;     // what a piece of a tile adds to its latency,
+constexpr double kBytesPerUs = 4e6;   // and the pieces' way out and back
+constexpr int64_t kMinSlabs = 2;      // of a worker
 
-// `groups` workgroups of `slabs` slabs each, all of one kind, on the chip.
-double rounds_us(const ProductCost &cost, int64_t groups, double slabs, double each) {
+// `groups` workgroups of `slabs` slabs each in `pieces` tiles, all of one kind, on the chip; `apart`: no two of them work
+// on the same slabs, which then come from beyond the L2 caches.
+constexpr double kApartBytesPerUs = 10e6;
+double rounds_us(const ProductCost &cost, int64_t groups, double slabs, double pieces, bool apart) {
   const int64_t full = groups / (kCus * cost.together);
   const int64_t rest = (groups - full * kCus * cost.together + kCus - 1) / kCus;
-  return static_cast<double>(full) * (slabs * cost.slab[cost.together - 1] + each) +
-         (rest > 0 ? slabs * cost.slab[rest - 1] + each : 0.0);
+  const auto round = [&](int64_t count) {
+    const double load = apart ? static_cast<double>(count * kCus * 256 * tile_size(cost.tiles)) / kApartBytesPerUs : 0.0;
+    return slabs * std::max(cost.slab[count - 1], load) + pieces * cost.around[count - 1];
+  };
+  return static_cast<double>(full) * round(cost.together) + (rest > 0 ? round(rest) : 0.0);
 }
 }  // namespace
 
@@ -64,13 +70,16 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int64_t batch, int ele
         return;
       }
       if (whole > 0) {
-        plan.us += rounds_us(cost, whole, static_cast<double>(slabs), cost.tile);
+        plan.us += rounds_us(cost, whole, static_cast<double>(slabs), 1.0, false);
       }
       if (plan.split > 0) {
-        // A worker whose run crosses a tile's end stores twice.
-        const double pieces = workers % plan.split == 0 ? 1.0 : 2.0;
-        plan.us += rounds_us(cost, workers, std::ceil(static_cast<double>(together) / static_cast<double>(workers)), cost.piece * pieces) +
-                   kJoinUs + static_cast<double>(product_scratch_bytes(plan)) / kBytesPerUs;
+        // A worker whose run crosses a tile's end has two pieces.
+        const bool even = workers % plan.split == 0 && together % workers == 0;
+        const double pieces = even ? 1.0 : 1.7;
+        const double each = std::ceil(static_cast<double>(together) / static_cast<double>(workers));
+        plan.us += rounds_us(cost, workers, each, pieces, !even) + kJoinUs +
+                   kPieceUs * static_cast<double>(workers) / static_cast<double>(plan.split) +
+                   static_cast<double>(product_scratch_bytes(plan)) / kBytesPerUs;
       }
       if (best.us < 0.0 || plan.us < best.us) {
         best = plan;
@@ -103,6 +112,15 @@ ProductLaunch make_product(const ProductArgs &args, const ProductPlan &plan, Pro
   record.split = static_cast<int32_t>(plan.split);
   record.workers = static_cast<int32_t>(plan.workers);
   const int size = tile_size(plan.tiles);
+  record.tile_rows = static_cast<int32_t>((args.m + size - 1) / size);
+  record.tile_cols = static_cast<int32_t>((args.n + size - 1) / size);
+  if (plan.split > 0) {
+    const int64_t slab = dtype == kDtypeF32 ? 32 : 64;
+    const int64_t together = plan.split * ((args.k + slab - 1) / slab);
+    record.share = static_cast<int32_t>(together / plan.workers);
+    record.longer = static_cast<int32_t>(together % plan.workers);
+    record.each = together % plan.workers == 0 && plan.workers % plan.split == 0 ? static_cast<int32_t>(plan.workers / plan.split) : 0;
+  }
   launches.main.func = dtype == kDtypeF32   ? ProductKernels<F32Payload>::main(plan.tiles, epilogue, a_cols, b_cols)
                        : dtype == kDtypeF16 ? ProductKernels<F16Payload>::main(plan.tiles, epilogue, a_cols, b_cols)
                                             : ProductKernels<Bf16Payload>::main(plan.tiles, epilogue, a_cols, b_cols);

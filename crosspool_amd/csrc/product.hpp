@@ -45,9 +45,14 @@ struct ProductArgs {
   float keep;
   float step;
   int32_t batch;
+  int32_t tile_rows;   // tiles down and across one matrix
+  int32_t tile_cols;
   int32_t whole;       // tiles that one workgroup computes each
   int32_t split;       // the tiles behind them, shared by
-  int32_t workers;     // as many workgroups
+  int32_t workers;     // as many workgroups,
+  int32_t share;       // `share` slabs each,
+  int32_t longer;      // the first `longer` of them one more
+  int32_t each;        // workers of a tile, where all have the same number
   int8_t out_dtype;
   int8_t base_dtype;
   int8_t extra_dtype;
@@ -56,7 +61,7 @@ struct ProductArgs {
   int8_t interleaved;  // kActivate, kGradient: Gate/Up pairs in neighbouring columns, else in halves
   ActivationArgs act;
 };
-static_assert(sizeof(ProductArgs) <= 256, "a kernel's argument record");
+static_assert(sizeof(ProductArgs) <= 288, "a kernel's argument record");
 
 // Tile sizes, stages of LDS and workgroups that a CU holds.
 enum class ProductTiles : int { k256 = 0, k128Pairs = 1, k128Deep = 2, k64 = 3 };
@@ -81,7 +86,7 @@ struct ProductLaunch {
   KernelLaunch main;
   KernelLaunch join;  // empty without split tiles
 };
-// `dtype` is that of the operands.  Fills whole, split and workers of the record from the plan.
+// `dtype` is that of the operands.  Fills the tiles' and workers' counts of the record from the plan.
 ProductLaunch make_product(const ProductArgs &args, const ProductPlan &plan, ProductEpilogue epilogue, bool a_cols, bool b_cols,
                            int dtype);
 

@@ -639,21 +639,23 @@ struct OperandFragments {
 // Tile t of all matrices' tiles, in blocks of GROUP tile rows walked column by column, so that neighbouring tiles
 // share the slabs of a few rows and columns.
 struct ProductTile {
-  int64_t m;       // tile row
-  int64_t n;       // tile column
-  int64_t matrix;  // of the batch
+  uint32_t m;       // tile row
+  uint32_t n;       // tile column
+  uint32_t matrix;  // of the batch
 };
 
+// (32-bit divisions throughout: a 64-bit one is some hundred instructions, and a small product's workgroups spend as
+// long finding their tile as multiplying it.)
 template <int GROUP>
-__device__ __forceinline__ ProductTile product_tile(const ProductArgs &a, int tile, int64_t t) {
-  const int64_t rows = (a.m + tile - 1) / tile;
-  const int64_t cols = (a.n + tile - 1) / tile;
-  const int64_t tiles = a.symmetric ? rows * (rows + 1) / 2 : rows * cols;
+__device__ __forceinline__ ProductTile product_tile(const ProductArgs &a, uint32_t t) {
+  const uint32_t rows = static_cast<uint32_t>(a.tile_rows);
+  const uint32_t cols = static_cast<uint32_t>(a.tile_cols);
+  const uint32_t tiles = a.symmetric ? rows * (rows + 1) / 2 : rows * cols;
   ProductTile found;
-  found.matrix = t / tiles;
-  const int64_t within = t - found.matrix * tiles;
+  found.matrix = a.batch == 1 ? 0 : t / tiles;
+  const uint32_t within = t - found.matrix * tiles;
   if (a.symmetric) {
-    int64_t i = static_cast<int64_t>((sqrtf(8.0f * static_cast<float>(within) + 1.0f) - 1.0f) * 0.5f);
+    uint32_t i = static_cast<uint32_t>((sqrtf(8.0f * static_cast<float>(within) + 1.0f) - 1.0f) * 0.5f);
     while (i * (i + 1) / 2 > within) {
       --i;
     }
@@ -663,9 +665,9 @@ __device__ __forceinline__ ProductTile product_tile(const ProductArgs &a, int ti
     found.m = i;
     found.n = within - i * (i + 1) / 2;
   } else {
-    const int64_t block = within / (GROUP * cols);
-    const int64_t in_block = within - block * GROUP * cols;
-    const int64_t height = rows - block * GROUP < GROUP ? rows - block * GROUP : GROUP;
+    const uint32_t block = within / (GROUP * cols);
+    const uint32_t in_block = within - block * GROUP * cols;
+    const uint32_t height = rows - block * GROUP < GROUP ? rows - block * GROUP : GROUP;
     found.n = in_block / height;
     found.m = block * GROUP + in_block - found.n * height;
   }
@@ -674,15 +676,24 @@ __device__ __forceinline__ ProductTile product_tile(const ProductArgs &a, int ti
 
 // Workgroups go to the 8 XCDs round robin by their number; XCD c takes one run of consecutive places among `count`,
 // so that the tiles it works on together meet in its L2.
-__device__ __forceinline__ int64_t place_of(uint32_t number, uint32_t count) {
+__device__ __forceinline__ uint32_t place_of(uint32_t number, uint32_t count) {
   const uint32_t xcd = number % 8;
   const uint32_t more = count % 8;
-  return static_cast<int64_t>(xcd * (count / 8) + (xcd < more ? xcd : more) + number / 8);
+  return xcd * (count / 8) + (xcd < more ? xcd : more) + number / 8;
 }
 
-// The split tiles' slabs, all in one row, are shared out evenly: worker q takes [split_begin(q), split_begin(q + 1)).
-__device__ __forceinline__ int64_t split_begin(const ProductArgs &a, int64_t slabs_together, int64_t q) {
-  return slabs_together * q / a.workers;
+// The split tiles' slabs, all in one row, are shared out evenly: worker q takes [split_begin(q), split_begin(q + 1)),
+// `share` slabs, the first `longer` workers one more.
+__device__ __forceinline__ uint32_t split_begin(const ProductArgs &a, uint32_t q) {
+  const uint32_t longer = static_cast<uint32_t>(a.longer);
+  return q * static_cast<uint32_t>(a.share) + (q < longer ? q : longer);
+}
+// The worker that holds slab x.
+__device__ __forceinline__ uint32_t split_worker(const ProductArgs &a, uint32_t x) {
+  const uint32_t share = static_cast<uint32_t>(a.share);
+  const uint32_t longer = static_cast<uint32_t>(a.longer);
+  const uint32_t behind = longer * (share + 1);
+  return x < behind ? x / (share + 1) : longer + (x - behind) / share;
 }
 template <int TILE>
 constexpr int kTileGroup = TILE == 256 ? 4 : 8;
@@ -721,15 +732,20 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 12
   const int wn = wave / WAVES_M;
   const bool loading_wave = wave < LOAD_WAVES;
 
-  const int64_t tile_slabs = (a.k + BK - 1) / BK;
+  const uint32_t tile_slabs = static_cast<uint32_t>((a.k + BK - 1) / BK);
   // Whole tiles first, one a workgroup; then the workers of the split tiles, each with one run of their slabs, the end
   // of one tile and the begin of the next among them (the host gives a worker at least one slab).
   constexpr bool SPLITS = TILE != 256;  // what a split saves 256 x 256 tiles goes into their pieces' 256 KB
-  const bool worker = SPLITS && blockIdx.x >= static_cast<uint32_t>(a.whole);
-  const int64_t q = worker ? place_of(blockIdx.x - static_cast<uint32_t>(a.whole), static_cast<uint32_t>(a.workers)) : 0;
-  const int64_t together = static_cast<int64_t>(a.split) * tile_slabs;
-  int64_t next = worker ? split_begin(a, together, q) : 0;
-  const int64_t stop = worker ? split_begin(a, together, q + 1) : tile_slabs;
+  const uint32_t whole = static_cast<uint32_t>(a.whole);
+  const bool worker = SPLITS && blockIdx.x >= whole;
+  // Where every tile has the same number of workers, those of one part of K come one after another: they share slabs.
+  uint32_t q = worker ? place_of(blockIdx.x - whole, static_cast<uint32_t>(a.workers)) : 0;
+  if (worker && a.each > 1) {
+    const uint32_t part = q / static_cast<uint32_t>(a.split);
+    q = (q - part * static_cast<uint32_t>(a.split)) * static_cast<uint32_t>(a.each) + part;
+  }
+  uint32_t next = worker ? split_begin(a, q) : 0;
+  const uint32_t stop = worker ? split_begin(a, q + 1) : tile_slabs;
   do {
   // Opaque, here and before the epilogue: what follows from it is computed where it is used, not kept in registers
   // around the loop (two workgroups of 128 x 128 no longer fit a CU then).
@@ -740,24 +756,24 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 12
   a_fragments.setup(0, wm * MT, lane);
   b_fragments.setup(REGION, wn * NT, lane);
   const lds_bytes_t shared = (lds_bytes_t)lds;
-  const int64_t local = next / tile_slabs;  // among the split tiles
-  const ProductTile at = product_tile<kTileGroup<TILE>>(
-      a, TILE, worker ? a.whole + local : place_of(blockIdx.x, static_cast<uint32_t>(a.whole)));
-  const int64_t first_slab = next - local * tile_slabs;
-  const int64_t slabs = tile_slabs - first_slab < stop - next ? tile_slabs - first_slab : stop - next;
-  next += slabs;
-  const int64_t m0 = at.m * TILE;
-  const int64_t n0 = at.n * TILE;
-  const int64_t k_begin = first_slab * BK;
-  const int64_t k_end = a.k - k_begin < slabs * BK ? a.k : k_begin + slabs * BK;
+  const uint32_t local = worker ? next / tile_slabs : 0;  // among the split tiles
+  const ProductTile at = product_tile<kTileGroup<TILE>>(a, worker ? whole + local : place_of(blockIdx.x, whole));
+  const uint32_t first_slab = next - local * tile_slabs;
+  const int slabs = static_cast<int>(tile_slabs - first_slab < stop - next ? tile_slabs - first_slab : stop - next);
+  next += static_cast<uint32_t>(slabs);
+  const int64_t m0 = static_cast<int64_t>(at.m) * TILE;
+  const int64_t n0 = static_cast<int64_t>(at.n) * TILE;
+  const int64_t k_begin = static_cast<int64_t>(first_slab) * BK;
+  const int64_t k_end = a.k - k_begin < static_cast<int64_t>(slabs) * BK ? a.k : k_begin + static_cast<int64_t>(slabs) * BK;
   ALoads a_loads;
   BLoads b_loads;
   a_loads.setup(static_cast<const unsigned char *>(a.a.data) + at.matrix * a.a.batch * ES, a.a.ld, m0, a.m - m0, wave, lane);
   b_loads.setup(static_cast<const unsigned char *>(a.b.data) + at.matrix * a.b.batch * ES, a.b.ld, n0, a.n - n0, wave, lane);
   const uint32_t lds_begin = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>((uintptr_t)shared)));
-  auto issue = [&](int64_t number, int stage) XP_INLINE {
-    const typename ALoads::Slab a_slab = a_loads.slab(k_begin + number * BK, k_end);
-    const typename BLoads::Slab b_slab = b_loads.slab(k_begin + number * BK, k_end);
+  auto issue = [&](int number, int stage) XP_INLINE {
+    const int64_t k_pos = k_begin + static_cast<int64_t>(number) * BK;
+    const typename ALoads::Slab a_slab = a_loads.slab(k_pos, k_end);
+    const typename BLoads::Slab b_slab = b_loads.slab(k_pos, k_end);
 #pragma unroll
     for (int q = 0; q < ALoads::LOADS; ++q) {
       a_loads.load(a_slab, q, lds_begin + stage * STAGE);
@@ -840,7 +856,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 12
   }
 
   constexpr int UNROLL = WHOLE_SLABS && STAGES % 2 != 0 ? 2 * STAGES : STAGES;
-  auto slab = [&](auto index, auto loads, int64_t number) XP_INLINE {
+  auto slab = [&](auto index, auto loads, int number) XP_INLINE {
     constexpr int S = decltype(index)::value % STAGES;
     constexpr int NEXT = (S + 1) % STAGES;
     constexpr bool LOADING = decltype(loads)::value;
@@ -871,7 +887,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 12
     multiply(1);
     __builtin_amdgcn_sched_barrier(0);
   };
-  int64_t number = 0;
+  int number = 0;
   auto main_loop = [&](auto loads) XP_INLINE {
     for (; number + UNROLL < slabs; number += UNROLL) {
       static_for<UNROLL>([&](auto j) XP_INLINE { slab(j, loads, number + decltype(j)::value); });
@@ -919,7 +935,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 12
   const int64_t row0 = m0 + wm * WTM;
   const int64_t col0 = n0 + wn * WTN;
   // A worker's sums go to its piece of the tile, [TILE, TILE]: piece q + local, counted along the split tiles' slabs.
-  float *partial = worker ? a.partials + (q + local) * (TILE * TILE) + (wm * WTM) * TILE + wn * WTN : nullptr;
+  float *partial = worker ? a.partials + static_cast<int64_t>(q + local) * (TILE * TILE) + (wm * WTM) * TILE + wn * WTN : nullptr;
   const bool mirrored = a.symmetric != 0 && at.m != at.n;
   const int chunk = lane % LANES;
   const int64_t col = col0 + chunk * CHUNK;
@@ -1038,21 +1054,19 @@ __global__ __launch_bounds__(256) void product_join_kernel(ProductArgs a) {
   __shared__ float staged[EPI == ProductEpilogue::kStore ? 32 * PITCH : 4 * 64 * 8];
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
-  const int64_t local = blockIdx.x / BLOCKS;
+  const uint32_t local = blockIdx.x / BLOCKS;
   const int block = static_cast<int>(blockIdx.x % BLOCKS);
   const int row_in = block / (TILE / 64) * 32;
   const int col_in = block % (TILE / 64) * 64;
-  const ProductTile at = product_tile<kTileGroup<TILE>>(a, TILE, a.whole + local);
-  const int64_t row0 = at.m * TILE + row_in;
-  const int64_t col0 = at.n * TILE + col_in;
+  const ProductTile at = product_tile<kTileGroup<TILE>>(a, static_cast<uint32_t>(a.whole) + local);
+  const int64_t row0 = static_cast<int64_t>(at.m) * TILE + row_in;
+  const int64_t col0 = static_cast<int64_t>(at.n) * TILE + col_in;
   if (row0 >= a.m || col0 >= a.n) {
     return;
   }
-  const int64_t tile_slabs = (a.k + 128 / kElementBytes<P> - 1) / (128 / kElementBytes<P>);
-  const int64_t together = static_cast<int64_t>(a.split) * tile_slabs;
-  // The workers that hold the tile's first and last slab: the last q that begins at or before them.
-  const int64_t first = ((local * tile_slabs + 1) * a.workers - 1) / together;
-  const int64_t last = ((local + 1) * tile_slabs * a.workers - 1) / together;
+  const uint32_t tile_slabs = static_cast<uint32_t>((a.k + 128 / kElementBytes<P> - 1) / (128 / kElementBytes<P>));
+  const uint32_t first = split_worker(a, local * tile_slabs);
+  const uint32_t last = split_worker(a, (local + 1) * tile_slabs - 1);
   const int64_t col = col0 + (lane % LANES) * CHUNK;
   const bool mirrored = a.symmetric != 0 && at.m != at.n;
   [[maybe_unused]] float sums[8] = {};
@@ -1065,9 +1079,9 @@ __global__ __launch_bounds__(256) void product_join_kernel(ProductArgs a) {
       const ChunkPlace place = chunk_place<EPI>(a, at.matrix, row, col);
       Beside<P, EPI> beside;
       request<P, EPI>(a, place, col, beside);
-      const float *from = a.partials + (first + local) * (TILE * TILE) + (row_in + row_at) * TILE + col_in + (lane % LANES) * CHUNK;
+      const float *from = a.partials + static_cast<int64_t>(first + local) * (TILE * TILE) + (row_in + row_at) * TILE + col_in + (lane % LANES) * CHUNK;
       __builtin_memcpy(value, __builtin_assume_aligned(from, 16), CHUNK * 4);
-      int64_t more = last - first;
+      uint32_t more = last - first;
       for (; more >= 4; more -= 4) {
         float pieces[4][CHUNK];
 #pragma unroll

@@ -8,7 +8,7 @@
 //
 // Operands whose rows are not whole 16-byte chunks are first copied with padded rows into the workspace.
 
-#include "product.hpp"
+#include "product_kernels.hpp"
 #include "xp_elements.hpp"
 #include "xp_entry.hpp"
 
@@ -18,38 +18,51 @@ namespace xp {
 namespace {
 
 // ------------------------------------------------------------------ rows of whole chunks
-struct PadArgs {
+struct PadJob {
   const void *source;
   void *target;
   int64_t rows;
   int64_t width;
   int64_t ld;
-  int64_t padded;  // row length of the target, a whole number of chunks
+  int64_t padded;    // row length of the target, a whole number of chunks
+  uint32_t blocks;
+};
+struct PadArgs {
+  PadJob job[3];
+  int32_t count;
 };
 
-// Rows of any alignment into rows of whole 16-byte chunks, zeros behind them.  One thread a chunk.
+// Rows of any alignment into rows of whole 16-byte chunks, zeros behind them: up to three operands in one launch.  One
+// thread a chunk.
 template <class P>
 __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
   constexpr int CHUNK = 16 / kElementBytes<P>;
-  const int64_t chunks = a.padded / CHUNK;
-  const int64_t index = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t row = index / chunks;
-  if (row >= a.rows) {
+  uint32_t block = blockIdx.x;
+  int at = 0;
+  while (at + 1 < a.count && block >= a.job[at].blocks) {
+    block -= a.job[at].blocks;
+    ++at;
+  }
+  const PadJob job = a.job[at];
+  const uint32_t chunks = static_cast<uint32_t>(job.padded / CHUNK);
+  const int64_t index = static_cast<int64_t>(block) * 256 + threadIdx.x;
+  const int64_t row = index < (int64_t{1} << 32) ? static_cast<uint32_t>(index) / chunks : index / chunks;
+  if (row >= job.rows) {
     return;
   }
   const int64_t column = (index - row * chunks) * CHUNK;
-  const unsigned char *from = static_cast<const unsigned char *>(a.source) + (row * a.ld + column) * kElementBytes<P>;
-  const u32x4 chunk = a.width - column >= CHUNK ? load16_any(from) : load_chunk_tail<P, P>(from, a.width - column);
-  store16(static_cast<unsigned char *>(a.target) + (row * a.padded + column) * kElementBytes<P>, chunk);
+  const unsigned char *from = static_cast<const unsigned char *>(job.source) + (row * job.ld + column) * kElementBytes<P>;
+  const u32x4 chunk = job.width - column >= CHUNK ? load16_any(from) : load_chunk_tail<P, P>(from, job.width - column);
+  store16(static_cast<unsigned char *>(job.target) + (row * job.padded + column) * kElementBytes<P>, chunk);
 }
 
 // Zeros in columns [width, padded) of every row of the target.
-__global__ __launch_bounds__(256) void clear_pad_kernel(PadArgs a, int element) {
-  const int64_t behind = (a.padded - a.width) * element / 2;  // 16-bit words
+__global__ __launch_bounds__(256) void clear_pad_kernel(PadJob job, int element) {
+  const int64_t behind = (job.padded - job.width) * element / 2;  // 16-bit words
   const int64_t index = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t row = index / behind;
-  if (row < a.rows) {
-    uint16_t *words = reinterpret_cast<uint16_t *>(static_cast<unsigned char *>(a.target) + (row * a.padded + a.width) * element);
+  if (row < job.rows) {
+    uint16_t *words = reinterpret_cast<uint16_t *>(static_cast<unsigned char *>(job.target) + (row * job.padded + job.width) * element);
     words[index - row * behind] = 0;
   }
 }
@@ -94,11 +107,12 @@ __global__ __launch_bounds__(256) void column_sum_kernel(ColumnSumArgs a) {
       }
     }
   }
-  float *to = a.bands + static_cast<int64_t>(blockIdx.y) * a.n + column;
+  const bool alone = a.band_count == 1;
+  float *to = (alone ? a.out : a.bands + static_cast<int64_t>(blockIdx.y) * a.n) + column;
 #pragma unroll
   for (int j = 0; j < CHUNK; ++j) {
     if (column + j < a.n) {
-      to[j] = sum[j];
+      to[j] = alone && a.accumulate ? to[j] + sum[j] : sum[j];
     }
   }
 }
@@ -116,6 +130,90 @@ __global__ __launch_bounds__(64) void band_sum_kernel(ColumnSumArgs a) {
     sum += from[band * a.n];
   }
   a.out[column] = a.accumulate ? a.out[column] + sum : sum;
+}
+
+// ------------------------------------------------------------------ weights' gradients of few rows
+struct ThinOuterArgs {
+  const void *a;  // [rows, m]
+  const void *b;  // [rows, n]
+  void *out;      // [m, n]
+  int64_t ld_a;
+  int64_t ld_b;
+  int64_t m;
+  int64_t n;
+  int32_t rows;
+  int32_t out_dtype;
+  int32_t accumulate;
+  int32_t lanes = 0;     // threads that share a row of the output
+  int32_t out_rows = 0;  // of a workgroup
+};
+
+// out (+)= a^T b over at most ROWS rows, in fp32 on the vector pipes, rows in order.  The output's bytes bound it; a
+// matrix core tile has one slab to multiply here and spends its time on its first loads and its epilogue.  A thread keeps eight
+// columns of b in registers and walks the output's rows, whose factors the workgroup holds in LDS: 16-byte stores,
+// neighbouring lanes side by side.  Operands of any alignment.  (2048 x 6144 of five bf16 rows: see the figures of
+// xp_projection_backward.)
+constexpr int kThinRows = 16;
+constexpr int kThinOutRows = 32;
+
+template <class P, int ROWS>
+__global__ __launch_bounds__(256) void thin_outer_kernel(ThinOuterArgs a) {
+  __shared__ __attribute__((aligned(16))) float factors[kThinOutRows][ROWS];
+  const int64_t first = static_cast<int64_t>(blockIdx.y) * a.out_rows;
+  for (int i = threadIdx.x; i < a.out_rows * ROWS; i += 256) {
+    const int row = i % a.out_rows;
+    const int t = i / a.out_rows;
+    factors[row][t] = t < a.rows && first + row < a.m ? load_value(a.a, t * a.ld_a + first + row, kDtypeOf<P>) : 0.0f;
+  }
+  const int lane = static_cast<int>(threadIdx.x) % a.lanes;
+  const int side = static_cast<int>(threadIdx.x) / a.lanes;
+  const int sides = 256 / a.lanes;
+  const int64_t column = (static_cast<int64_t>(blockIdx.x) * a.lanes + lane) * 8;
+  const int count = a.n - column < 8 ? static_cast<int>(a.n - column) : 8;
+  float b[ROWS][8] = {};
+  if (count > 0) {
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) {
+      if (t < a.rows) {
+        load_values(a.b, t * a.ld_b + column, kDtypeOf<P>, count, b[t]);
+      }
+    }
+  }
+  __syncthreads();
+  if (count <= 0 || side >= sides) {
+    return;
+  }
+  for (int row = side; row < a.out_rows && first + row < a.m; row += sides) {
+    float sum[8] = {};
+#pragma unroll
+    for (int t = 0; t < ROWS; t += 4) {
+      const f32x4 four = *reinterpret_cast<const f32x4 *>(&factors[row][t]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          sum[j] = fmaf(four[i], b[t + i][j], sum[j]);
+        }
+      }
+    }
+    const int64_t at = (first + row) * a.n + column;
+    if (a.accumulate) {
+      float held[8];
+      load_values(a.out, at, a.out_dtype, count, held);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sum[j] += held[j];
+      }
+    }
+    store_values(a.out, at, a.out_dtype, count, sum);
+  }
+}
+
+template <class P>
+const void *thin_outer_for(int rows) {
+  return rows <= 4   ? reinterpret_cast<const void *>(&thin_outer_kernel<P, 4>)
+         : rows <= 8 ? reinterpret_cast<const void *>(&thin_outer_kernel<P, 8>)
+                     : reinterpret_cast<const void *>(&thin_outer_kernel<P, kThinRows>);
 }
 
 // Zeros over whole rows of an output (its gradient over no rows).
@@ -179,20 +277,44 @@ struct Caller {
     return launch_product(args, epilogue, a_cols, b_cols, dtype, scratch_bytes, stream);
   }
 
-  // `source` itself where its rows are whole chunks, else a padded copy in `target`.
-  hipError_t padded(const void *source, int64_t rows, int64_t width, int64_t ld, void *target, ProductOperand &operand) const {
+  // `source` itself where its rows are whole chunks, else a padded copy in `target`, which `pads` then has to make.
+  ProductOperand padded(const void *source, int64_t rows, int64_t width, int64_t ld, void *target, PadArgs &pads) const {
     if (whole_rows(width, element)) {
-      operand = {source, ld, 0};
-      return hipSuccess;
+      return {source, ld, 0};
     }
     const int64_t length = padded_width(width, element);
-    operand = {target, length, 0};
+    const uint32_t blocks = blocks_of(rows * (length / static_cast<int64_t>(16 / element)), 256);
+    pads.job[pads.count++] = PadJob{source, target, rows, width, ld, length, blocks};
+    return {target, length, 0};
+  }
+
+  hipError_t pad(const PadArgs &pads) const {
     KernelLaunch kernel;
+    uint32_t blocks = 0;
+    for (int i = 0; i < pads.count; ++i) {
+      blocks += pads.job[i].blocks;
+    }
     kernel.func = element == 4 ? reinterpret_cast<const void *>(&pad_rows_kernel<F32Payload>)
                                : reinterpret_cast<const void *>(&pad_rows_kernel<Bf16Payload>);
-    kernel.grid = dim3(blocks_of(rows * (length / static_cast<int64_t>(16 / element)), 256));
+    kernel.grid = dim3(blocks);
     kernel.block = dim3(256);
-    kernel.set_args(PadArgs{source, target, rows, width, ld, length});
+    kernel.set_args(pads);
+    return pads.count == 0 ? hipSuccess : launch(kernel, stream);
+  }
+
+  hipError_t thin_outer(ThinOuterArgs args) const {
+    const int64_t chunks = (args.n + 7) / 8;
+    args.lanes = static_cast<int32_t>(std::min<int64_t>(chunks, 256));
+    const int64_t across = (chunks + args.lanes - 1) / args.lanes;
+    // Enough workgroups for the chip, each with as many rows as that leaves.
+    args.out_rows = static_cast<int32_t>(std::clamp<int64_t>(args.m * across / 1024, 4, kThinOutRows));
+    KernelLaunch kernel;
+    kernel.func = dtype == kDtypeF32   ? thin_outer_for<F32Payload>(args.rows)
+                  : dtype == kDtypeF16 ? thin_outer_for<F16Payload>(args.rows)
+                                       : thin_outer_for<Bf16Payload>(args.rows);
+    kernel.grid = dim3(static_cast<unsigned>(across), blocks_of(args.m, args.out_rows));
+    kernel.block = dim3(256);
+    kernel.set_args(args);
     return launch(kernel, stream);
   }
 
@@ -233,7 +355,7 @@ hipError_t Caller::column_sums(const void *source, int64_t rows, int64_t n, int6
   if (const hipError_t status = launch(kernel, stream); status != hipSuccess) {
     return status;
   }
-  return band_sums(args);
+  return args.band_count == 1 ? hipSuccess : band_sums(args);
 }
 
 // out (+)= sum over rows t of a[t][i] b[t][j]: a weight's gradient.
@@ -465,17 +587,28 @@ int xp_projection_backward(const void *x, int64_t ld_x, int64_t rows, int64_t k,
              "gradients and workspace must overlap neither the operands nor each other");
   call.scratch = at.scratch;
   call.scratch_bytes = at.scratch_bytes;
+  const bool thin = rows <= kThinRows;
+  PadArgs pads{};
   ProductOperand grad{};
-  XP_HIP_CHECK(call.padded(grad_out, rows, n, ld_grad, at.grad, grad));
+  ProductOperand weights{};
+  ProductOperand inputs{};
+  if (grad_x != nullptr || (grad_w != nullptr && !thin)) {
+    grad = call.padded(grad_out, rows, n, ld_grad, at.grad, pads);
+  }
   if (grad_x != nullptr) {
-    ProductOperand weights{};
-    XP_HIP_CHECK(call.padded(w, n, k, k, at.w, weights));
+    weights = call.padded(w, n, k, k, at.w, pads);
+  }
+  if (grad_w != nullptr && !thin) {
+    inputs = call.padded(x, rows, k, ld_x, at.x, pads);
+  }
+  XP_HIP_CHECK(call.pad(pads));
+  if (grad_x != nullptr) {
     ProductArgs args = inputs_args(grad, weights, rows, n, k, grad_x, ld_grad_x, dtype);
     XP_HIP_CHECK(call.product(args, ProductEpilogue::kStore, false, true));
   }
-  if (grad_w != nullptr) {
-    ProductOperand inputs{};
-    XP_HIP_CHECK(call.padded(x, rows, k, ld_x, at.x, inputs));
+  if (grad_w != nullptr && thin) {
+    XP_HIP_CHECK(call.thin_outer(ThinOuterArgs{grad_out, x, grad_w, ld_grad, ld_x, n, k, static_cast<int32_t>(rows), grad_w_dtype, accumulate}));
+  } else if (grad_w != nullptr) {
     ProductArgs args = outer_args(grad, n, inputs, k, rows, grad_w, grad_w_dtype, accumulate != 0);
     XP_HIP_CHECK(call.product(args, ProductEpilogue::kStore, true, true));
   }
@@ -518,8 +651,10 @@ int xp_projection_keep(const void *x, int64_t ld_x, int64_t rows, int64_t k, con
                     span_of(bias, bias == nullptr ? 0 : static_cast<size_t>(n) * 4)}),
              "outputs and workspace must overlap neither the operands nor each other");
   const Caller call{static_cast<hipStream_t>(stream), dtype, element, at.scratch, at.scratch_bytes};
-  XP_HIP_CHECK(call.padded(x, rows, k, ld_x, at.x, args.a));
-  XP_HIP_CHECK(call.padded(w, n, k, k, at.w, args.b));
+  PadArgs pads{};
+  args.a = call.padded(x, rows, k, ld_x, at.x, pads);
+  args.b = call.padded(w, n, k, k, at.w, pads);
+  XP_HIP_CHECK(call.pad(pads));
   args.m = rows;
   args.n = n;
   args.k = k;
@@ -613,14 +748,27 @@ int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden,
   call.scratch = at.scratch;
   call.scratch_bytes = at.scratch_bytes;
 
-  ProductOperand grad{};
-  XP_HIP_CHECK(call.padded(grad_out, rows, hidden, ld_grad, at.grad, grad));
+  const bool thin = rows <= kThinRows;
+  PadArgs pads{};
+  const ProductOperand grad = call.padded(grad_out, rows, hidden, ld_grad, at.grad, pads);
+  const ProductOperand w_out_rows = call.padded(w_out, hidden, width, width, at.w_out, pads);
+  XP_HIP_CHECK(call.pad(pads));
+  pads = PadArgs{};
+  ProductOperand w_in_rows{};
+  ProductOperand inputs{};
+  if (grad_x != nullptr) {
+    w_in_rows = call.padded(w_in, wide, hidden, hidden, at.w_in, pads);
+  }
+  if (grad_w_in != nullptr && !thin) {
+    inputs = call.padded(x, rows, hidden, ld_x, at.x, pads);
+  }
+  XP_HIP_CHECK(call.pad(pads));
   const int64_t through_ld = padded_width(wide, element);
   const ProductOperand through{at.through, through_ld, 0};
   const ProductOperand activated{at.activated, padded_width(width, element), 0};
   if (grad_x != nullptr || grad_w_in != nullptr || grad_bias_in != nullptr || grad_w_out != nullptr) {
     args.a = grad;
-    XP_HIP_CHECK(call.padded(w_out, hidden, width, width, at.w_out, args.b));
+    args.b = w_out_rows;
     args.m = rows;
     args.n = width;
     args.k = hidden;
@@ -635,28 +783,31 @@ int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden,
     args.alpha = 1.0f;
     XP_HIP_CHECK(call.product(args, ProductEpilogue::kGradient, false, true));
     if (grad_bias_in != nullptr) {
-      XP_HIP_CHECK(call.band_sums(ColumnSumArgs{nullptr, at.bands, grad_bias_in, rows, wide, 0, 0, (rows + kBandRows - 1) / kBandRows, accumulate}));
+      XP_HIP_CHECK(call.band_sums(
+          ColumnSumArgs{nullptr, at.bands, grad_bias_in, rows, wide, 0, 0, (rows + kBandRows - 1) / kBandRows, accumulate}));
     }
   }
   if (grad_x != nullptr) {
     if (through_ld != wide) {
       const int64_t words = rows * (through_ld - wide) * static_cast<int64_t>(element) / 2;
       clear_pad_kernel<<<blocks_of(words, 256), 256, 0, call.stream>>>(
-          PadArgs{nullptr, at.through, rows, wide, 0, through_ld}, static_cast<int>(element));
+          PadJob{nullptr, at.through, rows, wide, 0, through_ld, 0}, static_cast<int>(element));
       XP_HIP_CHECK(hipGetLastError());
     }
-    ProductOperand weights{};
-    XP_HIP_CHECK(call.padded(w_in, wide, hidden, hidden, at.w_in, weights));
-    ProductArgs product = inputs_args(through, weights, rows, wide, hidden, grad_x, ld_grad_x, dtype);
+    ProductArgs product = inputs_args(through, w_in_rows, rows, wide, hidden, grad_x, ld_grad_x, dtype);
     XP_HIP_CHECK(call.product(product, ProductEpilogue::kStore, false, true));
   }
-  if (grad_w_in != nullptr) {
-    ProductOperand inputs{};
-    XP_HIP_CHECK(call.padded(x, rows, hidden, ld_x, at.x, inputs));
+  if (grad_w_in != nullptr && thin) {
+    XP_HIP_CHECK(call.thin_outer(
+        ThinOuterArgs{at.through, x, grad_w_in, through_ld, ld_x, wide, hidden, static_cast<int32_t>(rows), grad_w_dtype, accumulate}));
+  } else if (grad_w_in != nullptr) {
     ProductArgs product = outer_args(through, wide, inputs, hidden, rows, grad_w_in, grad_w_dtype, accumulate != 0);
     XP_HIP_CHECK(call.product(product, ProductEpilogue::kStore, true, true));
   }
-  if (grad_w_out != nullptr) {
+  if (grad_w_out != nullptr && thin) {
+    XP_HIP_CHECK(call.thin_outer(ThinOuterArgs{grad_out, at.activated, grad_w_out, ld_grad, activated.ld, hidden, width,
+                                               static_cast<int32_t>(rows), grad_w_dtype, accumulate}));
+  } else if (grad_w_out != nullptr) {
     ProductArgs product = outer_args(grad, hidden, activated, width, rows, grad_w_out, grad_w_dtype, accumulate != 0);
     XP_HIP_CHECK(call.product(product, ProductEpilogue::kStore, true, true));
   }

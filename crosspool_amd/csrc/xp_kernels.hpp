@@ -21,7 +21,7 @@ struct KernelLaunch {
   dim3 grid{1, 1, 1};
   dim3 block{1, 1, 1};
   unsigned shmem = 0;
-  alignas(16) unsigned char args[256] = {};
+  alignas(16) unsigned char args[288] = {};
   size_t args_size = 0;
 
   template <class Args>
