@@ -8,7 +8,9 @@ A matrix ``G = U S V^T`` becomes nearly ``U V^T``:
 experts of a layer, or Gate and Up of an INTERLEAVED i_proj as a view (:func:`gate_up_matrices`).  The reference has no
 counterpart; plans and caller-owned workspaces follow the projections' (operators/linear.py:28-257).
 
-bf16 and fp16 matrices run on fp16 products with fp32 sums, fp32 ones on fp32 products.  Every launch goes to the HIP
+bf16 and fp16 matrices run on fp16 products with fp32 sums (a result carries about 2^-9.7 of itself, which bf16 rounds to
+2^-9; in fp16 that is less than the type holds), fp32 ones on fp32 products.  An update whose norm is a thousandth of ``eps``
+or less, whose result is small too, loses digits in the 16-bit types and goes to zero.  Every launch goes to the HIP
 library on the current torch stream and allocates nothing, so a call can be captured into a graph.
 """
 

@@ -280,3 +280,301 @@ def test_dense_training(device, rows, hidden, width, function, order, limit, off
     before = {name: getattr(into, name).clone() for name in ("i_values", "o_values", "i_bias", "o_bias")}
     grad_x = layer.backward(projected, into, accumulate=True)
     layer.check_backward(projected, grad_x, into, before)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("rows,k,n,strides", [
+    (33, 72, 136, (80, 200, 96)), (64, 61, 35, (64, 37, 100)), (40, 128, 64, (4096, 64, 128)), (5, 30, 50, (31, 51, 33)),
+    (1, 64, 48, (640, 480, 64)), (100, 257, 130, (300, 131, 257))])
+def test_projection_gradients_of_rows_any_stride_apart(device, rows, k, n, strides, dtype):
+    case = Projection(device, rows, k, n, dtype, bias=True)
+    plain_x = case.x
+    case.x, case.grad = rows_of(case.x, strides[0]), rows_of(case.grad, strides[1])
+    held = torch.full((rows, strides[2]), 7.0, dtype=dtype, device=device)
+    grad_x = held[:, :k]
+    grad_w, grad_b = torch.empty((n, k), dtype=dtype, device=device), torch.empty(n, device=device)
+    case.gemm.backward_into(case.x, case.grad, case.weights, grad_inputs=grad_x, grad_values=grad_w, grad_bias=grad_b)
+    assert bool((held[:, k:] == 7.0).all())  # what lies between the rows stays
+    case.x, case.grad = plain_x, case.grad.contiguous()
+    case.check(grad_x, grad_w, grad_b)
+
+
+def test_gradients_are_written_alone_and_behind_nothing(device):
+    """Each gradient by itself, in the middle of guarded memory."""
+
+    rows, k, n = 45, 130, 70
+    case = Projection(device, rows, k, n, BF16, bias=True, capacity=100)
+    for name, shape, dtype in (("grad_inputs", (rows, k), BF16), ("grad_values", (n, k), BF16), ("grad_bias", (n,), FP32)):
+        size = shape[0] if len(shape) == 1 else shape[0] * shape[1]
+        flat = torch.full((size + 64,), 3.0, dtype=dtype, device=device)
+        target = flat[32:32 + size].view(shape)
+        case.gemm.backward_into(case.x, case.grad, case.weights, **{name: target})
+        assert bool((flat[:32] == 3.0).all()) and bool((flat[32 + size:] == 3.0).all())
+        case.check(*(target if name == each else None for each in ("grad_inputs", "grad_values", "grad_bias")))
+    case.gemm.backward_into(case.x, case.grad, case.weights)  # nothing asked for
+
+
+def test_every_row_count_below_the_capacity(device):
+    """One workspace serves every number of rows, and a row's gradient does not depend on the workspace's contents."""
+
+    k, n = 264, 200
+    big = Projection(device, 300, k, n, BF16, bias=True)
+    x, grad = big.x, big.grad
+    for rows in (1, 2, 15, 16, 17, 63, 64, 65, 128, 129, 299):
+        big.x, big.grad = x[:rows], grad[:rows]
+        results = []
+        for fill in (0xFF, 0x00):
+            big.gemm.scratch.fill_(fill)
+            grad_x = torch.empty((rows, k), dtype=BF16, device=device)
+            grad_w, grad_b = torch.empty((n, k), device=device), torch.empty(n, device=device)
+            big.gemm.backward_into(big.x, big.grad, big.weights, grad_inputs=grad_x, grad_values=grad_w, grad_bias=grad_b)
+            results.append((grad_x, grad_w, grad_b))
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+        big.check(*results[0])
+
+
+def test_no_rows(device):
+    case = Projection(device, 8, 64, 48, BF16, bias=True)
+    empty_x, empty_grad = case.x[:0], case.grad[:0]
+    grad_w, grad_b = torch.ones((48, 64), dtype=BF16, device=device), torch.ones(48, device=device)
+    case.gemm.backward_into(empty_x, empty_grad, case.weights, grad_inputs=torch.empty((0, 64), dtype=BF16, device=device),
+                            grad_values=grad_w, grad_bias=grad_b, accumulate=True)
+    assert bool((grad_w == 1).all()) and bool((grad_b == 1).all())
+    case.gemm.backward_into(empty_x, empty_grad, case.weights, grad_values=grad_w, grad_bias=grad_b)
+    assert bool((grad_w == 0).all()) and bool((grad_b == 0).all())
+    layer = Layer(device, 8, 64, 40, BF16, bias=True)
+    layer.rows, layer.x, layer.grad = 0, layer.x[:0], layer.grad[:0]
+    projected, out = layer.forward()
+    assert projected.shape == (0, 80) and out.shape == (0, 64)
+    into = layer.gradients()
+    layer.backward(projected, into)
+    assert all(bool((t == 0).all()) for t in (into.i_values, into.o_values, into.i_bias, into.o_bias))
+
+
+def test_bad_values_stay_in_their_rows_and_columns(device):
+    """A NaN or infinity reaches what depends on it and nothing else, in tiles and beside ragged edges."""
+
+    for rows, k, n in ((70, 72, 136), (70, 61, 131), (9, 72, 40)):
+        case = Projection(device, rows, k, n, BF16, bias=True)
+        case.grad[3, 5] = float("nan")
+        case.x[rows - 1, k - 1] = float("inf")
+        grad_x = torch.empty((rows, k), dtype=BF16, device=device)
+        grad_w, grad_b = torch.empty((n, k), dtype=BF16, device=device), torch.empty(n, device=device)
+        case.gemm.backward_into(case.x, case.grad, case.weights, grad_inputs=grad_x, grad_values=grad_w, grad_bias=grad_b)
+        assert bool(grad_x[3].isnan().all()) and not bool(grad_x[torch.arange(rows) != 3].isnan().any())
+        assert bool(grad_w[5].isnan().all()) and not bool(grad_w[torch.arange(n) != 5, :k - 1].isnan().any())
+        assert not bool(grad_w[torch.arange(n) != 5, k - 1].isfinite().any())
+        assert bool(grad_b[5].isnan()) and not bool(grad_b[torch.arange(n) != 5].isnan().any())
+
+
+@pytest.mark.parametrize("order", [INTERLEAVED, CONCATENATED], ids=["pairs", "halves"])
+def test_clipped_and_bad_gates(device, order):
+    """At the limit a value has its gradient, past it none; NaN is past no limit; an infinite gate is what it is in the
+    activation and in its own gradient (-inf 0: NaN)."""
+
+    layer = Layer(device, 6, 64, 40, BF16, function="silu", order=order, limit=1.0, bias=True)
+    projected, _ = layer.forward()
+    gate, up = layer.split(projected)
+    gate[0], up[0] = 1.0, -1.0
+    gate[1], up[1] = 1.5, 0.5
+    gate[2], up[2] = 0.5, -1.5
+    gate[3, 7], up[4, 9] = float("nan"), float("nan")
+    gate[5], up[5] = float("-inf"), 0.25
+    into = layer.gradients()
+    grad_x = layer.backward(projected, into)
+    assert bool(grad_x[3].isnan().all())
+    # a NaN Up is in its Gate's gradient, which a clipped Gate does not have
+    assert bool(grad_x[4].isnan().all()) == bool(gate[4, 9] <= 1.0) and bool(grad_x[:3].isfinite().all())
+    apart = torch.empty((1, layer.wide), dtype=BF16, device=device)
+    layer.signature.activation.backward_into(inputs=projected[5:6], grad_output=torch.ones((1, 40), dtype=BF16, device=device),
+                                             grad_inputs=apart, order=order)
+    assert bool(grad_x[5].isnan().all()) == bool(apart.isnan().any())
+    layer.x, layer.grad, layer.rows = layer.x[:3].contiguous(), layer.grad[:3].contiguous(), 3
+    kept = projected[:3].contiguous()
+    grad_x = layer.backward(kept, into)
+    layer.check_backward(kept, grad_x, into)
+
+
+def test_offsets_past_32_bits(device):
+    """Rows of operands and outputs beyond 2^31 elements from their begin."""
+
+    rows, k, n = 2200, 64, 72
+    stride = 1 << 20
+    case = Projection(device, rows, k, n, BF16)
+    base = torch.zeros(rows * stride, dtype=BF16, device=device)
+    x = base.view(rows, stride)[:, 64:64 + k]
+    x.copy_(case.x)
+    grad = base.view(rows, stride)[:, 4096:4096 + n]
+    grad.copy_(case.grad)
+    grad_x = base.view(rows, stride)[:, 8192:8192 + k]
+    grad_w = torch.empty((n, k), dtype=BF16, device=device)
+    case.gemm.backward_into(x, grad, case.weights, grad_inputs=grad_x, grad_values=grad_w)
+    case.check(grad_x, grad_w, None)
+    del base
+
+
+@pytest.mark.parametrize("rows", [12, 200])
+def test_training_pass_in_a_graph(device, rows):
+    """Forward and backward captured once and replayed on other data, with eager work between the replays."""
+
+    layer = Layer(device, rows, 264, 200, BF16, function="gelu", bias=True)
+    projected = torch.empty((rows, layer.wide), dtype=BF16, device=device)
+    out = torch.empty((rows, layer.hidden), dtype=BF16, device=device)
+    grad_x = torch.empty((rows, layer.hidden), dtype=BF16, device=device)
+    into = layer.gradients()
+
+    def run():
+        layer.dense.run_into(hidden_states=layer.x, layer_weights=layer.weights, output=out, projected=projected)
+        layer.dense.backward_into(hidden_states=layer.x, layer_weights=layer.weights, projected=projected, grad_output=layer.grad,
+                                  grad_hidden_states=grad_x, gradients=into)
+
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    run()
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] == before  # no call allocates
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    targets = (projected, out, grad_x, into.i_values, into.o_values, into.i_bias, into.o_bias)
+    for seed in (1, 2, 3):
+        other = Layer(device, rows, 264, 200, BF16, function="gelu", bias=True, seed=seed)
+        layer.x.copy_(other.x)
+        layer.grad.copy_(other.grad)
+        layer.weights.i_proj.values.copy_(other.weights.i_proj.values)
+        for target in targets:
+            target.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [target.clone() for target in targets]
+        layer.check_forward(projected, out)
+        layer.check_backward(projected, grad_x, into)
+        run()
+        assert all(torch.equal(a, b) for a, b in zip(replayed, targets))
+
+
+def test_two_streams_with_their_own_scratch(device):
+    layers = [Layer(device, 150, 512, 264, BF16, bias=True, seed=s) for s in (1, 2)]
+    expected = []
+    for layer in layers:
+        projected, out = layer.forward()
+        into = layer.gradients()
+        expected.append((projected, out, layer.backward(projected, into), into.i_values, into.o_values, into.i_bias, into.o_bias))
+    streams = [torch.cuda.Stream() for _ in layers]
+    torch.cuda.synchronize()
+    found = [None, None]
+    for _ in range(3):
+        for index, (stream, layer) in enumerate(zip(streams, layers)):
+            with torch.cuda.stream(stream):
+                projected, out = layer.forward()
+                into = layer.gradients()
+                found[index] = (projected, out, layer.backward(projected, into), into.i_values, into.o_values, into.i_bias, into.o_bias)
+    torch.cuda.synchronize()
+    for wanted, got in zip(expected, found):
+        assert all(torch.equal(a, b) for a, b in zip(wanted, got))
+
+
+def test_gradients_against_differences(device):
+    """Directional derivatives of the layer, by central differences of the formula in 64 bits.  fp32 gradients sum at most
+    260 products: off by less than 2^-14 of their terms, and the directions' terms add up with random signs."""
+
+    layer = Layer(device, 20, 64, 130, FP32, function="gelu", bias=True)
+    projected, _ = layer.forward()
+    into = layer.gradients()
+    grad_x = layer.backward(projected, into)
+    w = layer.weights
+    leaves = [t.double() for t in (layer.x, w.i_proj.values, w.o_proj.values, w.i_proj.bias, w.o_proj.bias)]
+    grads = [t.double() for t in (grad_x, into.i_values, into.o_values, into.i_bias, into.o_bias)]
+
+    def loss(x, w_in, w_out, b_in, b_out):
+        f, _, _, factor, _, _ = layer.terms(x @ w_in.T + b_in)
+        return ((f * factor @ w_out.T + b_out) * layer.grad.double()).sum()
+
+    g = torch.Generator(device=device).manual_seed(3)
+    for index, grad in enumerate(grads):
+        direction = torch.randn(grad.shape, generator=g, device=device, dtype=torch.float64)
+        step = 1e-5
+        sides = [loss(*(leaf + sign * step * direction if i == index else leaf for i, leaf in enumerate(leaves))) for sign in (1, -1)]
+        difference = float((sides[0] - sides[1]) / (2 * step))
+        allowed = 2.0**-14 * float((grad.abs() * direction.abs()).sum()) + 1e-6
+        assert abs(difference - float((grad * direction).sum())) <= allowed
+
+
+def test_frozen_layer_carries_adapter_gradients(device):
+    """The gradient through a frozen projection is what an adapter's backward pass adds its own part to."""
+
+    from crosspool_amd.adapters import Adapter, AdapterPlan, AdapterWeights
+
+    case = Projection(device, 90, 256, 192, BF16)
+    g = torch.Generator(device=device).manual_seed(5)
+    a = (torch.randn((2, 8, 256), generator=g, device=device) / 16).to(BF16)
+    b = (torch.randn((2, 192, 8), generator=g, device=device) / 3).to(BF16)
+    ids = torch.randint(-1, 2, (90,), generator=g, device=device, dtype=torch.int32)
+    plan = AdapterPlan.prepare(row_capacity=90, adapter_count=2, max_rank=8, input_width=256, output_width=192, dtype=BF16, backward=True)
+    adapter = Adapter(plan, torch.empty(plan.workspace.nbytes, dtype=torch.uint8, device=device))
+    grad_x = torch.empty((90, 256), dtype=BF16, device=device)
+    grad_a, grad_b = torch.empty_like(a), torch.empty_like(b)
+    case.gemm.backward_into(case.x, case.grad, case.weights, grad_inputs=grad_x)
+    adapter.backward_into(case.x, case.grad, AdapterWeights(a, b), adapter_ids=ids, base=grad_x, grad_inputs=grad_x, grad_a=grad_a,
+                          grad_b=grad_b)
+    exact = case.grad.double() @ case.weights.values.double()
+    for index in range(2):
+        taken = (ids == index).double()[:, None]
+        exact += taken * (case.grad.double() @ b[index].double() @ a[index].double())
+    error = float((grad_x.double() - exact).norm() / exact.norm())
+    assert error <= 3 * 2 * 2.0**-9  # two rounded stages, as in the adapters' own tests
+
+
+def test_refusals(device):
+    case = Projection(device, 16, 64, 48, BF16, bias=True)
+    good = dict(grad_inputs=torch.empty((16, 64), dtype=BF16, device=device))
+    with pytest.raises(ValueError, match="output gradient"):
+        case.gemm.backward_into(case.x, case.grad.float(), case.weights, **good)
+    with pytest.raises(ValueError, match="inputs"):
+        case.gemm.backward_into(case.x[:8], case.grad, case.weights, **good)
+    with pytest.raises(ValueError, match="prepared layout"):
+        case.gemm.backward_into(torch.cat((case.x, case.x)), torch.cat((case.grad, case.grad)), case.weights)
+    with pytest.raises(ValueError, match="contiguous"):
+        case.gemm.backward_into(case.x, case.grad, case.weights, grad_inputs=torch.empty((64, 16), dtype=BF16, device=device).T)
+    with pytest.raises(ValueError, match="grad_values"):
+        case.gemm.backward_into(case.x, case.grad, case.weights, grad_values=torch.empty((48, 64), dtype=FP16, device=device))
+    with pytest.raises(ValueError, match="bias"):
+        case.gemm.backward_into(case.x, case.grad, ProjectionWeights(case.weights.values), **good)
+    with pytest.raises(RuntimeError, match="16-byte"):
+        wide = torch.zeros((16, 72), dtype=BF16, device=device)
+        case.gemm.backward_into(wide[:, 1:65], case.grad, case.weights, grad_values=torch.empty((48, 64), dtype=BF16, device=device))
+    with pytest.raises(RuntimeError, match="overlap"):
+        case.gemm.backward_into(case.x, case.grad, case.weights, grad_inputs=case.x,
+                                grad_values=torch.empty((48, 64), dtype=BF16, device=device))
+    forward_only = GemmPlan.prepare(
+        input_layout=TensorLayout((16, 64), BF16), weight_layout=ProjectionLayout.of(case.weights),
+        result_layout=TensorLayout((16, 48), BF16), activation=None)
+    gemm = Gemm(forward_only, torch.empty(max(16, forward_only.workspace.nbytes), dtype=torch.uint8, device=device))
+    with pytest.raises(ValueError, match="without backward"):
+        gemm.backward_into(case.x, case.grad, case.weights, **good)
+    layer = Layer(device, 16, 64, 40, BF16)
+    projected, _ = layer.forward()
+    with pytest.raises(ValueError, match="projected"):
+        layer.backward(projected[:, :40], layer.gradients())
+    with pytest.raises(ValueError, match="without a bias"):
+        layer.backward(projected, DenseGradients(i_bias=torch.empty(80, device=device)))
+    with pytest.raises(ValueError, match="i_proj gradient"):
+        layer.backward(projected, DenseGradients(i_values=torch.empty((40, 64), dtype=BF16, device=device)))
+    with pytest.raises(ValueError, match="projected"):
+        layer.dense.run_into(hidden_states=layer.x, layer_weights=layer.weights, output=torch.empty_like(layer.x),
+                             projected=torch.empty((16, 80), dtype=FP16, device=device))
+    plan = DenseExecutionPlan.prepare(layer.signature)
+    dense = Dense(plan, torch.empty(plan.workspace.nbytes, dtype=torch.uint8, device=device))
+    with pytest.raises(ValueError, match="without backward"):
+        dense.run_into(hidden_states=layer.x, layer_weights=layer.weights, output=torch.empty_like(layer.x), projected=projected)
+
+
+def test_the_forward_pass_of_a_trained_layer_is_the_served_one(device):
+    """With `projected` a layer gives what it gives without, up to the rounding of the projection."""
+
+    for function, order in (("silu", INTERLEAVED), ("gelu", CONCATENATED)):
+        layer = Layer(device, 130, 256, 264, BF16, function=function, order=order)
+        _, out = layer.forward()
+        served = torch.empty_like(out)
+        layer.dense.run_into(hidden_states=layer.x, layer_weights=layer.weights, output=served)
+        error = float((out.double() - served.double()).norm() / served.double().norm())
+        assert error <= 3 * 2.0**-9  # the projection's, the activation's and the output's half steps
