@@ -9,24 +9,26 @@ namespace xp {
 
 // A product's time in microseconds.  A CU's workgroups share its throughput: with i + 1 of them on it (as many as fit),
 // a slab in each takes `slab[i]`, and the first loads and the epilogue `around[i]`.  Fitted on MI355X to 1, 4, 12 and 48
-// slabs on 64 to 1536 workgroups; the three storage orders differ by less than 10 %.  Model and measured, us: bf16
+// slabs on 64 to 2048 workgroups; the three storage orders differ by less than 10 %.  Model and measured, us: bf16
 // 4096 x 12288 x 4096 299 / 294, 1000 x 2048 x 12288 63 / 61, fp16 symmetric 4096 x 12288 199 / 200; fp32 700 x 1536 x
 // 1536 40 / 41.
 namespace {
 struct ProductCost {
   ProductTiles tiles;
   int together;
-  double slab[3];
-  double around[3];
+  double slab[4];
+  double around[4];
 };
-constexpr ProductCost kCosts16[] = {{ProductTiles::k256, 1, {1.38, 0.0, 0.0}, {8.2, 0.0, 0.0}},
-                                    {ProductTiles::k128Pairs, 2, {0.73, 0.85, 0.0}, {4.7, 5.9, 0.0}},
-                                    {ProductTiles::k128Deep, 1, {0.5, 0.0, 0.0}, {6.3, 0.0, 0.0}},
-                                    {ProductTiles::k64, 3, {0.245, 0.38, 0.52}, {2.3, 3.0, 3.9}}};
-constexpr ProductCost kCosts32[] = {{ProductTiles::k256, 1, {7.4, 0.0, 0.0}, {14.0, 0.0, 0.0}},
-                                    {ProductTiles::k128Pairs, 2, {1.95, 3.67, 0.0}, {7.0, 7.5, 0.0}},
-                                    {ProductTiles::k128Deep, 1, {2.08, 0.0, 0.0}, {7.0, 0.0, 0.0}},
-                                    {ProductTiles::k64, 3, {0.62, 1.05, 1.49}, {2.4, 3.4, 4.6}}};
+constexpr ProductCost kCosts16[] = {{ProductTiles::k256, 1, {1.38}, {8.2}},
+                                    {ProductTiles::k128Pairs, 2, {0.73, 0.85}, {4.7, 5.9}},
+                                    {ProductTiles::k128Deep, 1, {0.5}, {6.3}},
+                                    {ProductTiles::k64, 3, {0.245, 0.38, 0.52}, {2.3, 3.0, 3.9}},
+                                    {ProductTiles::k32, 4, {0.155, 0.22, 0.36, 0.46}, {0.8, 1.1, 1.4, 1.7}}};
+constexpr ProductCost kCosts32[] = {{ProductTiles::k256, 1, {7.4}, {14.0}},
+                                    {ProductTiles::k128Pairs, 2, {1.95, 3.67}, {7.0, 7.5}},
+                                    {ProductTiles::k128Deep, 1, {2.08}, {7.0}},
+                                    {ProductTiles::k64, 3, {0.62, 1.05, 1.49}, {2.4, 3.4, 4.6}},
+                                    {ProductTiles::k32, 4, {0.235, 0.345, 0.48, 0.6}, {0.9, 1.3, 1.6, 2.0}}};
 constexpr int64_t kCus = 256;
 constexpr double kLaunchUs = 2.3;
 constexpr double kJoinUs = 3.0;       // its launch,
@@ -88,7 +90,7 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int64_t batch, int ele
     consider(tiles, 0);
     const int64_t slots = kCus * cost.together;
     const int64_t full = tiles / slots * slots;
-    if (full == tiles || cost.tiles == ProductTiles::k256) {
+    if (full == tiles || cost.tiles == ProductTiles::k256 || cost.tiles == ProductTiles::k32) {
       continue;
     }
     const int64_t split = tiles - full;

@@ -64,8 +64,10 @@ struct ProductArgs {
 static_assert(sizeof(ProductArgs) <= 288, "a kernel's argument record");
 
 // Tile sizes, stages of LDS and workgroups that a CU holds.
-enum class ProductTiles : int { k256 = 0, k128Pairs = 1, k128Deep = 2, k64 = 3 };
-constexpr int tile_size(ProductTiles tiles) { return tiles == ProductTiles::k256 ? 256 : tiles == ProductTiles::k64 ? 64 : 128; }
+enum class ProductTiles : int { k256 = 0, k128Pairs = 1, k128Deep = 2, k64 = 3, k32 = 4 };
+constexpr int tile_size(ProductTiles tiles) {
+  return tiles == ProductTiles::k256 ? 256 : tiles == ProductTiles::k64 ? 64 : tiles == ProductTiles::k32 ? 32 : 128;
+}
 
 struct ProductPlan {
   ProductTiles tiles;

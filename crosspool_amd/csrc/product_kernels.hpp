@@ -509,8 +509,8 @@ struct OperandLoads {
     } else {
       origin = static_cast<const unsigned char *>(data) + tile_first * ld * ES;
       span = static_cast<uint32_t>(rows_left < ROWS ? rows_left : ROWS) * ld_bytes;
-      // Eight rows a load: swizzle(8 g + row) = (row / 2) ^ (4 if g is odd).
-      lane_offset[0] = static_cast<uint32_t>(place ^ (row >> 1));
+      // Eight rows a load: swizzle(8 g + row) = (row / 2) ^ (4 if g is odd), g = first + q.
+      lane_offset[0] = static_cast<uint32_t>(place ^ (row >> 1) ^ (LOADS % 2 != 0 ? 4 * (first & 1) : 0));
       lane_offset[1] = lane_offset[0] ^ 4;
     }
   }
@@ -518,7 +518,9 @@ struct OperandLoads {
   // COLS: what the chunk index of reduction row k is xor-ed with; k's low bits follow from the load's variant
   // and the lane's row in it.
   __device__ static __forceinline__ int scramble(int variant, int row) {
-    if constexpr (ES == 4) {
+    if constexpr (ROWS == 32) {
+      return 0;                                       // four (16-bit) rows are a bank line
+    } else if constexpr (ES == 4) {
       return variant << 3;                            // bit 2 of k
     } else if constexpr (ROWS >= 256) {
       return ((2 * variant + row) & 3) << 2;          // k % 4, two rows a load
@@ -528,7 +530,7 @@ struct OperandLoads {
       return ((row >> 1) & 1) << 2;                   // two rows share a bank line
     }
   }
-  // The variant of load q of a wave (its loads start at a multiple of LOADS).
+  // The variant of load q of a wave (its loads start at a multiple of LOADS, which is even or 1).
   static constexpr int variant(int q) {
     if constexpr (!COLS) {
       return q & 1;
@@ -587,21 +589,24 @@ struct OperandFragments {
   static constexpr int BASES = COLS ? TILES : 4;
   uint32_t base[WINDOWS][BASES];
 
-  __device__ __forceinline__ void setup(int region, int first_tile, int lane) {
+  // `step0`: the k step that read's step 0 stands for.
+  __device__ __forceinline__ void setup(int region, int first_tile, int step0, int lane) {
     const int half = lane >> 5;
 #pragma unroll
     for (int i = 0; i < BASES; ++i) {
       int at;
       if constexpr (!COLS) {
         const int row = lane & 31;
-        at = (first_tile * 32 + row) * 128 + (((i * 2 + half) ^ swizzle(row)) << 4);
+        at = (first_tile * 32 + row) * 128 + (((((step0 + i) & 3) * 2 + half) ^ swizzle(row)) << 4);
       } else if constexpr (ES == 4) {
-        const int tile = (first_tile + i) ^ half;  // bit 2 of the reduction row is the lane's half
-        at = 4 * half * ROWS * 4 + tile * 128 + (lane & 31) * 4;
+        const int tile = ROWS == 32 ? 0 : (first_tile + i) ^ half;  // bit 2 of the reduction row is the lane's half
+        at = (8 * step0 + 4 * half) * ROWS * 4 + tile * 128 + (lane & 31) * 4;
       } else {
         const int within = lane & 15;
-        const int row = 8 * half + (within >> 2);
-        const int tile = ROWS >= 128 ? (first_tile + i) ^ (within >> 2) : (first_tile + i) ^ ((within >> 3) & 1);
+        const int row = 16 * step0 + 8 * half + (within >> 2);
+        const int tile = ROWS == 32    ? 0
+                         : ROWS >= 128 ? (first_tile + i) ^ (within >> 2)
+                                       : (first_tile + i) ^ ((within >> 3) & 1);
         at = row * ROWS * 2 + tile * 64 + ((lane >> 4) & 1) * 32 + (within & 3) * 8;
       }
 #pragma unroll
@@ -705,11 +710,14 @@ constexpr int kTileGroup = TILE == 256 ? 4 : 8;
 // projections' tile kernel: fragments are read one k step ahead of their MFMAs from two register sets, and the
 // barrier sits where the slab's last fragments have been read.
 template <class P, int TILE, int WAVES_M, int WAVES_N, int STAGES, bool A_COLS, bool B_COLS, ProductEpilogue EPI>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 128 && STAGES > 2 ? 1 : 2) void product_kernel(
+__global__ __launch_bounds__(TILE == 32 ? 256 : 64 * WAVES_M * WAVES_N, TILE == 32 ? 4 : TILE == 64 ? 3 : TILE == 128 && STAGES > 2 ? 1 : 2) void product_kernel(
     ProductArgs a) {
   constexpr int ES = kElementBytes<P>;
   constexpr int BK = 128 / ES;
-  constexpr int WAVES = WAVES_M * WAVES_N;
+  // 32 x 32 tiles: the four waves take one k step of every slab each and add their sums in the epilogue.
+  constexpr bool SPREAD = TILE == 32;
+  constexpr int WAVES = SPREAD ? 4 : WAVES_M * WAVES_N;
+  constexpr int STEPS = SPREAD ? 1 : 4;  // k steps of a slab that a wave multiplies
   constexpr int WTM = TILE / WAVES_M;
   constexpr int WTN = TILE / WAVES_N;
   constexpr int MT = WTM / 32;
@@ -728,14 +736,14 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 12
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * REGION];
 
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int wm = wave % WAVES_M;
-  const int wn = wave / WAVES_M;
+  const int wm = SPREAD ? 0 : wave % WAVES_M;
+  const int wn = SPREAD ? 0 : wave / WAVES_M;
   const bool loading_wave = wave < LOAD_WAVES;
 
   const uint32_t tile_slabs = static_cast<uint32_t>((a.k + BK - 1) / BK);
   // Whole tiles first, one a workgroup; then the workers of the split tiles, each with one run of their slabs, the end
   // of one tile and the begin of the next among them (the host gives a worker at least one slab).
-  constexpr bool SPLITS = TILE != 256;  // what a split saves 256 x 256 tiles goes into their pieces' 256 KB
+  constexpr bool SPLITS = TILE == 128 || TILE == 64;  // what a split saves 256 x 256 tiles goes into their pieces' 256 KB
   const uint32_t whole = static_cast<uint32_t>(a.whole);
   const bool worker = SPLITS && blockIdx.x >= whole;
   // Where every tile has the same number of workers, those of one part of K come one after another: they share slabs.
@@ -753,8 +761,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 12
   __asm__ volatile("" : "+v"(lane));
   OperandFragments<P, TILE, A_COLS, MT, STAGES> a_fragments;
   OperandFragments<P, TILE, B_COLS, NT, STAGES> b_fragments;
-  a_fragments.setup(0, wm * MT, lane);
-  b_fragments.setup(REGION, wn * NT, lane);
+  a_fragments.setup(0, wm * MT, SPREAD ? wave : 0, lane);
+  b_fragments.setup(REGION, wn * NT, SPREAD ? wave : 0, lane);
   const lds_bytes_t shared = (lds_bytes_t)lds;
   const uint32_t local = worker ? next / tile_slabs : 0;  // among the split tiles
   const ProductTile at = product_tile<kTileGroup<TILE>>(a, worker ? whole + local : place_of(blockIdx.x, whole));
@@ -798,8 +806,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 12
   // Wave tiles of up to four accumulators hold a whole slab's fragments twice: their few MFMAs a k step are shorter than
   // the LDS latency, so the next slab's are all read under this slab's MFMAs.  Larger ones read one k step ahead.
   constexpr bool WHOLE_SLABS = MT * NT == 1 || (MT * NT == 4 && STAGES > 2);
-  u32x4 af[WHOLE_SLABS ? 8 : 2][MT];
-  u32x4 bf[WHOLE_SLABS ? 8 : 2][NT];
+  u32x4 af[WHOLE_SLABS ? 2 * STEPS : 2][MT];
+  u32x4 bf[WHOLE_SLABS ? 2 * STEPS : 2][NT];
   auto read_fragments = [&](int stage, int ks, int slot) XP_INLINE {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -839,14 +847,14 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 12
   __syncthreads();
   auto read_slab = [&](int stage, int set) XP_INLINE {
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      read_fragments(stage, ks, set * 4 + ks);
+    for (int ks = 0; ks < STEPS; ++ks) {
+      read_fragments(stage, ks, set * STEPS + ks);
     }
   };
   auto multiply_slab = [&](int set) XP_INLINE {
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      multiply(set * 4 + ks);
+    for (int ks = 0; ks < STEPS; ++ks) {
+      multiply(set * STEPS + ks);
     }
   };
   if constexpr (WHOLE_SLABS) {
@@ -939,6 +947,72 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, TILE == 64 ? 3 : TILE == 12
   const bool mirrored = a.symmetric != 0 && at.m != at.n;
   const int chunk = lane % LANES;
   const int64_t col = col0 + chunk * CHUNK;
+  if constexpr (SPREAD) {
+    // The waves' sums side by side in LDS; each wave then finishes eight of the rows.
+    const float *all = reinterpret_cast<const float *>(lds);
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const f32x4 four = {acc[0][0][4 * q4], acc[0][0][4 * q4 + 1], acc[0][0][4 * q4 + 2], acc[0][0][4 * q4 + 3]};
+      *reinterpret_cast<f32x4 *>(rows + (lane & 31) * PITCH + 8 * q4 + 4 * (lane >> 5)) = four;
+    }
+    __syncthreads();
+    const auto total = [&](int row, int column) __attribute__((always_inline)) {
+      const float *from = all + row * PITCH + column;
+      return (from[0] + from[32 * PITCH]) + (from[64 * PITCH] + from[96 * PITCH]);
+    };
+    [[maybe_unused]] float sums[8] = {};
+    const int row = wave * 8 + lane / LANES;
+    if (lane / LANES < 8 && row0 + row < a.m && col < a.n) {
+      const ChunkPlace there = chunk_place<EPI>(a, at.matrix, row0 + row, col);
+      Beside<P, EPI> beside;
+      request<P, EPI>(a, there, col, beside);
+      float value[CHUNK];
+#pragma unroll
+      for (int j = 0; j < CHUNK; ++j) {
+        value[j] = total(row, chunk * CHUNK + j);
+      }
+      if constexpr (EPI == ProductEpilogue::kGradient) {
+        finish_gradient<P>(a, there, col, beside, value, sums);
+      } else {
+        finish<P, EPI>(a, there, col, beside, value);
+      }
+    }
+    if constexpr (EPI == ProductEpilogue::kStore) {
+      const int64_t to_row = col0 + (threadIdx.x & 31);
+      const int64_t to_col = row0 + (threadIdx.x >> 5) * 8;
+      if (mirrored && threadIdx.x < 128 && to_row < a.n && to_col < a.m) {
+        float value[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          value[j] = total(static_cast<int>(threadIdx.x >> 5) * 8 + j, static_cast<int>(threadIdx.x & 31));
+        }
+        const ChunkPlace across = chunk_place<EPI>(a, at.matrix, to_row, to_col);
+        Beside<P, EPI> beside;
+        request<P, EPI>(a, across, to_col, beside);
+        finish<P, EPI>(a, across, to_col, beside, value);
+      }
+    }
+    if constexpr (EPI == ProductEpilogue::kGradient) {
+      if (a.column_sums != nullptr) {
+        __syncthreads();
+        float *bands = reinterpret_cast<float *>(lds);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          bands[wave * 512 + j * 64 + lane] = sums[j];
+        }
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int in = j * 64 + lane;
+            sums[j] = (bands[in] + bands[512 + in]) + (bands[1024 + in] + bands[1536 + in]);
+          }
+          store_column_sums<LANES>(a, row0 / 32, col, sums, lane);
+        }
+      }
+    }
+    return;
+  }
   ChunkPlace place = chunk_place<EPI>(a, at.matrix, row0 + lane / LANES, col);
   constexpr int PASSES = 32 / ROWS_PER_PASS;
   constexpr int AHEAD = EPI == ProductEpilogue::kGradient ? PASSES : PASSES < 2 ? PASSES : 2;  // passes whose loads are in flight
@@ -1204,8 +1278,10 @@ const void *ProductKernels<P>::main(ProductTiles tiles, ProductEpilogue epilogue
       return product_tile_kernel<P, 128, 2, 2, 2>(epilogue, a_cols, b_cols);
     case ProductTiles::k128Deep:
       return product_tile_kernel<P, 128, 2, 2, 4>(epilogue, a_cols, b_cols);
-    default:
+    case ProductTiles::k64:
       return product_tile_kernel<P, 64, 2, 2, 3>(epilogue, a_cols, b_cols);
+    default:
+      return product_tile_kernel<P, 32, 1, 1, 4>(epilogue, a_cols, b_cols);
   }
 }
 

@@ -80,24 +80,29 @@ struct ColumnSumArgs {
   int32_t accumulate;
 };
 
-// fp32 sums of a band's rows, eight columns a thread.
+// fp32 sums of a band's rows.  A workgroup takes a chunk of columns per lane and the band's rows in turn over its four
+// waves, eight of a wave's in flight, and adds the waves' sums through LDS in wave order.
+constexpr int kBandRowsOfSum = 64;
+
 template <class P>
 __global__ __launch_bounds__(256) void column_sum_kernel(ColumnSumArgs a) {
   constexpr int ES = kElementBytes<P>;
   constexpr int CHUNK = 16 / ES;
-  const int64_t column = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * CHUNK;
-  if (column >= a.n) {
-    return;
-  }
+  constexpr int AHEAD = 8;
+  __shared__ float waves[4][CHUNK][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int64_t column = (static_cast<int64_t>(blockIdx.x) * 64 + lane) * CHUNK;
+  const bool live = column < a.n;
+  const bool whole = a.n - column >= CHUNK;
   const int64_t first = static_cast<int64_t>(blockIdx.y) * a.band_rows;
   const int64_t last = first + a.band_rows < a.rows ? first + a.band_rows : a.rows;
-  const bool whole = a.n - column >= CHUNK;
+  const auto row_at = [&](int64_t row) __attribute__((always_inline)) {
+    const unsigned char *from = static_cast<const unsigned char *>(a.source) + (row * a.ld + column) * ES;
+    return whole ? load16_any(from) : load_chunk_tail<P, P>(from, a.n - column);
+  };
   float sum[CHUNK] = {};
-  const unsigned char *from = static_cast<const unsigned char *>(a.source) + (first * a.ld + column) * ES;
-#pragma unroll 4
-  for (int64_t row = first; row < last; ++row) {
-    const u32x4 chunk = whole ? load16_any(from) : load_chunk_tail<P, P>(from, a.n - column);
-    from += a.ld * ES;
+  const auto add = [&](const u32x4 &chunk) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < CHUNK; ++j) {
       if constexpr (ES == 4) {
@@ -106,30 +111,63 @@ __global__ __launch_bounds__(256) void column_sum_kernel(ColumnSumArgs a) {
         sum[j] += P::widen(j % 2 == 0 ? chunk[j / 2] & 0xffffu : chunk[j / 2] >> 16);
       }
     }
+  };
+  int64_t row = first + wave;
+  if (live) {
+    for (; row + 4 * (AHEAD - 1) < last; row += 4 * AHEAD) {
+      u32x4 chunks[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        chunks[i] = row_at(row + 4 * i);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        add(chunks[i]);
+      }
+    }
+    for (; row < last; row += 4) {
+      add(row_at(row));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < CHUNK; ++j) {
+    waves[wave][j][lane] = sum[j];
+  }
+  __syncthreads();
+  if (wave != 0 || !live) {
+    return;
   }
   const bool alone = a.band_count == 1;
   float *to = (alone ? a.out : a.bands + static_cast<int64_t>(blockIdx.y) * a.n) + column;
 #pragma unroll
   for (int j = 0; j < CHUNK; ++j) {
     if (column + j < a.n) {
-      to[j] = alone && a.accumulate ? to[j] + sum[j] : sum[j];
+      const float total = (waves[0][j][lane] + waves[1][j][lane]) + (waves[2][j][lane] + waves[3][j][lane]);
+      to[j] = alone && a.accumulate ? to[j] + total : total;
     }
   }
 }
 
-// The bands' sums in band order.
-__global__ __launch_bounds__(64) void band_sum_kernel(ColumnSumArgs a) {
-  const int64_t column = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x;
-  if (column >= a.n) {
-    return;
-  }
+// The bands' sums: a workgroup's four waves take the bands in turn, and theirs are added in wave order.
+__global__ __launch_bounds__(256) void band_sum_kernel(ColumnSumArgs a) {
+  __shared__ float waves[4][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int64_t column = static_cast<int64_t>(blockIdx.x) * 64 + lane;
   float sum = 0.0f;
-  const float *from = a.bands + column;
+  if (column < a.n) {
+    const float *from = a.bands + column;
 #pragma unroll 8
-  for (int64_t band = 0; band < a.band_count; ++band) {
-    sum += from[band * a.n];
+    for (int64_t band = wave; band < a.band_count; band += 4) {
+      sum += from[band * a.n];
+    }
   }
-  a.out[column] = a.accumulate ? a.out[column] + sum : sum;
+  waves[wave][lane] = sum;
+  __syncthreads();
+  if (wave == 0 && column < a.n) {
+    const float total = (waves[0][lane] + waves[1][lane]) + (waves[2][lane] + waves[3][lane]);
+    a.out[column] = a.accumulate ? a.out[column] + total : total;
+  }
 }
 
 // ------------------------------------------------------------------ weights' gradients of few rows
@@ -328,7 +366,7 @@ struct Caller {
     KernelLaunch kernel;
     kernel.func = reinterpret_cast<const void *>(&band_sum_kernel);
     kernel.grid = dim3(blocks_of(args.n, 64));
-    kernel.block = dim3(64);
+    kernel.block = dim3(256);
     kernel.set_args(args);
     return launch(kernel, stream);
   }
@@ -336,8 +374,8 @@ struct Caller {
   hipError_t column_sums(const void *source, int64_t rows, int64_t n, int64_t ld, float *bands, float *out, bool accumulate) const;
 };
 
-// Bands of a column sum: enough workgroups for the chip, at least 16 rows each.
-int64_t column_sum_bands(int64_t rows) { return std::min<int64_t>((rows + 15) / 16, 64); }
+// Bands of a column sum: 64 rows, or more where that makes over 64 of them.
+int64_t column_sum_bands(int64_t rows) { return std::min<int64_t>((rows + kBandRowsOfSum - 1) / kBandRowsOfSum, 64); }
 
 hipError_t Caller::column_sums(const void *source, int64_t rows, int64_t n, int64_t ld, float *bands, float *out,
                                bool accumulate) const {
@@ -349,7 +387,7 @@ hipError_t Caller::column_sums(const void *source, int64_t rows, int64_t n, int6
   kernel.func = dtype == kDtypeF32   ? reinterpret_cast<const void *>(&column_sum_kernel<F32Payload>)
                 : dtype == kDtypeF16 ? reinterpret_cast<const void *>(&column_sum_kernel<F16Payload>)
                                      : reinterpret_cast<const void *>(&column_sum_kernel<Bf16Payload>);
-  kernel.grid = dim3(blocks_of(n, 256 * static_cast<int64_t>(16 / element)), static_cast<unsigned>(args.band_count));
+  kernel.grid = dim3(blocks_of(n, 64 * static_cast<int64_t>(16 / element)), static_cast<unsigned>(args.band_count));
   kernel.block = dim3(256);
   kernel.set_args(args);
   if (const hipError_t status = launch(kernel, stream); status != hipSuccess) {
