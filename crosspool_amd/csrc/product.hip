@@ -151,4 +151,73 @@ hipError_t launch_product(const ProductArgs &args, ProductEpilogue epilogue, boo
   return launch(launches.join, stream);
 }
 
+hipError_t launch_products(ProductGroup &group, const bool (&present)[3], int dtype, size_t scratch_bytes, hipStream_t stream) {
+  const int element = dtype == kDtypeF32 ? 4 : 2;
+  const int64_t slab = 128 / element;
+  double apart_us = 0.0;
+  int count = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (present[i]) {
+      const ProductArgs &part = group.part[i];
+      apart_us += plan_product(part.m, part.n, part.k, 1, element, false, scratch_bytes).us;
+      ++count;
+    }
+  }
+  // Together: the tiles in their order on a chip that is full to the last of them, or the longest tile's time.
+  double best_us = apart_us;
+  ProductTiles best = ProductTiles::k256;
+  for (const ProductCost &cost : element == 4 ? kCosts32 : kCosts16) {
+    if (count < 2 || cost.tiles == ProductTiles::k256 || cost.tiles == ProductTiles::k128Deep) {
+      continue;
+    }
+    const int64_t size = tile_size(cost.tiles);
+    double work = 0.0;
+    double longest = 0.0;
+    for (int i = 0; i < 3; ++i) {
+      if (present[i]) {
+        const ProductArgs &part = group.part[i];
+        const double slabs = static_cast<double>((part.k + slab - 1) / slab);
+        const double tiles = static_cast<double>(((part.m + size - 1) / size) * ((part.n + size - 1) / size));
+        const double each = slabs * cost.slab[cost.together - 1] + cost.around[cost.together - 1];
+        work += tiles * each / static_cast<double>(kCus * cost.together);
+        longest = std::max(longest, each);
+      }
+    }
+    const double us = kLaunchUs + std::max(longest, work + 0.5 * cost.around[cost.together - 1]);
+    if (us < best_us) {
+      best_us = us;
+      best = cost.tiles;
+    }
+  }
+  if (best == ProductTiles::k256) {
+    for (int i = 0; i < 3; ++i) {
+      if (present[i]) {
+        if (const hipError_t status = launch_product(group.part[i], ProductEpilogue::kStore, i > 0, true, dtype, scratch_bytes, stream);
+            status != hipSuccess) {
+          return status;
+        }
+      }
+    }
+    return hipSuccess;
+  }
+  int64_t blocks = 0;
+  for (int i = 0; i < 3; ++i) {
+    ProductArgs &part = group.part[i];
+    group.blocks[i] = 0;
+    if (present[i]) {
+      const int64_t size = tile_size(best);
+      part.tile_rows = static_cast<int32_t>((part.m + size - 1) / size);
+      part.tile_cols = static_cast<int32_t>((part.n + size - 1) / size);
+      part.whole = part.tile_rows * part.tile_cols;
+      group.blocks[i] = part.whole;
+      blocks += part.whole;
+    }
+  }
+  const void *kernel = dtype == kDtypeF32   ? ProductKernels<F32Payload>::group(best)
+                       : dtype == kDtypeF16 ? ProductKernels<F16Payload>::group(best)
+                                            : ProductKernels<Bf16Payload>::group(best);
+  void *params[] = {&group};
+  return hipLaunchKernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), params, 0, stream);
+}
+
 }  // namespace xp

@@ -96,8 +96,18 @@ ProductLaunch make_product(const ProductArgs &args, const ProductPlan &plan, Pro
 hipError_t launch_product(const ProductArgs &args, ProductEpilogue epilogue, bool a_cols, bool b_cols, int dtype,
                           size_t scratch_bytes, hipStream_t stream);
 
+// Products of one backward pass that do not depend on each other, kStore: an inputs' gradient (part 0, blocks 0 where there
+// is none) and up to two weights' gradients.
+struct ProductGroup {
+  ProductArgs part[3];
+  int32_t blocks[3];
+};
+// All of them, in one launch where that is modelled as faster than one after another.  `present` says which there are.
+hipError_t launch_products(ProductGroup &group, const bool (&present)[3], int dtype, size_t scratch_bytes, hipStream_t stream);
+
 template <class P>
 struct ProductKernels {
+  static const void *group(ProductTiles tiles);
   static const void *main(ProductTiles tiles, ProductEpilogue epilogue, bool a_cols, bool b_cols);
   static const void *join(int tile, ProductEpilogue epilogue);
 };

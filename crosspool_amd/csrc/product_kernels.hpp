@@ -709,9 +709,17 @@ constexpr int kTileGroup = TILE == 256 ? 4 : 8;
 // issues loads stalls, and its SIMD's other wave keeps the matrix pipe busy).  The slab schedule is that of the
 // projections' tile kernel: fragments are read one k step ahead of their MFMAs from two register sets, and the
 // barrier sits where the slab's last fragments have been read.
-template <class P, int TILE, int WAVES_M, int WAVES_N, int STAGES, bool A_COLS, bool B_COLS, ProductEpilogue EPI>
-__global__ __launch_bounds__(TILE == 32 ? 256 : 64 * WAVES_M * WAVES_N, TILE == 32 ? 4 : TILE == 64 ? 3 : TILE == 128 && STAGES > 2 ? 1 : 2) void product_kernel(
-    ProductArgs a) {
+template <int TILE, int STAGES>
+constexpr int kStageBytes = 2 * STAGES * TILE * 128;
+// Waves of a SIMD that the registers have to leave room for.
+template <int TILE, int STAGES>
+constexpr int kProductWaves = TILE == 32 ? 4 : TILE == 64 ? 3 : TILE == 128 && STAGES > 2 ? 1 : 2;
+template <int TILE, int WAVES_M, int WAVES_N>
+constexpr int kProductThreads = TILE == 32 ? 256 : 64 * WAVES_M * WAVES_N;
+
+// Workgroup `block` of a product's.  MAY_SPLIT: tiles behind the whole ones may be shared by workers.
+template <class P, int TILE, int WAVES_M, int WAVES_N, int STAGES, bool A_COLS, bool B_COLS, ProductEpilogue EPI, bool MAY_SPLIT>
+__device__ __forceinline__ void product_body(const ProductArgs &a, uint32_t block, unsigned char *lds) {
   constexpr int ES = kElementBytes<P>;
   constexpr int BK = 128 / ES;
   // 32 x 32 tiles: the four waves take one k step of every slab each and add their sums in the epilogue.
@@ -733,8 +741,7 @@ __global__ __launch_bounds__(TILE == 32 ? 256 : 64 * WAVES_M * WAVES_N, TILE == 
   constexpr int PITCH = WTN + 4;  // floats of a staged row of the epilogue
   static_assert(WAVES * 32 * PITCH * 4 <= 2 * REGION, "the epilogue's rows must fit the stages");
 
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * REGION];
-
+  static_assert(kStageBytes<TILE, STAGES> == 2 * REGION, "the kernel's LDS");
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int wm = SPREAD ? 0 : wave % WAVES_M;
   const int wn = SPREAD ? 0 : wave / WAVES_M;
@@ -743,11 +750,11 @@ __global__ __launch_bounds__(TILE == 32 ? 256 : 64 * WAVES_M * WAVES_N, TILE == 
   const uint32_t tile_slabs = static_cast<uint32_t>((a.k + BK - 1) / BK);
   // Whole tiles first, one a workgroup; then the workers of the split tiles, each with one run of their slabs, the end
   // of one tile and the begin of the next among them (the host gives a worker at least one slab).
-  constexpr bool SPLITS = TILE == 128 || TILE == 64;  // what a split saves 256 x 256 tiles goes into their pieces' 256 KB
+  constexpr bool SPLITS = MAY_SPLIT && (TILE == 128 || TILE == 64);  // what a split saves 256 x 256 tiles goes into their pieces' 256 KB
   const uint32_t whole = static_cast<uint32_t>(a.whole);
-  const bool worker = SPLITS && blockIdx.x >= whole;
+  const bool worker = SPLITS && block >= whole;
   // Where every tile has the same number of workers, those of one part of K come one after another: they share slabs.
-  uint32_t q = worker ? place_of(blockIdx.x - whole, static_cast<uint32_t>(a.workers)) : 0;
+  uint32_t q = worker ? place_of(block - whole, static_cast<uint32_t>(a.workers)) : 0;
   if (worker && a.each > 1) {
     const uint32_t part = q / static_cast<uint32_t>(a.split);
     q = (q - part * static_cast<uint32_t>(a.split)) * static_cast<uint32_t>(a.each) + part;
@@ -765,7 +772,7 @@ __global__ __launch_bounds__(TILE == 32 ? 256 : 64 * WAVES_M * WAVES_N, TILE == 
   b_fragments.setup(REGION, wn * NT, SPREAD ? wave : 0, lane);
   const lds_bytes_t shared = (lds_bytes_t)lds;
   const uint32_t local = worker ? next / tile_slabs : 0;  // among the split tiles
-  const ProductTile at = product_tile<kTileGroup<TILE>>(a, worker ? whole + local : place_of(blockIdx.x, whole));
+  const ProductTile at = product_tile<kTileGroup<TILE>>(a, worker ? whole + local : place_of(block, whole));
   const uint32_t first_slab = next - local * tile_slabs;
   const int slabs = static_cast<int>(tile_slabs - first_slab < stop - next ? tile_slabs - first_slab : stop - next);
   next += static_cast<uint32_t>(slabs);
@@ -1115,6 +1122,29 @@ __global__ __launch_bounds__(TILE == 32 ? 256 : 64 * WAVES_M * WAVES_N, TILE == 
   } while (SPLITS && next < stop);
 }
 
+template <class P, int TILE, int WAVES_M, int WAVES_N, int STAGES, bool A_COLS, bool B_COLS, ProductEpilogue EPI>
+__global__ __launch_bounds__((kProductThreads<TILE, WAVES_M, WAVES_N>), (kProductWaves<TILE, STAGES>)) void product_kernel(ProductArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[kStageBytes<TILE, STAGES>];
+  product_body<P, TILE, WAVES_M, WAVES_N, STAGES, A_COLS, B_COLS, EPI, true>(a, blockIdx.x, lds);
+}
+
+// Up to three products of one backward pass in one launch, whole tiles: their last rounds, which each by itself would leave
+// most CUs idle in, are one.  The first (of an empty grid where there is none) is an inputs' gradient, the others
+// weights' gradients.
+template <class P, int TILE, int WAVES_M, int WAVES_N, int STAGES>
+__global__ __launch_bounds__((kProductThreads<TILE, WAVES_M, WAVES_N>), (kProductWaves<TILE, STAGES>)) void product_group_kernel(ProductGroup g) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[kStageBytes<TILE, STAGES>];
+  uint32_t block = blockIdx.x;
+  if (block < static_cast<uint32_t>(g.blocks[0])) {
+    product_body<P, TILE, WAVES_M, WAVES_N, STAGES, false, true, ProductEpilogue::kStore, false>(g.part[0], block, lds);
+    return;
+  }
+  block -= static_cast<uint32_t>(g.blocks[0]);
+  const int at = block < static_cast<uint32_t>(g.blocks[1]) ? 1 : 2;
+  block -= at == 2 ? static_cast<uint32_t>(g.blocks[1]) : 0u;
+  product_body<P, TILE, WAVES_M, WAVES_N, STAGES, true, true, ProductEpilogue::kStore, false>(g.part[at], block, lds);
+}
+
 // ------------------------------------------------------------------ split tiles
 // The sum of a split tile's pieces in the order of their slabs, then the epilogue.  A workgroup takes 32 rows of 64
 // columns, with the loads of four pieces in flight; the column sums of its band are added through LDS in wave order.
@@ -1283,6 +1313,13 @@ const void *ProductKernels<P>::main(ProductTiles tiles, ProductEpilogue epilogue
     default:
       return product_tile_kernel<P, 32, 1, 1, 4>(epilogue, a_cols, b_cols);
   }
+}
+
+template <class P>
+const void *ProductKernels<P>::group(ProductTiles tiles) {
+  return tiles == ProductTiles::k128Pairs ? reinterpret_cast<const void *>(&product_group_kernel<P, 128, 2, 2, 2>)
+         : tiles == ProductTiles::k64     ? reinterpret_cast<const void *>(&product_group_kernel<P, 64, 2, 2, 3>)
+                                          : reinterpret_cast<const void *>(&product_group_kernel<P, 32, 1, 1, 4>);
 }
 
 template <class P>

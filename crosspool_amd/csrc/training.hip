@@ -94,12 +94,14 @@ __global__ __launch_bounds__(256) void column_sum_kernel(ColumnSumArgs a) {
   const int wave = threadIdx.x >> 6;
   const int64_t column = (static_cast<int64_t>(blockIdx.x) * 64 + lane) * CHUNK;
   const bool live = column < a.n;
-  const bool whole = a.n - column >= CHUNK;
+  // The last chunk of a ragged row is read where it ends with the row (its first columns again, which another lane stores).
+  const int64_t from_column = a.n - column >= CHUNK || a.n < CHUNK ? column : a.n - CHUNK;
+  const bool whole = a.n >= CHUNK;
   const int64_t first = static_cast<int64_t>(blockIdx.y) * a.band_rows;
   const int64_t last = first + a.band_rows < a.rows ? first + a.band_rows : a.rows;
   const auto row_at = [&](int64_t row) __attribute__((always_inline)) {
-    const unsigned char *from = static_cast<const unsigned char *>(a.source) + (row * a.ld + column) * ES;
-    return whole ? load16_any(from) : load_chunk_tail<P, P>(from, a.n - column);
+    const unsigned char *from = static_cast<const unsigned char *>(a.source) + (row * a.ld + from_column) * ES;
+    return whole ? load16_any(from) : load_chunk_tail<P, P>(from, a.n);
   };
   float sum[CHUNK] = {};
   const auto add = [&](const u32x4 &chunk) __attribute__((always_inline)) {
@@ -138,10 +140,10 @@ __global__ __launch_bounds__(256) void column_sum_kernel(ColumnSumArgs a) {
     return;
   }
   const bool alone = a.band_count == 1;
-  float *to = (alone ? a.out : a.bands + static_cast<int64_t>(blockIdx.y) * a.n) + column;
+  float *to = (alone ? a.out : a.bands + static_cast<int64_t>(blockIdx.y) * a.n) + from_column;
 #pragma unroll
   for (int j = 0; j < CHUNK; ++j) {
-    if (column + j < a.n) {
+    if (from_column + j >= column && from_column + j < a.n) {
       const float total = (waves[0][j][lane] + waves[1][j][lane]) + (waves[2][j][lane] + waves[3][j][lane]);
       to[j] = alone && a.accumulate ? to[j] + total : total;
     }
@@ -313,6 +315,14 @@ struct Caller {
     args.partials = scratch;
     args.batch = 1;
     return launch_product(args, epilogue, a_cols, b_cols, dtype, scratch_bytes, stream);
+  }
+
+  hipError_t products(ProductGroup &group, const bool (&present)[3]) const {
+    for (ProductArgs &part : group.part) {
+      part.partials = scratch;
+      part.batch = 1;
+    }
+    return launch_products(group, present, dtype, scratch_bytes, stream);
   }
 
   // `source` itself where its rows are whole chunks, else a padded copy in `target`, which `pads` then has to make.
@@ -640,15 +650,17 @@ int xp_projection_backward(const void *x, int64_t ld_x, int64_t rows, int64_t k,
     inputs = call.padded(x, rows, k, ld_x, at.x, pads);
   }
   XP_HIP_CHECK(call.pad(pads));
-  if (grad_x != nullptr) {
-    ProductArgs args = inputs_args(grad, weights, rows, n, k, grad_x, ld_grad_x, dtype);
-    XP_HIP_CHECK(call.product(args, ProductEpilogue::kStore, false, true));
+  ProductGroup group{};
+  const bool present[3] = {grad_x != nullptr, grad_w != nullptr && !thin, false};
+  if (present[0]) {
+    group.part[0] = inputs_args(grad, weights, rows, n, k, grad_x, ld_grad_x, dtype);
   }
+  if (present[1]) {
+    group.part[1] = outer_args(grad, n, inputs, k, rows, grad_w, grad_w_dtype, accumulate != 0);
+  }
+  XP_HIP_CHECK(call.products(group, present));
   if (grad_w != nullptr && thin) {
     XP_HIP_CHECK(call.thin_outer(ThinOuterArgs{grad_out, x, grad_w, ld_grad, ld_x, n, k, static_cast<int32_t>(rows), grad_w_dtype, accumulate}));
-  } else if (grad_w != nullptr) {
-    ProductArgs args = outer_args(grad, n, inputs, k, rows, grad_w, grad_w_dtype, accumulate != 0);
-    XP_HIP_CHECK(call.product(args, ProductEpilogue::kStore, true, true));
   }
   if (grad_bias != nullptr) {
     XP_HIP_CHECK(call.column_sums(grad_out, rows, n, ld_grad, at.bands, grad_bias, accumulate != 0));
@@ -832,22 +844,26 @@ int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden,
           PadJob{nullptr, at.through, rows, wide, 0, through_ld, 0}, static_cast<int>(element));
       XP_HIP_CHECK(hipGetLastError());
     }
-    ProductArgs product = inputs_args(through, w_in_rows, rows, wide, hidden, grad_x, ld_grad_x, dtype);
-    XP_HIP_CHECK(call.product(product, ProductEpilogue::kStore, false, true));
   }
-  if (grad_w_in != nullptr && thin) {
+  ProductGroup group{};
+  const bool present[3] = {grad_x != nullptr, grad_w_in != nullptr && !thin, grad_w_out != nullptr && !thin};
+  if (present[0]) {
+    group.part[0] = inputs_args(through, w_in_rows, rows, wide, hidden, grad_x, ld_grad_x, dtype);
+  }
+  if (present[1]) {
+    group.part[1] = outer_args(through, wide, inputs, hidden, rows, grad_w_in, grad_w_dtype, accumulate != 0);
+  }
+  if (present[2]) {
+    group.part[2] = outer_args(grad, hidden, activated, width, rows, grad_w_out, grad_w_dtype, accumulate != 0);
+  }
+  XP_HIP_CHECK(call.products(group, present));
+  if (thin && grad_w_in != nullptr) {
     XP_HIP_CHECK(call.thin_outer(
         ThinOuterArgs{at.through, x, grad_w_in, through_ld, ld_x, wide, hidden, static_cast<int32_t>(rows), grad_w_dtype, accumulate}));
-  } else if (grad_w_in != nullptr) {
-    ProductArgs product = outer_args(through, wide, inputs, hidden, rows, grad_w_in, grad_w_dtype, accumulate != 0);
-    XP_HIP_CHECK(call.product(product, ProductEpilogue::kStore, true, true));
   }
-  if (grad_w_out != nullptr && thin) {
+  if (thin && grad_w_out != nullptr) {
     XP_HIP_CHECK(call.thin_outer(ThinOuterArgs{grad_out, at.activated, grad_w_out, ld_grad, activated.ld, hidden, width,
                                                static_cast<int32_t>(rows), grad_w_dtype, accumulate}));
-  } else if (grad_w_out != nullptr) {
-    ProductArgs product = outer_args(grad, hidden, activated, width, rows, grad_w_out, grad_w_dtype, accumulate != 0);
-    XP_HIP_CHECK(call.product(product, ProductEpilogue::kStore, true, true));
   }
   if (grad_bias_out != nullptr) {
     XP_HIP_CHECK(call.column_sums(grad_out, rows, hidden, ld_grad, at.bands, grad_bias_out, accumulate != 0));
