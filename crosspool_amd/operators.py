@@ -521,7 +521,8 @@ class DenseExecutionPlan:
                 capacity, hidden, signature.local_intermediate_size, int(signature.activation.gate is not None), code))
             if needed == 0:
                 raise ValueError("a Dense layer's backward pass takes 1 to 2^24 rows, widths of 1 to 2^20 and bf16, fp16 or fp32")
-            needed = max(needed, int(lib.xp_projection_keep_workspace_bytes(capacity, wide, hidden, code)))
+            needed = max(needed, int(lib.xp_projection_keep_workspace_bytes(capacity, wide, hidden, code)),
+                         int(lib.xp_projection_keep_workspace_bytes(capacity, hidden, signature.local_intermediate_size, code)))
             regions.append((torch.uint8, (needed,)))
         return cls(signature, i_proj, o_proj, WorkspaceLayout.from_regions(tuple(regions)), adapters, *plans, backward)
 
@@ -643,7 +644,16 @@ class Dense:
         )
         if not fused:
             signature.activation.apply_into(inputs=projected, output=activated, order=order)
-        self.o_proj.run_into(activated, layer_weights.o_proj, output=output)
+        if dtype is not torch.float32:
+            self.o_proj.run_into(activated, layer_weights.o_proj, output=output)
+            return
+        # fp32: the training products' tiles (494 rows of 8288 x 11584: 711 us) rather than the general projection's (887).
+        width, bias = signature.local_intermediate_size, layer_weights.o_proj.bias
+        _native.call(
+            "xp_projection_keep", activated.data_ptr(), width, rows, width, layer_weights.o_proj.values.data_ptr(), hidden,
+            None if bias is None else bias.data_ptr(), output.data_ptr(), hidden, None, _DTYPE_CODES[dtype], None,
+            signature.payload_row_capacity, scratch.data_ptr(), scratch.numel(), _native.current_stream(index),
+        )
 
     def backward_into(
         self,
