@@ -458,9 +458,11 @@ __device__ __forceinline__ uint32_t read_word(lds_bytes_t at) {
 // resource's `bytes` write zeros.  Written as an instruction because the compiler, which does not know the stages
 // apart, waits for every load in flight before a ds_read_b64_tr (64 x 64 tiles: 0.57 us a slab instead of 0.27).  It
 // has no result in a register; the kernel waits for its arrival itself, before a barrier that is a memory clobber.
-// (One wait state between writing M0 and the load that takes its LDS address from it.)
+// The compiler does not see a memory instruction here and adds no wait states: a load needs one behind the write of M0
+// that it takes its LDS address from, and five behind a vector instruction that wrote one of its scalar registers (a
+// readlane that brings a spilled one back).
 __device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t to, uint32_t voffset, uint32_t soffset) {
-  __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                    :
                    : "s"(to), "v"(voffset), "s"(rsrc), "s"(soffset)
                    : "m0");

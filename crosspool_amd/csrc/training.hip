@@ -598,7 +598,7 @@ int xp_projection_backward(const void *x, int64_t ld_x, int64_t rows, int64_t k,
   const size_t element = dtype_bytes(dtype);
   XP_REQUIRE(element != 0, "payload dtype must be bf16, fp16 or fp32");
   XP_REQUIRE(extents_valid(rows, n, k) && rows <= capacity && capacity <= kMaxRows, kExtents);
-  XP_REQUIRE(w != nullptr && aligned16(w), "projection weights must be non-null and 16-byte aligned");
+  XP_TRY(check_rows("projection weights", w, k, k, element, true));
   if (grad_w != nullptr) {
     XP_TRY(check_weight_gradient("weight gradient", grad_w, grad_w_dtype, dtype));
   }
@@ -686,7 +686,7 @@ int xp_projection_keep(const void *x, int64_t ld_x, int64_t rows, int64_t k, con
   if (rows == 0) {
     return XP_OK;
   }
-  XP_REQUIRE(w != nullptr && aligned16(w), "projection weights must be non-null and 16-byte aligned");
+  XP_TRY(check_rows("projection weights", w, k, k, element, true));
   XP_TRY(check_rows("projection input", x, ld_x, k, element, true));
   XP_TRY(check_rows("kept projection", projected, ld_projected, n, element, false));
   XP_REQUIRE(aligned_to(bias, 4) && aligned_to(activated, element), "bias and activated outputs must be aligned to their element size");
@@ -774,8 +774,8 @@ int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden,
     }
     return XP_OK;
   }
-  XP_REQUIRE(w_in != nullptr && w_out != nullptr && aligned16(w_in) && aligned16(w_out),
-             "projection weights must be non-null and 16-byte aligned");
+  XP_TRY(check_rows("input projection's weights", w_in, hidden, hidden, element, true));
+  XP_TRY(check_rows("output projection's weights", w_out, width, width, element, true));
   XP_TRY(check_rows("kept projection", projected, ld_projected, wide, element, false));
   XP_TRY(check_rows("output gradient", grad_out, ld_grad, hidden, element, true));
   if (grad_w_in != nullptr) {

@@ -566,7 +566,7 @@ int xp_moe_experts(const void *hidden_states, int64_t rows, int64_t hidden, int6
  *   grad_x [rows, k] = grad_out . w,  grad_w [n, k] = grad_out^T . x,  grad_bias [n] (fp32) = sum of grad_out's rows,
  * each left out where NULL.  All of dtype (XP_DTYPE_BF16, F16 or F32) but grad_w, of grad_w_dtype: dtype or fp32.
  * accumulate adds grad_w and grad_bias to what they hold.  ld_x, ld_grad and ld_grad_x are row strides in elements;
- * w and grad_w are contiguous.  x and grad_out rows of whole 16 bytes must start on 16-byte boundaries, as must w.
+ * w and grad_w are contiguous.  Rows of x, w and grad_out of whole 16 bytes must start on 16-byte boundaries.
  * Sums are fp32 and have one order: repeated calls give the same bits.  No rows: grad_w and grad_bias are
  * cleared (accumulate: left).  Outputs and workspace may overlap neither the operands nor each other.
  * The workspace serves every row count up to `capacity`, the rows that its size was asked for.  No counterpart in the
