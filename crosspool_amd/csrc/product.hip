@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <iterator>
 
 namespace xp {
 
@@ -24,11 +25,19 @@ constexpr ProductCost kCosts16[] = {{ProductTiles::k256, 1, {1.38}, {8.2}},
                                     {ProductTiles::k128Deep, 1, {0.5}, {6.3}},
                                     {ProductTiles::k64, 3, {0.245, 0.38, 0.52}, {2.3, 3.0, 3.9}},
                                     {ProductTiles::k32, 4, {0.155, 0.22, 0.36, 0.46}, {0.8, 1.1, 1.4, 1.7}}};
-constexpr ProductCost kCosts32[] = {{ProductTiles::k256, 1, {7.4}, {14.0}},
-                                    {ProductTiles::k128Pairs, 2, {1.95, 3.67}, {7.0, 7.5}},
-                                    {ProductTiles::k128Deep, 1, {2.08}, {7.0}},
+constexpr ProductCost kCosts32[] = {{ProductTiles::k128Pairs, 2, {1.95, 3.67}, {7.0, 7.5}},
                                     {ProductTiles::k64, 3, {0.62, 1.05, 1.49}, {2.4, 3.4, 4.6}},
                                     {ProductTiles::k32, 4, {0.235, 0.345, 0.48, 0.6}, {0.9, 1.3, 1.6, 2.0}}};
+struct ProductCosts {
+  const ProductCost *first;
+  const ProductCost *last;
+  const ProductCost *begin() const { return first; }
+  const ProductCost *end() const { return last; }
+};
+ProductCosts costs_of(int element_bytes) {
+  return element_bytes == 4 ? ProductCosts{std::begin(kCosts32), std::end(kCosts32)}
+                            : ProductCosts{std::begin(kCosts16), std::end(kCosts16)};
+}
 constexpr int64_t kCus = 256;
 constexpr double kLaunchUs = 2.3;
 constexpr double kJoinUs = 3.0;       // its launch,
@@ -60,7 +69,7 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int64_t batch, int ele
   const int64_t slabs = (k + slab - 1) / slab;
   ProductPlan best{};
   best.us = -1.0;
-  for (const ProductCost &cost : element_bytes == 4 ? kCosts32 : kCosts16) {
+  for (const ProductCost &cost : costs_of(element_bytes)) {
     const int64_t size = tile_size(cost.tiles);
     const int64_t rows = (m + size - 1) / size;
     const int64_t cols = (n + size - 1) / size;
@@ -166,7 +175,7 @@ hipError_t launch_products(ProductGroup &group, const bool (&present)[3], int dt
   // Together: the tiles in their order on a chip that is full to the last of them, or the longest tile's time.
   double best_us = apart_us;
   ProductTiles best = ProductTiles::k256;
-  for (const ProductCost &cost : element == 4 ? kCosts32 : kCosts16) {
+  for (const ProductCost &cost : costs_of(element)) {
     if (count < 2 || cost.tiles == ProductTiles::k256 || cost.tiles == ProductTiles::k128Deep) {
       continue;
     }

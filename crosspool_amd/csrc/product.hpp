@@ -63,7 +63,7 @@ struct ProductArgs {
 };
 static_assert(sizeof(ProductArgs) <= 288, "a kernel's argument record");
 
-// Tile sizes, stages of LDS and workgroups that a CU holds.
+// Tile sizes, stages of LDS and workgroups that a CU holds (fp32: k128Pairs, k64 and k32).
 enum class ProductTiles : int { k256 = 0, k128Pairs = 1, k128Deep = 2, k64 = 3, k32 = 4 };
 constexpr int tile_size(ProductTiles tiles) {
   return tiles == ProductTiles::k256 ? 256 : tiles == ProductTiles::k64 ? 64 : tiles == ProductTiles::k32 ? 32 : 128;

@@ -461,12 +461,15 @@ __device__ __forceinline__ uint32_t read_word(lds_bytes_t at) {
 // The compiler does not see a memory instruction here and adds no wait states: a load needs one behind the write of M0
 // that it takes its LDS address from, and five behind a vector instruction that wrote one of its scalar registers (a
 // readlane that brings a spilled one back).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // M0 among the clobbers: the compiler keeps nothing in it
 __device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t to, uint32_t voffset, uint32_t soffset) {
   __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                    :
                    : "s"(to), "v"(voffset), "s"(rsrc), "s"(soffset)
                    : "m0");
 }
+#pragma clang diagnostic pop
 // The words of a raw buffer resource (make_rsrc), in scalar registers.
 __device__ __forceinline__ u32x4 resource_words(const void *base, uint32_t bytes) {
   const uint64_t address = reinterpret_cast<uint64_t>(base);
@@ -764,363 +767,363 @@ __device__ __forceinline__ void product_body(const ProductArgs &a, uint32_t bloc
   uint32_t next = worker ? split_begin(a, q) : 0;
   const uint32_t stop = worker ? split_begin(a, q + 1) : tile_slabs;
   do {
-  // Opaque, here and before the epilogue: what follows from it is computed where it is used, not kept in registers
-  // around the loop (two workgroups of 128 x 128 no longer fit a CU then).
-  int lane = threadIdx.x & 63;
-  __asm__ volatile("" : "+v"(lane));
-  OperandFragments<P, TILE, A_COLS, MT, STAGES> a_fragments;
-  OperandFragments<P, TILE, B_COLS, NT, STAGES> b_fragments;
-  a_fragments.setup(0, wm * MT, SPREAD ? wave : 0, lane);
-  b_fragments.setup(REGION, wn * NT, SPREAD ? wave : 0, lane);
-  const lds_bytes_t shared = (lds_bytes_t)lds;
-  const uint32_t local = worker ? next / tile_slabs : 0;  // among the split tiles
-  const ProductTile at = product_tile<kTileGroup<TILE>>(a, worker ? whole + local : place_of(block, whole));
-  const uint32_t first_slab = next - local * tile_slabs;
-  const int slabs = static_cast<int>(tile_slabs - first_slab < stop - next ? tile_slabs - first_slab : stop - next);
-  next += static_cast<uint32_t>(slabs);
-  const int64_t m0 = static_cast<int64_t>(at.m) * TILE;
-  const int64_t n0 = static_cast<int64_t>(at.n) * TILE;
-  const int64_t k_begin = static_cast<int64_t>(first_slab) * BK;
-  const int64_t k_end = a.k - k_begin < static_cast<int64_t>(slabs) * BK ? a.k : k_begin + static_cast<int64_t>(slabs) * BK;
-  ALoads a_loads;
-  BLoads b_loads;
-  a_loads.setup(static_cast<const unsigned char *>(a.a.data) + at.matrix * a.a.batch * ES, a.a.ld, m0, a.m - m0, wave, lane);
-  b_loads.setup(static_cast<const unsigned char *>(a.b.data) + at.matrix * a.b.batch * ES, a.b.ld, n0, a.n - n0, wave, lane);
-  const uint32_t lds_begin = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>((uintptr_t)shared)));
-  auto issue = [&](int number, int stage) XP_INLINE {
-    const int64_t k_pos = k_begin + static_cast<int64_t>(number) * BK;
-    const typename ALoads::Slab a_slab = a_loads.slab(k_pos, k_end);
-    const typename BLoads::Slab b_slab = b_loads.slab(k_pos, k_end);
+    // Opaque, here and before the epilogue: what follows from it is computed where it is used, not kept in registers
+    // around the loop (two workgroups of 128 x 128 no longer fit a CU then).
+    int lane = threadIdx.x & 63;
+    __asm__ volatile("" : "+v"(lane));
+    OperandFragments<P, TILE, A_COLS, MT, STAGES> a_fragments;
+    OperandFragments<P, TILE, B_COLS, NT, STAGES> b_fragments;
+    a_fragments.setup(0, wm * MT, SPREAD ? wave : 0, lane);
+    b_fragments.setup(REGION, wn * NT, SPREAD ? wave : 0, lane);
+    const lds_bytes_t shared = (lds_bytes_t)lds;
+    const uint32_t local = worker ? next / tile_slabs : 0;  // among the split tiles
+    const ProductTile at = product_tile<kTileGroup<TILE>>(a, worker ? whole + local : place_of(block, whole));
+    const uint32_t first_slab = next - local * tile_slabs;
+    const int slabs = static_cast<int>(tile_slabs - first_slab < stop - next ? tile_slabs - first_slab : stop - next);
+    next += static_cast<uint32_t>(slabs);
+    const int64_t m0 = static_cast<int64_t>(at.m) * TILE;
+    const int64_t n0 = static_cast<int64_t>(at.n) * TILE;
+    const int64_t k_begin = static_cast<int64_t>(first_slab) * BK;
+    const int64_t k_end = a.k - k_begin < static_cast<int64_t>(slabs) * BK ? a.k : k_begin + static_cast<int64_t>(slabs) * BK;
+    ALoads a_loads;
+    BLoads b_loads;
+    a_loads.setup(static_cast<const unsigned char *>(a.a.data) + at.matrix * a.a.batch * ES, a.a.ld, m0, a.m - m0, wave, lane);
+    b_loads.setup(static_cast<const unsigned char *>(a.b.data) + at.matrix * a.b.batch * ES, a.b.ld, n0, a.n - n0, wave, lane);
+    const uint32_t lds_begin = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>((uintptr_t)shared)));
+    auto issue = [&](int number, int stage) XP_INLINE {
+      const int64_t k_pos = k_begin + static_cast<int64_t>(number) * BK;
+      const typename ALoads::Slab a_slab = a_loads.slab(k_pos, k_end);
+      const typename BLoads::Slab b_slab = b_loads.slab(k_pos, k_end);
 #pragma unroll
-    for (int q = 0; q < ALoads::LOADS; ++q) {
-      a_loads.load(a_slab, q, lds_begin + stage * STAGE);
-    }
-#pragma unroll
-    for (int q = 0; q < BLoads::LOADS; ++q) {
-      b_loads.load(b_slab, q, lds_begin + REGION + stage * STAGE);
-    }
-  };
-
-  f32x16 acc[MT][NT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        acc[mt][nt][r] = 0.0f;
+      for (int q = 0; q < ALoads::LOADS; ++q) {
+        a_loads.load(a_slab, q, lds_begin + stage * STAGE);
       }
-    }
-  }
-  // Wave tiles of up to four accumulators hold a whole slab's fragments twice: their few MFMAs a k step are shorter than
-  // the LDS latency, so the next slab's are all read under this slab's MFMAs.  Larger ones read one k step ahead.
-  constexpr bool WHOLE_SLABS = MT * NT == 1 || (MT * NT == 4 && STAGES > 2);
-  u32x4 af[WHOLE_SLABS ? 2 * STEPS : 2][MT];
-  u32x4 bf[WHOLE_SLABS ? 2 * STEPS : 2][NT];
-  auto read_fragments = [&](int stage, int ks, int slot) XP_INLINE {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      af[slot][mt] = a_fragments.read(shared, stage, ks, mt);
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      bf[slot][nt] = b_fragments.read(shared, stage, ks, nt);
-    }
-  };
-  auto multiply = [&](int slot) XP_INLINE {
+      for (int q = 0; q < BLoads::LOADS; ++q) {
+        b_loads.load(b_slab, q, lds_begin + REGION + stage * STAGE);
+      }
+    };
+
+    f32x16 acc[MT][NT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        acc[mt][nt] = P::mfma32(bf[slot][nt], af[slot][mt], acc[mt][nt]);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          acc[mt][nt][r] = 0.0f;
+        }
       }
     }
-  };
-  // Each wave waits for its loads of the next slab and for its own LDS reads; past the barrier every wave may
-  // read the next slab and the stage just read may be refilled.
-  auto stage_barrier = []() XP_INLINE {
-    constexpr int N = LOADS * (STAGES - 2);
-    __builtin_amdgcn_s_waitcnt((N & 0xf) | ((N >> 4) << 14) | (0x7 << 4));  // vmcnt(N) lgkmcnt(0)
-    __builtin_amdgcn_sched_barrier(0);
-    __asm__ volatile("s_barrier" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-  };
+    // Wave tiles of up to four accumulators hold a whole slab's fragments twice: their few MFMAs a k step are shorter than
+    // the LDS latency, so the next slab's are all read under this slab's MFMAs.  Larger ones read one k step ahead.
+    constexpr bool WHOLE_SLABS = MT * NT == 1 || (MT * NT == 4 && STAGES > 2);
+    u32x4 af[WHOLE_SLABS ? 2 * STEPS : 2][MT];
+    u32x4 bf[WHOLE_SLABS ? 2 * STEPS : 2][NT];
+    auto read_fragments = [&](int stage, int ks, int slot) XP_INLINE {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        af[slot][mt] = a_fragments.read(shared, stage, ks, mt);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        bf[slot][nt] = b_fragments.read(shared, stage, ks, nt);
+      }
+    };
+    auto multiply = [&](int slot) XP_INLINE {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          acc[mt][nt] = P::mfma32(bf[slot][nt], af[slot][mt], acc[mt][nt]);
+        }
+      }
+    };
+    // Each wave waits for its loads of the next slab and for its own LDS reads; past the barrier every wave may
+    // read the next slab and the stage just read may be refilled.
+    auto stage_barrier = []() XP_INLINE {
+      constexpr int N = LOADS * (STAGES - 2);
+      __builtin_amdgcn_s_waitcnt((N & 0xf) | ((N >> 4) << 14) | (0x7 << 4));  // vmcnt(N) lgkmcnt(0)
+      __builtin_amdgcn_sched_barrier(0);
+      __asm__ volatile("s_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
 
-  if (loading_wave) {
+    if (loading_wave) {
 #pragma unroll
-    for (int s = 0; s < STAGES; ++s) {
-      issue(s, s);
+      for (int s = 0; s < STAGES; ++s) {
+        issue(s, s);
+      }
     }
-  }
-  wait_vmcnt<LOADS * (STAGES - 1)>();
-  __syncthreads();
-  auto read_slab = [&](int stage, int set) XP_INLINE {
+    wait_vmcnt<LOADS * (STAGES - 1)>();
+    __syncthreads();
+    auto read_slab = [&](int stage, int set) XP_INLINE {
 #pragma unroll
-    for (int ks = 0; ks < STEPS; ++ks) {
-      read_fragments(stage, ks, set * STEPS + ks);
-    }
-  };
-  auto multiply_slab = [&](int set) XP_INLINE {
+      for (int ks = 0; ks < STEPS; ++ks) {
+        read_fragments(stage, ks, set * STEPS + ks);
+      }
+    };
+    auto multiply_slab = [&](int set) XP_INLINE {
 #pragma unroll
-    for (int ks = 0; ks < STEPS; ++ks) {
-      multiply(set * STEPS + ks);
-    }
-  };
-  if constexpr (WHOLE_SLABS) {
-    read_slab(0, 0);
-  } else {
-    read_fragments(0, 0, 0);
-  }
-
-  constexpr int UNROLL = WHOLE_SLABS && STAGES % 2 != 0 ? 2 * STAGES : STAGES;
-  auto slab = [&](auto index, auto loads, int number) XP_INLINE {
-    constexpr int S = decltype(index)::value % STAGES;
-    constexpr int NEXT = (S + 1) % STAGES;
-    constexpr bool LOADING = decltype(loads)::value;
+      for (int ks = 0; ks < STEPS; ++ks) {
+        multiply(set * STEPS + ks);
+      }
+    };
     if constexpr (WHOLE_SLABS) {
-      constexpr int SET = decltype(index)::value % 2;
+      read_slab(0, 0);
+    } else {
+      read_fragments(0, 0, 0);
+    }
+
+    constexpr int UNROLL = WHOLE_SLABS && STAGES % 2 != 0 ? 2 * STAGES : STAGES;
+    auto slab = [&](auto index, auto loads, int number) XP_INLINE {
+      constexpr int S = decltype(index)::value % STAGES;
+      constexpr int NEXT = (S + 1) % STAGES;
+      constexpr bool LOADING = decltype(loads)::value;
+      if constexpr (WHOLE_SLABS) {
+        constexpr int SET = decltype(index)::value % 2;
+        stage_barrier();
+        if constexpr (LOADING) {
+          issue(number + STAGES, S);
+        }
+        read_slab(NEXT, 1 - SET);
+        multiply_slab(SET);
+        __builtin_amdgcn_sched_barrier(0);
+        return;
+      }
+      read_fragments(S, 1, 1);
+      multiply(0);
+      __builtin_amdgcn_sched_barrier(0);
+      read_fragments(S, 2, 0);
+      multiply(1);
+      __builtin_amdgcn_sched_barrier(0);
+      read_fragments(S, 3, 1);
+      multiply(0);
       stage_barrier();
+      read_fragments(NEXT, 0, 0);
       if constexpr (LOADING) {
         issue(number + STAGES, S);
       }
-      read_slab(NEXT, 1 - SET);
-      multiply_slab(SET);
+      multiply(1);
       __builtin_amdgcn_sched_barrier(0);
-      return;
+    };
+    int number = 0;
+    auto main_loop = [&](auto loads) XP_INLINE {
+      for (; number + UNROLL < slabs; number += UNROLL) {
+        static_for<UNROLL>([&](auto j) XP_INLINE { slab(j, loads, number + decltype(j)::value); });
+      }
+      static_for<UNROLL - 1>([&](auto j) XP_INLINE {
+        if (number + decltype(j)::value + 1 < slabs) {
+          slab(j, loads, number + decltype(j)::value);
+        }
+      });
+    };
+    if constexpr (LOAD_WAVES == WAVES) {
+      main_loop(std::true_type{});
+    } else if (loading_wave) {
+      main_loop(std::true_type{});
+    } else {
+      main_loop(std::false_type{});
     }
-    read_fragments(S, 1, 1);
-    multiply(0);
-    __builtin_amdgcn_sched_barrier(0);
-    read_fragments(S, 2, 0);
-    multiply(1);
-    __builtin_amdgcn_sched_barrier(0);
-    read_fragments(S, 3, 1);
-    multiply(0);
-    stage_barrier();
-    read_fragments(NEXT, 0, 0);
-    if constexpr (LOADING) {
-      issue(number + STAGES, S);
-    }
-    multiply(1);
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  int number = 0;
-  auto main_loop = [&](auto loads) XP_INLINE {
-    for (; number + UNROLL < slabs; number += UNROLL) {
-      static_for<UNROLL>([&](auto j) XP_INLINE { slab(j, loads, number + decltype(j)::value); });
-    }
-    static_for<UNROLL - 1>([&](auto j) XP_INLINE {
-      if (number + decltype(j)::value + 1 < slabs) {
-        slab(j, loads, number + decltype(j)::value);
+    static_for<UNROLL>([&](auto j) XP_INLINE {
+      if ((slabs - 1) % UNROLL == decltype(j)::value) {
+        if constexpr (WHOLE_SLABS) {
+          multiply_slab(decltype(j)::value % 2);
+        } else {
+          constexpr int S = decltype(j)::value % STAGES;
+          read_fragments(S, 1, 1);
+          multiply(0);
+          read_fragments(S, 2, 0);
+          multiply(1);
+          read_fragments(S, 3, 1);
+          multiply(0);
+          multiply(1);
+        }
       }
     });
-  };
-  if constexpr (LOAD_WAVES == WAVES) {
-    main_loop(std::true_type{});
-  } else if (loading_wave) {
-    main_loop(std::true_type{});
-  } else {
-    main_loop(std::false_type{});
-  }
-  static_for<UNROLL>([&](auto j) XP_INLINE {
-    if ((slabs - 1) % UNROLL == decltype(j)::value) {
-      if constexpr (WHOLE_SLABS) {
-        multiply_slab(decltype(j)::value % 2);
-      } else {
-        constexpr int S = decltype(j)::value % STAGES;
-        read_fragments(S, 1, 1);
-        multiply(0);
-        read_fragments(S, 2, 0);
-        multiply(1);
-        read_fragments(S, 3, 1);
-        multiply(0);
-        multiply(1);
-      }
-    }
-  });
-  // Refills past the end may still be landing in the stages that the epilogue reuses, and other waves reading.
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  __asm__ volatile("" : "+v"(lane));
-
-  // 32 rows at a time go through a part of LDS of the wave's own, so that a lane then holds CHUNK neighbouring
-  // columns of a row: whole 16-byte loads and stores, 128 contiguous bytes and more of each row.
-  constexpr int CHUNK = EPI == ProductEpilogue::kGradient ? 4 : 8;
-  constexpr int LANES = WTN / CHUNK;    // per row
-  constexpr int ROWS_PER_PASS = 64 / LANES;
-  float *rows = reinterpret_cast<float *>(lds) + wave * 32 * PITCH;
-  const int64_t row0 = m0 + wm * WTM;
-  const int64_t col0 = n0 + wn * WTN;
-  // A worker's sums go to its piece of the tile, [TILE, TILE]: piece q + local, counted along the split tiles' slabs.
-  float *partial = worker ? a.partials + static_cast<int64_t>(q + local) * (TILE * TILE) + (wm * WTM) * TILE + wn * WTN : nullptr;
-  const bool mirrored = a.symmetric != 0 && at.m != at.n;
-  const int chunk = lane % LANES;
-  const int64_t col = col0 + chunk * CHUNK;
-  if constexpr (SPREAD) {
-    // The waves' sums side by side in LDS; each wave then finishes eight of the rows.
-    const float *all = reinterpret_cast<const float *>(lds);
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      const f32x4 four = {acc[0][0][4 * q4], acc[0][0][4 * q4 + 1], acc[0][0][4 * q4 + 2], acc[0][0][4 * q4 + 3]};
-      *reinterpret_cast<f32x4 *>(rows + (lane & 31) * PITCH + 8 * q4 + 4 * (lane >> 5)) = four;
-    }
+    // Refills past the end may still be landing in the stages that the epilogue reuses, and other waves reading.
+    __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    const auto total = [&](int row, int column) __attribute__((always_inline)) {
-      const float *from = all + row * PITCH + column;
-      return (from[0] + from[32 * PITCH]) + (from[64 * PITCH] + from[96 * PITCH]);
-    };
-    [[maybe_unused]] float sums[8] = {};
-    const int row = wave * 8 + lane / LANES;
-    if (lane / LANES < 8 && row0 + row < a.m && col < a.n) {
-      const ChunkPlace there = chunk_place<EPI>(a, at.matrix, row0 + row, col);
-      Beside<P, EPI> beside;
-      request<P, EPI>(a, there, col, beside);
-      float value[CHUNK];
+    __asm__ volatile("" : "+v"(lane));
+
+    // 32 rows at a time go through a part of LDS of the wave's own, so that a lane then holds CHUNK neighbouring
+    // columns of a row: whole 16-byte loads and stores, 128 contiguous bytes and more of each row.
+    constexpr int CHUNK = EPI == ProductEpilogue::kGradient ? 4 : 8;
+    constexpr int LANES = WTN / CHUNK;    // per row
+    constexpr int ROWS_PER_PASS = 64 / LANES;
+    float *rows = reinterpret_cast<float *>(lds) + wave * 32 * PITCH;
+    const int64_t row0 = m0 + wm * WTM;
+    const int64_t col0 = n0 + wn * WTN;
+    // A worker's sums go to its piece of the tile, [TILE, TILE]: piece q + local, counted along the split tiles' slabs.
+    float *partial = worker ? a.partials + static_cast<int64_t>(q + local) * (TILE * TILE) + (wm * WTM) * TILE + wn * WTN : nullptr;
+    const bool mirrored = a.symmetric != 0 && at.m != at.n;
+    const int chunk = lane % LANES;
+    const int64_t col = col0 + chunk * CHUNK;
+    if constexpr (SPREAD) {
+      // The waves' sums side by side in LDS; each wave then finishes eight of the rows.
+      const float *all = reinterpret_cast<const float *>(lds);
 #pragma unroll
-      for (int j = 0; j < CHUNK; ++j) {
-        value[j] = total(row, chunk * CHUNK + j);
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const f32x4 four = {acc[0][0][4 * q4], acc[0][0][4 * q4 + 1], acc[0][0][4 * q4 + 2], acc[0][0][4 * q4 + 3]};
+        *reinterpret_cast<f32x4 *>(rows + (lane & 31) * PITCH + 8 * q4 + 4 * (lane >> 5)) = four;
       }
-      if constexpr (EPI == ProductEpilogue::kGradient) {
-        finish_gradient<P>(a, there, col, beside, value, sums);
-      } else {
-        finish<P, EPI>(a, there, col, beside, value);
-      }
-    }
-    if constexpr (EPI == ProductEpilogue::kStore) {
-      const int64_t to_row = col0 + (threadIdx.x & 31);
-      const int64_t to_col = row0 + (threadIdx.x >> 5) * 8;
-      if (mirrored && threadIdx.x < 128 && to_row < a.n && to_col < a.m) {
-        float value[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          value[j] = total(static_cast<int>(threadIdx.x >> 5) * 8 + j, static_cast<int>(threadIdx.x & 31));
-        }
-        const ChunkPlace across = chunk_place<EPI>(a, at.matrix, to_row, to_col);
+      __syncthreads();
+      const auto total = [&](int row, int column) __attribute__((always_inline)) {
+        const float *from = all + row * PITCH + column;
+        return (from[0] + from[32 * PITCH]) + (from[64 * PITCH] + from[96 * PITCH]);
+      };
+      [[maybe_unused]] float sums[8] = {};
+      const int row = wave * 8 + lane / LANES;
+      if (lane / LANES < 8 && row0 + row < a.m && col < a.n) {
+        const ChunkPlace there = chunk_place<EPI>(a, at.matrix, row0 + row, col);
         Beside<P, EPI> beside;
-        request<P, EPI>(a, across, to_col, beside);
-        finish<P, EPI>(a, across, to_col, beside, value);
-      }
-    }
-    if constexpr (EPI == ProductEpilogue::kGradient) {
-      if (a.column_sums != nullptr) {
-        __syncthreads();
-        float *bands = reinterpret_cast<float *>(lds);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          bands[wave * 512 + j * 64 + lane] = sums[j];
-        }
-        __syncthreads();
-        if (wave == 0) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int in = j * 64 + lane;
-            sums[j] = (bands[in] + bands[512 + in]) + (bands[1024 + in] + bands[1536 + in]);
-          }
-          store_column_sums<LANES>(a, row0 / 32, col, sums, lane);
-        }
-      }
-    }
-    return;
-  }
-  ChunkPlace place = chunk_place<EPI>(a, at.matrix, row0 + lane / LANES, col);
-  constexpr int PASSES = 32 / ROWS_PER_PASS;
-  constexpr int AHEAD = EPI == ProductEpilogue::kGradient ? PASSES : PASSES < 2 ? PASSES : 2;  // passes whose loads are in flight
-  Beside<P, EPI> beside[AHEAD];
-  // One copy of this code for all blocks: it runs once a tile, and straight-line code of several times the size took
-  // longer to fetch than to run (10 us a tile at 256 x 256).
-#pragma unroll 1
-  for (int mt = 0; mt < MT; ++mt) {
-    if (row0 + mt * 32 >= a.m) {
-      break;
-    }
-    [[maybe_unused]] float sums[8] = {};
-    ChunkPlace there = place;
-    auto request_pass = [&](int pass) XP_INLINE {
-      if (partial == nullptr && row0 + mt * 32 + pass * ROWS_PER_PASS + lane / LANES < a.m && col < a.n) {
-        request<P, EPI>(a, there, col, beside[pass % AHEAD]);
-      }
-      there.base += ROWS_PER_PASS * a.ld_base;
-      there.extra += ROWS_PER_PASS * a.ld_extra;
-    };
-#pragma unroll
-    for (int pass = 0; pass < AHEAD; ++pass) {
-      request_pass(pass);
-    }
-    __builtin_amdgcn_wave_barrier();
-    static_for<MT>([&](auto block) XP_INLINE {
-      constexpr int B = decltype(block)::value;
-      if (__builtin_amdgcn_readfirstlane(mt) == B) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x4 four = {acc[B][nt][4 * q], acc[B][nt][4 * q + 1], acc[B][nt][4 * q + 2], acc[B][nt][4 * q + 3]};
-            *reinterpret_cast<f32x4 *>(rows + (lane & 31) * PITCH + nt * 32 + 8 * q + 4 * (lane >> 5)) = four;
-          }
-        }
-      }
-    });
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int pass = 0; pass < PASSES; ++pass) {
-      const int row = pass * ROWS_PER_PASS + lane / LANES;
-      const int64_t to_row = row0 + mt * 32 + row;
-      if (to_row < a.m && col < a.n) {
+        request<P, EPI>(a, there, col, beside);
         float value[CHUNK];
 #pragma unroll
-        for (int part = 0; part < CHUNK / 4; ++part) {
-          const f32x4 four = *reinterpret_cast<const f32x4 *>(rows + row * PITCH + chunk * CHUNK + part * 4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            value[part * 4 + j] = four[j];
-          }
+        for (int j = 0; j < CHUNK; ++j) {
+          value[j] = total(row, chunk * CHUNK + j);
         }
-        if (partial != nullptr) {
-          __builtin_memcpy(__builtin_assume_aligned(partial + (mt * 32 + row) * TILE + chunk * CHUNK, 16), value, CHUNK * 4);
-        } else if constexpr (EPI == ProductEpilogue::kGradient) {
-          finish_gradient<P>(a, place, col, beside[pass % AHEAD], value, sums);
+        if constexpr (EPI == ProductEpilogue::kGradient) {
+          finish_gradient<P>(a, there, col, beside, value, sums);
         } else {
-          finish<P, EPI>(a, place, col, beside[pass % AHEAD], value);
+          finish<P, EPI>(a, there, col, beside, value);
         }
       }
-      if (pass + AHEAD < PASSES) {
-        request_pass(pass + AHEAD);
+      if constexpr (EPI == ProductEpilogue::kStore) {
+        const int64_t to_row = col0 + (threadIdx.x & 31);
+        const int64_t to_col = row0 + (threadIdx.x >> 5) * 8;
+        if (mirrored && threadIdx.x < 128 && to_row < a.n && to_col < a.m) {
+          float value[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            value[j] = total(static_cast<int>(threadIdx.x >> 5) * 8 + j, static_cast<int>(threadIdx.x & 31));
+          }
+          const ChunkPlace across = chunk_place<EPI>(a, at.matrix, to_row, to_col);
+          Beside<P, EPI> beside;
+          request<P, EPI>(a, across, to_col, beside);
+          finish<P, EPI>(a, across, to_col, beside, value);
+        }
       }
-      place.out += ROWS_PER_PASS * a.ld_out;
-      place.base += ROWS_PER_PASS * a.ld_base;
-      place.extra += ROWS_PER_PASS * a.ld_extra;
-    }
-    if constexpr (EPI == ProductEpilogue::kStore) {
-      if (mirrored && partial == nullptr) {
-        // The tile's transpose: eight rows of a column are eight neighbouring columns there.
-        for (int pass = 0; pass < WTN * 4 / 64; ++pass) {
-          const int column = (pass * 64 + lane) % WTN;
-          const int group = (pass * 64 + lane) / WTN;
-          const int64_t to_row = col0 + column;
-          const int64_t to_col = row0 + mt * 32 + group * 8;
-          if (to_row < a.n && to_col < a.m) {
-            float value[8];
+      if constexpr (EPI == ProductEpilogue::kGradient) {
+        if (a.column_sums != nullptr) {
+          __syncthreads();
+          float *bands = reinterpret_cast<float *>(lds);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            bands[wave * 512 + j * 64 + lane] = sums[j];
+          }
+          __syncthreads();
+          if (wave == 0) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              value[j] = rows[(group * 8 + j) * PITCH + column];
+              const int in = j * 64 + lane;
+              sums[j] = (bands[in] + bands[512 + in]) + (bands[1024 + in] + bands[1536 + in]);
             }
-            const ChunkPlace across = chunk_place<EPI>(a, at.matrix, to_row, to_col);
-            Beside<P, EPI> beside_it;
-            request<P, EPI>(a, across, to_col, beside_it);
-            finish<P, EPI>(a, across, to_col, beside_it, value);
+            store_column_sums<LANES>(a, row0 / 32, col, sums, lane);
           }
         }
       }
+      return;
     }
-    if constexpr (EPI == ProductEpilogue::kGradient) {
-      if (partial == nullptr && a.column_sums != nullptr) {
-        store_column_sums<LANES>(a, (row0 + mt * 32) / 32, col, sums, lane);
+    ChunkPlace place = chunk_place<EPI>(a, at.matrix, row0 + lane / LANES, col);
+    constexpr int PASSES = 32 / ROWS_PER_PASS;
+    constexpr int AHEAD = EPI == ProductEpilogue::kGradient ? PASSES : PASSES < 2 ? PASSES : 2;  // passes whose loads are in flight
+    Beside<P, EPI> beside[AHEAD];
+    // One copy of this code for all blocks: it runs once a tile, and straight-line code of several times the size took
+    // longer to fetch than to run (10 us a tile at 256 x 256).
+#pragma unroll 1
+    for (int mt = 0; mt < MT; ++mt) {
+      if (row0 + mt * 32 >= a.m) {
+        break;
+      }
+      [[maybe_unused]] float sums[8] = {};
+      ChunkPlace there = place;
+      auto request_pass = [&](int pass) XP_INLINE {
+        if (partial == nullptr && row0 + mt * 32 + pass * ROWS_PER_PASS + lane / LANES < a.m && col < a.n) {
+          request<P, EPI>(a, there, col, beside[pass % AHEAD]);
+        }
+        there.base += ROWS_PER_PASS * a.ld_base;
+        there.extra += ROWS_PER_PASS * a.ld_extra;
+      };
+#pragma unroll
+      for (int pass = 0; pass < AHEAD; ++pass) {
+        request_pass(pass);
+      }
+      __builtin_amdgcn_wave_barrier();
+      static_for<MT>([&](auto block) XP_INLINE {
+        constexpr int B = decltype(block)::value;
+        if (__builtin_amdgcn_readfirstlane(mt) == B) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const f32x4 four = {acc[B][nt][4 * q], acc[B][nt][4 * q + 1], acc[B][nt][4 * q + 2], acc[B][nt][4 * q + 3]};
+              *reinterpret_cast<f32x4 *>(rows + (lane & 31) * PITCH + nt * 32 + 8 * q + 4 * (lane >> 5)) = four;
+            }
+          }
+        }
+      });
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int pass = 0; pass < PASSES; ++pass) {
+        const int row = pass * ROWS_PER_PASS + lane / LANES;
+        const int64_t to_row = row0 + mt * 32 + row;
+        if (to_row < a.m && col < a.n) {
+          float value[CHUNK];
+#pragma unroll
+          for (int part = 0; part < CHUNK / 4; ++part) {
+            const f32x4 four = *reinterpret_cast<const f32x4 *>(rows + row * PITCH + chunk * CHUNK + part * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              value[part * 4 + j] = four[j];
+            }
+          }
+          if (partial != nullptr) {
+            __builtin_memcpy(__builtin_assume_aligned(partial + (mt * 32 + row) * TILE + chunk * CHUNK, 16), value, CHUNK * 4);
+          } else if constexpr (EPI == ProductEpilogue::kGradient) {
+            finish_gradient<P>(a, place, col, beside[pass % AHEAD], value, sums);
+          } else {
+            finish<P, EPI>(a, place, col, beside[pass % AHEAD], value);
+          }
+        }
+        if (pass + AHEAD < PASSES) {
+          request_pass(pass + AHEAD);
+        }
+        place.out += ROWS_PER_PASS * a.ld_out;
+        place.base += ROWS_PER_PASS * a.ld_base;
+        place.extra += ROWS_PER_PASS * a.ld_extra;
+      }
+      if constexpr (EPI == ProductEpilogue::kStore) {
+        if (mirrored && partial == nullptr) {
+          // The tile's transpose: eight rows of a column are eight neighbouring columns there.
+          for (int pass = 0; pass < WTN * 4 / 64; ++pass) {
+            const int column = (pass * 64 + lane) % WTN;
+            const int group = (pass * 64 + lane) / WTN;
+            const int64_t to_row = col0 + column;
+            const int64_t to_col = row0 + mt * 32 + group * 8;
+            if (to_row < a.n && to_col < a.m) {
+              float value[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                value[j] = rows[(group * 8 + j) * PITCH + column];
+              }
+              const ChunkPlace across = chunk_place<EPI>(a, at.matrix, to_row, to_col);
+              Beside<P, EPI> beside_it;
+              request<P, EPI>(a, across, to_col, beside_it);
+              finish<P, EPI>(a, across, to_col, beside_it, value);
+            }
+          }
+        }
+      }
+      if constexpr (EPI == ProductEpilogue::kGradient) {
+        if (partial == nullptr && a.column_sums != nullptr) {
+          store_column_sums<LANES>(a, (row0 + mt * 32) / 32, col, sums, lane);
+        }
       }
     }
-  }
-  if constexpr (SPLITS) {
-    __syncthreads();  // the next tile's loads land where the waves staged their rows
-  }
+    if constexpr (SPLITS) {
+      __syncthreads();  // the next tile's loads land where the waves staged their rows
+    }
   } while (SPLITS && next < stop);
 }
 
@@ -1303,13 +1306,17 @@ const void *product_join_for(ProductEpilogue epilogue) {
 
 template <class P>
 const void *ProductKernels<P>::main(ProductTiles tiles, ProductEpilogue epilogue, bool a_cols, bool b_cols) {
-  switch (tiles) {
-    case ProductTiles::k256:
+  if constexpr (kElementBytes<P> == 2) {  // fp32's matrix pipe is full with two 128 x 128 tiles on a CU
+    if (tiles == ProductTiles::k256) {
       return product_tile_kernel<P, 256, 2, 4, 2>(epilogue, a_cols, b_cols);
+    }
+    if (tiles == ProductTiles::k128Deep) {
+      return product_tile_kernel<P, 128, 2, 2, 4>(epilogue, a_cols, b_cols);
+    }
+  }
+  switch (tiles) {
     case ProductTiles::k128Pairs:
       return product_tile_kernel<P, 128, 2, 2, 2>(epilogue, a_cols, b_cols);
-    case ProductTiles::k128Deep:
-      return product_tile_kernel<P, 128, 2, 2, 4>(epilogue, a_cols, b_cols);
     case ProductTiles::k64:
       return product_tile_kernel<P, 64, 2, 2, 3>(epilogue, a_cols, b_cols);
     default:
@@ -1326,7 +1333,7 @@ const void *ProductKernels<P>::group(ProductTiles tiles) {
 
 template <class P>
 const void *ProductKernels<P>::join(int tile, ProductEpilogue epilogue) {
-  return tile == 256 ? product_join_for<P, 256>(epilogue) : tile == 128 ? product_join_for<P, 128>(epilogue) : product_join_for<P, 64>(epilogue);
+  return tile == 128 ? product_join_for<P, 128>(epilogue) : product_join_for<P, 64>(epilogue);
 }
 
 }  // namespace xp

@@ -301,6 +301,14 @@ def _check_projection(projection: ProjectionWeights, layout: ProjectionLayout, n
         raise ValueError(f"{name} bias presence disagrees with the prepared layout")
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two non-empty matrices of a training operator share addresses, the gaps between their rows among them."""
+
+    (a_begin, a_end), (b_begin, b_end) = (
+        (t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()) for t in (a, b))
+    return a_begin < b_end and b_begin < a_end
+
+
 def _require_current(index: int) -> None:
     if _native.current_device() != index:
         raise ValueError(f"operands on cuda:{index} need it as the current device")
@@ -630,6 +638,8 @@ class Dense:
         ld_hidden = _row_stride(hidden_states, "hidden states", (rows, hidden), dtype, index)
         for name, tensor, shape in (("projected", projected, (rows, wide)), ("output", output, (rows, hidden))):
             _check_gradient(tensor, name, shape, (dtype,), index)
+        if output.numel() and (_overlap(output, projected) or _overlap(output, hidden_states)):
+            raise ValueError("a trained Dense layer's output must not overlap its hidden states and kept values")
         order = signature.i_proj.gate_up_order
         activated = self.activated[:rows]
         fused = signature.activation.fused(order=order) is not None

@@ -283,3 +283,48 @@ def test_refusals(device):
         operator.step_into(weights=good, gradients=good, momentum=momentum, learning_rate=0.1)
     with pytest.raises(ValueError, match="GPU|device"):
         Muon(operator.plan, torch.empty(operator.plan.workspace.nbytes, dtype=torch.uint8))
+
+
+# Gram matrices and products of 256 x 256 and 128 x 128 tiles and of split ones, mirrored, in batches, wide and tall.
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("count,rows,columns", [(1, 1536, 6144), (1, 6144, 1536), (1, 2300, 2300), (2, 1031, 4103), (1, 2048, 5120),
+                                                (1, 4096, 12288), (3, 2561, 1025)])
+def test_large_orthogonalize(device, count, rows, columns, dtype):
+    if dtype is FP32 and columns > 12000:
+        pytest.skip("the 16-bit tiles' size")
+    source = updates(device, count, rows, columns, dtype)
+    operator = muon(device, count, rows, columns, dtype)
+    out = torch.full_like(source, float("nan"))
+    operator.orthogonalize_into(source, output=out)
+    near(out, orthogonal(source), tolerance(dtype, max(rows, columns)), "matrix")
+    operator.scratch.fill_(0xFF)
+    again = torch.empty_like(out)
+    operator.orthogonalize_into(source, output=again)
+    assert torch.equal(out, again)
+
+
+def test_large_step_in_place(device):
+    """Weights and momentum of a batch, in place and apart: the same bits, and the formula's."""
+
+    g = torch.Generator(device=device).manual_seed(11)
+    gradients = updates(device, 2, 2304, 2048, BF16, seed=4)
+    weights = (torch.randn(gradients.shape, generator=g, device=device) * 0.02).to(BF16)
+    momentum = torch.randn(gradients.shape, generator=g, device=device) * 0.01
+    operator = muon(device, 2, 2304, 2048, BF16)
+    new_weights, new_momentum = torch.full_like(weights, float("nan")), torch.full_like(momentum, float("nan"))
+    options = dict(learning_rate=0.02, weight_decay=0.1, momentum_factor=0.9)
+    operator.step_into(weights=weights, gradients=gradients, momentum=momentum, new_weights=new_weights, new_momentum=new_momentum,
+                       **options)
+    kept = 0.9 * momentum.double() + gradients.double()
+    exact = orthogonal(gradients.double() + 0.9 * kept)
+    step = 0.02 * math.sqrt(2304 / 2048)
+    expected = (1 - 0.002) * weights.double() - step * exact
+    # the factor, the product and the sum are off by half a step each, 2^-24 of terms no larger than the two magnitudes' sum
+    size = float((0.9 * momentum.double().abs() + gradients.double().abs()).max())
+    assert float((new_momentum.double() - kept).abs().max()) <= 3 * 2.0**-24 * size
+    # the update's error (its half step is not taken: it is added in fp32), and half a step of the new weights
+    for found, wanted, update in zip(new_weights.double(), expected, exact):
+        allowed = 2.0**-7.6 * step * float(update.norm()) + 2.0**-9 * float(wanted.norm()) * 2
+        assert float((found - wanted).norm()) <= allowed
+    operator.step_into(weights=weights, gradients=gradients, momentum=momentum, **options)
+    assert torch.equal(weights, new_weights) and torch.equal(momentum, new_momentum)

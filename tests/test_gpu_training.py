@@ -578,3 +578,83 @@ def test_the_forward_pass_of_a_trained_layer_is_the_served_one(device):
         layer.dense.run_into(hidden_states=layer.x, layer_weights=layer.weights, output=served)
         error = float((out.double() - served.double()).norm() / served.double().norm())
         assert error <= 3 * 2.0**-9  # the projection's, the activation's and the output's half steps
+
+
+# Sizes whose products take 256 x 256 tiles, both kinds of 128 x 128 ones, and 64 x 64 ones split along long sums, whole
+# and with a remainder that is shared out; long sums over rows, and ragged edges of each.
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,k,n", [
+    (2048, 2560, 4096), (2100, 2048, 8200), (2100, 4096, 2048), (1100, 2056, 5000), (300, 1032, 4096), (8200, 520, 520),
+    (8200, 1031, 1545), (9000, 2056, 2056)])
+def test_large_projection_gradients(device, rows, k, n, dtype):
+    case = Projection(device, rows, k, n, dtype, bias=True)
+    apart_x, both_x = (torch.full((rows, k), float("nan"), dtype=dtype, device=device) for _ in range(2))
+    apart_w, both_w = (torch.full((n, k), float("nan"), dtype=dtype, device=device) for _ in range(2))
+    grad_b = torch.full((n,), float("nan"), device=device)
+    case.gemm.backward_into(case.x, case.grad, case.weights, grad_inputs=apart_x)
+    case.gemm.backward_into(case.x, case.grad, case.weights, grad_values=apart_w)
+    case.check(apart_x, apart_w, None)
+    case.gemm.backward_into(case.x, case.grad, case.weights, grad_inputs=both_x, grad_values=both_w, grad_bias=grad_b)
+    case.check(both_x, both_w, grad_b)
+    before = both_w.clone(), grad_b.clone()
+    case.gemm.backward_into(case.x, case.grad, case.weights, grad_values=both_w, grad_bias=grad_b, accumulate=True)
+    case.check(None, both_w, grad_b, before)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("function,order", [("silu", INTERLEAVED), ("gelu", CONCATENATED), ("gelu_tanh", None)])
+@pytest.mark.parametrize("rows,hidden,width", [
+    (2100, 2048, 4096), (2500, 2064, 1528), (520, 4096, 520), (4300, 2048, 4096), (777, 1030, 2053)])
+def test_large_dense_training(device, rows, hidden, width, function, order, dtype):
+    if dtype is FP32 and order is CONCATENATED:
+        pytest.skip("gated fp32 layers are INTERLEAVED")
+    layer = Layer(device, rows, hidden, width, dtype, function=function, order=order, bias=True)
+    projected, out = layer.forward()
+    layer.check_forward(projected, out)
+    into = layer.gradients()
+    grad_x = layer.backward(projected, into)
+    layer.check_backward(projected, grad_x, into)
+    before = {name: getattr(into, name).clone() for name in ("i_values", "o_values", "i_bias", "o_bias")}
+    layer.backward(projected, into, accumulate=True)
+    layer.check_backward(projected, None, into, before)
+
+
+def test_large_gradients_are_the_same_every_time(device):
+    """Sums have one order: whatever the scratch held, and in a graph replayed with other work between."""
+
+    layer = Layer(device, 2100, 2048, 4096, BF16, bias=True)
+    projected, _ = layer.forward()
+    into = layer.gradients()
+    expected = [layer.backward(projected, into)] + [t.clone() for t in (into.i_values, into.o_values, into.i_bias, into.o_bias)]
+    again = layer.gradients()
+    grad_x = torch.empty_like(expected[0])
+    layer.dense.training_scratch.fill_(0xFF)
+
+    def run():
+        layer.dense.backward_into(hidden_states=layer.x, layer_weights=layer.weights, projected=projected, grad_output=layer.grad,
+                                  grad_hidden_states=grad_x, gradients=again)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(3):
+        layer.dense.training_scratch.fill_(0xFF)
+        graph.replay()
+        torch.cuda.synchronize()
+        found = (grad_x, again.i_values, again.o_values, again.i_bias, again.o_bias)
+        assert all(torch.equal(a, b) for a, b in zip(expected, found))
+        for target in found:
+            target.fill_(float("nan"))
+        layer.backward(projected, into)
+
+
+def test_kept_values_and_outputs_lie_apart(device):
+    """An output over the hidden states or the kept values would spoil what the backward pass reads: refused."""
+
+    for dtype in (BF16, FP32):
+        layer = Layer(device, 16, 64, 32, dtype)
+        shared = torch.empty((16, 64), dtype=dtype, device=device)
+        for projected, output in ((shared, shared), (shared, layer.x), (layer.x, shared)):
+            with pytest.raises((ValueError, RuntimeError), match="overlap"):
+                layer.dense.run_into(hidden_states=layer.x, layer_weights=layer.weights, output=output, projected=projected)
