@@ -150,6 +150,81 @@ __global__ __launch_bounds__(256) void column_sum_kernel(ColumnSumArgs a) {
   }
 }
 
+// All rows in one launch: sixteen waves take them in turn, four bytes a lane and sixteen rows in flight.  Bound by latency;
+// up to kRowsAtOnce rows shorter than bands and a launch that adds them (777 fp16 rows of 2053 columns 6.2 us against 7.4, of
+// 12288 5.2 against 7.7; 1024 rows of 2053 7.6 against 6.9).
+constexpr int64_t kRowsAtOnce = 896;
+
+template <class P>
+__global__ __launch_bounds__(1024) void column_sum_once_kernel(ColumnSumArgs a) {
+  constexpr int ES = kElementBytes<P>;
+  constexpr int COLS = 4 / ES;
+  constexpr int WAVES = 16;
+  constexpr int AHEAD = 16;
+  __shared__ float waves[WAVES][COLS][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int64_t column = (static_cast<int64_t>(blockIdx.x) * 64 + lane) * COLS;
+  const bool live = column < a.n;
+  const bool whole = a.n - column >= COLS;
+  float sum[COLS] = {};
+  const auto row_at = [&](int64_t row) __attribute__((always_inline)) {
+    const unsigned char *from = static_cast<const unsigned char *>(a.source) + (row * a.ld + column) * ES;
+    uint32_t word = 0;
+    if (whole) {
+      __builtin_memcpy(&word, from, 4);
+    } else {
+      word = *reinterpret_cast<const uint16_t *>(from);
+    }
+    return word;
+  };
+  const auto add = [&](uint32_t word) __attribute__((always_inline)) {
+    if constexpr (ES == 4) {
+      sum[0] += __uint_as_float(word);
+    } else {
+      sum[0] += P::widen(word & 0xffffu);
+      sum[1] += P::widen(word >> 16);
+    }
+  };
+  int64_t row = wave;
+  if (live) {
+    for (; row + WAVES * (AHEAD - 1) < a.rows; row += WAVES * AHEAD) {
+      uint32_t words[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        words[i] = row_at(row + WAVES * i);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        add(words[i]);
+      }
+    }
+#pragma unroll 4
+    for (; row < a.rows; row += WAVES) {
+      add(row_at(row));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < COLS; ++j) {
+    waves[wave][j][lane] = sum[j];
+  }
+  __syncthreads();
+  if (wave != 0 || !live) {
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < COLS; ++j) {
+    if (column + j < a.n) {
+      float total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        total += waves[w][j][lane];
+      }
+      a.out[column + j] = a.accumulate ? a.out[column + j] + total : total;
+    }
+  }
+}
+
 // The bands' sums: a workgroup's four waves take the bands in turn, and theirs are added in wave order.
 __global__ __launch_bounds__(256) void band_sum_kernel(ColumnSumArgs a) {
   __shared__ float waves[4][64];
@@ -185,21 +260,27 @@ struct ThinOuterArgs {
   int32_t out_dtype;
   int32_t accumulate;
   int32_t lanes = 0;     // threads that share a row of the output
+  int32_t across = 0;    // workgroups that share one
   int32_t out_rows = 0;  // of a workgroup
 };
 
 // out (+)= a^T b over at most ROWS rows, in fp32 on the vector pipes, rows in order.  The output's bytes bound it; a
 // matrix core tile has one slab to multiply here and spends its time on its first loads and its epilogue.  A thread keeps eight
 // columns of b in registers and walks the output's rows, whose factors the workgroup holds in LDS: 16-byte stores,
-// neighbouring lanes side by side.  Operands of any alignment.  (2048 x 6144 of five bf16 rows: see the figures of
-// xp_projection_backward.)
+// neighbouring lanes side by side.  Operands of any alignment.  2048 x 6144 of five bf16 rows: 9.4 us by itself (25 MB, 2.7
+// TB/s), 12.9 with the inputs' gradient beside it (50 MB, 3.9 TB/s; one after the other 17.6).  From nine rows on 16-bit
+// operands are faster on tiles (2048 x 6144 of sixteen 12.5 us against 18.8, 1030 x 2053 with the inputs' gradient 14 against
+// 22.7), fp32 ones, whose tiles work longer, from seventeen (2048 x 6144 with the inputs' gradient 29.6 against 42).
 constexpr int kThinRows = 16;
+bool thin_rows(int64_t rows, size_t element) { return rows <= (element == 4 ? kThinRows : kThinRows / 2); }
 constexpr int kThinOutRows = 32;
 
 template <class P, int ROWS>
-__global__ __launch_bounds__(256) void thin_outer_kernel(ThinOuterArgs a) {
-  __shared__ __attribute__((aligned(16))) float factors[kThinOutRows][ROWS];
-  const int64_t first = static_cast<int64_t>(blockIdx.y) * a.out_rows;
+__device__ __forceinline__ void thin_outer(const ThinOuterArgs &a, uint32_t block, unsigned char *lds) {
+  float (*factors)[ROWS] = reinterpret_cast<float (*)[ROWS]>(lds);
+  const uint32_t down = block / static_cast<uint32_t>(a.across);
+  const uint32_t along = block - down * static_cast<uint32_t>(a.across);
+  const int64_t first = static_cast<int64_t>(down) * a.out_rows;
   for (int i = threadIdx.x; i < a.out_rows * ROWS; i += 256) {
     const int row = i % a.out_rows;
     const int t = i / a.out_rows;
@@ -208,7 +289,7 @@ __global__ __launch_bounds__(256) void thin_outer_kernel(ThinOuterArgs a) {
   const int lane = static_cast<int>(threadIdx.x) % a.lanes;
   const int side = static_cast<int>(threadIdx.x) / a.lanes;
   const int sides = 256 / a.lanes;
-  const int64_t column = (static_cast<int64_t>(blockIdx.x) * a.lanes + lane) * 8;
+  const int64_t column = (static_cast<int64_t>(along) * a.lanes + lane) * 8;
   const int count = a.n - column < 8 ? static_cast<int>(a.n - column) : 8;
   float b[ROWS][8] = {};
   if (count > 0) {
@@ -249,11 +330,37 @@ __global__ __launch_bounds__(256) void thin_outer_kernel(ThinOuterArgs a) {
   }
 }
 
+// The gradients of few rows in one launch: an inputs' gradient (32 x 32 tiles of product_kernels.hpp; it reads the weights) and
+// up to two weights' gradients, which write as much.  Each by itself leaves half of the memory's directions idle.
+struct ThinArgs {
+  ProductArgs inputs;
+  ThinOuterArgs outer[2];
+  uint32_t blocks[3];
+};
+
+template <class P, int ROWS>
+__global__ __launch_bounds__(256, (ROWS > 8 ? 2 : 4)) void thin_gradients_kernel(ThinArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[kStageBytes<32, 4>];
+  static_assert(sizeof(float) * kThinOutRows * ROWS <= kStageBytes<32, 4>, "the factors fit the stages");
+  uint32_t block = blockIdx.x;
+  if (block < a.blocks[0]) {
+    product_body<P, 32, 1, 1, 4, false, true, ProductEpilogue::kStore, false>(a.inputs, block, lds);
+    return;
+  }
+  block -= a.blocks[0];
+  const int at = block < a.blocks[1] ? 0 : 1;
+  thin_outer<P, ROWS>(a.outer[at], at == 0 ? block : block - a.blocks[1], lds);
+}
+
 template <class P>
-const void *thin_outer_for(int rows) {
-  return rows <= 4   ? reinterpret_cast<const void *>(&thin_outer_kernel<P, 4>)
-         : rows <= 8 ? reinterpret_cast<const void *>(&thin_outer_kernel<P, 8>)
-                     : reinterpret_cast<const void *>(&thin_outer_kernel<P, kThinRows>);
+const void *thin_gradients_for(int rows) {
+  if constexpr (kElementBytes<P> == 4) {
+    if (rows > 8) {
+      return reinterpret_cast<const void *>(&thin_gradients_kernel<P, kThinRows>);
+    }
+  }
+  return rows <= 4 ? reinterpret_cast<const void *>(&thin_gradients_kernel<P, 4>)
+                   : reinterpret_cast<const void *>(&thin_gradients_kernel<P, 8>);
 }
 
 // Zeros over whole rows of an output (its gradient over no rows).
@@ -350,20 +457,47 @@ struct Caller {
     return pads.count == 0 ? hipSuccess : launch(kernel, stream);
   }
 
-  hipError_t thin_outer(ThinOuterArgs args) const {
-    const int64_t chunks = (args.n + 7) / 8;
-    args.lanes = static_cast<int32_t>(std::min<int64_t>(chunks, 256));
-    const int64_t across = (chunks + args.lanes - 1) / args.lanes;
-    // Enough workgroups for the chip, each with as many rows as that leaves.
-    args.out_rows = static_cast<int32_t>(std::clamp<int64_t>(args.m * across / 1024, 4, kThinOutRows));
-    KernelLaunch kernel;
-    kernel.func = dtype == kDtypeF32   ? thin_outer_for<F32Payload>(args.rows)
-                  : dtype == kDtypeF16 ? thin_outer_for<F16Payload>(args.rows)
-                                       : thin_outer_for<Bf16Payload>(args.rows);
-    kernel.grid = dim3(static_cast<unsigned>(across), blocks_of(args.m, args.out_rows));
-    kernel.block = dim3(256);
-    kernel.set_args(args);
-    return launch(kernel, stream);
+  // Gradients of few rows (thin_rows); `inputs` and those of `outer` may be null.
+  hipError_t thin_gradients(ProductArgs *inputs, std::initializer_list<const ThinOuterArgs *> outer, int rows) const {
+    ThinArgs args{};
+    if (inputs != nullptr) {
+      inputs->batch = 1;
+      inputs->partials = scratch;
+      const ProductPlan plan = plan_product(inputs->m, inputs->n, inputs->k, 1, static_cast<int>(element), false, scratch_bytes);
+      if (plan.tiles == ProductTiles::k32) {
+        args.inputs = *inputs;
+        args.inputs.tile_rows = static_cast<int32_t>((inputs->m + 31) / 32);
+        args.inputs.tile_cols = static_cast<int32_t>((inputs->n + 31) / 32);
+        args.inputs.whole = args.inputs.tile_rows * args.inputs.tile_cols;
+        args.blocks[0] = static_cast<uint32_t>(args.inputs.whole);
+      } else if (const hipError_t status = launch_product(*inputs, ProductEpilogue::kStore, false, true, dtype, scratch_bytes, stream);
+                 status != hipSuccess) {
+        return status;
+      }
+    }
+    int count = 0;
+    for (const ThinOuterArgs *each : outer) {
+      if (each == nullptr) {
+        continue;
+      }
+      ThinOuterArgs &part = args.outer[count];
+      part = *each;
+      const int64_t chunks = (part.n + 7) / 8;
+      part.lanes = static_cast<int32_t>(std::min<int64_t>(chunks, 256));
+      part.across = static_cast<int32_t>((chunks + part.lanes - 1) / part.lanes);
+      // Enough workgroups for the chip, each with as many rows as that leaves.
+      part.out_rows = static_cast<int32_t>(std::clamp<int64_t>(part.m * part.across / (rows > 8 ? 512 : 1024), 4, kThinOutRows));
+      args.blocks[++count] = static_cast<uint32_t>(part.across) * blocks_of(part.m, part.out_rows);
+    }
+    const uint32_t blocks = args.blocks[0] + args.blocks[1] + args.blocks[2];
+    if (blocks == 0) {
+      return hipSuccess;
+    }
+    const void *func = dtype == kDtypeF32   ? thin_gradients_for<F32Payload>(rows)
+                       : dtype == kDtypeF16 ? thin_gradients_for<F16Payload>(rows)
+                                            : thin_gradients_for<Bf16Payload>(rows);
+    void *params[] = {&args};
+    return hipLaunchKernel(func, dim3(blocks), dim3(256), params, 0, stream);
   }
 
   hipError_t clear(void *target, size_t bytes) const {
@@ -394,6 +528,15 @@ hipError_t Caller::column_sums(const void *source, int64_t rows, int64_t n, int6
   args.band_rows = (rows + wanted - 1) / wanted;
   args.band_count = (rows + args.band_rows - 1) / args.band_rows;
   KernelLaunch kernel;
+  if (rows <= kRowsAtOnce) {
+    kernel.func = dtype == kDtypeF32   ? reinterpret_cast<const void *>(&column_sum_once_kernel<F32Payload>)
+                  : dtype == kDtypeF16 ? reinterpret_cast<const void *>(&column_sum_once_kernel<F16Payload>)
+                                       : reinterpret_cast<const void *>(&column_sum_once_kernel<Bf16Payload>);
+    kernel.grid = dim3(blocks_of(n, 64 * static_cast<int64_t>(4 / element)));
+    kernel.block = dim3(1024);
+    kernel.set_args(args);
+    return launch(kernel, stream);
+  }
   kernel.func = dtype == kDtypeF32   ? reinterpret_cast<const void *>(&column_sum_kernel<F32Payload>)
                 : dtype == kDtypeF16 ? reinterpret_cast<const void *>(&column_sum_kernel<F16Payload>)
                                      : reinterpret_cast<const void *>(&column_sum_kernel<Bf16Payload>);
@@ -635,7 +778,7 @@ int xp_projection_backward(const void *x, int64_t ld_x, int64_t rows, int64_t k,
              "gradients and workspace must overlap neither the operands nor each other");
   call.scratch = at.scratch;
   call.scratch_bytes = at.scratch_bytes;
-  const bool thin = rows <= kThinRows;
+  const bool thin = thin_rows(rows, element);
   PadArgs pads{};
   ProductOperand grad{};
   ProductOperand weights{};
@@ -658,9 +801,12 @@ int xp_projection_backward(const void *x, int64_t ld_x, int64_t rows, int64_t k,
   if (present[1]) {
     group.part[1] = outer_args(grad, n, inputs, k, rows, grad_w, grad_w_dtype, accumulate != 0);
   }
-  XP_HIP_CHECK(call.products(group, present));
-  if (grad_w != nullptr && thin) {
-    XP_HIP_CHECK(call.thin_outer(ThinOuterArgs{grad_out, x, grad_w, ld_grad, ld_x, n, k, static_cast<int32_t>(rows), grad_w_dtype, accumulate}));
+  if (thin) {
+    const int few = static_cast<int>(rows);
+    const ThinOuterArgs outer{grad_out, x, grad_w, ld_grad, ld_x, n, k, few, grad_w_dtype, accumulate};
+    XP_HIP_CHECK(call.thin_gradients(present[0] ? &group.part[0] : nullptr, {grad_w == nullptr ? nullptr : &outer}, few));
+  } else {
+    XP_HIP_CHECK(call.products(group, present));
   }
   if (grad_bias != nullptr) {
     XP_HIP_CHECK(call.column_sums(grad_out, rows, n, ld_grad, at.bands, grad_bias, accumulate != 0));
@@ -798,7 +944,7 @@ int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden,
   call.scratch = at.scratch;
   call.scratch_bytes = at.scratch_bytes;
 
-  const bool thin = rows <= kThinRows;
+  const bool thin = thin_rows(rows, element);
   PadArgs pads{};
   const ProductOperand grad = call.padded(grad_out, rows, hidden, ld_grad, at.grad, pads);
   const ProductOperand w_out_rows = call.padded(w_out, hidden, width, width, at.w_out, pads);
@@ -856,14 +1002,14 @@ int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden,
   if (present[2]) {
     group.part[2] = outer_args(grad, hidden, activated, width, rows, grad_w_out, grad_w_dtype, accumulate != 0);
   }
-  XP_HIP_CHECK(call.products(group, present));
-  if (thin && grad_w_in != nullptr) {
-    XP_HIP_CHECK(call.thin_outer(
-        ThinOuterArgs{at.through, x, grad_w_in, through_ld, ld_x, wide, hidden, static_cast<int32_t>(rows), grad_w_dtype, accumulate}));
-  }
-  if (thin && grad_w_out != nullptr) {
-    XP_HIP_CHECK(call.thin_outer(ThinOuterArgs{grad_out, at.activated, grad_w_out, ld_grad, activated.ld, hidden, width,
-                                               static_cast<int32_t>(rows), grad_w_dtype, accumulate}));
+  if (thin) {
+    const int few = static_cast<int>(rows);
+    const ThinOuterArgs in{at.through, x, grad_w_in, through_ld, ld_x, wide, hidden, few, grad_w_dtype, accumulate};
+    const ThinOuterArgs out{grad_out, at.activated, grad_w_out, ld_grad, activated.ld, hidden, width, few, grad_w_dtype, accumulate};
+    XP_HIP_CHECK(call.thin_gradients(present[0] ? &group.part[0] : nullptr,
+                                     {grad_w_in == nullptr ? nullptr : &in, grad_w_out == nullptr ? nullptr : &out}, few));
+  } else {
+    XP_HIP_CHECK(call.products(group, present));
   }
   if (grad_bias_out != nullptr) {
     XP_HIP_CHECK(call.column_sums(grad_out, rows, hidden, ld_grad, at.bands, grad_bias_out, accumulate != 0));

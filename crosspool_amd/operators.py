@@ -654,11 +654,16 @@ class Dense:
         )
         if not fused:
             signature.activation.apply_into(inputs=projected, output=activated, order=order)
-        if dtype is not torch.float32:
+        width, bias = signature.local_intermediate_size, layer_weights.o_proj.bias
+        # What the general projection kernel would compute (fp32; sums of no whole 64s) is faster on the training products'
+        # tiles (fp16 777 x 2056 x 1032: 13.4 us against 25.6, fp32 494 x 11584 x 8288: 711 against 887), but where the rows
+        # are no whole 16 bytes their padded copies cost more than that for few rows (fp16 33 x 8003 x 4001: 40 against 22,
+        # 777: 110 against 113).
+        chunk = 16 // dtype.itemsize
+        general = self.plan.o_proj.kernel == "projection" and (dtype is torch.float32 or width % 64 != 0)
+        if not general or (width % chunk != 0 and rows < 512):
             self.o_proj.run_into(activated, layer_weights.o_proj, output=output)
             return
-        # fp32: the training products' tiles (494 rows of 8288 x 11584: 711 us) rather than the general projection's (887).
-        width, bias = signature.local_intermediate_size, layer_weights.o_proj.bias
         _native.call(
             "xp_projection_keep", activated.data_ptr(), width, rows, width, layer_weights.o_proj.values.data_ptr(), hidden,
             None if bias is None else bias.data_ptr(), output.data_ptr(), hidden, None, _DTYPE_CODES[dtype], None,
