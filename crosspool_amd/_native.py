@@ -136,7 +136,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "xp_projection_keep_workspace_bytes": (_SIZE, [_I64, _I64, _I64, _INT]),
     "xp_projection_keep": (
         _INT,
-        [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _INT, ctypes.POINTER(ActivationDesc), _I64, _P, _SIZE, _P],
+        [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _INT, _INT, ctypes.POINTER(ActivationDesc), _I64, _P, _SIZE, _P],
     ),
     "xp_dense_backward_workspace_bytes": (_SIZE, [_I64, _I64, _I64, _INT, _INT]),
     "xp_dense_backward": (

@@ -40,6 +40,7 @@ struct ProductArgs {
   int64_t batch_extra;
   const float *bias;   // fp32 [n] or null
   float *column_sums;  // kGradient: sums of the unrounded gradients over bands of rows [bands, 2 n or n], or null
+  int64_t halves;      // kActivate: not 0, B's rows and the output's columns are all Gates, then as many Ups; a tile works on pairs
   float alpha;
   float beta;          // 0: base is not read
   float keep;
@@ -58,7 +59,7 @@ struct ProductArgs {
   int8_t extra_dtype;
   int8_t symmetric;    // A and B are one operand: tiles below the diagonal are computed and mirrored
   int8_t padded_out;   // kStore: the output's rows are whole groups of eight columns, zeros behind column n
-  int8_t interleaved;  // kActivate, kGradient: Gate/Up pairs in neighbouring columns, else in halves
+  int8_t interleaved;  // kGradient: Gate/Up pairs in neighbouring columns, else in halves
   ActivationArgs act;
 };
 static_assert(sizeof(ProductArgs) <= 288, "a kernel's argument record");

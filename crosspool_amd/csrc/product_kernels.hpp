@@ -126,7 +126,7 @@ __device__ __forceinline__ ChunkPlace chunk_place(const ProductArgs &a, int64_t 
     return {matrix * a.batch_out + row * a.ld_out + col, matrix * a.batch_base + row * a.ld_base + col,
             matrix * a.batch_extra + row * a.ld_extra + col};
   } else if constexpr (EPI == ProductEpilogue::kActivate) {
-    return {row * a.ld_out + col, 0, row * a.ld_extra + (a.act.gated ? col / 2 : col)};
+    return {row * a.ld_out + (a.halves != 0 ? col / 2 : col), 0, row * a.ld_extra + (a.act.gated ? col / 2 : col)};
   } else {
     const int64_t wide = a.act.gated && a.interleaved ? 2 * col : col;
     return {row * a.ld_out + wide, row * a.ld_base + wide, row * a.ld_extra + col};
@@ -220,6 +220,49 @@ __device__ __forceinline__ void request(const ProductArgs &a, const ChunkPlace &
   }
 }
 
+template <class P>
+__device__ __forceinline__ void store_four(void *target, int64_t index, int count, const float (&value)[4]) {
+  if constexpr (kElementBytes<P> == 4) {
+    float *to = static_cast<float *>(target) + index;
+    if (count >= 4) {
+      __builtin_memcpy(to, value, 16);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j < count) {
+        to[j] = value[j];
+      }
+    }
+  } else {
+    uint16_t *to = static_cast<uint16_t *>(target) + index;
+    const u32x2 packed = {P::pack2(value[0], value[1]), P::pack2(value[2], value[3])};
+    if (count >= 4) {
+      __builtin_memcpy(to, &packed, 8);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j < count) {
+        to[j] = static_cast<uint16_t>(packed[j / 2] >> (16 * (j % 2)));
+      }
+    }
+  }
+}
+
+// The activation of a Gate and an Up.
+template <Slope KIND, bool PRECISE>
+__device__ __forceinline__ float gated_value(const ActivationArgs &act, float gate, float up) {
+  if (act.has_limit) {
+    gate = fminf(gate, act.limit);
+    up = fminf(fmaxf(up, -act.limit), act.limit);
+  }
+  float f;
+  float unused;
+  value_and_slope<KIND, PRECISE>(gate, act.alpha, f, unused);
+  return f * (up + act.up_offset);
+}
+
 // The epilogue (but kGradient's) of columns col .. col + 7, those below n, of one row.
 template <class P, ProductEpilogue EPI>
 __device__ __forceinline__ void finish(const ProductArgs &a, const ChunkPlace &at, int64_t col, const Beside<P, EPI> &beside,
@@ -255,6 +298,27 @@ __device__ __forceinline__ void finish(const ProductArgs &a, const ChunkPlace &a
       }
     }
     store_values(a.out, at.out, a.out_dtype, a.padded_out ? 8 : count, value);
+  } else if (a.halves != 0) {
+    // Gate and Up of four outputs, which lie in two runs.
+    float gate[4];
+    float up[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool with_bias = a.bias != nullptr && 2 * j < count;
+      gate[j] = value[2 * j] + (with_bias ? a.bias[col / 2 + j] : 0.0f);
+      up[j] = value[2 * j + 1] + (with_bias ? a.bias[a.halves + col / 2 + j] : 0.0f);
+    }
+    store_four<P>(a.out, at.out, count / 2, gate);
+    store_four<P>(a.out, at.out + a.halves, count / 2, up);
+    float activated[4];
+    with_function(a.act, [&](auto kind) XP_INLINE {
+      constexpr Slope KIND = decltype(kind)::value;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        activated[j] = gated_value<KIND, PRECISE>(a.act, gate[j], up[j]);
+      }
+    });
+    store_four<P>(a.extra, at.extra, count / 2, activated);
   } else {
     if (a.bias != nullptr) {
 #pragma unroll
@@ -275,15 +339,7 @@ __device__ __forceinline__ void finish(const ProductArgs &a, const ChunkPlace &a
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float gate = value[2 * j];
-        float up = value[2 * j + 1];
-        if (a.act.has_limit) {
-          gate = fminf(gate, a.act.limit);
-          up = fminf(fmaxf(up, -a.act.limit), a.act.limit);
-        }
-        float f;
-        value_and_slope<KIND, PRECISE>(gate, a.act.alpha, f, unused);
-        value[j] = f * (up + a.act.up_offset);
+        value[j] = gated_value<KIND, PRECISE>(a.act, value[2 * j], value[2 * j + 1]);
       }
     });
     if (!a.act.gated) {
@@ -305,36 +361,6 @@ __device__ __forceinline__ void finish(const ProductArgs &a, const ChunkPlace &a
 // kGradient for columns col .. col + 3: four pairs of INTERLEAVED Gate/Up are one 16-byte chunk of 16-bit values, so
 // that neighbouring lanes read and write neighbouring chunks.  `sums` gathers the gradients by column: [0, 4) of
 // Gate (or of ungated values), [4, 8) of Up.
-template <class P>
-__device__ __forceinline__ void store_four(void *target, int64_t index, int count, const float (&value)[4]) {
-  if constexpr (kElementBytes<P> == 4) {
-    float *to = static_cast<float *>(target) + index;
-    if (count >= 4) {
-      __builtin_memcpy(to, value, 16);
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j < count) {
-        to[j] = value[j];
-      }
-    }
-  } else {
-    uint16_t *to = static_cast<uint16_t *>(target) + index;
-    const u32x2 packed = {P::pack2(value[0], value[1]), P::pack2(value[2], value[3])};
-    if (count >= 4) {
-      __builtin_memcpy(to, &packed, 8);
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j < count) {
-        to[j] = static_cast<uint16_t>(packed[j / 2] >> (16 * (j % 2)));
-      }
-    }
-  }
-}
-
 template <class P>
 __device__ __forceinline__ void finish_gradient(const ProductArgs &a, const ChunkPlace &at, int64_t col,
                                                 const Beside<P, ProductEpilogue::kGradient> &beside, const float (&through)[4],
@@ -493,10 +519,14 @@ struct OperandLoads {
   uint32_t ld_bytes;
   uint32_t span;                // bytes of the rows that a resource covers
   uint32_t lane_offset[2];
+  uint32_t eight_bytes;         // between a load's rows and the next one's, and
+  uint32_t lane_row;            // from there to this lane's row (rows along the reduction axis)
   int first;                    // this wave's first load of a slab
 
-  // `rows` counts what is left of the operand from the tile's first row (column).
-  __device__ __forceinline__ void setup(const void *data, int64_t ld, int64_t tile_first, int64_t rows_left, int wave, int lane) {
+  // `rows_left` counts what is left of the operand from the tile's first row (column).  `halves`: not 0, rows 2 j and
+  // 2 j + 1 are the operand's rows j and halves + j (rows along the reduction axis; 2 halves rows in 31 bits of bytes).
+  __device__ __forceinline__ void setup(const void *data, int64_t ld, int64_t tile_first, int64_t rows_left, int wave, int lane,
+                                        int64_t halves = 0) {
     ld_bytes = static_cast<uint32_t>(ld * ES);
     first = (wave % LOAD_WAVES) * LOADS;
     const int row = lane / LANES_PER_ROW;
@@ -512,8 +542,17 @@ struct OperandLoads {
                                    : kOutOfRange;
       }
     } else {
-      origin = static_cast<const unsigned char *>(data) + tile_first * ld * ES;
-      span = static_cast<uint32_t>(rows_left < ROWS ? rows_left : ROWS) * ld_bytes;
+      if (halves != 0) {
+        origin = static_cast<const unsigned char *>(data) + tile_first / 2 * ld * ES;
+        span = static_cast<uint32_t>(2 * halves - tile_first / 2) * ld_bytes;
+        eight_bytes = 4 * ld_bytes;
+        lane_row = static_cast<uint32_t>(row >> 1) * ld_bytes + (row % 2 != 0 ? static_cast<uint32_t>(halves) * ld_bytes : 0u);
+      } else {
+        origin = static_cast<const unsigned char *>(data) + tile_first * ld * ES;
+        span = static_cast<uint32_t>(rows_left < ROWS ? rows_left : ROWS) * ld_bytes;
+        eight_bytes = 8 * ld_bytes;
+        lane_row = static_cast<uint32_t>(row) * ld_bytes;
+      }
       // Eight rows a load: swizzle(8 g + row) = (row / 2) ^ (4 if g is odd), g = first + q.
       lane_offset[0] = static_cast<uint32_t>(place ^ (row >> 1) ^ (LOADS % 2 != 0 ? 4 * (first & 1) : 0));
       lane_offset[1] = lane_offset[0] ^ 4;
@@ -576,9 +615,8 @@ struct OperandLoads {
       const uint32_t rows_before = static_cast<uint32_t>((first + q) * ROWS_PER_LOAD);
       load_lds16(from.rsrc, to, lane_offset[variant(q)] + rows_before * ld_bytes, 0);
     } else {
-      const uint32_t row = static_cast<uint32_t>((threadIdx.x & 63) >> 3);
       const uint32_t chunk = lane_offset[variant(q)];
-      const uint32_t offset = (static_cast<uint32_t>((first + q) * 8) + row) * ld_bytes + chunk * 16;
+      const uint32_t offset = static_cast<uint32_t>(first + q) * eight_bytes + lane_row + chunk * 16;
       load_lds16(from.rsrc, to, static_cast<int>(chunk) < from.chunks_left ? offset : kOutOfRange, from.k_bytes);
     }
   }
@@ -788,7 +826,8 @@ __device__ __forceinline__ void product_body(const ProductArgs &a, uint32_t bloc
     ALoads a_loads;
     BLoads b_loads;
     a_loads.setup(static_cast<const unsigned char *>(a.a.data) + at.matrix * a.a.batch * ES, a.a.ld, m0, a.m - m0, wave, lane);
-    b_loads.setup(static_cast<const unsigned char *>(a.b.data) + at.matrix * a.b.batch * ES, a.b.ld, n0, a.n - n0, wave, lane);
+    b_loads.setup(static_cast<const unsigned char *>(a.b.data) + at.matrix * a.b.batch * ES, a.b.ld, n0, a.n - n0, wave, lane,
+                EPI == ProductEpilogue::kActivate ? a.halves : 0);
     const uint32_t lds_begin = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>((uintptr_t)shared)));
     auto issue = [&](int number, int stage) XP_INLINE {
       const int64_t k_pos = k_begin + static_cast<int64_t>(number) * BK;

@@ -820,8 +820,9 @@ size_t xp_projection_keep_workspace_bytes(int64_t rows, int64_t n, int64_t k, in
 }
 
 int xp_projection_keep(const void *x, int64_t ld_x, int64_t rows, int64_t k, const void *w, int64_t n, const float *bias,
-                       void *projected, int64_t ld_projected, void *activated, int dtype, const xp_activation_desc *activation,
-                       int64_t capacity, void *workspace, size_t workspace_bytes, xp_stream_t stream) {
+                       void *projected, int64_t ld_projected, void *activated, int dtype, int order,
+                       const xp_activation_desc *activation, int64_t capacity, void *workspace, size_t workspace_bytes,
+                       xp_stream_t stream) {
   const size_t element = dtype_bytes(dtype);
   XP_REQUIRE(element != 0, "payload dtype must be bf16, fp16 or fp32");
   XP_REQUIRE(extents_valid(rows, n, k) && rows <= capacity && capacity <= kMaxRows, kExtents);
@@ -829,6 +830,11 @@ int xp_projection_keep(const void *x, int64_t ld_x, int64_t rows, int64_t k, con
   XP_REQUIRE(activated == nullptr || activation != nullptr, "activated outputs need an activation");
   XP_TRY(activation_record(activation, args.act));
   XP_REQUIRE(args.act.gated == 0 || n % 2 == 0, "a gated projection needs an even number of weight rows");
+  const bool halves = activated != nullptr && args.act.gated != 0 && order == XP_GATE_UP_CONCATENATED;
+  XP_REQUIRE(activated == nullptr || args.act.gated == 0 || halves || order == XP_GATE_UP_INTERLEAVED,
+             "gated activation requires a Gate/Up order");
+  XP_REQUIRE(!halves || n * padded_width(k, element) * static_cast<int64_t>(element) < int64_t{1} << 31,
+             "activated outputs of CONCATENATED weights need less than 2 GiB of weights");
   if (rows == 0) {
     return XP_OK;
   }
@@ -862,7 +868,7 @@ int xp_projection_keep(const void *x, int64_t ld_x, int64_t rows, int64_t k, con
   if (activated != nullptr) {
     args.extra = activated;
     args.ld_extra = outputs;
-    args.interleaved = 1;
+    args.halves = halves ? n / 2 : 0;
   }
   XP_HIP_CHECK(call.product(args, activated != nullptr ? ProductEpilogue::kActivate : ProductEpilogue::kStore, false, false));
   return XP_OK;

@@ -642,14 +642,16 @@ class Dense:
             raise ValueError("a trained Dense layer's output must not overlap its hidden states and kept values")
         order = signature.i_proj.gate_up_order
         activated = self.activated[:rows]
-        fused = signature.activation.fused(order=order) is not None
+        # The product works on pairs of Gate and Up rows in either order; halves of 2 GiB and more are past its offsets.
+        fused = signature.activation.fused(order=order) is not None or wide * (hidden + 7) * dtype.itemsize < 1 << 31
         bias = layer_weights.i_proj.bias
         scratch = self.training_scratch
         desc = signature.activation.descriptor()
         _native.call(
             "xp_projection_keep", hidden_states.data_ptr(), ld_hidden, rows, hidden, layer_weights.i_proj.values.data_ptr(),
             wide, None if bias is None else bias.data_ptr(), projected.data_ptr(), wide,
-            activated.data_ptr() if fused else None, _DTYPE_CODES[dtype], ctypes.byref(desc) if fused else None,
+            activated.data_ptr() if fused else None, _DTYPE_CODES[dtype], 0 if order is None else _ORDER_CODES[order],
+            ctypes.byref(desc) if fused else None,
             signature.payload_row_capacity, scratch.data_ptr(), scratch.numel(), _native.current_stream(index),
         )
         if not fused:
@@ -666,7 +668,7 @@ class Dense:
             return
         _native.call(
             "xp_projection_keep", activated.data_ptr(), width, rows, width, layer_weights.o_proj.values.data_ptr(), hidden,
-            None if bias is None else bias.data_ptr(), output.data_ptr(), hidden, None, _DTYPE_CODES[dtype], None,
+            None if bias is None else bias.data_ptr(), output.data_ptr(), hidden, None, _DTYPE_CODES[dtype], 0, None,
             signature.payload_row_capacity, scratch.data_ptr(), scratch.numel(), _native.current_stream(index),
         )
 

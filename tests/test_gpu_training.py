@@ -649,6 +649,34 @@ def test_large_gradients_are_the_same_every_time(device):
         layer.backward(projected, into)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("rows,hidden,width", [(5, 64, 40), (70, 72, 131), (300, 1032, 520), (1100, 2048, 2056), (4100, 1024, 4096)])
+def test_either_order_gives_the_same_layer(device, rows, hidden, width, dtype):
+    """Halves and pairs of the same Gate and Up rows: the same sums, so the same bits."""
+
+    pairs = Layer(device, rows, hidden, width, dtype, function="gelu", limit=1.5, offset=0.5, bias=True)
+    halves = Layer(device, rows, hidden, width, dtype, function="gelu", order=CONCATENATED, limit=1.5, offset=0.5, bias=True)
+    values, bias = pairs.weights.i_proj.values, pairs.weights.i_proj.bias
+    halves.weights.i_proj.values.copy_(torch.cat((values[0::2], values[1::2])))
+    halves.weights.i_proj.bias.copy_(torch.cat((bias[0::2], bias[1::2])))
+    halves.weights.o_proj.values.copy_(pairs.weights.o_proj.values)
+    halves.weights.o_proj.bias.copy_(pairs.weights.o_proj.bias)
+    halves.x.copy_(pairs.x)
+    kept_pairs, out_pairs = pairs.forward()
+    kept_halves, out_halves = halves.forward()
+    assert torch.equal(torch.cat((kept_pairs[:, 0::2], kept_pairs[:, 1::2]), 1), kept_halves)
+    assert torch.equal(out_pairs, out_halves)
+
+
+def test_halves_past_the_product_s_offsets(device):
+    """Weights of 2 GiB in halves take the activation by itself."""
+
+    rows, hidden, width = 3, 16384, 32768
+    layer = Layer(device, rows, hidden, width, BF16, order=CONCATENATED)
+    projected, out = layer.forward()
+    layer.check_forward(projected, out)
+
+
 def test_kept_values_and_outputs_lie_apart(device):
     """An output over the hidden states or the kept values would spoil what the backward pass reads: refused."""
 

@@ -37,7 +37,7 @@ def backward(**changes):
 
 def keep(**changes):
     call = dict(x=0x100000, ld_x=64, rows=8, k=64, w=0x200000, n=48, bias=None, projected=0x300000, ld_p=48, activated=0x400000,
-                dtype=BF16, act=SILU, capacity=8, ws=0x10000000, ws_bytes=BIG)
+                dtype=BF16, order=_native.XP_GATE_UP_INTERLEAVED, act=SILU, capacity=8, ws=0x10000000, ws_bytes=BIG)
     call.update(changes)
     return _native.library().xp_projection_keep(*call.values(), None)
 
@@ -87,6 +87,7 @@ def test_projection_gradient_refusals(changes):
     dict(dtype=9), dict(rows=9), dict(k=0), dict(n=47), dict(w=None), dict(x=None), dict(x=0x100008), dict(projected=None), dict(ld_p=40),
     dict(act=None), dict(bias=0x700002), dict(activated=0x400001), dict(ws=0x1000000C, k=61), dict(ws_bytes=16, k=61), dict(projected=0x400010), dict(activated=0x100000),
     dict(projected=0x200000), dict(act=ctypes.byref(_native.ActivationDesc(function=7))),
+    dict(order=0), dict(order=3), dict(order=_native.XP_GATE_UP_CONCATENATED, n=1 << 20, k=1 << 10, ld_x=1 << 10, ld_p=1 << 20),
 ])
 def test_kept_projection_refusals(changes):
     assert keep(**changes) == BAD, changes
