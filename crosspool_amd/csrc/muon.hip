@@ -98,7 +98,7 @@ __device__ __forceinline__ double group_sum(double value) {
 }
 
 // New momentum, and the sum of the update's squares per workgroup, in 64 bits: an fp32 update's squares may
-// pass fp32's range.  Bound by memory.
+// pass fp32's range.  Bound by memory: 32 bf16 gradients of 2048 x 768 with their momentum, 503 MB, 108 us (4.7 TB/s).
 __global__ __launch_bounds__(256) void muon_norm_kernel(MuonArgs a) {
   const int64_t groups = (a.columns + 7) / 8;
   const int64_t items = a.rows * groups;
@@ -121,7 +121,8 @@ __global__ __launch_bounds__(256) void muon_norm_kernel(MuonArgs a) {
   }
 }
 
-// X0 in rows of whole groups of eight columns, zeros behind the last column.
+// X0 in rows of whole groups of eight columns, zeros behind the last column.  Bound by memory (the same matrices 403 MB,
+// 80 us, 5 TB/s): the norm has to be known before the first value can be stored, so the update is read twice.
 __global__ __launch_bounds__(256) void muon_scale_kernel(MuonArgs a) {
   const int64_t groups = (a.columns + 7) / 8;
   const int64_t items = a.rows * groups;

@@ -10,7 +10,7 @@ namespace xp {
 // What a product does with its fp32 sums.
 enum class ProductEpilogue : int {
   kStore = 0,     // out = alpha sum + beta base + bias; or keep extra - step (alpha sum + beta base)
-  kActivate = 1,  // out = sum + bias rounded to the payload, extra = the activation of that
+  kActivate = 1,  // out = sum + bias rounded to the payload, extra = the activation of the unrounded value
   kGradient = 2,  // a gradient of an activation's outputs: out = the gradient of its inputs (base), extra = its outputs
 };
 

