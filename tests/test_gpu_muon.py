@@ -328,3 +328,20 @@ def test_large_step_in_place(device):
         assert float((found - wanted).norm()) <= allowed
     operator.step_into(weights=weights, gradients=gradients, momentum=momentum, **options)
     assert torch.equal(weights, new_weights) and torch.equal(momentum, new_momentum)
+
+
+@pytest.mark.parametrize("count,rows,columns", [(4096, 5, 9), (1000, 33, 8), (2, 3, 1 << 20), (1, 1 << 20, 2)])
+def test_many_and_long_matrices(device, count, rows, columns):
+    source = updates(device, count, rows, columns, BF16)
+    out = torch.full_like(source, float("nan"))
+    muon(device, count, rows, columns, BF16).orthogonalize_into(source, output=out)
+    exact = source.double()
+    exact = exact / (exact.flatten(1).norm(dim=1)[:, None, None] + 1e-7)
+    for _ in range(5):
+        if rows <= columns:
+            gram = torch.matmul(exact, exact.transpose(1, 2).contiguous())
+            exact = A * exact + torch.matmul(B * gram + C * torch.matmul(gram, gram), exact)
+        else:
+            gram = torch.matmul(exact.transpose(1, 2).contiguous(), exact)
+            exact = A * exact + torch.matmul(exact, B * gram + C * torch.matmul(gram, gram))
+    near(out, exact, tolerance(BF16, max(rows, columns)), "matrix")

@@ -686,3 +686,32 @@ def test_kept_values_and_outputs_lie_apart(device):
         for projected, output in ((shared, shared), (shared, layer.x), (layer.x, shared)):
             with pytest.raises((ValueError, RuntimeError), match="overlap"):
                 layer.dense.run_into(hidden_states=layer.x, layer_weights=layer.weights, output=output, projected=projected)
+
+
+@pytest.mark.parametrize("rows,k,n", [(1 << 20, 8, 8), (1 << 18, 9, 5), (8, 1 << 20, 8), (20, 1 << 20, 3), (8, 8, 1 << 20), (20, 3, 1 << 20)])
+def test_the_longest_rows_and_columns(device, rows, k, n):
+    """One extent at its largest, the others small: sums of a million products and outputs of a million columns."""
+
+    case = Projection(device, rows, k, n, BF16, bias=True)
+    grad_x = torch.full((rows, k), float("nan"), dtype=BF16, device=device)
+    grad_w = torch.full((n, k), float("nan"), device=device)
+    grad_b = torch.full((n,), float("nan"), device=device)
+    case.gemm.backward_into(case.x, case.grad, case.weights, grad_inputs=grad_x, grad_values=grad_w, grad_bias=grad_b)
+    case.check(grad_x, grad_w, grad_b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("rows", [4, 8, 9, 16, 17, 895, 896, 897])
+def test_borders_between_the_variants(device, rows, dtype):
+    """Row counts where weights' gradients and sums over rows change their kernel, with aligned and odd widths."""
+
+    for k, n in ((264, 136), (61, 131)):
+        case = Projection(device, rows, k, n, dtype, bias=True)
+        grad_x = torch.full((rows, k), float("nan"), dtype=dtype, device=device)
+        grad_w = torch.full((n, k), float("nan"), dtype=dtype, device=device)
+        grad_b = torch.full((n,), float("nan"), device=device)
+        case.gemm.backward_into(case.x, case.grad, case.weights, grad_inputs=grad_x, grad_values=grad_w, grad_bias=grad_b)
+        case.check(grad_x, grad_w, grad_b)
+        before = grad_w.clone(), grad_b.clone()
+        case.gemm.backward_into(case.x, case.grad, case.weights, grad_values=grad_w, grad_bias=grad_b, accumulate=True)
+        case.check(None, grad_w, grad_b, before)
