@@ -11,8 +11,8 @@ namespace xp {
 // A product's time in microseconds.  A CU's workgroups share its throughput: with i + 1 of them on it (as many as fit),
 // a slab in each takes `slab[i]`, and the first loads and the epilogue `around[i]`.  Fitted on MI355X to 1, 4, 12 and 48
 // slabs on 64 to 2048 workgroups; the three storage orders differ by less than 10 %.  Model and measured, us: bf16
-// 4096 x 12288 x 4096 299 / 294, 1000 x 2048 x 12288 63 / 61, fp16 symmetric 4096 x 12288 199 / 200; fp32 700 x 1536 x
-// 1536 40 / 41.
+// 4096 x 12288 x 4096 289 / 302, fp16 1000 x 2048 x 12288 65 / 60, 12288 x 2048 x 1000 61 / 60, symmetric 4096 x 12288
+// 197 / 202; fp32 700 x 1536 x 1536 41 / 41.
 namespace {
 struct ProductCost {
   ProductTiles tiles;
@@ -20,8 +20,8 @@ struct ProductCost {
   double slab[4];
   double around[4];
 };
-constexpr ProductCost kCosts16[] = {{ProductTiles::k256, 1, {1.38}, {8.2}},
-                                    {ProductTiles::k128Pairs, 2, {0.73, 0.85}, {4.7, 5.9}},
+constexpr ProductCost kCosts16[] = {{ProductTiles::k256, 1, {1.38}, {7.2}},
+                                    {ProductTiles::k128Pairs, 2, {0.73, 0.85}, {4.7, 7.0}},
                                     {ProductTiles::k128Deep, 1, {0.5}, {6.3}},
                                     {ProductTiles::k64, 3, {0.245, 0.38, 0.52}, {2.3, 3.0, 3.9}},
                                     {ProductTiles::k32, 4, {0.155, 0.22, 0.36, 0.46}, {0.8, 1.1, 1.4, 1.7}}};
