@@ -28,11 +28,11 @@ struct PadJob {
   uint32_t blocks;
 };
 struct PadArgs {
-  PadJob job[3];
+  PadJob job[4];
   int32_t count;
 };
 
-// Rows of any alignment into rows of whole 16-byte chunks, zeros behind them: up to three operands in one launch.  One
+// Rows of any alignment into rows of whole 16-byte chunks, zeros behind them: up to four operands in one launch.  One
 // thread a chunk.  Bound by latency at the sizes where it is a part of the whole (9 MB of fp16 weights, inputs and gradients of
 // 777 rows of 1030 x 2053: 6.6 us).
 template <class P>
@@ -141,32 +141,29 @@ __global__ __launch_bounds__(256) void column_sum_kernel(ColumnSumArgs a) {
   if (wave != 0 || !live) {
     return;
   }
-  const bool alone = a.band_count == 1;
-  float *to = (alone ? a.out : a.bands + static_cast<int64_t>(blockIdx.y) * a.n) + from_column;
+  float *to = a.bands + static_cast<int64_t>(blockIdx.y) * a.n + from_column;
 #pragma unroll
   for (int j = 0; j < CHUNK; ++j) {
     if (from_column + j >= column && from_column + j < a.n) {
-      const float total = (waves[0][j][lane] + waves[1][j][lane]) + (waves[2][j][lane] + waves[3][j][lane]);
-      to[j] = alone && a.accumulate ? to[j] + total : total;
+      to[j] = (waves[0][j][lane] + waves[1][j][lane]) + (waves[2][j][lane] + waves[3][j][lane]);
     }
   }
 }
 
-// All rows in one launch: sixteen waves take them in turn, four bytes a lane and sixteen rows in flight.  Bound by latency;
-// up to kRowsAtOnce rows shorter than bands and a launch that adds them (777 fp16 rows of 2053 columns 6.2 us against 7.4, of
-// 12288 5.2 against 7.7; 1024 rows of 2053 7.6 against 6.9).
-constexpr int64_t kRowsAtOnce = 896;
+// All rows by one workgroup: sixteen waves take them in turn, four bytes a lane and sixteen rows in flight.  Bound by latency;
+// up to kRowsAtOnce rows as short as bands and a launch that adds them, or shorter (777 fp16 rows of 2053 columns 6.2 us against
+// 7.4, of 12288 5.2 against 7.7; 1024 rows 7.6 against 6.9 and 6.0 against 7.1).  It adds the bands' sums too.
+constexpr int64_t kRowsAtOnce = 1024;
+constexpr int kSumWaves = 16;
 
 template <class P>
-__global__ __launch_bounds__(1024) void column_sum_once_kernel(ColumnSumArgs a) {
+__device__ __forceinline__ void sum_rows(const ColumnSumArgs &a, uint32_t block, float (&waves)[kSumWaves][2][64]) {
   constexpr int ES = kElementBytes<P>;
   constexpr int COLS = 4 / ES;
-  constexpr int WAVES = 16;
   constexpr int AHEAD = 16;
-  __shared__ float waves[WAVES][COLS][64];
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
-  const int64_t column = (static_cast<int64_t>(blockIdx.x) * 64 + lane) * COLS;
+  const int64_t column = (static_cast<int64_t>(block) * 64 + lane) * COLS;
   const bool live = column < a.n;
   const bool whole = a.n - column >= COLS;
   float sum[COLS] = {};
@@ -190,11 +187,11 @@ __global__ __launch_bounds__(1024) void column_sum_once_kernel(ColumnSumArgs a) 
   };
   int64_t row = wave;
   if (live) {
-    for (; row + WAVES * (AHEAD - 1) < a.rows; row += WAVES * AHEAD) {
+    for (; row + kSumWaves * (AHEAD - 1) < a.rows; row += kSumWaves * AHEAD) {
       uint32_t words[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        words[i] = row_at(row + WAVES * i);
+        words[i] = row_at(row + kSumWaves * i);
       }
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
@@ -202,7 +199,7 @@ __global__ __launch_bounds__(1024) void column_sum_once_kernel(ColumnSumArgs a) 
       }
     }
 #pragma unroll 4
-    for (; row < a.rows; row += WAVES) {
+    for (; row < a.rows; row += kSumWaves) {
       add(row_at(row));
     }
   }
@@ -219,7 +216,7 @@ __global__ __launch_bounds__(1024) void column_sum_once_kernel(ColumnSumArgs a) 
     if (column + j < a.n) {
       float total = 0.0f;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
+      for (int w = 0; w < kSumWaves; ++w) {
         total += waves[w][j][lane];
       }
       a.out[column + j] = a.accumulate ? a.out[column + j] + total : total;
@@ -227,25 +224,20 @@ __global__ __launch_bounds__(1024) void column_sum_once_kernel(ColumnSumArgs a) 
   }
 }
 
-// The bands' sums: a workgroup's four waves take the bands in turn, and theirs are added in wave order.
-__global__ __launch_bounds__(256) void band_sum_kernel(ColumnSumArgs a) {
-  __shared__ float waves[4][64];
-  const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
-  const int64_t column = static_cast<int64_t>(blockIdx.x) * 64 + lane;
-  float sum = 0.0f;
-  if (column < a.n) {
-    const float *from = a.bands + column;
-#pragma unroll 8
-    for (int64_t band = wave; band < a.band_count; band += 4) {
-      sum += from[band * a.n];
-    }
-  }
-  waves[wave][lane] = sum;
-  __syncthreads();
-  if (wave == 0 && column < a.n) {
-    const float total = (waves[0][lane] + waves[1][lane]) + (waves[2][lane] + waves[3][lane]);
-    a.out[column] = a.accumulate ? a.out[column] + total : total;
+// Sums of payload rows, and of fp32 bands' sums, in one launch.
+struct RowSums {
+  ColumnSumArgs rows;
+  ColumnSumArgs bands;
+  uint32_t row_blocks;
+};
+
+template <class P>
+__global__ __launch_bounds__(64 * kSumWaves) void row_sums_kernel(RowSums a) {
+  __shared__ float waves[kSumWaves][2][64];
+  if (blockIdx.x < a.row_blocks) {
+    sum_rows<P>(a.rows, blockIdx.x, waves);
+  } else {
+    sum_rows<F32Payload>(a.bands, blockIdx.x - a.row_blocks, waves);
   }
 }
 
@@ -508,13 +500,26 @@ struct Caller {
     return hipGetLastError();
   }
 
-  hipError_t band_sums(ColumnSumArgs args) const {
+  // Either may be null.
+  hipError_t row_sums(const ColumnSumArgs *rows, const ColumnSumArgs *bands) const {
+    RowSums args{};
+    uint32_t blocks = 0;
+    if (rows != nullptr) {
+      args.rows = *rows;
+      args.row_blocks = blocks = blocks_of(rows->n, 64 * static_cast<int64_t>(4 / element));
+    }
+    if (bands != nullptr) {
+      args.bands = *bands;
+      blocks += blocks_of(bands->n, 64);
+    }
     KernelLaunch kernel;
-    kernel.func = reinterpret_cast<const void *>(&band_sum_kernel);
-    kernel.grid = dim3(blocks_of(args.n, 64));
-    kernel.block = dim3(256);
+    kernel.func = dtype == kDtypeF32   ? reinterpret_cast<const void *>(&row_sums_kernel<F32Payload>)
+                  : dtype == kDtypeF16 ? reinterpret_cast<const void *>(&row_sums_kernel<F16Payload>)
+                                       : reinterpret_cast<const void *>(&row_sums_kernel<Bf16Payload>);
+    kernel.grid = dim3(blocks);
+    kernel.block = dim3(64 * kSumWaves);
     kernel.set_args(args);
-    return launch(kernel, stream);
+    return blocks == 0 ? hipSuccess : launch(kernel, stream);
   }
 
   hipError_t column_sums(const void *source, int64_t rows, int64_t n, int64_t ld, float *bands, float *out, bool accumulate) const;
@@ -531,13 +536,7 @@ hipError_t Caller::column_sums(const void *source, int64_t rows, int64_t n, int6
   args.band_count = (rows + args.band_rows - 1) / args.band_rows;
   KernelLaunch kernel;
   if (rows <= kRowsAtOnce) {
-    kernel.func = dtype == kDtypeF32   ? reinterpret_cast<const void *>(&column_sum_once_kernel<F32Payload>)
-                  : dtype == kDtypeF16 ? reinterpret_cast<const void *>(&column_sum_once_kernel<F16Payload>)
-                                       : reinterpret_cast<const void *>(&column_sum_once_kernel<Bf16Payload>);
-    kernel.grid = dim3(blocks_of(n, 64 * static_cast<int64_t>(4 / element)));
-    kernel.block = dim3(1024);
-    kernel.set_args(args);
-    return launch(kernel, stream);
+    return row_sums(&args, nullptr);
   }
   kernel.func = dtype == kDtypeF32   ? reinterpret_cast<const void *>(&column_sum_kernel<F32Payload>)
                 : dtype == kDtypeF16 ? reinterpret_cast<const void *>(&column_sum_kernel<F16Payload>)
@@ -548,7 +547,8 @@ hipError_t Caller::column_sums(const void *source, int64_t rows, int64_t n, int6
   if (const hipError_t status = launch(kernel, stream); status != hipSuccess) {
     return status;
   }
-  return args.band_count == 1 ? hipSuccess : band_sums(args);
+  const ColumnSumArgs sums{bands, nullptr, out, args.band_count, n, n, 0, 0, accumulate};
+  return row_sums(nullptr, &sums);
 }
 
 // out (+)= sum over rows t of a[t][i] b[t][j]: a weight's gradient.
@@ -956,8 +956,6 @@ int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden,
   PadArgs pads{};
   const ProductOperand grad = call.padded(grad_out, rows, hidden, ld_grad, at.grad, pads);
   const ProductOperand w_out_rows = call.padded(w_out, hidden, width, width, at.w_out, pads);
-  XP_HIP_CHECK(call.pad(pads));
-  pads = PadArgs{};
   ProductOperand w_in_rows{};
   ProductOperand inputs{};
   if (grad_x != nullptr) {
@@ -986,11 +984,12 @@ int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden,
     args.column_sums = grad_bias_in != nullptr ? at.bands : nullptr;
     args.alpha = 1.0f;
     XP_HIP_CHECK(call.product(args, ProductEpilogue::kGradient, false, true));
-    if (grad_bias_in != nullptr) {
-      XP_HIP_CHECK(call.band_sums(
-          ColumnSumArgs{nullptr, at.bands, grad_bias_in, rows, wide, 0, 0, (rows + kBandRows - 1) / kBandRows, accumulate}));
-    }
   }
+  // The biases' gradients, together where the outputs' needs no bands of its own (they would share the kept ones' place).
+  const ColumnSumArgs in_bands{at.bands, nullptr, grad_bias_in, (rows + kBandRows - 1) / kBandRows, wide, wide, 0, 0, accumulate};
+  const ColumnSumArgs out_rows{grad_out, nullptr, grad_bias_out, rows, hidden, ld_grad, 0, 0, accumulate};
+  const bool out_at_once = grad_bias_out != nullptr && rows <= kRowsAtOnce;
+  XP_HIP_CHECK(call.row_sums(out_at_once ? &out_rows : nullptr, grad_bias_in != nullptr ? &in_bands : nullptr));
   if (grad_x != nullptr) {
     if (through_ld != wide) {
       const int64_t words = rows * (through_ld - wide) * static_cast<int64_t>(element) / 2;
@@ -1019,7 +1018,7 @@ int xp_dense_backward(const void *x, int64_t ld_x, int64_t rows, int64_t hidden,
   } else {
     XP_HIP_CHECK(call.products(group, present));
   }
-  if (grad_bias_out != nullptr) {
+  if (grad_bias_out != nullptr && !out_at_once) {
     XP_HIP_CHECK(call.column_sums(grad_out, rows, hidden, ld_grad, at.bands, grad_bias_out, accumulate != 0));
   }
   return XP_OK;
