@@ -715,3 +715,33 @@ def test_borders_between_the_variants(device, rows, dtype):
         before = grad_w.clone(), grad_b.clone()
         case.gemm.backward_into(case.x, case.grad, case.weights, grad_values=grad_w, grad_bias=grad_b, accumulate=True)
         case.check(None, grad_w, grad_b, before)
+
+
+@pytest.mark.parametrize("rows,dtype", [(5, BF16), (13, FP32), (950, FP16), (1500, BF16)])
+def test_gradients_of_every_variant_in_a_graph(device, rows, dtype):
+    """Few rows in one launch, biases at once and in bands: replayed with other work between, as they are eager."""
+
+    layer = Layer(device, rows, 257, 131, dtype, bias=True)
+    projected, _ = layer.forward()
+    into, grad_x = layer.gradients(), torch.empty((rows, 257), dtype=dtype, device=device)
+    targets = (grad_x, into.i_values, into.o_values, into.i_bias, into.o_bias)
+
+    def run():
+        layer.dense.backward_into(hidden_states=layer.x, layer_weights=layer.weights, projected=projected, grad_output=layer.grad,
+                                  grad_hidden_states=grad_x, gradients=into)
+
+    run()
+    torch.cuda.synchronize()
+    expected = [target.clone() for target in targets]
+    layer.check_backward(projected, grad_x, into)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(3):
+        for target in targets:
+            target.fill_(float("nan"))
+        layer.dense.training_scratch.fill_(0xFF)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(expected, targets))
+        run()
