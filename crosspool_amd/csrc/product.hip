@@ -64,7 +64,8 @@ size_t product_scratch_bytes(const ProductPlan &plan) {
   return plan.split > 0 ? static_cast<size_t>(plan.workers + plan.split) * size * size * sizeof(float) : 0;
 }
 
-ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int64_t batch, int element_bytes, bool symmetric, size_t scratch) {
+namespace {
+ProductPlan find_plan(int64_t m, int64_t n, int64_t k, int64_t batch, int element_bytes, bool symmetric, size_t scratch) {
   const int64_t slab = 128 / element_bytes;
   const int64_t slabs = (k + slab - 1) / slab;
   ProductPlan best{};
@@ -113,6 +114,41 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int64_t batch, int ele
     }
   }
   return best;
+}
+
+struct PlanKey {
+  int64_t m;
+  int64_t n;
+  int64_t k;
+  int64_t batch;
+  size_t scratch;
+  int64_t kind;
+  bool operator==(const PlanKey &) const = default;
+};
+struct KnownPlan {
+  PlanKey key;
+  ProductPlan plan;
+};
+constexpr size_t kKnownPlans = 512;
+}  // namespace
+
+// A plan follows from its arguments alone.  A small call asks for some ten of them, workspace sizes among them, whose search
+// took longer than its launches (a backward pass of three rows of 256 x 256 17 us of host time): each thread keeps the last ones.
+ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int64_t batch, int element_bytes, bool symmetric, size_t scratch) {
+  static thread_local KnownPlan known[kKnownPlans];  // (no product has m = 0)
+  const PlanKey key{m, n, k, batch, scratch, element_bytes * 2 + (symmetric ? 1 : 0)};
+  uint64_t hash = 0;
+  for (const uint64_t part : {static_cast<uint64_t>(m), static_cast<uint64_t>(n), static_cast<uint64_t>(k), static_cast<uint64_t>(batch),
+                              static_cast<uint64_t>(scratch), static_cast<uint64_t>(key.kind)}) {
+    hash = (hash ^ part) * 0x9e3779b97f4a7c15ull;
+    hash ^= hash >> 29;
+  }
+  KnownPlan &place = known[hash % kKnownPlans];
+  if (!(place.key == key)) {
+    place.plan = find_plan(m, n, k, batch, element_bytes, symmetric, scratch);
+    place.key = key;
+  }
+  return place.plan;
 }
 
 ProductLaunch make_product(const ProductArgs &args, const ProductPlan &plan, ProductEpilogue epilogue, bool a_cols, bool b_cols,
