@@ -138,6 +138,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _INT,
         [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _INT, _INT, ctypes.POINTER(ActivationDesc), _I64, _P, _SIZE, _P],
     ),
+    "xp_kept_activation": (_INT, [_P, _P, _I64, _I64, _INT, _INT, ctypes.POINTER(ActivationDesc), _P]),
     "xp_dense_backward_workspace_bytes": (_SIZE, [_I64, _I64, _I64, _INT, _INT]),
     "xp_dense_backward": (
         _INT,

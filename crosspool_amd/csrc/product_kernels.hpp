@@ -256,12 +256,11 @@ __device__ __forceinline__ void store_four(void *target, int64_t index, int coun
   }
 }
 
-// The activation of a Gate and an Up.
+// The activation of a Gate and an Up.  NaN is past no limit, as in the backward pass of the same values.
 template <Slope KIND, bool PRECISE>
 __device__ __forceinline__ float gated_value(const ActivationArgs &act, float gate, float up) {
   if (act.has_limit) {
-    gate = fminf(gate, act.limit);
-    up = fminf(fmaxf(up, -act.limit), act.limit);
+    clip_keep_nan(gate, up, act.limit);
   }
   float f;
   float unused;

@@ -327,6 +327,8 @@ __global__ __launch_bounds__(256) void projection_reduce_kernel(ProjectionArgs a
 // ------------------------------------------------------------------ standalone activation
 // One thread per output element (grid-stride): gated reads Gate and Up from the layout the
 // order names; ungated ReLU works on the raw 16-bit patterns (bit-exact, in place allowed).
+// KEEP_NAN: a NaN Gate or Up is past no limit (kept values of a trained layer).
+template <bool KEEP_NAN>
 __global__ __launch_bounds__(256) void activation_kernel(ActivationLaunchArgs a) {
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
   for (int64_t index = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; index < a.elements;
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(256) void activation_kernel(ActivationLaunchArgs a)
     const int64_t up_at = a.interleaved ? gate_at + 1 : gate_at + a.width;
     const float gate = load_value(a.inputs, gate_at, a.dtype);
     const float up = load_value(a.inputs, up_at, a.dtype);
-    store_value(a.output, index, apply_gated(gate, up, a.act), a.dtype);
+    store_value(a.output, index, apply_gated<KEEP_NAN>(gate, up, a.act), a.dtype);
   }
 }
 
@@ -586,9 +588,10 @@ KernelLaunch make_projection_reduce(const ProjectionArgs &args, int64_t capacity
   return reduce;
 }
 
-KernelLaunch make_activation(const ActivationLaunchArgs &args) {
+KernelLaunch make_activation(const ActivationLaunchArgs &args, bool keep_nan) {
   KernelLaunch kernel;
-  kernel.func = reinterpret_cast<const void *>(&activation_kernel);
+  kernel.func = keep_nan ? reinterpret_cast<const void *>(&activation_kernel<true>)
+                         : reinterpret_cast<const void *>(&activation_kernel<false>);
   const int64_t blocks = (args.elements + 255) / 256;
   kernel.grid = dim3(static_cast<unsigned>(blocks < 4096 ? (blocks > 0 ? blocks : 1) : 4096), 1, 1);
   kernel.block = dim3(256, 1, 1);

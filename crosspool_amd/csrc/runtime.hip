@@ -1474,6 +1474,40 @@ GemmChoice choose_tuned_projection(int64_t capacity, int64_t n, int64_t k) {
   return refine_dense_choice(choose_gemm(capacity, n, k, false), capacity, n, k);
 }
 
+int run_activation(const void *inputs, void *output, int64_t rows, int64_t width, int dtype, int order,
+                   const xp_activation_desc *activation, bool keep_nan, xp_stream_t stream) {
+  XP_REQUIRE(activation != nullptr, "activation descriptor must be non-null");
+  XP_REQUIRE(rows >= 0 && width >= 0, "activation extents must be non-negative");
+  XP_REQUIRE(dtype == XP_DTYPE_BF16 || dtype == XP_DTYPE_F16, "standalone activations take bf16 or fp16 payloads");
+  ActivationLaunchArgs args{};
+  if (const int status = activation_record(activation, args.act); status != XP_OK) {
+    return status;
+  }
+  XP_REQUIRE(!args.act.gated || order == XP_GATE_UP_INTERLEAVED || order == XP_GATE_UP_CONCATENATED,
+             "gated activation requires a Gate/Up order");
+  const int64_t elements = rows * width;
+  if (elements == 0) {
+    return XP_OK;
+  }
+  XP_REQUIRE(inputs != nullptr && output != nullptr, "activation pointers must be non-null");
+  XP_REQUIRE(aligned_to(inputs, 2) && aligned_to(output, 2), "activation payloads must be 2-byte aligned");
+  const uintptr_t in_begin = reinterpret_cast<uintptr_t>(inputs);
+  const uintptr_t in_end = in_begin + static_cast<uintptr_t>(elements * (args.act.gated ? 2 : 1) * 2);
+  const uintptr_t out_begin = reinterpret_cast<uintptr_t>(output);
+  const uintptr_t out_end = out_begin + static_cast<uintptr_t>(elements * 2);
+  const bool overlap = in_begin < out_end && out_begin < in_end;
+  XP_REQUIRE(!overlap || (!args.act.gated && in_begin == out_begin),
+             "only an ungated activation may run in place, and only on the same range");
+  args.inputs = inputs;
+  args.output = output;
+  args.elements = elements;
+  args.width = width;
+  args.dtype = dtype;
+  args.interleaved = order == XP_GATE_UP_INTERLEAVED;
+  XP_HIP_CHECK(launch(make_activation(args, keep_nan), static_cast<hipStream_t>(stream)));
+  return XP_OK;
+}
+
 }  // namespace
 
 size_t xp_projection_workspace_bytes(int64_t rows, int64_t n, int64_t k, int dtype) {
@@ -1585,36 +1619,12 @@ int xp_projection_split(const void *x, int64_t rows, int64_t k, const void *w, i
 
 int xp_activation(const void *inputs, void *output, int64_t rows, int64_t width, int dtype, int order,
                   const xp_activation_desc *activation, xp_stream_t stream) {
-  XP_REQUIRE(activation != nullptr, "activation descriptor must be non-null");
-  XP_REQUIRE(rows >= 0 && width >= 0, "activation extents must be non-negative");
-  XP_REQUIRE(dtype == XP_DTYPE_BF16 || dtype == XP_DTYPE_F16, "standalone activations take bf16 or fp16 payloads");
-  ActivationLaunchArgs args{};
-  if (const int status = activation_record(activation, args.act); status != XP_OK) {
-    return status;
-  }
-  XP_REQUIRE(!args.act.gated || order == XP_GATE_UP_INTERLEAVED || order == XP_GATE_UP_CONCATENATED,
-             "gated activation requires a Gate/Up order");
-  const int64_t elements = rows * width;
-  if (elements == 0) {
-    return XP_OK;
-  }
-  XP_REQUIRE(inputs != nullptr && output != nullptr, "activation pointers must be non-null");
-  XP_REQUIRE(aligned_to(inputs, 2) && aligned_to(output, 2), "activation payloads must be 2-byte aligned");
-  const uintptr_t in_begin = reinterpret_cast<uintptr_t>(inputs);
-  const uintptr_t in_end = in_begin + static_cast<uintptr_t>(elements * (args.act.gated ? 2 : 1) * 2);
-  const uintptr_t out_begin = reinterpret_cast<uintptr_t>(output);
-  const uintptr_t out_end = out_begin + static_cast<uintptr_t>(elements * 2);
-  const bool overlap = in_begin < out_end && out_begin < in_end;
-  XP_REQUIRE(!overlap || (!args.act.gated && in_begin == out_begin),
-             "only an ungated activation may run in place, and only on the same range");
-  args.inputs = inputs;
-  args.output = output;
-  args.elements = elements;
-  args.width = width;
-  args.dtype = dtype;
-  args.interleaved = order == XP_GATE_UP_INTERLEAVED;
-  XP_HIP_CHECK(launch(make_activation(args), static_cast<hipStream_t>(stream)));
-  return XP_OK;
+  return run_activation(inputs, output, rows, width, dtype, order, activation, false, stream);
+}
+
+int xp_kept_activation(const void *projected, void *activated, int64_t rows, int64_t width, int dtype, int order,
+                       const xp_activation_desc *activation, xp_stream_t stream) {
+  return run_activation(projected, activated, rows, width, dtype, order, activation, true, stream);
 }
 
 int xp_activation_backward(const void *inputs, const void *grad_output, void *grad_inputs, int64_t rows, int64_t width,

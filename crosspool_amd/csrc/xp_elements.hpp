@@ -65,19 +65,24 @@ __device__ __forceinline__ float apply_function(float value, const ActivationArg
   }
 }
 
-__device__ __forceinline__ float apply_gated(float gate, float up, const ActivationArgs &act) {
-  if (act.has_limit) {
-    gate = fminf(gate, act.limit);
-    up = fminf(fmaxf(up, -act.limit), act.limit);
-  }
-  return apply_function(gate, act) * (up + act.up_offset);
-}
-
 // A gated pair within the limit.  NaN is past no limit and stays (fminf and fmaxf, which the projections'
-// and the standalone activation's epilogues above take, would make the limit of it).
+// and the standalone activation's epilogues below take, would make the limit of it).
 __device__ __forceinline__ void clip_keep_nan(float &gate, float &up, float limit) {
   gate = gate > limit ? limit : gate;
   up = up > limit ? limit : up < -limit ? -limit : up;
+}
+
+template <bool KEEP_NAN = false>
+__device__ __forceinline__ float apply_gated(float gate, float up, const ActivationArgs &act) {
+  if (act.has_limit) {
+    if constexpr (KEEP_NAN) {
+      clip_keep_nan(gate, up, act.limit);
+    } else {
+      gate = fminf(gate, act.limit);
+      up = fminf(fmaxf(up, -act.limit), act.limit);
+    }
+  }
+  return apply_function(gate, act) * (up + act.up_offset);
 }
 
 // ------------------------------------------------------------------ gradient of the activation

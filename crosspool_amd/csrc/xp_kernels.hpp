@@ -337,7 +337,8 @@ struct ActivationLaunchArgs {
   ActivationArgs act;
 };
 
-KernelLaunch make_activation(const ActivationLaunchArgs &args);
+// keep_nan: a limit leaves NaN as it is.
+KernelLaunch make_activation(const ActivationLaunchArgs &args, bool keep_nan);
 
 // grad_inputs (shaped as inputs) = the activation's gradient for grad_output [elements].
 struct ActivationBackwardArgs {

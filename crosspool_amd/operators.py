@@ -571,8 +571,9 @@ class Dense:
         """Write the complete rank-local partial of ``hidden_states`` into ``output``.
 
         ``projected`` (of a plan prepared with ``backward``; contiguous ``[rows, i_proj width]`` of the payload dtype)
-        gets the projected values that :meth:`backward_into` reads.  Its activation is that of the unrounded sums, so outputs may
-        differ in a last bit from those of a call without it.
+        gets the projected values that :meth:`backward_into` reads.  Its activation is that of the unrounded sums (of the kept
+        values for CONCATENATED weights of 2 GiB and more), so outputs may differ in a last bit from those of a call without
+        it; and a NaN Gate or Up is past no limit, as in the backward pass, where a call without it makes the limit of it.
 
         ``adapters`` (of a plan prepared for them) adds the low-rank adapters that ``adapter_ids`` (int32,
         one per row, -1: none) names to each projection; an id outside the pool gives a row of NaN and a
@@ -656,7 +657,10 @@ class Dense:
             signature.payload_row_capacity, scratch.data_ptr(), scratch.numel(), _native.current_stream(index),
         )
         if not fused:
-            signature.activation.apply_into(inputs=projected, output=activated, order=order)
+            _native.call(
+                "xp_kept_activation", projected.data_ptr(), activated.data_ptr(), rows, signature.local_intermediate_size,
+                _DTYPE_CODES[dtype], _ORDER_CODES[order], ctypes.byref(desc), _native.current_stream(index),
+            )
         width, bias = signature.local_intermediate_size, layer_weights.o_proj.bias
         # What the general projection kernel would compute (fp32; sums of no whole 64s) is faster on the training products'
         # tiles (fp16 777 x 2056 x 1032: 13.4 us against 25.6, fp32 494 x 11584 x 8288: 711 against 887), but where the rows

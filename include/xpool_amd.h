@@ -579,13 +579,19 @@ int xp_projection_backward(const void *x, int64_t ld_x, int64_t rows, int64_t k,
 
 /* A projection whose values before the activation are kept for a backward pass: projected [rows, n] = x . w^T + bias
  * rounded to dtype, and activated (contiguous [rows, n], gated [rows, n / 2]) = the activation of the unrounded fp32 values,
- * Gate/Up in `order` (CONCATENATED: weights below 2 GiB); activated NULL: the projection alone.  Strides, alignment,
+ * Gate/Up in `order` (CONCATENATED: weights below 2 GiB); activated NULL: the projection alone.  A NaN Gate or Up is not
+ * clipped (xp_activation makes the limit of it): its output is NaN, as its gradients are.  Strides, alignment,
  * workspace and capacity as above. */
 size_t xp_projection_keep_workspace_bytes(int64_t rows, int64_t n, int64_t k, int dtype);
 int xp_projection_keep(const void *x, int64_t ld_x, int64_t rows, int64_t k, const void *w, int64_t n, const float *bias,
                        void *projected, int64_t ld_projected, void *activated, int dtype, int order,
                        const xp_activation_desc *activation, int64_t capacity, void *workspace, size_t workspace_bytes,
                        xp_stream_t stream);
+
+/* The activation of kept values, where xp_projection_keep cannot give it: xp_activation in all but that a NaN Gate or Up is
+ * not clipped. */
+int xp_kept_activation(const void *projected, void *activated, int64_t rows, int64_t width, int dtype, int order,
+                       const xp_activation_desc *activation, xp_stream_t stream);
 
 /* Backward pass of a layer y = act(projected) . w_out^T + bias_out, projected = x . w_in^T + bias_in as kept by
  * xp_projection_keep: x [rows, hidden], w_in [2 intermediate (gated) or intermediate, hidden] in the Gate/Up `order`,
