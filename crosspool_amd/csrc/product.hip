@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 #include <iterator>
+#include <type_traits>
 
 namespace xp {
 
@@ -44,6 +45,10 @@ constexpr double kJoinUs = 3.0;       // its launch,
 constexpr double kPieceUs = 0.25;     // what a piece of a tile adds to its latency,
 constexpr double kBytesPerUs = 4e6;   // and the pieces' way out and back
 constexpr int64_t kMinSlabs = 2;      // of a worker
+// A launch holds fewer than 2^32 threads.
+bool launchable(int64_t groups, ProductTiles tiles) {
+  return groups < (int64_t{1} << 32) / (tiles == ProductTiles::k256 ? 512 : 256);
+}
 
 // `groups` workgroups of `slabs` slabs each in `pieces` tiles, all of one kind, on the chip; `apart`: no two of them work
 // on the same slabs, which then come from beyond the L2 caches.
@@ -79,6 +84,9 @@ ProductPlan find_plan(int64_t m, int64_t n, int64_t k, int64_t batch, int elemen
       ProductPlan plan{cost.tiles, whole, tiles - whole, workers, kLaunchUs};
       const int64_t together = plan.split * slabs;
       if (plan.split > 0 && (workers < plan.split || workers * kMinSlabs > together || product_scratch_bytes(plan) > scratch)) {
+        return;
+      }
+      if (!launchable(whole + workers, cost.tiles)) {
         return;
       }
       if (whole > 0) {
@@ -185,10 +193,38 @@ ProductLaunch make_product(const ProductArgs &args, const ProductPlan &plan, Pro
   return launches;
 }
 
+namespace {
+// `matrices` matrices further in an operand of `dtype`.
+template <class T>
+void advance(T *&data, int64_t matrices, int64_t batch, int dtype) {
+  using Byte = std::conditional_t<std::is_const_v<T>, const unsigned char, unsigned char>;
+  data = data == nullptr ? nullptr : static_cast<Byte *>(data) + matrices * batch * (dtype == kDtypeF32 ? 4 : 2);
+}
+}  // namespace
+
 hipError_t launch_product(const ProductArgs &args, ProductEpilogue epilogue, bool a_cols, bool b_cols, int dtype,
                           size_t scratch_bytes, hipStream_t stream) {
   const ProductPlan plan =
       plan_product(args.m, args.n, args.k, args.batch, dtype == kDtypeF32 ? 4 : 2, args.symmetric != 0, scratch_bytes);
+  if (plan.us < 0.0) {
+    // More tiles than one launch holds (over a thousand matrices of 1 x 2^20): in two halves.
+    if (args.batch < 2) {
+      return hipErrorInvalidConfiguration;
+    }
+    ProductArgs half = args;
+    half.batch = args.batch / 2;
+    if (const hipError_t status = launch_product(half, epilogue, a_cols, b_cols, dtype, scratch_bytes, stream); status != hipSuccess) {
+      return status;
+    }
+    const int64_t done = half.batch;
+    half.batch = args.batch - half.batch;
+    advance(half.a.data, done, half.a.batch, dtype);
+    advance(half.b.data, done, half.b.batch, dtype);
+    advance(half.out, done, half.batch_out, half.out_dtype);
+    advance(half.base, done, half.batch_base, half.base_dtype);
+    advance(half.extra, done, half.batch_extra, half.extra_dtype);
+    return launch_product(half, epilogue, a_cols, b_cols, dtype, scratch_bytes, stream);
+  }
   const ProductLaunch launches = make_product(args, plan, epilogue, a_cols, b_cols, dtype);
   if (const hipError_t status = launch(launches.main, stream); status != hipSuccess) {
     return status;
@@ -216,20 +252,23 @@ hipError_t launch_products(ProductGroup &group, const bool (&present)[3], int dt
       continue;
     }
     const int64_t size = tile_size(cost.tiles);
+    int64_t groups = 0;
     double work = 0.0;
     double longest = 0.0;
     for (int i = 0; i < 3; ++i) {
       if (present[i]) {
         const ProductArgs &part = group.part[i];
         const double slabs = static_cast<double>((part.k + slab - 1) / slab);
-        const double tiles = static_cast<double>(((part.m + size - 1) / size) * ((part.n + size - 1) / size));
+        const int64_t part_tiles = ((part.m + size - 1) / size) * ((part.n + size - 1) / size);
+        const double tiles = static_cast<double>(part_tiles);
         const double each = slabs * cost.slab[cost.together - 1] + cost.around[cost.together - 1];
+        groups += part_tiles;
         work += tiles * each / static_cast<double>(kCus * cost.together);
         longest = std::max(longest, each);
       }
     }
     const double us = kLaunchUs + std::max(longest, work + 0.5 * cost.around[cost.together - 1]);
-    if (us < best_us) {
+    if (us < best_us && launchable(groups, cost.tiles)) {
       best_us = us;
       best = cost.tiles;
     }

@@ -78,7 +78,8 @@ struct ProductPlan {
   double us;  // as modelled
 };
 
-// The fastest plan for a product in a workspace of `scratch` bytes for its split tiles' sums.
+// The fastest plan for a product in a workspace of `scratch` bytes for its split tiles' sums; `us` below 0 where no launch
+// holds all tiles.
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int64_t batch, int element_bytes, bool symmetric, size_t scratch);
 size_t product_scratch_bytes(const ProductPlan &plan);
 
@@ -93,7 +94,7 @@ struct ProductLaunch {
 ProductLaunch make_product(const ProductArgs &args, const ProductPlan &plan, ProductEpilogue epilogue, bool a_cols, bool b_cols,
                            int dtype);
 
-// The product as planned for its sizes.
+// The product as planned for its sizes, a batch of too many tiles for one launch in several.
 hipError_t launch_product(const ProductArgs &args, ProductEpilogue epilogue, bool a_cols, bool b_cols, int dtype,
                           size_t scratch_bytes, hipStream_t stream);
 
