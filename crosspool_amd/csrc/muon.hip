@@ -132,7 +132,10 @@ __global__ __launch_bounds__(256) void muon_scale_kernel(MuonArgs a) {
     squares += a.squares[matrix * a.parts + part];
   }
   const double norm = sqrt(group_sum(squares));
-  const float factor = static_cast<float>(static_cast<double>(a.scale) / (norm + static_cast<double>(a.eps)));
+  // A norm near the ends of fp32's range has a reciprocal past them (of a zero matrix and a tiny eps infinite: NaN): 64 bits.
+  const double exact = static_cast<double>(a.scale) / (norm + static_cast<double>(a.eps));
+  const float factor = static_cast<float>(exact);
+  const bool normal = factor >= 0x1p-126f && factor <= 0x1.fffffep127f;
   for (int64_t item = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; item < items; item += a.parts * 256) {
     const int64_t row = item / groups;
     const int64_t column = (item - row * groups) * 8;
@@ -141,7 +144,7 @@ __global__ __launch_bounds__(256) void muon_scale_kernel(MuonArgs a) {
     update_values(a, matrix, row, column, count, false, value);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      value[j] = j < count ? value[j] * factor : 0.0f;
+      value[j] = j >= count ? 0.0f : normal ? value[j] * factor : static_cast<float>(static_cast<double>(value[j]) * exact);
     }
     store_values(a.x, (matrix * a.rows + row) * a.padded + column, a.x_dtype, 8, value);
   }

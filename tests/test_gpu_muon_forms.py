@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_muon import A, B, C, muon, near, tolerance
+from test_gpu_muon import A, B, C, muon, near, orthogonal, tolerance, updates
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +60,30 @@ def test_step_of_more_tiles_than_a_launch_holds(device):
         for found, target, step in zip(weights[part].double(), moved, update):
             allowed = 0.5 * 2.0**-7.6 * float(step.norm()) + (2.0**-9 + 2.0**-22) * 2 * float(target.norm())
             assert float((found - target).norm()) <= allowed
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("eps", [1.2e-38, 1e-41, 1.4e-45])
+def test_zero_matrix_with_a_tiny_eps(device, dtype, eps):
+    """The reciprocal of a tiny eps is past fp32: a zero matrix stays zero beside one that is not."""
+
+    source = updates(device, 3, 72, 136, dtype)
+    source[1] = 0
+    out = torch.full_like(source, float("nan"))
+    muon(device, 3, 72, 136, dtype).orthogonalize_into(source, output=out, eps=eps)
+    assert bool((out[1] == 0).all())
+    near(out[0::2], orthogonal(source[0::2], eps=0.0), tolerance(dtype, 136), "matrix beside a zero one")
+
+
+@pytest.mark.parametrize("dtype,std", [(BF16, 2.0**-128), (FP32, 2.0**-130), (FP32, 2.0**125), (BF16, 2.0**124)])
+@pytest.mark.parametrize("rows,columns", [(1, 9), (72, 136), (1030, 1024)])
+def test_norms_at_the_ends_of_the_range(device, rows, columns, dtype, std):
+    """Values down to subnormal ones and up to the largest, whose norm or its reciprocal fp32 does not hold."""
+
+    g = torch.Generator(device=device).manual_seed(rows)
+    source = ((torch.randn((2, rows, columns), generator=g, device=device).clamp(-3.5, 3.5)).double() * std).to(dtype)
+    assert bool(source.isfinite().all())
+    eps = 2.0**-149  # fp32's smallest value
+    out = torch.full_like(source, float("nan"))
+    muon(device, 2, rows, columns, dtype).orthogonalize_into(source, output=out, eps=eps)
+    near(out, orthogonal(source, eps=eps), tolerance(dtype, max(rows, columns)), "matrix")
