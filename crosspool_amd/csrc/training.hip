@@ -32,8 +32,11 @@ struct PadArgs {
   int32_t count;
 };
 
+// Workgroups of an operand's copy: all four together stay below a launch's 2^32 threads.
+constexpr int64_t kPadBlocks = int64_t{1} << 21;
+
 // Rows of any alignment into rows of whole 16-byte chunks, zeros behind them: up to four operands in one launch.  One
-// thread a chunk.  Bound by latency at the sizes where it is a part of the whole (9 MB of fp16 weights, inputs and gradients of
+// thread a chunk (several chunks past 8 GiB of them).  Bound by latency at the sizes where it is a part of the whole (9 MB of fp16 weights, inputs and gradients of
 // 777 rows of 1030 x 2053: 6.6 us).
 template <class P>
 __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
@@ -46,15 +49,14 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
   }
   const PadJob job = a.job[at];
   const uint32_t chunks = static_cast<uint32_t>(job.padded / CHUNK);
-  const int64_t index = static_cast<int64_t>(block) * 256 + threadIdx.x;
-  const int64_t row = index < (int64_t{1} << 32) ? static_cast<uint32_t>(index) / chunks : index / chunks;
-  if (row >= job.rows) {
-    return;
+  const int64_t count = job.rows * chunks;
+  for (int64_t index = static_cast<int64_t>(block) * 256 + threadIdx.x; index < count; index += static_cast<int64_t>(job.blocks) * 256) {
+    const int64_t row = index < (int64_t{1} << 32) ? static_cast<uint32_t>(index) / chunks : index / chunks;
+    const int64_t column = (index - row * chunks) * CHUNK;
+    const unsigned char *from = static_cast<const unsigned char *>(job.source) + (row * job.ld + column) * kElementBytes<P>;
+    const u32x4 chunk = job.width - column >= CHUNK ? load16_any(from) : load_chunk_tail<P, P>(from, job.width - column);
+    store16(static_cast<unsigned char *>(job.target) + (row * job.padded + column) * kElementBytes<P>, chunk);
   }
-  const int64_t column = (index - row * chunks) * CHUNK;
-  const unsigned char *from = static_cast<const unsigned char *>(job.source) + (row * job.ld + column) * kElementBytes<P>;
-  const u32x4 chunk = job.width - column >= CHUNK ? load16_any(from) : load_chunk_tail<P, P>(from, job.width - column);
-  store16(static_cast<unsigned char *>(job.target) + (row * job.padded + column) * kElementBytes<P>, chunk);
 }
 
 // Zeros in columns [width, padded) of every row of the target.
@@ -432,7 +434,8 @@ struct Caller {
       return {source, ld, 0};
     }
     const int64_t length = padded_width(width, element);
-    const uint32_t blocks = blocks_of(rows * (length / static_cast<int64_t>(16 / element)), 256);
+    const int64_t chunks = rows * (length / static_cast<int64_t>(16 / element));
+    const uint32_t blocks = static_cast<uint32_t>(std::min((chunks + 255) / 256, kPadBlocks));
     pads.job[pads.count++] = PadJob{source, target, rows, width, ld, length, blocks};
     return {target, length, 0};
   }

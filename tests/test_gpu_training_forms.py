@@ -7,7 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_training import BF16, CONCATENATED, FP16, FP32, INTERLEAVED, Layer
+from test_gpu_training import BF16, CONCATENATED, FP16, FP32, INTERLEAVED, Layer, Projection, near, product
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,23 @@ def test_forward_pass_of_large_halves_does_not_clip_nan(device):
         gate_up[side][0, 7] = 0.0
     projected, out = layer.forward()
     layer.check_forward(projected, out)
+
+
+def test_padded_copies_of_more_chunks_than_a_launch_has_threads(device):
+    """2^24 rows of 257 chunks, the last cut: their padded copy is past 2^32 chunks."""
+
+    rows, k, n = 1 << 24, 8, 2049
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(device)[0] < 160 << 30:
+        pytest.skip("64 GiB of gradients and their copy do not fit the free memory")
+    case = Projection(device, 8, k, n, BF16, capacity=rows)
+    case.grad = torch.empty((rows, n), dtype=BF16, device=device).normal_(generator=torch.Generator(device=device).manual_seed(3))
+    case.x = torch.zeros((rows, k), dtype=BF16, device=device)
+    grad_x = torch.full((rows, k), float("nan"), dtype=BF16, device=device)
+    case.gemm.backward_into(case.x, case.grad, case.weights, grad_inputs=grad_x)
+    for first in range(0, rows, 1 << 18):
+        some = slice(first, first + (1 << 18))
+        exact, magnitude = product(case.grad[some], case.weights.values)
+        near(grad_x[some], exact, n * 2.0**-23 * magnitude, f"input gradient from row {first}")
+    del case, grad_x, exact, magnitude
+    torch.cuda.empty_cache()
