@@ -518,7 +518,7 @@ struct OperandLoads {
   static constexpr int LANES_PER_ROW = COLS ? ROWS * ES / 16 : 8;  // 16-byte chunks of one LDS row
   static constexpr int ROWS_PER_LOAD = 64 / LANES_PER_ROW;
   static_assert(ROWS % (8 * LOAD_WAVES) == 0, "stage rows must split evenly");
-  static_assert(!COLS || LANES_PER_ROW <= 64, "a load covers whole rows");
+  static_assert(!COLS || LANES_PER_ROW <= 32, "a load covers two rows at least");
 
   const unsigned char *origin;  // the tile's first row (COLS: first column of reduction row 0)
   uint32_t ld_bytes;
@@ -584,7 +584,7 @@ struct OperandLoads {
     if constexpr (!COLS) {
       return q & 1;
     } else if constexpr (ES == 4) {
-      return ROWS >= 256 ? (q >> 2) & 1 : ROWS == 128 ? (q >> 1) & 1 : q & 1;
+      return ROWS == 128 ? (q >> 1) & 1 : q & 1;
     } else {
       return ROWS >= 256 ? q & 1 : 0;
     }
