@@ -662,13 +662,16 @@ class Dense:
                 _DTYPE_CODES[dtype], _ORDER_CODES[order], ctypes.byref(desc), _native.current_stream(index),
             )
         width, bias = signature.local_intermediate_size, layer_weights.o_proj.bias
-        # What the general projection kernel would compute (fp32; sums of no whole 64s) is faster on the training products'
-        # tiles (fp16 777 x 2056 x 1032: 13.4 us against 25.6, fp32 494 x 11584 x 8288: 711 against 887), but where the rows
-        # are no whole 16 bytes their padded copies cost more than that for few rows (fp16 33 x 8003 x 4001: 40 against 22,
-        # 777: 110 against 113).
+        # What the general projection kernel would compute (fp32; sums of no whole 64s) is mostly faster on the training
+        # products' tiles (rows x width x hidden, us: fp16 777 x 2056 x 1032 14 against 25, fp32 494 x 11584 x 8288 711 against
+        # 887; the other way round fp16 777 x 6152 x 4096 68 against 65, 512 rows 59 against 44).  Where rows are no whole 16
+        # bytes the tiles' padded copies cost more than that for few rows.  Tiles / general, fp16, 777, 1024, 1500 and 4096
+        # rows: 2053 x 1030 24 / 30, 30 / 32, 33 / 32, 55 / 71; 6145 x 2050 71 / 60, 94 / 68, 84 / 92, 180 / 276; 8003 x 4001
+        # 105 / 102, 117 / 110, 162 / 171, 287 / 383.  fp32, 256, 512 and 777 rows: 31 / 23, 41 / 43, 54 / 69; 86 / 103,
+        # 148 / 171, 216 / 274; 201 / 183, 310 / 348, 468 / 517.
         chunk = 16 // dtype.itemsize
         general = self.plan.o_proj.kernel == "projection" and (dtype is torch.float32 or width % 64 != 0)
-        if not general or (width % chunk != 0 and rows < 512):
+        if not general or (width % chunk != 0 and rows < (512 if dtype is torch.float32 else 1280)):
             self.o_proj.run_into(activated, layer_weights.o_proj, output=output)
             return
         _native.call(

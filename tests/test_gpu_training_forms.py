@@ -241,3 +241,13 @@ def test_a_frozen_layer_in_a_graph(device, rows):
         layer.check_backward(projected, grad_x, DenseGradients())
         run()
         assert torch.equal(replayed, grad_x)
+
+
+@pytest.mark.parametrize("rows,dtype", [(511, FP32), (512, FP32), (512, BF16), (1279, BF16), (1280, BF16), (1279, FP16), (1280, FP16)])
+def test_output_projections_of_odd_widths(device, rows, dtype):
+    """Row counts where the output projection of a trained layer changes its kernel."""
+
+    for hidden, width in ((136, 131), (61, 77)):
+        layer = Layer(device, rows, hidden, width, dtype, function="gelu", order=INTERLEAVED, bias=True)
+        projected, out = layer.forward()
+        check_forward(layer, projected, out)
