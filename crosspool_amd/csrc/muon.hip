@@ -156,7 +156,7 @@ constexpr int64_t kMaxLong = int64_t{1} << 20;
 constexpr int64_t kMaxElements = int64_t{1} << 36;
 constexpr int64_t kMaxSteps = 16;
 constexpr const char *kMuonExtents =
-    "orthogonal updates take 1 to 4096 matrices with a short side of 1 to 65536 and a long side of at most 1048576";
+    "orthogonal updates take 1 to 4096 matrices with a short side of 1 to 65536 and a long side of at most 1048576, 2^36 values in all";
 
 struct MuonShape {
   int64_t matrices;

@@ -11,9 +11,12 @@ namespace xp {
 
 // A product's time in microseconds.  A CU's workgroups share its throughput: with i + 1 of them on it (as many as fit),
 // a slab in each takes `slab[i]`, and the first loads and the epilogue `around[i]`.  Fitted on MI355X to 1, 4, 12 and 48
-// slabs on 64 to 2048 workgroups; the three storage orders differ by less than 10 %.  Model and measured, us: bf16
-// 4096 x 12288 x 4096 289 / 302, fp16 1000 x 2048 x 12288 65 / 60, 12288 x 2048 x 1000 61 / 60, symmetric 4096 x 12288
-// 197 / 202; fp32 700 x 1536 x 1536 41 / 41.
+// slabs on 64 to 2048 workgroups; the three storage orders differ by less than 10 %.  Model and measured, us, of a product
+// repeated by itself: bf16 4096 x 12288 x 4096 289 / 311, fp16 1000 x 2048 x 12288 65 / 63 (its join among them),
+// 12288 x 2048 x 1000 61 / 62, 1000 x 6144 x 2048 37 / 35.  Among other launches, whose data it follows, the second takes 81
+// and the third 64.  The model knows kStore's plain epilogue alone: kGradient's loads and stores (1000 x 6144 x 2048 37 / 75),
+// mirrored tiles (fp16 symmetric 4096 x 12288 197 / 220, 32 of 768 x 768 26 / 45) and a base read back (32 of
+// 2048 x 768 x 768 74 / 99) come on top.
 namespace {
 struct ProductCost {
   ProductTiles tiles;

@@ -14,10 +14,15 @@
 // The MFMA's M operand is B, so that a lane's sums are four neighbouring columns n of one row m.
 //
 // What bounds them.  Large products: the matrix cores, at the rate the card's power allows on random operands (bf16
-// 4096 x 4096 x 24576 620 us, 1.33 PFLOP/s; fp16 4096 x 12288 x 4096 302 us, 1.37; a loop without loads 1.5 to 1.75).  The
-// epilogues of kActivate (4096 x 24576 x 4096 640 us for 825 GFLOP and 300 MB of stores) and kGradient (4096 x 12288 x 4096
-// 441 us against 335 without its 500 MB) move their bytes while the CU's matrix cores wait, since 256 x 256 accumulators leave
-// no registers for a second tile.  Few rows: the operands' bytes (five rows of 2048 x 6144 8.6 us, 2.9 TB/s).
+// 4096 x 4096 x 24576 625 us, 1.32 PFLOP/s; 4096 x 12288 x 4096 311 us, 1.32; fp16 649 and 331; a loop without loads 1.5 to
+// 1.75).  The epilogues of kActivate (bf16 4096 x 24576 x 4096 678 us against 628 without its activation and 100 MB of stores)
+// and kGradient (4096 x 12288 x 4096 460 us against 311 without its 400 MB) move their bytes while the CU's matrix cores wait, since
+// 256 x 256 accumulators leave no registers for a second tile.  Few rows: the operands' bytes (five rows of 2048 x 6144 8.8
+// us, 2.9 TB/s).
+//
+// Registers.  kStore and kActivate use no scratch memory.  kGradient's small arrays take 12 or 24 bytes a lane of it, and its
+// 256 x 256 tiles, which hold a block's kept values beside the accumulators, spill 126 registers in fp16 (132 bytes) and 6
+// in bf16 (48 bytes).
 #pragma once
 
 #include "product.hpp"

@@ -56,7 +56,8 @@ class MuonPlan:
         nbytes = int(_native.library().xp_muon_workspace_bytes(matrices, rows, columns, _DTYPE_CODES[dtype]))
         if nbytes == 0:
             raise ValueError(
-                "orthogonal updates take 1 to 4096 matrices with a short side of 1 to 65536 and a long side of at most 1048576"
+                "orthogonal updates take 1 to 4096 matrices with a short side of 1 to 65536 and a long side of at most 1048576, "
+                "2^36 values in all"
             )
         return cls(matrices, rows, columns, dtype, WorkspaceLayout.from_regions(((torch.uint8, (nbytes,)),)))
 

@@ -375,7 +375,7 @@ class Gemm:
 
         ``grad_inputs`` gets ``grad_output @ values``, ``grad_values`` (of the payload dtype or fp32)
         ``grad_output.T @ inputs`` and ``grad_bias`` (fp32) the sum of ``grad_output``'s rows; ``accumulate`` adds the last
-        two to what they hold.  Rows may lie any stride apart, but rows of whole 16 bytes on 16-byte boundaries.
+        two to what they hold.  Rows may lie any stride up to 2^20 elements apart, but rows of whole 16 bytes on 16-byte boundaries.
         Without rows the weights' and the bias's gradients are zero.
         """
 

@@ -565,8 +565,9 @@ int xp_moe_experts(const void *hidden_states, int64_t rows, int64_t hidden, int6
  * Gradients of a projection y = x . w^T + bias (x [rows, k], w [n, k]), of grad_out [rows, n]:
  *   grad_x [rows, k] = grad_out . w,  grad_w [n, k] = grad_out^T . x,  grad_bias [n] (fp32) = sum of grad_out's rows,
  * each left out where NULL.  All of dtype (XP_DTYPE_BF16, F16 or F32) but grad_w, of grad_w_dtype: dtype or fp32.
- * accumulate adds grad_w and grad_bias to what they hold.  ld_x, ld_grad and ld_grad_x are row strides in elements;
- * w and grad_w are contiguous.  Rows of x, w and grad_out of whole 16 bytes must start on 16-byte boundaries.
+ * accumulate adds grad_w and grad_bias to what they hold.  ld_x, ld_grad and ld_grad_x are row strides in elements, at
+ * most 2^20; w and grad_w are contiguous.  Up to 2^24 rows and widths of 1 to 2^20.  x may be NULL without grad_w.
+ * Rows of x, w and grad_out of whole 16 bytes must start on 16-byte boundaries.
  * Sums are fp32 and have one order: repeated calls give the same bits.  No rows: grad_w and grad_bias are
  * cleared (accumulate: left).  Outputs and workspace may overlap neither the operands nor each other.
  * The workspace serves every row count up to `capacity`, the rows that its size was asked for.  No counterpart in the
@@ -617,7 +618,8 @@ typedef struct {
 /* Orthogonalised updates: every matrix G of `updates` [matrices, rows, columns] (bf16, fp16 or fp32) becomes
  *   X0 = G / (|G| + eps) (Frobenius), then `steps` times X = a X + (b A + c A A) X with A = X X^T
  * (a, b, c = 3.4445, -4.7750, 2.0315; on the short side), rounded to dtype.  16-bit dtypes run on fp16 products with fp32
- * sums, fp32 on fp32 ones.  A matrix with an infinity or NaN becomes all NaN, a zero matrix zero.  The output may be
+ * sums, fp32 on fp32 ones.  Up to 4096 matrices with a short side of at most 2^16 and a long side of at most 2^20, 2^36
+ * values in all.  A matrix with an infinity or NaN becomes all NaN, a zero matrix zero.  The output may be
  * the updates themselves.  No counterpart in the reference. */
 size_t xp_muon_workspace_bytes(int64_t matrices, int64_t rows, int64_t columns, int dtype);
 int xp_muon_orthogonalize(const xp_matrices *updates, int64_t matrices, int64_t rows, int64_t columns, int dtype, int steps,
