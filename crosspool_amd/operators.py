@@ -362,7 +362,7 @@ class Gemm:
 
     def backward_into(
         self,
-        inputs: torch.Tensor,
+        inputs: torch.Tensor | None,
         grad_output: torch.Tensor,
         projection: ProjectionWeights,
         *,
@@ -375,7 +375,7 @@ class Gemm:
 
         ``grad_inputs`` gets ``grad_output @ values``, ``grad_values`` (of the payload dtype or fp32)
         ``grad_output.T @ inputs`` and ``grad_bias`` (fp32) the sum of ``grad_output``'s rows; ``accumulate`` adds the last
-        two to what they hold.  Rows may lie any stride up to 2^20 elements apart, but rows of whole 16 bytes on 16-byte boundaries.
+        two to what they hold.  Only ``grad_values`` reads ``inputs``, which may be None without it.  Rows may lie any stride up to 2^20 elements apart, but rows of whole 16 bytes on 16-byte boundaries.
         Without rows the weights' and the bias's gradients are zero.
         """
 
@@ -394,14 +394,16 @@ class Gemm:
         if grad_bias is not None and plan.weight_layout.bias is None:
             raise ValueError("a bias gradient of a projection without a bias")
         ld_grad = _row_stride(grad_output, "output gradient", (rows, width), dtype, index)
-        ld_inputs = _row_stride(inputs, "inputs", (rows, hidden), dtype, index)
+        if inputs is None and grad_values is not None:
+            raise ValueError("the gradient of a projection's values needs its inputs")
+        ld_inputs = hidden if inputs is None else _row_stride(inputs, "inputs", (rows, hidden), dtype, index)
         ld_grad_inputs = hidden
         if grad_inputs is not None:
             ld_grad_inputs = _row_stride(grad_inputs, "input gradient", (rows, hidden), dtype, index)
         values_at = _check_gradient(grad_values, "grad_values", (width, hidden), (dtype, torch.float32), index)
         bias_at = _check_gradient(grad_bias, "grad_bias", (width,), (torch.float32,), index)
         _native.call(
-            "xp_projection_backward", inputs.data_ptr(), ld_inputs, rows, hidden, projection.values.data_ptr(), width,
+            "xp_projection_backward", None if inputs is None else inputs.data_ptr(), ld_inputs, rows, hidden, projection.values.data_ptr(), width,
             grad_output.data_ptr(), ld_grad, _DTYPE_CODES[dtype], None if grad_inputs is None else grad_inputs.data_ptr(),
             ld_grad_inputs, values_at, _DTYPE_CODES[dtype if grad_values is None else grad_values.dtype], bias_at,
             int(accumulate), capacity, self.scratch.data_ptr(), self.scratch.numel(), _native.current_stream(index),
@@ -683,7 +685,7 @@ class Dense:
     def backward_into(
         self,
         *,
-        hidden_states: torch.Tensor,
+        hidden_states: torch.Tensor | None = None,
         layer_weights: DenseFfnWeights,
         projected: torch.Tensor,
         grad_output: torch.Tensor,
@@ -694,7 +696,8 @@ class Dense:
         """Gradients of :meth:`run_into` of the same rows, weights and kept ``projected`` (no counterpart in the reference).
 
         ``grad_hidden_states`` and what ``gradients`` names are written; ``accumulate`` adds the weights' and biases'
-        gradients to what they hold.  The gradient of the projected values is rounded to the payload dtype between
+        gradients to what they hold.  Only i_proj's gradient reads ``hidden_states``, which may be left out without it (a frozen
+        layer).  The gradient of the projected values is rounded to the payload dtype between
         the products, as the activated values are; the biases' gradients sum unrounded values.  Clipped values
         get no gradient, as in :meth:`Activation.backward_into`.
         """
@@ -706,13 +709,17 @@ class Dense:
         index = self._trained(layer_weights, rows)
         dtype, hidden, width = signature.payload_dtype, signature.hidden_size, signature.local_intermediate_size
         wide = signature.i_proj.values.shape[0]
-        ld_hidden = _row_stride(hidden_states, "hidden states", (rows, hidden), dtype, index)
+        ld_hidden = hidden
+        if hidden_states is not None:
+            ld_hidden = _row_stride(hidden_states, "hidden states", (rows, hidden), dtype, index)
         ld_projected = _row_stride(projected, "projected", (rows, wide), dtype, index)
         ld_grad = _row_stride(grad_output, "output gradient", (rows, hidden), dtype, index)
         ld_grad_hidden = hidden
         if grad_hidden_states is not None:
             ld_grad_hidden = _row_stride(grad_hidden_states, "gradient of the hidden states", (rows, hidden), dtype, index)
         into = DenseGradients() if gradients is None else gradients
+        if hidden_states is None and into.i_values is not None:
+            raise ValueError("the gradient of an i_proj's values needs the hidden states")
         for name, bias, projection in (("i_proj", into.i_bias, signature.i_proj), ("o_proj", into.o_bias, signature.o_proj)):
             if bias is not None and projection.bias is None:
                 raise ValueError(f"a bias gradient of an {name} without a bias")
@@ -726,7 +733,7 @@ class Dense:
         scratch = self.training_scratch
         desc = signature.activation.descriptor()
         _native.call(
-            "xp_dense_backward", hidden_states.data_ptr(), ld_hidden, rows, hidden, layer_weights.i_proj.values.data_ptr(),
+            "xp_dense_backward", None if hidden_states is None else hidden_states.data_ptr(), ld_hidden, rows, hidden, layer_weights.i_proj.values.data_ptr(),
             layer_weights.o_proj.values.data_ptr(), width, projected.data_ptr(), ld_projected, grad_output.data_ptr(), ld_grad,
             _DTYPE_CODES[dtype], 0 if order is None else _ORDER_CODES[order], ctypes.byref(desc),
             None if grad_hidden_states is None else grad_hidden_states.data_ptr(), ld_grad_hidden, i_values, o_values,

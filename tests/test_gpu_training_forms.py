@@ -251,3 +251,25 @@ def test_output_projections_of_odd_widths(device, rows, dtype):
         layer = Layer(device, rows, hidden, width, dtype, function="gelu", order=INTERLEAVED, bias=True)
         projected, out = layer.forward()
         check_forward(layer, projected, out)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("rows", [0, 5, 150])
+def test_frozen_weights_need_no_inputs(device, rows, dtype):
+    """Without the gradient of a projection's values its inputs are not kept."""
+
+    case = Projection(device, rows, 61, 131, dtype, bias=True)
+    grad_x, grad_b = torch.full((rows, 61), float("nan"), dtype=dtype, device=device), torch.full((131,), float("nan"), device=device)
+    case.gemm.backward_into(None, case.grad, case.weights, grad_inputs=grad_x, grad_bias=grad_b)
+    case.check(grad_x, None, grad_b)
+    with pytest.raises(ValueError, match="inputs"):
+        case.gemm.backward_into(None, case.grad, case.weights, grad_values=torch.empty((131, 61), dtype=dtype, device=device))
+    layer = Layer(device, rows, 136, 72, dtype, bias=True)
+    projected, _ = layer.forward()
+    full = layer.gradients()
+    into, grad_x = DenseGradients(o_values=full.o_values, i_bias=full.i_bias, o_bias=full.o_bias), torch.empty_like(layer.x)
+    layer.dense.backward_into(layer_weights=layer.weights, projected=projected, grad_output=layer.grad, grad_hidden_states=grad_x,
+                              gradients=into)
+    layer.check_backward(projected, grad_x, into)
+    with pytest.raises(ValueError, match="hidden states"):
+        layer.dense.backward_into(layer_weights=layer.weights, projected=projected, grad_output=layer.grad, gradients=full)
