@@ -375,7 +375,8 @@ class Gemm:
 
         ``grad_inputs`` gets ``grad_output @ values``, ``grad_values`` (of the payload dtype or fp32)
         ``grad_output.T @ inputs`` and ``grad_bias`` (fp32) the sum of ``grad_output``'s rows; ``accumulate`` adds the last
-        two to what they hold.  Only ``grad_values`` reads ``inputs``, which may be None without it.  Rows may lie any stride up to 2^20 elements apart, but rows of whole 16 bytes on 16-byte boundaries.
+        two to what they hold.  Only ``grad_values`` reads ``inputs``, which may be None without it.  Rows may lie any stride
+        up to 2^20 elements apart, but rows of whole 16 bytes on 16-byte boundaries.
         Without rows the weights' and the bias's gradients are zero.
         """
 
@@ -403,8 +404,9 @@ class Gemm:
         values_at = _check_gradient(grad_values, "grad_values", (width, hidden), (dtype, torch.float32), index)
         bias_at = _check_gradient(grad_bias, "grad_bias", (width,), (torch.float32,), index)
         _native.call(
-            "xp_projection_backward", None if inputs is None else inputs.data_ptr(), ld_inputs, rows, hidden, projection.values.data_ptr(), width,
-            grad_output.data_ptr(), ld_grad, _DTYPE_CODES[dtype], None if grad_inputs is None else grad_inputs.data_ptr(),
+            "xp_projection_backward", None if inputs is None else inputs.data_ptr(), ld_inputs, rows, hidden,
+            projection.values.data_ptr(), width, grad_output.data_ptr(), ld_grad, _DTYPE_CODES[dtype],
+            None if grad_inputs is None else grad_inputs.data_ptr(),
             ld_grad_inputs, values_at, _DTYPE_CODES[dtype if grad_values is None else grad_values.dtype], bias_at,
             int(accumulate), capacity, self.scratch.data_ptr(), self.scratch.numel(), _native.current_stream(index),
         )
@@ -733,8 +735,9 @@ class Dense:
         scratch = self.training_scratch
         desc = signature.activation.descriptor()
         _native.call(
-            "xp_dense_backward", None if hidden_states is None else hidden_states.data_ptr(), ld_hidden, rows, hidden, layer_weights.i_proj.values.data_ptr(),
-            layer_weights.o_proj.values.data_ptr(), width, projected.data_ptr(), ld_projected, grad_output.data_ptr(), ld_grad,
+            "xp_dense_backward", None if hidden_states is None else hidden_states.data_ptr(), ld_hidden, rows, hidden,
+            layer_weights.i_proj.values.data_ptr(), layer_weights.o_proj.values.data_ptr(), width, projected.data_ptr(),
+            ld_projected, grad_output.data_ptr(), ld_grad,
             _DTYPE_CODES[dtype], 0 if order is None else _ORDER_CODES[order], ctypes.byref(desc),
             None if grad_hidden_states is None else grad_hidden_states.data_ptr(), ld_grad_hidden, i_values, o_values,
             _DTYPE_CODES[dtype if kept is None else kept.dtype], i_bias, o_bias, int(accumulate),
